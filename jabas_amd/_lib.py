@@ -1,6 +1,6 @@
-"""ctypes binding of libjabas_sync.so (the C ABI declared in include/jabas_sync.h).
+"""ctypes binding of libjabas_sync.so (the C ABI declared in include/jabas_sync.h and include/jabas_loss.h).
 
-The structures below mirror the header field for field. There is no fallback: when
+The structures below mirror the headers field for field. There is no fallback: when
 the shared library is missing, :func:`lib` raises, and every product path that reaches
 for a kernel fails with that error instead of computing on the CPU.
 """
@@ -25,6 +25,9 @@ F32, BF16 = 0, 1
 SPAN_LOOSE_GRADS = 1
 OPT_NONE, OPT_SGD, OPT_ADAM, OPT_ADAMW, OPT_ADAM_AMSGRAD, OPT_ADAMW_AMSGRAD = 0, 1, 2, 3, 4, 5
 STATS_NONE, STATS_FULL, STATS_SIMILARITY, STATS_GRAM = 0, 1, 2, 3
+
+LOSS_MAX_ENTRIES = 255
+LOSS_NONE, LOSS_MEAN, LOSS_SUM = 0, 1, 2
 
 STAT_DOT_AB, STAT_NORM_A, STAT_NORM_B, STAT_NORM_AGG, STAT_NORM_VSW0 = 0, 1, 2, 3, 4
 
@@ -89,7 +92,35 @@ class JabasStepArgs(C.Structure):
     ]
 
 
-# name -> (restype, argtypes); one entry per symbol the header declares.
+class JabasLoss(C.Structure):
+    _fields_ = [
+        ("hidden", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("logits", C.c_void_p),
+        ("hidden_stride", C.c_int64),
+        ("weight_stride", C.c_int64),
+        ("logits_stride", C.c_int64),
+        ("rows", C.c_int64),
+        ("vocab", C.c_int64),
+        ("width", C.c_int64),
+        ("dtype", C.c_int32),
+        ("reduction", C.c_int32),
+        ("target", C.c_void_p),
+        ("ignore_index", C.c_int64),
+        ("label_smoothing", C.c_double),
+        ("teacher_index", C.c_void_p),
+        ("teacher_logits", C.c_void_p),
+        ("teacher_lse", C.c_void_p),
+        ("entries", C.c_int64),
+        ("temperature", C.c_double),
+        ("row_state", C.c_void_p),
+        ("entry_index", C.c_void_p),
+        ("entry_p", C.c_void_p),
+    ]
+
+
+# name -> (restype, argtypes); one entry per symbol jabas_sync.h declares.
 SIGNATURES = {
     "jabas_sync_version": (C.c_char_p, []),
     "jabas_status_string": (C.c_char_p, [C.c_int]),
@@ -131,6 +162,14 @@ SIGNATURES = {
     "jabas_rdv_reset": (C.c_int, [C.c_void_p]),
 }
 
+# jabas_loss.h
+LOSS_SIGNATURES = {
+    "jabas_loss_workspace_bytes": (C.c_size_t, [C.POINTER(JabasLoss), C.c_int32]),
+    "jabas_loss_forward": (C.c_int, [C.POINTER(JabasLoss), C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "jabas_loss_backward": (C.c_int, [C.POINTER(JabasLoss), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                      C.c_void_p, C.c_size_t, C.c_void_p]),
+}
+
 _lib = None
 
 
@@ -155,7 +194,7 @@ def lib():
                 f"{LIB_PATH} is not built; run `python -c 'import __graft_entry__ as g; g.build()'` "
                 "or `make -C jabas_amd/csrc` (needs hipcc). There is no CPU fallback.")
         handle = C.CDLL(LIB_PATH)
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in (SIGNATURES | LOSS_SIGNATURES).items():
             try:
                 fn = getattr(handle, name)
             except AttributeError:

@@ -1,0 +1,490 @@
+// Entry points of the losses: argument validation, workspace layout, and the order of the launches.
+#include <math.h>
+
+#include "loss_internal.h"
+
+#define JABAS_API extern "C" __attribute__((visibility("default")))
+
+namespace jabas {
+namespace loss {
+namespace {
+
+constexpr int64_t kMaxSize = int64_t{1} << 30;      // rows, tokens; the tiles' numbers and tokens are 32 bits in the kernels
+constexpr int64_t kMaxWidth = int64_t{1} << 20;
+
+inline int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+inline int64_t tiles(int64_t n) { return (n + kTile - 1) / kTile; }
+inline size_t element_bytes(int dtype) { return dtype == JABAS_F32 ? 4 : 2; }
+
+struct Shape {
+    bool linear, teacher;
+    int planes;                 // of the operands: fp32 takes two
+    int64_t depth;              // padded width
+    bool copy_x, copy_w;        // operands that a product cannot read as they are
+};
+
+bool misaligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
+
+void cut_rows(const JabasLoss* l, int64_t& splits, int64_t& chunk);
+
+int validate(const JabasLoss* l, Shape& s) {
+    if (!l) return JABAS_ERR_NULL;
+    if (l->dtype != JABAS_F32 && l->dtype != JABAS_BF16) return JABAS_ERR_DTYPE;
+    s.linear = l->hidden || l->weight;
+    s.teacher = l->entries != 0 || l->teacher_index || l->teacher_logits;
+    if (l->reduction < JABAS_LOSS_NONE || l->reduction > JABAS_LOSS_SUM) return JABAS_ERR_SIZE;
+    if (l->rows < 0 || l->rows > kMaxSize || l->vocab < 1 || l->vocab > kMaxSize) return JABAS_ERR_SIZE;
+    if (s.linear) {
+        if (!l->weight || (!l->hidden && l->rows) || l->logits) return JABAS_ERR_NULL;
+        if (l->width < 1 || l->width > kMaxWidth || l->hidden_stride < 0 || l->weight_stride < 0) return JABAS_ERR_SIZE;
+        if (tiles(l->rows) * tiles(l->vocab) > 0x7fffffff) return JABAS_ERR_SIZE;
+    } else {
+        if ((!l->logits && l->rows) || l->bias || !s.teacher) return JABAS_ERR_NULL;
+        int64_t splits, chunk;
+        cut_rows(l, splits, chunk);
+        if (l->logits_stride < 0 || splits * l->rows > 0x7fffffff) return JABAS_ERR_SIZE;
+    }
+    if (s.teacher) {
+        if (l->target || ((!l->teacher_index || !l->teacher_logits || !l->entry_index || !l->entry_p) && l->rows)) return JABAS_ERR_NULL;
+        if (l->entries < 1 || l->entries > JABAS_LOSS_MAX_ENTRIES) return JABAS_ERR_SIZE;
+        if (!(l->temperature > 0.0) || !isfinite(l->temperature) || l->label_smoothing != 0.0) return JABAS_ERR_SIZE;
+    } else {
+        if (!l->target && l->rows) return JABAS_ERR_NULL;
+        if (!(l->label_smoothing >= 0.0 && l->label_smoothing < 1.0) || l->temperature != 1.0 || l->teacher_lse) return JABAS_ERR_SIZE;
+    }
+    if (!l->row_state) return JABAS_ERR_NULL;
+    const size_t bytes = element_bytes(l->dtype);
+    if (misaligned(l->row_state, 16) || misaligned(l->hidden, bytes) || misaligned(l->weight, bytes) || misaligned(l->bias, bytes) ||
+        misaligned(l->logits, bytes) || misaligned(l->teacher_logits, bytes) || misaligned(l->teacher_index, 8) || misaligned(l->target, 8) ||
+        misaligned(l->teacher_lse, 4) || misaligned(l->entry_index, 4) || misaligned(l->entry_p, 4))
+        return JABAS_ERR_ALIGN;
+    s.planes = l->dtype == JABAS_F32 ? 2 : 1;
+    s.depth = round_up(s.linear ? l->width : 1, kDepth);
+    const auto as_is = [&](const void* p, int64_t stride) {
+        return s.planes == 1 && l->width % kDepth == 0 && stride % 8 == 0 && !misaligned(p, 16);
+    };
+    s.copy_x = !as_is(l->hidden, l->hidden_stride);
+    s.copy_w = !as_is(l->weight, l->weight_stride);
+    return JABAS_OK;
+}
+
+// Workspace: 256-byte aligned pieces one after the other. Without memory it only counts.
+struct Carver {
+    char* base;
+    size_t used;
+    template <class T>
+    T* take(size_t n) {
+        T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+        used += (n * sizeof(T) + 255) / 256 * 256;
+        return p;
+    }
+};
+
+// Tokens of a piece: what the pieces' copies may take is bounded, and a piece has whole tiles.
+constexpr int64_t kPieceBytes = int64_t{256} << 20;
+int64_t piece_tokens(const JabasLoss* l, const Shape& s, bool backward) {
+    int64_t per_token = 0;
+    if (s.copy_w) per_token += s.depth * 2 * s.planes;
+    if (backward) per_token += (2 * round_up(l->rows, kDepth) + l->width) * 2 * s.planes;
+    if (!per_token) return round_up(l->vocab, kTile);
+    int64_t n = kPieceBytes / per_token / kTile * kTile;
+    if (n < 4 * kTile) n = 4 * kTile;
+    const int64_t whole = round_up(l->vocab, kTile);
+    if (n >= whole) return whole;
+    const int64_t pieces = (whole + n - 1) / n;         // of about one size
+    return round_up((whole + pieces - 1) / pieces, kTile);
+}
+
+struct Forward {
+    float2* partial;
+    float* total;
+    float* entry_logit;
+    float4* teacher_row;
+    float* row_loss;
+    uint16_t *x, *w;
+    float *unscale_x, *unscale_w;
+    int64_t piece, splits, chunk;
+    int64_t tiles;
+};
+
+constexpr int64_t kSplitTokens = 32768;         // tokens of a workgroup over logits in hand, at most
+constexpr int64_t kLeastSplitTokens = 2048;
+constexpr int64_t kWantedGroups = 1024;
+
+// Workgroups per row over logits in hand: enough for the chip, none with less than a couple of passes.
+void cut_rows(const JabasLoss* l, int64_t& splits, int64_t& chunk) {
+    splits = (l->vocab + kSplitTokens - 1) / kSplitTokens;
+    const int64_t rows = l->rows > 0 ? l->rows : 1;
+    const int64_t want = (kWantedGroups + rows - 1) / rows, most = (l->vocab + kLeastSplitTokens - 1) / kLeastSplitTokens;
+    const int64_t more = want < most ? want : most;
+    if (splits < more) splits = more;
+    chunk = round_up((l->vocab + splits - 1) / splits, 32);
+    splits = (l->vocab + chunk - 1) / chunk;
+}
+
+size_t carve_forward(const JabasLoss* l, const Shape& s, char* base, Forward& f) {
+    Carver c{base, 0};
+    const int64_t rows = l->rows;
+    f = Forward{};
+    if (s.linear) {
+        f.tiles = tiles(l->vocab);
+        f.piece = piece_tokens(l, s, false);
+    } else {
+        cut_rows(l, f.splits, f.chunk);
+        f.tiles = f.splits;
+    }
+    f.partial = c.take<float2>(f.tiles * rows);
+    if (l->label_smoothing != 0.0) f.total = c.take<float>(f.tiles * rows);
+    f.entry_logit = c.take<float>(rows * (s.teacher ? l->entries : 1));
+    if (s.teacher) f.teacher_row = c.take<float4>(rows);
+    f.row_loss = c.take<float>(rows);
+    if (s.linear && s.copy_x) f.x = c.take<uint16_t>(rows * s.depth * s.planes);
+    if (s.linear && s.copy_w) f.w = c.take<uint16_t>(f.piece * s.depth * s.planes);
+    if (s.linear && s.planes == 2) {
+        f.unscale_x = c.take<float>(rows);
+        f.unscale_w = c.take<float>(f.piece);
+    }
+    return c.used;
+}
+
+struct Backward {
+    float *grad, *ratio, *peak;
+    uint16_t *x, *w, *xt, *wt, *dz, *dzt;
+    float *unscale_x, *unscale_w, *unscale_xt, *unscale_wt, *parts;
+    float *acc, *db;
+    int64_t piece, pad_rows, splits, chunk;
+};
+
+size_t carve_backward(const JabasLoss* l, const Shape& s, char* base, Backward& b) {
+    Carver c{base, 0};
+    const int64_t rows = l->rows;
+    b = Backward{};
+    b.grad = c.take<float>(rows);
+    b.ratio = c.take<float>(rows);
+    b.peak = c.take<float>(1);
+    if (!s.linear) {
+        cut_rows(l, b.splits, b.chunk);
+        return c.used;
+    }
+    b.piece = piece_tokens(l, s, true);
+    b.pad_rows = round_up(rows, kDepth);
+    if (s.copy_x) b.x = c.take<uint16_t>(rows * s.depth * s.planes);
+    if (s.copy_w) b.w = c.take<uint16_t>(b.piece * s.depth * s.planes);
+    b.unscale_x = c.take<float>(rows);
+    b.unscale_w = c.take<float>(b.piece);
+    b.unscale_xt = c.take<float>(1);
+    b.unscale_wt = c.take<float>(1);
+    b.parts = c.take<float>(kMaxParts);
+    b.xt = c.take<uint16_t>(l->width * b.pad_rows * s.planes);
+    b.wt = c.take<uint16_t>(l->width * b.piece * s.planes);
+    b.dz = c.take<uint16_t>(rows * b.piece * s.planes);
+    b.dzt = c.take<uint16_t>(b.piece * b.pad_rows * s.planes);
+    if (b.piece < l->vocab) b.acc = c.take<float>(rows * l->width);
+    b.db = c.take<float>(tiles(b.pad_rows) * b.piece);
+    return c.used;
+}
+
+Entries entries_of(const JabasLoss* l, const Shape& s) {
+    Entries e{};
+    e.target = l->target;
+    e.ignore_index = l->ignore_index;
+    if (s.teacher) {
+        e.index = l->entry_index;
+        e.p = l->entry_p;
+        e.k = static_cast<int32_t>(l->entries);
+    }
+    return e;
+}
+
+constexpr double kLog2e = 1.4426950408889634;
+
+const char* at(const void* p, int64_t elements, int dtype) {
+    return static_cast<const char*>(p) + elements * static_cast<int64_t>(element_bytes(dtype));
+}
+
+#define JABAS_TRY(call)                        \
+    do {                                       \
+        const int status_ = (call);            \
+        if (status_ != JABAS_OK) return status_; \
+    } while (0)
+
+// The hidden states as the products read them.
+int lay_x(const JabasLoss* l, const Shape& s, uint16_t* x, float* unscale, Operand& out, hipStream_t stream) {
+    out.rows = static_cast<int32_t>(l->rows);
+    if (!s.copy_x) {
+        out.p = l->hidden;
+        out.stride = l->hidden_stride;
+        out.plane = 0;
+        return JABAS_OK;
+    }
+    LayArgs a{};
+    a.in = l->hidden;
+    a.in_stride = l->hidden_stride;
+    a.in_dtype = l->dtype;
+    a.rows = static_cast<int32_t>(l->rows);
+    a.cols = static_cast<int32_t>(l->width);
+    a.out = x;
+    a.out_stride = s.depth;
+    a.out_plane = l->rows * s.depth;
+    a.pad = static_cast<int32_t>(s.depth);
+    a.planes = s.planes == 2 ? 2 : 0;
+    a.unscale = unscale;
+    out.p = x;
+    out.stride = a.out_stride;
+    out.plane = a.out_plane;
+    return launch_lay_rows(a, stream);
+}
+
+// The weight's rows of a piece.
+int lay_w(const JabasLoss* l, const Shape& s, int64_t first, int64_t n, int64_t piece, uint16_t* w, float* unscale, Operand& out, hipStream_t stream) {
+    out.rows = static_cast<int32_t>(n);
+    if (!s.copy_w) {
+        out.p = at(l->weight, first * l->weight_stride, l->dtype);
+        out.stride = l->weight_stride;
+        out.plane = 0;
+        return JABAS_OK;
+    }
+    LayArgs a{};
+    a.in = at(l->weight, first * l->weight_stride, l->dtype);
+    a.in_stride = l->weight_stride;
+    a.in_dtype = l->dtype;
+    a.rows = static_cast<int32_t>(n);
+    a.cols = static_cast<int32_t>(l->width);
+    a.out = w;
+    a.out_stride = s.depth;
+    a.out_plane = piece * s.depth;
+    a.pad = static_cast<int32_t>(s.depth);
+    a.planes = s.planes == 2 ? 2 : 0;
+    a.unscale = unscale;
+    out.p = w;
+    out.stride = a.out_stride;
+    out.plane = a.out_plane;
+    return launch_lay_rows(a, stream);
+}
+
+}  // namespace
+}  // namespace loss
+}  // namespace jabas
+
+using namespace jabas;
+using namespace jabas::loss;
+
+JABAS_API size_t jabas_loss_workspace_bytes(const JabasLoss* l, int32_t backward) {
+    Shape s;
+    if (validate(l, s) != JABAS_OK) return 0;
+    Forward f;
+    Backward b;
+    const size_t n = backward ? carve_backward(l, s, nullptr, b) : carve_forward(l, s, nullptr, f);
+    return n ? n : 256;
+}
+
+JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* workspace, size_t workspace_bytes, jabas_stream_t stream_) {
+    Shape s;
+    JABAS_TRY(validate(l, s));
+    hipStream_t stream = static_cast<hipStream_t>(stream_);
+    if (!loss_out && (l->rows || l->reduction != JABAS_LOSS_NONE)) return JABAS_ERR_NULL;
+    Forward f;
+    if (!workspace || misaligned(workspace, 256) || workspace_bytes < carve_forward(l, s, nullptr, f)) return JABAS_ERR_WORKSPACE;
+    carve_forward(l, s, static_cast<char*>(workspace), f);
+    RowState* state = reinterpret_cast<RowState*>(l->row_state);
+    float* reduce = l->row_state + 4 * l->rows;
+    if (!l->rows) return launch_reduce(f.row_loss, state, 0, l->reduction, loss_out, reduce, stream);
+    const float inv_t = static_cast<float>(1.0 / l->temperature), c = static_cast<float>(kLog2e / l->temperature);
+    const Entries entries = entries_of(l, s);
+    if (s.teacher) {
+        TeacherArgs t{};
+        t.index = l->teacher_index;
+        t.logits = l->teacher_logits;
+        t.dtype = l->dtype;
+        t.lse = l->teacher_lse;
+        t.rows = l->rows;
+        t.vocab = l->vocab;
+        t.k = static_cast<int32_t>(l->entries);
+        t.inv_t = inv_t;
+        t.entry_index = l->entry_index;
+        t.entry_p = l->entry_p;
+        t.row = f.teacher_row;
+        JABAS_TRY(launch_teacher(t, stream));
+    }
+    if (s.linear) {
+        LogitsArgs a{};
+        JABAS_TRY(lay_x(l, s, f.x, f.unscale_x, a.x, stream));
+        a.depth = static_cast<int32_t>(s.depth);
+        a.unscale_x = f.unscale_x;
+        a.unscale_w = f.unscale_w;
+        a.bias = l->bias;
+        a.bias_dtype = l->dtype;
+        a.c = c;
+        a.entries = entries;
+        a.partial = f.partial;
+        a.total = f.total;
+        a.entry_logit = f.entry_logit;
+        for (int64_t first = 0; first < l->vocab; first += f.piece) {
+            const int64_t n = l->vocab - first < f.piece ? l->vocab - first : f.piece;
+            JABAS_TRY(lay_w(l, s, first, n, f.piece, f.w, f.unscale_w, a.w, stream));
+            a.first = static_cast<int32_t>(first);
+            a.first_tile = static_cast<int32_t>(first / kTile);
+            JABAS_TRY(launch_logits_forward(a, s.planes, stream));
+        }
+    } else {
+        TopkArgs a{};
+        a.logits = l->logits;
+        a.stride = l->logits_stride;
+        a.dtype = l->dtype;
+        a.rows = l->rows;
+        a.vocab = l->vocab;
+        a.splits = static_cast<int32_t>(f.splits);
+        a.chunk = f.chunk;
+        a.c = c;
+        a.entries = entries;
+        a.partial = f.partial;
+        a.entry_logit = f.entry_logit;
+        JABAS_TRY(launch_topk_forward(a, stream));
+    }
+    JoinArgs j{};
+    j.partial = f.partial;
+    j.total = f.total;
+    j.entry_logit = f.entry_logit;
+    j.rows = l->rows;
+    j.vocab = l->vocab;
+    j.tiles = static_cast<int32_t>(f.tiles);
+    j.c = c;
+    j.inv_t = inv_t;
+    j.t = static_cast<float>(l->temperature);
+    j.smoothing = static_cast<float>(l->label_smoothing);
+    j.entries = entries;
+    j.teacher_row = f.teacher_row;
+    j.has_rest = l->teacher_lse != nullptr;
+    j.state = state;
+    j.row_loss = f.row_loss;
+    JABAS_TRY(launch_join(j, stream));
+    return launch_reduce(f.row_loss, state, l->rows, l->reduction, loss_out, reduce, stream);
+}
+
+JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, void* d_hidden, void* d_weight, void* d_bias, void* d_logits,
+                                  void* workspace, size_t workspace_bytes, jabas_stream_t stream_) {
+    Shape s;
+    JABAS_TRY(validate(l, s));
+    hipStream_t stream = static_cast<hipStream_t>(stream_);
+    if (!upstream && (l->rows || l->reduction != JABAS_LOSS_NONE)) return JABAS_ERR_NULL;
+    if (s.linear ? d_logits != nullptr : d_hidden || d_weight || d_bias) return JABAS_ERR_NULL;
+    if (d_bias && !l->bias) return JABAS_ERR_NULL;
+    const size_t bytes = element_bytes(l->dtype);
+    if (misaligned(d_hidden, bytes) || misaligned(d_weight, bytes) || misaligned(d_bias, bytes) || misaligned(d_logits, bytes) || misaligned(upstream, 4))
+        return JABAS_ERR_ALIGN;
+    Backward b;
+    if (!workspace || misaligned(workspace, 256) || workspace_bytes < carve_backward(l, s, nullptr, b)) return JABAS_ERR_WORKSPACE;
+    carve_backward(l, s, static_cast<char*>(workspace), b);
+    if (!l->rows) {
+        if (d_weight) JABAS_TRY(launch_zero(d_weight, static_cast<size_t>(l->vocab) * l->width * bytes, stream));
+        if (d_bias) JABAS_TRY(launch_zero(d_bias, static_cast<size_t>(l->vocab) * bytes, stream));
+        return JABAS_OK;
+    }
+    const RowState* state = reinterpret_cast<const RowState*>(l->row_state);
+    const float* reduce = l->row_state + 4 * l->rows;
+    const float c = static_cast<float>(kLog2e / l->temperature);
+    JABAS_TRY(launch_row_grad(upstream, l->reduction == JABAS_LOSS_NONE, reduce, static_cast<float>(l->temperature), state, l->rows, b.grad, b.ratio,
+                              b.peak, stream));
+    if (!s.linear) {
+        if (!d_logits) return JABAS_OK;
+        TopkArgs a{};
+        a.logits = l->logits;
+        a.stride = l->logits_stride;
+        a.dtype = l->dtype;
+        a.rows = l->rows;
+        a.vocab = l->vocab;
+        a.splits = static_cast<int32_t>(b.splits);
+        a.chunk = b.chunk;
+        a.c = c;
+        a.entries = entries_of(l, s);
+        a.state = state;
+        a.row_grad = b.grad;
+        a.out = d_logits;
+        return launch_topk_backward(a, stream);
+    }
+    if (!d_hidden && !d_weight && !d_bias) return JABAS_OK;
+    LogitsArgs a{};
+    JABAS_TRY(lay_x(l, s, b.x, b.unscale_x, a.x, stream));
+    a.depth = static_cast<int32_t>(s.depth);
+    a.unscale_x = b.unscale_x;
+    a.unscale_w = b.unscale_w;
+    a.bias = l->bias;
+    a.bias_dtype = l->dtype;
+    a.c = c;
+    a.entries = entries_of(l, s);
+    a.state = state;
+    a.row_grad = b.grad;
+    a.uniform = static_cast<float>(l->label_smoothing / static_cast<double>(l->vocab));
+    a.hit = static_cast<float>(1.0 - l->label_smoothing);
+    a.dz = d_hidden ? b.dz : nullptr;
+    a.dz_stride = b.piece;
+    a.dz_plane = l->rows * b.piece;
+    a.dzt = d_weight ? b.dzt : nullptr;
+    a.dzt_stride = b.pad_rows;
+    a.dzt_plane = b.piece * b.pad_rows;
+    a.db = d_bias ? b.db : nullptr;
+    a.pad_rows = static_cast<int32_t>(b.pad_rows);
+    LayArgs lay{};
+    lay.in_dtype = l->dtype;
+    lay.cols = static_cast<int32_t>(l->width);
+    lay.planes = s.planes;
+    lay.parts = b.parts;
+    if (d_weight) {
+        lay.in = l->hidden;
+        lay.in_stride = l->hidden_stride;
+        lay.rows = static_cast<int32_t>(l->rows);
+        lay.row_factor = b.ratio;
+        lay.out = b.xt;
+        lay.out_stride = b.pad_rows;
+        lay.out_plane = l->width * b.pad_rows;
+        lay.pad = static_cast<int32_t>(b.pad_rows);
+        lay.unscale = b.unscale_xt;
+        JABAS_TRY(launch_lay_columns(lay, stream));
+    }
+    lay.row_factor = nullptr;
+    for (int64_t first = 0; first < l->vocab; first += b.piece) {
+        const int64_t n = l->vocab - first < b.piece ? l->vocab - first : b.piece, pad = round_up(n, kDepth);
+        JABAS_TRY(lay_w(l, s, first, n, b.piece, b.w, b.unscale_w, a.w, stream));
+        a.first = static_cast<int32_t>(first);
+        a.pad_tokens = static_cast<int32_t>(pad);
+        JABAS_TRY(launch_logits_backward(a, s.planes, stream));
+        if (d_bias) JABAS_TRY(launch_bias_sum(b.db, static_cast<int32_t>(tiles(b.pad_rows)), n, n, static_cast<char*>(d_bias) + first * bytes, l->dtype, stream));
+        OutArgs o{};
+        o.scale = 1.0f / kDzScale;
+        o.out_stride = l->width;
+        o.out_dtype = l->dtype;
+        if (d_weight) {
+            o.a = Operand{b.dzt, a.dzt_stride, a.dzt_plane, static_cast<int32_t>(n)};
+            o.b = Operand{b.xt, b.pad_rows, l->width * b.pad_rows, static_cast<int32_t>(l->width)};
+            o.depth = static_cast<int32_t>(b.pad_rows);
+            o.unscale0 = b.unscale_xt;
+            o.unscale1 = b.peak;
+            o.out = static_cast<char*>(d_weight) + first * l->width * static_cast<int64_t>(bytes);
+            JABAS_TRY(launch_out(o, s.planes, stream));
+        }
+        if (d_hidden) {
+            lay.in = at(l->weight, first * l->weight_stride, l->dtype);
+            lay.in_stride = l->weight_stride;
+            lay.rows = static_cast<int32_t>(n);
+            lay.row_mask = l->bias ? at(l->bias, first, l->dtype) : nullptr;
+            lay.out = b.wt;
+            lay.out_stride = b.piece;
+            lay.out_plane = l->width * b.piece;
+            lay.pad = static_cast<int32_t>(pad);
+            lay.unscale = b.unscale_wt;
+            JABAS_TRY(launch_lay_columns(lay, stream));
+            o.a = Operand{b.dz, a.dz_stride, a.dz_plane, static_cast<int32_t>(l->rows)};
+            o.b = Operand{b.wt, b.piece, l->width * b.piece, static_cast<int32_t>(l->width)};
+            o.depth = static_cast<int32_t>(pad);
+            o.unscale0 = b.unscale_wt;
+            o.unscale1 = nullptr;
+            o.row_scale = b.grad;
+            o.acc = b.acc;
+            o.first = first == 0;
+            o.last = first + b.piece >= l->vocab;
+            o.out = d_hidden;
+            JABAS_TRY(launch_out(o, s.planes, stream));
+        }
+    }
+    return JABAS_OK;
+}

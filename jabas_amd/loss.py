@@ -1,0 +1,258 @@
+"""Losses over a large vocabulary, forward and backward, as hand-written kernels (``include/jabas_loss.h``).
+
+What ends a virtual stream worker's forward pass: cross entropy and distillation from a teacher's top logits, either over
+logits in hand or straight from the hidden states and the classifier's weight. The latter never keep the logits: the
+product is worked through in tiles whose maxima and sums are all that leaves the chip, and the backward pass computes them
+again, a piece of the vocabulary at a time. K workers on one GPU hold K sets of activations, and [tokens, vocabulary] logits
+are the largest of them (6400 tokens over 32317 in fp32: 0.83 GB per worker, once for the logits and once for their gradient).
+
+The classifiers and criteria these stand in for: the translation model's (examples/gnmt/seq2seq/models/decoder.py, label
+smoothing and a padding index; examples/gnmt/seq2seq/train/smoothing.py) and ``CrossEntropyLoss`` in the vision examples;
+a trainer calls them as ``criterion(model(x), y)`` (jabas/train/trainer.py:82-86, 171-174), see :class:`LinearCrossEntropy`
+and :class:`LinearTopkDistillation`.
+
+All of them are autograd functions on the current stream of the tensors' device; there is no CPU path. Every input keeps its
+place in memory: nothing is changed in place, nothing is kept between calls but what autograd saves (the inputs, 16 bytes a
+row, 8 bytes an entry of the teacher). Results are the same from run to run: no sum depends on the order of atomics.
+"""
+import ctypes as C
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+from .sync import _stream_ptr
+
+REDUCTIONS = {"none": L.LOSS_NONE, "mean": L.LOSS_MEAN, "sum": L.LOSS_SUM}
+MAX_ENTRIES = L.LOSS_MAX_ENTRIES
+
+
+def _matrix(t, what, dtype=None):
+    """``t`` as a matrix whose rows are contiguous: as it is where it has that form, else a copy."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what}: expected a tensor")
+    if t.device.type != "cuda":
+        raise ValueError(f"{what}: must live on the GPU, got {t.device}")
+    if dtype is None:
+        if t.dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError(f"{what}: must be float32 or bfloat16, got {t.dtype}")
+    elif t.dtype != dtype:
+        raise TypeError(f"{what}: expected {dtype}, got {t.dtype}")
+    return t
+
+
+def _rows_of(t):
+    """(tensor, element stride of its rows) of a 2-D tensor with contiguous rows; a copy where the rows are not."""
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.stride(0) < 0:
+        t = t.contiguous()
+    return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _check_row_tensor(t, shape, dtype, device, what):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what}: expected a tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{what}: expected {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{what}: on {t.device}, expected {device}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _reduction(name):
+    if name not in REDUCTIONS:
+        raise ValueError(f"unknown reduction {name!r}: none, mean or sum")
+    return REDUCTIONS[name]
+
+
+def _workspace(loss, backward, device):
+    n = L.lib().jabas_loss_workspace_bytes(C.byref(loss), int(backward))
+    # 256 bytes are what the caching allocator aligns to at least
+    return torch.empty(n, dtype=torch.uint8, device=device), n
+
+
+class _Loss(torch.autograd.Function):
+    """``spec``: what is no tensor. The tensors come one by one so that autograd sees them."""
+
+    @staticmethod
+    def forward(ctx, spec, hidden, weight, bias, logits, target, teacher_index, teacher_logits, teacher_lse):
+        main = logits if hidden is None else hidden
+        device, rows = main.device, main.shape[0]
+        if device.index != torch.cuda.current_device():
+            with torch.cuda.device(device):
+                return _Loss.forward(ctx, spec, hidden, weight, bias, logits, target, teacher_index, teacher_logits, teacher_lse)
+        state = torch.empty(4 * rows + 4, dtype=torch.float32, device=device)
+        k = 0 if teacher_index is None else teacher_index.shape[1]
+        entry_index = torch.empty(rows, k, dtype=torch.int32, device=device) if k else None
+        entry_p = torch.empty(rows, k, dtype=torch.float32, device=device) if k else None
+        kept = (hidden, weight, bias, logits, target, teacher_index, teacher_logits, teacher_lse, state, entry_index, entry_p)
+        c = _fill(spec, *kept)
+        out = torch.empty(rows if spec["reduction"] == L.LOSS_NONE else (), dtype=torch.float32, device=device)
+        ws, n = _workspace(c, False, device)
+        L.check(L.lib().jabas_loss_forward(C.byref(c), out.data_ptr(), ws.data_ptr(), n, _stream_ptr()), "jabas_loss_forward")
+        ctx.spec = spec
+        ctx.save_for_backward(*kept)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, upstream):
+        kept = ctx.saved_tensors
+        hidden, weight, bias, logits = kept[:4]
+        device = upstream.device
+        if device.index != torch.cuda.current_device():
+            with torch.cuda.device(device):
+                return _Loss._grads(ctx, kept, upstream)
+        return _Loss._grads(ctx, kept, upstream)
+
+    @staticmethod
+    def _grads(ctx, kept, upstream):
+        c = _fill(ctx.spec, *kept)
+        upstream = upstream.to(torch.float32).contiguous()
+        wanted = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and need else None
+                  for t, need in zip(kept[:4], ctx.needs_input_grad[1:5])]
+        ws, n = _workspace(c, True, upstream.device)
+        L.check(L.lib().jabas_loss_backward(C.byref(c), upstream.data_ptr(), *[None if t is None else t.data_ptr() for t in wanted],
+                                            ws.data_ptr(), n, _stream_ptr()), "jabas_loss_backward")
+        return (None, *wanted, None, None, None, None)
+
+
+def _fill(spec, hidden, weight, bias, logits, target, teacher_index, teacher_logits, teacher_lse, state, entry_index, entry_p):
+    def ptr(t):
+        return None if t is None else t.data_ptr()
+
+    c = L.JabasLoss()
+    main = logits if hidden is None else hidden
+    c.hidden, c.weight, c.bias, c.logits = ptr(hidden), ptr(weight), ptr(bias), ptr(logits)
+    if hidden is None:
+        c.rows, c.vocab = logits.shape
+        c.logits_stride = _rows_of(logits)[1]
+    else:
+        c.rows, c.width = hidden.shape
+        c.vocab = weight.shape[0]
+        c.hidden_stride, c.weight_stride = _rows_of(hidden)[1], _rows_of(weight)[1]
+    c.dtype = L.F32 if main.dtype == torch.float32 else L.BF16
+    c.reduction = spec["reduction"]
+    c.target, c.ignore_index, c.label_smoothing = ptr(target), spec.get("ignore_index", 0), spec.get("label_smoothing", 0.0)
+    c.teacher_index, c.teacher_logits, c.teacher_lse = ptr(teacher_index), ptr(teacher_logits), ptr(teacher_lse)
+    c.entries = 0 if teacher_index is None else teacher_index.shape[1]
+    c.temperature = spec.get("temperature", 1.0)
+    c.row_state, c.entry_index, c.entry_p = ptr(state), ptr(entry_index), ptr(entry_p)
+    return c
+
+
+def _linear_inputs(hidden, weight, bias):
+    _matrix(hidden, "hidden")
+    _matrix(weight, "weight", hidden.dtype)
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)}: the last sizes must agree, weight has two")
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError("weight: needs at least one token and one feature")
+    if weight.device != hidden.device:
+        raise ValueError(f"weight: on {weight.device}, expected {hidden.device}")
+    if bias is not None:
+        _check_row_tensor(bias, (weight.shape[0],), hidden.dtype, hidden.device, "bias")
+        bias = bias.contiguous()
+    return _rows_of(hidden.reshape(-1, hidden.shape[-1]))[0], _rows_of(weight)[0], bias
+
+
+def _teacher_inputs(lead, device, dtype, teacher_index, teacher_logits, teacher_lse, temperature):
+    if not isinstance(teacher_index, torch.Tensor) or teacher_index.dim() != len(lead) + 1:
+        raise ValueError(f"teacher_index: expected a tensor of shape {tuple(lead)} and the entries")
+    k = teacher_index.shape[-1]
+    if not 1 <= k <= MAX_ENTRIES:
+        raise ValueError(f"teacher_index: 1..{MAX_ENTRIES} entries per row, got {k}")
+    _check_row_tensor(teacher_index, (*lead, k), torch.int64, device, "teacher_index")
+    _check_row_tensor(teacher_logits, (*lead, k), dtype, device, "teacher_logits")
+    if teacher_lse is not None:
+        _check_row_tensor(teacher_lse, lead, torch.float32, device, "teacher_lse")
+        teacher_lse = teacher_lse.detach().reshape(-1).contiguous()
+    if not (temperature > 0.0 and temperature < float("inf")):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    return teacher_index.reshape(-1, k).contiguous(), teacher_logits.detach().reshape(-1, k).contiguous(), teacher_lse
+
+
+def linear_cross_entropy(hidden, weight, target, bias=None, *, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
+    """Cross entropy of the classifier ``hidden @ weight.T + bias`` against ``target``, without keeping the logits.
+
+    hidden: (..., width) float32 or bfloat16; weight: (vocab, width) of the same type; bias: (vocab,) of the same type or
+    None (-inf rules a token out); target: (...) int64. The loss of a row with logits z and label t is
+    ``logsumexp(z) - (1 - e) z[t] - e mean(z)``, e = label_smoothing. Rows whose label is ``ignore_index`` do not count:
+    loss and gradient are 0 whatever their hidden states hold. Any other label outside the vocabulary gives NaN.
+
+    reduction: "mean" over the rows that count (0 where none does), "sum" or "none" (the shape of target). The loss is
+    float32, sums are kept in 32 bits; gradients have the inputs' type. With bfloat16 the products take the inputs as they
+    are and the row gradients as fp16 in units of 2^-15 (rounded once, an eighth of bfloat16's step); with float32 every
+    factor is split into two fp16 planes (22 bits) and the products into three."""
+    x, w, b = _linear_inputs(hidden, weight, bias)
+    lead = hidden.shape[:-1]
+    _check_row_tensor(target, lead, torch.int64, hidden.device, "target")
+    if not 0.0 <= label_smoothing < 1.0:
+        raise ValueError(f"label_smoothing must be in [0, 1), got {label_smoothing}")
+    spec = dict(reduction=_reduction(reduction), ignore_index=int(ignore_index), label_smoothing=float(label_smoothing))
+    out = _Loss.apply(spec, x, w, b, None, target.reshape(-1).contiguous(), None, None, None)
+    return out.view(lead) if reduction == "none" else out
+
+
+def topk_distillation(logits, teacher_index, teacher_logits, *, temperature=1.0, teacher_lse=None, reduction="mean"):
+    """Distillation of ``logits`` (..., vocab) from a teacher's top logits, logits in hand.
+
+    teacher_index: (..., k) int64, the tokens the teacher's logits belong to, k up to 255; teacher_logits: (..., k) of the
+    logits' type. A place with a negative index or logit -inf holds no entry; a row without any does not count (loss and gradient
+    0); places that name one token are one event with the sum of their probabilities. With q = softmax(logits / T) over the
+    whole vocabulary the loss of a row is ``T^2 sum_j p_j (log p_j - log q_j)``:
+
+    - ``teacher_lse`` None: p is the softmax of the entries' logits / T;
+    - ``teacher_lse`` (...) float32, the teacher's logsumexp(logits / T) over its whole vocabulary: p are its true
+      probabilities, and what they leave, r = max(0, 1 - sum p), is one more event that the student meets with all tokens
+      that are no entry: ``+ T^2 r (log r - log sum_others q)``.
+
+    reduction as in :func:`linear_cross_entropy`. No gradient flows to the teacher."""
+    _matrix(logits, "logits")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError("logits: needs at least one token")
+    lead = logits.shape[:-1]
+    index, t, lse = _teacher_inputs(lead, logits.device, logits.dtype, teacher_index, teacher_logits, teacher_lse, temperature)
+    z = _rows_of(logits.reshape(-1, logits.shape[-1]))[0]
+    out = _Loss.apply(dict(reduction=_reduction(reduction), temperature=float(temperature)), None, None, None, z, None, index, t, lse)
+    return out.view(lead) if reduction == "none" else out
+
+
+def linear_topk_distillation(hidden, weight, teacher_index, teacher_logits, bias=None, *, temperature=1.0, teacher_lse=None,
+                             reduction="mean"):
+    """:func:`topk_distillation` of the classifier ``hidden @ weight.T + bias`` without keeping its logits; hidden, weight
+    and bias as in :func:`linear_cross_entropy`, teacher_logits of their type."""
+    x, w, b = _linear_inputs(hidden, weight, bias)
+    lead = hidden.shape[:-1]
+    index, t, lse = _teacher_inputs(lead, hidden.device, hidden.dtype, teacher_index, teacher_logits, teacher_lse, temperature)
+    out = _Loss.apply(dict(reduction=_reduction(reduction), temperature=float(temperature)), x, w, b, None, None, index, t, lse)
+    return out.view(lead) if reduction == "none" else out
+
+
+class LinearCrossEntropy(torch.nn.Module):
+    """:func:`linear_cross_entropy` as a trainer's criterion: ``criterion((hidden, weight, bias), target)`` for a model whose
+    forward returns its last hidden states with its classifier's weight and bias (None where it has none)."""
+
+    def __init__(self, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
+        super().__init__()
+        self.ignore_index, self.label_smoothing, self.reduction = ignore_index, label_smoothing, reduction
+
+    def forward(self, output, target):
+        hidden, weight, bias = output
+        return linear_cross_entropy(hidden, weight, target, bias, ignore_index=self.ignore_index,
+                                    label_smoothing=self.label_smoothing, reduction=self.reduction)
+
+
+class LinearTopkDistillation(torch.nn.Module):
+    """:func:`linear_topk_distillation` as a trainer's criterion: ``criterion((hidden, weight, bias), (teacher_index,
+    teacher_logits))`` or ``(teacher_index, teacher_logits, teacher_lse)``."""
+
+    def __init__(self, temperature=1.0, reduction="mean"):
+        super().__init__()
+        self.temperature, self.reduction = temperature, reduction
+
+    def forward(self, output, teacher):
+        hidden, weight, bias = output
+        index, logits, lse = teacher if len(teacher) == 3 else (*teacher, None)
+        return linear_topk_distillation(hidden, weight, index, logits, bias, temperature=self.temperature, teacher_lse=lse,
+                                        reduction=self.reduction)
