@@ -13,7 +13,7 @@ constexpr int64_t kMaxSize = int64_t{1} << 30;      // rows, tokens; the tiles' 
 constexpr int64_t kMaxWidth = int64_t{1} << 20;
 
 inline int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
-inline int64_t tiles(int64_t n) { return (n + kTile - 1) / kTile; }
+inline int64_t tiles(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
 inline size_t element_bytes(int dtype) { return dtype == JABAS_F32 ? 4 : 2; }
 
 struct Shape {
@@ -37,7 +37,7 @@ int validate(const JabasLoss* l, Shape& s) {
     if (s.linear) {
         if (!l->weight || (!l->hidden && l->rows) || l->logits) return JABAS_ERR_NULL;
         if (l->width < 1 || l->width > kMaxWidth || l->hidden_stride < 0 || l->weight_stride < 0) return JABAS_ERR_SIZE;
-        if (tiles(l->rows) * tiles(l->vocab) > 0x7fffffff) return JABAS_ERR_SIZE;
+        if (tiles(l->rows, 128) * tiles(l->vocab, 128) > 0x7fffffff) return JABAS_ERR_SIZE;
     } else {
         if ((!l->logits && l->rows) || l->bias || !s.teacher) return JABAS_ERR_NULL;
         int64_t splits, chunk;
@@ -61,7 +61,7 @@ int validate(const JabasLoss* l, Shape& s) {
     s.planes = l->dtype == JABAS_F32 ? 2 : 1;
     s.depth = round_up(s.linear ? l->width : 1, kDepth);
     const auto as_is = [&](const void* p, int64_t stride) {
-        return s.planes == 1 && l->width % kDepth == 0 && stride % 8 == 0 && !misaligned(p, 16);
+        return s.planes == 1 && l->width % kDepth == 0 && stride % 8 == 0 && stride <= kMaxStride && !misaligned(p, 16);
     };
     s.copy_x = !as_is(l->hidden, l->hidden_stride);
     s.copy_w = !as_is(l->weight, l->weight_stride);
@@ -85,7 +85,7 @@ constexpr int64_t kPieceBytes = int64_t{256} << 20;
 int64_t piece_tokens(const JabasLoss* l, const Shape& s, bool backward) {
     int64_t per_token = 0;
     if (s.copy_w) per_token += s.depth * 2 * s.planes;
-    if (backward) per_token += (2 * round_up(l->rows, kDepth) + l->width) * 2 * s.planes;
+    if (backward) per_token += (round_up(l->rows, kDepth) + s.depth) * 2 * s.planes;     // dz and the weight in fp16
     if (!per_token) return round_up(l->vocab, kTile);
     int64_t n = kPieceBytes / per_token / kTile * kTile;
     if (n < 4 * kTile) n = 4 * kTile;
@@ -105,6 +105,7 @@ struct Forward {
     float *unscale_x, *unscale_w;
     int64_t piece, splits, chunk;
     int64_t tiles;
+    bool large;
 };
 
 constexpr int64_t kSplitTokens = 32768;         // tokens of a workgroup over logits in hand, at most
@@ -127,7 +128,8 @@ size_t carve_forward(const JabasLoss* l, const Shape& s, char* base, Forward& f)
     const int64_t rows = l->rows;
     f = Forward{};
     if (s.linear) {
-        f.tiles = tiles(l->vocab);
+        f.large = large_tiles(l->vocab, rows, s.planes);
+        f.tiles = tiles(l->vocab, logits_tile_tokens(f.large));
         f.piece = piece_tokens(l, s, false);
     } else {
         cut_rows(l, f.splits, f.chunk);
@@ -149,10 +151,12 @@ size_t carve_forward(const JabasLoss* l, const Shape& s, char* base, Forward& f)
 
 struct Backward {
     float *grad, *ratio, *peak;
-    uint16_t *x, *w, *xt, *wt, *dz, *dzt;
-    float *unscale_x, *unscale_w, *unscale_xt, *unscale_wt, *parts;
+    uint16_t *x, *w;            // operands of the logits, where they are copies
+    uint16_t *x16, *w16, *dz;   // of the gradients' products
+    float *unscale_x, *unscale_w, *unscale_x16, *unscale_w16, *parts;
     float *acc, *db;
-    int64_t piece, pad_rows, splits, chunk;
+    int64_t piece, pad_rows, acc_stride, splits, chunk;
+    bool large;
 };
 
 size_t carve_backward(const JabasLoss* l, const Shape& s, char* base, Backward& b) {
@@ -172,15 +176,16 @@ size_t carve_backward(const JabasLoss* l, const Shape& s, char* base, Backward& 
     if (s.copy_w) b.w = c.take<uint16_t>(b.piece * s.depth * s.planes);
     b.unscale_x = c.take<float>(rows);
     b.unscale_w = c.take<float>(b.piece);
-    b.unscale_xt = c.take<float>(1);
-    b.unscale_wt = c.take<float>(1);
+    b.unscale_x16 = c.take<float>(1);
+    b.unscale_w16 = c.take<float>(1);
     b.parts = c.take<float>(kMaxParts);
-    b.xt = c.take<uint16_t>(l->width * b.pad_rows * s.planes);
-    b.wt = c.take<uint16_t>(l->width * b.piece * s.planes);
-    b.dz = c.take<uint16_t>(rows * b.piece * s.planes);
-    b.dzt = c.take<uint16_t>(b.piece * b.pad_rows * s.planes);
-    if (b.piece < l->vocab) b.acc = c.take<float>(rows * l->width);
-    b.db = c.take<float>(tiles(b.pad_rows) * b.piece);
+    b.x16 = c.take<uint16_t>(b.pad_rows * s.depth * s.planes);
+    b.w16 = c.take<uint16_t>(b.piece * s.depth * s.planes);
+    b.dz = c.take<uint16_t>(b.pad_rows * b.piece * s.planes);
+    b.acc_stride = round_up(l->width, 4);
+    if (b.piece < l->vocab) b.acc = c.take<float>(rows * b.acc_stride);
+    b.large = large_tiles(b.piece < l->vocab ? b.piece : l->vocab, rows, s.planes);
+    if (l->bias) b.db = c.take<float>(tiles(rows, logits_tile_rows(b.large, s.planes)) * b.piece);
     return c.used;
 }
 
@@ -323,8 +328,7 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
             const int64_t n = l->vocab - first < f.piece ? l->vocab - first : f.piece;
             JABAS_TRY(lay_w(l, s, first, n, f.piece, f.w, f.unscale_w, a.w, stream));
             a.first = static_cast<int32_t>(first);
-            a.first_tile = static_cast<int32_t>(first / kTile);
-            JABAS_TRY(launch_logits_forward(a, s.planes, stream));
+            JABAS_TRY(launch_logits_forward(a, s.planes, f.large, stream));
         }
     } else {
         TopkArgs a{};
@@ -416,73 +420,83 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     a.row_grad = b.grad;
     a.uniform = static_cast<float>(l->label_smoothing / static_cast<double>(l->vocab));
     a.hit = static_cast<float>(1.0 - l->label_smoothing);
-    a.dz = d_hidden ? b.dz : nullptr;
+    a.dz = d_hidden || d_weight ? b.dz : nullptr;
     a.dz_stride = b.piece;
-    a.dz_plane = l->rows * b.piece;
-    a.dzt = d_weight ? b.dzt : nullptr;
-    a.dzt_stride = b.pad_rows;
-    a.dzt_plane = b.piece * b.pad_rows;
+    a.dz_plane = b.pad_rows * b.piece;
     a.db = d_bias ? b.db : nullptr;
     a.pad_rows = static_cast<int32_t>(b.pad_rows);
+    const int32_t row_tiles = static_cast<int32_t>(tiles(l->rows, logits_tile_rows(b.large, s.planes)));
     LayArgs lay{};
     lay.in_dtype = l->dtype;
     lay.cols = static_cast<int32_t>(l->width);
+    lay.out_stride = s.depth;
+    lay.pad = static_cast<int32_t>(s.depth);
     lay.planes = s.planes;
     lay.parts = b.parts;
     if (d_weight) {
         lay.in = l->hidden;
         lay.in_stride = l->hidden_stride;
         lay.rows = static_cast<int32_t>(l->rows);
+        lay.pad_rows = static_cast<int32_t>(b.pad_rows);
         lay.row_factor = b.ratio;
-        lay.out = b.xt;
-        lay.out_stride = b.pad_rows;
-        lay.out_plane = l->width * b.pad_rows;
-        lay.pad = static_cast<int32_t>(b.pad_rows);
-        lay.unscale = b.unscale_xt;
-        JABAS_TRY(launch_lay_columns(lay, stream));
+        lay.out = b.x16;
+        lay.out_plane = b.pad_rows * s.depth;
+        lay.unscale = b.unscale_x16;
+        JABAS_TRY(launch_lay_whole(lay, stream));
     }
     lay.row_factor = nullptr;
+    const int32_t width = static_cast<int32_t>(l->width), depth = static_cast<int32_t>(s.depth), rows = static_cast<int32_t>(l->rows);
+    OutArgs o{};
+    o.scale = 1.0f / kDzScale;
+    o.m = width;
+    o.out_stride = l->width;
+    o.out_dtype = l->dtype;
     for (int64_t first = 0; first < l->vocab; first += b.piece) {
-        const int64_t n = l->vocab - first < b.piece ? l->vocab - first : b.piece, pad = round_up(n, kDepth);
+        const int64_t n = l->vocab - first < b.piece ? l->vocab - first : b.piece;
+        const int32_t pad = static_cast<int32_t>(round_up(n, kDepth));
         JABAS_TRY(lay_w(l, s, first, n, b.piece, b.w, b.unscale_w, a.w, stream));
         a.first = static_cast<int32_t>(first);
-        a.pad_tokens = static_cast<int32_t>(pad);
-        JABAS_TRY(launch_logits_backward(a, s.planes, stream));
-        if (d_bias) JABAS_TRY(launch_bias_sum(b.db, static_cast<int32_t>(tiles(b.pad_rows)), n, n, static_cast<char*>(d_bias) + first * bytes, l->dtype, stream));
-        OutArgs o{};
-        o.scale = 1.0f / kDzScale;
-        o.out_stride = l->width;
-        o.out_dtype = l->dtype;
-        if (d_weight) {
-            o.a = Operand{b.dzt, a.dzt_stride, a.dzt_plane, static_cast<int32_t>(n)};
-            o.b = Operand{b.xt, b.pad_rows, l->width * b.pad_rows, static_cast<int32_t>(l->width)};
+        a.pad_tokens = pad;
+        JABAS_TRY(launch_logits_backward(a, s.planes, b.large, stream));
+        if (d_bias) JABAS_TRY(launch_bias_sum(b.db, row_tiles, n, n, static_cast<char*>(d_bias) + first * bytes, l->dtype, stream));
+        if (d_weight) {     // sum over the rows of dz[row][token] x[row][feature]
+            o.a = Operand{b.x16, s.depth, b.pad_rows * s.depth, depth};
+            o.b = Operand{b.dz, a.dz_stride, a.dz_plane, pad};
+            o.b_rows_of_k = 1;
+            o.n = static_cast<int32_t>(n);
             o.depth = static_cast<int32_t>(b.pad_rows);
-            o.unscale0 = b.unscale_xt;
+            o.unscale0 = b.unscale_x16;
             o.unscale1 = b.peak;
+            o.row_scale = nullptr;
+            o.acc = nullptr;
             o.out = static_cast<char*>(d_weight) + first * l->width * static_cast<int64_t>(bytes);
+            o.out_aligned = width % 4 == 0 && !misaligned(o.out, 4 * bytes);
             JABAS_TRY(launch_out(o, s.planes, stream));
         }
-        if (d_hidden) {
+        if (d_hidden) {     // sum over the tokens of dz[row][token] w[token][feature]
             lay.in = at(l->weight, first * l->weight_stride, l->dtype);
             lay.in_stride = l->weight_stride;
             lay.rows = static_cast<int32_t>(n);
+            lay.pad_rows = pad;
             lay.row_mask = l->bias ? at(l->bias, first, l->dtype) : nullptr;
-            lay.out = b.wt;
-            lay.out_stride = b.piece;
-            lay.out_plane = l->width * b.piece;
-            lay.pad = static_cast<int32_t>(pad);
-            lay.unscale = b.unscale_wt;
-            JABAS_TRY(launch_lay_columns(lay, stream));
-            o.a = Operand{b.dz, a.dz_stride, a.dz_plane, static_cast<int32_t>(l->rows)};
-            o.b = Operand{b.wt, b.piece, l->width * b.piece, static_cast<int32_t>(l->width)};
-            o.depth = static_cast<int32_t>(pad);
-            o.unscale0 = b.unscale_wt;
+            lay.out = b.w16;
+            lay.out_plane = b.piece * s.depth;
+            lay.unscale = b.unscale_w16;
+            JABAS_TRY(launch_lay_whole(lay, stream));
+            o.a = Operand{b.w16, s.depth, b.piece * s.depth, depth};
+            o.b = Operand{b.dz, a.dz_stride, a.dz_plane, rows};
+            o.b_rows_of_k = 0;
+            o.n = rows;
+            o.depth = pad;
+            o.unscale0 = b.unscale_w16;
             o.unscale1 = nullptr;
             o.row_scale = b.grad;
             o.acc = b.acc;
+            o.acc_stride = b.acc_stride;
             o.first = first == 0;
             o.last = first + b.piece >= l->vocab;
             o.out = d_hidden;
+            o.out_aligned = width % 4 == 0 && !misaligned(o.out, 4 * bytes);
             JABAS_TRY(launch_out(o, s.planes, stream));
         }
     }

@@ -27,11 +27,14 @@ static_assert(sizeof(RowState) == 16, "a row's state is one 16-byte load");
 // second plane with 2^11 times what the first leaves: 22 bits down to 2^-25, smallest steps of 2^-50.
 constexpr float kDzScale = 32768.0f, kLowScale = 2048.0f;
 
-constexpr int kTile = 128;      // rows and columns of a product's output tile
+constexpr int kTile = 256;      // the largest output tile of a product; pieces of the vocabulary are whole ones
 constexpr int kDepth = 64;      // elements of a product's inner axis are padded to a multiple of this
+constexpr int64_t kMaxStride = int64_t{1} << 22;    // of an operand: offsets inside a tile are 32 bits
 
-// An operand of a product: rows whose inner axis is contiguous and padded with zeros to the depth the call names,
-// 16-byte aligned; `plane` elements further on the second plane, where there is one.
+// An operand of a product, 16-byte aligned rows `stride` elements apart (at most kMaxStride); `plane` elements further on
+// the second plane, where there is one. Either a row holds the inner axis, zeros up to the depth the call names, and there
+// are `rows` of them; or there is a row for each place of the inner axis, zeros up to the depth, and it holds `rows` elements,
+// a multiple of 8.
 struct Operand {
     const void* p;
     int64_t stride, plane;
@@ -61,40 +64,45 @@ struct LogitsArgs {
     float2* partial;            // [tile of the vocabulary][row]: maximum of the raw logits, sum of 2^((z - max) c)
     float* total;               // [tile][row]: sum of the logits (label smoothing), or NULL
     float* entry_logit;         // [row][max(k, 1)]
-    int32_t first_tile;         // of the piece
     // backward
     const RowState* state;
     const float* row_grad;      // gradient of row n in units of dz (bias gradient)
     float uniform;              // e / V
     float hit;                  // what a label takes off: 1 - e
-    void* dz;                   // [row][token of the piece], fp16 planes
+    void* dz;                   // [row][token of the piece], fp16 planes, or NULL
     int64_t dz_stride, dz_plane;
-    void* dzt;                  // [token of the piece][row]
-    int64_t dzt_stride, dzt_plane;
     float* db;                  // [tile of the rows][token of the piece], or NULL
-    int32_t pad_rows, pad_tokens;   // dz and dzt are written (with zeros) up to these
+    int32_t pad_rows, pad_tokens;   // dz is written (with zeros) up to these
 };
 
 struct OutArgs {
-    Operand a, b;               // out[m][n] = scale * row_scale[m] * sum_k a[m][k] b[n][k]
+    Operand a, b;               // out[n][m] = scale * row_scale[n] * sum_k a[k][m] b[n][k] (b_rows_of_k: b[k][n])
+    int32_t b_rows_of_k;
+    int32_t m, n;
     int32_t depth;
     const float* unscale0;      // device scalars, or NULL
     const float* unscale1;
-    const float* row_scale;     // per m, or NULL
+    const float* row_scale;     // per n, or NULL
     float scale;
     float* acc;                 // fp32 sums over the pieces, or NULL where there is one piece
+    int64_t acc_stride;         // a multiple of 4
     int32_t first, last;        // of the pieces
     void* out;
     int64_t out_stride;
     int32_t out_dtype;
+    int32_t out_aligned;        // four elements of a row can be written at once
 };
 
-int launch_logits_forward(const LogitsArgs& a, int planes, hipStream_t stream);
-int launch_logits_backward(const LogitsArgs& a, int planes, hipStream_t stream);
+// Whether a product of m x n takes the large tiles, and how many of an operand's rows a tile of logits has.
+bool large_tiles(int64_t m, int64_t n, int planes);
+int logits_tile_tokens(bool large);
+int logits_tile_rows(bool large, int planes);
+int launch_logits_forward(const LogitsArgs& a, int planes, bool large, hipStream_t stream);
+int launch_logits_backward(const LogitsArgs& a, int planes, bool large, hipStream_t stream);
 int launch_out(const OutArgs& a, int planes, hipStream_t stream);
 
 // Layout of operands: padded copies, split into fp16 planes and scaled by powers of two where the product asks for it.
-constexpr int kMaxParts = 256;
+constexpr int kMaxParts = 1024;
 struct LayArgs {
     const void* in;
     int64_t in_stride;
@@ -102,15 +110,15 @@ struct LayArgs {
     int32_t rows, cols;         // of `in`
     const float* row_factor;    // per row of `in`, or NULL: rows with factor 0 are zeros whatever they hold, others are multiplied
     const void* row_mask;       // per row of `in`, in_dtype, or NULL: rows with -inf here (tokens that the bias rules out) are zeros
-    void* out;                  // launch_lay_rows: [rows][pad]; launch_lay_columns: [cols][pad]
+    void* out;                  // [pad_rows][pad]
     int64_t out_stride, out_plane;
-    int32_t pad;
+    int32_t pad_rows, pad;      // multiples of 8 columns
     int32_t planes;             // 0: copied as they are; 1 or 2 planes of fp16
-    float* unscale;             // written: per row (launch_lay_rows, planes > 0) or one (launch_lay_columns)
-    float* parts;               // launch_lay_columns: kMaxParts partial maxima
+    float* unscale;             // written: a factor per row (launch_lay_rows, planes > 0) or one for all (launch_lay_whole)
+    float* parts;               // launch_lay_whole: kMaxParts partial maxima
 };
 int launch_lay_rows(const LayArgs& a, hipStream_t stream);
-int launch_lay_columns(const LayArgs& a, hipStream_t stream);
+int launch_lay_whole(const LayArgs& a, hipStream_t stream);
 
 // Rows.
 struct TeacherArgs {

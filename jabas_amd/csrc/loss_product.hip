@@ -1,31 +1,10 @@
 // Matrix products of the losses: logits of a tile of tokens and rows that never leave the registers (forward: their
 // maxima and sums; backward: the row gradients dz), and the products of dz with the weight and the hidden states.
-#include "loss_internal.h"
+#include "loss_core.h"
 
 namespace jabas {
 namespace loss {
 namespace {
-
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
-struct F16 {
-    using vec = f16x8;
-    static __device__ f32x16 mfma(vec a, vec b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-};
-struct BF16 {
-    using vec = bf16x8;
-    static __device__ f32x16 mfma(vec a, vec b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-};
-
-__device__ inline f16x8 lowered(f16x8 v) { return v * static_cast<_Float16>(1.0f / kLowScale); }
-__device__ inline bf16x8 lowered(bf16x8 v) { return v; }     // one plane only
-
-constexpr int kThreads = 256;               // four waves, each a quarter (64 x 64) of the tile
-constexpr int kChunks = kTile * 8 / kThreads;   // 16-byte chunks of one operand's tile per thread
 
 __device__ inline float load_as_float(const void* p, int64_t i, int dtype) {
     if (dtype == JABAS_F32) return static_cast<const float*>(p)[i];
@@ -38,377 +17,429 @@ __device__ inline uint16_t to_bf16(float x) {
     return static_cast<uint16_t>((u + 0x7fffu + ((u >> 16) & 1)) >> 16);
 }
 
-__device__ inline void store_as(void* p, int64_t i, int dtype, float v) {
-    if (dtype == JABAS_F32) static_cast<float*>(p)[i] = v;
-    else static_cast<uint16_t*>(p)[i] = to_bf16(v);
+template <class C>
+__host__ __device__ inline int tiles_m(int m) { return (m + C::kM - 1) / C::kM; }
+template <class C>
+__host__ __device__ inline int tiles_n(int n) { return (n + C::kN - 1) / C::kN; }
+
+// Tile of a workgroup. Workgroups go round the eight dies (XCDs), each with an L2 of its own: each die takes a run of
+// consecutive tiles, in bands of eight tiles of m, so that the 32 tiles in flight on a die share their operands' rows.
+__device__ inline void tile_of(int tm, int tn, int& m, int& n) {
+    const int total = tm * tn, die = blockIdx.x & 7, each = total >> 3, left = total & 7;
+    const int at = die * each + min(die, left) + (blockIdx.x >> 3);
+    const int band = at / (8 * tn), first = band * 8, height = min(8, tm - first), in = at - band * 8 * tn;
+    m = first + in % height;
+    n = in / height;
 }
 
-// A row of a staged tile is 128 bytes, eight chunks of 16: one plane of 64 elements, or two planes of 32. Chunk c of row r
-// lies at chunk c ^ (r & 7): lanes that read the same chunk of eight rows then touch all banks once.
-template <int P>
-__device__ inline const u32x4* chunk_address(const Operand& o, int row, int chunk, int step) {
-    row = row < o.rows ? row : o.rows - 1;          // rows past the end are read again, never written
-    const uint16_t* p = static_cast<const uint16_t*>(o.p) + static_cast<int64_t>(row) * o.stride;
-    if (P == 2) p += (chunk >> 2) * o.plane + step * 32 + (chunk & 3) * 8;
-    else p += step * 64 + chunk * 8;
-    return reinterpret_cast<const u32x4*>(p);
-}
-
-// acc[i][j]: 32 x 32 blocks of out[m][n] = sum_k a[m][k] b[n][k] over this wave's 64 x 64. Element e of a block is
-// m = 8 (e / 4) + 4 (lane / 32) + e % 4, n = lane % 32.
-// Two planes: (a0 + a1)(b0 + b1) without a1 b1, which is under 2^-22 of the whole. kRaised: a's second plane is kept
-// larger by kLowScale, so b0 is made as much smaller for it.
-template <class E, int P, bool kRaised>
-__device__ inline void product(const Operand& a, const Operand& b, int m0, int n0, int depth, char* smem, f32x16 (&acc)[2][2]) {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    constexpr int kBytes = kTile * 128;
-    u32x4 ra[kChunks], rb[kChunks];
-    const int steps = depth / (P == 2 ? 32 : 64);
-    auto fetch = [&](int s) {
-#pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-            const int at = i * kThreads + t;
-            ra[i] = *chunk_address<P>(a, m0 + (at >> 3), at & 7, s);
-            rb[i] = *chunk_address<P>(b, n0 + (at >> 3), at & 7, s);
-        }
-    };
-    auto stage = [&](int buf) {
-        char* base = smem + buf * 2 * kBytes;
-#pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-            const int at = i * kThreads + t, row = at >> 3, c = (at & 7) ^ (row & 7);
-            *reinterpret_cast<u32x4*>(base + row * 128 + c * 16) = ra[i];
-            *reinterpret_cast<u32x4*>(base + kBytes + row * 128 + c * 16) = rb[i];
-        }
-    };
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-    fetch(0);
-    stage(0);
-    __syncthreads();
-    for (int s = 0; s < steps; ++s) {
-        if (s + 1 < steps) fetch(s + 1);
-        const char* base = smem + (s & 1) * 2 * kBytes;
-        auto read = [&](int row, int chunk) {
-            return *reinterpret_cast<const typename E::vec*>(base + row * 128 + ((chunk ^ (row & 7)) * 16));
-        };
-        const int r = lane & 31, h = lane >> 5;
-        if (P == 1) {
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-                typename E::vec fa[2], fb[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    fa[i] = read(wm + i * 32 + r, kk * 2 + h);
-                    fb[i] = read(kTile + wn + i * 32 + r, kk * 2 + h);
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) acc[i][j] = E::mfma(fa[i], fb[j], acc[i][j]);
-            }
-        } else {
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                typename E::vec fa[2][2], fb[2][2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        fa[i][q] = read(wm + i * 32 + r, q * 4 + kk * 2 + h);
-                        fb[i][q] = read(kTile + wn + i * 32 + r, q * 4 + kk * 2 + h);
-                    }
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        acc[i][j] = E::mfma(fa[i][1], kRaised ? lowered(fb[j][0]) : fb[j][0], acc[i][j]);
-                        acc[i][j] = E::mfma(fa[i][0], fb[j][1], acc[i][j]);
-                        acc[i][j] = E::mfma(fa[i][0], fb[j][0], acc[i][j]);
-                    }
-            }
-        }
-        if (s + 1 < steps) stage((s + 1) & 1);
-        __syncthreads();
-    }
-}
-
-__device__ inline int block_m(int i, int e, int lane) { return i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
-
-constexpr int kMapStride = kTile + 4;       // bytes of a row of the entry map: lanes of 32 rows read 32 banks
-
-// Which tokens of the tile are entries of which row: byte [row][token] is 1 + the entry's number. Built over the
-// operands' buffers, which nobody reads any more.
+// Which tokens of the tile are entries of which row: the byte of token m and row n, in the word [m / 4][n], is 1 + the entry's
+// number. Built over the operands' buffers, which nobody reads any more.
+template <class C>
 __device__ inline void build_map(const Entries& en, char* map, int first, int n0, int rows) {
-    const int t = threadIdx.x;
-    for (int i = t; i < kTile * kMapStride / 4; i += kThreads) reinterpret_cast<uint32_t*>(map)[i] = 0;
+    const int t = threadIdx.x, lane = t & 63;
+    for (int i = t; i < C::kM * C::kN / 16; i += C::kThreads) reinterpret_cast<u32x4*>(map)[i] = u32x4{0, 0, 0, 0};
     __syncthreads();
-    const int here = min(kTile, rows - n0) * en.k;
-    for (int i = t; i < here; i += kThreads) {
-        const int n = i / en.k, j = i - n * en.k;
-        const int v = en.index[static_cast<int64_t>(n0) * en.k + i] - first;
-        if (v >= 0 && v < kTile) map[n * kMapStride + v] = static_cast<char>(1 + j);
+    const int here = min(C::kN, rows - n0);
+    for (int n = t >> 6; n < here; n += C::kThreads / 64)
+        for (int j = lane; j < en.k; j += 64) {
+            const int v = en.index[static_cast<int64_t>(n0 + n) * en.k + j] - first;
+            if (v >= 0 && v < C::kM) map[((v >> 2) * C::kN + n) * 4 + (v & 3)] = static_cast<char>(1 + j);
+        }
+    __syncthreads();
+}
+
+// What a tile's logits take besides the product: the tokens' biases and, with two planes, the factors that undo the scaling of their
+// rows, in LDS (kM floats each).
+template <int P, class C>
+__device__ inline void load_tokens(const LogitsArgs& a, int m0, float* tokens) {
+    const int m = threadIdx.x;
+    if (m >= C::kM) return;
+    const int at = min(m0 + m, a.w.rows - 1);
+    tokens[m] = a.bias ? load_as_float(a.bias, static_cast<int64_t>(a.first) + at, a.bias_dtype) : 0.0f;
+    if (P == 2) tokens[C::kM + m] = a.unscale_w[at];
+}
+
+// The tile's logits into c.acc. One plane: the sums start from the biases.
+template <int P, class C>
+__device__ inline void logits_of(const LogitsArgs& a, int m0, int n0, char* smem, float* tokens, C& c) {
+    const int wm = C::wave_m();
+    c.run(a.w, a.x, m0, n0, a.depth, smem, [&] { load_tokens<P, C>(a, m0, tokens); },
+          [&](int i, int e) { return P == 1 ? tokens[wm + C::block_m(i, e)] : 0.0f; });
+    if (P == 1) return;
+#pragma unroll
+    for (int j = 0; j < C::kJ; ++j) {
+        const float ux = a.unscale_x[min(n0 + C::wave_n() + j * 32 + static_cast<int>(threadIdx.x & 31), a.x.rows - 1)];
+#pragma unroll
+        for (int i = 0; i < C::kI; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int m = wm + C::block_m(i, e);
+                c.acc[i][j][e] = c.acc[i][j][e] * ux * tokens[C::kM + m] + tokens[m];
+            }
     }
-    __syncthreads();
 }
 
-__device__ inline void wave_range(int& wm, int& wn) {
-    const int wave = threadIdx.x >> 6;
-    wm = (wave >> 1) * 64;
-    wn = (wave & 1) * 64;
+// The label of row n as a token of the tile, or -1.
+template <class C>
+__device__ inline int label_of(const LogitsArgs& a, int m0, int n) {
+    if (n >= a.x.rows) return -1;
+    const int64_t label = a.entries.target[n] - a.first - m0;
+    return label >= 0 && label < C::kM ? static_cast<int>(label) : -1;
 }
 
-// The tile's logits out of the accumulators: scaling undone, bias added.
-template <int P>
-__device__ inline void logits_of(const LogitsArgs& a, int m0, int n0, f32x16 (&acc)[2][2]) {
-    const int lane = threadIdx.x & 63;
-    int wm, wn;
-    wave_range(wm, wn);
+// f(i, e) for the element of this lane's block column that is token `label` of the tile, if one is. Few waves hold one: the others
+// pay a compare.
+template <class C, class F>
+__device__ inline void at_label(int label, const F& f) {
+    const int mine = label - C::wave_m();
+    if (!__any(label >= 0 && mine >= 0 && mine < C::kI * 32)) return;
+    const int at = label < 0 ? -1000 : mine - 4 * ((threadIdx.x & 63) >> 5);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < C::kI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int m = min(m0 + wm + block_m(i, e, lane), a.w.rows - 1);
-            const float b = a.bias ? load_as_float(a.bias, static_cast<int64_t>(a.first) + m, a.bias_dtype) : 0.0f;
-            const float uw = P == 2 ? a.unscale_w[m] : 1.0f;
+        for (int e = 0; e < 16; ++e)
+            if (at == i * 32 + 8 * (e >> 2) + (e & 3)) f(i, e);
+}
+
+template <class E, int P, class C, bool TEACHER>
+__global__ __launch_bounds__(C::kThreads) void logits_forward_kernel(LogitsArgs a) {
+    __shared__ __align__(16) char smem[2 * C::kStage];
+    __shared__ float tokens[P * C::kM];
+    int tm, tn;
+    tile_of(tiles_m<C>(a.w.rows), tiles_n<C>(a.x.rows), tm, tn);
+    const int m0 = tm * C::kM, n0 = tn * C::kN, lane = threadIdx.x & 63;
+    C c;
+    logits_of<P>(a, m0, n0, smem, tokens, c);
+    const int wm = C::wave_m(), wn = C::wave_n();
+    float peak[C::kJ], sum[C::kJ], total[C::kJ];
+    if (m0 + C::kM > a.w.rows) {        // tokens past the end
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float z = acc[i][j][e];
-                if (P == 2) z = z * a.unscale_x[min(n0 + wn + j * 32 + (lane & 31), a.x.rows - 1)] * uw;
-                acc[i][j][e] = z + b;
+        for (int i = 0; i < C::kI; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const bool in = m0 + wm + C::block_m(i, e) < a.w.rows;
+#pragma unroll
+                for (int j = 0; j < C::kJ; ++j)
+                    if (!in) c.acc[i][j][e] = -INFINITY;
+            }
+    }
+    if (TEACHER) build_map<C>(a.entries, smem, a.first + m0, n0, a.x.rows);
+#pragma unroll
+    for (int j = 0; j < C::kJ; ++j) {
+        const int nl = wn + j * 32 + (lane & 31), n = n0 + nl;
+        total[j] = 0.0f;
+        if (TEACHER) {          // entries join their row later, each by itself
+#pragma unroll
+            for (int i = 0; i < C::kI; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t hits = reinterpret_cast<const uint32_t*>(smem)[((wm + C::block_m(i, q * 4)) >> 2) * C::kN + nl];
+                    if (hits)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t hit = (hits >> (8 * e)) & 0xff;
+                            if (hit) {
+                                a.entry_logit[static_cast<int64_t>(n) * a.entries.k + hit - 1] = c.acc[i][j][q * 4 + e];
+                                c.acc[i][j][q * 4 + e] = -INFINITY;
+                            }
+                        }
+                }
+        } else {
+            at_label<C>(label_of<C>(a, m0, n), [&](int i, int e) { a.entry_logit[n] = c.acc[i][j][e]; });
+            if (a.total) {
+#pragma unroll
+                for (int i = 0; i < C::kI; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) total[j] += m0 + C::kM <= a.w.rows || m0 + wm + C::block_m(i, e) < a.w.rows ? c.acc[i][j][e] : 0.0f;
+                total[j] += __shfl_xor(total[j], 32);
             }
         }
-}
-
-template <class E, int P>
-__global__ __launch_bounds__(kThreads) void logits_forward_kernel(LogitsArgs a) {
-    __shared__ __align__(16) char smem[4 * kTile * 128];
-    const int tiles_m = (a.w.rows + kTile - 1) / kTile;
-    const int tm = blockIdx.x % tiles_m, tn = blockIdx.x / tiles_m;
-    const int m0 = tm * kTile, n0 = tn * kTile, lane = threadIdx.x & 63;
-    f32x16 acc[2][2];
-    product<E, P, false>(a.w, a.x, m0, n0, a.depth, smem, acc);
-    logits_of<P>(a, m0, n0, acc);
-    int wm, wn;
-    wave_range(wm, wn);
-    const bool teacher = a.entries.index != nullptr;
-    if (teacher) build_map(a.entries, smem, a.first + m0, n0, a.x.rows);
-    float peak[2], sum[2], total[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int nl = wn + j * 32 + (lane & 31), n = n0 + nl;
-        const bool row = n < a.x.rows;
-        const int64_t label = !teacher && row ? a.entries.target[n] - a.first - m0 : -1;
         peak[j] = -INFINITY;
-        total[j] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < C::kI; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int ml = wm + block_m(i, q * 4, lane);
-                const uint32_t hits = teacher ? *reinterpret_cast<const uint32_t*>(smem + nl * kMapStride + ml) : 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float z = acc[i][j][q * 4 + e];
-                    const bool in = m0 + ml + e < a.w.rows;
-                    if (in) total[j] += z;
-                    const uint32_t hit = (hits >> (8 * e)) & 0xff;
-                    if (hit) a.entry_logit[static_cast<int64_t>(n) * a.entries.k + hit - 1] = z;
-                    if (in && label == ml + e) a.entry_logit[n] = z;
-                    acc[i][j][q * 4 + e] = in && !hit ? z : -INFINITY;     // entries join their row later, each by itself
-                    peak[j] = fmaxf(peak[j], acc[i][j][q * 4 + e]);
-                }
-            }
+            for (int e = 0; e < 16; ++e) peak[j] = fmaxf(peak[j], c.acc[i][j][e]);
         peak[j] = fmaxf(peak[j], __shfl_xor(peak[j], 32));
         const float base = peak[j] == -INFINITY ? 0.0f : peak[j];
         sum[j] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < C::kI; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sum[j] += __builtin_amdgcn_exp2f((acc[i][j][e] - base) * a.c);
+            for (int e = 0; e < 16; ++e) sum[j] += __builtin_amdgcn_exp2f((c.acc[i][j][e] - base) * a.c);
         sum[j] += __shfl_xor(sum[j], 32);
-        total[j] += __shfl_xor(total[j], 32);
     }
+    // the waves that share rows: [wave of m][row of the tile]
+    constexpr int kWaves = C::kM / (C::kI * 32);
+    float* merge = reinterpret_cast<float*>(smem);
     __syncthreads();
-    float* merge = reinterpret_cast<float*>(smem);       // [3][128] of the waves that hold the upper half of the tile's tokens
-    if (wm != 0 && lane < 32) {
+    if (lane < 32)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int nl = wn + j * 32 + lane;
-            merge[nl] = peak[j];
-            merge[kTile + nl] = sum[j];
-            merge[2 * kTile + nl] = total[j];
+        for (int j = 0; j < C::kJ; ++j) {
+            float* at = merge + (wm / (C::kI * 32)) * C::kN + wn + j * 32 + lane;
+            at[0] = peak[j];
+            at[kWaves * C::kN] = sum[j];
+            at[2 * kWaves * C::kN] = total[j];
         }
-    }
     __syncthreads();
-    if (wm == 0 && lane < 32) {
+    const int nl = threadIdx.x, n = n0 + nl;
+    if (nl >= C::kN || n >= a.x.rows) return;
+    float p = merge[nl], s = 0.0f, t = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int nl = wn + j * 32 + lane, n = n0 + nl;
-            const float p2 = merge[nl], s2 = merge[kTile + nl];
-            const float p = fmaxf(peak[j], p2);
-            float s = 0.0f;
-            if (sum[j] != 0.0f) s += sum[j] * __builtin_amdgcn_exp2f((peak[j] - p) * a.c);
-            if (s2 != 0.0f) s += s2 * __builtin_amdgcn_exp2f((p2 - p) * a.c);
-            if (n < a.x.rows) {
-                const int64_t at = static_cast<int64_t>(a.first_tile + tm) * a.x.rows + n;
-                a.partial[at] = make_float2(p, s);
-                if (a.total) a.total[at] = total[j] + merge[2 * kTile + nl];
-            }
-        }
+    for (int w = 1; w < kWaves; ++w) p = fmaxf(p, merge[w * C::kN + nl]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        const float part = merge[(kWaves + w) * C::kN + nl];
+        if (part != 0.0f) s += part * __builtin_amdgcn_exp2f((merge[w * C::kN + nl] - p) * a.c);
+        t += merge[(2 * kWaves + w) * C::kN + nl];
     }
+    const int64_t at = static_cast<int64_t>(a.first / C::kM + tm) * a.x.rows + n;
+    a.partial[at] = make_float2(p, s);
+    if (a.total) a.total[at] = t;
 }
 
-template <class E, int P>
-__global__ __launch_bounds__(kThreads) void logits_backward_kernel(LogitsArgs a) {
-    __shared__ __align__(16) char smem[4 * kTile * 128];
-    const int tiles_m = (a.pad_tokens + kTile - 1) / kTile;
-    const int tm = blockIdx.x % tiles_m, tn = blockIdx.x / tiles_m;
-    const int m0 = tm * kTile, n0 = tn * kTile, lane = threadIdx.x & 63;
-    f32x16 acc[2][2];
-    product<E, P, false>(a.w, a.x, m0, n0, a.depth, smem, acc);
-    logits_of<P>(a, m0, n0, acc);
-    int wm, wn;
-    wave_range(wm, wn);
-    const bool teacher = a.entries.index != nullptr;
-    if (teacher) build_map(a.entries, smem, a.first + m0, n0, a.x.rows);
-    float grad[2];
+// Sums over 32 lanes of 32 values a lane, half of them handed over at every step: lane l ends with the sum of value l % 32 in
+// v[0].
+template <int HALF>
+__device__ inline void scatter_sum(float (&v)[32]) {
+    const bool upper = threadIdx.x & HALF;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int i = 0; i < HALF; ++i) {
+        const float give = upper ? v[i] : v[i + HALF], keep = upper ? v[i + HALF] : v[i];
+        v[i] = keep + __shfl_xor(give, HALF);
+    }
+    if constexpr (HALF > 1) scatter_sum<HALF / 2>(v);
+}
+
+template <class E, int P, class C, bool TEACHER>
+__global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs a) {
+    __shared__ __align__(16) char smem[2 * C::kStage];
+    __shared__ float tokens[P * C::kM];
+    int tm, tn;
+    tile_of(tiles_m<C>(a.w.rows), tiles_n<C>(a.x.rows), tm, tn);
+    const int m0 = tm * C::kM, n0 = tn * C::kN, lane = threadIdx.x & 63;
+    C c;
+    logits_of<P>(a, m0, n0, smem, tokens, c);
+    const int wm = C::wave_m(), wn = C::wave_n();
+    if (TEACHER) build_map<C>(a.entries, smem, a.first + m0, n0, a.x.rows);
+    const float uniform = a.uniform * kDzScale;
+#pragma unroll
+    for (int j = 0; j < C::kJ; ++j) {
         const int nl = wn + j * 32 + (lane & 31), n = n0 + nl;
-        const bool row = n < a.x.rows;
-        const RowState st = row ? a.state[n] : RowState{0.0f, 0.0f, 0.0f, 0.0f};
+        const RowState st = n < a.x.rows ? a.state[n] : RowState{0.0f, 0.0f, 0.0f, 0.0f};
         const bool counts = !(st.slope == 0.0f && st.mass == 0.0f);
-        const int64_t label = !teacher && row ? a.entries.target[n] - a.first - m0 : -1;
-        grad[j] = row ? a.row_grad[n] : 0.0f;
+        const float slope = st.slope * kDzScale;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < C::kI; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int ml = wm + block_m(i, q * 4, lane);
-                const uint32_t hits = teacher ? *reinterpret_cast<const uint32_t*>(smem + nl * kMapStride + ml) : 0;
+                const uint32_t hits = TEACHER ? reinterpret_cast<const uint32_t*>(smem)[((wm + C::block_m(i, q * 4)) >> 2) * C::kN + nl] : 0;
                 float d[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float z = acc[i][j][q * 4 + e];
-                    const uint32_t hit = (hits >> (8 * e)) & 0xff;
-                    if (hit) d[e] = st.mass * __builtin_amdgcn_exp2f((z - st.peak) * a.c) - a.entries.p[static_cast<int64_t>(n) * a.entries.k + hit - 1];
-                    else d[e] = st.slope * __builtin_amdgcn_exp2f((z - st.peak_rest) * a.c) - a.uniform;
-                    if (label == ml + e) d[e] -= a.hit;
-                    if (!counts || m0 + ml + e >= a.w.rows) d[e] = 0.0f;
-                    acc[i][j][q * 4 + e] = d[e];
-                }
-                f16x4 hi, lo;
+                for (int e = 0; e < 4; ++e) d[e] = fmaf(slope, __builtin_amdgcn_exp2f((c.acc[i][j][q * 4 + e] - st.peak_rest) * a.c), -uniform);
+                if (TEACHER && hits)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float v = d[e] * kDzScale;
-                    hi[e] = static_cast<_Float16>(v);
-                    if (P == 2) lo[e] = static_cast<_Float16>((v - static_cast<float>(hi[e])) * kLowScale);
-                }
-                _Float16* dz = static_cast<_Float16*>(a.dz) + static_cast<int64_t>(n) * a.dz_stride + m0 + ml;
-                _Float16* dzt = static_cast<_Float16*>(a.dzt) + static_cast<int64_t>(m0 + ml) * a.dzt_stride + n;
-                if (a.dz && row && m0 + ml < a.pad_tokens) {
-                    *reinterpret_cast<f16x4*>(dz) = hi;
-                    if (P == 2) *reinterpret_cast<f16x4*>(dz + a.dz_plane) = lo;
-                }
-                if (a.dzt && n < a.pad_rows) {
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t hit = (hits >> (8 * e)) & 0xff;
+                        if (hit)
+                            d[e] = (st.mass * __builtin_amdgcn_exp2f((c.acc[i][j][q * 4 + e] - st.peak) * a.c) -
+                                    a.entries.p[static_cast<int64_t>(n) * a.entries.k + hit - 1]) * kDzScale;
+                    }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (m0 + ml + e < a.w.rows) {
-                            dzt[e * a.dzt_stride] = hi[e];
-                            if (P == 2) dzt[e * a.dzt_stride + a.dzt_plane] = lo[e];
-                        }
-                }
+                for (int e = 0; e < 4; ++e) c.acc[i][j][q * 4 + e] = d[e];
             }
-    }
-    if (a.db) {      // sums over this tile's rows: within the wave, then over the two waves that share tokens
-        __syncthreads();
-        float* merge = reinterpret_cast<float*>(smem);
+        if (!TEACHER) at_label<C>(label_of<C>(a, m0, n), [&](int i, int e) { c.acc[i][j][e] -= a.hit * kDzScale; });
+        if (__any(!counts)) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < C::kI; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) c.acc[i][j][e] = counts ? c.acc[i][j][e] : 0.0f;
+        }
+    }
+    if (m0 + C::kM > a.w.rows) {        // tokens past the end
+#pragma unroll
+        for (int i = 0; i < C::kI; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                float s = acc[i][0][e] * grad[0] + acc[i][1][e] * grad[1];
+                const bool in = m0 + wm + C::block_m(i, e) < a.w.rows;
 #pragma unroll
-                for (int x = 1; x < 32; x <<= 1) s += __shfl_xor(s, x);
-                if ((lane & 31) == 0) merge[(wn ? kTile : 0) + wm + block_m(i, e, lane)] = s;
+                for (int j = 0; j < C::kJ; ++j)
+                    if (!in) c.acc[i][j][e] = 0.0f;
             }
+    }
+    if (a.db) {      // sums over this tile's rows: within the wave, then over the waves that share tokens
+        __syncthreads();
+        float* merge = reinterpret_cast<float*>(smem);
+        float g[C::kJ];
+#pragma unroll
+        for (int j = 0; j < C::kJ; ++j) {
+            const int n = n0 + wn + j * 32 + (lane & 31);
+            g[j] = n < a.x.rows ? a.row_grad[n] * (1.0f / kDzScale) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < C::kI; i += 2) {
+            float v[32];
+#pragma unroll
+            for (int x = 0; x < 32; ++x) {
+                v[x] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < C::kJ; ++j) v[x] += c.acc[i + (x >> 4)][j][x & 15] * g[j];
+            }
+            scatter_sum<16>(v);
+            merge[wn / (C::kJ * 32) * C::kM + wm + C::block_m(i + ((lane & 31) >> 4), lane & 15)] = v[0];
+        }
         __syncthreads();
         const int m = threadIdx.x;
-        if (m < kTile && m0 + m < a.w.rows) a.db[static_cast<int64_t>(tn) * a.w.rows + m0 + m] = merge[m] + merge[kTile + m];
+        if (m < C::kM && m0 + m < a.w.rows) {
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < C::kN / (C::kJ * 32); ++w) s += merge[w * C::kM + m];
+            a.db[static_cast<int64_t>(tn) * a.w.rows + m0 + m] = s;
+        }
+    }
+    if (!a.dz) return;
+    __syncthreads();
+    // The wave's part of dz through LDS, so that lanes write 16 consecutive bytes of a row: row n of kChunks chunks, chunk k at k ^ n % kChunks.
+    constexpr int kRows = C::kJ * 32, kChunks = C::kI * 32 / 8;
+    char* mine = smem + (threadIdx.x >> 6) * (kRows * kChunks * 16);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+#pragma unroll
+        for (int j = 0; j < C::kJ; ++j)
+#pragma unroll
+            for (int i = 0; i < C::kI; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    f16x4 h;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float v = c.acc[i][j][q * 4 + e];
+                        h[e] = static_cast<_Float16>(v);
+                        if (p) h[e] = static_cast<_Float16>((v - static_cast<float>(h[e])) * kLowScale);
+                    }
+                    const int r = j * 32 + (lane & 31), m = C::block_m(i, q * 4);
+                    *reinterpret_cast<f16x4*>(mine + (r * kChunks + ((m >> 3) ^ (r % kChunks))) * 16 + (m & 4) * 2) = h;
+                }
+        uint16_t* out = static_cast<uint16_t*>(a.dz) + p * a.dz_plane;
+#pragma unroll
+        for (int x = 0; x < kRows * kChunks / 64; ++x) {
+            const int f = x * 64 + lane, r = f / kChunks, k = f % kChunks;
+            const u32x4 v = *reinterpret_cast<const u32x4*>(mine + (r * kChunks + (k ^ (r % kChunks))) * 16);
+            const int n = n0 + wn + r, m = m0 + wm + k * 8;
+            if (n < a.pad_rows && m < a.pad_tokens) *reinterpret_cast<u32x4*>(out + static_cast<int64_t>(n) * a.dz_stride + m) = v;
+        }
     }
 }
 
-template <int P>
-__global__ __launch_bounds__(kThreads) void out_kernel(OutArgs a) {
-    __shared__ __align__(16) char smem[4 * kTile * 128];
-    const int tiles_m = (a.a.rows + kTile - 1) / kTile;
-    const int tm = blockIdx.x % tiles_m, tn = blockIdx.x / tiles_m;
-    const int m0 = tm * kTile, n0 = tn * kTile, lane = threadIdx.x & 63;
-    f32x16 acc[2][2];
-    product<F16, P, P == 2>(a.a, a.b, m0, n0, a.depth, smem, acc);
-    int wm, wn;
-    wave_range(wm, wn);
+template <int P, class C>
+__global__ __launch_bounds__(C::kThreads) void out_kernel(OutArgs a) {
+    __shared__ __align__(16) char smem[2 * C::kStage];
+    int tm, tn;
+    tile_of(tiles_m<C>(a.m), tiles_n<C>(a.n), tm, tn);
+    const int m0 = tm * C::kM, n0 = tn * C::kN, lane = threadIdx.x & 63;
+    C c;
+    c.run(a.a, a.b, m0, n0, a.depth, smem, [] {}, [](int, int) { return 0.0f; });
+    const int wm = C::wave_m(), wn = C::wave_n();
     float scale = a.scale;
     if (a.unscale0) scale *= *a.unscale0;
     const float second = a.unscale1 ? *a.unscale1 : 1.0f;
+    // 32 rows of the wave at a time through LDS: row n of kChunks 16-byte chunks, chunk k at k ^ n % kChunks
+    constexpr int kChunks = C::kI * 32 / 4;
+    float* mine = reinterpret_cast<float*>(smem + (threadIdx.x >> 6) * (32 * kChunks * 16));
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < C::kJ; ++j) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int m = m0 + wm + block_m(i, e, lane);
-            if (m >= a.a.rows) continue;
-            const float rs = a.row_scale ? a.row_scale[m] : 1.0f;
+        for (int i = 0; i < C::kI; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int n = n0 + wn + j * 32 + (lane & 31);
-                if (n >= a.b.rows) continue;
-                float v = acc[i][j][e] * scale * second;        // the pieces of a sum have scales of their own
-                if (a.acc) {
-                    float* sum = a.acc + static_cast<int64_t>(m) * a.b.rows + n;
-                    if (!a.first) v += *sum;
-                    if (!a.last) {
-                        *sum = v;
-                        continue;
-                    }
+            for (int q = 0; q < 4; ++q) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = c.acc[i][j][q * 4 + e] * scale * second;    // the pieces of a sum have scales of their own
+                const int r = lane & 31, m = C::block_m(i, q * 4);
+                *reinterpret_cast<f32x4*>(mine + (r * kChunks + ((m >> 2) ^ (r % kChunks))) * 4) = v;
+            }
+#pragma unroll
+        for (int x = 0; x < 32 * kChunks / 64; ++x) {
+            const int f = x * 64 + lane, r = f / kChunks, k = f % kChunks;
+            f32x4 v = *reinterpret_cast<const f32x4*>(mine + (r * kChunks + (k ^ (r % kChunks))) * 4);
+            const int n = n0 + wn + j * 32 + r, m = m0 + wm + k * 4;
+            if (n >= a.n || m >= a.m) continue;
+            const int here = min(4, a.m - m);
+            if (a.acc) {
+                float* sum = a.acc + static_cast<int64_t>(n) * a.acc_stride + m;       // rows padded to four
+                if (!a.first) v += *reinterpret_cast<const f32x4*>(sum);
+                if (!a.last) {
+                    *reinterpret_cast<f32x4*>(sum) = v;
+                    continue;
                 }
-                // a row that does not count is zero even where its neighbours' scale is not finite
-                v = rs == 0.0f ? 0.0f : v * rs;
-                store_as(a.out, static_cast<int64_t>(m) * a.out_stride + n, a.out_dtype, v);
+            }
+            if (a.row_scale) {      // a row that does not count is zero even where its neighbours' scale is not finite
+                const float rs = a.row_scale[n];
+                v = rs == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v * rs;
+            }
+            const int64_t at = static_cast<int64_t>(n) * a.out_stride + m;
+            if (a.out_dtype == JABAS_F32) {
+                float* out = static_cast<float*>(a.out) + at;
+                if (a.out_aligned) *reinterpret_cast<f32x4*>(out) = v;
+                else
+                    for (int e = 0; e < here; ++e) out[e] = v[e];
+            } else {
+                uint16_t* out = static_cast<uint16_t*>(a.out) + at;
+                const uint16_t h[4] = {to_bf16(v[0]), to_bf16(v[1]), to_bf16(v[2]), to_bf16(v[3])};
+                if (a.out_aligned) *reinterpret_cast<uint64_t*>(out) = h[0] | static_cast<uint64_t>(h[1]) << 16 | static_cast<uint64_t>(h[2]) << 32 | static_cast<uint64_t>(h[3]) << 48;
+                else
+                    for (int e = 0; e < here; ++e) out[e] = h[e];
             }
         }
+    }
 }
 
-inline int tiles(int64_t n) { return static_cast<int>((n + kTile - 1) / kTile); }
-
-inline int launched() { return hipGetLastError() == hipSuccess ? JABAS_OK : JABAS_ERR_LAUNCH; }
 
 template <class K, class A>
-int launch(K kernel, unsigned grid, const A& args, hipStream_t stream) {
+int launch(K kernel, int64_t grid, int threads, const A& args, hipStream_t stream) {
     void* params[] = {const_cast<A*>(&args)};
-    return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3(grid), dim3(kThreads), params, 0, stream) == hipSuccess ? JABAS_OK : JABAS_ERR_LAUNCH;
+    return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3(static_cast<unsigned>(grid)), dim3(threads), params, 0, stream) == hipSuccess
+               ? JABAS_OK : JABAS_ERR_LAUNCH;
+}
+
+template <class E, int P, int TM, int TN, int WM, int WN>
+int logits(const LogitsArgs& a, bool backward, hipStream_t stream) {
+    using C = Core<E, P, TM, TN, WM, WN, false, false, false>;
+    const int64_t grid = static_cast<int64_t>(tiles_m<C>(a.w.rows)) * tiles_n<C>(a.x.rows);
+    if (a.entries.index)
+        return backward ? launch(logits_backward_kernel<E, P, C, true>, grid, C::kThreads, a, stream) : launch(logits_forward_kernel<E, P, C, true>, grid, C::kThreads, a, stream);
+    return backward ? launch(logits_backward_kernel<E, P, C, false>, grid, C::kThreads, a, stream) : launch(logits_forward_kernel<E, P, C, false>, grid, C::kThreads, a, stream);
+}
+
+int logits(const LogitsArgs& a, int planes, bool large, bool backward, hipStream_t stream) {
+    if (planes == 2) return large ? logits<F16, 2, 256, 128, 4, 2>(a, backward, stream) : logits<F16, 2, 128, 128, 2, 2>(a, backward, stream);
+    return large ? logits<BF16, 1, 256, 256, 2, 4>(a, backward, stream) : logits<BF16, 1, 128, 128, 2, 2>(a, backward, stream);
+}
+
+template <int P, int TM, int TN, int WM, int WN>
+int out(const OutArgs& a, hipStream_t stream) {
+    if (a.b_rows_of_k) {
+        using C = Core<F16, P, TM, TN, WM, WN, true, true, P == 2>;
+        return launch(out_kernel<P, C>, static_cast<int64_t>(tiles_m<C>(a.m)) * tiles_n<C>(a.n), C::kThreads, a, stream);
+    }
+    using C = Core<F16, P, TM, TN, WM, WN, true, false, P == 2>;
+    return launch(out_kernel<P, C>, static_cast<int64_t>(tiles_m<C>(a.m)) * tiles_n<C>(a.n), C::kThreads, a, stream);
 }
 
 }  // namespace
 
-int launch_logits_forward(const LogitsArgs& a, int planes, hipStream_t stream) {
-    const unsigned grid = static_cast<unsigned>(tiles(a.w.rows)) * tiles(a.x.rows);
-    return planes == 2 ? launch(logits_forward_kernel<F16, 2>, grid, a, stream) : launch(logits_forward_kernel<BF16, 1>, grid, a, stream);
+bool large_tiles(int64_t m, int64_t n, int planes) {
+    return ((m + 255) / 256) * (planes == 2 ? (n + 127) / 128 : (n + 255) / 256) >= 256;
 }
+int logits_tile_tokens(bool large) { return large ? 256 : 128; }
+int logits_tile_rows(bool large, int planes) { return large && planes == 1 ? 256 : 128; }
 
-int launch_logits_backward(const LogitsArgs& a, int planes, hipStream_t stream) {
-    const unsigned grid = static_cast<unsigned>(tiles(a.pad_tokens)) * tiles(a.pad_rows);
-    return planes == 2 ? launch(logits_backward_kernel<F16, 2>, grid, a, stream) : launch(logits_backward_kernel<BF16, 1>, grid, a, stream);
-}
-
+int launch_logits_forward(const LogitsArgs& a, int planes, bool large, hipStream_t stream) { return logits(a, planes, large, false, stream); }
+int launch_logits_backward(const LogitsArgs& a, int planes, bool large, hipStream_t stream) { return logits(a, planes, large, true, stream); }
 int launch_out(const OutArgs& a, int planes, hipStream_t stream) {
-    const unsigned grid = static_cast<unsigned>(tiles(a.a.rows)) * tiles(a.b.rows);
-    return planes == 2 ? launch(out_kernel<2>, grid, a, stream) : launch(out_kernel<1>, grid, a, stream);
+    const bool large = large_tiles(a.m, a.n, planes);
+    if (planes == 2) return large ? out<2, 256, 128, 4, 2>(a, stream) : out<2, 128, 128, 2, 2>(a, stream);
+    return large ? out<1, 256, 256, 2, 4>(a, stream) : out<1, 128, 128, 2, 2>(a, stream);
 }
 
 // ------------------------------------------------------------------ layout of operands
@@ -436,13 +467,38 @@ __device__ inline float wave_max(float x) {
     return x;
 }
 
-__device__ inline void put_planes(_Float16* p, int64_t plane, int planes, float v) {
-    const _Float16 hi = static_cast<_Float16>(v);
-    p[0] = hi;
-    if (planes == 2) {
-        const float f = static_cast<float>(hi);
-        p[plane] = static_cast<_Float16>(fabsf(f) < INFINITY ? v - f : 0.0f);
+// Eight elements of a row from column c on, zeros past the end; any alignment.
+struct __attribute__((packed, aligned(2))) Eight16 { uint16_t v[8]; };
+struct __attribute__((packed, aligned(4))) Eight32 { float v[8]; };
+__device__ inline void load_eight(const LayArgs& a, int64_t row, int c, float (&v)[8]) {
+    const int64_t at = row * a.in_stride + c;
+    if (c + 8 <= a.cols) {
+        if (a.in_dtype == JABAS_F32) {
+            const Eight32 x = *reinterpret_cast<const Eight32*>(static_cast<const float*>(a.in) + at);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = x.v[i];
+        } else {
+            const Eight16 x = *reinterpret_cast<const Eight16*>(static_cast<const uint16_t*>(a.in) + at);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(static_cast<uint32_t>(x.v[i]) << 16);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < a.cols ? load_as_float(a.in, at + i, a.in_dtype) : 0.0f;
     }
+}
+
+__device__ inline void store_eight(const LayArgs& a, int64_t row, int c, const float (&v)[8]) {
+    _Float16* p = static_cast<_Float16*>(a.out) + row * a.out_stride + c;
+    f16x8 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        hi[i] = static_cast<_Float16>(v[i]);
+        const float f = static_cast<float>(hi[i]);
+        lo[i] = static_cast<_Float16>(fabsf(f) < INFINITY ? v[i] - f : 0.0f);
+    }
+    *reinterpret_cast<f16x8*>(p) = hi;
+    if (a.planes == 2) *reinterpret_cast<f16x8*>(p + a.out_plane) = lo;
 }
 
 __device__ inline float row_keeps(const LayArgs& a, int row) {
@@ -454,79 +510,96 @@ __device__ inline float row_keeps(const LayArgs& a, int row) {
 __global__ __launch_bounds__(kLayThreads) void lay_rows_kernel(LayArgs a) {
     const int row = blockIdx.x * (kLayThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (row >= a.rows) return;
-    const int64_t at = static_cast<int64_t>(row) * a.in_stride;
     if (a.planes == 0) {
+        const uint16_t* in = static_cast<const uint16_t*>(a.in) + static_cast<int64_t>(row) * a.in_stride;
         uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(row) * a.out_stride;
-        for (int c = lane; c < a.pad; c += 64) out[c] = c < a.cols ? static_cast<const uint16_t*>(a.in)[at + c] : 0;
+        for (int c = lane * 8; c < a.pad; c += 512) {
+            Eight16 x;
+            if (c + 8 <= a.cols) x = *reinterpret_cast<const Eight16*>(in + c);
+            else
+                for (int i = 0; i < 8; ++i) x.v[i] = c + i < a.cols ? in[c + i] : 0;
+            u32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = x.v[2 * i] | static_cast<uint32_t>(x.v[2 * i + 1]) << 16;
+            *reinterpret_cast<u32x4*>(out + c) = v;
+        }
         return;
     }
-    float peak = 0.0f;
-    for (int c = lane; c < a.cols; c += 64) peak = fmaxf(peak, finite_size(load_as_float(a.in, at + c, a.in_dtype)));
+    float peak = 0.0f, v[8];
+    for (int c = lane * 8; c < a.cols; c += 512) {
+        load_eight(a, row, c, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) peak = fmaxf(peak, finite_size(v[i]));
+    }
     const int e = scale_exponent(wave_max(peak));
     const float scale = power_of_two(e);
-    _Float16* out = static_cast<_Float16*>(a.out) + static_cast<int64_t>(row) * a.out_stride;
-    for (int c = lane; c < a.pad; c += 64)
-        put_planes(out + c, a.out_plane, a.planes, c < a.cols ? load_as_float(a.in, at + c, a.in_dtype) * scale : 0.0f);
+    for (int c = lane * 8; c < a.pad; c += 512) {
+        load_eight(a, row, c, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= scale;
+        store_eight(a, row, c, v);
+    }
     if (lane == 0) a.unscale[row] = power_of_two(-e);
 }
 
 __global__ __launch_bounds__(kLayThreads) void absmax_kernel(LayArgs a) {
     __shared__ float merge[kLayThreads / 64];
-    float peak = 0.0f;
-    for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const int lane = threadIdx.x & 63;
+    float peak = 0.0f, v[8];
+    for (int row = blockIdx.x * (kLayThreads / 64) + (threadIdx.x >> 6); row < a.rows; row += gridDim.x * (kLayThreads / 64)) {
         const float f = row_keeps(a, row);
         if (f == 0.0f) continue;
-        float here = 0.0f;
-        for (int c = threadIdx.x; c < a.cols; c += kLayThreads)
-            here = fmaxf(here, finite_size(load_as_float(a.in, static_cast<int64_t>(row) * a.in_stride + c, a.in_dtype) * f));
-        peak = fmaxf(peak, here);
+        for (int c = lane * 8; c < a.cols; c += 512) {
+            load_eight(a, row, c, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) peak = fmaxf(peak, finite_size(v[i] * f));
+        }
     }
     peak = wave_max(peak);
-    if ((threadIdx.x & 63) == 0) merge[threadIdx.x >> 6] = peak;
+    if (lane == 0) merge[threadIdx.x >> 6] = peak;
     __syncthreads();
     if (threadIdx.x == 0) a.parts[blockIdx.x] = fmaxf(fmaxf(merge[0], merge[1]), fmaxf(merge[2], merge[3]));
 }
 
-// 64 x 64 elements through LDS: out[col][row].
-__global__ __launch_bounds__(kLayThreads) void lay_columns_kernel(LayArgs a) {
-    __shared__ float tile[64][65];
+// A wave per row, one scale for all of them.
+__global__ __launch_bounds__(kLayThreads) void lay_whole_kernel(LayArgs a) {
     __shared__ float merge[kLayThreads / 64];
-    const int t = threadIdx.x, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
-    float peak = wave_max(a.parts[t]);
-    static_assert(kMaxParts == kLayThreads, "a partial maximum per thread");
-    if ((t & 63) == 0) merge[t >> 6] = peak;
-    for (int i = t; i < 64 * 64; i += kLayThreads) {
-        const int r = i >> 6, c = i & 63;
-        float v = 0.0f;
-        if (r0 + r < a.rows && c0 + c < a.cols) {
-            const float f = row_keeps(a, r0 + r);
-            if (f != 0.0f) v = load_as_float(a.in, static_cast<int64_t>(r0 + r) * a.in_stride + c0 + c, a.in_dtype) * f;
-        }
-        tile[r][c] = v;
-    }
+    static_assert(kMaxParts % kLayThreads == 0, "as many partial maxima per thread");
+    const int t = threadIdx.x, lane = t & 63;
+    float peak = 0.0f, v[8];
+#pragma unroll
+    for (int i = 0; i < kMaxParts; i += kLayThreads) peak = fmaxf(peak, a.parts[i + t]);
+    peak = wave_max(peak);
+    if (lane == 0) merge[t >> 6] = peak;
     __syncthreads();
     peak = fmaxf(fmaxf(merge[0], merge[1]), fmaxf(merge[2], merge[3]));
     const int e = scale_exponent(peak);
-    const float scale = power_of_two(e);
-    if (t == 0 && blockIdx.x == 0 && blockIdx.y == 0) *a.unscale = power_of_two(-e);
-    for (int i = t; i < 64 * 64; i += kLayThreads) {
-        const int c = i >> 6, r = i & 63;
-        if (c0 + c < a.cols && r0 + r < a.pad)
-            put_planes(static_cast<_Float16*>(a.out) + static_cast<int64_t>(c0 + c) * a.out_stride + r0 + r, a.out_plane, a.planes, tile[r][c] * scale);
+    if (t == 0 && blockIdx.x == 0) *a.unscale = power_of_two(-e);
+    const int row = blockIdx.x * (kLayThreads / 64) + (t >> 6);
+    if (row >= a.pad_rows) return;
+    const float f = row < a.rows ? row_keeps(a, row) : 0.0f, scale = power_of_two(e);
+    for (int c = lane * 8; c < a.pad; c += 512) {
+        if (f != 0.0f) {
+            load_eight(a, row, c, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = v[i] * f * scale;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        }
+        store_eight(a, row, c, v);
     }
 }
 
 }  // namespace
 
 int launch_lay_rows(const LayArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL(lay_rows_kernel, dim3((a.rows + 3) / 4), dim3(kLayThreads), 0, stream, a);
-    return launched();
+    return launch(lay_rows_kernel, (a.rows + 3) / 4, kLayThreads, a, stream);
 }
 
-int launch_lay_columns(const LayArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL(absmax_kernel, dim3(kMaxParts), dim3(kLayThreads), 0, stream, a);
-    hipLaunchKernelGGL(lay_columns_kernel, dim3((a.pad + 63) / 64, (a.cols + 63) / 64), dim3(kLayThreads), 0, stream, a);
-    return launched();
+int launch_lay_whole(const LayArgs& a, hipStream_t stream) {
+    const int status = launch(absmax_kernel, kMaxParts, kLayThreads, a, stream);
+    return status != JABAS_OK ? status : launch(lay_whole_kernel, (a.pad_rows + 3) / 4, kLayThreads, a, stream);
 }
 
 }  // namespace loss
