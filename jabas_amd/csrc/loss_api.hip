@@ -11,6 +11,7 @@ namespace {
 
 constexpr int64_t kMaxSize = int64_t{1} << 30;      // rows, tokens; the tiles' numbers and tokens are 32 bits in the kernels
 constexpr int64_t kMaxWidth = int64_t{1} << 20;
+constexpr int64_t kMaxLinearRows = kMaxStride;      // a feature's hidden states are one row of an operand
 
 inline int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 inline int64_t tiles(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
@@ -36,7 +37,7 @@ int validate(const JabasLoss* l, Shape& s) {
     if (l->rows < 0 || l->rows > kMaxSize || l->vocab < 1 || l->vocab > kMaxSize) return JABAS_ERR_SIZE;
     if (s.linear) {
         if (!l->weight || (!l->hidden && l->rows) || l->logits) return JABAS_ERR_NULL;
-        if (l->width < 1 || l->width > kMaxWidth || l->hidden_stride < 0 || l->weight_stride < 0) return JABAS_ERR_SIZE;
+        if (l->rows > kMaxLinearRows || l->width < 1 || l->width > kMaxWidth || l->hidden_stride < 0 || l->weight_stride < 0) return JABAS_ERR_SIZE;
         if (tiles(l->rows, 128) * tiles(l->vocab, 128) > 0x7fffffff) return JABAS_ERR_SIZE;
     } else {
         if ((!l->logits && l->rows) || l->bias || !s.teacher) return JABAS_ERR_NULL;
@@ -154,8 +155,9 @@ struct Backward {
     uint16_t *x, *w;            // operands of the logits, where they are copies
     uint16_t *x16, *w16, *dz;   // of the gradients' products
     float *unscale_x, *unscale_w, *unscale_x16, *unscale_w16, *parts;
-    float *acc, *db;
-    int64_t piece, pad_rows, acc_stride, splits, chunk;
+    float *db, *part_w, *part_h;
+    int64_t piece, pad_rows, part_stride, splits, chunk;
+    Splits inner;
     bool large;
 };
 
@@ -179,12 +181,15 @@ size_t carve_backward(const JabasLoss* l, const Shape& s, char* base, Backward& 
     b.unscale_x16 = c.take<float>(1);
     b.unscale_w16 = c.take<float>(1);
     b.parts = c.take<float>(kMaxParts);
-    b.x16 = c.take<uint16_t>(b.pad_rows * s.depth * s.planes);
-    b.w16 = c.take<uint16_t>(b.piece * s.depth * s.planes);
+    b.x16 = c.take<uint16_t>(l->width * b.pad_rows * s.planes);
+    b.w16 = c.take<uint16_t>(l->width * b.piece * s.planes);
     b.dz = c.take<uint16_t>(b.pad_rows * b.piece * s.planes);
-    b.acc_stride = round_up(l->width, 4);
-    if (b.piece < l->vocab) b.acc = c.take<float>(rows * b.acc_stride);
-    b.large = large_tiles(b.piece < l->vocab ? b.piece : l->vocab, rows, s.planes);
+    b.part_stride = round_up(l->width, 4);
+    const int64_t tokens = b.piece < l->vocab ? b.piece : l->vocab;
+    b.inner = choose_splits(l->width, tokens, rows, true, true, b.piece < l->vocab, s.planes);
+    if (b.inner.w > 1) b.part_w = c.take<float>(b.inner.w * tokens * b.part_stride);
+    if (b.inner.h > 1 || b.piece < l->vocab) b.part_h = c.take<float>(b.inner.h * rows * b.part_stride);
+    b.large = large_tiles(tokens, rows, s.planes);
     if (l->bias) b.db = c.take<float>(tiles(rows, logits_tile_rows(b.large, s.planes)) * b.piece);
     return c.used;
 }
@@ -289,8 +294,7 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     if (!loss_out && (l->rows || l->reduction != JABAS_LOSS_NONE)) return JABAS_ERR_NULL;
     Forward f;
-    if (!workspace || misaligned(workspace, 256) || workspace_bytes < carve_forward(l, s, nullptr, f)) return JABAS_ERR_WORKSPACE;
-    carve_forward(l, s, static_cast<char*>(workspace), f);
+    if (!workspace || misaligned(workspace, 256) || workspace_bytes < carve_forward(l, s, static_cast<char*>(workspace), f)) return JABAS_ERR_WORKSPACE;
     RowState* state = reinterpret_cast<RowState*>(l->row_state);
     float* reduce = l->row_state + 4 * l->rows;
     if (!l->rows) return launch_reduce(f.row_loss, state, 0, l->reduction, loss_out, reduce, stream);
@@ -377,8 +381,7 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     if (misaligned(d_hidden, bytes) || misaligned(d_weight, bytes) || misaligned(d_bias, bytes) || misaligned(d_logits, bytes) || misaligned(upstream, 4))
         return JABAS_ERR_ALIGN;
     Backward b;
-    if (!workspace || misaligned(workspace, 256) || workspace_bytes < carve_backward(l, s, nullptr, b)) return JABAS_ERR_WORKSPACE;
-    carve_backward(l, s, static_cast<char*>(workspace), b);
+    if (!workspace || misaligned(workspace, 256) || workspace_bytes < carve_backward(l, s, static_cast<char*>(workspace), b)) return JABAS_ERR_WORKSPACE;
     if (!l->rows) {
         if (d_weight) JABAS_TRY(launch_zero(d_weight, static_cast<size_t>(l->vocab) * l->width * bytes, stream));
         if (d_bias) JABAS_TRY(launch_zero(d_bias, static_cast<size_t>(l->vocab) * bytes, stream));
@@ -429,28 +432,38 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     LayArgs lay{};
     lay.in_dtype = l->dtype;
     lay.cols = static_cast<int32_t>(l->width);
-    lay.out_stride = s.depth;
-    lay.pad = static_cast<int32_t>(s.depth);
     lay.planes = s.planes;
     lay.parts = b.parts;
     if (d_weight) {
         lay.in = l->hidden;
         lay.in_stride = l->hidden_stride;
         lay.rows = static_cast<int32_t>(l->rows);
-        lay.pad_rows = static_cast<int32_t>(b.pad_rows);
         lay.row_factor = b.ratio;
         lay.out = b.x16;
-        lay.out_plane = b.pad_rows * s.depth;
+        lay.out_stride = b.pad_rows;
+        lay.out_plane = l->width * b.pad_rows;
+        lay.pad = static_cast<int32_t>(b.pad_rows);
         lay.unscale = b.unscale_x16;
-        JABAS_TRY(launch_lay_whole(lay, stream));
+        JABAS_TRY(launch_lay_columns(lay, stream));
     }
     lay.row_factor = nullptr;
-    const int32_t width = static_cast<int32_t>(l->width), depth = static_cast<int32_t>(s.depth), rows = static_cast<int32_t>(l->rows);
-    OutArgs o{};
-    o.scale = 1.0f / kDzScale;
-    o.m = width;
-    o.out_stride = l->width;
-    o.out_dtype = l->dtype;
+    lay.in_stride = l->weight_stride;
+    lay.out = b.w16;
+    lay.out_stride = b.piece;
+    lay.out_plane = l->width * b.piece;
+    lay.unscale = b.unscale_w16;
+    const int32_t width = static_cast<int32_t>(l->width), rows = static_cast<int32_t>(l->rows);
+    const auto each = [](int64_t depth, int splits) { return static_cast<int32_t>(round_up((depth + splits - 1) / splits, kDepth)); };
+    const auto splits = [](int64_t depth, int64_t each) { return static_cast<int32_t>((depth + each - 1) / each); };
+    GradArgs g{};
+    const int64_t whole = round_up(l->vocab < b.piece ? l->vocab : b.piece, kDepth);        // the first piece, the largest
+    g.h.each = each(whole, b.inner.h);
+    const int32_t splits_h = splits(whole, g.h.each);
+    g.w.scale = g.h.scale = 1.0f / kDzScale;
+    g.w.out_stride = g.h.out_stride = l->width;
+    g.w.out_dtype = g.h.out_dtype = l->dtype;
+    g.w.part_stride = g.h.part_stride = b.part_stride;
+    g.w.splits = g.h.splits = 1;
     for (int64_t first = 0; first < l->vocab; first += b.piece) {
         const int64_t n = l->vocab - first < b.piece ? l->vocab - first : b.piece;
         const int32_t pad = static_cast<int32_t>(round_up(n, kDepth));
@@ -459,46 +472,48 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
         a.pad_tokens = pad;
         JABAS_TRY(launch_logits_backward(a, s.planes, b.large, stream));
         if (d_bias) JABAS_TRY(launch_bias_sum(b.db, row_tiles, n, n, static_cast<char*>(d_bias) + first * bytes, l->dtype, stream));
+        if (!d_weight && !d_hidden) continue;
         if (d_weight) {     // sum over the rows of dz[row][token] x[row][feature]
-            o.a = Operand{b.x16, s.depth, b.pad_rows * s.depth, depth};
-            o.b = Operand{b.dz, a.dz_stride, a.dz_plane, pad};
-            o.b_rows_of_k = 1;
-            o.n = static_cast<int32_t>(n);
-            o.depth = static_cast<int32_t>(b.pad_rows);
-            o.unscale0 = b.unscale_x16;
-            o.unscale1 = b.peak;
-            o.row_scale = nullptr;
-            o.acc = nullptr;
-            o.out = static_cast<char*>(d_weight) + first * l->width * static_cast<int64_t>(bytes);
-            o.out_aligned = width % 4 == 0 && !misaligned(o.out, 4 * bytes);
-            JABAS_TRY(launch_out(o, s.planes, stream));
+            g.w.a = Operand{b.x16, b.pad_rows, l->width * b.pad_rows, width};
+            g.w.b = Operand{b.dz, a.dz_stride, a.dz_plane, pad};
+            g.w.m = width;
+            g.w.n = static_cast<int32_t>(n);
+            g.w.depth = static_cast<int32_t>(b.pad_rows);
+            g.w.each = each(b.pad_rows, b.inner.w);
+            g.w.splits = splits(b.pad_rows, g.w.each);
+            g.w.unscale0 = b.unscale_x16;
+            g.w.unscale1 = b.peak;
+            g.w.part = g.w.splits > 1 ? b.part_w : nullptr;
+            g.w.part_plane = n * b.part_stride;
+            g.w.first = g.w.keep = 1;
+            g.w.out = static_cast<char*>(d_weight) + first * l->width * static_cast<int64_t>(bytes);
+            g.w.out_aligned = width % 4 == 0 && !misaligned(g.w.out, 4 * bytes);
         }
         if (d_hidden) {     // sum over the tokens of dz[row][token] w[token][feature]
             lay.in = at(l->weight, first * l->weight_stride, l->dtype);
-            lay.in_stride = l->weight_stride;
             lay.rows = static_cast<int32_t>(n);
-            lay.pad_rows = pad;
             lay.row_mask = l->bias ? at(l->bias, first, l->dtype) : nullptr;
-            lay.out = b.w16;
-            lay.out_plane = b.piece * s.depth;
-            lay.unscale = b.unscale_w16;
-            JABAS_TRY(launch_lay_whole(lay, stream));
-            o.a = Operand{b.w16, s.depth, b.piece * s.depth, depth};
-            o.b = Operand{b.dz, a.dz_stride, a.dz_plane, rows};
-            o.b_rows_of_k = 0;
-            o.n = rows;
-            o.depth = pad;
-            o.unscale0 = b.unscale_w16;
-            o.unscale1 = nullptr;
-            o.row_scale = b.grad;
-            o.acc = b.acc;
-            o.acc_stride = b.acc_stride;
-            o.first = first == 0;
-            o.last = first + b.piece >= l->vocab;
-            o.out = d_hidden;
-            o.out_aligned = width % 4 == 0 && !misaligned(o.out, 4 * bytes);
-            JABAS_TRY(launch_out(o, s.planes, stream));
+            lay.pad = pad;
+            JABAS_TRY(launch_lay_columns(lay, stream));
+            g.h.a = Operand{b.w16, b.piece, l->width * b.piece, width};
+            g.h.b = Operand{b.dz, a.dz_stride, a.dz_plane, rows};
+            g.h.m = width;
+            g.h.n = rows;
+            g.h.depth = pad;
+            g.h.splits = splits(pad, g.h.each);     // a shorter last piece adds to the first of them
+            g.h.unscale0 = b.unscale_w16;
+            g.h.row_scale = b.grad;
+            g.h.part = b.part_h;
+            g.h.part_plane = l->rows * b.part_stride;
+            g.h.first = first == 0;
+            g.h.keep = splits_h > 1 || first + b.piece < l->vocab;
+            g.h.out = d_hidden;
+            g.h.out_aligned = width % 4 == 0 && !misaligned(d_hidden, 4 * bytes);
         }
+        JABAS_TRY(launch_grads(g, s.planes, stream));
+        if (g.w.splits > 1) JABAS_TRY(launch_join_splits(g.w, stream));
     }
-    return JABAS_OK;
+    if (!d_hidden || splits_h == 1) return JABAS_OK;
+    g.h.splits = splits_h;
+    return launch_join_splits(g.h, stream);
 }

@@ -75,31 +75,40 @@ struct LogitsArgs {
     int32_t pad_rows, pad_tokens;   // dz is written (with zeros) up to these
 };
 
-struct OutArgs {
-    Operand a, b;               // out[n][m] = scale * row_scale[n] * sum_k a[k][m] b[n][k] (b_rows_of_k: b[k][n])
-    int32_t b_rows_of_k;
-    int32_t m, n;
-    int32_t depth;
+// out[n][m] = scale * row_scale[n] * sum_k a[m][k] b[n][k] (rows_of_k: b[k][n]), the inner axis in `splits` ranges of `each`
+// elements (the last may be shorter), whose sums are joined afterwards where there are several.
+struct Job {
+    Operand a, b;
+    int32_t m, n, depth, splits, each;
     const float* unscale0;      // device scalars, or NULL
     const float* unscale1;
     const float* row_scale;     // per n, or NULL
     float scale;
-    float* acc;                 // fp32 sums over the pieces, or NULL where there is one piece
-    int64_t acc_stride;         // a multiple of 4
-    int32_t first, last;        // of the pieces
+    float* part;                // fp32 sums [split][n][part_stride] over the pieces of the inner axis, or NULL: written to `out` at once
+    int64_t part_stride, part_plane;        // a multiple of 4; splits apart
+    int32_t first;              // of the pieces: what `part` holds does not count
+    int32_t keep;               // the sums stay in `part`, to be joined or added to; else they go to `out` with what `part` holds
     void* out;
     int64_t out_stride;
     int32_t out_dtype;
     int32_t out_aligned;        // four elements of a row can be written at once
 };
-
+// The gradients' products of a piece in one launch: `w` sums over rows of k of dz, `h` over contiguous ones. Either may have m = 0.
+struct GradArgs {
+    Job w, h;
+    int32_t h_first;            // workgroups of h come first: they take longer
+};
 // Whether a product of m x n takes the large tiles, and how many of an operand's rows a tile of logits has.
 bool large_tiles(int64_t m, int64_t n, int planes);
 int logits_tile_tokens(bool large);
 int logits_tile_rows(bool large, int planes);
 int launch_logits_forward(const LogitsArgs& a, int planes, bool large, hipStream_t stream);
 int launch_logits_backward(const LogitsArgs& a, int planes, bool large, hipStream_t stream);
-int launch_out(const OutArgs& a, int planes, hipStream_t stream);
+struct Splits { int w, h; };
+// How often to split the inner axes of a piece's products: features x tokens over `rows`, features x rows over `tokens`.
+Splits choose_splits(int64_t features, int64_t tokens, int64_t rows, bool w, bool h, bool many_pieces, int planes);
+int launch_grads(GradArgs& a, int planes, hipStream_t stream);
+int launch_join_splits(const Job& j, hipStream_t stream);
 
 // Layout of operands: padded copies, split into fp16 planes and scaled by powers of two where the product asks for it.
 constexpr int kMaxParts = 1024;
@@ -110,15 +119,15 @@ struct LayArgs {
     int32_t rows, cols;         // of `in`
     const float* row_factor;    // per row of `in`, or NULL: rows with factor 0 are zeros whatever they hold, others are multiplied
     const void* row_mask;       // per row of `in`, in_dtype, or NULL: rows with -inf here (tokens that the bias rules out) are zeros
-    void* out;                  // [pad_rows][pad]
+    void* out;                  // launch_lay_rows: [rows][pad]; launch_lay_columns: [cols][pad]
     int64_t out_stride, out_plane;
-    int32_t pad_rows, pad;      // multiples of 8 columns
+    int32_t pad;                // a multiple of 64
     int32_t planes;             // 0: copied as they are; 1 or 2 planes of fp16
-    float* unscale;             // written: a factor per row (launch_lay_rows, planes > 0) or one for all (launch_lay_whole)
-    float* parts;               // launch_lay_whole: kMaxParts partial maxima
+    float* unscale;             // written: a factor per row (launch_lay_rows, planes > 0) or one for all (launch_lay_columns)
+    float* parts;               // launch_lay_columns: kMaxParts partial maxima
 };
 int launch_lay_rows(const LayArgs& a, hipStream_t stream);
-int launch_lay_whole(const LayArgs& a, hipStream_t stream);
+int launch_lay_columns(const LayArgs& a, hipStream_t stream);
 
 // Rows.
 struct TeacherArgs {

@@ -24,9 +24,9 @@ __host__ __device__ inline int tiles_n(int n) { return (n + C::kN - 1) / C::kN; 
 
 // Tile of a workgroup. Workgroups go round the eight dies (XCDs), each with an L2 of its own: each die takes a run of
 // consecutive tiles, in bands of eight tiles of m, so that the 32 tiles in flight on a die share their operands' rows.
-__device__ inline void tile_of(int tm, int tn, int& m, int& n) {
-    const int total = tm * tn, die = blockIdx.x & 7, each = total >> 3, left = total & 7;
-    const int at = die * each + min(die, left) + (blockIdx.x >> 3);
+__device__ inline void tile_of(int block, int tm, int tn, int& m, int& n) {
+    const int total = tm * tn, die = block & 7, each = total >> 3, left = total & 7;
+    const int at = die * each + min(die, left) + (block >> 3);
     const int band = at / (8 * tn), first = band * 8, height = min(8, tm - first), in = at - band * 8 * tn;
     m = first + in % height;
     n = in / height;
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(C::kThreads) void logits_forward_kernel(LogitsArgs 
     __shared__ __align__(16) char smem[2 * C::kStage];
     __shared__ float tokens[P * C::kM];
     int tm, tn;
-    tile_of(tiles_m<C>(a.w.rows), tiles_n<C>(a.x.rows), tm, tn);
+    tile_of(blockIdx.x, tiles_m<C>(a.w.rows), tiles_n<C>(a.x.rows), tm, tn);
     const int m0 = tm * C::kM, n0 = tn * C::kN, lane = threadIdx.x & 63;
     C c;
     logits_of<P>(a, m0, n0, smem, tokens, c);
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs
     __shared__ __align__(16) char smem[2 * C::kStage];
     __shared__ float tokens[P * C::kM];
     int tm, tn;
-    tile_of(tiles_m<C>(a.w.rows), tiles_n<C>(a.x.rows), tm, tn);
+    tile_of(blockIdx.x, tiles_m<C>(a.w.rows), tiles_n<C>(a.x.rows), tm, tn);
     const int m0 = tm * C::kM, n0 = tn * C::kN, lane = threadIdx.x & 63;
     C c;
     logits_of<P>(a, m0, n0, smem, tokens, c);
@@ -330,18 +330,45 @@ __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs
     }
 }
 
-template <int P, class C>
-__global__ __launch_bounds__(C::kThreads) void out_kernel(OutArgs a) {
-    __shared__ __align__(16) char smem[2 * C::kStage];
+// Results of four consecutive m of a row.
+__device__ inline void put_four(const Job& a, int n, int m, f32x4 v) {
+    const int here = min(4, a.m - m);
+    if (a.row_scale) {      // a row that does not count is zero even where its neighbours' scale is not finite
+        const float rs = a.row_scale[n];
+        v = rs == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v * rs;
+    }
+    const int64_t at = static_cast<int64_t>(n) * a.out_stride + m;
+    if (a.out_dtype == JABAS_F32) {
+        float* out = static_cast<float*>(a.out) + at;
+        if (a.out_aligned) *reinterpret_cast<f32x4*>(out) = v;
+        else
+            for (int e = 0; e < here; ++e) out[e] = v[e];
+    } else {
+        uint16_t* out = static_cast<uint16_t*>(a.out) + at;
+        const uint16_t h[4] = {to_bf16(v[0]), to_bf16(v[1]), to_bf16(v[2]), to_bf16(v[3])};
+        if (a.out_aligned) *reinterpret_cast<uint64_t*>(out) = h[0] | static_cast<uint64_t>(h[1]) << 16 | static_cast<uint64_t>(h[2]) << 32 | static_cast<uint64_t>(h[3]) << 48;
+        else
+            for (int e = 0; e < here; ++e) out[e] = h[e];
+    }
+}
+
+template <class C>
+__device__ inline void run_job(const Job& a, int unit, char* smem) {
+    const int tiles = tiles_m<C>(a.m) * tiles_n<C>(a.n), split = unit / tiles;
     int tm, tn;
-    tile_of(tiles_m<C>(a.m), tiles_n<C>(a.n), tm, tn);
+    tile_of(unit - split * tiles, tiles_m<C>(a.m), tiles_n<C>(a.n), tm, tn);
     const int m0 = tm * C::kM, n0 = tn * C::kN, lane = threadIdx.x & 63;
+    Operand x = a.a, y = a.b;
+    const int k0 = split * a.each;
+    x.p = static_cast<const uint16_t*>(x.p) + k0;
+    y.p = static_cast<const uint16_t*>(y.p) + (C::kTb ? k0 * y.stride : k0);
     C c;
-    c.run(a.a, a.b, m0, n0, a.depth, smem, [] {}, [](int, int) { return 0.0f; });
+    c.run(x, y, m0, n0, min(a.each, a.depth - k0), smem, [] {}, [](int, int) { return 0.0f; });
     const int wm = C::wave_m(), wn = C::wave_n();
     float scale = a.scale;
     if (a.unscale0) scale *= *a.unscale0;
     const float second = a.unscale1 ? *a.unscale1 : 1.0f;
+    float* part = a.part ? a.part + split * a.part_plane : nullptr;
     // 32 rows of the wave at a time through LDS: row n of kChunks 16-byte chunks, chunk k at k ^ n % kChunks
     constexpr int kChunks = C::kI * 32 / 4;
     float* mine = reinterpret_cast<float*>(smem + (threadIdx.x >> 6) * (32 * kChunks * 16));
@@ -364,36 +391,38 @@ __global__ __launch_bounds__(C::kThreads) void out_kernel(OutArgs a) {
             f32x4 v = *reinterpret_cast<const f32x4*>(mine + (r * kChunks + (k ^ (r % kChunks))) * 4);
             const int n = n0 + wn + j * 32 + r, m = m0 + wm + k * 4;
             if (n >= a.n || m >= a.m) continue;
-            const int here = min(4, a.m - m);
-            if (a.acc) {
-                float* sum = a.acc + static_cast<int64_t>(n) * a.acc_stride + m;       // rows padded to four
+            if (part) {
+                float* sum = part + static_cast<int64_t>(n) * a.part_stride + m;       // rows padded to four
                 if (!a.first) v += *reinterpret_cast<const f32x4*>(sum);
-                if (!a.last) {
+                if (a.keep) {
                     *reinterpret_cast<f32x4*>(sum) = v;
                     continue;
                 }
             }
-            if (a.row_scale) {      // a row that does not count is zero even where its neighbours' scale is not finite
-                const float rs = a.row_scale[n];
-                v = rs == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v * rs;
-            }
-            const int64_t at = static_cast<int64_t>(n) * a.out_stride + m;
-            if (a.out_dtype == JABAS_F32) {
-                float* out = static_cast<float*>(a.out) + at;
-                if (a.out_aligned) *reinterpret_cast<f32x4*>(out) = v;
-                else
-                    for (int e = 0; e < here; ++e) out[e] = v[e];
-            } else {
-                uint16_t* out = static_cast<uint16_t*>(a.out) + at;
-                const uint16_t h[4] = {to_bf16(v[0]), to_bf16(v[1]), to_bf16(v[2]), to_bf16(v[3])};
-                if (a.out_aligned) *reinterpret_cast<uint64_t*>(out) = h[0] | static_cast<uint64_t>(h[1]) << 16 | static_cast<uint64_t>(h[2]) << 32 | static_cast<uint64_t>(h[3]) << 48;
-                else
-                    for (int e = 0; e < here; ++e) out[e] = h[e];
-            }
+            put_four(a, n, m, v);
         }
     }
 }
 
+template <class CW, class CH>
+__global__ __launch_bounds__(CW::kThreads) void grads_kernel(GradArgs a) {
+    static_assert(CW::kStage == CH::kStage && CW::kThreads == CH::kThreads, "one launch shape");
+    __shared__ __align__(16) char smem[2 * CW::kStage];
+    const int units_w = tiles_m<CW>(a.w.m) * tiles_n<CW>(a.w.n) * a.w.splits, units_h = tiles_m<CH>(a.h.m) * tiles_n<CH>(a.h.n) * a.h.splits;
+    const int block = blockIdx.x, lead = a.h_first ? units_h : units_w;
+    if ((block < lead) == (a.h_first != 0)) run_job<CH>(a.h, a.h_first ? block : block - lead, smem);
+    else run_job<CW>(a.w, a.h_first ? block - lead : block, smem);
+}
+
+__global__ __launch_bounds__(256) void join_splits_kernel(Job a) {
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int quads = (a.m + 3) / 4, n = static_cast<int>(at / quads), m = static_cast<int>(at % quads) * 4;
+    if (n >= a.n) return;
+    const float* part = a.part + n * a.part_stride + m;
+    f32x4 v = *reinterpret_cast<const f32x4*>(part);
+    for (int i = 1; i < a.splits; ++i) v += *reinterpret_cast<const f32x4*>(part + i * a.part_plane);
+    put_four(a, n, m, v);
+}
 
 template <class K, class A>
 int launch(K kernel, int64_t grid, int threads, const A& args, hipStream_t stream) {
@@ -417,14 +446,16 @@ int logits(const LogitsArgs& a, int planes, bool large, bool backward, hipStream
 }
 
 template <int P, int TM, int TN, int WM, int WN>
-int out(const OutArgs& a, hipStream_t stream) {
-    if (a.b_rows_of_k) {
-        using C = Core<F16, P, TM, TN, WM, WN, true, true, P == 2>;
-        return launch(out_kernel<P, C>, static_cast<int64_t>(tiles_m<C>(a.m)) * tiles_n<C>(a.n), C::kThreads, a, stream);
-    }
-    using C = Core<F16, P, TM, TN, WM, WN, true, false, P == 2>;
-    return launch(out_kernel<P, C>, static_cast<int64_t>(tiles_m<C>(a.m)) * tiles_n<C>(a.n), C::kThreads, a, stream);
+int grads(const GradArgs& a, hipStream_t stream) {
+    using CW = Core<F16, P, TM, TN, WM, WN, false, true, P == 2>;
+    using CH = Core<F16, P, TM, TN, WM, WN, false, false, P == 2>;
+    const int64_t grid = static_cast<int64_t>(tiles_m<CW>(a.w.m)) * tiles_n<CW>(a.w.n) * a.w.splits + static_cast<int64_t>(tiles_m<CH>(a.h.m)) * tiles_n<CH>(a.h.n) * a.h.splits;
+    return launch(grads_kernel<CW, CH>, grid, CW::kThreads, a, stream);
 }
+
+struct Tile { int m, n; };
+bool large_grads(int64_t features, int64_t tokens, int64_t rows) { return features > 128 && (tokens > 128 || rows > 128) && rows > 128; }
+Tile grads_tile(bool large, int planes) { return large ? Tile{256, planes == 2 ? 128 : 256} : Tile{128, 128}; }
 
 }  // namespace
 
@@ -436,10 +467,90 @@ int logits_tile_rows(bool large, int planes) { return large && planes == 1 ? 256
 
 int launch_logits_forward(const LogitsArgs& a, int planes, bool large, hipStream_t stream) { return logits(a, planes, large, false, stream); }
 int launch_logits_backward(const LogitsArgs& a, int planes, bool large, hipStream_t stream) { return logits(a, planes, large, true, stream); }
-int launch_out(const OutArgs& a, int planes, hipStream_t stream) {
-    const bool large = large_tiles(a.m, a.n, planes);
-    if (planes == 2) return large ? out<2, 256, 128, 4, 2>(a, stream) : out<2, 128, 128, 2, 2>(a, stream);
-    return large ? out<1, 256, 256, 2, 4>(a, stream) : out<1, 128, 128, 2, 2>(a, stream);
+
+// Time, in steps of a tile, that `slots` workgroups take for `na` units of length `la`, then `nb` of length `lb`, each taken by whoever is
+// free first. Workgroups that get free together are counted together.
+namespace {
+double makespan(int slots, int64_t na, double la, int64_t nb, double lb) {
+    struct Group { double free; int64_t n; } g[64] = {{0.0, slots}};
+    int groups = 1;
+    double end = 0.0;
+    for (int kind = 0; kind < 2; ++kind) {
+        int64_t left = kind ? nb : na;
+        const double length = kind ? lb : la;
+        while (left > 0) {
+            int at = 0;
+            for (int i = 1; i < groups; ++i)
+                if (g[i].free < g[at].free) at = i;
+            if (groups == 1 && left > 8 * g[0].n) {     // whole rounds of one kind
+                const int64_t rounds = left / g[0].n - 4;
+                g[0].free += rounds * length;
+                left -= rounds * g[0].n;
+                continue;
+            }
+            const int64_t take = left < g[at].n ? left : g[at].n;
+            const double until = g[at].free + length;
+            left -= take;
+            if (until > end) end = until;
+            if (take == g[at].n) {
+                g[at].free = until;
+            } else {
+                g[at].n -= take;
+                if (groups == 64) return end + left * length / slots;
+                g[groups++] = {until, take};
+            }
+            for (int i = 0; i < groups; ++i)            // those that are free at one time, together
+                for (int j = i + 1; j < groups; ++j)
+                    if (g[i].free == g[j].free) {
+                        g[i].n += g[j].n;
+                        g[j--] = g[--groups];
+                    }
+        }
+    }
+    return end;
+}
+}  // namespace
+
+// The split that the model above says ends first. A unit costs its steps of 64 elements and kUnit more for its start and its results; fp32
+// sums that are written, read and joined cost what their bytes take of the chip's bandwidth (a step of a 256 x 256 tile is 1.8 us at
+// 1.2 PFLOP/s, in which HBM moves 9 MB). Without splits 1600 x 1024 sums over 16 thousand tokens ran on 104 of 256 CUs: 406 us,
+// 182 with them.
+Splits choose_splits(int64_t features, int64_t tokens, int64_t rows, bool w, bool h, bool many_pieces, int planes) {
+    const bool large = large_grads(features, tokens, rows);
+    const Tile t = grads_tile(large, planes);
+    const int slots = large ? 256 : 512;
+    const double kUnit = 6.0, bytes_per_step = (large ? 9e6 : 4.5e6) * (planes == 2 ? 1.5 : 1.0);
+    const int64_t fm = (features + t.m - 1) / t.m, tw = w ? fm * ((tokens + t.n - 1) / t.n) : 0, th = h ? fm * ((rows + t.n - 1) / t.n) : 0;
+    const double kw = (rows + 63) / 64, kh = (tokens + 63) / 64;
+    Splits best = {1, 1};
+    double least = 0.0;
+    static const int kTries[] = {1, 2, 3, 4, 5, 6, 8, 12, 16};
+    for (int sw : kTries)
+        for (int sh : kTries) {
+            if (sw > (w && tw < 2 * slots ? 4 : 1) || sh > (h && th < 2 * slots ? 16 : 1) || (sw > 1 && kw / sw < 4) || (sh > 1 && kh / sh < 4)) continue;
+            const double lw = kw / sw + kUnit, lh = kh / sh + kUnit;
+            double time = lh > lw ? makespan(slots, th * sh, lh, tw * sw, lw) : makespan(slots, tw * sw, lw, th * sh, lh);
+            const double sums_w = sw > 1 ? 4.0 * features * tokens * sw * 2 : 0.0;
+            const double sums_h = sh > 1 || many_pieces ? 4.0 * features * rows * sh * 2 : 0.0;
+            time += (sums_w + sums_h) / bytes_per_step;
+            if ((sw == 1 && sh == 1) || time < least * 0.98) {
+                least = time;
+                best = {sw, sh};
+            }
+        }
+    return best;
+}
+
+int launch_grads(GradArgs& a, int planes, hipStream_t stream) {
+    const int64_t features = a.w.m > a.h.m ? a.w.m : a.h.m;
+    a.h_first = !a.w.m || (a.h.m && a.h.each > a.w.each);
+    const bool large = large_grads(features, a.w.m ? a.w.n : a.h.depth, a.h.m ? a.h.n : a.w.depth);
+    if (planes == 2) return large ? grads<2, 256, 128, 4, 2>(a, stream) : grads<2, 128, 128, 2, 2>(a, stream);
+    return large ? grads<1, 256, 256, 2, 4>(a, stream) : grads<1, 128, 128, 2, 2>(a, stream);
+}
+
+int launch_join_splits(const Job& j, hipStream_t stream) {
+    return launch(join_splits_kernel, (static_cast<int64_t>((j.m + 3) / 4) * j.n + 255) / 256, 256, j, stream);
 }
 
 // ------------------------------------------------------------------ layout of operands
@@ -561,33 +672,36 @@ __global__ __launch_bounds__(kLayThreads) void absmax_kernel(LayArgs a) {
     if (threadIdx.x == 0) a.parts[blockIdx.x] = fmaxf(fmaxf(merge[0], merge[1]), fmaxf(merge[2], merge[3]));
 }
 
-// A wave per row, one scale for all of them.
-__global__ __launch_bounds__(kLayThreads) void lay_whole_kernel(LayArgs a) {
-    __shared__ float merge[kLayThreads / 64];
+// 64 x 64 elements through LDS: out[col][row], one scale for all of them.
+__global__ __launch_bounds__(kLayThreads) void lay_columns_kernel(LayArgs a) {
+    __shared__ float merge[kLayThreads / 64], tile[64][65];
     static_assert(kMaxParts % kLayThreads == 0, "as many partial maxima per thread");
-    const int t = threadIdx.x, lane = t & 63;
+    const int t = threadIdx.x, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
     float peak = 0.0f, v[8];
 #pragma unroll
     for (int i = 0; i < kMaxParts; i += kLayThreads) peak = fmaxf(peak, a.parts[i + t]);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int r = x * 32 + (t >> 3), c = (t & 7) * 8;
+        const float f = r0 + r < a.rows ? row_keeps(a, r0 + r) : 0.0f;
+        if (f != 0.0f) load_eight(a, r0 + r, c0 + c, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) tile[r][c + i] = f != 0.0f ? v[i] * f : 0.0f;
+    }
     peak = wave_max(peak);
-    if (lane == 0) merge[t >> 6] = peak;
+    if ((t & 63) == 0) merge[t >> 6] = peak;
     __syncthreads();
     peak = fmaxf(fmaxf(merge[0], merge[1]), fmaxf(merge[2], merge[3]));
     const int e = scale_exponent(peak);
-    if (t == 0 && blockIdx.x == 0) *a.unscale = power_of_two(-e);
-    const int row = blockIdx.x * (kLayThreads / 64) + (t >> 6);
-    if (row >= a.pad_rows) return;
-    const float f = row < a.rows ? row_keeps(a, row) : 0.0f, scale = power_of_two(e);
-    for (int c = lane * 8; c < a.pad; c += 512) {
-        if (f != 0.0f) {
-            load_eight(a, row, c, v);
+    const float scale = power_of_two(e);
+    if (t == 0 && blockIdx.x == 0 && blockIdx.y == 0) *a.unscale = power_of_two(-e);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = v[i] * f * scale;
-        } else {
+    for (int x = 0; x < 2; ++x) {
+        const int c = x * 32 + (t >> 3), r = (t & 7) * 8;
+        if (c0 + c >= a.cols || r0 + r >= a.pad) continue;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-        }
-        store_eight(a, row, c, v);
+        for (int i = 0; i < 8; ++i) v[i] = tile[r + i][c] * scale;
+        store_eight(a, c0 + c, r0 + r, v);
     }
 }
 
@@ -597,9 +711,12 @@ int launch_lay_rows(const LayArgs& a, hipStream_t stream) {
     return launch(lay_rows_kernel, (a.rows + 3) / 4, kLayThreads, a, stream);
 }
 
-int launch_lay_whole(const LayArgs& a, hipStream_t stream) {
+int launch_lay_columns(const LayArgs& a, hipStream_t stream) {
     const int status = launch(absmax_kernel, kMaxParts, kLayThreads, a, stream);
-    return status != JABAS_OK ? status : launch(lay_whole_kernel, (a.pad_rows + 3) / 4, kLayThreads, a, stream);
+    if (status != JABAS_OK) return status;
+    void* params[] = {const_cast<LayArgs*>(&a)};
+    return hipLaunchKernel(reinterpret_cast<const void*>(lay_columns_kernel), dim3(a.pad / 64, (a.cols + 63) / 64), dim3(kLayThreads), params, 0, stream) == hipSuccess
+               ? JABAS_OK : JABAS_ERR_LAUNCH;
 }
 
 }  // namespace loss
