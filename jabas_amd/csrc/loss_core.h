@@ -86,17 +86,15 @@ struct Core {
                 }
             }
         }
-        // `to`: byte address in LDS of the operand's stage
-        __device__ void issue(uint32_t to) {
+        // Load `l` of kLoads of a step. `to`: byte address in LDS of the operand's stage
+        __device__ void issue(uint32_t to, int l) {
             const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63u);
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                         :: "s"(to + static_cast<uint32_t>(l * kThreads * 16) + wave * 16), "v"(offset[l % kEach]), "s"(base[l / kEach]) : "memory", "m0");
+        }
+        __device__ void advance() {
 #pragma unroll
-            for (int q = 0; q < P; ++q) {
-#pragma unroll
-                for (int i = 0; i < kEach; ++i)
-                    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                                 :: "s"(to + static_cast<uint32_t>((q * kEach + i) * kThreads * 16) + wave * 16), "v"(offset[i]), "s"(base[q]) : "memory", "m0");
-                base[q] += step;
-            }
+            for (int q = 0; q < P; ++q) base[q] += step;
         }
     };
 
@@ -130,7 +128,11 @@ struct Core {
             for (int i = 0; i < kI; ++i) f.a[i][q] = fragment<TM, TA>(stage, wm + i * 32, kk, q);
         }
     }
-    __device__ void multiply(const Fragments& f) {
+    // `between(t)` runs behind product t of kProducts.
+    static constexpr int kProducts = kI * kJ * (P == 2 ? 3 : 1);
+    template <class Between>
+    __device__ void multiply(const Fragments& f, const Between& between) {
+        int t = 0;
 #pragma unroll
         for (int i = 0; i < kI; ++i) {
             const vec a0 = RAISED ? E::lowered(f.a[i][0]) : f.a[i][0];
@@ -138,9 +140,12 @@ struct Core {
             for (int j = 0; j < kJ; ++j) {
                 if (P == 2) {       // (a0 + a1)(b0 + b1) without a1 b1, which is under 2^-22 of the whole
                     acc[i][j] = E::mfma(f.a[i][P - 1], f.b[j][0], acc[i][j]);
+                    between(t++);
                     acc[i][j] = E::mfma(a0, f.b[j][P - 1], acc[i][j]);
+                    between(t++);
                 }
                 acc[i][j] = E::mfma(f.a[i][0], f.b[j][0], acc[i][j]);
+                between(t++);
             }
         }
     }
@@ -157,9 +162,18 @@ struct Core {
         Source<TM, TA> sa(a, m0);
         Source<TN, TB> sb(b, n0);
         const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem));
+        const auto load = [&](int stage, int l) {
+            const uint32_t to = lds + stage * kStage;
+            if (l < kLoadsA) sa.issue(to, l);
+            else sb.issue(to + kBytesA, l - kLoadsA);
+            if (l == kLoadsA + kLoadsB - 1) {
+                sa.advance();
+                sb.advance();
+            }
+        };
         const auto issue = [&](int stage) {
-            sa.issue(lds + stage * kStage);
-            sb.issue(lds + stage * kStage + kBytesA);
+#pragma unroll
+            for (int l = 0; l < kLoadsA + kLoadsB; ++l) load(stage, l);
         };
         const int steps = depth / kStep;        // at least one
         issue(0);
@@ -176,22 +190,35 @@ struct Core {
             }
         Fragments f[2];
         read(f[0], smem, 0);
-        for (int s = 0; s < steps; ++s) {
+        const auto pass = [&](int s, auto more) {       // more: a step after the next is to be loaded
             const char* stage = smem + (s & 1) * kStage;
 #pragma unroll
             for (int kk = 0; kk < kParts; ++kk) {
-                if (kk + 1 < kParts) {
+                const bool last = kk + 1 == kParts;
+                if (!last) {
                     read(f[(kk + 1) & 1], stage, kk + 1);
                 } else {
                     arrive();
-                    if (s + 2 < steps) issue(s & 1);
                     read(f[0], smem + ((s + 1) & 1) * kStage, 0);       // behind the last step: read, not used
                 }
                 __builtin_amdgcn_sched_barrier(0);
-                multiply(f[kk & 1]);
+                multiply(f[kk & 1], [&](int t) {
+                    if (more() && last) {
+                        constexpr int kLoads = kLoadsA + kLoadsB;
+                        const int from = t * kLoads / kProducts, to = (t + 1) * kLoads / kProducts;
+                        if (from == to) return;
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int l = from; l < to; ++l) load(s & 1, l);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                });
                 __builtin_amdgcn_sched_barrier(0);
             }
-        }
+        };
+        int s = 0;
+        for (; s + 2 < steps; ++s) pass(s, [] { return true; });
+        for (; s < steps; ++s) pass(s, [] { return false; });
     }
 };
 
