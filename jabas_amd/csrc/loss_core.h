@@ -38,8 +38,12 @@ struct BF16 {
 //   rows of k: chunk c of row k at c ^ 4 (k % 4): the transposing 8-byte reads take four rows and 32 bytes of each at a time.
 // The last fragments of a step are in registers before the barrier that gives its stage to the loads of the step after the
 // next, and are multiplied behind it, while the next step's first fragments are read: neither the barrier nor the first read
-// leaves the matrix cores waiting. The loads are inline assembly because the compiler would wait for all of them before any
-// later LDS read; they have no register outputs, and the wait in front of the barrier covers them.
+// leaves the matrix cores waiting. Reads and loads go between the products one by one: in a row in front of them they fill the
+// LDS and memory pipes and hold the products up (matrix cores busy 75 % of the cycles, 83 % so, at 16384 x 4096 x 4096).
+// What bounds it then is power: the clock falls as the cores get busier (1.56 GHz there, 2.1 with LDS and memory idle). Waves of
+// 128 x 128, which read LDS a third less, came out even.
+// The loads are inline assembly because the compiler would wait for all of them before any later LDS read; they have no
+// register outputs, and the wait in front of the barrier covers them.
 template <class E, int P, int TM, int TN, int WM, int WN, bool TA, bool TB, bool RAISED>
 struct Core {
     static constexpr bool kTb = TB;
@@ -118,16 +122,14 @@ struct Core {
     struct Fragments {
         vec a[kI][P], b[kJ][P];
     };
-    static __device__ void read(Fragments& f, const char* stage, int kk) {
-        const int wm = wave_m(), wn = wave_n();
-#pragma unroll
-        for (int q = 0; q < P; ++q) {
-#pragma unroll
-            for (int j = 0; j < kJ; ++j) f.b[j][q] = fragment<TN, TB>(stage + kBytesA, wn + j * 32, kk, q);
-#pragma unroll
-            for (int i = 0; i < kI; ++i) f.a[i][q] = fragment<TM, TA>(stage, wm + i * 32, kk, q);
-        }
+    // Fragment `r` of the kReads of a part of a step, those that are multiplied first first.
+    static constexpr int kReads = (kI + kJ) * P;
+    static __device__ void read(Fragments& f, const char* stage, int kk, int r) {
+        const int x = r / P, q = r % P;
+        if (x < kJ) f.b[x][q] = fragment<TN, TB>(stage + kBytesA, wave_n() + x * 32, kk, q);
+        else f.a[x - kJ][q] = fragment<TM, TA>(stage, wave_m() + (x - kJ) * 32, kk, q);
     }
+
     // `between(t)` runs behind product t of kProducts.
     static constexpr int kProducts = kI * kJ * (P == 2 ? 3 : 1);
     template <class Between>
@@ -171,15 +173,15 @@ struct Core {
                 sb.advance();
             }
         };
-        const auto issue = [&](int stage) {
-#pragma unroll
-            for (int l = 0; l < kLoadsA + kLoadsB; ++l) load(stage, l);
-        };
         const int steps = depth / kStep;        // at least one
-        issue(0);
+        constexpr int kLoads = kLoadsA + kLoadsB;
+#pragma unroll
+        for (int l = 0; l < kLoads; ++l) load(0, l);
         prepare();
         arrive();
-        if (steps > 1) issue(1);
+        if (steps > 1)
+#pragma unroll
+            for (int l = 0; l < kLoads / 2; ++l) load(1, l);
 #pragma unroll
         for (int i = 0; i < kI; ++i)
 #pragma unroll
@@ -189,36 +191,40 @@ struct Core {
                 for (int j = 0; j < kJ; ++j) acc[i][j][e] = x;
             }
         Fragments f[2];
-        read(f[0], smem, 0);
-        const auto pass = [&](int s, auto more) {       // more: a step after the next is to be loaded
+#pragma unroll
+        for (int r = 0; r < kReads; ++r) read(f[0], smem, 0, r);
+        // One step. `next`: there is another, the second half of whose loads goes between the first products; `after`: there is one more, the
+        // first half of whose loads goes between the last products, behind the barrier that frees its stage.
+        const auto pass = [&](int s, auto next, auto after) {
             const char* stage = smem + (s & 1) * kStage;
 #pragma unroll
             for (int kk = 0; kk < kParts; ++kk) {
-                const bool last = kk + 1 == kParts;
-                if (!last) {
-                    read(f[(kk + 1) & 1], stage, kk + 1);
-                } else {
-                    arrive();
-                    read(f[0], smem + ((s + 1) & 1) * kStage, 0);       // behind the last step: read, not used
-                }
+                const bool first = kk == 0, last = kk + 1 == kParts;
+                if (last) arrive();
                 __builtin_amdgcn_sched_barrier(0);
                 multiply(f[kk & 1], [&](int t) {
-                    if (more() && last) {
-                        constexpr int kLoads = kLoadsA + kLoadsB;
-                        const int from = t * kLoads / kProducts, to = (t + 1) * kLoads / kProducts;
-                        if (from == to) return;
-                        __builtin_amdgcn_sched_barrier(0);
+                    const auto share = [&](int n, int at) { return min(n, at * n * 5 / (4 * kProducts)); };     // done at four fifths of the products
 #pragma unroll
-                        for (int l = from; l < to; ++l) load(s & 1, l);
-                        __builtin_amdgcn_sched_barrier(0);
+                    for (int r = share(kReads, t); r < share(kReads, t + 1); ++r) {       // of the next part; behind the last step: read, not used
+                        if (last) read(f[0], smem + ((s + 1) & 1) * kStage, 0, r);
+                        else read(f[(kk + 1) & 1], stage, kk + 1, r);
                     }
+                    if (first && next())
+#pragma unroll
+                        for (int l = kLoads / 2 + t * (kLoads - kLoads / 2) / kProducts; l < kLoads / 2 + (t + 1) * (kLoads - kLoads / 2) / kProducts; ++l) load((s + 1) & 1, l);
+                    if (last && after())
+#pragma unroll
+                        for (int l = t * (kLoads / 2) / kProducts; l < (t + 1) * (kLoads / 2) / kProducts; ++l) load(s & 1, l);
+                    __builtin_amdgcn_sched_barrier(0);
                 });
-                __builtin_amdgcn_sched_barrier(0);
             }
         };
+        const auto yes = [] { return true; };
+        const auto no = [] { return false; };
         int s = 0;
-        for (; s + 2 < steps; ++s) pass(s, [] { return true; });
-        for (; s < steps; ++s) pass(s, [] { return false; });
+        for (; s + 2 < steps; ++s) pass(s, yes, yes);
+        if (s + 1 < steps) pass(s++, yes, no);
+        pass(s, no, no);
     }
 };
 
