@@ -26,7 +26,7 @@ struct Shape {
 
 bool misaligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
 
-void cut_rows(const JabasLoss* l, int64_t& splits, int64_t& chunk);
+void cut_rows(const JabasLoss* l, bool forward, int64_t& splits, int64_t& chunk);
 
 int validate(const JabasLoss* l, Shape& s) {
     if (!l) return JABAS_ERR_NULL;
@@ -42,7 +42,7 @@ int validate(const JabasLoss* l, Shape& s) {
     } else {
         if ((!l->logits && l->rows) || l->bias || !s.teacher) return JABAS_ERR_NULL;
         int64_t splits, chunk;
-        cut_rows(l, splits, chunk);
+        cut_rows(l, false, splits, chunk);
         if (l->logits_stride < 0 || splits * l->rows > 0x7fffffff) return JABAS_ERR_SIZE;
     }
     if (s.teacher) {
@@ -79,6 +79,7 @@ struct Carver {
         used += (n * sizeof(T) + 255) / 256 * 256;
         return p;
     }
+    size_t all() const { return used ? used : 256; }
 };
 
 // Tokens of a piece: what the pieces' copies may take is bounded, and a piece has whole tiles.
@@ -109,17 +110,21 @@ struct Forward {
     bool large;
 };
 
-constexpr int64_t kSplitTokens = 32768;         // tokens of a workgroup over logits in hand, at most
+// Logits in hand, workgroups per row. A row is one workgroup's where there are rows enough for the chip (kFullRows), where it is short
+// (kShortRow), and as far as the mask of its entries fits LDS (a bit a token: kMaskTokens). 5 x 131072 fp32: 36 us with a split, 60 without.
+constexpr int64_t kMaskTokens = int64_t{1} << 18;
+constexpr int64_t kFullRows = 512, kShortRow = 8192;
 constexpr int64_t kLeastSplitTokens = 2048;
 constexpr int64_t kWantedGroups = 1024;
 
-// Workgroups per row over logits in hand: enough for the chip, none with less than a couple of passes.
-void cut_rows(const JabasLoss* l, int64_t& splits, int64_t& chunk) {
-    splits = (l->vocab + kSplitTokens - 1) / kSplitTokens;
+void cut_rows(const JabasLoss* l, bool forward, int64_t& splits, int64_t& chunk) {
     const int64_t rows = l->rows > 0 ? l->rows : 1;
-    const int64_t want = (kWantedGroups + rows - 1) / rows, most = (l->vocab + kLeastSplitTokens - 1) / kLeastSplitTokens;
-    const int64_t more = want < most ? want : most;
-    if (splits < more) splits = more;
+    splits = forward ? (l->vocab + kMaskTokens - 1) / kMaskTokens : (l->vocab + 32767) / 32768;
+    if (rows < kFullRows && l->vocab > kShortRow) {
+        const int64_t want = (kWantedGroups + rows - 1) / rows, most = (l->vocab + kLeastSplitTokens - 1) / kLeastSplitTokens;
+        const int64_t more = want < most ? want : most;
+        if (splits < more) splits = more;
+    }
     chunk = round_up((l->vocab + splits - 1) / splits, 32);
     splits = (l->vocab + chunk - 1) / chunk;
 }
@@ -133,13 +138,13 @@ size_t carve_forward(const JabasLoss* l, const Shape& s, char* base, Forward& f)
         f.tiles = tiles(l->vocab, logits_tile_tokens(f.large));
         f.piece = piece_tokens(l, s, false);
     } else {
-        cut_rows(l, f.splits, f.chunk);
+        cut_rows(l, true, f.splits, f.chunk);
         f.tiles = f.splits;
     }
     f.partial = c.take<float2>(f.tiles * rows);
     if (l->label_smoothing != 0.0) f.total = c.take<float>(f.tiles * rows);
-    f.entry_logit = c.take<float>(rows * (s.teacher ? l->entries : 1));
-    if (s.teacher) f.teacher_row = c.take<float4>(rows);
+    if (s.linear) f.entry_logit = c.take<float>(rows * (s.teacher ? l->entries : 1));
+    if (s.linear && s.teacher) f.teacher_row = c.take<float4>(rows);
     f.row_loss = c.take<float>(rows);
     if (s.linear && s.copy_x) f.x = c.take<uint16_t>(rows * s.depth * s.planes);
     if (s.linear && s.copy_w) f.w = c.take<uint16_t>(f.piece * s.depth * s.planes);
@@ -147,7 +152,7 @@ size_t carve_forward(const JabasLoss* l, const Shape& s, char* base, Forward& f)
         f.unscale_x = c.take<float>(rows);
         f.unscale_w = c.take<float>(f.piece);
     }
-    return c.used;
+    return c.all();
 }
 
 struct Backward {
@@ -165,13 +170,13 @@ size_t carve_backward(const JabasLoss* l, const Shape& s, char* base, Backward& 
     Carver c{base, 0};
     const int64_t rows = l->rows;
     b = Backward{};
+    if (!s.linear) {
+        cut_rows(l, false, b.splits, b.chunk);
+        return c.all();
+    }
     b.grad = c.take<float>(rows);
     b.ratio = c.take<float>(rows);
     b.peak = c.take<float>(1);
-    if (!s.linear) {
-        cut_rows(l, b.splits, b.chunk);
-        return c.used;
-    }
     b.piece = piece_tokens(l, s, true);
     b.pad_rows = round_up(rows, kDepth);
     if (s.copy_x) b.x = c.take<uint16_t>(rows * s.depth * s.planes);
@@ -191,7 +196,7 @@ size_t carve_backward(const JabasLoss* l, const Shape& s, char* base, Backward& 
     if (b.inner.h > 1 || b.piece < l->vocab) b.part_h = c.take<float>(b.inner.h * rows * b.part_stride);
     b.large = large_tiles(tokens, rows, s.planes);
     if (l->bias) b.db = c.take<float>(tiles(rows, logits_tile_rows(b.large, s.planes)) * b.piece);
-    return c.used;
+    return c.all();
 }
 
 Entries entries_of(const JabasLoss* l, const Shape& s) {
@@ -284,8 +289,7 @@ JABAS_API size_t jabas_loss_workspace_bytes(const JabasLoss* l, int32_t backward
     if (validate(l, s) != JABAS_OK) return 0;
     Forward f;
     Backward b;
-    const size_t n = backward ? carve_backward(l, s, nullptr, b) : carve_forward(l, s, nullptr, f);
-    return n ? n : 256;
+    return backward ? carve_backward(l, s, nullptr, b) : carve_forward(l, s, nullptr, f);
 }
 
 JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* workspace, size_t workspace_bytes, jabas_stream_t stream_) {
@@ -300,8 +304,8 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
     if (!l->rows) return launch_reduce(f.row_loss, state, 0, l->reduction, loss_out, reduce, stream);
     const float inv_t = static_cast<float>(1.0 / l->temperature), c = static_cast<float>(kLog2e / l->temperature);
     const Entries entries = entries_of(l, s);
+    TeacherArgs t{};
     if (s.teacher) {
-        TeacherArgs t{};
         t.index = l->teacher_index;
         t.logits = l->teacher_logits;
         t.dtype = l->dtype;
@@ -310,10 +314,11 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
         t.vocab = l->vocab;
         t.k = static_cast<int32_t>(l->entries);
         t.inv_t = inv_t;
+        t.t = static_cast<float>(l->temperature);
         t.entry_index = l->entry_index;
         t.entry_p = l->entry_p;
         t.row = f.teacher_row;
-        JABAS_TRY(launch_teacher(t, stream));
+        if (s.linear) JABAS_TRY(launch_teacher(t, stream));
     }
     if (s.linear) {
         LogitsArgs a{};
@@ -344,10 +349,12 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
         a.splits = static_cast<int32_t>(f.splits);
         a.chunk = f.chunk;
         a.c = c;
-        a.entries = entries;
+        a.teacher = t;
         a.partial = f.partial;
-        a.entry_logit = f.entry_logit;
+        a.state = state;
+        a.row_loss = f.row_loss;
         JABAS_TRY(launch_topk_forward(a, stream));
+        return launch_reduce(f.row_loss, state, l->rows, l->reduction, loss_out, reduce, stream);
     }
     JoinArgs j{};
     j.partial = f.partial;
@@ -357,12 +364,10 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
     j.vocab = l->vocab;
     j.tiles = static_cast<int32_t>(f.tiles);
     j.c = c;
-    j.inv_t = inv_t;
-    j.t = static_cast<float>(l->temperature);
     j.smoothing = static_cast<float>(l->label_smoothing);
     j.entries = entries;
     j.teacher_row = f.teacher_row;
-    j.has_rest = l->teacher_lse != nullptr;
+    j.teacher = t;
     j.state = state;
     j.row_loss = f.row_loss;
     JABAS_TRY(launch_join(j, stream));
@@ -390,8 +395,7 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     const RowState* state = reinterpret_cast<const RowState*>(l->row_state);
     const float* reduce = l->row_state + 4 * l->rows;
     const float c = static_cast<float>(kLog2e / l->temperature);
-    JABAS_TRY(launch_row_grad(upstream, l->reduction == JABAS_LOSS_NONE, reduce, static_cast<float>(l->temperature), state, l->rows, b.grad, b.ratio,
-                              b.peak, stream));
+    const int per_row = l->reduction == JABAS_LOSS_NONE;
     if (!s.linear) {
         if (!d_logits) return JABAS_OK;
         TopkArgs a{};
@@ -404,12 +408,16 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
         a.chunk = b.chunk;
         a.c = c;
         a.entries = entries_of(l, s);
-        a.state = state;
-        a.row_grad = b.grad;
+        a.t = static_cast<float>(l->temperature);
+        a.state = const_cast<RowState*>(state);
+        a.upstream = upstream;
+        a.per_row = per_row;
+        a.reduce = reduce;
         a.out = d_logits;
         return launch_topk_backward(a, stream);
     }
     if (!d_hidden && !d_weight && !d_bias) return JABAS_OK;
+    JABAS_TRY(launch_row_grad(upstream, per_row, reduce, static_cast<float>(l->temperature), state, l->rows, b.grad, b.ratio, b.peak, stream));
     LogitsArgs a{};
     JABAS_TRY(lay_x(l, s, b.x, b.unscale_x, a.x, stream));
     a.depth = static_cast<int32_t>(s.depth);

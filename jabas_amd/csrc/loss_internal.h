@@ -137,7 +137,7 @@ struct TeacherArgs {
     const float* lse;
     int64_t rows, vocab;
     int32_t k;
-    float inv_t;
+    float inv_t, t;
     int32_t* entry_index;
     float* entry_p;
     float4* row;                // mass, sum p log p, counts, -
@@ -150,11 +150,11 @@ struct JoinArgs {
     const float* entry_logit;
     int64_t rows, vocab;
     int32_t tiles;
-    float c, inv_t, t;
+    float c;
     float smoothing;
     Entries entries;
     const float4* teacher_row;
-    int32_t has_rest;           // teacher_lse was given
+    TeacherArgs teacher;
     RowState* state;
     float* row_loss;
 };
@@ -170,19 +170,23 @@ int launch_row_grad(const float* upstream, int per_row, const float* reduce, flo
 int launch_bias_sum(const float* parts, int32_t tiles, int64_t stride, int64_t n, void* out, int32_t dtype, hipStream_t stream);
 int launch_zero(void* p, size_t bytes, hipStream_t stream);
 
+// Logits in hand. One split: a workgroup per row; else a workgroup per `chunk` tokens of a row.
 struct TopkArgs {
     const void* logits;
     int64_t stride;
     int32_t dtype;
     int64_t rows, vocab;
     int32_t splits;
-    int64_t chunk;              // tokens of a split
-    float c;
-    Entries entries;
-    float2* partial;            // [split][row]
-    float* entry_logit;
-    const RowState* state;
-    const float* row_grad;
+    int64_t chunk;              // a multiple of 32
+    float c, t;
+    TeacherArgs teacher;
+    float2* partial;            // [row][split]
+    RowState* state;
+    float* row_loss;
+    Entries entries;            // backward
+    const float* upstream;
+    int32_t per_row;
+    const float* reduce;
     void* out;                  // [row][vocab]
 };
 int launch_topk_forward(const TopkArgs& a, hipStream_t stream);

@@ -46,77 +46,148 @@ __device__ inline float rescale(float s, float from, float to, float c) {
 constexpr int kEntriesPerLane = 4;
 static_assert(64 * kEntriesPerLane > JABAS_LOSS_MAX_ENTRIES, "a row's entries fit a wave");
 
-// One wave per row. Entries that name a token twice are one event with both probabilities: the first keeps the sum.
-__global__ __launch_bounds__(kThreads) void teacher_kernel(TeacherArgs a) {
-    __shared__ int64_t names[kThreads / 64][64 * kEntriesPerLane];
-    __shared__ float probs[kThreads / 64][64 * kEntriesPerLane];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + wave;
-    const bool here = row < a.rows;
-    int64_t idx[kEntriesPerLane];
-    float t[kEntriesPerLane], p[kEntriesPerLane];
-    bool is[kEntriesPerLane];
-    float peak = -INFINITY, sum = 0.0f;
-    bool outside = false;
+// A row's entries, entry lane + 64 i in place i of the lanes that hold it.
+struct WaveEntries {
+    int32_t index[kEntriesPerLane];     // -1: none (also where a name outside the vocabulary makes the row's loss NaN)
+    float p[kEntriesPerLane];
+    float mass, entropy;                // sums of p and p log p; the latter NaN with a name outside the vocabulary
+    bool counts;
+};
+
+// The teacher's probabilities of a row, by one wave. Entries that name a token twice are one event with both probabilities: the first keeps
+// the sum. `names` and `probs`: 256 places of LDS of the wave's own.
+__device__ inline WaveEntries wave_entries(const TeacherArgs& a, int64_t row, int32_t* names, float* probs) {
+    const int lane = threadIdx.x & 63;
+    WaveEntries w;
+    float t[kEntriesPerLane], logp[kEntriesPerLane], peak = -INFINITY, sum = 0.0f;
+    bool is[kEntriesPerLane], outside = false;
+#pragma unroll
     for (int i = 0; i < kEntriesPerLane; ++i) {
         const int j = lane + 64 * i;
-        const bool valid = here && j < a.k;
-        idx[i] = valid ? a.index[row * a.k + j] : -1;
-        t[i] = valid ? load_as_float(a.logits, row * a.k + j, a.dtype) : -INFINITY;
-        is[i] = idx[i] >= 0 && !(t[i] == -INFINITY);
-        outside |= is[i] && idx[i] >= a.vocab;
+        const int64_t name = j < a.k ? a.index[row * a.k + j] : -1;
+        t[i] = j < a.k ? load_as_float(a.logits, row * a.k + j, a.dtype) : -INFINITY;
+        is[i] = name >= 0 && !(t[i] == -INFINITY);
+        outside |= is[i] && name >= a.vocab;
+        w.index[i] = is[i] ? static_cast<int32_t>(name < a.vocab ? name : a.vocab) : -1;
         if (is[i]) peak = fmaxf(peak, t[i]);
     }
     peak = wave_max(peak);
     outside = __any(outside);
-    float norm = 0.0f;
+    float norm;
     if (a.lse) {
-        norm = here ? a.lse[row] : 0.0f;
+        norm = a.lse[row];
     } else {
+#pragma unroll
         for (int i = 0; i < kEntriesPerLane; ++i)
             if (is[i]) sum += expf((t[i] - peak) * a.inv_t);
         norm = logf(wave_sum(sum));
     }
-    float logp[kEntriesPerLane];
+    bool any = false;
+#pragma unroll
     for (int i = 0; i < kEntriesPerLane; ++i) {
         logp[i] = a.lse ? t[i] * a.inv_t - norm : (t[i] - peak) * a.inv_t - norm;
-        p[i] = is[i] ? expf(logp[i]) : 0.0f;
-        names[wave][lane + 64 * i] = is[i] ? idx[i] : -1;
-        probs[wave][lane + 64 * i] = p[i];
+        w.p[i] = is[i] ? expf(logp[i]) : 0.0f;
+        any |= is[i];
+        names[lane + 64 * i] = w.index[i];
+        probs[lane + 64 * i] = w.p[i];
     }
-    __syncthreads();
-    float mass = 0.0f, entropy = 0.0f, count = 0.0f;
+    w.counts = __any(any);
+    asm volatile("" ::: "memory");        // the wave's own writes, in order: read back as they were written
+    int again[kEntriesPerLane] = {};        // how many of the names are this one
+    for (int o = 0; o < a.k; o += 4) {
+        const int4 four = *reinterpret_cast<const int4*>(names + o);
+#pragma unroll
+        for (int i = 0; i < kEntriesPerLane; ++i) again[i] += (four.x == w.index[i]) + (four.y == w.index[i]) + (four.z == w.index[i]) + (four.w == w.index[i]);
+    }
+    w.mass = w.entropy = 0.0f;
+#pragma unroll
     for (int i = 0; i < kEntriesPerLane; ++i) {
-        const int j = lane + 64 * i;
-        if (is[i]) {
-            bool first = true, twice = false;
-            float all = p[i];
+        if (is[i] && again[i] > 1) {        // seldom
+            const int j = lane + 64 * i;
+            float all = 0.0f;
+            bool first = true;
             for (int o = 0; o < a.k; ++o)
-                if (o != j && names[wave][o] == idx[i]) {
-                    if (o < j) first = false;
-                    all += probs[wave][o];
-                    twice = true;
+                if (names[o] == w.index[i]) {
+                    first &= o >= j;
+                    all += probs[o];
                 }
-            count += 1.0f;
-            if (!first) is[i] = false;
-            else if (twice) {
-                p[i] = all;
-                logp[i] = logf(all);
-            }
+            is[i] = first;
+            w.p[i] = first ? all : 0.0f;
+            logp[i] = logf(all);
         }
         if (is[i]) {
-            mass += p[i];
-            if (p[i] != 0.0f) entropy += p[i] * logp[i];
+            w.mass += w.p[i];
+            if (w.p[i] != 0.0f) w.entropy += w.p[i] * logp[i];
         }
-        if (here && j < a.k) {
-            a.entry_index[row * a.k + j] = is[i] && !outside ? static_cast<int32_t>(idx[i]) : -1;
-            a.entry_p[row * a.k + j] = is[i] ? p[i] : 0.0f;
+        if (!is[i] || outside) w.index[i] = -1;
+    }
+    w.mass = wave_sum(w.mass);
+    w.entropy = outside ? NAN : wave_sum(w.entropy);
+    return w;
+}
+
+__device__ inline void keep_entries(const TeacherArgs& a, int64_t row, const WaveEntries& w) {
+#pragma unroll
+    for (int i = 0; i < kEntriesPerLane; ++i) {
+        const int j = (threadIdx.x & 63) + 64 * i;
+        if (j < a.k) {
+            a.entry_index[row * a.k + j] = w.index[i];
+            a.entry_p[row * a.k + j] = w.p[i];
         }
     }
-    mass = wave_sum(mass);
-    entropy = wave_sum(entropy);
-    count = wave_sum(count);
-    if (here && lane == 0) a.row[row] = make_float4(mass, outside ? NAN : entropy, count, 0.0f);
+}
+
+// What a row's entries, their logits and the rest of its tokens (peak and sum) make of it, by one wave.
+struct RowResult {
+    RowState state;
+    float loss;
+};
+__device__ inline RowResult row_result(const TeacherArgs& a, const WaveEntries& w, const float (&z)[kEntriesPerLane], float rest_peak, float rest_sum) {
+    const float c = a.inv_t * kLog2e;
+    float top = rest_peak;
+#pragma unroll
+    for (int i = 0; i < kEntriesPerLane; ++i)
+        if (w.index[i] >= 0) top = fmaxf(top, z[i]);
+    top = wave_max(top);
+    float held = 0.0f, cross = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kEntriesPerLane; ++i)
+        if (w.index[i] >= 0 && z[i] != -INFINITY) held += __builtin_amdgcn_exp2f((z[i] - top) * c);
+    held = wave_sum(held);
+    const float all = held + rescale(rest_sum, rest_peak, top, c), log_all = logf(all);
+#pragma unroll
+    for (int i = 0; i < kEntriesPerLane; ++i)
+        if (w.index[i] >= 0 && w.p[i] != 0.0f) cross += w.p[i] * ((z[i] - top) * a.inv_t - log_all);
+    cross = wave_sum(cross);
+    RowResult r = {{0.0f, 0.0f, 0.0f, 0.0f}, 0.0f};
+    if (!w.counts) return r;
+    const bool others = rest_sum != 0.0f;
+    const float left = a.lse && others ? fmaxf(1.0f - w.mass, 0.0f) : 0.0f, mass = w.mass + left;
+    float rest = 0.0f, share = 0.0f;        // of the student: log R and R
+    if (others) {
+        rest = (rest_peak - top) * a.inv_t + logf(rest_sum) - log_all;
+        share = expf(rest);
+    }
+    r.loss = w.entropy - cross;
+    if (left != 0.0f) r.loss += left * (logf(left) - rest);
+    r.loss *= a.t * a.t;
+    r.state.peak_rest = others ? rest_peak : 0.0f;
+    r.state.slope = others ? (mass * share - left) / rest_sum : 0.0f;
+    r.state.peak = top;
+    r.state.mass = mass / all;
+    if (w.entropy != w.entropy) r.state.slope = r.state.mass = NAN;
+    return r;
+}
+
+__global__ __launch_bounds__(kThreads) void teacher_kernel(TeacherArgs a) {
+    __shared__ __align__(16) int32_t names[kThreads / 64][64 * kEntriesPerLane];
+    __shared__ float probs[kThreads / 64][64 * kEntriesPerLane];
+    const int wave = threadIdx.x >> 6;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + wave;
+    if (row >= a.rows) return;
+    const WaveEntries w = wave_entries(a, row, names[wave], probs[wave]);
+    keep_entries(a, row, w);
+    if ((threadIdx.x & 63) == 0) a.row[row] = make_float4(w.mass, w.entropy, w.counts ? 1.0f : 0.0f, 0.0f);
 }
 
 constexpr int kJoinThreads = 1024, kJoinRows = 64, kJoinWaves = kJoinThreads / 64;
@@ -174,51 +245,24 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(JoinArgs a) {
     }
     for (int r = wave; r < kJoinRows && first + r < a.rows; r += kJoinWaves) {
         const int64_t row = first + r;
-        const float rest_peak = peaks[0][r], rest_sum = sums[0][r];
         const float4 teacher = a.teacher_row[row];
-        float top = rest_peak;
-        for (int j = lane; j < a.entries.k; j += 64)
-            if (a.entries.index[row * a.entries.k + j] >= 0) top = fmaxf(top, a.entry_logit[row * a.entries.k + j]);
-        top = wave_max(top);
-        float held = 0.0f;
-        for (int j = lane; j < a.entries.k; j += 64)
-            if (a.entries.index[row * a.entries.k + j] >= 0) {
-                const float z = a.entry_logit[row * a.entries.k + j];
-                if (z != -INFINITY) held += __builtin_amdgcn_exp2f((z - top) * a.c);
-            }
-        held = wave_sum(held);
-        const float all = held + rescale(rest_sum, rest_peak, top, a.c), log_all = logf(all);
-        float cross = 0.0f;
-        for (int j = lane; j < a.entries.k; j += 64)
-            if (a.entries.index[row * a.entries.k + j] >= 0) {
-                const float p = a.entries.p[row * a.entries.k + j];
-                if (p != 0.0f) cross += p * ((a.entry_logit[row * a.entries.k + j] - top) * a.inv_t - log_all);
-            }
-        cross = wave_sum(cross);
-        if (lane) continue;
-        RowState st = {0.0f, 0.0f, 0.0f, 0.0f};
-        float loss = 0.0f;
-        if (teacher.z != 0.0f) {
-            const bool others = rest_sum != 0.0f;
-            float left = a.has_rest && others ? 1.0f - teacher.x : 0.0f;
-            if (left < 0.0f) left = 0.0f;
-            const float mass = teacher.x + left;
-            float rest = 0.0f, share = 0.0f;    // of the student: log R and R
-            if (others) {
-                rest = (rest_peak - top) * a.inv_t + logf(rest_sum) - log_all;
-                share = expf(rest);
-            }
-            loss = teacher.y - cross;
-            if (left != 0.0f) loss += left * (logf(left) - rest);
-            loss *= a.t * a.t;
-            st.peak_rest = others ? rest_peak : 0.0f;
-            st.slope = others ? (mass * share - left) / rest_sum : 0.0f;
-            st.peak = top;
-            st.mass = mass / all;
-            if (teacher.y != teacher.y) st.slope = st.mass = NAN;       // a name outside the vocabulary
+        WaveEntries w;
+        w.mass = teacher.x;
+        w.entropy = teacher.y;
+        w.counts = teacher.z != 0.0f;
+        float z[kEntriesPerLane];
+#pragma unroll
+        for (int i = 0; i < kEntriesPerLane; ++i) {
+            const int j = lane + 64 * i;
+            w.index[i] = j < a.entries.k ? a.entries.index[row * a.entries.k + j] : -1;
+            w.p[i] = j < a.entries.k ? a.entries.p[row * a.entries.k + j] : 0.0f;
+            z[i] = w.index[i] >= 0 ? a.entry_logit[row * a.entries.k + j] : 0.0f;
         }
-        a.state[row] = st;
-        a.row_loss[row] = loss;
+        const RowResult result = row_result(a.teacher, w, z, peaks[0][r], sums[0][r]);
+        if (lane == 0) {
+            a.state[row] = result.state;
+            a.row_loss[row] = result.loss;
+        }
     }
 }
 
@@ -251,14 +295,18 @@ __global__ __launch_bounds__(kJoinThreads) void reduce_kernel(const float* row_l
     if (reduction != JABAS_LOSS_NONE) *loss_out = static_cast<float>(sum * share);
 }
 
+// The gradient of a row's loss in units of dz; 0 where it does not count.
+__device__ inline float row_gradient(const float* upstream, int per_row, const float* reduce, float t, const RowState& st, int64_t row) {
+    return counts(st) ? upstream[per_row ? row : 0] * (*reduce * t) : 0.0f;
+}
+
 __global__ __launch_bounds__(kJoinThreads) void row_grad_kernel(const float* upstream, int per_row, const float* reduce, float t, const RowState* state,
                                                                 int64_t rows, float* grad, float* ratio, float* peak) {
     __shared__ float peaks[kJoinWaves];
-    const float share = *reduce * t;
     float top = 0.0f;
     bool bad = false;
     for (int64_t i = threadIdx.x; i < rows; i += kJoinThreads) {
-        const float g = counts(state[i]) ? upstream[per_row ? i : 0] * share : 0.0f;
+        const float g = row_gradient(upstream, per_row, reduce, t, state[i], i);
         grad[i] = g;
         bad |= !(fabsf(g) < INFINITY);
         top = fmaxf(top, fabsf(g));
@@ -272,7 +320,7 @@ __global__ __launch_bounds__(kJoinThreads) void row_grad_kernel(const float* ups
     const bool whole = top < INFINITY;
     if (threadIdx.x == 0) *peak = whole ? top : NAN;
     for (int64_t i = threadIdx.x; i < rows; i += kJoinThreads) {
-        const float g = counts(state[i]) ? upstream[per_row ? i : 0] * share : 0.0f;
+        const float g = row_gradient(upstream, per_row, reduce, t, state[i], i);
         ratio[i] = g == 0.0f ? 0.0f : whole ? g / top : 1.0f;
     }
 }
@@ -291,8 +339,6 @@ __global__ __launch_bounds__(kThreads) void zero_kernel(uint16_t* p, size_t n) {
 }
 
 // ------------------------------------------------------------------ logits in hand
-
-constexpr int kMaskTokens = 32768;      // tokens of a split at most: a bit for each in LDS
 
 template <class T>
 struct Vec;
@@ -317,71 +363,166 @@ struct __attribute__((packed, aligned(sizeof(T)))) Pack {
     T v[Vec<T>::n];
 };
 
-// Bits of the split's tokens that are entries of the row.
-__device__ inline void build_mask(const Entries& en, int64_t row, int64_t begin, int64_t end, uint32_t* mask) {
-    const int words = static_cast<int>((end - begin + 31) / 32);
-    for (int i = threadIdx.x; i < words; i += kThreads) mask[i] = 0;
-    __syncthreads();
-    for (int j = threadIdx.x; j < en.k; j += kThreads) {
-        const int64_t v = static_cast<int64_t>(en.index[row * en.k + j]) - begin;
-        if (v >= 0 && v < end - begin) atomicOr(&mask[v >> 5], 1u << (v & 31));
-    }
-    __syncthreads();
+// Bits of the tokens [begin, end) that are entries of a row, by thread j for entry j; `mask` holds zeros.
+static_assert(JABAS_LOSS_MAX_ENTRIES <= kThreads, "a thread per entry");
+__device__ inline void mark(uint32_t* mask, int64_t name, int64_t begin, int64_t end) {
+    if (name >= begin && name < end) atomicOr(&mask[(name - begin) >> 5], 1u << ((name - begin) & 31));
 }
 
+// Running maximum and sum of 2^((z - max) c) over the tokens [begin, end) of a row that the mask leaves, for the workgroup: each thread
+// takes kUnroll vectors at a time, so that 64 bytes of each are on their way; its maximum moves once for all of them.
+constexpr int kUnroll = 4;
 template <class T>
-__global__ __launch_bounds__(kThreads) void topk_forward_kernel(TopkArgs a) {
-    __shared__ uint32_t mask[kMaskTokens / 32];
-    __shared__ float peaks[kThreads / 64], sums[kThreads / 64];
+__device__ inline void stream_row(const T* z, int64_t begin, int64_t end, const uint32_t* mask, float c, float& peak, float& sum) {
     constexpr int n = Vec<T>::n;
-    const int64_t row = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
-    const int64_t begin = split * a.chunk, end = min(a.vocab, begin + a.chunk);
-    const T* z = static_cast<const T*>(a.logits) + row * a.stride;
-    build_mask(a.entries, row, begin, end, mask);
-    for (int j = threadIdx.x; j < a.entries.k; j += kThreads) {
-        const int64_t v = a.entries.index[row * a.entries.k + j];
-        if (v >= begin && v < end) a.entry_logit[row * a.entries.k + j] = Vec<T>::get(z[v]);
-    }
-    float peak = -INFINITY, sum = 0.0f;
-    for (int64_t at = begin + threadIdx.x * n; at < end; at += kThreads * n) {
-        float x[n];
-        if (at + n <= end) {
-            const Pack<T> p = *reinterpret_cast<const Pack<T>*>(z + at);
-#pragma unroll
-            for (int i = 0; i < n; ++i) x[i] = Vec<T>::get(p.v[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < n; ++i) x[i] = at + i < end ? Vec<T>::get(z[at + i]) : -INFINITY;
-        }
-        const int off = static_cast<int>(at - begin);
-        const uint32_t hits = mask[off >> 5] >> (off & 31);     // n divides 32: one word holds them all
+    peak = -INFINITY;
+    sum = 0.0f;
+    const auto take = [&](float (&x)[kUnroll * n]) {
         float top = peak;
 #pragma unroll
-        for (int i = 0; i < n; ++i) {
-            if ((hits >> i) & 1) x[i] = -INFINITY;
-            top = fmaxf(top, x[i]);
-        }
+        for (int i = 0; i < kUnroll * n; ++i) top = fmaxf(top, x[i]);
         const float base = top == -INFINITY ? 0.0f : top;
-        sum = rescale(sum, peak, base, a.c);
+        float more = 0.0f;
 #pragma unroll
-        for (int i = 0; i < n; ++i) sum += __builtin_amdgcn_exp2f((x[i] - base) * a.c);
+        for (int i = 0; i < kUnroll * n; ++i) more += __builtin_amdgcn_exp2f((x[i] - base) * c);
+        sum = rescale(sum, peak, base, c) + more;
         peak = top;
+    };
+    const auto drop = [&](float* x, int64_t at) {       // n divides 32: one word holds a vector's bits
+        const int off = static_cast<int>(at - begin);
+        const uint32_t hits = mask[off >> 5] >> (off & 31) & ((1u << n) - 1);
+        if (hits)
+#pragma unroll
+            for (int i = 0; i < n; ++i)
+                if ((hits >> i) & 1) x[i] = -INFINITY;
+    };
+    int64_t first = begin;
+    constexpr int64_t kRound = static_cast<int64_t>(kThreads) * n * kUnroll;
+    for (; first + kRound <= end; first += kRound) {
+        Pack<T> p[kUnroll];
+        float x[kUnroll * n];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) p[u] = *reinterpret_cast<const Pack<T>*>(z + first + (u * kThreads + threadIdx.x) * n);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+#pragma unroll
+            for (int i = 0; i < n; ++i) x[u * n + i] = Vec<T>::get(p[u].v[i]);
+            drop(x + u * n, first + (u * kThreads + threadIdx.x) * n);
+        }
+        take(x);
     }
+    if (first + static_cast<int>(threadIdx.x) * n < end) {
+        float x[kUnroll * n];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int64_t at = first + (u * kThreads + threadIdx.x) * n;
+            if (at + n <= end) {
+                const Pack<T> p = *reinterpret_cast<const Pack<T>*>(z + at);
+#pragma unroll
+                for (int i = 0; i < n; ++i) x[u * n + i] = Vec<T>::get(p.v[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < n; ++i) x[u * n + i] = at + i < end ? Vec<T>::get(z[at + i]) : -INFINITY;
+            }
+            if (at < end) drop(x + u * n, at);
+        }
+        take(x);
+    }
+    __shared__ float peaks[kThreads / 64], sums[kThreads / 64];
     const float top = wave_max(peak);
-    sum = wave_sum(rescale(sum, peak, top, a.c));
+    sum = wave_sum(rescale(sum, peak, top, c));
     if ((threadIdx.x & 63) == 0) {
         peaks[threadIdx.x >> 6] = top;
         sums[threadIdx.x >> 6] = sum;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        float p = peaks[0], s = sums[0];
-        for (int i = 1; i < kThreads / 64; ++i) {
-            const float q = fmaxf(p, peaks[i]);
-            s = rescale(s, p, q, a.c) + rescale(sums[i], peaks[i], q, a.c);
-            p = q;
-        }
-        a.partial[split * a.rows + row] = make_float2(p, s);
+    peak = peaks[0];
+    sum = sums[0];
+#pragma unroll
+    for (int i = 1; i < kThreads / 64; ++i) {
+        const float p = fmaxf(peak, peaks[i]);
+        sum = rescale(sum, peak, p, c) + rescale(sums[i], peaks[i], p, c);
+        peak = p;
+    }
+}
+
+// A row per workgroup: entries, stream, loss and state in one launch. Wave 0 sees to the entries.
+template <class T>
+__global__ __launch_bounds__(kThreads) void topk_row_kernel(TopkArgs a) {
+    extern __shared__ __align__(16) uint32_t mask[];
+    __shared__ __align__(16) int32_t names[64 * kEntriesPerLane];
+    __shared__ float probs[64 * kEntriesPerLane];
+    const int64_t row = blockIdx.x;
+    const int t = threadIdx.x;
+    const T* z = static_cast<const T*>(a.logits) + row * a.stride;
+    const int64_t name = t < a.teacher.k ? a.teacher.index[row * a.teacher.k + t] : -1;
+    const bool is = name >= 0 && name < a.vocab && !(load_as_float(a.teacher.logits, row * a.teacher.k + t, a.dtype) == -INFINITY);
+    const int words = static_cast<int>((a.vocab + 31) / 32);
+    for (int i = t; i < words; i += kThreads) mask[i] = 0;
+    __syncthreads();
+    if (is) mark(mask, name, 0, a.vocab);
+    __syncthreads();
+    float peak, sum;
+    stream_row(z, 0, a.vocab, mask, a.c, peak, sum);
+    if (t >= 64) return;
+    const WaveEntries w = wave_entries(a.teacher, row, names, probs);
+    keep_entries(a.teacher, row, w);
+    float logits[kEntriesPerLane];
+#pragma unroll
+    for (int i = 0; i < kEntriesPerLane; ++i) logits[i] = w.index[i] >= 0 ? Vec<T>::get(z[w.index[i]]) : 0.0f;
+    const RowResult r = row_result(a.teacher, w, logits, peak, sum);
+    if (t == 0) {
+        a.state[row] = r.state;
+        a.row_loss[row] = r.loss;
+    }
+}
+
+// Few rows: a chunk of a row per workgroup, joined by topk_join_kernel.
+template <class T>
+__global__ __launch_bounds__(kThreads) void topk_split_kernel(TopkArgs a) {
+    extern __shared__ __align__(16) uint32_t mask[];
+    const int64_t row = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+    const int64_t begin = split * a.chunk, end = min(a.vocab, begin + a.chunk);
+    const int t = threadIdx.x;
+    const int64_t name = t < a.teacher.k ? a.teacher.index[row * a.teacher.k + t] : -1;
+    const bool is = name >= 0 && name < a.vocab && !(load_as_float(a.teacher.logits, row * a.teacher.k + t, a.dtype) == -INFINITY);
+    const int words = static_cast<int>((end - begin + 31) / 32);
+    for (int i = t; i < words; i += kThreads) mask[i] = 0;
+    __syncthreads();
+    if (is) mark(mask, name, begin, end);
+    __syncthreads();
+    float peak, sum;
+    stream_row(static_cast<const T*>(a.logits) + row * a.stride, begin, end, mask, a.c, peak, sum);
+    if (t == 0) a.partial[row * a.splits + split] = make_float2(peak, sum);
+}
+
+// A wave per row.
+template <class T>
+__global__ __launch_bounds__(kThreads) void topk_join_kernel(TopkArgs a) {
+    __shared__ __align__(16) int32_t names[kThreads / 64][64 * kEntriesPerLane];
+    __shared__ float probs[kThreads / 64][64 * kEntriesPerLane];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + wave;
+    if (row >= a.rows) return;
+    float peak = -INFINITY, sum = 0.0f;
+    for (int i = lane; i < a.splits; i += 64) {
+        const float2 part = a.partial[row * a.splits + i];
+        const float p = fmaxf(peak, part.x);
+        sum = rescale(sum, peak, p, a.c) + rescale(part.y, part.x, p, a.c);
+        peak = p;
+    }
+    const float top = wave_max(peak);
+    sum = wave_sum(rescale(sum, peak, top, a.c));
+    const WaveEntries w = wave_entries(a.teacher, row, names[wave], probs[wave]);
+    keep_entries(a.teacher, row, w);
+    const T* z = static_cast<const T*>(a.logits) + row * a.stride;
+    float logits[kEntriesPerLane];
+#pragma unroll
+    for (int i = 0; i < kEntriesPerLane; ++i) logits[i] = w.index[i] >= 0 ? Vec<T>::get(z[w.index[i]]) : 0.0f;
+    const RowResult r = row_result(a.teacher, w, logits, top, sum);
+    if (lane == 0) {
+        a.state[row] = r.state;
+        a.row_loss[row] = r.loss;
     }
 }
 
@@ -393,39 +534,53 @@ __global__ __launch_bounds__(kThreads) void topk_backward_kernel(TopkArgs a) {
     const T* z = static_cast<const T*>(a.logits) + row * a.stride;
     T* out = static_cast<T*>(a.out) + row * a.vocab;
     const RowState st = a.state[row];
-    const float g = a.row_grad[row];
-    const bool live = counts(st) && g != 0.0f;
+    const float g = row_gradient(a.upstream, a.per_row, a.reduce, a.t, st, row);
+    const bool live = g != 0.0f;
     const float slope = st.slope * g;
-    for (int64_t at = begin + threadIdx.x * n; at < end; at += kThreads * n) {
+    const auto grad = [&](T x) { return Vec<T>::put(live ? slope * __builtin_amdgcn_exp2f((Vec<T>::get(x) - st.peak_rest) * a.c) : 0.0f); };
+    int64_t first = begin;
+    constexpr int64_t kRound = static_cast<int64_t>(kThreads) * n * kUnroll;
+    for (; first + kRound <= end; first += kRound) {
+        Pack<T> p[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) p[u] = *reinterpret_cast<const Pack<T>*>(z + first + (u * kThreads + threadIdx.x) * n);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+#pragma unroll
+            for (int i = 0; i < n; ++i) p[u].v[i] = grad(p[u].v[i]);
+            *reinterpret_cast<Pack<T>*>(out + first + (u * kThreads + threadIdx.x) * n) = p[u];
+        }
+    }
+    for (int64_t at = first + threadIdx.x * n; at < end; at += kThreads * n) {
         if (at + n <= end) {
             Pack<T> p = *reinterpret_cast<const Pack<T>*>(z + at);
 #pragma unroll
-            for (int i = 0; i < n; ++i)
-                p.v[i] = Vec<T>::put(live ? slope * __builtin_amdgcn_exp2f((Vec<T>::get(p.v[i]) - st.peak_rest) * a.c) : 0.0f);
+            for (int i = 0; i < n; ++i) p.v[i] = grad(p.v[i]);
             *reinterpret_cast<Pack<T>*>(out + at) = p;
         } else {
-            for (int64_t i = at; i < end; ++i)
-                out[i] = Vec<T>::put(live ? slope * __builtin_amdgcn_exp2f((Vec<T>::get(z[i]) - st.peak_rest) * a.c) : 0.0f);
+            for (int64_t i = at; i < end; ++i) out[i] = grad(z[i]);
         }
     }
     if (!live) return;
     __syncthreads();            // the entries' places are written again: behind the stores above, which the barrier waits for
-    for (int j = threadIdx.x; j < a.entries.k; j += kThreads) {
-        const int64_t v = a.entries.index[row * a.entries.k + j];
-        if (v >= begin && v < end)
-            out[v] = Vec<T>::put(g * (st.mass * __builtin_amdgcn_exp2f((Vec<T>::get(z[v]) - st.peak) * a.c) - a.entries.p[row * a.entries.k + j]));
-    }
+    const int j = threadIdx.x;
+    if (j >= a.entries.k) return;
+    const int64_t v = a.entries.index[row * a.entries.k + j];
+    if (v >= begin && v < end)
+        out[v] = Vec<T>::put(g * (st.mass * __builtin_amdgcn_exp2f((Vec<T>::get(z[v]) - st.peak) * a.c) - a.entries.p[row * a.entries.k + j]));
 }
 
-inline int launched() { return hipGetLastError() == hipSuccess ? JABAS_OK : JABAS_ERR_LAUNCH; }
-
 template <class... P, class... A>
-int launch(void (*kernel)(P...), unsigned grid, unsigned block, hipStream_t stream, A... args) {
+int launch_with(size_t lds, void (*kernel)(P...), unsigned grid, unsigned block, hipStream_t stream, A... args) {
     std::tuple<P...> held(args...);
     void* params[sizeof...(P)];
     size_t i = 0;
     std::apply([&](auto&... x) { ((params[i++] = &x), ...); }, held);
-    return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3(grid), dim3(block), params, 0, stream) == hipSuccess ? JABAS_OK : JABAS_ERR_LAUNCH;
+    return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3(grid), dim3(block), params, lds, stream) == hipSuccess ? JABAS_OK : JABAS_ERR_LAUNCH;
+}
+template <class... P, class... A>
+int launch(void (*kernel)(P...), unsigned grid, unsigned block, hipStream_t stream, A... args) {
+    return launch_with(0, kernel, grid, block, stream, args...);
 }
 
 }  // namespace
@@ -451,9 +606,15 @@ int launch_zero(void* p, size_t bytes, hipStream_t stream) {
     const size_t blocks = (n + kThreads - 1) / kThreads;
     return launch(zero_kernel, static_cast<unsigned>(blocks < 4096 ? blocks : 4096), kThreads, stream, static_cast<uint16_t*>(p), n);
 }
+template <class T>
+static int topk_forward(const TopkArgs& a, hipStream_t stream) {
+    const size_t lds = static_cast<size_t>((a.chunk + 31) / 32) * 4;
+    if (a.splits == 1) return launch_with(lds, topk_row_kernel<T>, static_cast<unsigned>(a.rows), kThreads, stream, a);
+    const int status = launch_with(lds, topk_split_kernel<T>, static_cast<unsigned>(a.rows * a.splits), kThreads, stream, a);
+    return status != JABAS_OK ? status : launch(topk_join_kernel<T>, static_cast<unsigned>((a.rows + kThreads / 64 - 1) / (kThreads / 64)), kThreads, stream, a);
+}
 int launch_topk_forward(const TopkArgs& a, hipStream_t stream) {
-    const unsigned grid = static_cast<unsigned>(a.rows * a.splits);
-    return a.dtype == JABAS_F32 ? launch(topk_forward_kernel<float>, grid, kThreads, stream, a) : launch(topk_forward_kernel<uint16_t>, grid, kThreads, stream, a);
+    return a.dtype == JABAS_F32 ? topk_forward<float>(a, stream) : topk_forward<uint16_t>(a, stream);
 }
 int launch_topk_backward(const TopkArgs& a, hipStream_t stream) {
     const unsigned grid = static_cast<unsigned>(a.rows * a.splits);
