@@ -17,8 +17,10 @@ inline int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; 
 inline int64_t tiles(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
 inline size_t element_bytes(int dtype) { return dtype == JABAS_F32 ? 4 : 2; }
 
+constexpr int64_t kNarrowPiece = int64_t{1} << 17;          // tokens whose row gradients are kept at once, in fp32: 32 MiB at most
+
 struct Shape {
-    bool linear, teacher;
+    bool linear, teacher, narrow;
     int planes;                 // of the operands: fp32 takes two
     int64_t depth;              // padded width
     bool copy_x, copy_w;        // operands that a product cannot read as they are
@@ -60,6 +62,7 @@ int validate(const JabasLoss* l, Shape& s) {
         misaligned(l->teacher_lse, 4) || misaligned(l->entry_index, 4) || misaligned(l->entry_p, 4))
         return JABAS_ERR_ALIGN;
     s.planes = l->dtype == JABAS_F32 ? 2 : 1;
+    s.narrow = s.linear && l->rows > 0 && l->rows <= kNarrowRows;
     s.depth = round_up(s.linear ? l->width : 1, kDepth);
     const auto as_is = [&](const void* p, int64_t stride) {
         return s.planes == 1 && l->width % kDepth == 0 && stride % 8 == 0 && stride <= kMaxStride && !misaligned(p, 16);
@@ -105,6 +108,7 @@ struct Forward {
     float* row_loss;
     uint16_t *x, *w;
     float *unscale_x, *unscale_w;
+    uint32_t* ticket;
     int64_t piece, splits, chunk;
     int64_t tiles;
     bool large;
@@ -133,7 +137,10 @@ size_t carve_forward(const JabasLoss* l, const Shape& s, char* base, Forward& f)
     Carver c{base, 0};
     const int64_t rows = l->rows;
     f = Forward{};
-    if (s.linear) {
+    if (s.narrow) {
+        f.tiles = narrow_tiles(l->vocab);
+        f.ticket = c.take<uint32_t>(1);
+    } else if (s.linear) {
         f.large = large_tiles(l->vocab, rows, s.planes);
         f.tiles = tiles(l->vocab, logits_tile_tokens(f.large));
         f.piece = piece_tokens(l, s, false);
@@ -145,7 +152,8 @@ size_t carve_forward(const JabasLoss* l, const Shape& s, char* base, Forward& f)
     if (l->label_smoothing != 0.0) f.total = c.take<float>(f.tiles * rows);
     if (s.linear) f.entry_logit = c.take<float>(rows * (s.teacher ? l->entries : 1));
     if (s.linear && s.teacher) f.teacher_row = c.take<float4>(rows);
-    f.row_loss = c.take<float>(rows);
+    f.row_loss = c.take<float>(s.narrow ? 2 * rows : rows);
+    if (s.narrow) return c.all();
     if (s.linear && s.copy_x) f.x = c.take<uint16_t>(rows * s.depth * s.planes);
     if (s.linear && s.copy_w) f.w = c.take<uint16_t>(f.piece * s.depth * s.planes);
     if (s.linear && s.planes == 2) {
@@ -164,6 +172,8 @@ struct Backward {
     int64_t piece, pad_rows, part_stride, splits, chunk;
     Splits inner;
     bool large;
+    float* narrow_dz;
+    NarrowSplits narrow;
 };
 
 size_t carve_backward(const JabasLoss* l, const Shape& s, char* base, Backward& b) {
@@ -172,6 +182,14 @@ size_t carve_backward(const JabasLoss* l, const Shape& s, char* base, Backward& 
     b = Backward{};
     if (!s.linear) {
         cut_rows(l, false, b.splits, b.chunk);
+        return c.all();
+    }
+    if (s.narrow) {
+        b.piece = l->vocab < kNarrowPiece ? l->vocab : kNarrowPiece;
+        b.narrow = narrow_splits(b.piece, l->width);
+        b.narrow_dz = c.take<float>((rows <= 32 ? 32 : 64) * narrow_tiles(b.piece) * 32);
+        b.part_stride = round_up(l->width, 4);
+        if (b.narrow.n > 1 || b.piece < l->vocab) b.part_h = c.take<float>(b.narrow.n * rows * b.part_stride);
         return c.all();
     }
     b.grad = c.take<float>(rows);
@@ -212,6 +230,21 @@ Entries entries_of(const JabasLoss* l, const Shape& s) {
 }
 
 constexpr double kLog2e = 1.4426950408889634;
+
+NarrowArgs narrow_args(const JabasLoss* l, const Entries& entries, float c) {
+    NarrowArgs a{};
+    a.x = l->hidden;
+    a.w = l->weight;
+    a.bias = l->bias;
+    a.x_stride = l->hidden_stride;
+    a.w_stride = l->weight_stride;
+    a.vocab = l->vocab;
+    a.rows = static_cast<int32_t>(l->rows);
+    a.width = static_cast<int32_t>(l->width);
+    a.c = c;
+    a.entries = entries;
+    return a;
+}
 
 const char* at(const void* p, int64_t elements, int dtype) {
     return static_cast<const char*>(p) + elements * static_cast<int64_t>(element_bytes(dtype));
@@ -320,7 +353,14 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
         t.row = f.teacher_row;
         if (s.linear) JABAS_TRY(launch_teacher(t, stream));
     }
-    if (s.linear) {
+    if (s.narrow) {
+        NarrowArgs a = narrow_args(l, entries, c);
+        a.partial = f.partial;
+        a.total = f.total;
+        a.entry_logit = f.entry_logit;
+        a.ticket = f.ticket;
+        JABAS_TRY(launch_narrow_forward(a, l->dtype, stream));
+    } else if (s.linear) {
         LogitsArgs a{};
         JABAS_TRY(lay_x(l, s, f.x, f.unscale_x, a.x, stream));
         a.depth = static_cast<int32_t>(s.depth);
@@ -370,6 +410,7 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
     j.teacher = t;
     j.state = state;
     j.row_loss = f.row_loss;
+    if (s.narrow) return launch_narrow_join(NarrowJoinArgs{j, f.ticket, l->reduction, loss_out, reduce}, stream);
     JABAS_TRY(launch_join(j, stream));
     return launch_reduce(f.row_loss, state, l->rows, l->reduction, loss_out, reduce, stream);
 }
@@ -417,6 +458,46 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
         return launch_topk_backward(a, stream);
     }
     if (!d_hidden && !d_weight && !d_bias) return JABAS_OK;
+    const float uniform = static_cast<float>(l->label_smoothing / static_cast<double>(l->vocab)), hit = static_cast<float>(1.0 - l->label_smoothing);
+    if (s.narrow) {
+        NarrowArgs a = narrow_args(l, entries_of(l, s), c);
+        a.state = state;
+        a.upstream = upstream;
+        a.per_row = per_row;
+        a.reduce = reduce;
+        a.t = static_cast<float>(l->temperature);
+        a.uniform = uniform;
+        a.hit = hit;
+        a.dz = d_hidden || d_weight ? b.narrow_dz : nullptr;
+        a.dz_stride = narrow_tiles(b.piece) * 32;
+        a.d_bias = d_bias;
+        a.d_weight = d_weight;
+        a.d_hidden = d_hidden;
+        a.each = b.narrow.each;
+        a.part = b.part_h;
+        a.part_stride = b.part_stride;
+        a.part_plane = l->rows * b.part_stride;
+        for (a.first = 0; a.first < l->vocab; a.first += b.piece) {
+            a.tokens = l->vocab - a.first < b.piece ? l->vocab - a.first : b.piece;
+            a.hidden_units = d_hidden ? (l->width + 127) / 128 * ((a.tokens + a.each - 1) / a.each) : 0;
+            a.add = a.first > 0;        // a shorter last piece adds to the first of the splits
+            JABAS_TRY(launch_narrow_backward(a, l->dtype, stream));
+            if (a.dz) JABAS_TRY(launch_narrow_grads(a, l->dtype, stream));
+        }
+        if (!d_hidden || !a.part) return JABAS_OK;
+        Job j{};
+        j.m = a.width;
+        j.n = a.rows;
+        j.splits = b.narrow.n;
+        j.part = a.part;
+        j.part_stride = a.part_stride;
+        j.part_plane = a.part_plane;
+        j.out = d_hidden;
+        j.out_stride = l->width;
+        j.out_dtype = l->dtype;
+        j.out_aligned = l->width % 4 == 0 && !misaligned(d_hidden, 4 * bytes);
+        return launch_join_splits(j, stream);
+    }
     JABAS_TRY(launch_row_grad(upstream, per_row, reduce, static_cast<float>(l->temperature), state, l->rows, b.grad, b.ratio, b.peak, stream));
     LogitsArgs a{};
     JABAS_TRY(lay_x(l, s, b.x, b.unscale_x, a.x, stream));
@@ -429,8 +510,8 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     a.entries = entries_of(l, s);
     a.state = state;
     a.row_grad = b.grad;
-    a.uniform = static_cast<float>(l->label_smoothing / static_cast<double>(l->vocab));
-    a.hit = static_cast<float>(1.0 - l->label_smoothing);
+    a.uniform = uniform;
+    a.hit = hit;
     a.dz = d_hidden || d_weight ? b.dz : nullptr;
     a.dz_stride = b.piece;
     a.dz_plane = b.pad_rows * b.piece;

@@ -170,6 +170,54 @@ int launch_row_grad(const float* upstream, int per_row, const float* reduce, flo
 int launch_bias_sum(const float* parts, int32_t tiles, int64_t stride, int64_t n, void* out, int32_t dtype, hipStream_t stream);
 int launch_zero(void* p, size_t bytes, hipStream_t stream);
 
+// Few rows, hidden states and weight as they lie (loss_narrow.hip).
+constexpr int kNarrowRows = 64;
+struct NarrowArgs {
+    const void *x, *w, *bias;
+    int64_t x_stride, w_stride, vocab;
+    int32_t rows, width;
+    float c;
+    Entries entries;
+    // forward
+    float2* partial;            // [row][tile]
+    float* total;               // [row][tile], or NULL
+    float* entry_logit;
+    uint32_t* ticket;           // set to 0
+    // backward
+    const RowState* state;
+    const float* upstream;
+    int32_t per_row;
+    const float* reduce;
+    float t;
+    float uniform, hit;
+    float* dz;                  // [32 or 64 rows][dz_stride tokens], in the units of the result, or NULL
+    int64_t dz_stride;          // the tokens in whole tiles
+    void* d_bias;
+    void* d_weight;
+    void* d_hidden;
+    int64_t first, tokens;      // of the piece, from a whole tile on
+    int64_t hidden_units;       // workgroups of dX
+    int64_t each;               // tokens of a split
+    float* part;                // [split][row][part_stride], or NULL: one split, one piece
+    int64_t part_stride, part_plane;
+    int32_t add;                // to what `part` holds
+};
+int64_t narrow_tiles(int64_t vocab);
+struct NarrowSplits { int64_t each; int32_t n; };
+NarrowSplits narrow_splits(int64_t tokens, int64_t width);
+int launch_narrow_forward(const NarrowArgs& a, int dtype, hipStream_t stream);
+int launch_narrow_backward(const NarrowArgs& a, int dtype, hipStream_t stream);
+int launch_narrow_grads(const NarrowArgs& a, int dtype, hipStream_t stream);
+// A workgroup per row; the last to finish reduces over the rows.
+struct NarrowJoinArgs {
+    JoinArgs join;              // partial and total: [row][tile]
+    uint32_t* ticket;
+    int32_t reduction;
+    float* loss_out;
+    float* reduce;
+};
+int launch_narrow_join(const NarrowJoinArgs& a, hipStream_t stream);
+
 // Logits in hand. One split: a workgroup per row; else a workgroup per `chunk` tokens of a row.
 struct TopkArgs {
     const void* logits;

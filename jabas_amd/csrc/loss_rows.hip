@@ -44,6 +44,7 @@ __device__ inline float rescale(float s, float from, float to, float c) {
 }
 
 constexpr int kEntriesPerLane = 4;
+static_assert(kNarrowRows <= 64, "a lane per row");
 static_assert(64 * kEntriesPerLane > JABAS_LOSS_MAX_ENTRIES, "a row's entries fit a wave");
 
 // A row's entries, entry lane + 64 i in place i of the lanes that hold it.
@@ -190,6 +191,41 @@ __global__ __launch_bounds__(kThreads) void teacher_kernel(TeacherArgs a) {
     if ((threadIdx.x & 63) == 0) a.row[row] = make_float4(w.mass, w.entropy, w.counts ? 1.0f : 0.0f, 0.0f);
 }
 
+// A row against its entries, as the teacher's kernel and the logits' kernels left them, by one wave.
+__device__ inline RowResult entries_result(const JoinArgs& a, int64_t row, float peak, float sum) {
+    const float4 teacher = a.teacher_row[row];
+    WaveEntries w;
+    w.mass = teacher.x;
+    w.entropy = teacher.y;
+    w.counts = teacher.z != 0.0f;
+    float z[kEntriesPerLane];
+#pragma unroll
+    for (int i = 0; i < kEntriesPerLane; ++i) {
+        const int j = (threadIdx.x & 63) + 64 * i;
+        w.index[i] = j < a.entries.k ? a.entries.index[row * a.entries.k + j] : -1;
+        w.p[i] = j < a.entries.k ? a.entries.p[row * a.entries.k + j] : 0.0f;
+        z[i] = w.index[i] >= 0 ? a.entry_logit[row * a.entries.k + j] : 0.0f;
+    }
+    return row_result(a.teacher, w, z, peak, sum);
+}
+
+// A row against its label.
+__device__ inline RowResult label_result(const JoinArgs& a, int64_t row, float peak, float sum, float total) {
+    RowResult r = {{0.0f, 0.0f, 0.0f, 0.0f}, 0.0f};
+    const int64_t label = a.entries.target[row];
+    if (label == a.entries.ignore_index) return r;
+    r.state.peak_rest = r.state.peak = peak;
+    r.state.slope = r.state.mass = 1.0f / sum;
+    const float e = a.smoothing;
+    if (label < 0 || label >= a.vocab) {
+        r.loss = r.state.slope = r.state.mass = NAN;
+    } else {
+        r.loss = logf(sum) + (1.0f - e) * (peak - a.entry_logit[row]);
+        if (e != 0.0f) r.loss += e * (peak - total / static_cast<float>(a.vocab));
+    }
+    return r;
+}
+
 constexpr int kJoinThreads = 1024, kJoinRows = 64, kJoinWaves = kJoinThreads / 64;
 
 // 64 rows per workgroup: each wave joins a sixteenth of the vocabulary's tiles with a row per lane, then the waves' results
@@ -225,40 +261,14 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(JoinArgs a) {
     __syncthreads();
     if (!a.entries.index) {
         if (wave != 0 || mine >= a.rows) return;
-        const int64_t label = a.entries.target[mine];
-        RowState st = {0.0f, 0.0f, 0.0f, 0.0f};
-        float loss = 0.0f;
-        if (label != a.entries.ignore_index) {
-            st.peak_rest = st.peak = peak;
-            st.slope = st.mass = 1.0f / sum;
-            const float e = a.smoothing;
-            if (label < 0 || label >= a.vocab) {
-                loss = st.slope = st.mass = NAN;
-            } else {
-                loss = logf(sum) + (1.0f - e) * (peak - a.entry_logit[mine]);
-                if (e != 0.0f) loss += e * (peak - total / static_cast<float>(a.vocab));
-            }
-        }
-        a.state[mine] = st;
-        a.row_loss[mine] = loss;
+        const RowResult r = label_result(a, mine, peak, sum, total);
+        a.state[mine] = r.state;
+        a.row_loss[mine] = r.loss;
         return;
     }
     for (int r = wave; r < kJoinRows && first + r < a.rows; r += kJoinWaves) {
         const int64_t row = first + r;
-        const float4 teacher = a.teacher_row[row];
-        WaveEntries w;
-        w.mass = teacher.x;
-        w.entropy = teacher.y;
-        w.counts = teacher.z != 0.0f;
-        float z[kEntriesPerLane];
-#pragma unroll
-        for (int i = 0; i < kEntriesPerLane; ++i) {
-            const int j = lane + 64 * i;
-            w.index[i] = j < a.entries.k ? a.entries.index[row * a.entries.k + j] : -1;
-            w.p[i] = j < a.entries.k ? a.entries.p[row * a.entries.k + j] : 0.0f;
-            z[i] = w.index[i] >= 0 ? a.entry_logit[row * a.entries.k + j] : 0.0f;
-        }
-        const RowResult result = row_result(a.teacher, w, z, peaks[0][r], sums[0][r]);
+        const RowResult result = entries_result(a, row, peaks[0][r], sums[0][r]);
         if (lane == 0) {
             a.state[row] = result.state;
             a.row_loss[row] = result.loss;
@@ -293,6 +303,65 @@ __global__ __launch_bounds__(kJoinThreads) void reduce_kernel(const float* row_l
     const double share = reduction == JABAS_LOSS_MEAN && number > 0.0 ? 1.0 / number : 1.0;
     *reduce = static_cast<float>(share);
     if (reduction != JABAS_LOSS_NONE) *loss_out = static_cast<float>(sum * share);
+}
+
+// Few rows: a workgroup joins a row's tiles; the last one to finish sums the rows' losses, in order.
+__global__ __launch_bounds__(kThreads) void narrow_join_kernel(NarrowJoinArgs args) {
+    const JoinArgs& a = args.join;
+    __shared__ float peaks[kThreads / 64], sums[kThreads / 64], totals[kThreads / 64];
+    const int t = threadIdx.x, wave = t >> 6;
+    const int64_t row = blockIdx.x;
+    float peak = -INFINITY, sum = 0.0f, total = 0.0f;
+    for (int i = t; i < a.tiles; i += kThreads) {
+        const float2 part = a.partial[row * a.tiles + i];
+        const float p = fmaxf(peak, part.x);
+        sum = rescale(sum, peak, p, a.c) + rescale(part.y, part.x, p, a.c);
+        peak = p;
+        if (a.total) total += a.total[row * a.tiles + i];
+    }
+    const float top = wave_max(peak);
+    sum = wave_sum(rescale(sum, peak, top, a.c));
+    total = wave_sum(total);
+    if ((t & 63) == 0) {
+        peaks[wave] = top;
+        sums[wave] = sum;
+        totals[wave] = total;
+    }
+    __syncthreads();
+    if (wave) return;
+    peak = peaks[0];
+    sum = sums[0];
+    total = totals[0];
+    for (int i = 1; i < kThreads / 64; ++i) {
+        const float p = fmaxf(peak, peaks[i]);
+        sum = rescale(sum, peak, p, a.c) + rescale(sums[i], peaks[i], p, a.c);
+        peak = p;
+        total += totals[i];
+    }
+    const RowResult r = a.entries.index ? entries_result(a, row, peak, sum) : label_result(a, row, peak, sum, total);
+    uint32_t done = 0;
+    if (t == 0) {
+        a.state[row] = r.state;
+        // what the last workgroup reads of the others: written through to the chip's memory, then the ticket
+        __hip_atomic_store(a.row_loss + row, r.loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(a.row_loss + a.rows + row, counts(r.state) ? 1.0f : 0.0f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (args.reduction == JABAS_LOSS_NONE) args.loss_out[row] = r.loss;
+        done = __hip_atomic_fetch_add(args.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    done = __builtin_amdgcn_readfirstlane(done);
+    if (done + 1 != a.rows) return;
+    const int lane = t & 63;
+    double loss = 0.0, number = 0.0;
+    if (lane < a.rows) {
+        loss = __hip_atomic_load(a.row_loss + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        number = __hip_atomic_load(a.row_loss + a.rows + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    loss = wave_sum(loss);
+    number = wave_sum(number);
+    if (lane) return;
+    const double share = args.reduction == JABAS_LOSS_MEAN && number > 0.0 ? 1.0 / number : 1.0;
+    *args.reduce = static_cast<float>(share);
+    if (args.reduction != JABAS_LOSS_NONE) *args.loss_out = static_cast<float>(loss * share);
 }
 
 // The gradient of a row's loss in units of dz; 0 where it does not count.
@@ -590,6 +659,9 @@ int launch_teacher(const TeacherArgs& a, hipStream_t stream) {
 }
 int launch_join(const JoinArgs& a, hipStream_t stream) {
     return launch(join_kernel, static_cast<unsigned>((a.rows + kJoinRows - 1) / kJoinRows), kJoinThreads, stream, a);
+}
+int launch_narrow_join(const NarrowJoinArgs& a, hipStream_t stream) {
+    return launch(narrow_join_kernel, static_cast<unsigned>(a.join.rows), kThreads, stream, a);
 }
 int launch_reduce(const float* row_loss, const RowState* state, int64_t rows, int reduction, float* loss_out, float* reduce, hipStream_t stream) {
     return launch(reduce_kernel, 1, kJoinThreads, stream, row_loss, state, rows, reduction, loss_out, reduce);
