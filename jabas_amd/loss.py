@@ -16,6 +16,7 @@ place in memory: nothing is changed in place, nothing is kept between calls but 
 row, 8 bytes an entry of the teacher). Results are the same from run to run: no sum depends on the order of atomics.
 """
 import ctypes as C
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -28,24 +29,27 @@ MAX_ENTRIES = L.LOSS_MAX_ENTRIES
 
 
 def _matrix(t, what, dtype=None):
-    """``t`` as a matrix whose rows are contiguous: as it is where it has that form, else a copy."""
+    """Refuses what is no fp32 or bf16 tensor (``dtype``: none of that type) on the GPU."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: expected a tensor")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{what}: must live on the GPU, got {t.device}")
     if dtype is None:
         if t.dtype not in (torch.float32, torch.bfloat16):
             raise TypeError(f"{what}: must be float32 or bfloat16, got {t.dtype}")
     elif t.dtype != dtype:
         raise TypeError(f"{what}: expected {dtype}, got {t.dtype}")
-    return t
 
 
 def _rows_of(t):
-    """(tensor, element stride of its rows) of a 2-D tensor with contiguous rows; a copy where the rows are not."""
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.stride(0) < 0:
-        t = t.contiguous()
-    return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    """``t`` as a matrix (its leading sizes as one) of contiguous rows: as it lies where it has that form, else a copy."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _check_row_tensor(t, shape, dtype, device, what):
@@ -55,8 +59,12 @@ def _check_row_tensor(t, shape, dtype, device, what):
         raise TypeError(f"{what}: expected {dtype}, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{what}: on {t.device}, expected {device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _flat(t):
+    return t if t.dim() == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
 
 
 def _reduction(name):
@@ -65,80 +73,95 @@ def _reduction(name):
     return REDUCTIONS[name]
 
 
-def _workspace(loss, backward, device):
-    n = L.lib().jabas_loss_workspace_bytes(C.byref(loss), int(backward))
+# JabasLoss as one write: a foreign assignment per field costs more than the launches of a short call (10 us in a backward thread)
+_LOSS = struct.Struct("4Q6q2iQqd3Qqd3Q")
+assert _LOSS.size == C.sizeof(L.JabasLoss)
+
+
+def _call(spec, hidden, weight, bias, logits, target, teacher_index, teacher_logits, teacher_lse, state):
+    """The JabasLoss of a call. ``spec``: reduction, ignore_index, label_smoothing, temperature; ``state``: the rows' states, then the
+    entries' probabilities, then their tokens."""
+    if hidden is None:
+        rows, vocab = logits.shape
+        ptrs, strides, width, dtype = (0, 0, 0, logits.data_ptr()), (0, 0, _row_stride(logits)), 0, logits.dtype
+    else:
+        rows, width = hidden.shape
+        vocab, dtype = weight.shape[0], hidden.dtype
+        ptrs = hidden.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), 0
+        strides = _row_stride(hidden), _row_stride(weight), 0
+    at = state.data_ptr()
+    if teacher_index is None:
+        k, against, entries = 0, (0, 0, 0), (0, 0)
+    else:
+        k = teacher_index.shape[1]
+        against = teacher_index.data_ptr(), teacher_logits.data_ptr(), 0 if teacher_lse is None else teacher_lse.data_ptr()
+        p = at + 16 * rows + 16
+        entries = p + 4 * rows * k, p
+    c = L.JabasLoss()
+    reduction, ignore_index, smoothing, temperature = spec
+    _LOSS.pack_into(c, 0, *ptrs, *strides, rows, vocab, width, L.F32 if dtype == torch.float32 else L.BF16, reduction,
+                    0 if target is None else target.data_ptr(), ignore_index, smoothing, *against, k, temperature, at, *entries)
+    return c
+
+
+def _workspace(c, backward, device):
+    n = L.lib().jabas_loss_workspace_bytes(C.byref(c), backward)
     # 256 bytes are what the caching allocator aligns to at least
     return torch.empty(n, dtype=torch.uint8, device=device), n
+
+
+def _forward(spec, tensors):
+    """(loss, state) on the current stream of the tensors' device."""
+    main = tensors[3] if tensors[0] is None else tensors[0]
+    device, rows = main.device, main.shape[0]
+    if device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return _forward(spec, tensors)
+    k = 0 if tensors[5] is None else tensors[5].shape[1]
+    state = torch.empty(4 * rows + 4 + 2 * rows * k, dtype=torch.float32, device=device)
+    out = torch.empty(rows if spec[0] == L.LOSS_NONE else (), dtype=torch.float32, device=device)
+    c = _call(spec, *tensors, state)
+    ws, n = _workspace(c, 0, device)
+    L.check(L.lib().jabas_loss_forward(C.byref(c), out.data_ptr(), ws.data_ptr(), n, _stream_ptr()), "jabas_loss_forward")
+    return out, state
+
+
+def _backward(spec, tensors, state, needs, upstream):
+    device = upstream.device
+    if device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return _backward(spec, tensors, state, needs, upstream)
+    if upstream.dtype != torch.float32 or not upstream.is_contiguous():
+        upstream = upstream.to(torch.float32).contiguous()
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=device) if t is not None and need else None for t, need in zip(tensors, needs)]
+    c = _call(spec, *tensors, state)
+    ws, n = _workspace(c, 1, device)
+    L.check(L.lib().jabas_loss_backward(C.byref(c), upstream.data_ptr(), *[None if t is None else t.data_ptr() for t in grads],
+                                        ws.data_ptr(), n, _stream_ptr()), "jabas_loss_backward")
+    return grads
 
 
 class _Loss(torch.autograd.Function):
     """``spec``: what is no tensor. The tensors come one by one so that autograd sees them."""
 
     @staticmethod
-    def forward(ctx, spec, hidden, weight, bias, logits, target, teacher_index, teacher_logits, teacher_lse):
-        main = logits if hidden is None else hidden
-        device, rows = main.device, main.shape[0]
-        if device.index != torch.cuda.current_device():
-            with torch.cuda.device(device):
-                return _Loss.forward(ctx, spec, hidden, weight, bias, logits, target, teacher_index, teacher_logits, teacher_lse)
-        state = torch.empty(4 * rows + 4, dtype=torch.float32, device=device)
-        k = 0 if teacher_index is None else teacher_index.shape[1]
-        entry_index = torch.empty(rows, k, dtype=torch.int32, device=device) if k else None
-        entry_p = torch.empty(rows, k, dtype=torch.float32, device=device) if k else None
-        kept = (hidden, weight, bias, logits, target, teacher_index, teacher_logits, teacher_lse, state, entry_index, entry_p)
-        c = _fill(spec, *kept)
-        out = torch.empty(rows if spec["reduction"] == L.LOSS_NONE else (), dtype=torch.float32, device=device)
-        ws, n = _workspace(c, False, device)
-        L.check(L.lib().jabas_loss_forward(C.byref(c), out.data_ptr(), ws.data_ptr(), n, _stream_ptr()), "jabas_loss_forward")
+    def forward(ctx, spec, *tensors):
+        out, state = _forward(spec, tensors)
         ctx.spec = spec
-        ctx.save_for_backward(*kept)
+        ctx.save_for_backward(*tensors, state)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, upstream):
-        kept = ctx.saved_tensors
-        hidden, weight, bias, logits = kept[:4]
-        device = upstream.device
-        if device.index != torch.cuda.current_device():
-            with torch.cuda.device(device):
-                return _Loss._grads(ctx, kept, upstream)
-        return _Loss._grads(ctx, kept, upstream)
-
-    @staticmethod
-    def _grads(ctx, kept, upstream):
-        c = _fill(ctx.spec, *kept)
-        upstream = upstream.to(torch.float32).contiguous()
-        wanted = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and need else None
-                  for t, need in zip(kept[:4], ctx.needs_input_grad[1:5])]
-        ws, n = _workspace(c, True, upstream.device)
-        L.check(L.lib().jabas_loss_backward(C.byref(c), upstream.data_ptr(), *[None if t is None else t.data_ptr() for t in wanted],
-                                            ws.data_ptr(), n, _stream_ptr()), "jabas_loss_backward")
-        return (None, *wanted, None, None, None, None)
+        *tensors, state = ctx.saved_tensors
+        return (None, *_backward(ctx.spec, tensors, state, ctx.needs_input_grad[1:5], upstream), None, None, None, None)
 
 
-def _fill(spec, hidden, weight, bias, logits, target, teacher_index, teacher_logits, teacher_lse, state, entry_index, entry_p):
-    def ptr(t):
-        return None if t is None else t.data_ptr()
-
-    c = L.JabasLoss()
-    main = logits if hidden is None else hidden
-    c.hidden, c.weight, c.bias, c.logits = ptr(hidden), ptr(weight), ptr(bias), ptr(logits)
-    if hidden is None:
-        c.rows, c.vocab = logits.shape
-        c.logits_stride = _rows_of(logits)[1]
-    else:
-        c.rows, c.width = hidden.shape
-        c.vocab = weight.shape[0]
-        c.hidden_stride, c.weight_stride = _rows_of(hidden)[1], _rows_of(weight)[1]
-    c.dtype = L.F32 if main.dtype == torch.float32 else L.BF16
-    c.reduction = spec["reduction"]
-    c.target, c.ignore_index, c.label_smoothing = ptr(target), spec.get("ignore_index", 0), spec.get("label_smoothing", 0.0)
-    c.teacher_index, c.teacher_logits, c.teacher_lse = ptr(teacher_index), ptr(teacher_logits), ptr(teacher_lse)
-    c.entries = 0 if teacher_index is None else teacher_index.shape[1]
-    c.temperature = spec.get("temperature", 1.0)
-    c.row_state, c.entry_index, c.entry_p = ptr(state), ptr(entry_index), ptr(entry_p)
-    return c
+def _apply(spec, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors[:4]):
+        return _Loss.apply(spec, *tensors)
+    return _forward(spec, tensors)[0]
 
 
 def _linear_inputs(hidden, weight, bias):
@@ -151,9 +174,9 @@ def _linear_inputs(hidden, weight, bias):
     if weight.device != hidden.device:
         raise ValueError(f"weight: on {weight.device}, expected {hidden.device}")
     if bias is not None:
-        _check_row_tensor(bias, (weight.shape[0],), hidden.dtype, hidden.device, "bias")
+        _check_row_tensor(bias, weight.shape[:1], hidden.dtype, hidden.device, "bias")
         bias = bias.contiguous()
-    return _rows_of(hidden.reshape(-1, hidden.shape[-1]))[0], _rows_of(weight)[0], bias
+    return _rows_of(hidden), _rows_of(weight), bias
 
 
 def _teacher_inputs(lead, device, dtype, teacher_index, teacher_logits, teacher_lse, temperature):
@@ -166,8 +189,8 @@ def _teacher_inputs(lead, device, dtype, teacher_index, teacher_logits, teacher_
     _check_row_tensor(teacher_logits, (*lead, k), dtype, device, "teacher_logits")
     if teacher_lse is not None:
         _check_row_tensor(teacher_lse, lead, torch.float32, device, "teacher_lse")
-        teacher_lse = teacher_lse.detach().reshape(-1).contiguous()
-    if not (temperature > 0.0 and temperature < float("inf")):
+        teacher_lse = _flat(teacher_lse.detach())
+    if not 0.0 < temperature < float("inf"):
         raise ValueError(f"temperature must be positive and finite, got {temperature}")
     return teacher_index.reshape(-1, k).contiguous(), teacher_logits.detach().reshape(-1, k).contiguous(), teacher_lse
 
@@ -189,8 +212,8 @@ def linear_cross_entropy(hidden, weight, target, bias=None, *, ignore_index=-100
     _check_row_tensor(target, lead, torch.int64, hidden.device, "target")
     if not 0.0 <= label_smoothing < 1.0:
         raise ValueError(f"label_smoothing must be in [0, 1), got {label_smoothing}")
-    spec = dict(reduction=_reduction(reduction), ignore_index=int(ignore_index), label_smoothing=float(label_smoothing))
-    out = _Loss.apply(spec, x, w, b, None, target.reshape(-1).contiguous(), None, None, None)
+    spec = _reduction(reduction), int(ignore_index), float(label_smoothing), 1.0
+    out = _apply(spec, x, w, b, None, _flat(target), None, None, None)
     return out.view(lead) if reduction == "none" else out
 
 
@@ -213,8 +236,7 @@ def topk_distillation(logits, teacher_index, teacher_logits, *, temperature=1.0,
         raise ValueError("logits: needs at least one token")
     lead = logits.shape[:-1]
     index, t, lse = _teacher_inputs(lead, logits.device, logits.dtype, teacher_index, teacher_logits, teacher_lse, temperature)
-    z = _rows_of(logits.reshape(-1, logits.shape[-1]))[0]
-    out = _Loss.apply(dict(reduction=_reduction(reduction), temperature=float(temperature)), None, None, None, z, None, index, t, lse)
+    out = _apply((_reduction(reduction), 0, 0.0, float(temperature)), None, None, None, _rows_of(logits), None, index, t, lse)
     return out.view(lead) if reduction == "none" else out
 
 
@@ -225,7 +247,7 @@ def linear_topk_distillation(hidden, weight, teacher_index, teacher_logits, bias
     x, w, b = _linear_inputs(hidden, weight, bias)
     lead = hidden.shape[:-1]
     index, t, lse = _teacher_inputs(lead, hidden.device, hidden.dtype, teacher_index, teacher_logits, teacher_lse, temperature)
-    out = _Loss.apply(dict(reduction=_reduction(reduction), temperature=float(temperature)), x, w, b, None, None, index, t, lse)
+    out = _apply((_reduction(reduction), 0, 0.0, float(temperature)), x, w, b, None, None, index, t, lse)
     return out.view(lead) if reduction == "none" else out
 
 
