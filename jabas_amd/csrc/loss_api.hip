@@ -141,8 +141,8 @@ size_t carve_forward(const JabasLoss* l, const Shape& s, char* base, Forward& f)
         f.tiles = narrow_tiles(l->vocab);
         f.ticket = c.take<uint32_t>(1);
     } else if (s.linear) {
-        f.large = large_tiles(l->vocab, rows, s.planes);
-        f.tiles = tiles(l->vocab, logits_tile_tokens(f.large));
+        f.large = large_tiles(l->vocab, rows);
+        f.tiles = tiles(l->vocab, logits_tile(f.large));
         f.piece = piece_tokens(l, s, false);
     } else {
         cut_rows(l, true, f.splits, f.chunk);
@@ -212,8 +212,8 @@ size_t carve_backward(const JabasLoss* l, const Shape& s, char* base, Backward& 
     b.inner = choose_splits(l->width, tokens, rows, true, true, b.piece < l->vocab, s.planes);
     if (b.inner.w > 1) b.part_w = c.take<float>(b.inner.w * tokens * b.part_stride);
     if (b.inner.h > 1 || b.piece < l->vocab) b.part_h = c.take<float>(b.inner.h * rows * b.part_stride);
-    b.large = large_tiles(tokens, rows, s.planes);
-    if (l->bias) b.db = c.take<float>(tiles(rows, logits_tile_rows(b.large, s.planes)) * b.piece);
+    b.large = large_tiles(tokens, rows);
+    if (l->bias) b.db = c.take<float>(tiles(rows, logits_tile(b.large)) * b.piece);
     return c.all();
 }
 
@@ -517,7 +517,7 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     a.dz_plane = b.pad_rows * b.piece;
     a.db = d_bias ? b.db : nullptr;
     a.pad_rows = static_cast<int32_t>(b.pad_rows);
-    const int32_t row_tiles = static_cast<int32_t>(tiles(l->rows, logits_tile_rows(b.large, s.planes)));
+    const int32_t row_tiles = static_cast<int32_t>(tiles(l->rows, logits_tile(b.large)));
     LayArgs lay{};
     lay.in_dtype = l->dtype;
     lay.cols = static_cast<int32_t>(l->width);

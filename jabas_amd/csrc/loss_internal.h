@@ -98,10 +98,9 @@ struct GradArgs {
     Job w, h;
     int32_t h_first;            // workgroups of h come first: they take longer
 };
-// Whether a product of m x n takes the large tiles, and how many of an operand's rows a tile of logits has.
-bool large_tiles(int64_t m, int64_t n, int planes);
-int logits_tile_tokens(bool large);
-int logits_tile_rows(bool large, int planes);
+// Whether a product of m x n takes the large tiles, and how many tokens and rows a tile of logits has.
+bool large_tiles(int64_t m, int64_t n);
+int logits_tile(bool large);
 int launch_logits_forward(const LogitsArgs& a, int planes, bool large, hipStream_t stream);
 int launch_logits_backward(const LogitsArgs& a, int planes, bool large, hipStream_t stream);
 struct Splits { int w, h; };

@@ -59,23 +59,39 @@ __device__ inline void load_tokens(const LogitsArgs& a, int m0, float* tokens) {
     if (P == 2) tokens[C::kM + m] = a.unscale_w[at];
 }
 
-// The tile's logits into c.acc. One plane: the sums start from the biases.
+// Nothing read from memory in front of this is kept for what follows: the accumulators leave no room for it.
+__device__ inline void keep_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+// `x` is computed here, not where it is first used.
+__device__ inline void settle(float& x) { asm volatile("" : "+v"(x)); }
+
+// The tile's logits, element e of block (i, j) of the lane. One plane: the sums start from the biases. Plain numbers: the accumulators'
+// blocks of 16 registers would be copied whole for every element that changes.
+template <class C>
+struct Tile {
+    float v[C::kI][C::kJ][16];
+};
 template <int P, class C>
-__device__ inline void logits_of(const LogitsArgs& a, int m0, int n0, char* smem, float* tokens, C& c) {
+__device__ inline void logits_of(const LogitsArgs& a, int m0, int n0, char* smem, float* tokens, Tile<C>& z) {
     const int wm = C::wave_m();
+    C c;
     c.run(a.w, a.x, m0, n0, a.depth, smem, [&] { load_tokens<P, C>(a, m0, tokens); },
           [&](int i, int e) { return P == 1 ? tokens[wm + C::block_m(i, e)] : 0.0f; });
-    if (P == 1) return;
 #pragma unroll
     for (int j = 0; j < C::kJ; ++j) {
-        const float ux = a.unscale_x[min(n0 + C::wave_n() + j * 32 + static_cast<int>(threadIdx.x & 31), a.x.rows - 1)];
+        const float ux = P == 2 ? a.unscale_x[min(n0 + C::wave_n() + j * 32 + static_cast<int>(threadIdx.x & 31), a.x.rows - 1)] : 1.0f;
 #pragma unroll
-        for (int i = 0; i < C::kI; ++i)
+        for (int i = 0; i < C::kI; ++i) {
+            if (P == 2) keep_order();
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int m = wm + C::block_m(i, e);
-                c.acc[i][j][e] = c.acc[i][j][e] * ux * tokens[C::kM + m] + tokens[m];
+                z.v[i][j][e] = P == 2 ? c.acc[i][j][e] * ux * tokens[C::kM + m] + tokens[m] : c.acc[i][j][e];
+                if (P == 2) settle(z.v[i][j][e]);
             }
+        }
     }
 }
 
@@ -108,8 +124,8 @@ __global__ __launch_bounds__(C::kThreads) void logits_forward_kernel(LogitsArgs 
     int tm, tn;
     tile_of(blockIdx.x, tiles_m<C>(a.w.rows), tiles_n<C>(a.x.rows), tm, tn);
     const int m0 = tm * C::kM, n0 = tn * C::kN, lane = threadIdx.x & 63;
-    C c;
-    logits_of<P>(a, m0, n0, smem, tokens, c);
+    Tile<C> z;
+    logits_of<P>(a, m0, n0, smem, tokens, z);
     const int wm = C::wave_m(), wn = C::wave_n();
     float peak[C::kJ], sum[C::kJ], total[C::kJ];
     if (m0 + C::kM > a.w.rows) {        // tokens past the end
@@ -120,7 +136,7 @@ __global__ __launch_bounds__(C::kThreads) void logits_forward_kernel(LogitsArgs 
                 const bool in = m0 + wm + C::block_m(i, e) < a.w.rows;
 #pragma unroll
                 for (int j = 0; j < C::kJ; ++j)
-                    if (!in) c.acc[i][j][e] = -INFINITY;
+                    if (!in) z.v[i][j][e] = -INFINITY;
             }
     }
     if (TEACHER) build_map<C>(a.entries, smem, a.first + m0, n0, a.x.rows);
@@ -139,18 +155,18 @@ __global__ __launch_bounds__(C::kThreads) void logits_forward_kernel(LogitsArgs 
                         for (int e = 0; e < 4; ++e) {
                             const uint32_t hit = (hits >> (8 * e)) & 0xff;
                             if (hit) {
-                                a.entry_logit[static_cast<int64_t>(n) * a.entries.k + hit - 1] = c.acc[i][j][q * 4 + e];
-                                c.acc[i][j][q * 4 + e] = -INFINITY;
+                                a.entry_logit[static_cast<int64_t>(n) * a.entries.k + hit - 1] = z.v[i][j][q * 4 + e];
+                                z.v[i][j][q * 4 + e] = -INFINITY;
                             }
                         }
                 }
         } else {
-            at_label<C>(label_of<C>(a, m0, n), [&](int i, int e) { a.entry_logit[n] = c.acc[i][j][e]; });
+            at_label<C>(label_of<C>(a, m0, n), [&](int i, int e) { a.entry_logit[n] = z.v[i][j][e]; });
             if (a.total) {
 #pragma unroll
                 for (int i = 0; i < C::kI; ++i)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) total[j] += m0 + C::kM <= a.w.rows || m0 + wm + C::block_m(i, e) < a.w.rows ? c.acc[i][j][e] : 0.0f;
+                    for (int e = 0; e < 16; ++e) total[j] += m0 + C::kM <= a.w.rows || m0 + wm + C::block_m(i, e) < a.w.rows ? z.v[i][j][e] : 0.0f;
                 total[j] += __shfl_xor(total[j], 32);
             }
         }
@@ -158,14 +174,14 @@ __global__ __launch_bounds__(C::kThreads) void logits_forward_kernel(LogitsArgs 
 #pragma unroll
         for (int i = 0; i < C::kI; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) peak[j] = fmaxf(peak[j], c.acc[i][j][e]);
+            for (int e = 0; e < 16; ++e) peak[j] = fmaxf(peak[j], z.v[i][j][e]);
         peak[j] = fmaxf(peak[j], __shfl_xor(peak[j], 32));
         const float base = peak[j] == -INFINITY ? 0.0f : peak[j];
         sum[j] = 0.0f;
 #pragma unroll
         for (int i = 0; i < C::kI; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sum[j] += __builtin_amdgcn_exp2f((c.acc[i][j][e] - base) * a.c);
+            for (int e = 0; e < 16; ++e) sum[j] += __builtin_amdgcn_exp2f((z.v[i][j][e] - base) * a.c);
         sum[j] += __shfl_xor(sum[j], 32);
     }
     // the waves that share rows: [wave of m][row of the tile]
@@ -217,42 +233,48 @@ __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs
     int tm, tn;
     tile_of(blockIdx.x, tiles_m<C>(a.w.rows), tiles_n<C>(a.x.rows), tm, tn);
     const int m0 = tm * C::kM, n0 = tn * C::kN, lane = threadIdx.x & 63;
-    C c;
-    logits_of<P>(a, m0, n0, smem, tokens, c);
+    Tile<C> z;
+    logits_of<P>(a, m0, n0, smem, tokens, z);
     const int wm = C::wave_m(), wn = C::wave_n();
     if (TEACHER) build_map<C>(a.entries, smem, a.first + m0, n0, a.x.rows);
     const float uniform = a.uniform * kDzScale;
 #pragma unroll
     for (int j = 0; j < C::kJ; ++j) {
+        keep_order();
         const int nl = wn + j * 32 + (lane & 31), n = n0 + nl;
         const RowState st = n < a.x.rows ? a.state[n] : RowState{0.0f, 0.0f, 0.0f, 0.0f};
         const bool counts = !(st.slope == 0.0f && st.mass == 0.0f);
         const float slope = st.slope * kDzScale;
 #pragma unroll
-        for (int i = 0; i < C::kI; ++i)
+        for (int i = 0; i < C::kI; ++i) {
+            if (P == 2) keep_order();
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const uint32_t hits = TEACHER ? reinterpret_cast<const uint32_t*>(smem)[((wm + C::block_m(i, q * 4)) >> 2) * C::kN + nl] : 0;
                 float d[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) d[e] = fmaf(slope, __builtin_amdgcn_exp2f((c.acc[i][j][q * 4 + e] - st.peak_rest) * a.c), -uniform);
+                for (int e = 0; e < 4; ++e) d[e] = fmaf(slope, __builtin_amdgcn_exp2f((z.v[i][j][q * 4 + e] - st.peak_rest) * a.c), -uniform);
                 if (TEACHER && hits)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const uint32_t hit = (hits >> (8 * e)) & 0xff;
                         if (hit)
-                            d[e] = (st.mass * __builtin_amdgcn_exp2f((c.acc[i][j][q * 4 + e] - st.peak) * a.c) -
+                            d[e] = (st.mass * __builtin_amdgcn_exp2f((z.v[i][j][q * 4 + e] - st.peak) * a.c) -
                                     a.entries.p[static_cast<int64_t>(n) * a.entries.k + hit - 1]) * kDzScale;
                     }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) c.acc[i][j][q * 4 + e] = d[e];
+                for (int e = 0; e < 4; ++e) {
+                    z.v[i][j][q * 4 + e] = d[e];
+                    if (P == 2) settle(z.v[i][j][q * 4 + e]);
+                }
             }
-        if (!TEACHER) at_label<C>(label_of<C>(a, m0, n), [&](int i, int e) { c.acc[i][j][e] -= a.hit * kDzScale; });
+        }
+        if (!TEACHER) at_label<C>(label_of<C>(a, m0, n), [&](int i, int e) { z.v[i][j][e] -= a.hit * kDzScale; });
         if (__any(!counts)) {
 #pragma unroll
             for (int i = 0; i < C::kI; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) c.acc[i][j][e] = counts ? c.acc[i][j][e] : 0.0f;
+                for (int e = 0; e < 16; ++e) z.v[i][j][e] = counts ? z.v[i][j][e] : 0.0f;
         }
     }
     if (m0 + C::kM > a.w.rows) {        // tokens past the end
@@ -263,7 +285,7 @@ __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs
                 const bool in = m0 + wm + C::block_m(i, e) < a.w.rows;
 #pragma unroll
                 for (int j = 0; j < C::kJ; ++j)
-                    if (!in) c.acc[i][j][e] = 0.0f;
+                    if (!in) z.v[i][j][e] = 0.0f;
             }
     }
     if (a.db) {      // sums over this tile's rows: within the wave, then over the waves that share tokens
@@ -282,7 +304,7 @@ __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs
             for (int x = 0; x < 32; ++x) {
                 v[x] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < C::kJ; ++j) v[x] += c.acc[i + (x >> 4)][j][x & 15] * g[j];
+                for (int j = 0; j < C::kJ; ++j) v[x] += z.v[i + (x >> 4)][j][x & 15] * g[j];
             }
             scatter_sum<16>(v);
             merge[wn / (C::kJ * 32) * C::kM + wm + C::block_m(i + ((lane & 31) >> 4), lane & 15)] = v[0];
@@ -301,26 +323,42 @@ __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs
     // The wave's part of dz through LDS, so that lanes write 16 consecutive bytes of a row: row n of kChunks chunks, chunk k at k ^ n % kChunks.
     constexpr int kRows = C::kJ * 32, kChunks = C::kI * 32 / 8;
     char* mine = smem + (threadIdx.x >> 6) * (kRows * kChunks * 16);
+    if (P == 2) {       // both planes of an element in the register that held it
+#pragma unroll
+        for (int j = 0; j < C::kJ; ++j)
+#pragma unroll
+            for (int i = 0; i < C::kI; ++i) {
+                keep_order();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const _Float16 hi = static_cast<_Float16>(z.v[i][j][e]);
+                    const _Float16 lo = static_cast<_Float16>((z.v[i][j][e] - static_cast<float>(hi)) * kLowScale);
+                    z.v[i][j][e] = __uint_as_float(__builtin_bit_cast(uint16_t, hi) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, lo)) << 16);
+                    settle(z.v[i][j][e]);
+                }
+            }
+    }
 #pragma unroll
     for (int p = 0; p < P; ++p) {
 #pragma unroll
         for (int j = 0; j < C::kJ; ++j)
 #pragma unroll
-            for (int i = 0; i < C::kI; ++i)
+            for (int i = 0; i < C::kI; ++i) {
+                keep_order();
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     f16x4 h;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float v = c.acc[i][j][q * 4 + e];
-                        h[e] = static_cast<_Float16>(v);
-                        if (p) h[e] = static_cast<_Float16>((v - static_cast<float>(h[e])) * kLowScale);
+                        const float v = z.v[i][j][q * 4 + e];
+                        h[e] = P == 2 ? __builtin_bit_cast(_Float16, static_cast<uint16_t>(__float_as_uint(v) >> (16 * p))) : static_cast<_Float16>(v);
                     }
                     const int r = j * 32 + (lane & 31), m = C::block_m(i, q * 4);
                     *reinterpret_cast<f16x4*>(mine + (r * kChunks + ((m >> 3) ^ (r % kChunks))) * 16 + (m & 4) * 2) = h;
                 }
+            }
         uint16_t* out = static_cast<uint16_t*>(a.dz) + p * a.dz_plane;
-#pragma unroll
+#pragma unroll 4
         for (int x = 0; x < kRows * kChunks / 64; ++x) {
             const int f = x * 64 + lane, r = f / kChunks, k = f % kChunks;
             const u32x4 v = *reinterpret_cast<const u32x4*>(mine + (r * kChunks + (k ^ (r % kChunks))) * 16);
@@ -441,7 +479,7 @@ int logits(const LogitsArgs& a, bool backward, hipStream_t stream) {
 }
 
 int logits(const LogitsArgs& a, int planes, bool large, bool backward, hipStream_t stream) {
-    if (planes == 2) return large ? logits<F16, 2, 256, 128, 4, 2>(a, backward, stream) : logits<F16, 2, 128, 128, 2, 2>(a, backward, stream);
+    if (planes == 2) return large ? logits<F16, 2, 256, 256, 2, 4>(a, backward, stream) : logits<F16, 2, 128, 128, 2, 2>(a, backward, stream);
     return large ? logits<BF16, 1, 256, 256, 2, 4>(a, backward, stream) : logits<BF16, 1, 128, 128, 2, 2>(a, backward, stream);
 }
 
@@ -453,17 +491,14 @@ int grads(const GradArgs& a, hipStream_t stream) {
     return launch(grads_kernel<CW, CH>, grid, CW::kThreads, a, stream);
 }
 
-struct Tile { int m, n; };
+struct Sizes { int m, n; };
 bool large_grads(int64_t features, int64_t tokens, int64_t rows) { return features > 128 && (tokens > 128 || rows > 128) && rows > 128; }
-Tile grads_tile(bool large, int planes) { return large ? Tile{256, planes == 2 ? 128 : 256} : Tile{128, 128}; }
+Sizes grads_tile(bool large) { return large ? Sizes{256, 256} : Sizes{128, 128}; }
 
 }  // namespace
 
-bool large_tiles(int64_t m, int64_t n, int planes) {
-    return ((m + 255) / 256) * (planes == 2 ? (n + 127) / 128 : (n + 255) / 256) >= 256;
-}
-int logits_tile_tokens(bool large) { return large ? 256 : 128; }
-int logits_tile_rows(bool large, int planes) { return large && planes == 1 ? 256 : 128; }
+bool large_tiles(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) >= 256; }
+int logits_tile(bool large) { return large ? 256 : 128; }
 
 int launch_logits_forward(const LogitsArgs& a, int planes, bool large, hipStream_t stream) { return logits(a, planes, large, false, stream); }
 int launch_logits_backward(const LogitsArgs& a, int planes, bool large, hipStream_t stream) { return logits(a, planes, large, true, stream); }
@@ -517,9 +552,9 @@ double makespan(int slots, int64_t na, double la, int64_t nb, double lb) {
 // 182 with them.
 Splits choose_splits(int64_t features, int64_t tokens, int64_t rows, bool w, bool h, bool many_pieces, int planes) {
     const bool large = large_grads(features, tokens, rows);
-    const Tile t = grads_tile(large, planes);
+    const Sizes t = grads_tile(large);
     const int slots = large ? 256 : 512;
-    const double kUnit = 6.0, bytes_per_step = (large ? 9e6 : 4.5e6) * (planes == 2 ? 1.5 : 1.0);
+    const double kUnit = 6.0, bytes_per_step = (large ? 9e6 : 4.5e6) * (planes == 2 ? 3 : 1);
     const int64_t fm = (features + t.m - 1) / t.m, tw = w ? fm * ((tokens + t.n - 1) / t.n) : 0, th = h ? fm * ((rows + t.n - 1) / t.n) : 0;
     const double kw = (rows + 63) / 64, kh = (tokens + 63) / 64;
     Splits best = {1, 1};
@@ -545,7 +580,7 @@ int launch_grads(GradArgs& a, int planes, hipStream_t stream) {
     const int64_t features = a.w.m > a.h.m ? a.w.m : a.h.m;
     a.h_first = !a.w.m || (a.h.m && a.h.each > a.w.each);
     const bool large = large_grads(features, a.w.m ? a.w.n : a.h.depth, a.h.m ? a.h.n : a.w.depth);
-    if (planes == 2) return large ? grads<2, 256, 128, 4, 2>(a, stream) : grads<2, 128, 128, 2, 2>(a, stream);
+    if (planes == 2) return large ? grads<2, 256, 256, 2, 4>(a, stream) : grads<2, 128, 128, 2, 2>(a, stream);
     return large ? grads<1, 256, 256, 2, 4>(a, stream) : grads<1, 128, 128, 2, 2>(a, stream);
 }
 
