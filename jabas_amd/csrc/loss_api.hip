@@ -23,7 +23,7 @@ struct Shape {
     bool linear, teacher, narrow;
     int planes;                 // of the operands: fp32 takes two
     int64_t depth;              // padded width
-    bool copy_x, copy_w;        // operands that a product cannot read as they are
+    bool copy_w;                // the products cannot read the weight as it is
 };
 
 bool misaligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
@@ -64,11 +64,7 @@ int validate(const JabasLoss* l, Shape& s) {
     s.planes = l->dtype == JABAS_F32 ? 2 : 1;
     s.narrow = s.linear && l->rows > 0 && l->rows <= kNarrowRows;
     s.depth = round_up(s.linear ? l->width : 1, kDepth);
-    const auto as_is = [&](const void* p, int64_t stride) {
-        return s.planes == 1 && l->width % kDepth == 0 && stride % 8 == 0 && stride <= kMaxStride && !misaligned(p, 16);
-    };
-    s.copy_x = !as_is(l->hidden, l->hidden_stride);
-    s.copy_w = !as_is(l->weight, l->weight_stride);
+    s.copy_w = !(s.planes == 1 && l->width % kDepth == 0 && l->weight_stride % 8 == 0 && l->weight_stride <= kMaxStride && !misaligned(l->weight, 16));
     return JABAS_OK;
 }
 
@@ -109,6 +105,7 @@ struct Forward {
     uint16_t *x, *w;
     float *unscale_x, *unscale_w;
     uint32_t* ticket;
+    int32_t *map, *live;
     int64_t piece, splits, chunk;
     int64_t tiles;
     bool large;
@@ -154,7 +151,11 @@ size_t carve_forward(const JabasLoss* l, const Shape& s, char* base, Forward& f)
     if (s.linear && s.teacher) f.teacher_row = c.take<float4>(rows);
     f.row_loss = c.take<float>(s.narrow ? 2 * rows : rows);
     if (s.narrow) return c.all();
-    if (s.linear && s.copy_x) f.x = c.take<uint16_t>(rows * s.depth * s.planes);
+    if (s.linear) {
+        f.map = c.take<int32_t>(rows);
+        f.live = c.take<int32_t>(1);
+    }
+    if (s.linear) f.x = c.take<uint16_t>(rows * s.depth * s.planes);
     if (s.linear && s.copy_w) f.w = c.take<uint16_t>(f.piece * s.depth * s.planes);
     if (s.linear && s.planes == 2) {
         f.unscale_x = c.take<float>(rows);
@@ -165,8 +166,9 @@ size_t carve_forward(const JabasLoss* l, const Shape& s, char* base, Forward& f)
 
 struct Backward {
     float *grad, *ratio, *peak;
-    uint16_t *x, *w;            // operands of the logits, where they are copies
+    uint16_t *x, *w;            // operands of the logits; w where it is a copy
     uint16_t *x16, *w16, *dz;   // of the gradients' products
+    int32_t *map, *live;
     float *unscale_x, *unscale_w, *unscale_x16, *unscale_w16, *parts;
     float *db, *part_w, *part_h;
     int64_t piece, pad_rows, part_stride, splits, chunk;
@@ -195,9 +197,11 @@ size_t carve_backward(const JabasLoss* l, const Shape& s, char* base, Backward& 
     b.grad = c.take<float>(rows);
     b.ratio = c.take<float>(rows);
     b.peak = c.take<float>(1);
+    b.map = c.take<int32_t>(rows);
+    b.live = c.take<int32_t>(1);
     b.piece = piece_tokens(l, s, true);
     b.pad_rows = round_up(rows, kDepth);
-    if (s.copy_x) b.x = c.take<uint16_t>(rows * s.depth * s.planes);
+    b.x = c.take<uint16_t>(rows * s.depth * s.planes);
     if (s.copy_w) b.w = c.take<uint16_t>(b.piece * s.depth * s.planes);
     b.unscale_x = c.take<float>(rows);
     b.unscale_w = c.take<float>(b.piece);
@@ -256,16 +260,11 @@ const char* at(const void* p, int64_t elements, int dtype) {
         if (status_ != JABAS_OK) return status_; \
     } while (0)
 
-// The hidden states as the products read them.
-int lay_x(const JabasLoss* l, const Shape& s, uint16_t* x, float* unscale, Operand& out, hipStream_t stream) {
+// The hidden states of the rows that count.
+int lay_x(const JabasLoss* l, const Shape& s, const Live& live, uint16_t* x, float* unscale, Operand& out, hipStream_t stream) {
     out.rows = static_cast<int32_t>(l->rows);
-    if (!s.copy_x) {
-        out.p = l->hidden;
-        out.stride = l->hidden_stride;
-        out.plane = 0;
-        return JABAS_OK;
-    }
     LayArgs a{};
+    a.live = live;
     a.in = l->hidden;
     a.in_stride = l->hidden_stride;
     a.in_dtype = l->dtype;
@@ -362,7 +361,18 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
         JABAS_TRY(launch_narrow_forward(a, l->dtype, stream));
     } else if (s.linear) {
         LogitsArgs a{};
-        JABAS_TRY(lay_x(l, s, f.x, f.unscale_x, a.x, stream));
+        LiveArgs live{};
+        live.target = l->target;
+        live.ignore_index = l->ignore_index;
+        live.teacher_row = f.teacher_row;
+        live.rows = l->rows;
+        live.map = f.map;
+        live.live = f.live;
+        live.state = state;
+        live.row_loss = f.row_loss;
+        JABAS_TRY(launch_live(live, stream));
+        a.rows = Live{f.map, f.live};
+        JABAS_TRY(lay_x(l, s, a.rows, f.x, f.unscale_x, a.x, stream));
         a.depth = static_cast<int32_t>(s.depth);
         a.unscale_x = f.unscale_x;
         a.unscale_w = f.unscale_w;
@@ -397,6 +407,7 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
         return launch_reduce(f.row_loss, state, l->rows, l->reduction, loss_out, reduce, stream);
     }
     JoinArgs j{};
+    j.live = Live{f.map, f.live};
     j.partial = f.partial;
     j.total = f.total;
     j.entry_logit = f.entry_logit;
@@ -498,9 +509,24 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
         j.out_aligned = l->width % 4 == 0 && !misaligned(d_hidden, 4 * bytes);
         return launch_join_splits(j, stream);
     }
-    JABAS_TRY(launch_row_grad(upstream, per_row, reduce, static_cast<float>(l->temperature), state, l->rows, b.grad, b.ratio, b.peak, stream));
+    RowGradArgs r{};
+    r.upstream = upstream;
+    r.per_row = per_row;
+    r.reduce = reduce;
+    r.t = static_cast<float>(l->temperature);
+    r.state = state;
+    r.rows = l->rows;
+    r.grad = b.grad;
+    r.ratio = b.ratio;
+    r.peak = b.peak;
+    r.map = b.map;
+    r.live = b.live;
+    JABAS_TRY(launch_row_grad(r, stream));
+    if (d_hidden) JABAS_TRY(launch_zero_rows(state, l->rows, l->width, l->dtype, d_hidden, stream));
+    const Live live = {b.map, b.live};
     LogitsArgs a{};
-    JABAS_TRY(lay_x(l, s, b.x, b.unscale_x, a.x, stream));
+    a.rows = live;
+    JABAS_TRY(lay_x(l, s, live, b.x, b.unscale_x, a.x, stream));
     a.depth = static_cast<int32_t>(s.depth);
     a.unscale_x = b.unscale_x;
     a.unscale_w = b.unscale_w;
@@ -516,8 +542,6 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     a.dz_stride = b.piece;
     a.dz_plane = b.pad_rows * b.piece;
     a.db = d_bias ? b.db : nullptr;
-    a.pad_rows = static_cast<int32_t>(b.pad_rows);
-    const int32_t row_tiles = static_cast<int32_t>(tiles(l->rows, logits_tile(b.large)));
     LayArgs lay{};
     lay.in_dtype = l->dtype;
     lay.cols = static_cast<int32_t>(l->width);
@@ -527,6 +551,7 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
         lay.in = l->hidden;
         lay.in_stride = l->hidden_stride;
         lay.rows = static_cast<int32_t>(l->rows);
+        lay.live = live;
         lay.row_factor = b.ratio;
         lay.out = b.x16;
         lay.out_stride = b.pad_rows;
@@ -535,6 +560,7 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
         lay.unscale = b.unscale_x16;
         JABAS_TRY(launch_lay_columns(lay, stream));
     }
+    lay.live = Live{};
     lay.row_factor = nullptr;
     lay.in_stride = l->weight_stride;
     lay.out = b.w16;
@@ -553,6 +579,8 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     g.w.out_dtype = g.h.out_dtype = l->dtype;
     g.w.part_stride = g.h.part_stride = b.part_stride;
     g.w.splits = g.h.splits = 1;
+    g.w.rows = g.h.rows = live;
+    g.w.live_depth = g.h.live_n = 1;
     for (int64_t first = 0; first < l->vocab; first += b.piece) {
         const int64_t n = l->vocab - first < b.piece ? l->vocab - first : b.piece;
         const int32_t pad = static_cast<int32_t>(round_up(n, kDepth));
@@ -560,7 +588,7 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
         a.first = static_cast<int32_t>(first);
         a.pad_tokens = pad;
         JABAS_TRY(launch_logits_backward(a, s.planes, b.large, stream));
-        if (d_bias) JABAS_TRY(launch_bias_sum(b.db, row_tiles, n, n, static_cast<char*>(d_bias) + first * bytes, l->dtype, stream));
+        if (d_bias) JABAS_TRY(launch_bias_sum(b.db, b.live, logits_tile(b.large), n, n, static_cast<char*>(d_bias) + first * bytes, l->dtype, stream));
         if (!d_weight && !d_hidden) continue;
         if (d_weight) {     // sum over the rows of dz[row][token] x[row][feature]
             g.w.a = Operand{b.x16, b.pad_rows, l->width * b.pad_rows, width};

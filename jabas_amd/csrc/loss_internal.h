@@ -41,6 +41,12 @@ struct Operand {
     int32_t rows;
 };
 
+// The rows that count, in order: row c of the products is row map[c] of the call, c < *live. Rows that do not count cost nothing but this.
+struct Live {
+    const int32_t* map;
+    const int32_t* live;
+};
+
 // Entries of a row: the labels (entry_index NULL) or the teacher's.
 struct Entries {
     const int64_t* target;
@@ -51,7 +57,8 @@ struct Entries {
 };
 
 struct LogitsArgs {
-    Operand w, x;               // M = tokens of the piece, N = rows
+    Operand w, x;               // M = tokens of the piece, N = rows that count (at most x.rows of them)
+    Live rows;
     int32_t depth;              // padded width
     const float* unscale_w;     // factors that undo the scaling of the operands' rows, or NULL
     const float* unscale_x;
@@ -61,18 +68,18 @@ struct LogitsArgs {
     float c;                    // log2(e) / T
     Entries entries;
     // forward
-    float2* partial;            // [tile of the vocabulary][row]: maximum of the raw logits, sum of 2^((z - max) c)
-    float* total;               // [tile][row]: sum of the logits (label smoothing), or NULL
-    float* entry_logit;         // [row][max(k, 1)]
+    float2* partial;            // [tile of the vocabulary][row that counts]: maximum of the raw logits, sum of 2^((z - max) c)
+    float* total;               // [tile][row that counts]: sum of the logits (label smoothing), or NULL
+    float* entry_logit;         // [row of the call][max(k, 1)]
     // backward
     const RowState* state;
     const float* row_grad;      // gradient of row n in units of dz (bias gradient)
     float uniform;              // e / V
     float hit;                  // what a label takes off: 1 - e
-    void* dz;                   // [row][token of the piece], fp16 planes, or NULL
+    void* dz;                   // [row that counts][token of the piece], fp16 planes, or NULL
     int64_t dz_stride, dz_plane;
     float* db;                  // [tile of the rows][token of the piece], or NULL
-    int32_t pad_rows, pad_tokens;   // dz is written (with zeros) up to these
+    int32_t pad_tokens;         // dz is written (with zeros) up to this, and to whole steps of rows
 };
 
 // out[n][m] = scale * row_scale[n] * sum_k a[m][k] b[n][k] (rows_of_k: b[k][n]), the inner axis in `splits` ranges of `each`
@@ -80,9 +87,12 @@ struct LogitsArgs {
 struct Job {
     Operand a, b;
     int32_t m, n, depth, splits, each;
+    Live rows;
+    int32_t live_depth;         // the inner axis is the rows that count: `depth` is what they are at most
+    int32_t live_n;             // n is
     const float* unscale0;      // device scalars, or NULL
     const float* unscale1;
-    const float* row_scale;     // per n, or NULL
+    const float* row_scale;     // per row of the call, or NULL
     float scale;
     float* part;                // fp32 sums [split][n][part_stride] over the pieces of the inner axis, or NULL: written to `out` at once
     int64_t part_stride, part_plane;        // a multiple of 4; splits apart
@@ -116,6 +126,7 @@ struct LayArgs {
     int64_t in_stride;
     int32_t in_dtype;
     int32_t rows, cols;         // of `in`
+    Live live;                  // the rows of `in` that are laid out, or all of them
     const float* row_factor;    // per row of `in`, or NULL: rows with factor 0 are zeros whatever they hold, others are multiplied
     const void* row_mask;       // per row of `in`, in_dtype, or NULL: rows with -inf here (tokens that the bias rules out) are zeros
     void* out;                  // launch_lay_rows: [rows][pad]; launch_lay_columns: [cols][pad]
@@ -144,6 +155,7 @@ struct TeacherArgs {
 int launch_teacher(const TeacherArgs& a, hipStream_t stream);
 
 struct JoinArgs {
+    Live live;                  // of launch_join
     const float2* partial;
     const float* total;
     const float* entry_logit;
@@ -162,11 +174,35 @@ int launch_join(const JoinArgs& a, hipStream_t stream);
 // loss_out and reduce[0] = 1 / rows that count (mean) or 1
 int launch_reduce(const float* row_loss, const RowState* state, int64_t rows, int reduction, float* loss_out, float* reduce, hipStream_t stream);
 
-// grad[n] = upstream * T * reduce[0] (0 for rows that do not count), ratio[n] = grad[n] / *peak, *peak the largest |grad|
-int launch_row_grad(const float* upstream, int per_row, const float* reduce, float t, const RowState* state, int64_t rows,
-                    float* grad, float* ratio, float* peak, hipStream_t stream);
+// Which rows count: map and *live; the others' state and loss become zeros.
+struct LiveArgs {
+    const int64_t* target;
+    int64_t ignore_index;
+    const float4* teacher_row;  // instead of labels
+    int64_t rows;
+    int32_t *map, *live;
+    RowState* state;
+    float* row_loss;
+};
+int launch_live(const LiveArgs& a, hipStream_t stream);
 
-int launch_bias_sum(const float* parts, int32_t tiles, int64_t stride, int64_t n, void* out, int32_t dtype, hipStream_t stream);
+// grad[n] = upstream * T * reduce[0] (0 for rows that do not count), ratio[n] = grad[n] / *peak, *peak the largest |grad|, and which rows
+// count, from their states; d_hidden's rows that do not are zeroed.
+struct RowGradArgs {
+    const float* upstream;
+    int32_t per_row;
+    const float* reduce;
+    float t;
+    const RowState* state;
+    int64_t rows;
+    float *grad, *ratio, *peak;
+    int32_t *map, *live;
+};
+int launch_row_grad(const RowGradArgs& a, hipStream_t stream);
+int launch_zero_rows(const RowState* state, int64_t rows, int64_t width, int32_t dtype, void* d_hidden, hipStream_t stream);
+
+// out[i] = sum of parts[t][i] over the tiles of `tile` rows that count
+int launch_bias_sum(const float* parts, const int32_t* live, int32_t tile, int64_t stride, int64_t n, void* out, int32_t dtype, hipStream_t stream);
 int launch_zero(void* p, size_t bytes, hipStream_t stream);
 
 // Few rows, hidden states and weight as they lie (loss_narrow.hip).

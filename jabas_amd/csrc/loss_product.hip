@@ -35,16 +35,22 @@ __device__ inline void tile_of(int block, int tm, int tn, int& m, int& n) {
 // Which tokens of the tile are entries of which row: the byte of token m and row n, in the word [m / 4][n], is 1 + the entry's
 // number. Built over the operands' buffers, which nobody reads any more.
 template <class C>
-__device__ inline void build_map(const Entries& en, char* map, int first, int n0, int rows) {
+__device__ inline void build_map(const Entries& en, const int32_t* live, char* map, int first, int n0, int rows) {
     const int t = threadIdx.x, lane = t & 63;
     for (int i = t; i < C::kM * C::kN / 16; i += C::kThreads) reinterpret_cast<u32x4*>(map)[i] = u32x4{0, 0, 0, 0};
     __syncthreads();
-    const int here = min(C::kN, rows - n0);
-    for (int n = t >> 6; n < here; n += C::kThreads / 64)
+    constexpr int kWaves = C::kThreads / 64;
+    static_assert(C::kN / kWaves <= 64, "a lane for each row of a wave");
+    const int here = min(C::kN, rows - n0), wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int32_t mine = wave + kWaves * lane < here ? live[n0 + wave + kWaves * lane] : 0;
+#pragma unroll 4
+    for (int n = wave; n < here; n += kWaves) {
+        const int32_t* index = en.index + static_cast<int64_t>(__builtin_amdgcn_readlane(mine, n / kWaves)) * en.k;
         for (int j = lane; j < en.k; j += 64) {
-            const int v = en.index[static_cast<int64_t>(n0 + n) * en.k + j] - first;
+            const int v = index[j] - first;
             if (v >= 0 && v < C::kM) map[((v >> 2) * C::kN + n) * 4 + (v & 3)] = static_cast<char>(1 + j);
         }
+    }
     __syncthreads();
 }
 
@@ -73,15 +79,17 @@ template <class C>
 struct Tile {
     float v[C::kI][C::kJ][16];
 };
-template <int P, class C>
-__device__ inline void logits_of(const LogitsArgs& a, int m0, int n0, char* smem, float* tokens, Tile<C>& z) {
+template <int P, class C, class Prepare>
+__device__ inline void logits_of(const LogitsArgs& a, int rows, int m0, int n0, char* smem, float* tokens, Tile<C>& z, const Prepare& prepare) {
     const int wm = C::wave_m();
+    Operand x = a.x;
+    x.rows = rows;
     C c;
-    c.run(a.w, a.x, m0, n0, a.depth, smem, [&] { load_tokens<P, C>(a, m0, tokens); },
+    c.run(a.w, x, m0, n0, a.depth, smem, [&] { load_tokens<P, C>(a, m0, tokens); prepare(); },
           [&](int i, int e) { return P == 1 ? tokens[wm + C::block_m(i, e)] : 0.0f; });
 #pragma unroll
     for (int j = 0; j < C::kJ; ++j) {
-        const float ux = P == 2 ? a.unscale_x[min(n0 + C::wave_n() + j * 32 + static_cast<int>(threadIdx.x & 31), a.x.rows - 1)] : 1.0f;
+        const float ux = P == 2 ? a.unscale_x[min(n0 + C::wave_n() + j * 32 + static_cast<int>(threadIdx.x & 31), rows - 1)] : 1.0f;
 #pragma unroll
         for (int i = 0; i < C::kI; ++i) {
             if (P == 2) keep_order();
@@ -95,10 +103,10 @@ __device__ inline void logits_of(const LogitsArgs& a, int m0, int n0, char* smem
     }
 }
 
-// The label of row n as a token of the tile, or -1.
+// The label of row n of the call (-1: none) as a token of the tile, or -1.
 template <class C>
 __device__ inline int label_of(const LogitsArgs& a, int m0, int n) {
-    if (n >= a.x.rows) return -1;
+    if (n < 0) return -1;
     const int64_t label = a.entries.target[n] - a.first - m0;
     return label >= 0 && label < C::kM ? static_cast<int>(label) : -1;
 }
@@ -121,12 +129,22 @@ template <class E, int P, class C, bool TEACHER>
 __global__ __launch_bounds__(C::kThreads) void logits_forward_kernel(LogitsArgs a) {
     __shared__ __align__(16) char smem[2 * C::kStage];
     __shared__ float tokens[P * C::kM];
+    const int rows = *a.rows.live, across = tiles_m<C>(a.w.rows);
+    if (static_cast<int>(blockIdx.x) >= across * tiles_n<C>(rows)) return;
     int tm, tn;
-    tile_of(blockIdx.x, tiles_m<C>(a.w.rows), tiles_n<C>(a.x.rows), tm, tn);
+    tile_of(blockIdx.x, across, tiles_n<C>(rows), tm, tn);
     const int m0 = tm * C::kM, n0 = tn * C::kN, lane = threadIdx.x & 63;
-    Tile<C> z;
-    logits_of<P>(a, m0, n0, smem, tokens, z);
     const int wm = C::wave_m(), wn = C::wave_n();
+    int row[C::kJ], label[C::kJ];       // rows of the call and their labels, asked for while the first operands are on their way
+    Tile<C> z;
+    logits_of<P>(a, rows, m0, n0, smem, tokens, z, [&] {
+#pragma unroll
+        for (int j = 0; j < C::kJ; ++j) {
+            const int n = n0 + wn + j * 32 + (lane & 31);
+            row[j] = n < rows ? a.rows.map[n] : -1;
+            label[j] = TEACHER ? -1 : label_of<C>(a, m0, row[j]);
+        }
+    });
     float peak[C::kJ], sum[C::kJ], total[C::kJ];
     if (m0 + C::kM > a.w.rows) {        // tokens past the end
 #pragma unroll
@@ -139,10 +157,10 @@ __global__ __launch_bounds__(C::kThreads) void logits_forward_kernel(LogitsArgs 
                     if (!in) z.v[i][j][e] = -INFINITY;
             }
     }
-    if (TEACHER) build_map<C>(a.entries, smem, a.first + m0, n0, a.x.rows);
+    if (TEACHER) build_map<C>(a.entries, a.rows.map, smem, a.first + m0, n0, rows);
 #pragma unroll
     for (int j = 0; j < C::kJ; ++j) {
-        const int nl = wn + j * 32 + (lane & 31), n = n0 + nl;
+        const int nl = wn + j * 32 + (lane & 31), n = row[j];
         total[j] = 0.0f;
         if (TEACHER) {          // entries join their row later, each by itself
 #pragma unroll
@@ -161,7 +179,7 @@ __global__ __launch_bounds__(C::kThreads) void logits_forward_kernel(LogitsArgs 
                         }
                 }
         } else {
-            at_label<C>(label_of<C>(a, m0, n), [&](int i, int e) { a.entry_logit[n] = z.v[i][j][e]; });
+            at_label<C>(label[j], [&](int i, int e) { a.entry_logit[n] = z.v[i][j][e]; });
             if (a.total) {
 #pragma unroll
                 for (int i = 0; i < C::kI; ++i)
@@ -198,7 +216,7 @@ __global__ __launch_bounds__(C::kThreads) void logits_forward_kernel(LogitsArgs 
         }
     __syncthreads();
     const int nl = threadIdx.x, n = n0 + nl;
-    if (nl >= C::kN || n >= a.x.rows) return;
+    if (nl >= C::kN || n >= rows) return;
     float p = merge[nl], s = 0.0f, t = 0.0f;
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) p = fmaxf(p, merge[w * C::kN + nl]);
@@ -230,19 +248,29 @@ template <class E, int P, class C, bool TEACHER>
 __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs a) {
     __shared__ __align__(16) char smem[2 * C::kStage];
     __shared__ float tokens[P * C::kM];
+    const int rows = *a.rows.live, across = tiles_m<C>(a.w.rows);
+    if (static_cast<int>(blockIdx.x) >= across * tiles_n<C>(rows)) return;
     int tm, tn;
-    tile_of(blockIdx.x, tiles_m<C>(a.w.rows), tiles_n<C>(a.x.rows), tm, tn);
+    tile_of(blockIdx.x, across, tiles_n<C>(rows), tm, tn);
     const int m0 = tm * C::kM, n0 = tn * C::kN, lane = threadIdx.x & 63;
-    Tile<C> z;
-    logits_of<P>(a, m0, n0, smem, tokens, z);
     const int wm = C::wave_m(), wn = C::wave_n();
-    if (TEACHER) build_map<C>(a.entries, smem, a.first + m0, n0, a.x.rows);
+    int row[C::kJ], label[C::kJ];       // as in the forward pass
+    Tile<C> z;
+    logits_of<P>(a, rows, m0, n0, smem, tokens, z, [&] {
+#pragma unroll
+        for (int j = 0; j < C::kJ; ++j) {
+            const int n = n0 + wn + j * 32 + (lane & 31);
+            row[j] = n < rows ? a.rows.map[n] : -1;
+            label[j] = TEACHER ? -1 : label_of<C>(a, m0, row[j]);
+        }
+    });
+    if (TEACHER) build_map<C>(a.entries, a.rows.map, smem, a.first + m0, n0, rows);
     const float uniform = a.uniform * kDzScale;
 #pragma unroll
     for (int j = 0; j < C::kJ; ++j) {
         keep_order();
-        const int nl = wn + j * 32 + (lane & 31), n = n0 + nl;
-        const RowState st = n < a.x.rows ? a.state[n] : RowState{0.0f, 0.0f, 0.0f, 0.0f};
+        const int nl = wn + j * 32 + (lane & 31), n = row[j];
+        const RowState st = n >= 0 ? a.state[n] : RowState{0.0f, 0.0f, 0.0f, 0.0f};
         const bool counts = !(st.slope == 0.0f && st.mass == 0.0f);
         const float slope = st.slope * kDzScale;
 #pragma unroll
@@ -269,7 +297,7 @@ __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs
                 }
             }
         }
-        if (!TEACHER) at_label<C>(label_of<C>(a, m0, n), [&](int i, int e) { z.v[i][j][e] -= a.hit * kDzScale; });
+        if (!TEACHER) at_label<C>(label[j], [&](int i, int e) { z.v[i][j][e] -= a.hit * kDzScale; });
         if (__any(!counts)) {
 #pragma unroll
             for (int i = 0; i < C::kI; ++i)
@@ -294,8 +322,7 @@ __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs
         float g[C::kJ];
 #pragma unroll
         for (int j = 0; j < C::kJ; ++j) {
-            const int n = n0 + wn + j * 32 + (lane & 31);
-            g[j] = n < a.x.rows ? a.row_grad[n] * (1.0f / kDzScale) : 0.0f;
+            g[j] = row[j] >= 0 ? a.row_grad[row[j]] * (1.0f / kDzScale) : 0.0f;
         }
 #pragma unroll
         for (int i = 0; i < C::kI; i += 2) {
@@ -319,6 +346,7 @@ __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs
         }
     }
     if (!a.dz) return;
+    const int pad_rows = (rows + kDepth - 1) / kDepth * kDepth;
     __syncthreads();
     // The wave's part of dz through LDS, so that lanes write 16 consecutive bytes of a row: row n of kChunks chunks, chunk k at k ^ n % kChunks.
     constexpr int kRows = C::kJ * 32, kChunks = C::kI * 32 / 8;
@@ -363,7 +391,7 @@ __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs
             const int f = x * 64 + lane, r = f / kChunks, k = f % kChunks;
             const u32x4 v = *reinterpret_cast<const u32x4*>(mine + (r * kChunks + (k ^ (r % kChunks))) * 16);
             const int n = n0 + wn + r, m = m0 + wm + k * 8;
-            if (n < a.pad_rows && m < a.pad_tokens) *reinterpret_cast<u32x4*>(out + static_cast<int64_t>(n) * a.dz_stride + m) = v;
+            if (n < pad_rows && m < a.pad_tokens) *reinterpret_cast<u32x4*>(out + static_cast<int64_t>(n) * a.dz_stride + m) = v;
         }
     }
 }
@@ -371,6 +399,7 @@ __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs
 // Results of four consecutive m of a row.
 __device__ inline void put_four(const Job& a, int n, int m, f32x4 v) {
     const int here = min(4, a.m - m);
+    if (a.live_n) n = a.rows.map[n];
     if (a.row_scale) {      // a row that does not count is zero even where its neighbours' scale is not finite
         const float rs = a.row_scale[n];
         v = rs == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v * rs;
@@ -390,18 +419,31 @@ __device__ inline void put_four(const Job& a, int n, int m, f32x4 v) {
     }
 }
 
+__device__ inline int live_or(const Job& a, int32_t is_live, int otherwise) { return is_live ? *a.rows.live : otherwise; }
+
 template <class C>
 __device__ inline void run_job(const Job& a, int unit, char* smem) {
-    const int tiles = tiles_m<C>(a.m) * tiles_n<C>(a.n), split = unit / tiles;
+    const int n_here = live_or(a, a.live_n, a.n), depth = (live_or(a, a.live_depth, a.depth) + kDepth - 1) / kDepth * kDepth;
+    const int tiles = tiles_m<C>(a.m) * tiles_n<C>(n_here), split = unit / tiles;
     int tm, tn;
-    tile_of(unit - split * tiles, tiles_m<C>(a.m), tiles_n<C>(a.n), tm, tn);
+    tile_of(unit - split * tiles, tiles_m<C>(a.m), tiles_n<C>(n_here), tm, tn);
     const int m0 = tm * C::kM, n0 = tn * C::kN, lane = threadIdx.x & 63;
     Operand x = a.a, y = a.b;
     const int k0 = split * a.each;
     x.p = static_cast<const uint16_t*>(x.p) + k0;
     y.p = static_cast<const uint16_t*>(y.p) + (C::kTb ? k0 * y.stride : k0);
+    if (a.live_n) y.rows = n_here;
     C c;
-    c.run(x, y, m0, n0, min(a.each, a.depth - k0), smem, [] {}, [](int, int) { return 0.0f; });
+    if (k0 < depth) {
+        c.run(x, y, m0, n0, min(a.each, depth - k0), smem, [] {}, [](int, int) { return 0.0f; });
+    } else {        // fewer rows count than the splits were made for
+#pragma unroll
+        for (int i = 0; i < C::kI; ++i)
+#pragma unroll
+            for (int j = 0; j < C::kJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) c.acc[i][j][e] = 0.0f;
+    }
     const int wm = C::wave_m(), wn = C::wave_n();
     float scale = a.scale;
     if (a.unscale0) scale *= *a.unscale0;
@@ -428,7 +470,7 @@ __device__ inline void run_job(const Job& a, int unit, char* smem) {
             const int f = x * 64 + lane, r = f / kChunks, k = f % kChunks;
             f32x4 v = *reinterpret_cast<const f32x4*>(mine + (r * kChunks + (k ^ (r % kChunks))) * 4);
             const int n = n0 + wn + j * 32 + r, m = m0 + wm + k * 4;
-            if (n >= a.n || m >= a.m) continue;
+            if (n >= n_here || m >= a.m) continue;
             if (part) {
                 float* sum = part + static_cast<int64_t>(n) * a.part_stride + m;       // rows padded to four
                 if (!a.first) v += *reinterpret_cast<const f32x4*>(sum);
@@ -446,8 +488,10 @@ template <class CW, class CH>
 __global__ __launch_bounds__(CW::kThreads) void grads_kernel(GradArgs a) {
     static_assert(CW::kStage == CH::kStage && CW::kThreads == CH::kThreads, "one launch shape");
     __shared__ __align__(16) char smem[2 * CW::kStage];
-    const int units_w = tiles_m<CW>(a.w.m) * tiles_n<CW>(a.w.n) * a.w.splits, units_h = tiles_m<CH>(a.h.m) * tiles_n<CH>(a.h.n) * a.h.splits;
+    const int units_w = tiles_m<CW>(a.w.m) * tiles_n<CW>(a.w.n) * a.w.splits;
+    const int units_h = tiles_m<CH>(a.h.m) * tiles_n<CH>(live_or(a.h, a.h.live_n, a.h.n)) * a.h.splits;
     const int block = blockIdx.x, lead = a.h_first ? units_h : units_w;
+    if (block >= units_w + units_h) return;
     if ((block < lead) == (a.h_first != 0)) run_job<CH>(a.h, a.h_first ? block : block - lead, smem);
     else run_job<CW>(a.w, a.h_first ? block - lead : block, smem);
 }
@@ -455,7 +499,7 @@ __global__ __launch_bounds__(CW::kThreads) void grads_kernel(GradArgs a) {
 __global__ __launch_bounds__(256) void join_splits_kernel(Job a) {
     const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     const int quads = (a.m + 3) / 4, n = static_cast<int>(at / quads), m = static_cast<int>(at % quads) * 4;
-    if (n >= a.n) return;
+    if (n >= live_or(a, a.live_n, a.n)) return;
     const float* part = a.part + n * a.part_stride + m;
     f32x4 v = *reinterpret_cast<const f32x4*>(part);
     for (int i = 1; i < a.splits; ++i) v += *reinterpret_cast<const f32x4*>(part + i * a.part_plane);
@@ -652,13 +696,18 @@ __device__ inline float row_keeps(const LayArgs& a, int row) {
     return a.row_factor ? a.row_factor[row] : 1.0f;
 }
 
+// Row r that is laid out: rows and places.
+__device__ inline int rows_of(const LayArgs& a) { return a.live.live ? *a.live.live : a.rows; }
+__device__ inline int row_of(const LayArgs& a, int r) { return a.live.map ? a.live.map[r] : r; }
+
 // One wave per row: padded, and scaled by the row's own power of two.
 __global__ __launch_bounds__(kLayThreads) void lay_rows_kernel(LayArgs a) {
-    const int row = blockIdx.x * (kLayThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (row >= a.rows) return;
+    const int place = blockIdx.x * (kLayThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (place >= rows_of(a)) return;
+    const int row = row_of(a, place);
     if (a.planes == 0) {
         const uint16_t* in = static_cast<const uint16_t*>(a.in) + static_cast<int64_t>(row) * a.in_stride;
-        uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(row) * a.out_stride;
+        uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(place) * a.out_stride;
         for (int c = lane * 8; c < a.pad; c += 512) {
             Eight16 x;
             if (c + 8 <= a.cols) x = *reinterpret_cast<const Eight16*>(in + c);
@@ -683,16 +732,18 @@ __global__ __launch_bounds__(kLayThreads) void lay_rows_kernel(LayArgs a) {
         load_eight(a, row, c, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] *= scale;
-        store_eight(a, row, c, v);
+        store_eight(a, place, c, v);
     }
-    if (lane == 0) a.unscale[row] = power_of_two(-e);
+    if (lane == 0) a.unscale[place] = power_of_two(-e);
 }
 
 __global__ __launch_bounds__(kLayThreads) void absmax_kernel(LayArgs a) {
     __shared__ float merge[kLayThreads / 64];
     const int lane = threadIdx.x & 63;
     float peak = 0.0f, v[8];
-    for (int row = blockIdx.x * (kLayThreads / 64) + (threadIdx.x >> 6); row < a.rows; row += gridDim.x * (kLayThreads / 64)) {
+    const int rows = rows_of(a);
+    for (int place = blockIdx.x * (kLayThreads / 64) + (threadIdx.x >> 6); place < rows; place += gridDim.x * (kLayThreads / 64)) {
+        const int row = row_of(a, place);
         const float f = row_keeps(a, row);
         if (f == 0.0f) continue;
         for (int c = lane * 8; c < a.cols; c += 512) {
@@ -711,15 +762,17 @@ __global__ __launch_bounds__(kLayThreads) void absmax_kernel(LayArgs a) {
 __global__ __launch_bounds__(kLayThreads) void lay_columns_kernel(LayArgs a) {
     __shared__ float merge[kLayThreads / 64], tile[64][65];
     static_assert(kMaxParts % kLayThreads == 0, "as many partial maxima per thread");
-    const int t = threadIdx.x, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+    const int t = threadIdx.x, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, rows = rows_of(a), pad = (rows + 63) / 64 * 64;
+    if (r0 >= pad && r0) return;        // the first writes the scale, whatever there is to lay out
     float peak = 0.0f, v[8];
 #pragma unroll
     for (int i = 0; i < kMaxParts; i += kLayThreads) peak = fmaxf(peak, a.parts[i + t]);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int r = x * 32 + (t >> 3), c = (t & 7) * 8;
-        const float f = r0 + r < a.rows ? row_keeps(a, r0 + r) : 0.0f;
-        if (f != 0.0f) load_eight(a, r0 + r, c0 + c, v);
+        const int row = r0 + r < rows ? row_of(a, r0 + r) : 0;
+        const float f = r0 + r < rows ? row_keeps(a, row) : 0.0f;
+        if (f != 0.0f) load_eight(a, row, c0 + c, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) tile[r][c + i] = f != 0.0f ? v[i] * f : 0.0f;
     }
@@ -733,7 +786,7 @@ __global__ __launch_bounds__(kLayThreads) void lay_columns_kernel(LayArgs a) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int c = x * 32 + (t >> 3), r = (t & 7) * 8;
-        if (c0 + c >= a.cols || r0 + r >= a.pad) continue;
+        if (c0 + c >= a.cols || r0 + r >= pad) continue;
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = tile[r + i][c] * scale;
         store_eight(a, c0 + c, r0 + r, v);

@@ -233,9 +233,10 @@ constexpr int kJoinThreads = 1024, kJoinRows = 64, kJoinWaves = kJoinThreads / 6
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(JoinArgs a) {
     __shared__ float peaks[kJoinWaves][kJoinRows], sums[kJoinWaves][kJoinRows], totals[kJoinWaves][kJoinRows];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kJoinRows, mine = first + lane;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kJoinRows, mine = first + lane, rows = *a.live.live;
+    if (first >= rows) return;
     float peak = -INFINITY, sum = 0.0f, total = 0.0f;
-    if (mine < a.rows)
+    if (mine < rows)
         for (int i = wave; i < a.tiles; i += kJoinWaves) {
             const float2 part = a.partial[static_cast<int64_t>(i) * a.rows + mine];
             const float p = fmaxf(peak, part.x);
@@ -260,14 +261,15 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(JoinArgs a) {
     }
     __syncthreads();
     if (!a.entries.index) {
-        if (wave != 0 || mine >= a.rows) return;
-        const RowResult r = label_result(a, mine, peak, sum, total);
-        a.state[mine] = r.state;
-        a.row_loss[mine] = r.loss;
+        if (wave != 0 || mine >= rows) return;
+        const int32_t row = a.live.map[mine];
+        const RowResult r = label_result(a, row, peak, sum, total);
+        a.state[row] = r.state;
+        a.row_loss[row] = r.loss;
         return;
     }
-    for (int r = wave; r < kJoinRows && first + r < a.rows; r += kJoinWaves) {
-        const int64_t row = first + r;
+    for (int r = wave; r < kJoinRows && first + r < rows; r += kJoinWaves) {
+        const int64_t row = a.live.map[first + r];
         const RowResult result = entries_result(a, row, peaks[0][r], sums[0][r]);
         if (lane == 0) {
             a.state[row] = result.state;
@@ -369,17 +371,65 @@ __device__ inline float row_gradient(const float* upstream, int per_row, const f
     return counts(st) ? upstream[per_row ? row : 0] * (*reduce * t) : 0.0f;
 }
 
-__global__ __launch_bounds__(kJoinThreads) void row_grad_kernel(const float* upstream, int per_row, const float* reduce, float t, const RowState* state,
-                                                                int64_t rows, float* grad, float* ratio, float* peak) {
+// The rows for which is(n), in order, by one workgroup: a run of kRun rows a thread at a time.
+constexpr int kRun = 8;
+template <class F>
+__device__ inline void list_live(int64_t rows, int32_t* map, int32_t* live, const F& is) {
+    __shared__ int32_t counts_of[kJoinWaves];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    int32_t before = 0;
+    for (int64_t first = 0; first < rows; first += kJoinThreads * kRun) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) {
+            const int64_t n = first + t * kRun + i;
+            if (n < rows && is(n)) bits |= 1u << i;
+        }
+        const int32_t mine = __popc(bits);
+        int32_t upto = mine;        // of the wave's lanes up to this one
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) {
+            const int32_t other = __shfl_up(upto, x);
+            if (lane >= x) upto += other;
+        }
+        if (lane == 63) counts_of[wave] = upto;
+        __syncthreads();
+        int32_t at = before + upto - mine;
+        for (int i = 0; i < kJoinWaves; ++i) {
+            if (i < wave) at += counts_of[i];
+            before += counts_of[i];
+        }
+#pragma unroll
+        for (int i = 0; i < kRun; ++i)
+            if ((bits >> i) & 1) map[at++] = static_cast<int32_t>(first + t * kRun + i);
+        __syncthreads();
+    }
+    if (t == 0) *live = before;
+}
+
+__global__ __launch_bounds__(kJoinThreads) void live_kernel(LiveArgs a) {
+    list_live(a.rows, a.map, a.live, [&](int64_t n) {
+        const bool is = a.teacher_row ? a.teacher_row[n].z != 0.0f : a.target[n] != a.ignore_index;
+        if (!is) {
+            a.state[n] = RowState{0.0f, 0.0f, 0.0f, 0.0f};
+            a.row_loss[n] = 0.0f;
+        }
+        return is;
+    });
+}
+
+__global__ __launch_bounds__(kJoinThreads) void row_grad_kernel(RowGradArgs a) {
     __shared__ float peaks[kJoinWaves];
     float top = 0.0f;
     bool bad = false;
-    for (int64_t i = threadIdx.x; i < rows; i += kJoinThreads) {
-        const float g = row_gradient(upstream, per_row, reduce, t, state[i], i);
-        grad[i] = g;
+    list_live(a.rows, a.map, a.live, [&](int64_t n) {
+        const RowState st = a.state[n];
+        const float g = row_gradient(a.upstream, a.per_row, a.reduce, a.t, st, n);
+        a.grad[n] = g;
         bad |= !(fabsf(g) < INFINITY);
         top = fmaxf(top, fabsf(g));
-    }
+        return counts(st);
+    });
     top = wave_max(top);
     if (__any(bad)) top = INFINITY;
     if ((threadIdx.x & 63) == 0) peaks[threadIdx.x >> 6] = top;
@@ -387,16 +437,25 @@ __global__ __launch_bounds__(kJoinThreads) void row_grad_kernel(const float* ups
     for (int i = 0; i < kJoinWaves; ++i) top = fmaxf(top, peaks[i]);
     // rows of a gradient that is not finite make everything that sums over rows NaN: the ratio says 1 for all that count
     const bool whole = top < INFINITY;
-    if (threadIdx.x == 0) *peak = whole ? top : NAN;
-    for (int64_t i = threadIdx.x; i < rows; i += kJoinThreads) {
-        const float g = row_gradient(upstream, per_row, reduce, t, state[i], i);
-        ratio[i] = g == 0.0f ? 0.0f : whole ? g / top : 1.0f;
+    if (threadIdx.x == 0) *a.peak = whole ? top : NAN;
+    for (int64_t i = threadIdx.x; i < a.rows; i += kJoinThreads) {
+        const float g = a.grad[i];
+        a.ratio[i] = g == 0.0f ? 0.0f : whole ? g / top : 1.0f;
     }
 }
 
-__global__ __launch_bounds__(kThreads) void bias_sum_kernel(const float* parts, int32_t tiles, int64_t stride, int64_t n, void* out, int32_t dtype) {
+// A wave per row.
+__global__ __launch_bounds__(kThreads) void zero_rows_kernel(const RowState* state, int64_t rows, int64_t bytes, char* out) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
+    if (row >= rows || counts(state[row])) return;
+    uint16_t* p = reinterpret_cast<uint16_t*>(out + row * bytes);
+    for (int64_t i = threadIdx.x & 63; i < bytes / 2; i += 64) p[i] = 0;
+}
+
+__global__ __launch_bounds__(kThreads) void bias_sum_kernel(const float* parts, const int32_t* live, int32_t tile, int64_t stride, int64_t n, void* out, int32_t dtype) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
     if (i >= n) return;
+    const int32_t tiles = (*live + tile - 1) / tile;
     float sum = 0.0f;
     for (int t = 0; t < tiles; ++t) sum += parts[t * stride + i];
     if (dtype == JABAS_F32) static_cast<float*>(out)[i] = sum;
@@ -666,12 +725,14 @@ int launch_narrow_join(const NarrowJoinArgs& a, hipStream_t stream) {
 int launch_reduce(const float* row_loss, const RowState* state, int64_t rows, int reduction, float* loss_out, float* reduce, hipStream_t stream) {
     return launch(reduce_kernel, 1, kJoinThreads, stream, row_loss, state, rows, reduction, loss_out, reduce);
 }
-int launch_row_grad(const float* upstream, int per_row, const float* reduce, float t, const RowState* state, int64_t rows,
-                    float* grad, float* ratio, float* peak, hipStream_t stream) {
-    return launch(row_grad_kernel, 1, kJoinThreads, stream, upstream, per_row, reduce, t, state, rows, grad, ratio, peak);
+int launch_live(const LiveArgs& a, hipStream_t stream) { return launch(live_kernel, 1, kJoinThreads, stream, a); }
+int launch_row_grad(const RowGradArgs& a, hipStream_t stream) { return launch(row_grad_kernel, 1, kJoinThreads, stream, a); }
+int launch_zero_rows(const RowState* state, int64_t rows, int64_t width, int32_t dtype, void* d_hidden, hipStream_t stream) {
+    return launch(zero_rows_kernel, static_cast<unsigned>((rows + kThreads / 64 - 1) / (kThreads / 64)), kThreads, stream, state, rows,
+                  width * (dtype == JABAS_F32 ? 4 : 2), static_cast<char*>(d_hidden));
 }
-int launch_bias_sum(const float* parts, int32_t tiles, int64_t stride, int64_t n, void* out, int32_t dtype, hipStream_t stream) {
-    return launch(bias_sum_kernel, static_cast<unsigned>((n + kThreads - 1) / kThreads), kThreads, stream, parts, tiles, stride, n, out, dtype);
+int launch_bias_sum(const float* parts, const int32_t* live, int32_t tile, int64_t stride, int64_t n, void* out, int32_t dtype, hipStream_t stream) {
+    return launch(bias_sum_kernel, static_cast<unsigned>((n + kThreads - 1) / kThreads), kThreads, stream, parts, live, tile, stride, n, out, dtype);
 }
 int launch_zero(void* p, size_t bytes, hipStream_t stream) {
     const size_t n = bytes / 2;
