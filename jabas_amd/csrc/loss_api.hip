@@ -154,6 +154,7 @@ size_t carve_forward(const JabasLoss* l, const Shape& s, char* base, Forward& f)
     if (s.linear) {
         f.map = c.take<int32_t>(rows);
         f.live = c.take<int32_t>(1);
+        f.ticket = c.take<uint32_t>(1);
     }
     if (s.linear) f.x = c.take<uint16_t>(rows * s.depth * s.planes);
     if (s.linear && s.copy_w) f.w = c.take<uint16_t>(f.piece * s.depth * s.planes);
@@ -260,11 +261,12 @@ const char* at(const void* p, int64_t elements, int dtype) {
         if (status_ != JABAS_OK) return status_; \
     } while (0)
 
-// The hidden states of the rows that count.
-int lay_x(const JabasLoss* l, const Shape& s, const Live& live, uint16_t* x, float* unscale, Operand& out, hipStream_t stream) {
+// The hidden states of the rows that count; the other rows of `zero` become zeros.
+int lay_x(const JabasLoss* l, const Shape& s, const Live& live, void* zero, uint16_t* x, float* unscale, Operand& out, hipStream_t stream) {
     out.rows = static_cast<int32_t>(l->rows);
     LayArgs a{};
     a.live = live;
+    a.zero = zero;
     a.in = l->hidden;
     a.in_stride = l->hidden_stride;
     a.in_dtype = l->dtype;
@@ -333,6 +335,7 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
     if (!workspace || misaligned(workspace, 256) || workspace_bytes < carve_forward(l, s, static_cast<char*>(workspace), f)) return JABAS_ERR_WORKSPACE;
     RowState* state = reinterpret_cast<RowState*>(l->row_state);
     float* reduce = l->row_state + 4 * l->rows;
+    if (s.linear && !s.narrow && l->reduction == JABAS_LOSS_NONE) f.row_loss = loss_out;
     if (!l->rows) return launch_reduce(f.row_loss, state, 0, l->reduction, loss_out, reduce, stream);
     const float inv_t = static_cast<float>(1.0 / l->temperature), c = static_cast<float>(kLog2e / l->temperature);
     const Entries entries = entries_of(l, s);
@@ -368,11 +371,12 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
         live.rows = l->rows;
         live.map = f.map;
         live.live = f.live;
+        live.ticket = f.ticket;
         live.state = state;
         live.row_loss = f.row_loss;
         JABAS_TRY(launch_live(live, stream));
         a.rows = Live{f.map, f.live};
-        JABAS_TRY(lay_x(l, s, a.rows, f.x, f.unscale_x, a.x, stream));
+        JABAS_TRY(lay_x(l, s, a.rows, nullptr, f.x, f.unscale_x, a.x, stream));
         a.depth = static_cast<int32_t>(s.depth);
         a.unscale_x = f.unscale_x;
         a.unscale_w = f.unscale_w;
@@ -421,9 +425,11 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
     j.teacher = t;
     j.state = state;
     j.row_loss = f.row_loss;
-    if (s.narrow) return launch_narrow_join(NarrowJoinArgs{j, f.ticket, l->reduction, loss_out, reduce}, stream);
-    JABAS_TRY(launch_join(j, stream));
-    return launch_reduce(f.row_loss, state, l->rows, l->reduction, loss_out, reduce, stream);
+    j.ticket = f.ticket;
+    j.reduction = l->reduction;
+    j.loss_out = loss_out;
+    j.reduce = reduce;
+    return s.narrow ? launch_narrow_join(j, stream) : launch_join(j, stream);
 }
 
 JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, void* d_hidden, void* d_weight, void* d_bias, void* d_logits,
@@ -522,11 +528,10 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     r.map = b.map;
     r.live = b.live;
     JABAS_TRY(launch_row_grad(r, stream));
-    if (d_hidden) JABAS_TRY(launch_zero_rows(state, l->rows, l->width, l->dtype, d_hidden, stream));
     const Live live = {b.map, b.live};
     LogitsArgs a{};
     a.rows = live;
-    JABAS_TRY(lay_x(l, s, live, b.x, b.unscale_x, a.x, stream));
+    JABAS_TRY(lay_x(l, s, live, d_hidden, b.x, b.unscale_x, a.x, stream));
     a.depth = static_cast<int32_t>(s.depth);
     a.unscale_x = b.unscale_x;
     a.unscale_w = b.unscale_w;

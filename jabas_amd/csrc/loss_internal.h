@@ -41,7 +41,8 @@ struct Operand {
     int32_t rows;
 };
 
-// The rows that count, in order: row c of the products is row map[c] of the call, c < *live. Rows that do not count cost nothing but this.
+// The rows that count, in order: row c of the products is row map[c] of the call, c < *live; map holds the others behind them. Rows that do
+// not count cost nothing but this.
 struct Live {
     const int32_t* map;
     const int32_t* live;
@@ -133,6 +134,7 @@ struct LayArgs {
     int64_t out_stride, out_plane;
     int32_t pad;                // a multiple of 64
     int32_t planes;             // 0: copied as they are; 1 or 2 planes of fp16
+    void* zero;                 // launch_lay_rows: [row of the call][cols] of in_dtype whose rows that do not count are zeroed, or NULL
     float* unscale;             // written: a factor per row (launch_lay_rows, planes > 0) or one for all (launch_lay_columns)
     float* parts;               // launch_lay_columns: kMaxParts partial maxima
 };
@@ -168,8 +170,14 @@ struct JoinArgs {
     TeacherArgs teacher;
     RowState* state;
     float* row_loss;
+    // launch_join: the last workgroup to finish reduces over the rows
+    uint32_t* ticket;
+    int32_t reduction;
+    float* loss_out;
+    float* reduce;
 };
 int launch_join(const JoinArgs& a, hipStream_t stream);
+int launch_narrow_join(const JoinArgs& a, hipStream_t stream);        // a workgroup per row; partial and total: [row][tile]
 
 // loss_out and reduce[0] = 1 / rows that count (mean) or 1
 int launch_reduce(const float* row_loss, const RowState* state, int64_t rows, int reduction, float* loss_out, float* reduce, hipStream_t stream);
@@ -181,13 +189,14 @@ struct LiveArgs {
     const float4* teacher_row;  // instead of labels
     int64_t rows;
     int32_t *map, *live;
+    uint32_t* ticket;           // set to 0
     RowState* state;
     float* row_loss;
 };
 int launch_live(const LiveArgs& a, hipStream_t stream);
 
 // grad[n] = upstream * T * reduce[0] (0 for rows that do not count), ratio[n] = grad[n] / *peak, *peak the largest |grad|, and which rows
-// count, from their states; d_hidden's rows that do not are zeroed.
+// count, from their states.
 struct RowGradArgs {
     const float* upstream;
     int32_t per_row;
@@ -199,7 +208,6 @@ struct RowGradArgs {
     int32_t *map, *live;
 };
 int launch_row_grad(const RowGradArgs& a, hipStream_t stream);
-int launch_zero_rows(const RowState* state, int64_t rows, int64_t width, int32_t dtype, void* d_hidden, hipStream_t stream);
 
 // out[i] = sum of parts[t][i] over the tiles of `tile` rows that count
 int launch_bias_sum(const float* parts, const int32_t* live, int32_t tile, int64_t stride, int64_t n, void* out, int32_t dtype, hipStream_t stream);
@@ -243,15 +251,6 @@ NarrowSplits narrow_splits(int64_t tokens, int64_t width);
 int launch_narrow_forward(const NarrowArgs& a, int dtype, hipStream_t stream);
 int launch_narrow_backward(const NarrowArgs& a, int dtype, hipStream_t stream);
 int launch_narrow_grads(const NarrowArgs& a, int dtype, hipStream_t stream);
-// A workgroup per row; the last to finish reduces over the rows.
-struct NarrowJoinArgs {
-    JoinArgs join;              // partial and total: [row][tile]
-    uint32_t* ticket;
-    int32_t reduction;
-    float* loss_out;
-    float* reduce;
-};
-int launch_narrow_join(const NarrowJoinArgs& a, hipStream_t stream);
 
 // Logits in hand. One split: a workgroup per row; else a workgroup per `chunk` tokens of a row.
 struct TopkArgs {

@@ -703,8 +703,15 @@ __device__ inline int row_of(const LayArgs& a, int r) { return a.live.map ? a.li
 // One wave per row: padded, and scaled by the row's own power of two.
 __global__ __launch_bounds__(kLayThreads) void lay_rows_kernel(LayArgs a) {
     const int place = blockIdx.x * (kLayThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (place >= rows_of(a)) return;
+    if (place >= a.rows) return;
     const int row = row_of(a, place);
+    if (place >= rows_of(a)) {
+        if (!a.zero) return;
+        const int64_t bytes = static_cast<int64_t>(a.cols) * (a.in_dtype == JABAS_F32 ? 4 : 2);
+        uint16_t* out = reinterpret_cast<uint16_t*>(static_cast<char*>(a.zero) + row * bytes);
+        for (int64_t i = lane; i < bytes / 2; i += 64) out[i] = 0;
+        return;
+    }
     if (a.planes == 0) {
         const uint16_t* in = static_cast<const uint16_t*>(a.in) + static_cast<int64_t>(row) * a.in_stride;
         uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(place) * a.out_stride;

@@ -228,13 +228,46 @@ __device__ inline RowResult label_result(const JoinArgs& a, int64_t row, float p
 
 constexpr int kJoinThreads = 1024, kJoinRows = 64, kJoinWaves = kJoinThreads / 64;
 
+__device__ inline bool counts(const RowState& st) { return !(st.slope == 0.0f && st.mass == 0.0f); }
+
+// The loss and the share of a row from every thread's sums, by a workgroup of kJoinThreads.
+__device__ inline void finish(double sum, double number, int reduction, float* loss_out, float* reduce) {
+    __shared__ double sums[kJoinWaves];
+    sum = wave_sum(sum);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int i = 1; i < kJoinWaves; ++i) sum += sums[i];
+    const double share = reduction == JABAS_LOSS_MEAN && number > 0.0 ? 1.0 / number : 1.0;
+    *reduce = static_cast<float>(share);
+    if (reduction != JABAS_LOSS_NONE) *loss_out = static_cast<float>(sum * share);
+}
+
+__global__ __launch_bounds__(kJoinThreads) void reduce_kernel(const float* row_loss, const RowState* state, int64_t rows, int reduction,
+                                                              float* loss_out, float* reduce) {
+    __shared__ double numbers[kJoinWaves];
+    double sum = 0.0, number = 0.0;
+    for (int64_t i = threadIdx.x; i < rows; i += kJoinThreads) {
+        const float loss = row_loss[i];
+        sum += loss;
+        number += counts(state[i]) ? 1.0 : 0.0;
+        if (reduction == JABAS_LOSS_NONE) loss_out[i] = loss;
+    }
+    number = wave_sum(number);
+    if ((threadIdx.x & 63) == 0) numbers[threadIdx.x >> 6] = number;
+    __syncthreads();
+    number = 0.0;
+    for (int i = 0; i < kJoinWaves; ++i) number += numbers[i];
+    finish(sum, number, reduction, loss_out, reduce);
+}
+
 // 64 rows per workgroup: each wave joins a sixteenth of the vocabulary's tiles with a row per lane, then the waves' results
 // are joined, and each wave takes the entries of its rows in turn.
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(JoinArgs a) {
     __shared__ float peaks[kJoinWaves][kJoinRows], sums[kJoinWaves][kJoinRows], totals[kJoinWaves][kJoinRows];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int64_t first = static_cast<int64_t>(blockIdx.x) * kJoinRows, mine = first + lane, rows = *a.live.live;
-    if (first >= rows) return;
+    if (first >= rows && first) return;
     float peak = -INFINITY, sum = 0.0f, total = 0.0f;
     if (mine < rows)
         for (int i = wave; i < a.tiles; i += kJoinWaves) {
@@ -260,56 +293,39 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(JoinArgs a) {
         totals[0][lane] = total;
     }
     __syncthreads();
-    if (!a.entries.index) {
-        if (wave != 0 || mine >= rows) return;
+    if (!a.entries.index && wave == 0 && mine < rows) {
         const int32_t row = a.live.map[mine];
         const RowResult r = label_result(a, row, peak, sum, total);
         a.state[row] = r.state;
-        a.row_loss[row] = r.loss;
-        return;
+        __hip_atomic_store(a.row_loss + row, r.loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    for (int r = wave; r < kJoinRows && first + r < rows; r += kJoinWaves) {
+    for (int r = wave; a.entries.index && r < kJoinRows && first + r < rows; r += kJoinWaves) {
         const int64_t row = a.live.map[first + r];
         const RowResult result = entries_result(a, row, peaks[0][r], sums[0][r]);
         if (lane == 0) {
             a.state[row] = result.state;
-            a.row_loss[row] = result.loss;
+            __hip_atomic_store(a.row_loss + row, result.loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
     }
-}
-
-__device__ inline bool counts(const RowState& st) { return !(st.slope == 0.0f && st.mass == 0.0f); }
-
-__global__ __launch_bounds__(kJoinThreads) void reduce_kernel(const float* row_loss, const RowState* state, int64_t rows, int reduction,
-                                                              float* loss_out, float* reduce) {
-    __shared__ double sums[kJoinWaves], numbers[kJoinWaves];
-    double sum = 0.0, number = 0.0;
-    for (int64_t i = threadIdx.x; i < rows; i += kJoinThreads) {
-        const float loss = row_loss[i];
-        sum += loss;
-        number += counts(state[i]) ? 1.0 : 0.0;
-        if (reduction == JABAS_LOSS_NONE) loss_out[i] = loss;
+    if (a.reduction == JABAS_LOSS_NONE) {       // row_loss is the result
+        if (first == 0 && threadIdx.x == 0) *a.reduce = 1.0f;
+        return;
     }
-    sum = wave_sum(sum);
-    number = wave_sum(number);
-    if ((threadIdx.x & 63) == 0) {
-        sums[threadIdx.x >> 6] = sum;
-        numbers[threadIdx.x >> 6] = number;
-    }
+    // The last workgroup to finish sums the rows' losses, in order. They were stored past the dies' own caches, so one thread's release is
+    // enough, and they are loaded past them.
+    __shared__ uint32_t done;
     __syncthreads();
-    if (threadIdx.x) return;
-    for (int i = 1; i < kJoinWaves; ++i) {
-        sum += sums[i];
-        number += numbers[i];
-    }
-    const double share = reduction == JABAS_LOSS_MEAN && number > 0.0 ? 1.0 / number : 1.0;
-    *reduce = static_cast<float>(share);
-    if (reduction != JABAS_LOSS_NONE) *loss_out = static_cast<float>(sum * share);
+    if (threadIdx.x == 0) done = __hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (done + 1 != (rows > kJoinRows ? static_cast<uint32_t>((rows + kJoinRows - 1) / kJoinRows) : 1)) return;
+    double loss = 0.0;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < a.rows; i += kJoinThreads) loss += __hip_atomic_load(a.row_loss + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    finish(loss, static_cast<double>(rows), a.reduction, a.loss_out, a.reduce);
 }
 
 // Few rows: a workgroup joins a row's tiles; the last one to finish sums the rows' losses, in order.
-__global__ __launch_bounds__(kThreads) void narrow_join_kernel(NarrowJoinArgs args) {
-    const JoinArgs& a = args.join;
+__global__ __launch_bounds__(kThreads) void narrow_join_kernel(JoinArgs a) {
     __shared__ float peaks[kThreads / 64], sums[kThreads / 64], totals[kThreads / 64];
     const int t = threadIdx.x, wave = t >> 6;
     const int64_t row = blockIdx.x;
@@ -347,8 +363,8 @@ __global__ __launch_bounds__(kThreads) void narrow_join_kernel(NarrowJoinArgs ar
         // what the last workgroup reads of the others: written through to the chip's memory, then the ticket
         __hip_atomic_store(a.row_loss + row, r.loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __hip_atomic_store(a.row_loss + a.rows + row, counts(r.state) ? 1.0f : 0.0f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (args.reduction == JABAS_LOSS_NONE) args.loss_out[row] = r.loss;
-        done = __hip_atomic_fetch_add(args.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        if (a.reduction == JABAS_LOSS_NONE) a.loss_out[row] = r.loss;
+        done = __hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
     }
     done = __builtin_amdgcn_readfirstlane(done);
     if (done + 1 != a.rows) return;
@@ -361,9 +377,9 @@ __global__ __launch_bounds__(kThreads) void narrow_join_kernel(NarrowJoinArgs ar
     loss = wave_sum(loss);
     number = wave_sum(number);
     if (lane) return;
-    const double share = args.reduction == JABAS_LOSS_MEAN && number > 0.0 ? 1.0 / number : 1.0;
-    *args.reduce = static_cast<float>(share);
-    if (args.reduction != JABAS_LOSS_NONE) *args.loss_out = static_cast<float>(loss * share);
+    const double share = a.reduction == JABAS_LOSS_MEAN && number > 0.0 ? 1.0 / number : 1.0;
+    *a.reduce = static_cast<float>(share);
+    if (a.reduction != JABAS_LOSS_NONE) *a.loss_out = static_cast<float>(loss * share);
 }
 
 // The gradient of a row's loss in units of dz; 0 where it does not count.
@@ -371,64 +387,73 @@ __device__ inline float row_gradient(const float* upstream, int per_row, const f
     return counts(st) ? upstream[per_row ? row : 0] * (*reduce * t) : 0.0f;
 }
 
-// The rows for which is(n), in order, by one workgroup: a run of kRun rows a thread at a time.
+// Lists the rows for which is(n, load(n)), in order, and from the end of the list on those for which not, by one workgroup: kRun rows a
+// thread at a time, whose loads are all under way before the first is looked at.
 constexpr int kRun = 8;
-template <class F>
-__device__ inline void list_live(int64_t rows, int32_t* map, int32_t* live, const F& is) {
-    __shared__ int32_t counts_of[kJoinWaves];
+template <class L, class F>
+__device__ inline void list_live(int64_t rows, int32_t* map, int32_t* live, const L& load, const F& is) {
+    __shared__ int32_t counts_of[kRun][kJoinWaves];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     int32_t before = 0;
     for (int64_t first = 0; first < rows; first += kJoinThreads * kRun) {
-        uint32_t bits = 0;
+        decltype(load(0)) held[kRun];
+        uint64_t bits[kRun];        // of the wave's 64 rows in run i
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) held[i] = load(min(first + i * kJoinThreads + t, rows - 1));
 #pragma unroll
         for (int i = 0; i < kRun; ++i) {
-            const int64_t n = first + t * kRun + i;
-            if (n < rows && is(n)) bits |= 1u << i;
+            const int64_t n = first + i * kJoinThreads + t;
+            bits[i] = __ballot(n < rows && is(n, held[i]));
+            if (lane == 0) counts_of[i][wave] = __popcll(bits[i]);
         }
-        const int32_t mine = __popc(bits);
-        int32_t upto = mine;        // of the wave's lanes up to this one
-#pragma unroll
-        for (int x = 1; x < 64; x <<= 1) {
-            const int32_t other = __shfl_up(upto, x);
-            if (lane >= x) upto += other;
-        }
-        if (lane == 63) counts_of[wave] = upto;
         __syncthreads();
-        int32_t at = before + upto - mine;
-        for (int i = 0; i < kJoinWaves; ++i) {
-            if (i < wave) at += counts_of[i];
-            before += counts_of[i];
-        }
 #pragma unroll
-        for (int i = 0; i < kRun; ++i)
-            if ((bits >> i) & 1) map[at++] = static_cast<int32_t>(first + t * kRun + i);
+        for (int i = 0; i < kRun; ++i) {
+            int32_t at = before;
+#pragma unroll
+            for (int w = 0; w < kJoinWaves; ++w) {
+                if (w < wave) at += counts_of[i][w];
+                before += counts_of[i][w];
+            }
+            at += __popcll(bits[i] & ((uint64_t{1} << lane) - 1));
+            const int64_t n = first + i * kJoinThreads + t;
+            if (n < rows) map[(bits[i] >> lane) & 1 ? at : rows - 1 - (n - at)] = static_cast<int32_t>(n);     // n - at: rows before n not on the list
+        }
         __syncthreads();
     }
     if (t == 0) *live = before;
 }
 
 __global__ __launch_bounds__(kJoinThreads) void live_kernel(LiveArgs a) {
-    list_live(a.rows, a.map, a.live, [&](int64_t n) {
-        const bool is = a.teacher_row ? a.teacher_row[n].z != 0.0f : a.target[n] != a.ignore_index;
+    if (threadIdx.x == 0) *a.ticket = 0;
+    const auto drop = [&](int64_t n, bool is) {
         if (!is) {
             a.state[n] = RowState{0.0f, 0.0f, 0.0f, 0.0f};
             a.row_loss[n] = 0.0f;
         }
         return is;
-    });
+    };
+    if (a.teacher_row)
+        list_live(a.rows, a.map, a.live, [&](int64_t n) { return a.teacher_row[n].z; }, [&](int64_t n, float z) { return drop(n, z != 0.0f); });
+    else
+        list_live(a.rows, a.map, a.live, [&](int64_t n) { return a.target[n]; }, [&](int64_t n, int64_t label) { return drop(n, label != a.ignore_index); });
 }
 
 __global__ __launch_bounds__(kJoinThreads) void row_grad_kernel(RowGradArgs a) {
     __shared__ float peaks[kJoinWaves];
     float top = 0.0f;
     bool bad = false;
-    list_live(a.rows, a.map, a.live, [&](int64_t n) {
-        const RowState st = a.state[n];
-        const float g = row_gradient(a.upstream, a.per_row, a.reduce, a.t, st, n);
+    const float share = *a.reduce * a.t;
+    struct Row {
+        RowState state;
+        float upstream;
+    };
+    list_live(a.rows, a.map, a.live, [&](int64_t n) { return Row{a.state[n], a.upstream[a.per_row ? n : 0]}; }, [&](int64_t n, const Row& r) {
+        const float g = counts(r.state) ? r.upstream * share : 0.0f;
         a.grad[n] = g;
         bad |= !(fabsf(g) < INFINITY);
         top = fmaxf(top, fabsf(g));
-        return counts(st);
+        return counts(r.state);
     });
     top = wave_max(top);
     if (__any(bad)) top = INFINITY;
@@ -438,18 +463,15 @@ __global__ __launch_bounds__(kJoinThreads) void row_grad_kernel(RowGradArgs a) {
     // rows of a gradient that is not finite make everything that sums over rows NaN: the ratio says 1 for all that count
     const bool whole = top < INFINITY;
     if (threadIdx.x == 0) *a.peak = whole ? top : NAN;
-    for (int64_t i = threadIdx.x; i < a.rows; i += kJoinThreads) {
-        const float g = a.grad[i];
-        a.ratio[i] = g == 0.0f ? 0.0f : whole ? g / top : 1.0f;
+    for (int64_t first = threadIdx.x; first < a.rows; first += kJoinThreads * kRun) {
+        float g[kRun];
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) g[i] = a.grad[min(first + i * kJoinThreads, a.rows - 1)];
+#pragma unroll
+        for (int i = 0; i < kRun; ++i)
+            if (first + i * kJoinThreads < a.rows)
+                a.ratio[first + i * kJoinThreads] = g[i] == 0.0f ? 0.0f : whole ? g[i] / top : 1.0f;
     }
-}
-
-// A wave per row.
-__global__ __launch_bounds__(kThreads) void zero_rows_kernel(const RowState* state, int64_t rows, int64_t bytes, char* out) {
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
-    if (row >= rows || counts(state[row])) return;
-    uint16_t* p = reinterpret_cast<uint16_t*>(out + row * bytes);
-    for (int64_t i = threadIdx.x & 63; i < bytes / 2; i += 64) p[i] = 0;
 }
 
 __global__ __launch_bounds__(kThreads) void bias_sum_kernel(const float* parts, const int32_t* live, int32_t tile, int64_t stride, int64_t n, void* out, int32_t dtype) {
@@ -719,18 +741,14 @@ int launch_teacher(const TeacherArgs& a, hipStream_t stream) {
 int launch_join(const JoinArgs& a, hipStream_t stream) {
     return launch(join_kernel, static_cast<unsigned>((a.rows + kJoinRows - 1) / kJoinRows), kJoinThreads, stream, a);
 }
-int launch_narrow_join(const NarrowJoinArgs& a, hipStream_t stream) {
-    return launch(narrow_join_kernel, static_cast<unsigned>(a.join.rows), kThreads, stream, a);
+int launch_narrow_join(const JoinArgs& a, hipStream_t stream) {
+    return launch(narrow_join_kernel, static_cast<unsigned>(a.rows), kThreads, stream, a);
 }
 int launch_reduce(const float* row_loss, const RowState* state, int64_t rows, int reduction, float* loss_out, float* reduce, hipStream_t stream) {
     return launch(reduce_kernel, 1, kJoinThreads, stream, row_loss, state, rows, reduction, loss_out, reduce);
 }
 int launch_live(const LiveArgs& a, hipStream_t stream) { return launch(live_kernel, 1, kJoinThreads, stream, a); }
 int launch_row_grad(const RowGradArgs& a, hipStream_t stream) { return launch(row_grad_kernel, 1, kJoinThreads, stream, a); }
-int launch_zero_rows(const RowState* state, int64_t rows, int64_t width, int32_t dtype, void* d_hidden, hipStream_t stream) {
-    return launch(zero_rows_kernel, static_cast<unsigned>((rows + kThreads / 64 - 1) / (kThreads / 64)), kThreads, stream, state, rows,
-                  width * (dtype == JABAS_F32 ? 4 : 2), static_cast<char*>(d_hidden));
-}
 int launch_bias_sum(const float* parts, const int32_t* live, int32_t tile, int64_t stride, int64_t n, void* out, int32_t dtype, hipStream_t stream) {
     return launch(bias_sum_kernel, static_cast<unsigned>((n + kThreads - 1) / kThreads), kThreads, stream, parts, live, tile, stride, n, out, dtype);
 }
