@@ -10,6 +10,8 @@ namespace loss {
 namespace {
 
 constexpr int64_t kMaxSize = int64_t{1} << 30;      // rows, tokens; the tiles' numbers and tokens are 32 bits in the kernels
+constexpr int64_t kMaxLinearVocab = int64_t{1} << 28;
+constexpr int64_t kMaxGroups = int64_t{1} << 23;    // a launch has less than 2^32 threads, up to 512 a workgroup
 constexpr int64_t kMaxWidth = int64_t{1} << 20;
 constexpr int64_t kMaxLinearRows = kMaxStride;      // a feature's hidden states are one row of an operand
 
@@ -17,7 +19,9 @@ inline int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; 
 inline int64_t tiles(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
 inline size_t element_bytes(int dtype) { return dtype == JABAS_F32 ? 4 : 2; }
 
-constexpr int64_t kNarrowPiece = int64_t{1} << 17;          // tokens whose row gradients are kept at once, in fp32: 32 MiB at most
+// Tokens whose row gradients are kept at once, in fp32: 32 MiB at most. 32 x 262144 x 1024 with 2^14, 2^16, 2^17 and 2^18: fp32 1684, 1435,
+// 1455 and 1426 us, bf16 1321, 1120, 1121 and 1160.
+constexpr int64_t kNarrowPiece = int64_t{1} << 17;
 
 struct Shape {
     bool linear, teacher, narrow;
@@ -40,12 +44,12 @@ int validate(const JabasLoss* l, Shape& s) {
     if (s.linear) {
         if (!l->weight || (!l->hidden && l->rows) || l->logits) return JABAS_ERR_NULL;
         if (l->rows > kMaxLinearRows || l->width < 1 || l->width > kMaxWidth || l->hidden_stride < 0 || l->weight_stride < 0) return JABAS_ERR_SIZE;
-        if (tiles(l->rows, 128) * tiles(l->vocab, 128) > 0x7fffffff) return JABAS_ERR_SIZE;
+        if (l->vocab > kMaxLinearVocab || tiles(l->rows, kTile) * tiles(l->vocab, kTile) >= kMaxGroups) return JABAS_ERR_SIZE;
     } else {
         if ((!l->logits && l->rows) || l->bias || !s.teacher) return JABAS_ERR_NULL;
         int64_t splits, chunk;
         cut_rows(l, false, splits, chunk);
-        if (l->logits_stride < 0 || splits * l->rows > 0x7fffffff) return JABAS_ERR_SIZE;
+        if (l->logits_stride < 0 || splits * l->rows >= 2 * kMaxGroups) return JABAS_ERR_SIZE;
     }
     if (s.teacher) {
         if (l->target || ((!l->teacher_index || !l->teacher_logits || !l->entry_index || !l->entry_p) && l->rows)) return JABAS_ERR_NULL;
@@ -62,7 +66,8 @@ int validate(const JabasLoss* l, Shape& s) {
         misaligned(l->teacher_lse, 4) || misaligned(l->entry_index, 4) || misaligned(l->entry_p, 4))
         return JABAS_ERR_ALIGN;
     s.planes = l->dtype == JABAS_F32 ? 2 : 1;
-    s.narrow = s.linear && l->rows > 0 && l->rows <= kNarrowRows;
+    s.narrow = s.linear && l->rows > 0 && l->rows <= kNarrowRows &&
+               (l->dtype == JABAS_F32 || l->rows <= kNarrowRows / 2 || l->vocab * l->width <= kNarrowWeight);
     s.depth = round_up(s.linear ? l->width : 1, kDepth);
     s.copy_w = !(s.planes == 1 && l->width % kDepth == 0 && l->weight_stride % 8 == 0 && l->weight_stride <= kMaxStride && !misaligned(l->weight, 16));
     return JABAS_OK;
@@ -82,13 +87,16 @@ struct Carver {
 };
 
 // Tokens of a piece: what the pieces' copies may take is bounded, and a piece has whole tiles.
-constexpr int64_t kPieceBytes = int64_t{256} << 20;
+// fp32's pieces are larger: their planes take twice the bytes, and a piece's start and end more time. Forward and backward with 128, 256 and
+// 768 MiB: 4096 x 131072 x 4096 bf16 15.38, 15.19 and 15.17 ms; 1024 x 131072 x 1024 fp32 4.66, 4.64 and 4.04; 2048 x 65536 x 4096 fp32
+// 14.90, 13.59 and 13.04.
+constexpr int64_t kPieceBytes[2] = {int64_t{256} << 20, int64_t{768} << 20};
 int64_t piece_tokens(const JabasLoss* l, const Shape& s, bool backward) {
     int64_t per_token = 0;
     if (s.copy_w) per_token += s.depth * 2 * s.planes;
     if (backward) per_token += (round_up(l->rows, kDepth) + s.depth) * 2 * s.planes;     // dz and the weight in fp16
     if (!per_token) return round_up(l->vocab, kTile);
-    int64_t n = kPieceBytes / per_token / kTile * kTile;
+    int64_t n = kPieceBytes[s.planes - 1] / per_token / kTile * kTile;
     if (n < 4 * kTile) n = 4 * kTile;
     const int64_t whole = round_up(l->vocab, kTile);
     if (n >= whole) return whole;
@@ -111,23 +119,25 @@ struct Forward {
     bool large;
 };
 
-// Logits in hand, workgroups per row. A row is one workgroup's where there are rows enough for the chip (kFullRows), where it is short
-// (kShortRow), and as far as the mask of its entries fits LDS (a bit a token: kMaskTokens). 5 x 131072 fp32: 36 us with a split, 60 without.
+// Logits in hand, workgroups per row, as many as their masks of entries (a bit a token) ask for, LDS's 32 KiB each, and more for a few
+// long rows. Forward, the parts of a row cost a launch that joins them, so that only rows of kLongRow on are cut where there are less
+// than kFullRows: 16 x 131072 bf16 25.7 us whole, 19.3 in parts; 16 x 49152 18.4 and 18.1; 16 x 16000 fp32 18.2 and 20.1;
+// 192 x 131072 30.3 and 28.3; 256 x 131072 fp32 34.8 and 36.6; 512 x 32317 21.6 and 24.1. Backward, 256 x 131072 bf16 takes 53 us with 256
+// workgroups, 50.6 with 1024.
 constexpr int64_t kMaskTokens = int64_t{1} << 18;
-constexpr int64_t kFullRows = 512, kShortRow = 8192;
-constexpr int64_t kLeastSplitTokens = 2048;
-constexpr int64_t kWantedGroups = 1024;
+constexpr int64_t kFullRows = 192, kLongRow = 49152;
+constexpr int64_t kChunk = 32768, kLeastChunk = 2048, kWantedGroups = 1024;
 
 void cut_rows(const JabasLoss* l, bool forward, int64_t& splits, int64_t& chunk) {
-    const int64_t rows = l->rows > 0 ? l->rows : 1;
-    splits = forward ? (l->vocab + kMaskTokens - 1) / kMaskTokens : (l->vocab + 32767) / 32768;
-    if (rows < kFullRows && l->vocab > kShortRow) {
-        const int64_t want = (kWantedGroups + rows - 1) / rows, most = (l->vocab + kLeastSplitTokens - 1) / kLeastSplitTokens;
+    const int64_t rows = l->rows > 0 ? l->rows : 1, largest = forward ? kMaskTokens : kChunk;
+    splits = tiles(l->vocab, largest);
+    if (!forward || (rows < kFullRows && l->vocab >= kLongRow)) {
+        const int64_t want = tiles(kWantedGroups, rows), most = tiles(l->vocab, kLeastChunk);
         const int64_t more = want < most ? want : most;
         if (splits < more) splits = more;
     }
-    chunk = round_up((l->vocab + splits - 1) / splits, 32);
-    splits = (l->vocab + chunk - 1) / chunk;
+    chunk = round_up(tiles(l->vocab, splits), 32);
+    splits = tiles(l->vocab, chunk);
 }
 
 size_t carve_forward(const JabasLoss* l, const Shape& s, char* base, Forward& f) {
@@ -138,9 +148,9 @@ size_t carve_forward(const JabasLoss* l, const Shape& s, char* base, Forward& f)
         f.tiles = narrow_tiles(l->vocab);
         f.ticket = c.take<uint32_t>(1);
     } else if (s.linear) {
-        f.large = large_tiles(l->vocab, rows);
-        f.tiles = tiles(l->vocab, logits_tile(f.large));
         f.piece = piece_tokens(l, s, false);
+        f.large = large_tiles(f.piece < l->vocab ? f.piece : l->vocab, rows);
+        f.tiles = tiles(l->vocab, logits_tile(f.large));
     } else {
         cut_rows(l, true, f.splits, f.chunk);
         f.tiles = f.splits;

@@ -213,8 +213,12 @@ int launch_row_grad(const RowGradArgs& a, hipStream_t stream);
 int launch_bias_sum(const float* parts, const int32_t* live, int32_t tile, int64_t stride, int64_t n, void* out, int32_t dtype, hipStream_t stream);
 int launch_zero(void* p, size_t bytes, hipStream_t stream);
 
-// Few rows, hidden states and weight as they lie (loss_narrow.hip).
+// Few rows, hidden states and weight as they lie (loss_narrow.hip): their gradients' products are fp32's, which with one plane is slower
+// than laying the weight out for tiles as rows and weight grow. Forward and backward, this and the tiles: fp32 16 x 32317 x 1024 178 and
+// 434 us, 64 x 32317 x 1024 396 and 457, 64 x 131072 x 4096 4387 and 8716; bf16 1 x 32317 x 1024 132 and 166, 32 x 32317 x 1024 168 and 175,
+// 33 x 4000 x 768 74 and 89, 64 x 4000 x 768 89 and 89, 64 x 8000 x 768 121 and 97, 64 x 32317 x 1024 348 and 178.
 constexpr int kNarrowRows = 64;
+constexpr int64_t kNarrowWeight = int64_t{3} << 20;
 struct NarrowArgs {
     const void *x, *w, *bias;
     int64_t x_stride, w_stride, vocab;

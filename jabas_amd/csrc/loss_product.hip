@@ -536,12 +536,20 @@ int grads(const GradArgs& a, hipStream_t stream) {
 }
 
 struct Sizes { int m, n; };
-bool large_grads(int64_t features, int64_t tokens, int64_t rows) { return features > 128 && (tokens > 128 || rows > 128) && rows > 128; }
+// Tiles of the gradients' products. Small ones where a side is one of them, and for less than 12e9 products of either: forward and
+// backward, small and large, 256 x 32317 x 1024 fp32 548 and 579 us, bf16 206 and 200; 6400 x 1000 x 768 fp32 252 and 278, bf16 143
+// and 150; 1600 x 8192 x 1024 fp32 476 and 463, bf16 205 and 198; 512 x 32317 x 1024 bf16 292 and 277; 128 x 16384 x 1024 fp32 257 and 280.
+bool large_grads(int64_t features, int64_t tokens, int64_t rows) {
+    return features > 128 && rows > 128 && static_cast<double>(features) * tokens * rows >= 12e9;
+}
 Sizes grads_tile(bool large) { return large ? Sizes{256, 256} : Sizes{128, 128}; }
 
 }  // namespace
 
-bool large_tiles(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) >= 256; }
+// A CU holds one workgroup of a large tile or two of a small one: 512 small tiles, 128 large ones, are one round, and from there on large
+// tiles take one where small ones take two. Forward, large and small: 512 x 16384 x 1024 (128) fp32 118 and 106 us, bf16 49.5 and 43.5;
+// 256 x 33280 (130) 155 and 161, 52.0 and 57.4; 768 x 16384 (192) 130 and 142, 53.0 and 57.2; 1600 x 32317 (889) 412 and 416, 142 and 145.
+bool large_tiles(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) > 128; }
 int logits_tile(bool large) { return large ? 256 : 128; }
 
 int launch_logits_forward(const LogitsArgs& a, int planes, bool large, hipStream_t stream) { return logits(a, planes, large, false, stream); }
@@ -592,8 +600,9 @@ double makespan(int slots, int64_t na, double la, int64_t nb, double lb) {
 
 // The split that the model above says ends first. A unit costs its steps of 64 elements and kUnit more for its start and its results; fp32
 // sums that are written, read and joined cost what their bytes take of the chip's bandwidth (a step of a 256 x 256 tile is 1.8 us at
-// 1.2 PFLOP/s, in which HBM moves 9 MB). Without splits 1600 x 1024 sums over 16 thousand tokens ran on 104 of 256 CUs: 406 us,
-// 182 with them.
+// 1.2 PFLOP/s, in which HBM moves 9 MB). Forward and backward,
+// fp32, without splits and with those chosen: 100 x 16384 x 1024 615 and 250 us, 256 x 32317 2201 and 581, 1600 x 32317 2896 and 1637,
+// 6400 x 32317 5288 and 5365; none of 2, 4, 8 or 16 splits of dX alone is over 4 % faster than the choice, bf16 included.
 Splits choose_splits(int64_t features, int64_t tokens, int64_t rows, bool w, bool h, bool many_pieces, int planes) {
     const bool large = large_grads(features, tokens, rows);
     const Sizes t = grads_tile(large);
