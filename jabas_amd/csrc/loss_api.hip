@@ -149,7 +149,7 @@ size_t carve_forward(const JabasLoss* l, const Shape& s, char* base, Forward& f)
         f.ticket = c.take<uint32_t>(1);
     } else if (s.linear) {
         f.piece = piece_tokens(l, s, false);
-        f.large = large_tiles(f.piece < l->vocab ? f.piece : l->vocab, rows);
+        f.large = large_tiles(f.piece < l->vocab ? f.piece : l->vocab, rows, s.planes, false);
         f.tiles = tiles(l->vocab, logits_tile(f.large));
     } else {
         cut_rows(l, true, f.splits, f.chunk);
@@ -227,7 +227,7 @@ size_t carve_backward(const JabasLoss* l, const Shape& s, char* base, Backward& 
     b.inner = choose_splits(l->width, tokens, rows, true, true, b.piece < l->vocab, s.planes);
     if (b.inner.w > 1) b.part_w = c.take<float>(b.inner.w * tokens * b.part_stride);
     if (b.inner.h > 1 || b.piece < l->vocab) b.part_h = c.take<float>(b.inner.h * rows * b.part_stride);
-    b.large = large_tiles(tokens, rows);
+    b.large = large_tiles(tokens, rows, s.planes, true);
     if (l->bias) b.db = c.take<float>(tiles(rows, logits_tile(b.large)) * b.piece);
     return c.all();
 }

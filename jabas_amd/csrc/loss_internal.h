@@ -109,8 +109,8 @@ struct GradArgs {
     Job w, h;
     int32_t h_first;            // workgroups of h come first: they take longer
 };
-// Whether a product of m x n takes the large tiles, and how many tokens and rows a tile of logits has.
-bool large_tiles(int64_t m, int64_t n);
+// Whether the logits of a piece take the large tiles, and how many tokens and rows a tile of logits has.
+bool large_tiles(int64_t tokens, int64_t rows, int planes, bool backward);
 int logits_tile(bool large);
 int launch_logits_forward(const LogitsArgs& a, int planes, bool large, hipStream_t stream);
 int launch_logits_backward(const LogitsArgs& a, int planes, bool large, hipStream_t stream);

@@ -546,10 +546,15 @@ Sizes grads_tile(bool large) { return large ? Sizes{256, 256} : Sizes{128, 128};
 
 }  // namespace
 
-// A CU holds one workgroup of a large tile or two of a small one: 512 small tiles, 128 large ones, are one round, and from there on large
-// tiles take one where small ones take two. Forward, large and small: 512 x 16384 x 1024 (128) fp32 118 and 106 us, bf16 49.5 and 43.5;
-// 256 x 33280 (130) 155 and 161, 52.0 and 57.4; 768 x 16384 (192) 130 and 142, 53.0 and 57.2; 1600 x 32317 (889) 412 and 416, 142 and 145.
-bool large_tiles(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) > 128; }
+// A CU holds one workgroup of a large tile or two of a small one, whose round takes 0.6 of a large one's, or 0.55 behind fp32's backward
+// pass, whose large tile runs out of registers. Forward, then forward and backward, small and large, by 1024: 512 x 16384 (128 large tiles)
+// fp32 106 and 118 us; 512 x 32317 (254) fp32 185 and 170, 710 and 669, bf16 64.7 and 56.6, 286 and 274; 640 x 32317 (381) 231 and 237,
+// 829 and 876, 79 and 83, 341 and 349; 1280 x 32317 (635) 345 and 331, 1266 and 1286, 124 and 118, 496 and 491; 5120 x 32317 (2540) 1072
+// and 962, 4143 and 3988, 386 and 344, 1521 and 1430. 256 x 128 was no faster than the better of the two at any of these.
+bool large_tiles(int64_t tokens, int64_t rows, int planes, bool backward) {
+    const auto rounds = [&](int64_t tile, int64_t slots) { return ((tokens + tile - 1) / tile * ((rows + tile - 1) / tile) + slots - 1) / slots; };
+    return rounds(128, 512) * (planes == 2 && backward ? 0.55 : 0.6) >= rounds(256, 256);
+}
 int logits_tile(bool large) { return large ? 256 : 128; }
 
 int launch_logits_forward(const LogitsArgs& a, int planes, bool large, hipStream_t stream) { return logits(a, planes, large, false, stream); }

@@ -226,7 +226,7 @@ __device__ inline RowResult label_result(const JoinArgs& a, int64_t row, float p
     return r;
 }
 
-constexpr int kJoinThreads = 1024, kJoinRows = 64, kJoinWaves = kJoinThreads / 64;
+constexpr int kJoinThreads = 1024, kJoinRows = 16, kJoinWaves = kJoinThreads / 64;
 
 __device__ inline bool counts(const RowState& st) { return !(st.slope == 0.0f && st.mass == 0.0f); }
 
@@ -261,47 +261,63 @@ __global__ __launch_bounds__(kJoinThreads) void reduce_kernel(const float* row_l
     finish(sum, number, reduction, loss_out, reduce);
 }
 
-// 64 rows per workgroup: each wave joins a sixteenth of the vocabulary's tiles with a row per lane, then the waves' results
-// are joined, and each wave takes the entries of its rows in turn.
+// A row of a part of the vocabulary joined with another's: (peak, sum) of both.
+__device__ inline void merge(float& peak, float& sum, float other_peak, float other_sum, float c) {
+    const float p = fmaxf(peak, other_peak);
+    sum = rescale(sum, peak, p, c) + rescale(other_sum, other_peak, p, c);
+    peak = p;
+}
+
+// The wave's stores are in memory, not only on their way.
+__device__ inline void stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// kJoinRows rows per workgroup: 16 lanes of a wave take a row each, a sixty-fourth of the vocabulary's tiles; then the parts are joined,
+// and each wave takes the entries of its row.
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(JoinArgs a) {
+    constexpr int kParts = kJoinThreads / kJoinRows;
+    static_assert(kJoinRows == kJoinWaves, "a row's entries per wave");
     __shared__ float peaks[kJoinWaves][kJoinRows], sums[kJoinWaves][kJoinRows], totals[kJoinWaves][kJoinRows];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kJoinRows, mine = first + lane, rows = *a.live.live;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, at = lane % kJoinRows;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kJoinRows, mine = first + at, rows = *a.live.live;
     if (first >= rows && first) return;
     float peak = -INFINITY, sum = 0.0f, total = 0.0f;
     if (mine < rows)
-        for (int i = wave; i < a.tiles; i += kJoinWaves) {
+        for (int i = threadIdx.x / kJoinRows; i < a.tiles; i += kParts) {
             const float2 part = a.partial[static_cast<int64_t>(i) * a.rows + mine];
-            const float p = fmaxf(peak, part.x);
-            sum = rescale(sum, peak, p, a.c) + rescale(part.y, part.x, p, a.c);
-            peak = p;
+            merge(peak, sum, part.x, part.y, a.c);
             if (a.total) total += a.total[static_cast<int64_t>(i) * a.rows + mine];
         }
-    peaks[wave][lane] = peak;
-    sums[wave][lane] = sum;
-    totals[wave][lane] = total;
+#pragma unroll
+    for (int x = kJoinRows; x < 64; x *= 2) {
+        merge(peak, sum, __shfl_xor(peak, x), __shfl_xor(sum, x), a.c);
+        total += __shfl_xor(total, x);
+    }
+    if (lane < kJoinRows) {
+        peaks[wave][at] = peak;
+        sums[wave][at] = sum;
+        totals[wave][at] = total;
+    }
     __syncthreads();
     if (wave == 0) {
         for (int i = 1; i < kJoinWaves; ++i) {
-            const float p = fmaxf(peak, peaks[i][lane]);
-            sum = rescale(sum, peak, p, a.c) + rescale(sums[i][lane], peaks[i][lane], p, a.c);
-            peak = p;
-            total += totals[i][lane];
+            merge(peak, sum, peaks[i][at], sums[i][at], a.c);
+            total += totals[i][at];
         }
-        peaks[0][lane] = peak;
-        sums[0][lane] = sum;
-        totals[0][lane] = total;
+        if (lane < kJoinRows) {
+            peaks[0][at] = peak;
+            sums[0][at] = sum;
+        }
     }
     __syncthreads();
-    if (!a.entries.index && wave == 0 && mine < rows) {
+    if (!a.entries.index && threadIdx.x < kJoinRows && mine < rows) {
         const int32_t row = a.live.map[mine];
         const RowResult r = label_result(a, row, peak, sum, total);
         a.state[row] = r.state;
         __hip_atomic_store(a.row_loss + row, r.loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    for (int r = wave; a.entries.index && r < kJoinRows && first + r < rows; r += kJoinWaves) {
-        const int64_t row = a.live.map[first + r];
-        const RowResult result = entries_result(a, row, peaks[0][r], sums[0][r]);
+    if (a.entries.index && first + wave < rows) {
+        const int64_t row = a.live.map[first + wave];
+        const RowResult result = entries_result(a, row, peaks[0][wave], sums[0][wave]);
         if (lane == 0) {
             a.state[row] = result.state;
             __hip_atomic_store(a.row_loss + row, result.loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -311,9 +327,10 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(JoinArgs a) {
         if (first == 0 && threadIdx.x == 0) *a.reduce = 1.0f;
         return;
     }
-    // The last workgroup to finish sums the rows' losses, in order. They were stored past the dies' own caches, so one thread's release is
-    // enough, and they are loaded past them.
+    // The last workgroup to finish sums the rows' losses, in order. They were stored past the dies' own caches, where every wave waits for
+    // them to be, so one thread's release is enough, and they are loaded past them.
     __shared__ uint32_t done;
+    stores_done();
     __syncthreads();
     if (threadIdx.x == 0) done = __hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
@@ -734,7 +751,8 @@ __global__ __launch_bounds__(kThreads) void topk_backward_kernel(TopkArgs a) {
         }
     }
     if (!live) return;
-    __syncthreads();            // the entries' places are written again: behind the stores above, which the barrier waits for
+    stores_done();
+    __syncthreads();            // the entries' places are written again
     const int j = threadIdx.x;
     if (j >= a.entries.k) return;
     const int64_t v = a.entries.index[row * a.entries.k + j];
