@@ -76,8 +76,10 @@ class Reference:
                 if rest:
                     size[r][~named] += T * rest * (logq[~named] - others).exp()
             counted[r] = True
-            here = z[r][torch.isfinite(z[r])].abs().max().item() if x is None else (x[r].abs() @ w.abs().t()).max().item() + (0.0 if b is None else b[torch.isfinite(b)].abs().max().item())
-            Z = max(Z, here / T)
+            if x is None:
+                Z = max(Z, z[r][torch.isfinite(z[r])].abs().max().item() / T)
+        if x is not None and bool(counted.any()):
+            Z = ((x[counted].abs() @ w.abs().t()).max().item() + (0.0 if b is None else b[torch.isfinite(b)].abs().max().item())) / T
         self.Z, self.counted, self.T = Z, counted, T
         share = 1.0 / max(1, int(counted.sum())) if reduction == "mean" else 1.0
         g = (torch.ones(n, dtype=F64) if upstream is None else upstream.detach().cpu().to(F64).expand(n)) * share
@@ -277,6 +279,114 @@ def test_several_pieces_of_the_vocabulary(gpu):
             loss = losses.linear_cross_entropy(x, w, target.to(gpu), b)
             ref = Reference(x, w, b, target=target)
         ref.check(loss, _grads(loss, (x, w, b)), dtype)
+
+
+@pytest.mark.parametrize("dtype,rows,vocab,width", [("bf16", 64, 1000, 100), ("bf16", 40, 3300, 1000), ("bf16", 64, 3300, 1000), ("fp32", 64, 3300, 1000),
+                                                    ("fp32", 65, 3300, 128), ("bf16", 20, 140001, 64), ("fp32", 40, 140001, 64)])
+def test_few_rows(gpu, dtype, rows, vocab, width):
+    """Either side of the sizes up to which few rows have kernels of their own, and more tokens than those keep row gradients of."""
+    (x, w, b), gen = _inputs(gpu, rows, vocab, width, dtype, True, seed=rows)
+    target = torch.randint(0, vocab, (rows,), generator=gen)
+    target[1::6] = IGNORE
+    loss = losses.linear_cross_entropy(x, w, target.to(gpu), b, label_smoothing=0.1)
+    Reference(x, w, b, target=target, smoothing=0.1).check(loss, _grads(loss, (x, w, b)), dtype)
+    index = torch.randint(0, vocab // 30, (rows, 30), generator=gen) + torch.arange(30) * (vocab // 30)
+    teacher = torch.randn(rows, 30, generator=gen).to(TYPES[dtype])
+    lse = torch.logsumexp(teacher.float(), 1) + 0.5
+    loss = losses.linear_topk_distillation(x, w, index.to(gpu), teacher.to(gpu), b, teacher_lse=lse.to(gpu))
+    Reference(x, w, b, index=index, teacher=teacher, lse=lse).check(loss, _grads(loss, (x, w, b)), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("form", ["labels", "entries"])
+@pytest.mark.parametrize("rows,vocab,width", [(300, 22001, 128), (300, 22001, 1900), (514, 17000, 72)])
+def test_large_tiles(gpu, dtype, form, rows, vocab, width):
+    """Enough tiles for the large ones, of the logits and (1900 features) of the gradients, whose last row, token and feature tiles are odd."""
+    (x, w, b), gen = _inputs(gpu, rows, vocab, width, dtype, form == "labels", seed=width)
+    if form == "labels":
+        target = torch.randint(0, vocab, (rows,), generator=gen)
+        target[torch.randperm(rows, generator=gen)[:rows // 9]] = IGNORE
+        loss = losses.linear_cross_entropy(x, w, target.to(gpu), b, label_smoothing=0.1, reduction="sum")
+        ref = Reference(x, w, b, target=target, smoothing=0.1, reduction="sum")
+    else:
+        index = torch.randint(0, vocab // 64, (rows, 64), generator=gen) + torch.arange(64) * (vocab // 64)
+        index[torch.randperm(rows, generator=gen)[:rows // 9]] = -1
+        teacher = (torch.randn(rows, 64, generator=gen) * 2).to(TYPES[dtype])
+        lse = torch.logsumexp(teacher.float() / 2, 1) + torch.rand(rows, generator=gen)
+        loss = losses.linear_topk_distillation(x, w, index.to(gpu), teacher.to(gpu), temperature=2.0, teacher_lse=lse.to(gpu))
+        ref = Reference(x, w, index=index, teacher=teacher, lse=lse, T=2.0)
+    ref.check(loss, _grads(loss, (x, w) if b is None else (x, w, b)), dtype)
+
+
+def test_forward_pieces_of_the_vocabulary(gpu):
+    """A wide weight in 32 bits, whose planes are kept for a part of the vocabulary at a time in the forward pass too."""
+    rows, vocab, width = 66, 50001, 4096
+    (x, w, _), gen = _inputs(gpu, rows, vocab, width, "fp32", seed=3)
+    target = torch.randint(0, vocab, (rows,), generator=gen)
+    target[:2] = torch.tensor([vocab - 1, 0])
+    loss = losses.linear_cross_entropy(x, w, target.to(gpu))
+    Reference(x, w, target=target).check(loss, _grads(loss, (x, w)), "fp32")
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows", [70, 300])
+@pytest.mark.parametrize("counted", [0, 1])
+def test_hardly_a_row_counts(gpu, dtype, rows, counted):
+    vocab, width = 22001, 70
+    (x, w, b), gen = _inputs(gpu, rows, vocab, width, dtype, True, seed=rows)
+    target = torch.full((rows,), IGNORE)
+    target[rows - 3:rows - 3 + counted] = 4242
+    loss = losses.linear_cross_entropy(x, w, target.to(gpu), b)
+    grads = _grads(loss, (x, w, b))
+    if counted:
+        Reference(x, w, b, target=target).check(loss, grads, dtype)
+    else:
+        assert float(loss.detach()) == 0.0 and not any(bool(g.any()) for g in grads)
+    index = torch.full((rows, 3), -1)
+    index[5:5 + counted] = torch.tensor([7, 22000, 9])
+    teacher = torch.randn(rows, 3, generator=gen).to(TYPES[dtype])
+    loss = losses.linear_topk_distillation(x, w, index.to(gpu), teacher.to(gpu), b)
+    grads = _grads(loss, (x, w, b))
+    if counted:
+        Reference(x, w, b, index=index, teacher=teacher).check(loss, grads, dtype)
+    else:
+        assert float(loss.detach()) == 0.0 and not any(bool(g.any()) for g in grads)
+
+
+@pytest.mark.parametrize("dtype,rows,vocab", [("fp32", 520, 131071), ("bf16", 1100, 131071), ("bf16", 192, 262147), ("fp32", 191, 49153), ("fp32", 20, 524289),
+                                              ("bf16", 700, 9001)])
+def test_many_and_long_rows_of_logits(gpu, dtype, rows, vocab):
+    """Rows whole and in parts, through the caches and past them; some of the rows are checked, each by itself."""
+    gen = _gen(rows)
+    z = torch.empty(rows, vocab, dtype=TYPES[dtype], device=gpu).normal_(std=2.0, generator=torch.Generator(device=gpu).manual_seed(rows))
+    index = torch.randint(0, vocab // 16, (rows, 16), generator=gen) + torch.arange(16) * (vocab // 16)
+    index[:, 15] = vocab - 1
+    teacher = (torch.randn(rows, 16, generator=gen) * 2).to(TYPES[dtype])
+    lse = torch.logsumexp(teacher.float(), 1) + 0.5
+    up = torch.randn(rows, generator=gen)
+    z.requires_grad_(True)
+    loss = losses.topk_distillation(z, index.to(gpu), teacher.to(gpu), teacher_lse=lse.to(gpu), reduction="none")
+    grad = _grads(loss, (z,), up.to(gpu))[0]
+    some = [0, 1, rows // 2, rows - 2, rows - 1]
+    Reference(logits=z[some], index=index[some], teacher=teacher[some], lse=lse[some], reduction="none", upstream=up[some]).check(loss[some], [grad[some]], dtype)
+    # a row's gradient sums to nothing: of the sizes' sum, bf16's results are off by 2^-9 each, fp32's by 2^-20 times a few
+    mass = grad.float().sum(1).cpu()
+    size = grad.float().abs().sum(1).cpu()
+    assert bool((mass.abs() <= size * (2.0 ** -8 if dtype == "bf16" else 2.0 ** -17)).all())
+
+
+def test_criteria_are_the_functions(gpu):
+    (x, w, b), gen = _inputs(gpu, 20, 300, 64, "fp32", True)
+    target = torch.randint(0, 300, (4, 5), generator=gen).to(gpu)
+    target[0, 2] = 0
+    hidden = x.view(4, 5, 64)
+    a = losses.LinearCrossEntropy(ignore_index=0, label_smoothing=0.1)((hidden, w, b), target)
+    assert torch.equal(a, losses.linear_cross_entropy(hidden, w, target, b, ignore_index=0, label_smoothing=0.1))
+    index, teacher = (t.view(4, 5, 6).to(gpu) for t in _entries(gen, 20, 300, 6, "fp32"))
+    lse = torch.logsumexp(teacher, 2) + 0.1
+    d = losses.LinearTopkDistillation(temperature=2.0, reduction="sum")
+    assert torch.equal(d((hidden, w, None), (index, teacher)), losses.linear_topk_distillation(hidden, w, index, teacher, temperature=2.0, reduction="sum"))
+    assert torch.equal(d((hidden, w, b), (index, teacher, lse)), losses.linear_topk_distillation(hidden, w, index, teacher, b, temperature=2.0, teacher_lse=lse, reduction="sum"))
 
 
 # ------------------------------------------------------------------ masks and values

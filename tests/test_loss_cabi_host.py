@@ -90,6 +90,8 @@ def test_backward_workspace_does_not_grow_with_the_vocabulary(dtype, rows):
     (_linear, dict(dtype=2), L.ERR_DTYPE), (_linear, dict(reduction=3), L.ERR_SIZE), (_linear, dict(rows=-1), L.ERR_SIZE),
     (_linear, dict(vocab=0), L.ERR_SIZE), (_linear, dict(width=0), L.ERR_SIZE), (_linear, dict(vocab=1 << 31), L.ERR_SIZE),
     (_linear, dict(rows=1 << 30, vocab=1 << 30), L.ERR_SIZE), (_linear, dict(weight_stride=-1), L.ERR_SIZE),
+    (_linear, dict(vocab=(1 << 28) + 1), L.ERR_SIZE), (_linear, dict(rows=(1 << 22) + 1), L.ERR_SIZE), (_linear, dict(rows=1 << 22, vocab=1 << 18), L.ERR_SIZE),
+    (_topk, dict(rows=1 << 24, vocab=8), L.ERR_SIZE), (_linear, dict(width=(1 << 20) + 1), L.ERR_SIZE),
     (_linear, dict(weight=None), L.ERR_NULL), (_linear, dict(hidden=None), L.ERR_NULL), (_linear, dict(target=None), L.ERR_NULL),
     (_linear, dict(row_state=None), L.ERR_NULL), (_linear, dict(logits=ADDRESS), L.ERR_NULL),
     (_linear, dict(label_smoothing=1.0), L.ERR_SIZE), (_linear, dict(label_smoothing=-0.1), L.ERR_SIZE),
