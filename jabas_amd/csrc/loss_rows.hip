@@ -644,14 +644,14 @@ __global__ __launch_bounds__(kThreads) void topk_row_kernel(TopkArgs a) {
     const int t = threadIdx.x;
     const T* z = static_cast<const T*>(a.logits) + row * a.stride;
     const int64_t name = t < a.teacher.k ? a.teacher.index[row * a.teacher.k + t] : -1;
-    const bool is = name >= 0 && name < a.vocab && !(load_as_float(a.teacher.logits, row * a.teacher.k + t, a.dtype) == -INFINITY);
+    const bool is = name >= 0 && !(load_as_float(a.teacher.logits, row * a.teacher.k + t, a.dtype) == -INFINITY);
     const int words = static_cast<int>((a.vocab + 31) / 32);
     for (int i = t; i < words; i += kThreads) mask[i] = 0;
-    __syncthreads();
+    const bool counts = __syncthreads_or(is);
     if (is) mark(mask, name, 0, a.vocab);
     __syncthreads();
-    float peak, sum;
-    stream_row<STREAM>(z, 0, a.vocab, mask, a.c, peak, sum);
+    float peak = -INFINITY, sum = 0.0f;
+    if (counts) stream_row<STREAM>(z, 0, a.vocab, mask, a.c, peak, sum);
     if (t >= 64) return;
     const WaveEntries w = wave_entries(a.teacher, row, names, probs);
     keep_entries(a.teacher, row, w);
@@ -674,14 +674,14 @@ __global__ __launch_bounds__(kThreads) void topk_split_kernel(TopkArgs a) {
     const int t = threadIdx.x;
     const T* z = static_cast<const T*>(a.logits) + row * a.stride;
     const int64_t name = t < a.teacher.k ? a.teacher.index[row * a.teacher.k + t] : -1;
-    const bool is = name >= 0 && name < a.vocab && !(load_as_float(a.teacher.logits, row * a.teacher.k + t, a.dtype) == -INFINITY);
+    const bool is = name >= 0 && !(load_as_float(a.teacher.logits, row * a.teacher.k + t, a.dtype) == -INFINITY);
     const int words = static_cast<int>((end - begin + 31) / 32);
     for (int i = t; i < words; i += kThreads) mask[i] = 0;
-    __syncthreads();
+    const bool counts = __syncthreads_or(is);
     if (is) mark(mask, name, begin, end);
     __syncthreads();
-    float peak, sum;
-    stream_row<STREAM>(z, begin, end, mask, a.c, peak, sum);
+    float peak = -INFINITY, sum = 0.0f;
+    if (counts) stream_row<STREAM>(z, begin, end, mask, a.c, peak, sum);
     if (t == 0) a.partial[row * a.splits + split] = make_float2(peak, sum);
 }
 
@@ -724,9 +724,16 @@ __global__ __launch_bounds__(kThreads) void topk_backward_kernel(TopkArgs a) {
     T* out = static_cast<T*>(a.out) + row * a.vocab;
     const RowState st = a.state[row];
     const float g = row_gradient(a.upstream, a.per_row, a.reduce, a.t, st, row);
-    const bool live = g != 0.0f;
+    if (g == 0.0f) {            // nothing to read
+        for (int64_t at = begin + threadIdx.x * n; at < end; at += kThreads * n) {
+            if (at + n <= end) store_pack<STREAM>(out + at, Pack<T>{});
+            else
+                for (int64_t i = at; i < end; ++i) out[i] = T(0);
+        }
+        return;
+    }
     const float slope = st.slope * g;
-    const auto grad = [&](T x) { return Vec<T>::put(live ? slope * __builtin_amdgcn_exp2f((Vec<T>::get(x) - st.peak_rest) * a.c) : 0.0f); };
+    const auto grad = [&](T x) { return Vec<T>::put(slope * __builtin_amdgcn_exp2f((Vec<T>::get(x) - st.peak_rest) * a.c)); };
     int64_t first = begin;
     constexpr int64_t kRound = static_cast<int64_t>(kThreads) * n * kUnroll;
     for (; first + kRound <= end; first += kRound) {
@@ -750,7 +757,6 @@ __global__ __launch_bounds__(kThreads) void topk_backward_kernel(TopkArgs a) {
             for (int64_t i = at; i < end; ++i) out[i] = grad(z[i]);
         }
     }
-    if (!live) return;
     stores_done();
     __syncthreads();            // the entries' places are written again
     const int j = threadIdx.x;
