@@ -154,12 +154,13 @@ size_t carve_forward(const JabasLoss* l, const Shape& s, char* base, Forward& f)
     } else {
         cut_rows(l, true, f.splits, f.chunk);
         f.tiles = f.splits;
+        f.ticket = c.take<uint32_t>(1);
     }
     f.partial = c.take<float2>(f.tiles * rows);
     if (l->label_smoothing != 0.0) f.total = c.take<float>(f.tiles * rows);
     if (s.linear) f.entry_logit = c.take<float>(rows * (s.teacher ? l->entries : 1));
     if (s.linear && s.teacher) f.teacher_row = c.take<float4>(rows);
-    f.row_loss = c.take<float>(s.narrow ? 2 * rows : rows);
+    f.row_loss = c.take<float>(s.narrow || f.splits > 1 ? 2 * rows : rows);
     if (s.narrow) return c.all();
     if (s.linear) {
         f.map = c.take<int32_t>(rows);
@@ -417,8 +418,11 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
         a.partial = f.partial;
         a.state = state;
         a.row_loss = f.row_loss;
-        JABAS_TRY(launch_topk_forward(a, stream));
-        return launch_reduce(f.row_loss, state, l->rows, l->reduction, loss_out, reduce, stream);
+        a.ticket = f.ticket;
+        a.reduction = l->reduction;
+        a.loss_out = loss_out;
+        a.reduce_out = reduce;
+        return launch_topk_forward(a, stream);
     }
     JoinArgs j{};
     j.live = Live{f.map, f.live};

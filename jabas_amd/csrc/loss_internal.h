@@ -268,7 +268,10 @@ struct TopkArgs {
     TeacherArgs teacher;
     float2* partial;            // [row][split]
     RowState* state;
-    float* row_loss;
+    float* row_loss;            // where a row has parts: and, behind the rows' losses, whether they count
+    uint32_t* ticket;
+    int32_t reduction;
+    float *loss_out, *reduce_out;
     Entries entries;            // backward
     const float* upstream;
     int32_t per_row;

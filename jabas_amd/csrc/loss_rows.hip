@@ -230,14 +230,21 @@ constexpr int kJoinThreads = 1024, kJoinRows = 16, kJoinWaves = kJoinThreads / 6
 
 __device__ inline bool counts(const RowState& st) { return !(st.slope == 0.0f && st.mass == 0.0f); }
 
-// The loss and the share of a row from every thread's sums, by a workgroup of kJoinThreads.
-__device__ inline void finish(double sum, double number, int reduction, float* loss_out, float* reduce) {
-    __shared__ double sums[kJoinWaves];
-    sum = wave_sum(sum);
-    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
+// The sum over a workgroup of WAVES waves, in thread 0.
+template <int WAVES>
+__device__ inline double group_sum(double x) {
+    __shared__ double sums[WAVES];
+    x = wave_sum(x);
     __syncthreads();
-    if (threadIdx.x) return;
-    for (int i = 1; i < kJoinWaves; ++i) sum += sums[i];
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = sums[0];
+    for (int i = 1; i < WAVES; ++i) x += sums[i];
+    return x;
+}
+
+// The loss and the share of a row from the sums, by one thread.
+__device__ inline void finish(double sum, double number, int reduction, float* loss_out, float* reduce) {
     const double share = reduction == JABAS_LOSS_MEAN && number > 0.0 ? 1.0 / number : 1.0;
     *reduce = static_cast<float>(share);
     if (reduction != JABAS_LOSS_NONE) *loss_out = static_cast<float>(sum * share);
@@ -245,7 +252,6 @@ __device__ inline void finish(double sum, double number, int reduction, float* l
 
 __global__ __launch_bounds__(kJoinThreads) void reduce_kernel(const float* row_loss, const RowState* state, int64_t rows, int reduction,
                                                               float* loss_out, float* reduce) {
-    __shared__ double numbers[kJoinWaves];
     double sum = 0.0, number = 0.0;
     for (int64_t i = threadIdx.x; i < rows; i += kJoinThreads) {
         const float loss = row_loss[i];
@@ -253,13 +259,17 @@ __global__ __launch_bounds__(kJoinThreads) void reduce_kernel(const float* row_l
         number += counts(state[i]) ? 1.0 : 0.0;
         if (reduction == JABAS_LOSS_NONE) loss_out[i] = loss;
     }
-    number = wave_sum(number);
-    if ((threadIdx.x & 63) == 0) numbers[threadIdx.x >> 6] = number;
-    __syncthreads();
-    number = 0.0;
-    for (int i = 0; i < kJoinWaves; ++i) number += numbers[i];
-    finish(sum, number, reduction, loss_out, reduce);
+    sum = group_sum<kJoinWaves>(sum);
+    number = group_sum<kJoinWaves>(number);
+    if (threadIdx.x == 0) finish(sum, number, reduction, loss_out, reduce);
 }
+
+// A row's loss, and whether it counts, stored past the dies' own caches for the workgroup that sums over the rows.
+__device__ inline void hand_over(float* row_loss, int64_t rows, int64_t row, float loss, bool counts) {
+    __hip_atomic_store(row_loss + row, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(row_loss + rows + row, counts ? 1.0f : 0.0f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline float handed_over(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 // A row of a part of the vocabulary joined with another's: (peak, sum) of both.
 __device__ inline void merge(float& peak, float& sum, float other_peak, float other_sum, float c) {
@@ -337,8 +347,9 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(JoinArgs a) {
     if (done + 1 != (rows > kJoinRows ? static_cast<uint32_t>((rows + kJoinRows - 1) / kJoinRows) : 1)) return;
     double loss = 0.0;
 #pragma unroll 4
-    for (int64_t i = threadIdx.x; i < a.rows; i += kJoinThreads) loss += __hip_atomic_load(a.row_loss + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    finish(loss, static_cast<double>(rows), a.reduction, a.loss_out, a.reduce);
+    for (int64_t i = threadIdx.x; i < a.rows; i += kJoinThreads) loss += handed_over(a.row_loss + i);
+    loss = group_sum<kJoinWaves>(loss);
+    if (threadIdx.x == 0) finish(loss, static_cast<double>(rows), a.reduction, a.loss_out, a.reduce);
 }
 
 // Few rows: a workgroup joins a row's tiles; the last one to finish sums the rows' losses, in order.
@@ -377,9 +388,7 @@ __global__ __launch_bounds__(kThreads) void narrow_join_kernel(JoinArgs a) {
     uint32_t done = 0;
     if (t == 0) {
         a.state[row] = r.state;
-        // what the last workgroup reads of the others: written through to the chip's memory, then the ticket
-        __hip_atomic_store(a.row_loss + row, r.loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(a.row_loss + a.rows + row, counts(r.state) ? 1.0f : 0.0f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        hand_over(a.row_loss, a.rows, row, r.loss, counts(r.state));
         if (a.reduction == JABAS_LOSS_NONE) a.loss_out[row] = r.loss;
         done = __hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
     }
@@ -388,15 +397,12 @@ __global__ __launch_bounds__(kThreads) void narrow_join_kernel(JoinArgs a) {
     const int lane = t & 63;
     double loss = 0.0, number = 0.0;
     if (lane < a.rows) {
-        loss = __hip_atomic_load(a.row_loss + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        number = __hip_atomic_load(a.row_loss + a.rows + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        loss = handed_over(a.row_loss + lane);
+        number = handed_over(a.row_loss + a.rows + lane);
     }
     loss = wave_sum(loss);
     number = wave_sum(number);
-    if (lane) return;
-    const double share = a.reduction == JABAS_LOSS_MEAN && number > 0.0 ? 1.0 / number : 1.0;
-    *a.reduce = static_cast<float>(share);
-    if (a.reduction != JABAS_LOSS_NONE) *a.loss_out = static_cast<float>(loss * share);
+    if (lane == 0) finish(loss, number, a.reduction, a.loss_out, a.reduce);
 }
 
 // The gradient of a row's loss in units of dz; 0 where it does not count.
@@ -665,7 +671,7 @@ __global__ __launch_bounds__(kThreads) void topk_row_kernel(TopkArgs a) {
     }
 }
 
-// Few rows: a chunk of a row per workgroup, joined by topk_join_kernel.
+// A chunk of a row per workgroup, joined by topk_join_kernel.
 template <class T, bool STREAM>
 __global__ __launch_bounds__(kThreads) void topk_split_kernel(TopkArgs a) {
     extern __shared__ __align__(16) uint32_t mask[];
@@ -682,37 +688,55 @@ __global__ __launch_bounds__(kThreads) void topk_split_kernel(TopkArgs a) {
     __syncthreads();
     float peak = -INFINITY, sum = 0.0f;
     if (counts) stream_row<STREAM>(z, begin, end, mask, a.c, peak, sum);
-    if (t == 0) a.partial[row * a.splits + split] = make_float2(peak, sum);
+    if (t == 0) {
+        a.partial[row * a.splits + split] = make_float2(peak, sum);
+        if (blockIdx.x == 0) *a.ticket = 0;
+    }
 }
 
-// A wave per row.
+// A wave per row; the last workgroup to finish sums the rows' losses, in order.
 template <class T>
 __global__ __launch_bounds__(kThreads) void topk_join_kernel(TopkArgs a) {
-    __shared__ __align__(16) int32_t names[kThreads / 64][64 * kEntriesPerLane];
-    __shared__ float probs[kThreads / 64][64 * kEntriesPerLane];
+    constexpr int kWaves = kThreads / 64;
+    __shared__ __align__(16) int32_t names[kWaves][64 * kEntriesPerLane];
+    __shared__ float probs[kWaves][64 * kEntriesPerLane];
+    __shared__ uint32_t done;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + wave;
-    if (row >= a.rows) return;
-    float peak = -INFINITY, sum = 0.0f;
-    for (int i = lane; i < a.splits; i += 64) {
-        const float2 part = a.partial[row * a.splits + i];
-        const float p = fmaxf(peak, part.x);
-        sum = rescale(sum, peak, p, a.c) + rescale(part.y, part.x, p, a.c);
-        peak = p;
-    }
-    const float top = wave_max(peak);
-    sum = wave_sum(rescale(sum, peak, top, a.c));
-    const WaveEntries w = wave_entries(a.teacher, row, names[wave], probs[wave]);
-    keep_entries(a.teacher, row, w);
-    const T* z = static_cast<const T*>(a.logits) + row * a.stride;
-    float logits[kEntriesPerLane];
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + wave;
+    if (row < a.rows) {
+        float peak = -INFINITY, sum = 0.0f;
+        for (int i = lane; i < a.splits; i += 64) {
+            const float2 part = a.partial[row * a.splits + i];
+            merge(peak, sum, part.x, part.y, a.c);
+        }
+        const float top = wave_max(peak);
+        sum = wave_sum(rescale(sum, peak, top, a.c));
+        const WaveEntries w = wave_entries(a.teacher, row, names[wave], probs[wave]);
+        keep_entries(a.teacher, row, w);
+        const T* z = static_cast<const T*>(a.logits) + row * a.stride;
+        float logits[kEntriesPerLane];
 #pragma unroll
-    for (int i = 0; i < kEntriesPerLane; ++i) logits[i] = w.index[i] >= 0 ? Vec<T>::get(z[w.index[i]]) : 0.0f;
-    const RowResult r = row_result(a.teacher, w, logits, top, sum);
-    if (lane == 0) {
-        a.state[row] = r.state;
-        a.row_loss[row] = r.loss;
+        for (int i = 0; i < kEntriesPerLane; ++i) logits[i] = w.index[i] >= 0 ? Vec<T>::get(z[w.index[i]]) : 0.0f;
+        const RowResult r = row_result(a.teacher, w, logits, top, sum);
+        if (lane == 0) {
+            a.state[row] = r.state;
+            hand_over(a.row_loss, a.rows, row, r.loss, counts(r.state));
+            if (a.reduction == JABAS_LOSS_NONE) a.loss_out[row] = r.loss;
+        }
     }
+    stores_done();
+    __syncthreads();
+    if (threadIdx.x == 0) done = __hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (done + 1 != gridDim.x) return;
+    double loss = 0.0, number = 0.0;
+    for (int64_t i = threadIdx.x; i < a.rows; i += kThreads) {
+        loss += handed_over(a.row_loss + i);
+        number += handed_over(a.row_loss + a.rows + i);
+    }
+    loss = group_sum<kWaves>(loss);
+    number = group_sum<kWaves>(number);
+    if (threadIdx.x == 0) finish(loss, number, a.reduction, a.loss_out, a.reduce_out);
 }
 
 template <class T, bool STREAM>
@@ -806,7 +830,10 @@ int launch_zero(void* p, size_t bytes, hipStream_t stream) {
 template <class T, bool STREAM>
 static int topk_forward(const TopkArgs& a, hipStream_t stream) {
     const size_t lds = static_cast<size_t>((a.chunk + 31) / 32) * 4;
-    if (a.splits == 1) return launch_with(lds, topk_row_kernel<T, STREAM>, static_cast<unsigned>(a.rows), kThreads, stream, a);
+    if (a.splits == 1) {
+        const int status = launch_with(lds, topk_row_kernel<T, STREAM>, static_cast<unsigned>(a.rows), kThreads, stream, a);
+        return status != JABAS_OK ? status : launch_reduce(a.row_loss, a.state, a.rows, a.reduction, a.loss_out, a.reduce_out, stream);
+    }
     const int status = launch_with(lds, topk_split_kernel<T, STREAM>, static_cast<unsigned>(a.rows * a.splits), kThreads, stream, a);
     return status != JABAS_OK ? status : launch(topk_join_kernel<T>, static_cast<unsigned>((a.rows + kThreads / 64 - 1) / (kThreads / 64)), kThreads, stream, a);
 }
