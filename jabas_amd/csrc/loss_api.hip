@@ -94,7 +94,7 @@ constexpr int64_t kPieceBytes[2] = {int64_t{256} << 20, int64_t{768} << 20};
 int64_t piece_tokens(const JabasLoss* l, const Shape& s, bool backward) {
     int64_t per_token = 0;
     if (s.copy_w) per_token += s.depth * 2 * s.planes;
-    if (backward) per_token += (round_up(l->rows, kDepth) + s.depth) * 2 * s.planes;     // dz and the weight in fp16
+    if (backward) per_token += (round_up(l->rows, kDepth) + (s.planes == 1 ? s.depth : 0)) * 2 * s.planes;     // dz, bf16's weight in fp16
     if (!per_token) return round_up(l->vocab, kTile);
     int64_t n = kPieceBytes[s.planes - 1] / per_token / kTile * kTile;
     if (n < 4 * kTile) n = 4 * kTile;
@@ -221,7 +221,7 @@ size_t carve_backward(const JabasLoss* l, const Shape& s, char* base, Backward& 
     b.unscale_w16 = c.take<float>(1);
     b.parts = c.take<float>(kMaxParts);
     b.x16 = c.take<uint16_t>(l->width * b.pad_rows * s.planes);
-    b.w16 = c.take<uint16_t>(l->width * b.piece * s.planes);
+    if (s.planes == 1) b.w16 = c.take<uint16_t>(l->width * b.piece);
     b.dz = c.take<uint16_t>(b.pad_rows * b.piece * s.planes);
     b.part_stride = round_up(l->width, 4);
     const int64_t tokens = b.piece < l->vocab ? b.piece : l->vocab;
@@ -295,8 +295,10 @@ int lay_x(const JabasLoss* l, const Shape& s, const Live& live, void* zero, uint
     return launch_lay_rows(a, stream);
 }
 
-// The weight's rows of a piece.
-int lay_w(const JabasLoss* l, const Shape& s, int64_t first, int64_t n, int64_t piece, uint16_t* w, float* unscale, Operand& out, hipStream_t stream) {
+// The weight's rows of a piece. `parts`: two planes with one scale for all, fit for a product that sums over the tokens too: those that the
+// bias rules out are zeros, and as many more as make whole steps.
+int lay_w(const JabasLoss* l, const Shape& s, int64_t first, int64_t n, int64_t piece, uint16_t* w, float* unscale, float* parts, float* unscale_all,
+          Operand& out, hipStream_t stream) {
     out.rows = static_cast<int32_t>(n);
     if (!s.copy_w) {
         out.p = at(l->weight, first * l->weight_stride, l->dtype);
@@ -316,6 +318,12 @@ int lay_w(const JabasLoss* l, const Shape& s, int64_t first, int64_t n, int64_t 
     a.pad = static_cast<int32_t>(s.depth);
     a.planes = s.planes == 2 ? 2 : 0;
     a.unscale = unscale;
+    if (parts) {
+        a.parts = parts;
+        a.unscale_all = unscale_all;
+        a.row_mask = l->bias ? at(l->bias, first, l->dtype) : nullptr;
+        a.pad_rows = static_cast<int32_t>(round_up(n, kDepth));
+    }
     out.p = w;
     out.stride = a.out_stride;
     out.plane = a.out_plane;
@@ -400,7 +408,7 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
         a.entry_logit = f.entry_logit;
         for (int64_t first = 0; first < l->vocab; first += f.piece) {
             const int64_t n = l->vocab - first < f.piece ? l->vocab - first : f.piece;
-            JABAS_TRY(lay_w(l, s, first, n, f.piece, f.w, f.unscale_w, a.w, stream));
+            JABAS_TRY(lay_w(l, s, first, n, f.piece, f.w, f.unscale_w, nullptr, nullptr, a.w, stream));
             a.first = static_cast<int32_t>(first);
             JABAS_TRY(launch_logits_forward(a, s.planes, f.large, stream));
         }
@@ -603,7 +611,7 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     for (int64_t first = 0; first < l->vocab; first += b.piece) {
         const int64_t n = l->vocab - first < b.piece ? l->vocab - first : b.piece;
         const int32_t pad = static_cast<int32_t>(round_up(n, kDepth));
-        JABAS_TRY(lay_w(l, s, first, n, b.piece, b.w, b.unscale_w, a.w, stream));
+        JABAS_TRY(lay_w(l, s, first, n, b.piece, b.w, b.unscale_w, s.planes == 2 && d_hidden ? b.parts : nullptr, b.unscale_w16, a.w, stream));
         a.first = static_cast<int32_t>(first);
         a.pad_tokens = pad;
         JABAS_TRY(launch_logits_backward(a, s.planes, b.large, stream));
@@ -626,12 +634,16 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
             g.w.out_aligned = width % 4 == 0 && !misaligned(g.w.out, 4 * bytes);
         }
         if (d_hidden) {     // sum over the tokens of dz[row][token] w[token][feature]
-            lay.in = at(l->weight, first * l->weight_stride, l->dtype);
-            lay.rows = static_cast<int32_t>(n);
-            lay.row_mask = l->bias ? at(l->bias, first, l->dtype) : nullptr;
-            lay.pad = pad;
-            JABAS_TRY(launch_lay_columns(lay, stream));
-            g.h.a = Operand{b.w16, b.piece, l->width * b.piece, width};
+            if (s.planes == 1) {
+                lay.in = at(l->weight, first * l->weight_stride, l->dtype);
+                lay.rows = static_cast<int32_t>(n);
+                lay.row_mask = l->bias ? at(l->bias, first, l->dtype) : nullptr;
+                lay.pad = pad;
+                JABAS_TRY(launch_lay_columns(lay, stream));
+                g.h.a = Operand{b.w16, b.piece, 0, width};
+            } else {            // as it lies for the logits
+                g.h.a = Operand{a.w.p, a.w.stride, a.w.plane, static_cast<int32_t>(s.depth)};
+            }
             g.h.b = Operand{b.dz, a.dz_stride, a.dz_plane, rows};
             g.h.m = width;
             g.h.n = rows;

@@ -46,7 +46,7 @@ struct BF16 {
 // register outputs, and the wait in front of the barrier covers them.
 template <class E, int P, int TM, int TN, int WM, int WN, bool TA, bool TB, bool RAISED>
 struct Core {
-    static constexpr bool kTb = TB;
+    static constexpr bool kTa = TA, kTb = TB;
     static constexpr int kM = TM, kN = TN, kThreads = 64 * WM * WN;
     static constexpr int kI = TM / WM / 32, kJ = TN / WN / 32;
     static constexpr int kBytesA = TM * 128, kBytesB = TN * 128, kStage = kBytesA + kBytesB;

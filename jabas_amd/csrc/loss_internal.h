@@ -136,7 +136,9 @@ struct LayArgs {
     int32_t planes;             // 0: copied as they are; 1 or 2 planes of fp16
     void* zero;                 // launch_lay_rows: [row of the call][cols] of in_dtype whose rows that do not count are zeroed, or NULL
     float* unscale;             // written: a factor per row (launch_lay_rows, planes > 0) or one for all (launch_lay_columns)
-    float* parts;               // launch_lay_columns: kMaxParts partial maxima
+    float* parts;               // kMaxParts partial maxima; launch_lay_rows: NULL, or one scale for all rows, written to unscale_all too
+    float* unscale_all;
+    int32_t pad_rows;           // launch_lay_rows with parts: places from rows to here become zeros
 };
 int launch_lay_rows(const LayArgs& a, hipStream_t stream);
 int launch_lay_columns(const LayArgs& a, hipStream_t stream);

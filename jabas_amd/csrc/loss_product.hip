@@ -430,7 +430,7 @@ __device__ inline void run_job(const Job& a, int unit, char* smem) {
     const int m0 = tm * C::kM, n0 = tn * C::kN, lane = threadIdx.x & 63;
     Operand x = a.a, y = a.b;
     const int k0 = split * a.each;
-    x.p = static_cast<const uint16_t*>(x.p) + k0;
+    x.p = static_cast<const uint16_t*>(x.p) + (C::kTa ? k0 * x.stride : k0);
     y.p = static_cast<const uint16_t*>(y.p) + (C::kTb ? k0 * y.stride : k0);
     if (a.live_n) y.rows = n_here;
     C c;
@@ -530,7 +530,7 @@ int logits(const LogitsArgs& a, int planes, bool large, bool backward, hipStream
 template <int P, int TM, int TN, int WM, int WN>
 int grads(const GradArgs& a, hipStream_t stream) {
     using CW = Core<F16, P, TM, TN, WM, WN, false, true, P == 2>;
-    using CH = Core<F16, P, TM, TN, WM, WN, false, false, P == 2>;
+    using CH = Core<F16, P, TM, TN, WM, WN, P == 2, false, P == 2>;
     const int64_t grid = static_cast<int64_t>(tiles_m<CW>(a.w.m)) * tiles_n<CW>(a.w.n) * a.w.splits + static_cast<int64_t>(tiles_m<CH>(a.h.m)) * tiles_n<CH>(a.h.n) * a.h.splits;
     return launch(grads_kernel<CW, CH>, grid, CW::kThreads, a, stream);
 }
@@ -651,8 +651,8 @@ namespace {
 
 constexpr int kLayThreads = 256;
 
-// The power of two that takes `peak` to [2^14, 2^15): both planes of an element then fit fp16, and elements down to
-// 2^-24 of the largest keep 22 bits.
+// The power of two that takes `peak` to [2^14, 2^15): both planes of an element then fit fp16, elements down to 2^-16
+// of the largest keep 22 bits, and smaller ones are off by 2^-40 of it at most.
 __device__ inline int scale_exponent(float peak) {
     if (!(peak > 0.0f)) return 0;
     int e = static_cast<int>((__float_as_uint(peak) >> 23) & 0xff) - 126;
@@ -714,9 +714,37 @@ __device__ inline float row_keeps(const LayArgs& a, int row) {
 __device__ inline int rows_of(const LayArgs& a) { return a.live.live ? *a.live.live : a.rows; }
 __device__ inline int row_of(const LayArgs& a, int r) { return a.live.map ? a.live.map[r] : r; }
 
-// One wave per row: padded, and scaled by the row's own power of two.
+// The largest of the partial maxima, for every thread of the workgroup.
+__device__ inline float join_parts(const float* parts) {
+    __shared__ float merge[kLayThreads / 64];
+    static_assert(kMaxParts % kLayThreads == 0, "as many partial maxima per thread");
+    float peak = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMaxParts; i += kLayThreads) peak = fmaxf(peak, parts[i + threadIdx.x]);
+    peak = wave_max(peak);
+    if ((threadIdx.x & 63) == 0) merge[threadIdx.x >> 6] = peak;
+    __syncthreads();
+    return fmaxf(fmaxf(merge[0], merge[1]), fmaxf(merge[2], merge[3]));
+}
+
+// One wave per row: padded, and scaled by the row's own power of two, or all by one.
 __global__ __launch_bounds__(kLayThreads) void lay_rows_kernel(LayArgs a) {
     const int place = blockIdx.x * (kLayThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (a.parts) {
+        const int e = scale_exponent(join_parts(a.parts));
+        if (place >= a.pad_rows) return;
+        const float scale = place < a.rows ? row_keeps(a, place) * power_of_two(e) : 0.0f;
+        float v[8];
+        for (int c = lane * 8; c < a.pad; c += 512) {
+            if (scale != 0.0f) load_eight(a, place, c, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = scale != 0.0f ? v[i] * scale : 0.0f;
+            store_eight(a, place, c, v);
+        }
+        if (lane == 0 && place < a.rows) a.unscale[place] = power_of_two(-e);
+        if (lane == 0 && place == 0) *a.unscale_all = power_of_two(-e);
+        return;
+    }
     if (place >= a.rows) return;
     const int row = row_of(a, place);
     if (place >= rows_of(a)) {
@@ -781,13 +809,10 @@ __global__ __launch_bounds__(kLayThreads) void absmax_kernel(LayArgs a) {
 
 // 64 x 64 elements through LDS: out[col][row], one scale for all of them.
 __global__ __launch_bounds__(kLayThreads) void lay_columns_kernel(LayArgs a) {
-    __shared__ float merge[kLayThreads / 64], tile[64][65];
-    static_assert(kMaxParts % kLayThreads == 0, "as many partial maxima per thread");
+    __shared__ float tile[64][65];
     const int t = threadIdx.x, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, rows = rows_of(a), pad = (rows + 63) / 64 * 64;
     if (r0 >= pad && r0) return;        // the first writes the scale, whatever there is to lay out
-    float peak = 0.0f, v[8];
-#pragma unroll
-    for (int i = 0; i < kMaxParts; i += kLayThreads) peak = fmaxf(peak, a.parts[i + t]);
+    float v[8];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int r = x * 32 + (t >> 3), c = (t & 7) * 8;
@@ -797,11 +822,7 @@ __global__ __launch_bounds__(kLayThreads) void lay_columns_kernel(LayArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) tile[r][c + i] = f != 0.0f ? v[i] * f : 0.0f;
     }
-    peak = wave_max(peak);
-    if ((t & 63) == 0) merge[t >> 6] = peak;
-    __syncthreads();
-    peak = fmaxf(fmaxf(merge[0], merge[1]), fmaxf(merge[2], merge[3]));
-    const int e = scale_exponent(peak);
+    const int e = scale_exponent(join_parts(a.parts));      // its barrier stands behind the writes of `tile` too
     const float scale = power_of_two(e);
     if (t == 0 && blockIdx.x == 0 && blockIdx.y == 0) *a.unscale = power_of_two(-e);
 #pragma unroll
@@ -817,7 +838,9 @@ __global__ __launch_bounds__(kLayThreads) void lay_columns_kernel(LayArgs a) {
 }  // namespace
 
 int launch_lay_rows(const LayArgs& a, hipStream_t stream) {
-    return launch(lay_rows_kernel, (a.rows + 3) / 4, kLayThreads, a, stream);
+    if (!a.parts) return launch(lay_rows_kernel, (a.rows + 3) / 4, kLayThreads, a, stream);
+    const int status = launch(absmax_kernel, kMaxParts, kLayThreads, a, stream);
+    return status != JABAS_OK ? status : launch(lay_rows_kernel, (a.pad_rows + 3) / 4, kLayThreads, a, stream);
 }
 
 int launch_lay_columns(const LayArgs& a, hipStream_t stream) {
