@@ -393,6 +393,7 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
         live.ticket = f.ticket;
         live.state = state;
         live.row_loss = f.row_loss;
+        live.down = reduce + 1;
         JABAS_TRY(launch_live(live, stream));
         a.rows = Live{f.map, f.live};
         JABAS_TRY(lay_x(l, s, a.rows, nullptr, f.x, f.unscale_x, a.x, stream));
@@ -563,6 +564,7 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     a.entries = entries_of(l, s);
     a.state = state;
     a.row_grad = b.grad;
+    a.down = reduce + 1;
     a.uniform = uniform;
     a.hit = hit;
     a.dz = d_hidden || d_weight ? b.dz : nullptr;

@@ -24,7 +24,9 @@ static_assert(sizeof(RowState) == 16, "a row's state is one 16-byte load");
 
 // The row gradients dz travel between kernels as fp16 in units of 2^-15: |dz| <= 1 in units of upstream * T, so the range
 // is used to the top and the smallest steps are 2^-39. Three more bits than bf16 at the same matrix rate; fp32 calls carry a
-// second plane with 2^11 times what the first leaves: 22 bits down to 2^-25, smallest steps of 2^-50.
+// second plane with 2^11 times what the first leaves: 22 bits down to 2^-25, smallest steps of 2^-50. Where a row's probabilities sum
+// to more than 1 (a teacher_lse below its entries', a token named often) |dz| is as much larger: then a power of two, `down`, takes
+// all rows' dz into the range, and their gradients carry its inverse.
 constexpr float kDzScale = 32768.0f, kLowScale = 2048.0f;
 
 constexpr int kTile = 256;      // the largest output tile of a product; pieces of the vocabulary are whole ones
@@ -75,6 +77,7 @@ struct LogitsArgs {
     // backward
     const RowState* state;
     const float* row_grad;      // gradient of row n in units of dz (bias gradient)
+    const float* down;          // see kDzScale
     float uniform;              // e / V
     float hit;                  // what a label takes off: 1 - e
     void* dz;                   // [row that counts][token of the piece], fp16 planes, or NULL
@@ -194,15 +197,16 @@ struct LiveArgs {
     uint32_t* ticket;           // set to 0
     RowState* state;
     float* row_loss;
+    float* down;                // written: see kDzScale
 };
 int launch_live(const LiveArgs& a, hipStream_t stream);
 
-// grad[n] = upstream * T * reduce[0] (0 for rows that do not count), ratio[n] = grad[n] / *peak, *peak the largest |grad|, and which rows
+// grad[n] = upstream * T * reduce[0] / reduce[1] (0 for rows that do not count), ratio[n] = grad[n] / *peak, *peak the largest |grad|, and which rows
 // count, from their states.
 struct RowGradArgs {
     const float* upstream;
     int32_t per_row;
-    const float* reduce;
+    const float* reduce;        // the share of a row, the factor of dz
     float t;
     const RowState* state;
     int64_t rows;

@@ -265,14 +265,14 @@ __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs
         }
     });
     if (TEACHER) build_map<C>(a.entries, a.rows.map, smem, a.first + m0, n0, rows);
-    const float uniform = a.uniform * kDzScale;
+    const float scale = kDzScale * *a.down, uniform = a.uniform * scale;
 #pragma unroll
     for (int j = 0; j < C::kJ; ++j) {
         keep_order();
         const int nl = wn + j * 32 + (lane & 31), n = row[j];
         const RowState st = n >= 0 ? a.state[n] : RowState{0.0f, 0.0f, 0.0f, 0.0f};
         const bool counts = !(st.slope == 0.0f && st.mass == 0.0f);
-        const float slope = st.slope * kDzScale;
+        const float slope = st.slope * scale;
 #pragma unroll
         for (int i = 0; i < C::kI; ++i) {
             if (P == 2) keep_order();
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs
                         const uint32_t hit = (hits >> (8 * e)) & 0xff;
                         if (hit)
                             d[e] = (st.mass * __builtin_amdgcn_exp2f((z.v[i][j][q * 4 + e] - st.peak) * a.c) -
-                                    a.entries.p[static_cast<int64_t>(n) * a.entries.k + hit - 1]) * kDzScale;
+                                    a.entries.p[static_cast<int64_t>(n) * a.entries.k + hit - 1]) * scale;
                     }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs
                 }
             }
         }
-        if (!TEACHER) at_label<C>(label[j], [&](int i, int e) { z.v[i][j][e] -= a.hit * kDzScale; });
+        if (!TEACHER) at_label<C>(label[j], [&](int i, int e) { z.v[i][j][e] -= a.hit * scale; });
         if (__any(!counts)) {
 #pragma unroll
             for (int i = 0; i < C::kI; ++i)

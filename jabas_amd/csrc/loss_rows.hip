@@ -456,17 +456,30 @@ __global__ __launch_bounds__(kJoinThreads) void live_kernel(LiveArgs a) {
         }
         return is;
     };
+    float mass = 0.0f;
     if (a.teacher_row)
-        list_live(a.rows, a.map, a.live, [&](int64_t n) { return a.teacher_row[n].z; }, [&](int64_t n, float z) { return drop(n, z != 0.0f); });
+        list_live(a.rows, a.map, a.live, [&](int64_t n) { return a.teacher_row[n]; }, [&](int64_t n, const float4& t) {
+            mass = fmaxf(mass, t.x);
+            return drop(n, t.z != 0.0f);
+        });
     else
         list_live(a.rows, a.map, a.live, [&](int64_t n) { return a.target[n]; }, [&](int64_t n, int64_t label) { return drop(n, label != a.ignore_index); });
+    __shared__ float masses[kJoinWaves];
+    mass = wave_max(mass);
+    if ((threadIdx.x & 63) == 0) masses[threadIdx.x >> 6] = mass;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int i = 1; i < kJoinWaves; ++i) mass = fmaxf(mass, masses[i]);
+    float down = 1.0f;          // fp16 holds up to 2 in units of dz; a row whose own sum is not finite is NaN by itself
+    while (mass * down > 1.9f && down > 0x1p-100f) down *= 0.5f;
+    *a.down = down;
 }
 
 __global__ __launch_bounds__(kJoinThreads) void row_grad_kernel(RowGradArgs a) {
     __shared__ float peaks[kJoinWaves];
     float top = 0.0f;
     bool bad = false;
-    const float share = *a.reduce * a.t;
+    const float share = a.reduce[0] * a.t / a.reduce[1];
     struct Row {
         RowState state;
         float upstream;

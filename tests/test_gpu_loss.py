@@ -527,6 +527,30 @@ def test_tokens_named_twice_are_one_event(gpu, tail):
     Reference(logits=z, index=index, teacher=teacher, lse=lse).check(loss, _grads(loss, (z,)), "fp32")
 
 
+@pytest.mark.parametrize("rows", [20, 80, 300])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("why", ["low_lse", "one_token_often"])
+def test_probabilities_that_sum_to_more_than_one(gpu, dtype, rows, why):
+    """A teacher_lse below its entries' own, or one token named in many places: the formula holds, with the sum far above 1 in some rows."""
+    vocab, width, k = 22001, 64, 40
+    (x, w, b), gen = _inputs(gpu, rows, vocab, width, dtype, True, seed=rows)
+    index = torch.randint(0, vocab // k, (rows, k), generator=gen) + torch.arange(k) * (vocab // k)
+    teacher = (torch.randn(rows, k, generator=gen) * 2).to(TYPES[dtype])
+    lse = torch.logsumexp(teacher.float(), 1) + 0.5
+    if why == "low_lse":
+        lse[::5] -= 6.0
+    else:
+        index[3::7] = 11
+        teacher[3::7] = 4.0
+        lse[3::7] = 4.2
+    index[1] = -1
+    loss = losses.linear_topk_distillation(x, w, index.to(gpu), teacher.to(gpu), b, teacher_lse=lse.to(gpu))
+    Reference(x, w, b, index=index, teacher=teacher, lse=lse).check(loss, _grads(loss, (x, w, b)), dtype)
+    z = (x.detach().float() @ w.detach().float().t()).to(TYPES[dtype]).requires_grad_(True)
+    loss = losses.topk_distillation(z, index.to(gpu), teacher.to(gpu), teacher_lse=lse.to(gpu))
+    Reference(logits=z, index=index, teacher=teacher, lse=lse).check(loss, _grads(loss, (z,)), dtype)
+
+
 def test_entries_far_above_the_rest(gpu):
     """The student's rest is e^-200 of its row: the slope of the other tokens is still finite and right."""
     z = torch.zeros(1, 1000)
