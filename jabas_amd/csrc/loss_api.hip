@@ -19,8 +19,8 @@ inline int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; 
 inline int64_t tiles(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
 inline size_t element_bytes(int dtype) { return dtype == JABAS_F32 ? 4 : 2; }
 
-// Tokens whose row gradients are kept at once, in fp32: 32 MiB at most. 32 x 262144 x 1024 with 2^14, 2^16, 2^17 and 2^18: fp32 1684, 1435,
-// 1455 and 1426 us, bf16 1321, 1120, 1121 and 1160.
+// Tokens whose row gradients are kept at once: 64 MiB at most. 32 x 262144 x 1024 fp32 with 2^14, 2^16, 2^17 and 2^18: 1684, 1435, 1455 and
+// 1426 us.
 constexpr int64_t kNarrowPiece = int64_t{1} << 17;
 
 struct Shape {
@@ -201,7 +201,7 @@ size_t carve_backward(const JabasLoss* l, const Shape& s, char* base, Backward& 
     if (s.narrow) {
         b.piece = l->vocab < kNarrowPiece ? l->vocab : kNarrowPiece;
         b.narrow = narrow_splits(b.piece, l->width);
-        b.narrow_dz = c.take<float>((rows <= 32 ? 32 : 64) * narrow_tiles(b.piece) * 32);
+        b.narrow_dz = c.take<float>((rows <= 32 ? 32 : 64) * narrow_tiles(b.piece) * 32 * (s.planes == 1 ? 2 : 1));
         b.part_stride = round_up(l->width, 4);
         if (b.narrow.n > 1 || b.piece < l->vocab) b.part_h = c.take<float>(b.narrow.n * rows * b.part_stride);
         return c.all();
@@ -519,7 +519,7 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
         a.part_plane = l->rows * b.part_stride;
         for (a.first = 0; a.first < l->vocab; a.first += b.piece) {
             a.tokens = l->vocab - a.first < b.piece ? l->vocab - a.first : b.piece;
-            a.hidden_units = d_hidden ? (l->width + 127) / 128 * ((a.tokens + a.each - 1) / a.each) : 0;
+            a.hidden_units = d_hidden ? tiles(l->width, 128) * tiles(a.tokens, a.each) : 0;
             a.add = a.first > 0;        // a shorter last piece adds to the first of the splits
             JABAS_TRY(launch_narrow_backward(a, l->dtype, stream));
             if (a.dz) JABAS_TRY(launch_narrow_grads(a, l->dtype, stream));

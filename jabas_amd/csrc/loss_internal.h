@@ -219,12 +219,13 @@ int launch_row_grad(const RowGradArgs& a, hipStream_t stream);
 int launch_bias_sum(const float* parts, const int32_t* live, int32_t tile, int64_t stride, int64_t n, void* out, int32_t dtype, hipStream_t stream);
 int launch_zero(void* p, size_t bytes, hipStream_t stream);
 
-// Few rows, hidden states and weight as they lie (loss_narrow.hip): their gradients' products are fp32's, which with one plane is slower
-// than laying the weight out for tiles as rows and weight grow. Forward and backward, this and the tiles: fp32 16 x 32317 x 1024 178 and
-// 434 us, 64 x 32317 x 1024 396 and 457, 64 x 131072 x 4096 4387 and 8716; bf16 1 x 32317 x 1024 132 and 166, 32 x 32317 x 1024 168 and 175,
-// 33 x 4000 x 768 74 and 89, 64 x 4000 x 768 89 and 89, 64 x 8000 x 768 121 and 97, 64 x 32317 x 1024 348 and 178.
+// Few rows, hidden states and weight as they lie (loss_narrow.hip). With bf16, whose tiles read the weight as it lies too, a second block
+// of rows pays for small weights only. Forward and backward, this and the tiles: fp32 16 x 32317 x 1024 170 and 434 us, 64 x 32317 x 1024 380
+// and 457, 64 x 131072 x 4096 4387 and 8716; bf16 1 x 32317 x 1024 107 and 171, 32 x 32317 x 1024 119 and 176, 32 x 131072 x 4096 1225 and
+// 2070, 64 x 4000 x 768 72 and 89, 64 x 8000 x 768 76 and 101, 33 x 16000 x 768 106 and 115, 64 x 16000 x 768 117 and 117,
+// 40 x 32317 x 1024 188 and 176, 64 x 32317 x 1024 209 and 177.
 constexpr int kNarrowRows = 64;
-constexpr int64_t kNarrowWeight = int64_t{3} << 20;
+constexpr int64_t kNarrowWeight = int64_t{12} << 20;       // elements of the weight
 struct NarrowArgs {
     const void *x, *w, *bias;
     int64_t x_stride, w_stride, vocab;
@@ -243,7 +244,7 @@ struct NarrowArgs {
     const float* reduce;
     float t;
     float uniform, hit;
-    float* dz;                  // [32 or 64 rows][dz_stride tokens], in the units of the result, or NULL
+    float* dz;                  // [32 or 64 rows][dz_stride tokens], in the units of the result, or NULL; bf16: two planes, and once more by tokens
     int64_t dz_stride;          // the tokens in whole tiles
     void* d_bias;
     void* d_weight;

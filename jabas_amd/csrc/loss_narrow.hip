@@ -6,8 +6,13 @@
 // token r: which elements of the inner axis meet in one matrix instruction is free as long as both operands agree, so each lane reads
 // whole 64 or 128 bytes. bf16 through 32x32x16, fp32 through 32x32x2: its rate (16 bytes of weight per clock and CU at 32 rows) is above
 // what memory gives.
-// Gradients: dz in fp32, in the units of the result, so that the row gradients are exact whatever their size. Its products take
-// 32x32x2 for both types: a lane holds one element of the inner axis, so operands whose rows are that axis need no transposing.
+// It takes 21 us for 66 MB of weight and one row (3.2 TB/s), 280 us for 1.07 GB and eight (3.8 TB/s): a load of a wave touches 32 rows, and
+// what it would take to load whole lines through LDS gives a tenth at most.
+// Gradients: dz in the units of the result, fp32, or for bf16 two bf16 planes (16 bits, where the results have 8), so that the row
+// gradients keep their bits whatever their size. fp32's products take 32x32x2, whose lane holds one element of the inner axis, so that
+// operands whose rows are that axis need no transposing; bf16's take 32x32x16 with four features of eight rows turned about in a lane's
+// registers. 8 rows, 131072 x 4096: dX 230 us with bf16 (4.7 TB/s), 525 with fp32 (4.1 TB/s), dW 300 and 457 us; with 32x32x2 and checked
+// loads for bf16 too both took 1081 us, 546 now. What bounds them is how much a CU has on its way: two workgroups' registers fill it.
 #include "loss_internal.h"
 
 namespace jabas {
@@ -184,6 +189,20 @@ __global__ __launch_bounds__(kThreads) void narrow_forward_kernel(NarrowArgs a) 
     if (a.total) a.total[tile] = t;
 }
 
+// bf16 calls: dz as two bf16 planes, [plane][row][token] for dX and [plane][token][row] for dW.
+template <int R>
+struct Planes {
+    uint16_t *rows, *tokens;
+    int64_t plane;
+    __device__ explicit Planes(const NarrowArgs& a) : rows(reinterpret_cast<uint16_t*>(a.dz)), plane(R * a.dz_stride) { tokens = rows + 2 * plane; }
+};
+// x in 16 bits, and what that leaves in the upper half.
+__device__ inline uint32_t split(float x) {
+    const uint32_t hi = to_bf16(x);
+    const float left = x - widen<uint16_t>(static_cast<uint16_t>(hi));
+    return hi | (fabsf(left) < INFINITY ? static_cast<uint32_t>(to_bf16(left)) << 16 : 0);      // not finite: the first plane says it
+}
+
 // The row gradient of n; 0 for rows that do not count.
 __device__ inline float row_gradient(const NarrowArgs& a, int n) {
     if (n >= a.rows) return 0.0f;
@@ -228,9 +247,25 @@ __global__ __launch_bounds__(kThreads) void narrow_backward_kernel(NarrowArgs a)
         static_cast<T*>(a.d_bias)[first + threadIdx.x] = narrow<T>(s);
     }
     if (!a.dz) return;
-    for (int i = threadIdx.x; i < R * kTokens; i += kThreads) {
-        const int n = i / kTokens, m = i % kTokens;
-        a.dz[n * a.dz_stride + from + m] = ds[n][m];
+    if constexpr (sizeof(T) == 2) {
+        Planes<R> p(a);
+        for (int i = threadIdx.x; i < R * kTokens; i += kThreads) {
+            const int n = i / kTokens, m = i % kTokens;
+            const uint32_t v = split(ds[n][m]);
+            p.rows[n * a.dz_stride + from + m] = static_cast<uint16_t>(v);
+            p.rows[p.plane + n * a.dz_stride + from + m] = static_cast<uint16_t>(v >> 16);
+        }
+        for (int i = threadIdx.x; i < R * kTokens; i += kThreads) {
+            const int m = i / R, n = i % R;
+            const uint32_t v = split(ds[n][m]);
+            p.tokens[(from + m) * R + n] = static_cast<uint16_t>(v);
+            p.tokens[p.plane + (from + m) * R + n] = static_cast<uint16_t>(v >> 16);
+        }
+    } else {
+        for (int i = threadIdx.x; i < R * kTokens; i += kThreads) {
+            const int n = i / kTokens, m = i % kTokens;
+            a.dz[n * a.dz_stride + from + m] = ds[n][m];
+        }
     }
 }
 
@@ -296,6 +331,174 @@ __device__ inline void narrow_weight(const NarrowArgs& a, int64_t unit) {
     }
 }
 
+// bf16's products take 32x32x16, whose operands hold eight elements of the inner axis a lane: F consecutive features of eight rows (of the
+// weight or of the hidden states), turned about in registers, are the operands of F columns of the result each.
+constexpr int F = 4;
+struct Turned {
+    uint32_t v[F][4];
+    __device__ explicit Turned(const Some<uint16_t, F> (&x)[8]) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            uint32_t even[F / 2], odd[F / 2];
+            __builtin_memcpy(even, &x[2 * p], 2 * F);
+            __builtin_memcpy(odd, &x[2 * p + 1], 2 * F);
+#pragma unroll
+            for (int c = 0; c < F; ++c) v[c][p] = __builtin_amdgcn_perm(odd[c / 2], even[c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+        }
+    }
+    __device__ bf16x8 operator[](int c) const {
+        bf16x8 x;
+        __builtin_memcpy(&x, v[c], 16);
+        return x;
+    }
+};
+__device__ inline Some<uint16_t, F> load_some(const uint16_t* row, int c, int cols) {
+    if (c + F <= cols) return *reinterpret_cast<const Some<uint16_t, F>*>(row + c);
+    Some<uint16_t, F> x;
+#pragma unroll
+    for (int i = 0; i < F; ++i) x.v[i] = c + i < cols ? row[c + i] : 0;
+    return x;
+}
+__device__ inline bf16x8 load_eight(const uint16_t* p) { return *reinterpret_cast<const bf16x8*>(p); }
+
+// dW of 32 tokens: the rows are the inner axis, 16 at a time; the waves take 32 F features in turn.
+template <int RB>
+__device__ inline void narrow_weight_bf16(const NarrowArgs& a, int64_t unit) {
+    constexpr int R = RB * 32;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, half = lane >> 5;
+    const int64_t from = unit * kTokens, first = a.first + from;
+    const Planes<R> p(a);
+    bf16x8 d[R / 16][2];
+#pragma unroll
+    for (int k = 0; k < R / 16; ++k)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) d[k][q] = load_eight(p.tokens + q * p.plane + (from + r) * R + k * 16 + half * 8);
+    const uint64_t live = __ballot(row_gradient(a, lane) != 0.0f);     // rows that count: the hidden states of others are zeros whatever they hold
+    for (int h = wave * 32 * F; h < a.width; h += 128 * F) {
+        const bool whole = h + 32 * F <= a.width;
+        f32x16 acc[F];
+#pragma unroll
+        for (int c = 0; c < F; ++c)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[c][e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < R / 16; ++k) {
+            if (k * 16 >= a.rows) break;
+            Some<uint16_t, F> x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint16_t* row = static_cast<const uint16_t*>(a.x) + static_cast<int64_t>(min(k * 16 + half * 8 + j, a.rows - 1)) * a.x_stride;
+                x[j] = whole ? *reinterpret_cast<const Some<uint16_t, F>*>(row + h + F * r) : load_some(row, h + F * r, a.width);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (!((live >> (k * 16 + half * 8 + j)) & 1)) x[j] = Some<uint16_t, F>{};
+            const Turned b(x);
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int c = 0; c < F; ++c) acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(d[k][q], b[c], acc[c], 0, 0, 0);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int64_t v = first + block_m(e);
+            if (v >= a.vocab) continue;
+            uint16_t* out = static_cast<uint16_t*>(a.d_weight) + v * a.width;
+            Some<uint16_t, F> y;
+#pragma unroll
+            for (int c = 0; c < F; ++c) y.v[c] = to_bf16(acc[c][e]);
+            if (h + F * r + F <= a.width) *reinterpret_cast<Some<uint16_t, F>*>(out + h + F * r) = y;
+            else
+#pragma unroll
+                for (int c = 0; c < F; ++c)
+                    if (h + F * r + c < a.width) out[h + F * r + c] = y.v[c];
+        }
+    }
+}
+
+// Four features of the sums of the workgroup's waves, a block of 32 rows: merge[wave - 1][32 rows][128], then to where they go.
+template <class T>
+__device__ inline void narrow_merge(const NarrowArgs& a, int b, int split, int feature, const f32x16& x, const f32x16& y, const f32x16& z, const f32x16& w, float* merge) {
+    const int wave = threadIdx.x >> 6, r = threadIdx.x & 31;
+    __syncthreads();
+    if (wave)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) *reinterpret_cast<f32x4*>(merge + ((wave - 1) * 32 + block_m(e)) * 128 + 4 * r) = f32x4{x[e], y[e], z[e], w[e]};
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const int m = block_m(e), n = b * 32 + m;
+        f32x4 v = {x[e], y[e], z[e], w[e]};
+#pragma unroll
+        for (int i = 0; i < 3; ++i) v += *reinterpret_cast<const f32x4*>(merge + (i * 32 + m) * 128 + 4 * r);
+        if (n >= a.rows) continue;
+        if (a.part) {
+            if (feature >= a.width) continue;
+            f32x4* sum = reinterpret_cast<f32x4*>(a.part + split * a.part_plane + n * a.part_stride + feature);
+            *sum = a.add ? *sum + v : v;
+        } else {
+            store_four(static_cast<T*>(a.d_hidden) + static_cast<int64_t>(n) * a.width, feature, a.width, v);
+        }
+    }
+}
+
+// dX of 32 F features over a range of tokens: 16 at a time; the waves take blocks of 32 tokens in turn.
+template <int RB>
+__device__ inline void narrow_hidden_bf16(const NarrowArgs& a, int64_t unit, float* merge) {
+    constexpr int R = RB * 32;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, half = lane >> 5;
+    const int slices = (a.width + 32 * F - 1) / (32 * F), h = static_cast<int>(unit % slices) * 32 * F, split = static_cast<int>(unit / slices);
+    const int64_t begin = split * a.each, end = min(begin + a.each, a.tokens);
+    const Planes<R> p(a);
+    f32x16 acc[RB][F];
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int c = 0; c < F; ++c)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[b][c][e] = 0.0f;
+    // Whole blocks and slices take their loads without a check, all at once.
+    const bool whole = h + 32 * F <= a.width && a.first + end <= a.vocab && end - begin == a.each;
+    for (int64_t v = begin + wave * 32; v < end; v += 128) {
+        Some<uint16_t, F> w[2][8];
+        const uint16_t* row = static_cast<const uint16_t*>(a.w) + (a.first + v + half * 8) * a.w_stride + h + F * r;
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j / 8][j % 8] = *reinterpret_cast<const Some<uint16_t, F>*>(row + (j / 8 * 16 + j % 8) * a.w_stride);
+        } else {
+#pragma unroll 1
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {       // tokens past the end: the last one again, against a zero of dz
+                    const int64_t at = min(a.first + v + s * 16 + half * 8 + j, a.vocab - 1);
+                    const Some<uint16_t, F> x = load_some(static_cast<const uint16_t*>(a.w) + at * a.w_stride, h + F * r, a.width);
+                    if (s) w[1][j] = x;
+                    else w[0][j] = x;
+                }
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            bf16x8 d[RB][2];
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) d[b][q] = load_eight(p.rows + q * p.plane + (b * 32 + r) * a.dz_stride + v + s * 16 + half * 8);
+            const Turned t(w[s]);
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int c = 0; c < F; ++c) acc[b][c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(d[b][q], t[c], acc[b][c], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int g = 0; g < F; g += 4) narrow_merge<uint16_t>(a, b, split, h + F * r + g, acc[b][g], acc[b][g + 1], acc[b][g + 2], acc[b][g + 3], merge);
+}
+
 // dX of 128 features over a range of tokens: eight at a time, four to each half of a wave; the waves take blocks of 32 tokens in turn.
 template <class T, int RB>
 __device__ inline void narrow_hidden(const NarrowArgs& a, int64_t unit, float* merge) {
@@ -309,15 +512,22 @@ __device__ inline void narrow_hidden(const NarrowArgs& a, int64_t unit, float* m
         for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[b][c][e] = 0.0f;
+    const bool whole = h + 128 <= a.width && a.first + end <= a.vocab && end - begin == a.each;
     for (int64_t v = begin + wave * 32; v < end; v += 128) {
         f32x4 d[4][RB], w[4][4];
+        const T* row = static_cast<const T*>(a.w) + (a.first + v + half * 4) * a.w_stride + h + 4 * r;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
 #pragma unroll
             for (int b = 0; b < RB; ++b) d[q][b] = *reinterpret_cast<const f32x4*>(a.dz + (b * 32 + r) * a.dz_stride + v + q * 8 + half * 4);
+            if (whole) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t)     // tokens past the end: the last one again, against a zero of dz
-                w[q][t] = load_four(static_cast<const T*>(a.w) + min(a.first + v + q * 8 + half * 4 + t, a.vocab - 1) * a.w_stride, h + 4 * r, a.width);
+                for (int t = 0; t < 4; ++t) w[q][t] = load_four(row + (q * 8 + t) * a.w_stride, 0, 4);
+            } else {
+#pragma unroll
+                for (int t = 0; t < 4; ++t)     // tokens past the end: the last one again, against a zero of dz
+                    w[q][t] = load_four(static_cast<const T*>(a.w) + min(a.first + v + q * 8 + half * 4 + t, a.vocab - 1) * a.w_stride, h + 4 * r, a.width);
+            }
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q)
@@ -328,39 +538,20 @@ __device__ inline void narrow_hidden(const NarrowArgs& a, int64_t unit, float* m
 #pragma unroll
                     for (int c = 0; c < 4; ++c) acc[b][c] = __builtin_amdgcn_mfma_f32_32x32x2f32(d[q][b][t], w[q][t][c], acc[b][c], 0, 0, 0);
     }
-    // the four waves' sums: merge[wave - 1][32 rows][128 features], one block of rows after the other
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-        __syncthreads();
-        if (wave)
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                *reinterpret_cast<f32x4*>(merge + ((wave - 1) * 32 + block_m(e)) * 128 + 4 * r) = f32x4{acc[b][0][e], acc[b][1][e], acc[b][2][e], acc[b][3][e]};
-        __syncthreads();
-        if (wave) continue;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int m = block_m(e), n = b * 32 + m;
-            f32x4 v = {acc[b][0][e], acc[b][1][e], acc[b][2][e], acc[b][3][e]};
-#pragma unroll
-            for (int i = 0; i < 3; ++i) v += *reinterpret_cast<const f32x4*>(merge + (i * 32 + m) * 128 + 4 * r);
-            if (n >= a.rows) continue;
-            if (a.part) {
-                if (h + 4 * r >= a.width) continue;
-                f32x4* sum = reinterpret_cast<f32x4*>(a.part + split * a.part_plane + n * a.part_stride + h + 4 * r);
-                *sum = a.add ? *sum + v : v;
-            } else {
-                store_four(static_cast<T*>(a.d_hidden) + static_cast<int64_t>(n) * a.width, h + 4 * r, a.width, v);
-            }
-        }
-    }
+    for (int b = 0; b < RB; ++b) narrow_merge<T>(a, b, split, h + 4 * r, acc[b][0], acc[b][1], acc[b][2], acc[b][3], merge);
 }
 
 template <class T, int RB>
-__global__ __launch_bounds__(kThreads) void narrow_grads_kernel(NarrowArgs a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void narrow_grads_kernel(NarrowArgs a) {
     __shared__ __align__(16) float merge[3 * 32 * 128];
-    if (blockIdx.x < a.hidden_units) narrow_hidden<T, RB>(a, blockIdx.x, merge);
-    else narrow_weight<T, RB>(a, blockIdx.x - a.hidden_units);
+    if constexpr (sizeof(T) == 2) {
+        if (blockIdx.x < a.hidden_units) narrow_hidden_bf16<RB>(a, blockIdx.x, merge);
+        else narrow_weight_bf16<RB>(a, blockIdx.x - a.hidden_units);
+    } else {
+        if (blockIdx.x < a.hidden_units) narrow_hidden<T, RB>(a, blockIdx.x, merge);
+        else narrow_weight<T, RB>(a, blockIdx.x - a.hidden_units);
+    }
 }
 
 template <class A>
@@ -383,14 +574,12 @@ int backward(const NarrowArgs& a, int64_t grid, hipStream_t stream) {
 
 int64_t narrow_tiles(int64_t vocab) { return (vocab + kTokens - 1) / kTokens; }
 
-// Token ranges of dX: 256 workgroups, one a CU beside those of dW, none with less than 128 tokens, a block for each wave, nor with more than
-// 8192, which would end after all others. Forward and backward with 128, 256 and 512 workgroups: 1 row, 32317 x 1024 bf16 176, 127 and
-// 132 us, fp32 162, 152 and 166; 48 rows fp32 316, 336 and 358; 8 rows, 131072 x 4096 bf16 (16384 tokens at 256) 3014, 1908 and 1640.
+// Token ranges of dX: 256 workgroups, one a CU beside those of dW, none with less than 128 tokens, a block for each wave. Forward and
+// backward with 128, 256 and 512 workgroups: 1 row, 32317 x 1024 bf16 144, 106 and 114 us, fp32 161, 154 and 168; 48 rows fp32 319, 335 and
+// 357; 8 rows, 131072 x 4096 bf16 1118, 1095 and 1119.
 NarrowSplits narrow_splits(int64_t tokens, int64_t width) {
-    const int64_t slices = (width + 127) / 128, most = (tokens + 127) / 128, least = (tokens + 8191) / 8192;
-    int64_t n = (256 + slices - 1) / slices;
-    if (n < least) n = least;
-    if (n > most) n = most;
+    const int64_t slices = (width + 127) / 128, most = (tokens + 127) / 128, want = (256 + slices - 1) / slices;
+    const int64_t n = want < most ? want : most;
     NarrowSplits s;
     s.each = ((tokens + n - 1) / n + 127) / 128 * 128;
     s.n = static_cast<int32_t>((tokens + s.each - 1) / s.each);

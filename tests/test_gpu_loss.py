@@ -281,7 +281,7 @@ def test_several_pieces_of_the_vocabulary(gpu):
         ref.check(loss, _grads(loss, (x, w, b)), dtype)
 
 
-@pytest.mark.parametrize("dtype,rows,vocab,width", [("bf16", 64, 1000, 100), ("bf16", 40, 3300, 1000), ("bf16", 64, 3300, 1000), ("fp32", 64, 3300, 1000),
+@pytest.mark.parametrize("dtype,rows,vocab,width", [("bf16", 64, 1000, 100), ("bf16", 40, 3300, 1000), ("bf16", 48, 13000, 1000), ("bf16", 64, 3300, 1000), ("fp32", 64, 3300, 1000),
                                                     ("fp32", 65, 3300, 128), ("bf16", 20, 140001, 64), ("fp32", 40, 140001, 64)])
 def test_few_rows(gpu, dtype, rows, vocab, width):
     """Either side of the sizes up to which few rows have kernels of their own, and more tokens than those keep row gradients of."""
