@@ -6,10 +6,9 @@ product is worked through in tiles whose maxima and sums are all that leaves the
 again, a piece of the vocabulary at a time. K workers on one GPU hold K sets of activations, and [tokens, vocabulary] logits
 are the largest of them (6400 tokens over 32317 in fp32: 0.83 GB per worker, once for the logits and once for their gradient).
 
-The classifiers and criteria these stand in for: the translation model's (examples/gnmt/seq2seq/models/decoder.py, label
-smoothing and a padding index; examples/gnmt/seq2seq/train/smoothing.py) and ``CrossEntropyLoss`` in the vision examples;
-a trainer calls them as ``criterion(model(x), y)`` (jabas/train/trainer.py:82-86, 171-174), see :class:`LinearCrossEntropy`
-and :class:`LinearTopkDistillation`.
+They stand in for the translation model's classifier (examples/gnmt/seq2seq/models/decoder.py) with its criterion and for
+the vision examples' ``CrossEntropyLoss``; a trainer calls them as ``criterion(model(x), y)`` (jabas/train/trainer.py:82-86,
+171-174), see :class:`LinearCrossEntropy` and :class:`LinearTopkDistillation`.
 
 All of them are autograd functions on the current stream of the tensors' device; there is no CPU path. Every input keeps its
 place in memory: nothing is changed in place, nothing is kept between calls but what autograd saves (the inputs, 16 bytes a
@@ -205,8 +204,9 @@ def linear_cross_entropy(hidden, weight, target, bias=None, *, ignore_index=-100
 
     reduction: "mean" over the rows that count (0 where none does), "sum" or "none" (the shape of target). The loss is
     float32, sums are kept in 32 bits; gradients have the inputs' type. With bfloat16 the products take the inputs as they
-    are and the row gradients as fp16 in units of 2^-15 (rounded once, an eighth of bfloat16's step); with float32 every
-    factor is split into two fp16 planes (22 bits) and the products into three."""
+    are and the row gradients as fp16 in units of 2^-15 (rounded once, an eighth of bfloat16's step), few rows' as two
+    bfloat16 planes (16 bits); with float32 every factor is split into two fp16 planes (22 bits) and the products into
+    three, few rows' products are float32's."""
     x, w, b = _linear_inputs(hidden, weight, bias)
     lead = hidden.shape[:-1]
     _check_row_tensor(target, lead, torch.int64, hidden.device, "target")
