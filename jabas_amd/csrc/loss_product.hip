@@ -125,6 +125,10 @@ __device__ inline void at_label(int label, const F& f) {
             if (at == i * 32 + 8 * (e >> 2) + (e & 3)) f(i, e);
 }
 
+// Forward: a tile's product, then per row its maximum and the sum of 2^((z - max) c) over the tile's tokens, so that 16 bytes a row and tile
+// leave the chip instead of the logits. Matrix cores bind it, and the clock they leave: 4096 x 131072 x 4096 bf16 3.2 ms, 1.38 PFLOP/s,
+// cores busy 79 % of the cycles at 1.65 GHz; with an inner axis of 768 to 1024 the start and the exponentials of a tile weigh more:
+// 4099 x 50001 x 768 bf16 328 us, 0.96; 1280 x 32317 x 1024 fp32 308 us, 0.83 (three products).
 template <class E, int P, class C, bool TEACHER>
 __global__ __launch_bounds__(C::kThreads) void logits_forward_kernel(LogitsArgs a) {
     __shared__ __align__(16) char smem[2 * C::kStage];
@@ -244,6 +248,9 @@ __device__ inline void scatter_sum(float (&v)[32]) {
     if constexpr (HALF > 1) scatter_sum<HALF / 2>(v);
 }
 
+// Backward: the same product, and dz = slope 2^((z - peak) c) - what the label or the entries take off, written once as fp16 through LDS, 16
+// bytes a lane. db's sums over a tile's rows are taken here, in 32 bits, where dz is still exact. Bound by the matrix cores
+// as the forward pass: 4096 x 16384 x 4096 bf16 442 us, 1.25 PFLOP/s; 1280 x 32317 x 1024 fp32 338 us, 0.75.
 template <class E, int P, class C, bool TEACHER>
 __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs a) {
     __shared__ __align__(16) char smem[2 * C::kStage];
@@ -484,6 +491,9 @@ __device__ inline void run_job(const Job& a, int unit, char* smem) {
     }
 }
 
+// dW and dX of a piece in one launch, the longer units first, so that neither's last round leaves CUs idle. dz is the right operand of
+// both: rows of k for dW, through transposing reads, and as it lies for dX. Bound by the matrix cores: 4096 x 16384 x 4096 bf16
+// 926 us, 1.19 PFLOP/s (dW and dX alone take the same each); 1280 x 32317 x 1024 fp32 546 us, 0.93.
 template <class CW, class CH>
 __global__ __launch_bounds__(CW::kThreads) void grads_kernel(GradArgs a) {
     static_assert(CW::kStage == CH::kStage && CW::kThreads == CH::kThreads, "one launch shape");
@@ -496,6 +506,7 @@ __global__ __launch_bounds__(CW::kThreads) void grads_kernel(GradArgs a) {
     else run_job<CW>(a.w, a.h_first ? block - lead : block, smem);
 }
 
+// Bound by memory: 5120 rows x 1024 from 5 splits 13 us, 1600 x 1024 from 4 9 us.
 __global__ __launch_bounds__(256) void join_splits_kernel(Job a) {
     const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     const int quads = (a.m + 3) / 4, n = static_cast<int>(at / quads), m = static_cast<int>(at % quads) * 4;
@@ -727,7 +738,8 @@ __device__ inline float join_parts(const float* parts) {
     return fmaxf(fmaxf(merge[0], merge[1]), fmaxf(merge[2], merge[3]));
 }
 
-// One wave per row: padded, and scaled by the row's own power of two, or all by one.
+// One wave per row: padded, and scaled by the row's own power of two, or all by one. Bound by memory: 32317 x 1024 fp32, 132 MB read and as
+// much written, 50 us (5.3 TB/s); a row's second read comes from the caches.
 __global__ __launch_bounds__(kLayThreads) void lay_rows_kernel(LayArgs a) {
     const int place = blockIdx.x * (kLayThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (a.parts) {
@@ -786,6 +798,7 @@ __global__ __launch_bounds__(kLayThreads) void lay_rows_kernel(LayArgs a) {
     if (lane == 0) a.unscale[place] = power_of_two(-e);
 }
 
+// Bound by memory: 134 MB in 21 us (6.4 TB/s).
 __global__ __launch_bounds__(kLayThreads) void absmax_kernel(LayArgs a) {
     __shared__ float merge[kLayThreads / 64];
     const int lane = threadIdx.x & 63;
@@ -807,7 +820,7 @@ __global__ __launch_bounds__(kLayThreads) void absmax_kernel(LayArgs a) {
     if (threadIdx.x == 0) a.parts[blockIdx.x] = fmaxf(fmaxf(merge[0], merge[1]), fmaxf(merge[2], merge[3]));
 }
 
-// 64 x 64 elements through LDS: out[col][row], one scale for all of them.
+// 64 x 64 elements through LDS: out[col][row], one scale for all of them. Bound by memory: 16384 x 4096 bf16 to fp16 42 us (6.4 TB/s).
 __global__ __launch_bounds__(kLayThreads) void lay_columns_kernel(LayArgs a) {
     __shared__ float tile[64][65];
     const int t = threadIdx.x, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, rows = rows_of(a), pad = (rows + 63) / 64 * 64;
