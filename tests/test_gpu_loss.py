@@ -516,6 +516,24 @@ def test_labels_outside_the_vocabulary_give_nan(gpu, label):
     assert bool(g[1].isnan().all()) and not bool(g[0].isnan().any())
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(6, 50000), (200, 3000)])
+def test_rows_of_logits_without_entries_or_outside(gpu, dtype, rows, vocab):
+    """Rows in parts and whole: none of a row's places an entry, and one outside the vocabulary, beside rows that are neither."""
+    gen = _gen(31)
+    z = torch.randn(rows, vocab, generator=gen).to(TYPES[dtype])
+    index, teacher = _entries(gen, rows, vocab, 5, dtype)
+    index[1], teacher[2], index[4, 3] = -1, -math.inf, vocab
+    clean, keep = z.clone(), [r for r in range(rows) if r != 4]
+    z[1], z[2] = float("nan"), float("inf")
+    z = z.to(gpu).requires_grad_(True)
+    loss = losses.topk_distillation(z, index.to(gpu), teacher.to(gpu), reduction="none")
+    grad = _grads(loss.sum(), (z,))[0]
+    assert bool(loss[4].isnan()) and bool(grad[4].isnan().all())
+    assert not bool(grad[1:3].any()) and float(loss[1].detach()) == float(loss[2].detach()) == 0.0
+    Reference(logits=clean[keep], index=index[keep], teacher=teacher[keep], reduction="none").check(loss[keep], [grad[keep]], dtype)
+
+
 @pytest.mark.parametrize("tail", [False, True])
 def test_tokens_named_twice_are_one_event(gpu, tail):
     gen = _gen(3)
@@ -655,6 +673,51 @@ def test_replays_of_a_recorded_step(gpu):
         with torch.no_grad():
             x.copy_(torch.randn(rows, width, generator=gen).to(gpu))
             target.copy_(torch.randint(0, vocab, (rows,), generator=gen))
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(recorded, step()):
+            assert torch.equal(p, q)
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("which", ["tiles_fp32", "tiles_bf16", "entries_bf16", "parts_of_rows", "whole_rows"])
+def test_replays_of_other_recorded_steps(gpu, which):
+    """The same for the calls of many rows and for logits in hand; the number of rows that count changes from replay to replay."""
+    gen = _gen(21)
+    dtype = "fp32" if which.endswith("fp32") or which == "parts_of_rows" else "bf16"
+    rows, vocab, width = {"parts_of_rows": (7, 60001, 0), "whole_rows": (90, 5001, 0)}.get(which, (300, 9000, 72))
+    index, teacher = (t.to(gpu) for t in _entries(gen, rows, vocab, 9, dtype))
+    target = torch.randint(0, vocab, (rows,), generator=gen).to(gpu)
+    if width:
+        leaves, _ = _inputs(gpu, rows, vocab, width, dtype, True, seed=4)
+        x, w, b = leaves
+        call = (lambda: losses.linear_topk_distillation(x, w, index, teacher, b, temperature=2.0)) if which.startswith("entries") else \
+               (lambda: losses.linear_cross_entropy(x, w, target, b, label_smoothing=0.1))
+    else:
+        z = torch.randn(rows, vocab, generator=gen).to(TYPES[dtype]).to(gpu).requires_grad_(True)
+        leaves = [z]
+        call = lambda: losses.topk_distillation(z, index, teacher)
+
+    def step():
+        loss = call()
+        return [loss.detach(), *_grads(loss, leaves)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        recorded = step()
+    for i in range(4):
+        with torch.no_grad():
+            leaves[0].copy_(torch.randn(leaves[0].shape, generator=gen).to(gpu))
+            target.copy_(torch.randint(0, vocab, (rows,), generator=gen))
+            target[: i * rows // 4] = IGNORE
+            index.copy_(_entries(gen, rows, vocab, 9, dtype)[0])
+            index[: i * rows // 4] = -1
         graph.replay()
         torch.cuda.synchronize()
         for p, q in zip(recorded, step()):
