@@ -12,7 +12,9 @@
 // gradients keep their bits whatever their size. fp32's products take 32x32x2, whose lane holds one element of the inner axis, so that
 // operands whose rows are that axis need no transposing; bf16's take 32x32x16 with four features of eight rows turned about in a lane's
 // registers. 8 rows, 131072 x 4096: dX 230 us with bf16 (4.7 TB/s), 525 with fp32 (4.1 TB/s), dW 300 and 457 us; with 32x32x2 and checked
-// loads for bf16 too both took 1081 us, 546 now. What bounds them is how much a CU has on its way: two workgroups' registers fill it.
+// loads for bf16 too both took 1081 us, 546 now. What bounds them is how much a CU has on its way, so two
+// workgroups have to fit one, with 33 to 64 rows too: 64 x 32317 x 1024 fp32 374 us with one, 329 with two, 64 x 131072 x 4096 4360 and 3880.
+// The logits' kernels do so with bf16 (64 x 16000 x 768 116 and 104 us); fp32's would have to spill (64 x 32317 x 1024 forward 93 and 120 us).
 #include "loss_internal.h"
 
 namespace jabas {
@@ -134,7 +136,7 @@ __device__ inline void narrow_logits(const NarrowArgs& a, int64_t first, float (
 }
 
 template <class T, int RB, bool TEACHER>
-__global__ __launch_bounds__(kThreads) void narrow_forward_kernel(NarrowArgs a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void narrow_forward_kernel(NarrowArgs a) {
     constexpr int R = RB * 32, kGroups = kThreads / R, kEach = kTokens / kGroups;
     __shared__ float zs[R][kPitch], part[3][R][kPitch];
     const int64_t first = static_cast<int64_t>(blockIdx.x) * kTokens;
@@ -211,7 +213,7 @@ __device__ inline float row_gradient(const NarrowArgs& a, int n) {
 }
 
 template <class T, int RB, bool TEACHER>
-__global__ __launch_bounds__(kThreads) void narrow_backward_kernel(NarrowArgs a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void narrow_backward_kernel(NarrowArgs a) {
     constexpr int R = RB * 32;
     __shared__ float zs[R][kPitch], part[3][R][kPitch], grad[R];
     __shared__ RowState states[R];
@@ -543,7 +545,7 @@ __device__ inline void narrow_hidden(const NarrowArgs& a, int64_t unit, float* m
 }
 
 template <class T, int RB>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void narrow_grads_kernel(NarrowArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void narrow_grads_kernel(NarrowArgs a) {
     __shared__ __align__(16) float merge[3 * 32 * 128];
     if constexpr (sizeof(T) == 2) {
         if (blockIdx.x < a.hidden_units) narrow_hidden_bf16<RB>(a, blockIdx.x, merge);
@@ -575,8 +577,8 @@ int backward(const NarrowArgs& a, int64_t grid, hipStream_t stream) {
 int64_t narrow_tiles(int64_t vocab) { return (vocab + kTokens - 1) / kTokens; }
 
 // Token ranges of dX: 256 workgroups, one a CU beside those of dW, none with less than 128 tokens, a block for each wave. Forward and
-// backward with 128, 256 and 512 workgroups: 1 row, 32317 x 1024 bf16 144, 106 and 114 us, fp32 161, 154 and 168; 48 rows fp32 319, 335 and
-// 357; 8 rows, 131072 x 4096 bf16 1118, 1095 and 1119.
+// backward with 128, 256 and 512 workgroups: 1 row, 32317 x 1024 bf16 144, 106 and 114 us, fp32 161, 154 and 168; 16 rows fp32 170, 171 and
+// 184; 8 rows, 131072 x 4096 bf16 1118, 1095 and 1119.
 NarrowSplits narrow_splits(int64_t tokens, int64_t width) {
     const int64_t slices = (width + 127) / 128, most = (tokens + 127) / 128, want = (256 + slices - 1) / slices;
     const int64_t n = want < most ? want : most;
