@@ -9,7 +9,8 @@
  *     without teacher_lse: p = softmax of the entries' logits / T, rest = 0
  *     with teacher_lse:    p_j = exp(t_j/T - teacher_lse_n); what the entries leave, r = max(0, 1 - sum p), is one
  *                          more event: rest = r (log r - log R), R = q of all tokens that are no entry
- *                          (rest = 0 where every token is an entry)
+ *                          (rest = 0 where every token is an entry; where there are others and all of them are at
+ *                          -inf, R = 0: an infinite loss where r > 0, and no gradient for them)
  *
  * The conventions of jabas_sync.h hold: plain C types, caller-owned device memory, nothing allocated, freed or
  * synchronised, all work on the stream passed in, a negative JabasStatus before anything is launched. Nothing is

@@ -161,19 +161,24 @@ __device__ inline RowResult row_result(const TeacherArgs& a, const WaveEntries& 
         if (w.index[i] >= 0 && w.p[i] != 0.0f) cross += w.p[i] * ((z[i] - top) * a.inv_t - log_all);
     cross = wave_sum(cross);
     RowResult r = {{0.0f, 0.0f, 0.0f, 0.0f}, 0.0f};
+    int named = 0;
+#pragma unroll
+    for (int i = 0; i < kEntriesPerLane; ++i) named += __popcll(__ballot(w.index[i] >= 0));
     if (!w.counts) return r;
-    const bool others = rest_sum != 0.0f;
+    // Tokens that are no entry may all be at -inf (their sum is 0): the student cannot meet what is left then, R = 0 and the loss is
+    // infinite. M holds it all the same; r q / R, which has no value at those tokens, is taken as 0.
+    const bool others = named < a.vocab, met = rest_sum != 0.0f;
     const float left = a.lse && others ? fmaxf(1.0f - w.mass, 0.0f) : 0.0f, mass = w.mass + left;
-    float rest = 0.0f, share = 0.0f;        // of the student: log R and R
-    if (others) {
+    float rest = -INFINITY, share = 0.0f;       // of the student: log R and R
+    if (met) {
         rest = (rest_peak - top) * a.inv_t + logf(rest_sum) - log_all;
         share = expf(rest);
     }
     r.loss = w.entropy - cross;
     if (left != 0.0f) r.loss += left * (logf(left) - rest);
     r.loss *= a.t * a.t;
-    r.state.peak_rest = others ? rest_peak : 0.0f;
-    r.state.slope = others ? (mass * share - left) / rest_sum : 0.0f;
+    r.state.peak_rest = met ? rest_peak : 0.0f;
+    r.state.slope = met ? (mass * share - left) / rest_sum : 0.0f;
     r.state.peak = top;
     r.state.mass = mass / all;
     if (w.entropy != w.entropy) r.state.slope = r.state.mass = NAN;

@@ -228,7 +228,8 @@ def topk_distillation(logits, teacher_index, teacher_logits, *, temperature=1.0,
     - ``teacher_lse`` None: p is the softmax of the entries' logits / T;
     - ``teacher_lse`` (...) float32, the teacher's logsumexp(logits / T) over its whole vocabulary: p are its true
       probabilities, and what they leave, r = max(0, 1 - sum p), is one more event that the student meets with all tokens
-      that are no entry: ``+ T^2 r (log r - log sum_others q)``.
+      that are no entry: ``+ T^2 r (log r - log sum_others q)``. Where all of those are ruled out (logits of -inf) a rest costs an
+      infinite loss, as a label does that is ruled out: entries that are all there is to choose from take no ``teacher_lse``.
 
     reduction as in :func:`linear_cross_entropy`. No gradient flows to the teacher."""
     _matrix(logits, "logits")

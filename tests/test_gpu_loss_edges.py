@@ -1,0 +1,107 @@
+"""The losses (jabas_amd.loss) where their paths have to agree with the definition and with each other: rests that no token can meet, rows of any
+size beside ordinary ones, weights of very different sizes, tokens ruled out that are named all the same, recorders, and means.
+
+The bounds are those of ``Reference`` in test_gpu_loss.py, in whose terms a case says where it needs another.
+"""
+import math
+
+import pytest
+import torch
+
+from jabas_amd import loss as losses
+from tests.test_gpu_loss import F64, IGNORE, TYPES, Reference, _entries, _gen, _grads, _inputs
+
+pytestmark = pytest.mark.gpu
+
+
+def _cpu(t):
+    return None if t is None else t.detach().cpu().to(F64)
+
+
+class Given(Reference):
+    """The bounds of ``Reference`` for row gradients that a test states itself: ``dz``, ``size`` (what their parts sum to without
+    their signs) and the rows' losses, all without the upstream gradient ``up``."""
+
+    def __init__(self, dz, size, row_losses, Z, up, hidden=None, weight=None, bias=None, T=1.0):
+        x, w, b = _cpu(hidden), _cpu(weight), _cpu(bias)
+        self.Z, self.T, self.counted = Z, T, torch.ones(len(dz), dtype=torch.bool)
+        self.loss, self.loss_size = row_losses, row_losses.abs()
+        dz, size = dz * up[:, None], size * up[:, None].abs()
+        self.dz, self.size = dz, size
+        if x is None:
+            self.grads, self.sizes = [dz], [size]
+        else:
+            self.grads, self.sizes = [dz @ w, dz.t() @ x], [size @ w.abs(), size.t() @ x.abs()]
+            if b is not None:
+                self.grads.append(dz.sum(0))
+                self.sizes.append(size.sum(0))
+
+
+def _largest_logit(x, w, b=None):
+    x, w, b = _cpu(x), _cpu(w), _cpu(b)
+    return (x.abs() @ w.abs().t()).max().item() + (0.0 if b is None else b[torch.isfinite(b)].abs().max().item())
+
+
+PATHS = {"whole": (200, 3000, 0), "parts": (6, 50000, 0), "few": (20, 600, 64), "tiles": (80, 600, 64), "large_tiles": (514, 17000, 64)}
+
+
+# ------------------------------------------------------------------ what the entries leave
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("mask", ["-inf", "lowest"])
+@pytest.mark.parametrize("path", list(PATHS))
+def test_a_rest_that_no_token_can_meet(gpu, path, mask, dtype):
+    """Every token but the entries is ruled out and the teacher leaves a rest: the loss is infinite (at the lowest finite value as large as
+    that makes it), the entries' gradients are T (M q - p) with the rest in M, and the tokens at -inf have none. Without a rest (a teacher whose entries sum to
+    more than 1) the loss is finite."""
+    rows, vocab, width = PATHS[path]
+    k, gen = 5, _gen(rows)
+    low = -math.inf if mask == "-inf" else torch.finfo(TYPES[dtype]).min
+    names = torch.randperm(vocab, generator=gen)[:k]
+    index = torch.stack([names[torch.randperm(k, generator=gen)] for _ in range(rows)])
+    teacher = torch.randn(rows, k, generator=gen).to(TYPES[dtype])
+    lse = torch.logsumexp(teacher.float(), 1) + 0.5
+    lse[::3] -= 1.5
+    others = torch.ones(vocab, dtype=torch.bool)
+    others[names] = False
+    up = torch.rand(rows, generator=gen) + 0.5
+    args = index.to(gpu), teacher.to(gpu)
+    if width:
+        (x, w, b), _ = _inputs(gpu, rows, vocab, width, dtype, True, seed=rows)
+        with torch.no_grad():
+            b[others.to(gpu)] = low
+        loss = losses.linear_topk_distillation(x, w, *args, b, teacher_lse=lse.to(gpu), reduction="none")
+        grads = _grads(loss, (x, w, b), up.to(gpu))
+        z = _cpu(x) @ _cpu(w)[names].t() + _cpu(b)[names]
+        Z = _largest_logit(x, w, b.detach().clamp(min=-100.0))
+    else:
+        x = w = b = None
+        logits = torch.randn(rows, vocab, generator=gen).to(TYPES[dtype])
+        logits[:, others] = low
+        logits = logits.to(gpu).requires_grad_(True)
+        loss = losses.topk_distillation(logits, *args, teacher_lse=lse.to(gpu), reduction="none")
+        grads = _grads(loss, (logits,), up.to(gpu))
+        z = _cpu(logits)[:, names]
+        Z = z.abs().max().item()
+    at = torch.argsort(names)[torch.searchsorted(names.sort().values, index)]       # which of the names an entry is
+    p = torch.zeros(rows, k, dtype=F64).scatter_(1, at, (teacher.to(F64) - lse.to(F64)[:, None]).exp())
+    r = (1.0 - p.sum(1)).clamp(min=0.0)
+    logq = torch.log_softmax(z, 1)
+    M = p.sum(1) + r
+    dz, size = torch.zeros(rows, vocab, dtype=F64), torch.zeros(rows, vocab, dtype=F64)
+    dz[:, names], size[:, names] = M[:, None] * logq.exp() - p, M[:, None] * logq.exp() + p
+    if mask == "lowest":        # equal logits share what the rest asks for
+        dz[:, others] = -(r / int(others.sum()))[:, None]
+        size[:, others] = -dz[:, others]
+    finite = (p * (p.log() - logq)).sum(1)
+    got = loss.detach().cpu().to(F64)
+    left = r > 0
+    assert bool(left.any()) and not bool(left.all())
+    if mask == "-inf":
+        assert bool((got[left] == math.inf).all())
+    else:
+        assert bool((got[left] >= 0.99 * r[left] * -low).all())
+    ref = Given(dz, size, finite, Z, up.to(F64), x, w, b)
+    ref.loss, ref.loss_size = finite[~left], finite[~left].abs()
+    ref.check(loss[~left.to(gpu)], grads, dtype)
+    if mask == "-inf":
+        assert not bool((grads[1][others.to(gpu)] if width else grads[0][:, others.to(gpu)]).any())
