@@ -181,6 +181,7 @@ __device__ inline RowResult row_result(const TeacherArgs& a, const WaveEntries& 
     r.state.slope = met ? (mass * share - left) / rest_sum : 0.0f;
     r.state.peak = top;
     r.state.mass = mass / all;
+    if (r.state.slope == 0.0f && r.state.mass == 0.0f) r.state.mass = 0x1p-149f;       // every token an entry, every p next to nothing: it counts all the same
     if (w.entropy != w.entropy) r.state.slope = r.state.mass = NAN;
     return r;
 }

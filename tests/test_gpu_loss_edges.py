@@ -105,3 +105,23 @@ def test_a_rest_that_no_token_can_meet(gpu, path, mask, dtype):
     ref.check(loss[~left.to(gpu)], grads, dtype)
     if mask == "-inf":
         assert not bool((grads[1][others.to(gpu)] if width else grads[0][:, others.to(gpu)]).any())
+
+
+@pytest.mark.parametrize("path", ["whole", "few", "tiles"])
+def test_rows_whose_entries_are_all_there_is_count(gpu, path):
+    """Every token is an entry of a teacher that gives all of them next to nothing: a loss of 0, in a mean over all the rows."""
+    rows, _, width = PATHS[path]
+    gen = _gen(2)
+    index = torch.arange(3).expand(rows, 3).contiguous()
+    teacher = torch.randn(rows, 3, generator=gen)
+    lse = torch.logsumexp(teacher, 1) + 0.25
+    lse[::2] = 300.0
+    if width:
+        (x, w, _), _ = _inputs(gpu, rows, 3, width, "fp32", seed=1)
+        call = lambda reduction: losses.linear_topk_distillation(x, w, index.to(gpu), teacher.to(gpu), teacher_lse=lse.to(gpu), reduction=reduction)
+    else:
+        z = torch.randn(rows, 3, generator=gen).to(gpu)
+        call = lambda reduction: losses.topk_distillation(z, index.to(gpu), teacher.to(gpu), teacher_lse=lse.to(gpu), reduction=reduction)
+    each = call("none").detach().cpu().to(F64)
+    assert not bool(each[::2].any()) and bool(each[1::2].any())
+    assert float(call("mean").detach()) == pytest.approx(float(each.sum()) / rows, rel=2.0 ** -22)
