@@ -177,11 +177,12 @@ size_t carve_forward(const JabasLoss* l, const Shape& s, char* base, Forward& f)
 }
 
 struct Backward {
-    float *grad, *ratio, *peak;
+    float *grad, *ratio, *peak, *down;
     uint16_t *x, *w;            // operands of the logits; w where it is a copy
     uint16_t *x16, *w16, *dz;   // of the gradients' products
     int32_t *map, *live;
     float *unscale_x, *unscale_w, *unscale_x16, *unscale_w16, *parts;
+    float* peaks;               // of the columns of x16
     float *db, *part_w, *part_h;
     int64_t piece, pad_rows, part_stride, splits, chunk;
     Splits inner;
@@ -209,6 +210,7 @@ size_t carve_backward(const JabasLoss* l, const Shape& s, char* base, Backward& 
     b.grad = c.take<float>(rows);
     b.ratio = c.take<float>(rows);
     b.peak = c.take<float>(1);
+    if (s.teacher) b.down = c.take<float>(rows);
     b.map = c.take<int32_t>(rows);
     b.live = c.take<int32_t>(1);
     b.piece = piece_tokens(l, s, true);
@@ -217,13 +219,14 @@ size_t carve_backward(const JabasLoss* l, const Shape& s, char* base, Backward& 
     if (s.copy_w) b.w = c.take<uint16_t>(b.piece * s.depth * s.planes);
     b.unscale_x = c.take<float>(rows);
     b.unscale_w = c.take<float>(b.piece);
-    b.unscale_x16 = c.take<float>(1);
+    b.part_stride = round_up(l->width, 4);
+    b.peaks = c.take<float>(kPeakParts * b.part_stride);
+    b.unscale_x16 = c.take<float>(b.part_stride);
     b.unscale_w16 = c.take<float>(1);
     b.parts = c.take<float>(kMaxParts);
     b.x16 = c.take<uint16_t>(l->width * b.pad_rows * s.planes);
     if (s.planes == 1) b.w16 = c.take<uint16_t>(l->width * b.piece);
     b.dz = c.take<uint16_t>(b.pad_rows * b.piece * s.planes);
-    b.part_stride = round_up(l->width, 4);
     const int64_t tokens = b.piece < l->vocab ? b.piece : l->vocab;
     b.inner = choose_splits(l->width, tokens, rows, true, true, b.piece < l->vocab, s.planes);
     if (b.inner.w > 1) b.part_w = c.take<float>(b.inner.w * tokens * b.part_stride);
@@ -393,7 +396,6 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
         live.ticket = f.ticket;
         live.state = state;
         live.row_loss = f.row_loss;
-        live.down = reduce + 1;
         JABAS_TRY(launch_live(live, stream));
         a.rows = Live{f.map, f.live};
         JABAS_TRY(lay_x(l, s, a.rows, nullptr, f.x, f.unscale_x, a.x, stream));
@@ -542,6 +544,7 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     r.upstream = upstream;
     r.per_row = per_row;
     r.reduce = reduce;
+    r.down = b.down;
     r.t = static_cast<float>(l->temperature);
     r.state = state;
     r.rows = l->rows;
@@ -550,6 +553,7 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     r.peak = b.peak;
     r.map = b.map;
     r.live = b.live;
+    if (s.teacher) JABAS_TRY(launch_down(l->entry_p, l->rows, static_cast<int32_t>(l->entries), b.down, stream));
     JABAS_TRY(launch_row_grad(r, stream));
     const Live live = {b.map, b.live};
     LogitsArgs a{};
@@ -564,7 +568,7 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     a.entries = entries_of(l, s);
     a.state = state;
     a.row_grad = b.grad;
-    a.down = reduce + 1;
+    a.down = b.down;
     a.uniform = uniform;
     a.hit = hit;
     a.dz = d_hidden || d_weight ? b.dz : nullptr;
@@ -577,6 +581,8 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     lay.planes = s.planes;
     lay.parts = b.parts;
     if (d_weight) {
+        lay.peaks = b.peaks;        // a feature of large values, or a row of a large gradient, takes no bits from the other features
+        lay.peak_stride = b.part_stride;
         lay.in = l->hidden;
         lay.in_stride = l->hidden_stride;
         lay.rows = static_cast<int32_t>(l->rows);
@@ -589,6 +595,7 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
         lay.unscale = b.unscale_x16;
         JABAS_TRY(launch_lay_columns(lay, stream));
     }
+    lay.peaks = nullptr;
     lay.live = Live{};
     lay.row_factor = nullptr;
     lay.in_stride = l->weight_stride;
@@ -627,7 +634,7 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
             g.w.depth = static_cast<int32_t>(b.pad_rows);
             g.w.each = each(b.pad_rows, b.inner.w);
             g.w.splits = splits(b.pad_rows, g.w.each);
-            g.w.unscale0 = b.unscale_x16;
+            g.w.unscale_m = b.unscale_x16;
             g.w.unscale1 = b.peak;
             g.w.part = g.w.splits > 1 ? b.part_w : nullptr;
             g.w.part_plane = n * b.part_stride;

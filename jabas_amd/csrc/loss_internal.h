@@ -25,8 +25,8 @@ static_assert(sizeof(RowState) == 16, "a row's state is one 16-byte load");
 // The row gradients dz travel between kernels as fp16 in units of 2^-15: |dz| <= 1 in units of upstream * T, so the range
 // is used to the top and the smallest steps are 2^-39. Three more bits than bf16 at the same matrix rate; fp32 calls carry a
 // second plane with 2^11 times what the first leaves: 22 bits down to 2^-25, smallest steps of 2^-50. Where a row's probabilities sum
-// to more than 1 (a teacher_lse below its entries', a token named often) |dz| is as much larger: then a power of two, `down`, takes
-// all rows' dz into the range, and their gradients carry its inverse.
+// to more than 1 (a teacher_lse below its entries', a token named often) |dz| is as much larger: then a power of two of the row's own, `down`,
+// takes its dz into the range, and its row gradient carries the inverse. No row has a say in another's steps.
 constexpr float kDzScale = 32768.0f, kLowScale = 2048.0f;
 
 constexpr int kTile = 256;      // the largest output tile of a product; pieces of the vocabulary are whole ones
@@ -77,7 +77,7 @@ struct LogitsArgs {
     // backward
     const RowState* state;
     const float* row_grad;      // gradient of row n in units of dz (bias gradient)
-    const float* down;          // see kDzScale
+    const float* down;          // [row of the call]: see kDzScale, with entries
     float uniform;              // e / V
     float hit;                  // what a label takes off: 1 - e
     void* dz;                   // [row that counts][token of the piece], fp16 planes, or NULL
@@ -96,6 +96,7 @@ struct Job {
     int32_t live_n;             // n is
     const float* unscale0;      // device scalars, or NULL
     const float* unscale1;
+    const float* unscale_m;     // per m, readable up to a multiple of four, or NULL
     const float* row_scale;     // per row of the call, or NULL
     float scale;
     float* part;                // fp32 sums [split][n][part_stride] over the pieces of the inner axis, or NULL: written to `out` at once
@@ -124,7 +125,7 @@ int launch_grads(GradArgs& a, int planes, hipStream_t stream);
 int launch_join_splits(const Job& j, hipStream_t stream);
 
 // Layout of operands: padded copies, split into fp16 planes and scaled by powers of two where the product asks for it.
-constexpr int kMaxParts = 1024;
+constexpr int kMaxParts = 1024, kPeakParts = 64;
 struct LayArgs {
     const void* in;
     int64_t in_stride;
@@ -138,7 +139,9 @@ struct LayArgs {
     int32_t pad;                // a multiple of 64
     int32_t planes;             // 0: copied as they are; 1 or 2 planes of fp16
     void* zero;                 // launch_lay_rows: [row of the call][cols] of in_dtype whose rows that do not count are zeroed, or NULL
-    float* unscale;             // written: a factor per row (launch_lay_rows, planes > 0) or one for all (launch_lay_columns)
+    float* unscale;             // written: a factor per row (launch_lay_rows, planes > 0), or (launch_lay_columns) one for all, with peaks per column
+    float* peaks;               // launch_lay_columns: [kPeakParts][peak_stride] partial maxima of the columns, or NULL
+    int64_t peak_stride;
     float* parts;               // kMaxParts partial maxima; launch_lay_rows: NULL, or one scale for all rows, written to unscale_all too
     float* unscale_all;
     int32_t pad_rows;           // launch_lay_rows with parts: places from rows to here become zeros
@@ -197,16 +200,19 @@ struct LiveArgs {
     uint32_t* ticket;           // set to 0
     RowState* state;
     float* row_loss;
-    float* down;                // written: see kDzScale
 };
 int launch_live(const LiveArgs& a, hipStream_t stream);
 
-// grad[n] = upstream * T * reduce[0] / reduce[1] (0 for rows that do not count), ratio[n] = grad[n] / *peak, *peak the largest |grad|, and which rows
+// down[n] of rows x k entries: see kDzScale
+int launch_down(const float* p, int64_t rows, int32_t k, float* down, hipStream_t stream);
+
+// grad[n] = upstream * T * reduce[0] / down[n] (0 for rows that do not count), ratio[n] = grad[n] / *peak, *peak the largest |grad|, and which rows
 // count, from their states.
 struct RowGradArgs {
     const float* upstream;
     int32_t per_row;
-    const float* reduce;        // the share of a row, the factor of dz
+    const float* reduce;        // the share of a row
+    const float* down;          // or NULL: 1
     float t;
     const RowState* state;
     int64_t rows;

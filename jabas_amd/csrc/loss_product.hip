@@ -272,11 +272,11 @@ __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs
         }
     });
     if (TEACHER) build_map<C>(a.entries, a.rows.map, smem, a.first + m0, n0, rows);
-    const float scale = kDzScale * *a.down, uniform = a.uniform * scale;
 #pragma unroll
     for (int j = 0; j < C::kJ; ++j) {
         keep_order();
         const int nl = wn + j * 32 + (lane & 31), n = row[j];
+        const float scale = TEACHER && n >= 0 ? kDzScale * a.down[n] : kDzScale, uniform = TEACHER ? 0.0f : a.uniform * kDzScale;
         const RowState st = n >= 0 ? a.state[n] : RowState{0.0f, 0.0f, 0.0f, 0.0f};
         const bool counts = !(st.slope == 0.0f && st.mass == 0.0f);
         const float slope = st.slope * scale;
@@ -478,6 +478,7 @@ __device__ inline void run_job(const Job& a, int unit, char* smem) {
             f32x4 v = *reinterpret_cast<const f32x4*>(mine + (r * kChunks + (k ^ (r % kChunks))) * 4);
             const int n = n0 + wn + j * 32 + r, m = m0 + wm + k * 4;
             if (n >= n_here || m >= a.m) continue;
+            if (a.unscale_m) v *= *reinterpret_cast<const f32x4*>(a.unscale_m + m);
             if (part) {
                 float* sum = part + static_cast<int64_t>(n) * a.part_stride + m;       // rows padded to four
                 if (!a.first) v += *reinterpret_cast<const f32x4*>(sum);
@@ -798,6 +799,39 @@ __global__ __launch_bounds__(kLayThreads) void lay_rows_kernel(LayArgs a) {
     if (lane == 0) a.unscale[place] = power_of_two(-e);
 }
 
+// The largest size of each column, kPeakParts parts of the rows. A wave takes 512 columns of eight rows at a time.
+__global__ __launch_bounds__(kLayThreads) void column_peaks_kernel(LayArgs a) {
+    __shared__ float merge[kLayThreads / 64][512];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = blockIdx.y * 512, c = first + lane * 8, rows = rows_of(a);
+    constexpr int kOnTheirWay = 8;
+    const int apart = gridDim.x * (kLayThreads / 64);
+    float peak[8] = {};
+    if (c < a.cols)
+        for (int place = blockIdx.x * (kLayThreads / 64) + wave; place < rows; place += kOnTheirWay * apart) {
+            float v[kOnTheirWay][8], f[kOnTheirWay];
+            int row[kOnTheirWay];
+#pragma unroll
+            for (int u = 0; u < kOnTheirWay; ++u) row[u] = row_of(a, min(place + u * apart, rows - 1));       // past the end: the last again
+#pragma unroll
+            for (int u = 0; u < kOnTheirWay; ++u) {
+                load_eight(a, row[u], c, v[u]);
+                f[u] = row_keeps(a, row[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < kOnTheirWay; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) peak[i] = fmaxf(peak[i], f[u] == 0.0f ? 0.0f : finite_size(v[u][i] * f[u]));
+        }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) merge[wave][i * 64 + lane] = peak[i];
+    __syncthreads();
+    for (int x = threadIdx.x; x < 512; x += kLayThreads) {
+        const int at = first + (x & 63) * 8 + (x >> 6);
+        const float top = fmaxf(fmaxf(merge[0][x], merge[1][x]), fmaxf(merge[2][x], merge[3][x]));
+        if (at < a.cols) a.peaks[blockIdx.x * a.peak_stride + at] = top;
+    }
+}
+
 // Bound by memory: 134 MB in 21 us (6.4 TB/s).
 __global__ __launch_bounds__(kLayThreads) void absmax_kernel(LayArgs a) {
     __shared__ float merge[kLayThreads / 64];
@@ -820,11 +854,11 @@ __global__ __launch_bounds__(kLayThreads) void absmax_kernel(LayArgs a) {
     if (threadIdx.x == 0) a.parts[blockIdx.x] = fmaxf(fmaxf(merge[0], merge[1]), fmaxf(merge[2], merge[3]));
 }
 
-// 64 x 64 elements through LDS: out[col][row], one scale for all of them. Bound by memory: 16384 x 4096 bf16 to fp16 42 us (6.4 TB/s).
+// 64 x 64 elements through LDS: out[col][row], one scale for all of them or (peaks) one per column, which is a row of the product. Bound by memory: 16384 x 4096 bf16 to fp16 42 us (6.4 TB/s).
 __global__ __launch_bounds__(kLayThreads) void lay_columns_kernel(LayArgs a) {
-    __shared__ float tile[64][65];
+    __shared__ float tile[64][65], peaks[kLayThreads / 64][64];
     const int t = threadIdx.x, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, rows = rows_of(a), pad = (rows + 63) / 64 * 64;
-    if (r0 >= pad && r0) return;        // the first writes the scale, whatever there is to lay out
+    if (r0 >= pad && r0) return;        // the first writes the scales, whatever there is to lay out
     float v[8];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -835,13 +869,25 @@ __global__ __launch_bounds__(kLayThreads) void lay_columns_kernel(LayArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) tile[r][c + i] = f != 0.0f ? v[i] * f : 0.0f;
     }
-    const int e = scale_exponent(join_parts(a.parts));      // its barrier stands behind the writes of `tile` too
-    const float scale = power_of_two(e);
-    if (t == 0 && blockIdx.x == 0 && blockIdx.y == 0) *a.unscale = power_of_two(-e);
+    float whole = 0.0f;
+    if (a.peaks) {
+        const int c = c0 + (t & 63);
+        float peak = 0.0f;
+#pragma unroll
+        for (int i = t >> 6; i < kPeakParts; i += kLayThreads / 64) peak = fmaxf(peak, c < a.cols ? a.peaks[i * a.peak_stride + c] : 0.0f);
+        peaks[t >> 6][t & 63] = peak;
+        __syncthreads();
+    } else {
+        whole = join_parts(a.parts);        // its barrier stands behind the writes of `tile` too
+    }
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int c = x * 32 + (t >> 3), r = (t & 7) * 8;
-        if (c0 + c >= a.cols || r0 + r >= pad) continue;
+        if (c0 + c >= a.cols) continue;
+        const int e = scale_exponent(a.peaks ? fmaxf(fmaxf(peaks[0][c], peaks[1][c]), fmaxf(peaks[2][c], peaks[3][c])) : whole);
+        const float scale = power_of_two(e);
+        if (r0 + r == 0 && (a.peaks || c0 + c == 0)) a.unscale[c0 + c] = power_of_two(-e);
+        if (r0 + r >= pad) continue;
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = tile[r + i][c] * scale;
         store_eight(a, c0 + c, r0 + r, v);
@@ -857,9 +903,10 @@ int launch_lay_rows(const LayArgs& a, hipStream_t stream) {
 }
 
 int launch_lay_columns(const LayArgs& a, hipStream_t stream) {
-    const int status = launch(absmax_kernel, kMaxParts, kLayThreads, a, stream);
-    if (status != JABAS_OK) return status;
     void* params[] = {const_cast<LayArgs*>(&a)};
+    const hipError_t error = a.peaks ? hipLaunchKernel(reinterpret_cast<const void*>(column_peaks_kernel), dim3(kPeakParts, (a.cols + 511) / 512), dim3(kLayThreads), params, 0, stream)
+                                     : hipLaunchKernel(reinterpret_cast<const void*>(absmax_kernel), dim3(kMaxParts), dim3(kLayThreads), params, 0, stream);
+    if (error != hipSuccess) return JABAS_ERR_LAUNCH;
     return hipLaunchKernel(reinterpret_cast<const void*>(lay_columns_kernel), dim3(a.pad / 64, (a.cols + 63) / 64), dim3(kLayThreads), params, 0, stream) == hipSuccess
                ? JABAS_OK : JABAS_ERR_LAUNCH;
 }

@@ -465,23 +465,26 @@ __global__ __launch_bounds__(kJoinThreads) void live_kernel(LiveArgs a) {
         }
         return is;
     };
-    float mass = 0.0f;
     if (a.teacher_row)
-        list_live(a.rows, a.map, a.live, [&](int64_t n) { return a.teacher_row[n]; }, [&](int64_t n, const float4& t) {
-            mass = fmaxf(mass, t.x);
-            return drop(n, t.z != 0.0f);
-        });
+        list_live(a.rows, a.map, a.live, [&](int64_t n) { return a.teacher_row[n].z; }, [&](int64_t n, float counts) { return drop(n, counts != 0.0f); });
     else
         list_live(a.rows, a.map, a.live, [&](int64_t n) { return a.target[n]; }, [&](int64_t n, int64_t label) { return drop(n, label != a.ignore_index); });
-    __shared__ float masses[kJoinWaves];
-    mass = wave_max(mass);
-    if ((threadIdx.x & 63) == 0) masses[threadIdx.x >> 6] = mass;
-    __syncthreads();
-    if (threadIdx.x) return;
-    for (int i = 1; i < kJoinWaves; ++i) mass = fmaxf(mass, masses[i]);
-    float down = 1.0f;          // fp16 holds up to 2 in units of dz; a row whose own sum is not finite is NaN by itself
-    while (mass * down > 1.9f && down > 0x1p-100f) down *= 0.5f;
-    *a.down = down;
+}
+
+// A wave per row. fp16 holds up to 2 in units of dz; a row whose sum is not finite has no gradient that is.
+__global__ __launch_bounds__(kThreads) void down_kernel(const float* p, int64_t rows, int32_t k, float* down) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int lane = threadIdx.x & 63;
+    float mass = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kEntriesPerLane; ++i)
+        if (lane + 64 * i < k) mass += p[row * k + lane + 64 * i];
+    mass = wave_sum(mass);
+    if (lane) return;
+    int e;
+    frexpf(mass, &e);
+    down[row] = mass > 1.9f && mass < INFINITY ? ldexpf(1.0f, -e) : 1.0f;
 }
 
 // As above: 6400 rows 12 us, 1600 9 us.
@@ -489,13 +492,13 @@ __global__ __launch_bounds__(kJoinThreads) void row_grad_kernel(RowGradArgs a) {
     __shared__ float peaks[kJoinWaves];
     float top = 0.0f;
     bool bad = false;
-    const float share = a.reduce[0] * a.t / a.reduce[1];
+    const float share = a.reduce[0] * a.t;
     struct Row {
         RowState state;
-        float upstream;
+        float upstream, down;
     };
-    list_live(a.rows, a.map, a.live, [&](int64_t n) { return Row{a.state[n], a.upstream[a.per_row ? n : 0]}; }, [&](int64_t n, const Row& r) {
-        const float g = counts(r.state) ? r.upstream * share : 0.0f;
+    list_live(a.rows, a.map, a.live, [&](int64_t n) { return Row{a.state[n], a.upstream[a.per_row ? n : 0], a.down ? a.down[n] : 1.0f}; }, [&](int64_t n, const Row& r) {
+        const float g = counts(r.state) ? r.upstream * share / r.down : 0.0f;
         a.grad[n] = g;
         bad |= !(fabsf(g) < INFINITY);
         top = fmaxf(top, fabsf(g));
@@ -845,6 +848,9 @@ int launch_reduce(const float* row_loss, const RowState* state, int64_t rows, in
     return launch(reduce_kernel, 1, kJoinThreads, stream, row_loss, state, rows, reduction, loss_out, reduce);
 }
 int launch_live(const LiveArgs& a, hipStream_t stream) { return launch(live_kernel, 1, kJoinThreads, stream, a); }
+int launch_down(const float* p, int64_t rows, int32_t k, float* down, hipStream_t stream) {
+    return launch(down_kernel, static_cast<unsigned>((rows + 3) / 4), kThreads, stream, p, rows, k, down);
+}
 int launch_row_grad(const RowGradArgs& a, hipStream_t stream) { return launch(row_grad_kernel, 1, kJoinThreads, stream, a); }
 int launch_bias_sum(const float* parts, const int32_t* live, int32_t tile, int64_t stride, int64_t n, void* out, int32_t dtype, hipStream_t stream) {
     return launch(bias_sum_kernel, static_cast<unsigned>((n + kThreads - 1) / kThreads), kThreads, stream, parts, live, tile, stride, n, out, dtype);

@@ -125,3 +125,31 @@ def test_rows_whose_entries_are_all_there_is_count(gpu, path):
     each = call("none").detach().cpu().to(F64)
     assert not bool(each[::2].any()) and bool(each[1::2].any())
     assert float(call("mean").detach()) == pytest.approx(float(each.sum()) / rows, rel=2.0 ** -22)
+
+
+# ------------------------------------------------------------------ rows and weights of any size
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows", [20, 80, 300])
+@pytest.mark.parametrize("how", ["2^42", "inf"])
+def test_a_row_far_above_one_leaves_the_others_alone(gpu, rows, dtype, how):
+    """One row's probabilities sum to 2^42, or to infinity: the losses and the hidden states' gradients of the other rows are what they are without it. The
+    row's own p are off by the rounding of t - teacher_lse, 2^-24 (|t| + |lse| + |t - lse|) < 2^-17."""
+    vocab, width, k, far = 2001, 64, 8, 7
+    (x, w, b), gen = _inputs(gpu, rows, vocab, width, dtype, True, seed=rows)
+    index, teacher = _entries(gen, rows, vocab, k, dtype)
+    lse = torch.logsumexp(teacher.float(), 1) + 0.5
+    lse[far] = lse[far] - 30.0 if how == "2^42" else -math.inf
+    up = torch.rand(rows, generator=gen) + 0.5
+    loss = losses.linear_topk_distillation(x, w, index.to(gpu), teacher.to(gpu), b, teacher_lse=lse.to(gpu), reduction="none")
+    grads = _grads(loss, (x, w, b), up.to(gpu))
+    keep = torch.arange(rows) != far
+    ref = Reference(x[keep.to(gpu)], w, b, index=index[keep], teacher=teacher[keep], lse=lse[keep], reduction="none", upstream=up[keep])
+    ref.check(loss[keep.to(gpu)], [grads[0][keep.to(gpu)]], dtype)
+    if how == "inf":
+        assert not bool(loss[far].isfinite())
+        return
+    ref = Reference(x, w, b, index=index, teacher=teacher, lse=lse, reduction="none", upstream=up)
+    rel = 2.0 ** -20 * (ref.Z + 4.0) + 2.0 ** -17 + (2.0 ** -10 if dtype == "bf16" else 0.0)
+    last = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -22
+    for g, want, size in zip(grads, ref.grads, ref.sizes):
+        assert bool(((_cpu(g) - want).abs() <= rel * size + last * want.abs()).all())
