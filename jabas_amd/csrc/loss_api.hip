@@ -183,6 +183,7 @@ struct Backward {
     int32_t *map, *live;
     float *unscale_x, *unscale_w, *unscale_x16, *unscale_w16, *parts;
     float* peaks;               // of the columns of x16
+    uint32_t* named;
     float *db, *part_w, *part_h;
     int64_t piece, pad_rows, part_stride, splits, chunk;
     Splits inner;
@@ -221,6 +222,7 @@ size_t carve_backward(const JabasLoss* l, const Shape& s, char* base, Backward& 
     b.unscale_w = c.take<float>(b.piece);
     b.part_stride = round_up(l->width, 4);
     b.peaks = c.take<float>(kPeakParts * b.part_stride);
+    if (l->bias) b.named = c.take<uint32_t>(tiles(l->vocab, 32));
     b.unscale_x16 = c.take<float>(b.part_stride);
     b.unscale_w16 = c.take<float>(1);
     b.parts = c.take<float>(kMaxParts);
@@ -275,12 +277,15 @@ const char* at(const void* p, int64_t elements, int dtype) {
         if (status_ != JABAS_OK) return status_; \
     } while (0)
 
-// The hidden states of the rows that count; the other rows of `zero` become zeros.
-int lay_x(const JabasLoss* l, const Shape& s, const Live& live, void* zero, uint16_t* x, float* unscale, Operand& out, hipStream_t stream) {
+// The hidden states of the rows that count; the other rows of `zero` become zeros, and the tokens the rows name are marked in `name`.
+int lay_x(const JabasLoss* l, const Shape& s, const Live& live, void* zero, uint32_t* name, uint16_t* x, float* unscale, Operand& out, hipStream_t stream) {
     out.rows = static_cast<int32_t>(l->rows);
     LayArgs a{};
     a.live = live;
     a.zero = zero;
+    a.name = name;
+    a.entries = entries_of(l, s);
+    a.vocab = l->vocab;
     a.in = l->hidden;
     a.in_stride = l->hidden_stride;
     a.in_dtype = l->dtype;
@@ -299,9 +304,9 @@ int lay_x(const JabasLoss* l, const Shape& s, const Live& live, void* zero, uint
 }
 
 // The weight's rows of a piece. `parts`: two planes with one scale for all, fit for a product that sums over the tokens too: those that the
-// bias rules out are zeros, and as many more as make whole steps.
+// bias rules out are zeros (those that are `named` are not), and as many more as make whole steps.
 int lay_w(const JabasLoss* l, const Shape& s, int64_t first, int64_t n, int64_t piece, uint16_t* w, float* unscale, float* parts, float* unscale_all,
-          Operand& out, hipStream_t stream) {
+          const uint32_t* named, Operand& out, hipStream_t stream) {
     out.rows = static_cast<int32_t>(n);
     if (!s.copy_w) {
         out.p = at(l->weight, first * l->weight_stride, l->dtype);
@@ -324,7 +329,9 @@ int lay_w(const JabasLoss* l, const Shape& s, int64_t first, int64_t n, int64_t 
     if (parts) {
         a.parts = parts;
         a.unscale_all = unscale_all;
-        a.row_mask = l->bias ? at(l->bias, first, l->dtype) : nullptr;
+        a.row_mask = named ? at(l->bias, first, l->dtype) : nullptr;
+        a.named = named;
+        a.first = static_cast<int32_t>(first);
         a.pad_rows = static_cast<int32_t>(round_up(n, kDepth));
     }
     out.p = w;
@@ -398,7 +405,7 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
         live.row_loss = f.row_loss;
         JABAS_TRY(launch_live(live, stream));
         a.rows = Live{f.map, f.live};
-        JABAS_TRY(lay_x(l, s, a.rows, nullptr, f.x, f.unscale_x, a.x, stream));
+        JABAS_TRY(lay_x(l, s, a.rows, nullptr, nullptr, f.x, f.unscale_x, a.x, stream));
         a.depth = static_cast<int32_t>(s.depth);
         a.unscale_x = f.unscale_x;
         a.unscale_w = f.unscale_w;
@@ -411,7 +418,7 @@ JABAS_API int jabas_loss_forward(const JabasLoss* l, float* loss_out, void* work
         a.entry_logit = f.entry_logit;
         for (int64_t first = 0; first < l->vocab; first += f.piece) {
             const int64_t n = l->vocab - first < f.piece ? l->vocab - first : f.piece;
-            JABAS_TRY(lay_w(l, s, first, n, f.piece, f.w, f.unscale_w, nullptr, nullptr, a.w, stream));
+            JABAS_TRY(lay_w(l, s, first, n, f.piece, f.w, f.unscale_w, nullptr, nullptr, nullptr, a.w, stream));
             a.first = static_cast<int32_t>(first);
             JABAS_TRY(launch_logits_forward(a, s.planes, f.large, stream));
         }
@@ -553,12 +560,16 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     r.peak = b.peak;
     r.map = b.map;
     r.live = b.live;
+    // Tokens that the bias rules out may hold any weight: dz is 0 there, but at a label or an entry, and everywhere under label smoothing.
+    uint32_t* named = l->bias && d_hidden && l->label_smoothing == 0.0 ? b.named : nullptr;
+    r.zero = named;
+    r.zeros = tiles(l->vocab, 32);
     if (s.teacher) JABAS_TRY(launch_down(l->entry_p, l->rows, static_cast<int32_t>(l->entries), b.down, stream));
     JABAS_TRY(launch_row_grad(r, stream));
     const Live live = {b.map, b.live};
     LogitsArgs a{};
     a.rows = live;
-    JABAS_TRY(lay_x(l, s, live, d_hidden, b.x, b.unscale_x, a.x, stream));
+    JABAS_TRY(lay_x(l, s, live, d_hidden, named, b.x, b.unscale_x, a.x, stream));
     a.depth = static_cast<int32_t>(s.depth);
     a.unscale_x = b.unscale_x;
     a.unscale_w = b.unscale_w;
@@ -620,7 +631,7 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     for (int64_t first = 0; first < l->vocab; first += b.piece) {
         const int64_t n = l->vocab - first < b.piece ? l->vocab - first : b.piece;
         const int32_t pad = static_cast<int32_t>(round_up(n, kDepth));
-        JABAS_TRY(lay_w(l, s, first, n, b.piece, b.w, b.unscale_w, s.planes == 2 && d_hidden ? b.parts : nullptr, b.unscale_w16, a.w, stream));
+        JABAS_TRY(lay_w(l, s, first, n, b.piece, b.w, b.unscale_w, s.planes == 2 && d_hidden ? b.parts : nullptr, b.unscale_w16, named, a.w, stream));
         a.first = static_cast<int32_t>(first);
         a.pad_tokens = pad;
         JABAS_TRY(launch_logits_backward(a, s.planes, b.large, stream));
@@ -646,7 +657,9 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
             if (s.planes == 1) {
                 lay.in = at(l->weight, first * l->weight_stride, l->dtype);
                 lay.rows = static_cast<int32_t>(n);
-                lay.row_mask = l->bias ? at(l->bias, first, l->dtype) : nullptr;
+                lay.row_mask = named ? at(l->bias, first, l->dtype) : nullptr;
+                lay.named = named;
+                lay.first = static_cast<int32_t>(first);
                 lay.pad = pad;
                 JABAS_TRY(launch_lay_columns(lay, stream));
                 g.h.a = Operand{b.w16, b.piece, 0, width};

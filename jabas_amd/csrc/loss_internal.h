@@ -133,12 +133,17 @@ struct LayArgs {
     int32_t rows, cols;         // of `in`
     Live live;                  // the rows of `in` that are laid out, or all of them
     const float* row_factor;    // per row of `in`, or NULL: rows with factor 0 are zeros whatever they hold, others are multiplied
-    const void* row_mask;       // per row of `in`, in_dtype, or NULL: rows with -inf here (tokens that the bias rules out) are zeros
+    const void* row_mask;       // per row of `in`, in_dtype, or NULL: rows with -inf here (tokens that the bias rules out) are zeros, but for those
+    const uint32_t* named;      // whose bit of the vocabulary is set here: they are a label or an entry, with a dz of their own
+    int32_t first;              // token of row 0
     void* out;                  // launch_lay_rows: [rows][pad]; launch_lay_columns: [cols][pad]
     int64_t out_stride, out_plane;
     int32_t pad;                // a multiple of 64
     int32_t planes;             // 0: copied as they are; 1 or 2 planes of fp16
     void* zero;                 // launch_lay_rows: [row of the call][cols] of in_dtype whose rows that do not count are zeroed, or NULL
+    uint32_t* name;             // launch_lay_rows: zeros, in which the bits of the rows' labels and entries are set, or NULL
+    Entries entries;
+    int64_t vocab;
     float* unscale;             // written: a factor per row (launch_lay_rows, planes > 0), or (launch_lay_columns) one for all, with peaks per column
     float* peaks;               // launch_lay_columns: [kPeakParts][peak_stride] partial maxima of the columns, or NULL
     int64_t peak_stride;
@@ -218,6 +223,8 @@ struct RowGradArgs {
     int64_t rows;
     float *grad, *ratio, *peak;
     int32_t *map, *live;
+    uint32_t* zero;             // `zeros` words set to 0, or NULL
+    int64_t zeros;
 };
 int launch_row_grad(const RowGradArgs& a, hipStream_t stream);
 

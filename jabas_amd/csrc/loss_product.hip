@@ -718,13 +718,30 @@ __device__ inline void store_eight(const LayArgs& a, int64_t row, int c, const f
 }
 
 __device__ inline float row_keeps(const LayArgs& a, int row) {
-    if (a.row_mask && load_as_float(a.row_mask, row, a.in_dtype) == -INFINITY) return 0.0f;
+    if (a.row_mask && load_as_float(a.row_mask, row, a.in_dtype) == -INFINITY) {
+        const int token = a.first + row;
+        if (!((a.named[token >> 5] >> (token & 31)) & 1)) return 0.0f;
+    }
     return a.row_factor ? a.row_factor[row] : 1.0f;
 }
 
 // Row r that is laid out: rows and places.
 __device__ inline int rows_of(const LayArgs& a) { return a.live.live ? *a.live.live : a.rows; }
 __device__ inline int row_of(const LayArgs& a, int r) { return a.live.map ? a.live.map[r] : r; }
+
+// The tokens that a row of the call has a dz of its own for, whatever rules them out, by one wave.
+__device__ inline void name_tokens(const LayArgs& a, int row, int lane) {
+    const auto name = [&](int64_t token) {
+        if (token >= 0 && token < a.vocab) atomicOr(a.name + (token >> 5), 1u << (token & 31));
+    };
+    if (!a.entries.index) {
+        if (lane == 0) name(a.entries.target[row]);
+        return;
+    }
+    const int64_t first = static_cast<int64_t>(row) * a.entries.k;
+    for (int j = lane; j < a.entries.k; j += 64)
+        if (a.entries.p[first + j] != 0.0f) name(a.entries.index[first + j]);
+}
 
 // The largest of the partial maxima, for every thread of the workgroup.
 __device__ inline float join_parts(const float* parts) {
@@ -767,6 +784,7 @@ __global__ __launch_bounds__(kLayThreads) void lay_rows_kernel(LayArgs a) {
         for (int64_t i = lane; i < bytes / 2; i += 64) out[i] = 0;
         return;
     }
+    if (a.name) name_tokens(a, row, lane);
     if (a.planes == 0) {
         const uint16_t* in = static_cast<const uint16_t*>(a.in) + static_cast<int64_t>(row) * a.in_stride;
         uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(place) * a.out_stride;

@@ -493,6 +493,8 @@ __global__ __launch_bounds__(kJoinThreads) void row_grad_kernel(RowGradArgs a) {
     float top = 0.0f;
     bool bad = false;
     const float share = a.reduce[0] * a.t;
+    if (a.zero)
+        for (int64_t i = threadIdx.x; i < a.zeros; i += kJoinThreads) a.zero[i] = 0;
     struct Row {
         RowState state;
         float upstream, down;

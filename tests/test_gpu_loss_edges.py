@@ -153,3 +153,49 @@ def test_a_row_far_above_one_leaves_the_others_alone(gpu, rows, dtype, how):
     last = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -22
     for g, want, size in zip(grads, ref.grads, ref.sizes):
         assert bool(((_cpu(g) - want).abs() <= rel * size + last * want.abs()).all())
+
+
+# ------------------------------------------------------------------ tokens ruled out, and named all the same
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows", [20, 80, 514])
+@pytest.mark.parametrize("form", ["labels", "smoothed", "entries"])
+def test_ruled_out_tokens_that_are_named(gpu, rows, dtype, form):
+    """A bias of -inf at a token that is a row's label or entry: the loss is infinite, and the gradients are dz W and dz^T X all the same,
+    with dz = -p there; under label smoothing every token is named. Tokens that are ruled out and not named have none, whatever their weight."""
+    vocab, width = 17000 if rows == 514 else 700, 64
+    (x, w, b), gen = _inputs(gpu, rows, vocab, width, dtype, True, seed=rows)
+    out = torch.arange(3, vocab, 5)
+    with torch.no_grad():
+        b[out.to(gpu)] = -math.inf
+        if form != "smoothed":
+            w[out[4::7].to(gpu)] = 1e30
+    e = 0.1 if form == "smoothed" else 0.0
+    fine = torch.tensor([v for v in range(vocab) if v % 5 != 3])
+    target = fine[torch.randint(0, len(fine), (rows,), generator=gen)]
+    target[::4] = out[2]
+    up = torch.rand(rows, generator=gen) + 0.5
+    p = torch.zeros(rows, vocab, dtype=F64)
+    if form == "entries":
+        index = torch.stack([target, fine[torch.randint(0, len(fine), (rows,), generator=gen)]], 1)
+        teacher = torch.randn(rows, 2, generator=gen).to(TYPES[dtype])
+        loss = losses.linear_topk_distillation(x, w, index.to(gpu), teacher.to(gpu), b, reduction="none")
+        p.scatter_add_(1, index, torch.softmax(teacher.to(F64), 1))
+    else:
+        loss = losses.linear_cross_entropy(x, w, target.to(gpu), b, label_smoothing=e, reduction="none")
+        p.scatter_(1, target[:, None], 1.0 - e)
+        p += e / vocab
+    grads = _grads(loss, (x, w, b), up.to(gpu))
+    wd = _cpu(w)
+    if form != "smoothed":
+        wd[out[4::7]] = 0.0
+    z = _cpu(x) @ wd.t() + _cpu(b)
+    q = torch.softmax(z, 1)
+    infinite = torch.ones(rows, dtype=torch.bool) if e else target == int(out[2])
+    assert bool((loss.detach().cpu()[infinite] == math.inf).all())
+    row_losses = torch.where(p > 0, p * (p.clamp(min=1e-300).log() * (form == "entries") - torch.log_softmax(z, 1)), torch.zeros_like(p)).sum(1)
+    ref = Given(q - p, q + p, row_losses[~infinite], _largest_logit(x, wd, b), up.to(F64), x, wd, b)
+    if infinite.all():
+        ref.loss = ref.loss_size = torch.zeros((), dtype=F64)
+        ref.check(torch.zeros(()), grads, dtype)
+    else:
+        ref.check(loss[~infinite.to(gpu)], grads, dtype)
