@@ -17,8 +17,9 @@
  * kept between calls but what the caller keeps (row_state, entry_index, entry_p).
  *
  * Rows that do not count (target == ignore_index; no teacher entry) have loss 0 and gradient 0 whatever their
- * hidden state or logits hold. A label, or a teacher index, outside the vocabulary (a negative teacher index is
- * "no entry") makes its row's loss and gradients NaN; no memory outside the tensors is read.
+ * hidden state or logits hold, and a row whose upstream gradient is 0 has gradient 0. A label, or a teacher index,
+ * outside the vocabulary (a negative teacher index is "no entry") makes its row's loss and gradients NaN; no memory
+ * outside the tensors is read.
  *
  * Sizes: from hidden and weight rows <= 2^22, vocab <= 2^28, width <= 2^20 and less than 2^23 tiles of 256 rows and 256
  * tokens; over logits rows times the parts of 32768 tokens of a row (more of them where rows are few) less than 2^24,

@@ -212,7 +212,7 @@ int launch_live(const LiveArgs& a, hipStream_t stream);
 int launch_down(const float* p, int64_t rows, int32_t k, float* down, hipStream_t stream);
 
 // grad[n] = upstream * T * reduce[0] / down[n] (0 for rows that do not count), ratio[n] = grad[n] / *peak, *peak the largest |grad|, and which rows
-// count, from their states.
+// have a grad.
 struct RowGradArgs {
     const float* upstream;
     int32_t per_row;

@@ -407,10 +407,7 @@ __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs
 __device__ inline void put_four(const Job& a, int n, int m, f32x4 v) {
     const int here = min(4, a.m - m);
     if (a.live_n) n = a.rows.map[n];
-    if (a.row_scale) {      // a row that does not count is zero even where its neighbours' scale is not finite
-        const float rs = a.row_scale[n];
-        v = rs == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v * rs;
-    }
+    if (a.row_scale) v *= a.row_scale[n];
     const int64_t at = static_cast<int64_t>(n) * a.out_stride + m;
     if (a.out_dtype == JABAS_F32) {
         float* out = static_cast<float*>(a.out) + at;

@@ -504,7 +504,7 @@ __global__ __launch_bounds__(kJoinThreads) void row_grad_kernel(RowGradArgs a) {
         a.grad[n] = g;
         bad |= !(fabsf(g) < INFINITY);
         top = fmaxf(top, fabsf(g));
-        return counts(r.state);
+        return g != 0.0f;       // rows without an upstream gradient have no part in the products either, whatever they hold
     });
     top = wave_max(top);
     if (__any(bad)) top = INFINITY;

@@ -200,7 +200,7 @@ def linear_cross_entropy(hidden, weight, target, bias=None, *, ignore_index=-100
     hidden: (..., width) float32 or bfloat16; weight: (vocab, width) of the same type; bias: (vocab,) of the same type or
     None (-inf rules a token out); target: (...) int64. The loss of a row with logits z and label t is
     ``logsumexp(z) - (1 - e) z[t] - e mean(z)``, e = label_smoothing. Rows whose label is ``ignore_index`` do not count:
-    loss and gradient are 0 whatever their hidden states hold. Any other label outside the vocabulary gives NaN.
+    loss and gradient are 0 whatever their hidden states hold; a row whose upstream gradient is 0 has gradient 0 too. Any other label outside the vocabulary gives NaN.
 
     reduction: "mean" over the rows that count (0 where none does), "sum" or "none" (the shape of target). The loss is
     float32, sums are kept in 32 bits; gradients have the inputs' type. With bfloat16 the products take the inputs as they

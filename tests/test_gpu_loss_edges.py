@@ -199,3 +199,37 @@ def test_ruled_out_tokens_that_are_named(gpu, rows, dtype, form):
         ref.check(torch.zeros(()), grads, dtype)
     else:
         ref.check(loss[~infinite.to(gpu)], grads, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("path", list(PATHS))
+def test_rows_without_upstream_have_no_gradient(gpu, path, dtype):
+    """Rows whose upstream gradient is 0 (a program that weighs the losses itself), over hidden states or logits that are NaN: as if they were not there."""
+    rows, vocab, width = PATHS[path]
+    gen = _gen(rows)
+    up = torch.rand(rows, generator=gen) + 0.5
+    up[::3] = 0.0
+    keep = up != 0
+    index, teacher = _entries(gen, rows, vocab, 4, dtype)
+    if not width:
+        z = torch.randn(rows, vocab, generator=gen).to(TYPES[dtype]).to(gpu)
+        z[::3] = float("nan")
+        z.requires_grad_(True)
+        loss = losses.topk_distillation(z, index.to(gpu), teacher.to(gpu), reduction="none")
+        grad = _grads(loss, (z,), up.to(gpu))[0]
+        assert not bool(grad[::3].any())
+        Reference(logits=z[keep.to(gpu)], index=index[keep], teacher=teacher[keep], reduction="none", upstream=up[keep]).check(
+            loss[keep.to(gpu)], [grad[keep.to(gpu)]], dtype)
+        return
+    (x, w, b), _ = _inputs(gpu, rows, vocab, width, dtype, True, seed=1)
+    with torch.no_grad():
+        x[::3] = float("nan")
+    target = torch.randint(0, vocab, (rows,), generator=gen)
+    for call, held in ((lambda: losses.linear_cross_entropy(x, w, target.to(gpu), b, reduction="none"), dict(target=target[keep])),
+                       (lambda: losses.linear_topk_distillation(x, w, index.to(gpu), teacher.to(gpu), b, reduction="none"),
+                        dict(index=index[keep], teacher=teacher[keep]))):
+        loss = call()
+        grads = _grads(loss, (x, w, b), up.to(gpu))
+        assert not bool(grads[0][::3].any())
+        Reference(x[keep.to(gpu)], w, b, reduction="none", upstream=up[keep], **held).check(
+            loss[keep.to(gpu)], [grads[0][keep.to(gpu)], *grads[1:]], dtype)
