@@ -296,6 +296,7 @@ int lay_x(const JabasLoss* l, const Shape& s, const Live& live, void* zero, uint
     a.out_plane = l->rows * s.depth;
     a.pad = static_cast<int32_t>(s.depth);
     a.planes = s.planes == 2 ? 2 : 0;
+    a.low = 1.0f;
     a.unscale = unscale;
     out.p = x;
     out.stride = a.out_stride;
@@ -325,6 +326,7 @@ int lay_w(const JabasLoss* l, const Shape& s, int64_t first, int64_t n, int64_t 
     a.out_plane = piece * s.depth;
     a.pad = static_cast<int32_t>(s.depth);
     a.planes = s.planes == 2 ? 2 : 0;
+    a.low = kLowScale;
     a.unscale = unscale;
     if (parts) {
         a.parts = parts;
@@ -590,6 +592,7 @@ JABAS_API int jabas_loss_backward(const JabasLoss* l, const float* upstream, voi
     lay.in_dtype = l->dtype;
     lay.cols = static_cast<int32_t>(l->width);
     lay.planes = s.planes;
+    lay.low = 1.0f;
     lay.parts = b.parts;
     if (d_weight) {
         lay.peaks = b.peaks;        // a feature of large values, or a row of a large gradient, takes no bits from the other features

@@ -28,7 +28,7 @@ struct BF16 {
 
 // Tile: kM x kN of the output, by WM x WN waves, each kI x kJ blocks of 32 x 32. P planes of an operand. An
 // operand lies with its inner axis contiguous (rows of m or n), or, TA / TB, the other way round: rows of k, m or n contiguous.
-// RAISED: b's second plane is kLowScale times what it stands for, so a's first is made as much smaller for it.
+// RA / RB: a's / b's second plane is kLowScale times what it stands for, so the other's first is made as much smaller for it.
 //
 // The inner axis goes in steps of 64 elements (two planes: 32 of each) through two stages of LDS. The loads write LDS
 // themselves, 16 bytes a lane in lane order, so what keeps banks apart is which element a lane fetches:
@@ -44,7 +44,7 @@ struct BF16 {
 // 128 x 128, which read LDS a third less, came out even.
 // The loads are inline assembly because the compiler would wait for all of them before any later LDS read; they have no
 // register outputs, and the wait in front of the barrier covers them.
-template <class E, int P, int TM, int TN, int WM, int WN, bool TA, bool TB, bool RAISED>
+template <class E, int P, int TM, int TN, int WM, int WN, bool TA, bool TB, bool RA, bool RB>
 struct Core {
     static constexpr bool kTa = TA, kTb = TB;
     static constexpr int kM = TM, kN = TN, kThreads = 64 * WM * WN;
@@ -135,13 +135,16 @@ struct Core {
     template <class Between>
     __device__ void multiply(const Fragments& f, const Between& between) {
         int t = 0;
+        vec b0[kJ];
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) b0[j] = RA ? E::lowered(f.b[j][0]) : f.b[j][0];
 #pragma unroll
         for (int i = 0; i < kI; ++i) {
-            const vec a0 = RAISED ? E::lowered(f.a[i][0]) : f.a[i][0];
+            const vec a0 = RB ? E::lowered(f.a[i][0]) : f.a[i][0];
 #pragma unroll
             for (int j = 0; j < kJ; ++j) {
                 if (P == 2) {       // (a0 + a1)(b0 + b1) without a1 b1, which is under 2^-22 of the whole
-                    acc[i][j] = E::mfma(f.a[i][P - 1], f.b[j][0], acc[i][j]);
+                    acc[i][j] = E::mfma(f.a[i][P - 1], b0[j], acc[i][j]);
                     between(t++);
                     acc[i][j] = E::mfma(a0, f.b[j][P - 1], acc[i][j]);
                     between(t++);

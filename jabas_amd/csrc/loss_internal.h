@@ -140,6 +140,7 @@ struct LayArgs {
     int64_t out_stride, out_plane;
     int32_t pad;                // a multiple of 64
     int32_t planes;             // 0: copied as they are; 1 or 2 planes of fp16
+    float low;                  // what the second plane is multiplied by: 1 or kLowScale
     void* zero;                 // launch_lay_rows: [row of the call][cols] of in_dtype whose rows that do not count are zeroed, or NULL
     uint32_t* name;             // launch_lay_rows: zeros, in which the bits of the rows' labels and entries are set, or NULL
     Entries entries;

@@ -524,7 +524,7 @@ int launch(K kernel, int64_t grid, int threads, const A& args, hipStream_t strea
 
 template <class E, int P, int TM, int TN, int WM, int WN>
 int logits(const LogitsArgs& a, bool backward, hipStream_t stream) {
-    using C = Core<E, P, TM, TN, WM, WN, false, false, false>;
+    using C = Core<E, P, TM, TN, WM, WN, false, false, P == 2, false>;
     const int64_t grid = static_cast<int64_t>(tiles_m<C>(a.w.rows)) * tiles_n<C>(a.x.rows);
     if (a.entries.index)
         return backward ? launch(logits_backward_kernel<E, P, C, true>, grid, C::kThreads, a, stream) : launch(logits_forward_kernel<E, P, C, true>, grid, C::kThreads, a, stream);
@@ -538,8 +538,8 @@ int logits(const LogitsArgs& a, int planes, bool large, bool backward, hipStream
 
 template <int P, int TM, int TN, int WM, int WN>
 int grads(const GradArgs& a, hipStream_t stream) {
-    using CW = Core<F16, P, TM, TN, WM, WN, false, true, P == 2>;
-    using CH = Core<F16, P, TM, TN, WM, WN, P == 2, false, P == 2>;
+    using CW = Core<F16, P, TM, TN, WM, WN, false, true, false, P == 2>;
+    using CH = Core<F16, P, TM, TN, WM, WN, P == 2, false, P == 2, P == 2>;
     const int64_t grid = static_cast<int64_t>(tiles_m<CW>(a.w.m)) * tiles_n<CW>(a.w.n) * a.w.splits + static_cast<int64_t>(tiles_m<CH>(a.h.m)) * tiles_n<CH>(a.h.n) * a.h.splits;
     return launch(grads_kernel<CW, CH>, grid, CW::kThreads, a, stream);
 }
@@ -661,7 +661,10 @@ namespace {
 constexpr int kLayThreads = 256;
 
 // The power of two that takes `peak` to [2^14, 2^15): both planes of an element then fit fp16, elements down to 2^-16
-// of the largest keep 22 bits, and smaller ones are off by 2^-40 of it at most.
+// of the largest keep 22 bits, and smaller ones are off by 2^-40 of it at most. With a second plane that is raised by kLowScale they are off by
+// 2^-51: the weight's is, because the backward pass takes a piece of it by one scale for the product that sums over the tokens, and a weight
+// of 1e6 among others of 0.03 would leave their logits at 4e-5 where the forward pass, a scale per token, has them at 1e-7. What it costs is
+// one more multiplication of the other operand's fragments: 1600 x 32317 x 1024 1.5 % of a pass.
 __device__ inline int scale_exponent(float peak) {
     if (!(peak > 0.0f)) return 0;
     int e = static_cast<int>((__float_as_uint(peak) >> 23) & 0xff) - 126;
@@ -708,7 +711,7 @@ __device__ inline void store_eight(const LayArgs& a, int64_t row, int c, const f
     for (int i = 0; i < 8; ++i) {
         hi[i] = static_cast<_Float16>(v[i]);
         const float f = static_cast<float>(hi[i]);
-        lo[i] = static_cast<_Float16>(fabsf(f) < INFINITY ? v[i] - f : 0.0f);
+        lo[i] = static_cast<_Float16>(fabsf(f) < INFINITY ? (v[i] - f) * a.low : 0.0f);
     }
     *reinterpret_cast<f16x8*>(p) = hi;
     if (a.planes == 2) *reinterpret_cast<f16x8*>(p + a.out_plane) = lo;

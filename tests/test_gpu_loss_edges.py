@@ -155,6 +155,34 @@ def test_a_row_far_above_one_leaves_the_others_alone(gpu, rows, dtype, how):
         assert bool(((_cpu(g) - want).abs() <= rel * size + last * want.abs()).all())
 
 
+@pytest.mark.parametrize("rows", [20, 80, 300, 514])
+@pytest.mark.parametrize("form", ["labels", "entries"])
+@pytest.mark.parametrize("outlier", [1e5, 1e8])
+def test_one_large_weight_does_not_blur_the_others(gpu, rows, form, outlier):
+    """fp32, one weight far above the others in a feature that no hidden state uses: the logits of the backward pass are as good as the
+    forward pass's, so dW and db are. dX sums over the tokens, and its planes of the weight have one scale for a piece: off by 2^-40 of the largest
+    weight for each unit of a row's dz."""
+    vocab, width = 17000 if rows == 514 else 2001, 64
+    (x, w, b), gen = _inputs(gpu, rows, vocab, width, "fp32", True, seed=rows)
+    with torch.no_grad():
+        x[:, 5] = 0.0
+        w[77, 5] = outlier
+    if form == "labels":
+        target = torch.randint(0, vocab, (rows,), generator=gen)
+        loss = losses.linear_cross_entropy(x, w, target.to(gpu), b)
+        ref = Reference(x, w, b, target=target)
+    else:
+        index, teacher = _entries(gen, rows, vocab, 9, "fp32")
+        loss = losses.linear_topk_distillation(x, w, index.to(gpu), teacher.to(gpu), b)
+        ref = Reference(x, w, b, index=index, teacher=teacher)
+    grads = _grads(loss, (x, w, b))
+    gx, sx = ref.grads.pop(0), ref.sizes.pop(0)
+    ref.check(loss, grads[1:], "fp32")
+    each = ref.sizes[1].sum() / rows * 1.5                   # the sum of a row's |dz|, about the same for all of them
+    unit = 2.0 ** -20 * (ref.Z + 4.0)
+    assert bool(((_cpu(grads[0]) - gx).abs() <= (unit + 2.0 ** -20) * sx + 2.0 ** -40 * outlier * each + 2.0 ** -22 * gx.abs()).all())
+
+
 # ------------------------------------------------------------------ tokens ruled out, and named all the same
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("rows", [20, 80, 514])
