@@ -10,7 +10,9 @@ They stand in for the translation model's classifier (examples/gnmt/seq2seq/mode
 the vision examples' ``CrossEntropyLoss``; a trainer calls them as ``criterion(model(x), y)`` (jabas/train/trainer.py:82-86,
 171-174), see :class:`LinearCrossEntropy` and :class:`LinearTopkDistillation`.
 
-All of them are autograd functions on the current stream of the tensors' device; there is no CPU path. Every input keeps its
+All of them are autograd functions on the current stream of the tensors' device; there is no CPU path. What records or replaces
+operations (torch.jit.trace, make_fx, torch.compile, a dispatch or function mode) sees them as the operators ``jabas::loss_forward`` and
+``jabas::loss_backward``. Every input keeps its
 place in memory: nothing is changed in place, nothing is kept between calls but what autograd saves (the inputs, 16 bytes a
 row, 8 bytes an entry of the teacher). Results are the same from run to run: no sum depends on the order of atomics.
 """
@@ -21,7 +23,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
-from .sync import _stream_ptr
+from .sync import _stream_ptr, _watched
 
 REDUCTIONS = {"none": L.LOSS_NONE, "mean": L.LOSS_MEAN, "sum": L.LOSS_SUM}
 MAX_ENTRIES = L.LOSS_MAX_ENTRIES
@@ -103,6 +105,11 @@ def _call(spec, hidden, weight, bias, logits, target, teacher_index, teacher_log
     return c
 
 
+def _sizes(rows, k, reduction):
+    """Shapes of the loss and of the state."""
+    return (rows,) if reduction == L.LOSS_NONE else (), 4 * rows + 4 + 2 * rows * k
+
+
 def _workspace(c, backward, device):
     n = L.lib().jabas_loss_workspace_bytes(C.byref(c), backward)
     # 256 bytes are what the caching allocator aligns to at least
@@ -117,8 +124,9 @@ def _forward(spec, tensors):
         with torch.cuda.device(device):
             return _forward(spec, tensors)
     k = 0 if tensors[5] is None else tensors[5].shape[1]
-    state = torch.empty(4 * rows + 4 + 2 * rows * k, dtype=torch.float32, device=device)
-    out = torch.empty(rows if spec[0] == L.LOSS_NONE else (), dtype=torch.float32, device=device)
+    shape, words = _sizes(rows, k, spec[0])
+    state = torch.empty(words, dtype=torch.float32, device=device)
+    out = torch.empty(shape, dtype=torch.float32, device=device)
     c = _call(spec, *tensors, state)
     ws, n = _workspace(c, 0, device)
     L.check(L.lib().jabas_loss_forward(C.byref(c), out.data_ptr(), ws.data_ptr(), n, _stream_ptr()), "jabas_loss_forward")
@@ -140,6 +148,80 @@ def _backward(spec, tensors, state, needs, upstream):
     return grads
 
 
+# The same two steps as operators, for whoever watches operations: a launch through the C ABI is not seen by a recorder, which would hold
+# the results' memory and nothing that writes it. Their dispatch costs more than a small call's launches, so others go without.
+_LIBRARY = torch.library.Library("jabas", "DEF")
+_TENSORS = ("hidden", "weight", "bias", "logits", "target", "teacher_index", "teacher_logits", "teacher_lse")
+_CALL = ", ".join(f"Tensor? {t}" for t in _TENSORS) + ", int reduction, int ignore_index, float label_smoothing, float temperature"
+_LIBRARY.define(f"loss_forward({_CALL}) -> (Tensor, Tensor)")
+_LIBRARY.define(f"loss_backward({_CALL}, Tensor state, Tensor upstream, bool[] needs) -> Tensor[]")
+
+
+def _op_forward(*args):
+    return _forward(args[8:12], args[:8])
+
+
+def _op_backward(*args):
+    *_, state, upstream, needs = args
+    return [g for g in _backward(args[8:12], args[:8], state, needs, upstream) if g is not None]
+
+
+_LIBRARY.impl("loss_forward", _op_forward, "CUDA")
+_LIBRARY.impl("loss_backward", _op_backward, "CUDA")
+
+
+@torch.library.register_fake("jabas::loss_forward", lib=_LIBRARY)
+def _fake_forward(*args):
+    main = args[3] if args[0] is None else args[0]
+    shape, words = _sizes(main.shape[0], 0 if args[5] is None else args[5].shape[1], args[8])
+    return main.new_empty(shape, dtype=torch.float32), main.new_empty(words, dtype=torch.float32)
+
+
+@torch.library.register_fake("jabas::loss_backward", lib=_LIBRARY)
+def _fake_backward(*args):
+    return [t.new_empty(t.shape) for t, need in zip(args[:4], args[-1]) if t is not None and need]
+
+
+def _op_setup(ctx, inputs, output):
+    ctx.spec = inputs[8:]
+    ctx.save_for_backward(*inputs[:8], output[1])
+
+
+def _op_grads(spec, tensors, state, needs, upstream):
+    """What ``_backward`` returns, through the operator."""
+    needs = [t is not None and need for t, need in zip(tensors, needs)]
+    grads = iter(torch.ops.jabas.loss_backward(*tensors, *spec, state, upstream, needs))
+    return [next(grads) if need else None for need in needs]
+
+
+def _op_gradient(ctx, upstream, _):
+    *tensors, state = ctx.saved_tensors
+    return (*_op_grads(ctx.spec, tensors, state, ctx.needs_input_grad[:4], upstream), *[None] * 8)
+
+
+def _op_no_gradient(ctx, *upstream):
+    raise RuntimeError("the losses can be differentiated once")
+
+
+torch.library.register_autograd("jabas::loss_forward", _op_gradient, setup_context=_op_setup, lib=_LIBRARY)
+torch.library.register_autograd("jabas::loss_backward", _op_no_gradient, lib=_LIBRARY)
+_HELD = torch.Tensor, torch.nn.Parameter
+_compiles, _traces, _transform = torch.compiler.is_dynamo_compiling, torch._C._is_tracing, torch._C._functorch.peek_interpreter_stack
+_dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+
+
+def _direct(*tensors):
+    """Whether kernels may read the tensors, and write others, without anyone being told: nothing watches (``_watched``, in fewer steps: a
+    small call's time is the host's), no function transform is under way, and memory holds what the tensors stand for (tensors
+    without memory of their own have no address to ask for)."""
+    if _compiles() or _traces() or _dispatch_modes() or _transform() is not None or (_function_modes() and _watched()):
+        return False
+    for t in tensors:
+        if t is not None and (type(t) not in _HELD or t.is_neg() or t._is_zerotensor()):
+            return False
+    return True
+
+
 class _Loss(torch.autograd.Function):
     """``spec``: what is no tensor. The tensors come one by one so that autograd sees them."""
 
@@ -154,10 +236,13 @@ class _Loss(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, upstream):
         *tensors, state = ctx.saved_tensors
-        return (None, *_backward(ctx.spec, tensors, state, ctx.needs_input_grad[1:5], upstream), None, None, None, None)
+        run = _backward if _direct(upstream) else _op_grads         # the others are what the forward pass read
+        return (None, *run(ctx.spec, tensors, state, ctx.needs_input_grad[1:5], upstream), None, None, None, None)
 
 
 def _apply(spec, *tensors):
+    if not _direct(*tensors):
+        return torch.ops.jabas.loss_forward(*tensors, *spec)[0]
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors[:4]):
         return _Loss.apply(spec, *tensors)
     return _forward(spec, tensors)[0]

@@ -261,3 +261,100 @@ def test_rows_without_upstream_have_no_gradient(gpu, path, dtype):
         assert not bool(grads[0][::3].any())
         Reference(x[keep.to(gpu)], w, b, reduction="none", upstream=up[keep], **held).check(
             loss[keep.to(gpu)], [grads[0][keep.to(gpu)], *grads[1:]], dtype)
+
+
+# ------------------------------------------------------------------ recorders, derivatives, streams
+def _scored(gpu, seed, rows=70):
+    (x, w, b), gen = _inputs(gpu, rows, 300, 64, "fp32", True, seed=seed)
+    target = torch.randint(0, 300, (rows,), generator=gen).to(gpu)
+    index, teacher = (t.to(gpu) for t in _entries(gen, rows, 300, 5, "fp32"))
+    return [t.detach() for t in (x, w, b)], target, index, teacher
+
+
+def _score(x, w, b, target, index, teacher):
+    return (losses.linear_cross_entropy(x, w, target, b, reduction="none"), losses.linear_topk_distillation(x, w, index, teacher, b),
+            losses.topk_distillation(x, index % 64, teacher, temperature=2.0))
+
+
+def _train(x, w, b, target, index, teacher):
+    x, w, b = (t.detach().requires_grad_(True) for t in (x, w, b))
+    a, c, d = _score(x, w, b, target, index, teacher)
+    return a, c, d, *torch.autograd.grad(a.sum() + c + d, (x, w, b))
+
+
+@pytest.mark.parametrize("rows", [20, 70])
+@pytest.mark.parametrize("recorder,what", [(r, _score) for r in ("trace", "real", "fake", "symbolic", "aot_eager")] +
+                         [(r, _train) for r in ("real", "fake", "symbolic")])        # the other two record no backward pass inside a program
+def test_recorded_calls_answer_for_other_inputs(gpu, recorder, what, rows):
+    """A recording of a call holds the loss, not the memory that it was written to."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    (leaves, *rest), (others, *others_rest) = _scored(gpu, 1, rows), _scored(gpu, 2, rows)
+    args, other = (*leaves, *rest), (*others, *others_rest)
+    if recorder == "trace":
+        recorded = torch.jit.trace(what, args, check_trace=False)
+    elif recorder == "aot_eager":
+        recorded = torch.compile(what, backend="aot_eager")
+        recorded(*args)
+    else:
+        recorded = make_fx(what, tracing_mode=recorder)(*args)
+    want = what(*other)
+    torch.empty(1 << 20, device=gpu).fill_(float("nan"))
+    for got in (recorded(*other), recorded(*other)):
+        assert len(got) == len(want)
+        for p, q in zip(got, want):
+            assert torch.equal(p, q)
+
+
+def test_a_traced_module_trains(gpu):
+    """The gradients of a recorded call are the eager ones."""
+    (x, w, b), target, _, _ = _scored(gpu, 1)
+    (y, v, c), t, _, _ = _scored(gpu, 2)
+    call = lambda x, w, b, t: losses.linear_cross_entropy(x, w, t, b, label_smoothing=0.1)
+    leaves = [t.requires_grad_(True) for t in (y, v, c)]
+    want = torch.autograd.grad(call(*leaves, t), leaves)
+    for recorded in (torch.jit.trace(call, (x.requires_grad_(True), w, b, target), check_trace=False), torch.compile(call, backend="aot_eager")):
+        for _ in range(2):
+            for p, q in zip(torch.autograd.grad(recorded(*leaves, t), leaves), want):
+                assert torch.equal(p, q)
+
+
+def test_calls_under_modes_are_the_same(gpu):
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Above(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    seen = []
+
+    class Below(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    leaves, *rest = _scored(gpu, 3)
+    want = _train(*leaves, *rest)
+    for mode in (Above(), Below(), torch.device("cpu")):
+        with mode:
+            got = _train(*leaves, *rest)
+        for p, q in zip(got, want):
+            assert torch.equal(p, q)
+    assert sum("jabas" in s for s in seen) == 6         # three losses and their gradients are seen
+
+
+def test_values_that_memory_does_not_hold(gpu):
+    """A lazy negation is taken as what it stands for; so are tensors inside a function transform."""
+    (x, w, b), target, index, teacher = _scored(gpu, 4)
+    got = losses.linear_cross_entropy(torch._neg_view(x), torch._neg_view(w), target, torch._neg_view(b), reduction="none")
+    assert torch.equal(got, losses.linear_cross_entropy(-x, -w, target, -b, reduction="none"))
+    got = losses.topk_distillation(torch._neg_view(x), index % 64, torch._neg_view(teacher), reduction="none")
+    assert torch.equal(got, losses.topk_distillation(-x, index % 64, -teacher, reduction="none"))
+    call = lambda x: losses.linear_cross_entropy(x, w, target, b)
+    leaf = x.clone().requires_grad_(True)
+    up = torch._neg_view(torch.rand(len(x), device=gpu))
+    each = losses.linear_cross_entropy(leaf, w, target, b, reduction="none")
+    assert torch.equal(torch.autograd.grad(each, leaf, up, retain_graph=True)[0], torch.autograd.grad(each, leaf, up.clone())[0])
+    assert torch.equal(torch.func.vmap(call)(torch.stack([x, -x])), torch.stack([call(x), call(-x)]))
+    with pytest.raises(RuntimeError):       # refused, not lost
+        torch.func.grad(call)(x)
