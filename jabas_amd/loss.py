@@ -20,6 +20,7 @@ import ctypes as C
 import struct
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -241,6 +242,8 @@ class _Loss(torch.autograd.Function):
 
 
 def _apply(spec, *tensors):
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors[:4]):
+        raise RuntimeError("the losses have no forward-mode derivative")
     if not _direct(*tensors):
         return torch.ops.jabas.loss_forward(*tensors, *spec)[0]
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors[:4]):

@@ -358,3 +358,24 @@ def test_values_that_memory_does_not_hold(gpu):
     assert torch.equal(torch.func.vmap(call)(torch.stack([x, -x])), torch.stack([call(x), call(-x)]))
     with pytest.raises(RuntimeError):       # refused, not lost
         torch.func.grad(call)(x)
+
+
+def test_forward_mode_is_refused(gpu):
+    """There is no forward-mode derivative, and none is lost silently."""
+    import torch.autograd.forward_ad as forward
+    (x, w, b), target, index, teacher = _scored(gpu, 5)
+    with forward.dual_level():
+        dual = forward.make_dual(x, torch.ones_like(x))
+        calls = [lambda: losses.linear_cross_entropy(dual, w, target, b), lambda: losses.linear_topk_distillation(dual, w, index, teacher, b),
+                 lambda: losses.topk_distillation(dual, index % 64, teacher),
+                 lambda: losses.linear_cross_entropy(x, w, target, forward.make_dual(b, b)),
+                 lambda: losses.linear_cross_entropy(dual, w.clone().requires_grad_(True), target, b)]
+        for call in calls:
+            with pytest.raises(RuntimeError):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError):
+                call()
+        losses.linear_cross_entropy(x, w, target, b)
+        losses.topk_distillation(x, index % 64, forward.make_dual(teacher, teacher))       # nothing flows to the teacher
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: losses.linear_cross_entropy(x, w, target, b), (x,), (x,))
