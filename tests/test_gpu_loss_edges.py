@@ -183,6 +183,30 @@ def test_one_large_weight_does_not_blur_the_others(gpu, rows, form, outlier):
     assert bool(((_cpu(grads[0]) - gx).abs() <= (unit + 2.0 ** -20) * sx + 2.0 ** -40 * outlier * each + 2.0 ** -22 * gx.abs()).all())
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows", [80, 514])
+def test_improbable_tokens_to_the_absolute_step(gpu, rows, dtype):
+    """Tokens whose every probability is about e^-25: with many rows their row gradients are held in steps of 2^-39 (bf16) and 2^-50 (fp32) of the
+    upstream gradient, so their rows of dW are off by half a step for each hidden state beside what is relative."""
+    vocab, width = 17000, 64
+    (x, w, b), gen = _inputs(gpu, rows, vocab, width, dtype, True, seed=rows)
+    with torch.no_grad():
+        b[1000:1200] -= 25.0
+        b[1200:1300] -= 15.0
+    target = torch.randint(0, 1000, (rows,), generator=gen)
+    loss = losses.linear_cross_entropy(x, w, target.to(gpu), b, reduction="sum")
+    grads = _grads(loss, (x, w, b))
+    ref = Reference(x, w, b, target=target, reduction="sum")
+    half = 2.0 ** (-40 if dtype == "bf16" else -51)
+    unit = 2.0 ** -20 * (ref.Z + 4.0) + (2.0 ** -10 if dtype == "bf16" else 2.0 ** -20)
+    last = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -22
+    off, rare = (_cpu(grads[1]) - ref.grads[1]).abs(), slice(1000, 1300)
+    assert bool((off <= unit * ref.sizes[1] + half * _cpu(x).abs().sum(0) + last * ref.grads[1].abs())[rare].all())
+    # db is summed in 32 bits in front of the rounding
+    off = (_cpu(grads[2]) - ref.grads[2]).abs()
+    assert bool((off <= (unit + last) * ref.sizes[2])[rare].all())
+
+
 # ------------------------------------------------------------------ tokens ruled out, and named all the same
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("rows", [20, 80, 514])
@@ -261,6 +285,59 @@ def test_rows_without_upstream_have_no_gradient(gpu, path, dtype):
         assert not bool(grads[0][::3].any())
         Reference(x[keep.to(gpu)], w, b, reduction="none", upstream=up[keep], **held).check(
             loss[keep.to(gpu)], [grads[0][keep.to(gpu)], *grads[1:]], dtype)
+
+
+# ------------------------------------------------------------------ means, and weights past 32 bits
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows,vocab,width", [(20, 3001, 64), (64, 3001, 64), (130, 1003, 192), (514, 17000, 72), (2500, 2001, 70)])
+def test_a_mean_is_as_good_as_its_rows(gpu, rows, vocab, width, dtype):
+    """A mean of rows that are each off by 2^-19 (Z + 4) T^2 and 2^-20 of themselves is off by no more."""
+    (x, w, b), gen = _inputs(gpu, rows, vocab, width, dtype, True, seed=rows)
+    target = torch.randint(0, vocab, (rows,), generator=gen)
+    target[::7] = IGNORE
+    index = torch.randint(0, vocab // 8, (rows, 8), generator=gen) + torch.arange(8) * (vocab // 8)
+    index[1::7] = -1
+    teacher = torch.randn(rows, 8, generator=gen).to(TYPES[dtype])
+    lse = torch.logsumexp(teacher.float(), 1) + 0.5
+    z = (x.detach().float() @ w.detach().float().t()).to(TYPES[dtype])
+    entries = index.to(gpu), teacher.to(gpu)
+    for loss, ref in ((losses.linear_cross_entropy(x, w, target.to(gpu), b, label_smoothing=0.1), Reference(x, w, b, target=target, smoothing=0.1)),
+                      (losses.linear_topk_distillation(x, w, *entries, b, teacher_lse=lse.to(gpu)), Reference(x, w, b, index=index, teacher=teacher, lse=lse)),
+                      (losses.topk_distillation(z, *entries, teacher_lse=lse.to(gpu)), Reference(logits=z, index=index, teacher=teacher, lse=lse))):
+        bound = 2.0 ** -19 * (ref.Z + 4.0) + 2.0 ** -20 * float(ref.loss_size)
+        assert abs(float(loss.detach()) - float(ref.loss)) <= bound
+
+
+def test_gradients_of_a_weight_past_32_bits_of_offset(gpu):
+    """Two rows against 2.2e9 elements of weight: dX, summed over five pieces of the vocabulary, and dW at the pieces' borders and past element 2^31. dz is held
+    in two bf16 planes (2^-16), the logits are off by 2^-20 Z, and a result by a unit of its own (2^-8)."""
+    rows, vocab, width = 2, 540000, 4096
+    w = torch.empty(vocab, width, dtype=torch.bfloat16, device=gpu)
+    w.normal_(std=0.02, generator=torch.Generator(device=gpu).manual_seed(2))
+    x = torch.randn(rows, width, generator=_gen(3)).bfloat16().to(gpu).requires_grad_(True)
+    target = torch.tensor([vocab - 3, 1 << 17])
+    w.requires_grad_(True)
+    loss = losses.linear_cross_entropy(x, w, target.to(gpu), reduction="none")
+    gx, gw = _grads(loss.sum(), (x, w))
+    pieces = range(0, vocab, 30000)
+    xd, wd = x.detach().to(F64), w.detach()
+    z = torch.cat([xd @ wd[i:i + 30000].to(F64).t() for i in pieces], 1)
+    Z = max(float((xd.abs() @ wd[i:i + 30000].to(F64).abs().t()).max()) for i in pieces)
+    dz = torch.log_softmax(z, 1).exp_()
+    size = dz.clone()
+    for r in range(rows):
+        dz[r, target[r]] -= 1.0
+        size[r, target[r]] += 1.0
+    rel = 2.0 ** -20 * (Z + 4.0) + 2.0 ** -15
+    ref, sizes = torch.zeros(rows, width, dtype=F64, device=gpu), torch.zeros(rows, width, dtype=F64, device=gpu)
+    for i in pieces:
+        ref += dz[:, i:i + 30000] @ wd[i:i + 30000].to(F64)
+        sizes += size[:, i:i + 30000] @ wd[i:i + 30000].to(F64).abs()
+    assert bool(((gx.to(F64) - ref).abs() <= rel * sizes + 2.0 ** -8 * ref.abs()).all())
+    for at in (0, 1 << 17, 1 << 18, 3 << 17, 1 << 19, vocab):        # 2^31 elements: token 2^19
+        s = slice(max(0, at - 64), min(vocab, at + 64))
+        ref, sizes = dz[:, s].t() @ xd, size[:, s].t() @ xd.abs()
+        assert bool(((gw[s].to(F64) - ref).abs() <= rel * sizes + 2.0 ** -8 * ref.abs()).all())
 
 
 # ------------------------------------------------------------------ recorders, derivatives, streams
@@ -379,3 +456,32 @@ def test_forward_mode_is_refused(gpu):
         losses.topk_distillation(x, index % 64, forward.make_dual(teacher, teacher))       # nothing flows to the teacher
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda x: losses.linear_cross_entropy(x, w, target, b), (x,), (x,))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_calls_of_several_streams_at_once(gpu, dtype):
+    """Workers of different sizes on streams of their own, none waiting for another: each gets what it gets alone."""
+    work = []
+    for i, (rows, vocab, width) in enumerate([(300, 9000, 128), (20, 9000, 128), (514, 17000, 64), (90, 3000, 256)]):
+        (x, w, b), gen = _inputs(gpu, rows, vocab, width, dtype, True, seed=i)
+        target = torch.randint(0, vocab, (rows,), generator=gen).to(gpu)
+        index, teacher = (t.to(gpu) for t in _entries(gen, rows, vocab, 20, dtype))
+        work.append((x, w, b, target, index, teacher))
+
+    def step(x, w, b, target, index, teacher):
+        a = losses.linear_cross_entropy(x, w, target, b, label_smoothing=0.1)
+        c = losses.linear_topk_distillation(x, w, index, teacher, b, temperature=2.0)
+        return [a.detach(), c.detach(), *_grads(a, (x, w, b)), *_grads(c, (x, w, b))]
+
+    alone = [step(*job) for job in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    for _ in range(3):
+        got = []
+        for stream, job in zip(streams, work):
+            with torch.cuda.stream(stream):
+                got.append(step(*job))
+        torch.cuda.synchronize()
+        for a, b in zip(got, alone):
+            for p, q in zip(a, b):
+                assert torch.equal(p, q)
