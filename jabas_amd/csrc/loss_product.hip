@@ -818,14 +818,15 @@ __global__ __launch_bounds__(kLayThreads) void lay_rows_kernel(LayArgs a) {
 }
 
 // The largest size of each column, kPeakParts parts of the rows. A wave takes 512 columns of eight rows at a time.
-__global__ __launch_bounds__(kLayThreads) void column_peaks_kernel(LayArgs a) {
-    __shared__ float merge[kLayThreads / 64][512];
+constexpr int kPeakWaves = 16;
+__global__ __launch_bounds__(64 * kPeakWaves) void column_peaks_kernel(LayArgs a) {
+    __shared__ float merge[kPeakWaves][512];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = blockIdx.y * 512, c = first + lane * 8, rows = rows_of(a);
     constexpr int kOnTheirWay = 8;
-    const int apart = gridDim.x * (kLayThreads / 64);
+    const int apart = gridDim.x * kPeakWaves;
     float peak[8] = {};
     if (c < a.cols)
-        for (int place = blockIdx.x * (kLayThreads / 64) + wave; place < rows; place += kOnTheirWay * apart) {
+        for (int place = blockIdx.x * kPeakWaves + wave; place < rows; place += kOnTheirWay * apart) {
             float v[kOnTheirWay][8], f[kOnTheirWay];
             int row[kOnTheirWay];
 #pragma unroll
@@ -843,11 +844,12 @@ __global__ __launch_bounds__(kLayThreads) void column_peaks_kernel(LayArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) merge[wave][i * 64 + lane] = peak[i];
     __syncthreads();
-    for (int x = threadIdx.x; x < 512; x += kLayThreads) {
-        const int at = first + (x & 63) * 8 + (x >> 6);
-        const float top = fmaxf(fmaxf(merge[0][x], merge[1][x]), fmaxf(merge[2][x], merge[3][x]));
-        if (at < a.cols) a.peaks[blockIdx.x * a.peak_stride + at] = top;
-    }
+    const int x = threadIdx.x, at = first + (x & 63) * 8 + (x >> 6);
+    if (x >= 512 || at >= a.cols) return;
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPeakWaves; ++i) top = fmaxf(top, merge[i][x]);
+    a.peaks[blockIdx.x * a.peak_stride + at] = top;
 }
 
 // Bound by memory: 134 MB in 21 us (6.4 TB/s).
@@ -892,7 +894,7 @@ __global__ __launch_bounds__(kLayThreads) void lay_columns_kernel(LayArgs a) {
         const int c = c0 + (t & 63);
         float peak = 0.0f;
 #pragma unroll
-        for (int i = t >> 6; i < kPeakParts; i += kLayThreads / 64) peak = fmaxf(peak, c < a.cols ? a.peaks[i * a.peak_stride + c] : 0.0f);
+        for (int i = 0; i < kPeakParts; i += kLayThreads / 64) peak = fmaxf(peak, c < a.cols ? a.peaks[(i + (t >> 6)) * a.peak_stride + c] : 0.0f);
         peaks[t >> 6][t & 63] = peak;
         __syncthreads();
     } else {
@@ -922,7 +924,7 @@ int launch_lay_rows(const LayArgs& a, hipStream_t stream) {
 
 int launch_lay_columns(const LayArgs& a, hipStream_t stream) {
     void* params[] = {const_cast<LayArgs*>(&a)};
-    const hipError_t error = a.peaks ? hipLaunchKernel(reinterpret_cast<const void*>(column_peaks_kernel), dim3(kPeakParts, (a.cols + 511) / 512), dim3(kLayThreads), params, 0, stream)
+    const hipError_t error = a.peaks ? hipLaunchKernel(reinterpret_cast<const void*>(column_peaks_kernel), dim3(kPeakParts, (a.cols + 511) / 512), dim3(64 * kPeakWaves), params, 0, stream)
                                      : hipLaunchKernel(reinterpret_cast<const void*>(absmax_kernel), dim3(kMaxParts), dim3(kLayThreads), params, 0, stream);
     if (error != hipSuccess) return JABAS_ERR_LAUNCH;
     return hipLaunchKernel(reinterpret_cast<const void*>(lay_columns_kernel), dim3(a.pad / 64, (a.cols + 63) / 64), dim3(kLayThreads), params, 0, stream) == hipSuccess
