@@ -272,16 +272,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void narrow_backw
 }
 
 // Four consecutive elements of a row from column c on, zeros past the end.
-template <class T>
-__device__ inline f32x4 load_four(const T* row, int c, int cols) {
+__device__ inline f32x4 load_four(const float* row, int c, int cols) {
     f32x4 v;
     if (c + 4 <= cols) {
-        const Some<T, 4> x = *reinterpret_cast<const Some<T, 4>*>(row + c);
+        const Some<float, 4> x = *reinterpret_cast<const Some<float, 4>*>(row + c);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = widen(x.v[i]);
+        for (int i = 0; i < 4; ++i) v[i] = x.v[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = c + i < cols ? widen(row[c + i]) : 0.0f;
+        for (int i = 0; i < 4; ++i) v[i] = c + i < cols ? row[c + i] : 0.0f;
     }
     return v;
 }
@@ -299,9 +298,9 @@ __device__ inline void store_four(T* row, int c, int cols, f32x4 v) {
     }
 }
 
-// dW of 32 tokens: the sum over rows is the inner axis, two at a time; the waves take 128 features in turn.
-template <class T, int RB>
-__device__ inline void narrow_weight(const NarrowArgs& a, int64_t unit) {
+// dW of 32 tokens, fp32: the sum over rows is the inner axis, two at a time; the waves take 128 features in turn.
+template <int RB>
+__device__ inline void narrow_weight_fp32(const NarrowArgs& a, int64_t unit) {
     constexpr int R = RB * 32;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, half = lane >> 5;
     const int64_t from = unit * kTokens, first = a.first + from;
@@ -320,7 +319,7 @@ __device__ inline void narrow_weight(const NarrowArgs& a, int64_t unit) {
         for (int i = 0; i < R / 2; ++i) {
             if (2 * i >= a.rows) break;
             const int n = 2 * i + half;
-            f32x4 x = load_four(static_cast<const T*>(a.x) + static_cast<int64_t>(min(n, a.rows - 1)) * a.x_stride, h + 4 * r, a.width);
+            f32x4 x = load_four(static_cast<const float*>(a.x) + static_cast<int64_t>(min(n, a.rows - 1)) * a.x_stride, h + 4 * r, a.width);
             if (!((live >> n) & 1)) x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(d[i], x[c], acc[c], 0, 0, 0);
@@ -328,7 +327,7 @@ __device__ inline void narrow_weight(const NarrowArgs& a, int64_t unit) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const int64_t v = first + block_m(e);
-            if (v < a.vocab) store_four(static_cast<T*>(a.d_weight) + v * a.width, h + 4 * r, a.width, f32x4{acc[0][e], acc[1][e], acc[2][e], acc[3][e]});
+            if (v < a.vocab) store_four(static_cast<float*>(a.d_weight) + v * a.width, h + 4 * r, a.width, f32x4{acc[0][e], acc[1][e], acc[2][e], acc[3][e]});
         }
     }
 }
@@ -501,9 +500,9 @@ __device__ inline void narrow_hidden_bf16(const NarrowArgs& a, int64_t unit, flo
         for (int g = 0; g < F; g += 4) narrow_merge<uint16_t>(a, b, split, h + F * r + g, acc[b][g], acc[b][g + 1], acc[b][g + 2], acc[b][g + 3], merge);
 }
 
-// dX of 128 features over a range of tokens: eight at a time, four to each half of a wave; the waves take blocks of 32 tokens in turn.
-template <class T, int RB>
-__device__ inline void narrow_hidden(const NarrowArgs& a, int64_t unit, float* merge) {
+// dX of 128 features over a range of tokens, fp32: eight at a time, four to each half of a wave; the waves take blocks of 32 tokens in turn.
+template <int RB>
+__device__ inline void narrow_hidden_fp32(const NarrowArgs& a, int64_t unit, float* merge) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, half = lane >> 5;
     const int slices = (a.width + 127) / 128, h = static_cast<int>(unit % slices) * 128, split = static_cast<int>(unit / slices);
     const int64_t begin = split * a.each, end = min(begin + a.each, a.tokens);
@@ -517,7 +516,7 @@ __device__ inline void narrow_hidden(const NarrowArgs& a, int64_t unit, float* m
     const bool whole = h + 128 <= a.width && a.first + end <= a.vocab && end - begin == a.each;
     for (int64_t v = begin + wave * 32; v < end; v += 128) {
         f32x4 d[4][RB], w[4][4];
-        const T* row = static_cast<const T*>(a.w) + (a.first + v + half * 4) * a.w_stride + h + 4 * r;
+        const float* row = static_cast<const float*>(a.w) + (a.first + v + half * 4) * a.w_stride + h + 4 * r;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
 #pragma unroll
@@ -528,7 +527,7 @@ __device__ inline void narrow_hidden(const NarrowArgs& a, int64_t unit, float* m
             } else {
 #pragma unroll
                 for (int t = 0; t < 4; ++t)     // tokens past the end: the last one again, against a zero of dz
-                    w[q][t] = load_four(static_cast<const T*>(a.w) + min(a.first + v + q * 8 + half * 4 + t, a.vocab - 1) * a.w_stride, h + 4 * r, a.width);
+                    w[q][t] = load_four(static_cast<const float*>(a.w) + min(a.first + v + q * 8 + half * 4 + t, a.vocab - 1) * a.w_stride, h + 4 * r, a.width);
             }
         }
 #pragma unroll
@@ -541,7 +540,7 @@ __device__ inline void narrow_hidden(const NarrowArgs& a, int64_t unit, float* m
                     for (int c = 0; c < 4; ++c) acc[b][c] = __builtin_amdgcn_mfma_f32_32x32x2f32(d[q][b][t], w[q][t][c], acc[b][c], 0, 0, 0);
     }
 #pragma unroll
-    for (int b = 0; b < RB; ++b) narrow_merge<T>(a, b, split, h + 4 * r, acc[b][0], acc[b][1], acc[b][2], acc[b][3], merge);
+    for (int b = 0; b < RB; ++b) narrow_merge<float>(a, b, split, h + 4 * r, acc[b][0], acc[b][1], acc[b][2], acc[b][3], merge);
 }
 
 template <class T, int RB>
@@ -551,8 +550,8 @@ __global__ __launch_bounds__(kThreads, 2) void narrow_grads_kernel(NarrowArgs a)
         if (blockIdx.x < a.hidden_units) narrow_hidden_bf16<RB>(a, blockIdx.x, merge);
         else narrow_weight_bf16<RB>(a, blockIdx.x - a.hidden_units);
     } else {
-        if (blockIdx.x < a.hidden_units) narrow_hidden<T, RB>(a, blockIdx.x, merge);
-        else narrow_weight<T, RB>(a, blockIdx.x - a.hidden_units);
+        if (blockIdx.x < a.hidden_units) narrow_hidden_fp32<RB>(a, blockIdx.x, merge);
+        else narrow_weight_fp32<RB>(a, blockIdx.x - a.hidden_units);
     }
 }
 
