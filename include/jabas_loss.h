@@ -21,6 +21,10 @@
  * outside the vocabulary (a negative teacher index is "no entry") makes its row's loss and gradients NaN; no memory
  * outside the tensors is read.
  *
+ * Row gradients dL/dz of many rows (over 64; bf16 over a large weight: 32) are held in fp16 between kernels: 11 bits
+ * (bf16 calls) or 22 (fp32) of them, and below 2^-29 or 2^-25 of the row's upstream gradient times T in steps of 2^-39 or
+ * 2^-50 of it; few rows keep 16 and 24 bits at any size.
+ *
  * Sizes: from hidden and weight rows <= 2^22, vocab <= 2^28, width <= 2^20 and less than 2^23 tiles of 256 rows and 256
  * tokens; over logits rows times the parts of 32768 tokens of a row (more of them where rows are few) less than 2^24,
  * vocab <= 2^30. Others are JABAS_ERR_SIZE.

@@ -234,8 +234,8 @@ int launch_bias_sum(const float* parts, const int32_t* live, int32_t tile, int64
 int launch_zero(void* p, size_t bytes, hipStream_t stream);
 
 // Few rows, hidden states and weight as they lie (loss_narrow.hip). With bf16, whose tiles read the weight as it lies too, a second block
-// of rows pays for small weights only. Forward and backward, this and the tiles: fp32 16 x 32317 x 1024 170 and 434 us, 64 x 32317 x 1024 329
-// and 457, 64 x 131072 x 4096 3880 and 8716; bf16 1 x 32317 x 1024 107 and 171, 32 x 32317 x 1024 119 and 176, 32 x 131072 x 4096 1225 and
+// of rows pays for small weights only. Forward and backward, this and the tiles: fp32 16 x 32317 x 1024 170 and 434 us, 64 x 32317 x 1024 320
+// and 457, 64 x 131072 x 4096 3805 and 8716; bf16 1 x 32317 x 1024 107 and 171, 32 x 32317 x 1024 119 and 176, 32 x 131072 x 4096 1225 and
 // 2070, 64 x 4000 x 768 72 and 89, 64 x 8000 x 768 76 and 101, 64 x 16000 x 768 103 and 117,
 // 40 x 32317 x 1024 188 and 176, 64 x 32317 x 1024 209 and 177.
 constexpr int kNarrowRows = 64;

@@ -13,8 +13,10 @@
 // operands whose rows are that axis need no transposing; bf16's take 32x32x16 with four features of eight rows turned about in a lane's
 // registers. 8 rows, 131072 x 4096: dX 230 us with bf16 (4.7 TB/s), 525 with fp32 (4.1 TB/s), dW 300 and 457 us; with 32x32x2 and checked
 // loads for bf16 too both took 1081 us, 546 now. What bounds them is how much a CU has on its way, so two
-// workgroups have to fit one, with 33 to 64 rows too: 64 x 32317 x 1024 fp32 374 us with one, 329 with two, 64 x 131072 x 4096 4360 and 3880.
-// The logits' kernels do so with bf16 (64 x 16000 x 768 116 and 104 us); fp32's would have to spill (64 x 32317 x 1024 forward 93 and 120 us).
+// workgroups have to fit one, with 33 to 64 rows too, though registers run out there (120 bytes a lane with fp32, 260 with bf16 go to scratch
+// memory): 64 x 32317 x 1024 fp32 374 us with one, 320 with two, 64 x 131072 x 4096 4360 and 3805.
+// The logits' kernels do so with bf16 (64 x 16000 x 768 116 and 104 us); fp32's would have to spill (64 x 32317 x 1024 forward 93 and 120 us), so that
+// one wave a SIMD is left with 33 to 64 rows.
 #include "loss_internal.h"
 
 namespace jabas {

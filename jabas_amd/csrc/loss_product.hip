@@ -556,7 +556,7 @@ Sizes grads_tile(bool large) { return large ? Sizes{256, 256} : Sizes{128, 128};
 }  // namespace
 
 // A CU holds one workgroup of a large tile or two of a small one, whose round takes 0.6 of a large one's, or 0.55 behind fp32's backward
-// pass, whose large tile runs out of registers. Forward, then forward and backward, small and large, by 1024: 512 x 16384 (128 large tiles)
+// pass, whose large tile runs out of registers (112 bytes a lane go to scratch memory, 56 with entries; 48 in fp32's forward pass). Forward, then forward and backward, small and large, by 1024: 512 x 16384 (128 large tiles)
 // fp32 106 and 118 us; 512 x 32317 (254) fp32 185 and 170, 710 and 669, bf16 64.7 and 56.6, 286 and 274; 640 x 32317 (381) 231 and 237,
 // 829 and 876, 79 and 83, 341 and 349; 1280 x 32317 (635) 345 and 331, 1266 and 1286, 124 and 118, 496 and 491; 5120 x 32317 (2540) 1072
 // and 962, 4143 and 3988, 386 and 344, 1521 and 1430. 256 x 128 was no faster than the better of the two at any of these.

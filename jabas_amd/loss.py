@@ -5,16 +5,21 @@ logits in hand or straight from the hidden states and the classifier's weight. T
 product is worked through in tiles whose maxima and sums are all that leaves the chip, and the backward pass computes them
 again, a piece of the vocabulary at a time. K workers on one GPU hold K sets of activations, and [tokens, vocabulary] logits
 are the largest of them (6400 tokens over 32317 in fp32: 0.83 GB per worker, once for the logits and once for their gradient).
+Between the passes a call holds nothing of that size; while one runs, its workspace holds copies of the operands and a piece's
+row gradients: over a vocabulary of 32317 and 1024 features, forward and backward, 169 and 672 MB for 6400 rows in fp32, 23 and
+324 in bf16. Logits and their gradient would be 1655 and 827; up to about 1600 rows (142 and 396 MB in fp32, 414 of logits) they would be
+the smaller, so few tokens gain what is not held between the passes, and nothing at the peak.
 
 They stand in for the translation model's classifier (examples/gnmt/seq2seq/models/decoder.py) with its criterion and for
 the vision examples' ``CrossEntropyLoss``; a trainer calls them as ``criterion(model(x), y)`` (jabas/train/trainer.py:82-86,
 171-174), see :class:`LinearCrossEntropy` and :class:`LinearTopkDistillation`.
 
-All of them are autograd functions on the current stream of the tensors' device; there is no CPU path. What records or replaces
-operations (torch.jit.trace, make_fx, torch.compile, a dispatch or function mode) sees them as the operators ``jabas::loss_forward`` and
-``jabas::loss_backward``. Every input keeps its
-place in memory: nothing is changed in place, nothing is kept between calls but what autograd saves (the inputs, 16 bytes a
-row, 8 bytes an entry of the teacher). Results are the same from run to run: no sum depends on the order of atomics.
+All of them are autograd functions on the current stream of the tensors' device, once differentiable; there is no CPU path, and a
+forward-mode derivative or a function transform that differentiates is refused. What records or replaces operations (torch.jit.trace,
+make_fx, torch.compile, a dispatch or function mode) sees them as the operators ``jabas::loss_forward`` and ``jabas::loss_backward``.
+Every input keeps its place in memory: nothing is changed in place, nothing is kept between calls but what autograd saves (the
+inputs, 16 bytes a row, 8 bytes an entry of the teacher). Results are the same from run to run: no sum depends on the order of
+atomics.
 """
 import ctypes as C
 import struct
@@ -288,13 +293,19 @@ def linear_cross_entropy(hidden, weight, target, bias=None, *, ignore_index=-100
     hidden: (..., width) float32 or bfloat16; weight: (vocab, width) of the same type; bias: (vocab,) of the same type or
     None (-inf rules a token out); target: (...) int64. The loss of a row with logits z and label t is
     ``logsumexp(z) - (1 - e) z[t] - e mean(z)``, e = label_smoothing. Rows whose label is ``ignore_index`` do not count:
-    loss and gradient are 0 whatever their hidden states hold; a row whose upstream gradient is 0 has gradient 0 too. Any other label outside the vocabulary gives NaN.
+    loss and gradient are 0 whatever their hidden states hold; a row whose upstream gradient is 0 has gradient 0 too. Any
+    other label outside the vocabulary gives NaN, one that is ruled out an infinite loss.
 
     reduction: "mean" over the rows that count (0 where none does), "sum" or "none" (the shape of target). The loss is
-    float32, sums are kept in 32 bits; gradients have the inputs' type. With bfloat16 the products take the inputs as they
-    are and the row gradients as fp16 in units of 2^-15 (rounded once, an eighth of bfloat16's step), few rows' as two
-    bfloat16 planes (16 bits); with float32 every factor is split into two fp16 planes (22 bits) and the products into
-    three, few rows' products are float32's."""
+    float32, sums are kept in 32 bits; gradients have the inputs' type.
+
+    Up to 64 rows (bfloat16 over a large weight: 32) the products are float32's, or with bfloat16 take the inputs as they are
+    and the row gradients dz = dL/dz as two bfloat16 planes (16 bits at any size). More rows take dz as fp16: with bfloat16 one plane,
+    an eighth of bfloat16's step down to 2^-29 of the row's upstream gradient and steps of 2^-39 of it below, so that the part of dW or of
+    dX that comes from tokens less probable than 2^-40 is 0; with float32 two, 22 bits down to 2^-25 and steps of 2^-50. float32's
+    other factors are two fp16 planes too, the products three: 22 bits of a hidden state down to 2^-16 of the largest of its row
+    (for dW: of its feature), of a weight down to 2^-27 of the largest of its token (in the backward pass: of a piece of the vocabulary),
+    and a fixed step below."""
     x, w, b = _linear_inputs(hidden, weight, bias)
     lead = hidden.shape[:-1]
     _check_row_tensor(target, lead, torch.int64, hidden.device, "target")

@@ -418,6 +418,11 @@ def test_calls_under_modes_are_the_same(gpu):
         for p, q in zip(got, want):
             assert torch.equal(p, q)
     assert sum("jabas" in s for s in seen) == 6         # three losses and their gradients are seen
+    x = leaves[0].clone().requires_grad_(True)
+    with Below():
+        grad = torch.autograd.grad(losses.linear_cross_entropy(x, *leaves[1:2], rest[0]), x, create_graph=True)[0]
+        with pytest.raises(RuntimeError):
+            grad.sum().backward()               # once differentiable
 
 
 def test_values_that_memory_does_not_hold(gpu):
