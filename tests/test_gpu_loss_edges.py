@@ -490,3 +490,44 @@ def test_calls_of_several_streams_at_once(gpu, dtype):
         for a, b in zip(got, alone):
             for p, q in zip(a, b):
                 assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("rows", [80, 514])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("scale", [1e-30, 1e-6, 1e20])
+def test_many_rows_of_any_size_keep_their_bits(gpu, rows, dtype, scale):
+    """hidden * scale against weight / scale with many rows, whose operands are laid out by powers of two; the scale is one itself, so nothing is
+    rounded on the way."""
+    vocab, width = 17000 if rows == 514 else 700, 72
+    (x, w, _), gen = _inputs(gpu, rows, vocab, width, dtype, seed=rows)
+    scale = 2.0 ** round(math.log2(scale))
+    target = torch.randint(0, vocab, (rows,), generator=gen)
+    x, w = (x.detach() * scale).requires_grad_(True), (w.detach() / scale).requires_grad_(True)
+    loss = losses.linear_cross_entropy(x, w, target.to(gpu))
+    Reference(x, w, target=target).check(loss, _grads(loss, (x, w)), dtype)
+
+
+@pytest.mark.parametrize("rows", [80, 514])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("name", ["first", "padding", 1 << 40, -7])
+def test_names_outside_the_vocabulary_with_many_rows(gpu, rows, dtype, name):
+    """A label or an entry past the vocabulary, inside the last tile's padding too: its row is NaN, the others' losses and gradients of hidden states are
+    what they are without it."""
+    vocab, width, bad = 17000 if rows == 514 else 700, 64, 5
+    (x, w, b), gen = _inputs(gpu, rows, vocab, width, dtype, True, seed=rows)
+    name = {"first": vocab, "padding": vocab + 60}.get(name, name)
+    keep = torch.arange(rows) != bad
+    on = keep.to(gpu)
+    target = torch.randint(0, vocab, (rows,), generator=gen)
+    target[bad] = name
+    index, teacher = _entries(gen, rows, vocab, 4, dtype)
+    index[bad, 2] = name
+    calls = [(lambda: losses.linear_cross_entropy(x, w, target.to(gpu), b, reduction="none"), dict(target=target[keep]))]
+    if name >= 0:       # a negative one is no entry
+        calls.append((lambda: losses.linear_topk_distillation(x, w, index.to(gpu), teacher.to(gpu), b, reduction="none"),
+                      dict(index=index[keep], teacher=teacher[keep])))
+    for call, held in calls:
+        loss = call()
+        grads = _grads(loss, (x, w, b), torch.ones(rows, device=gpu))
+        assert bool(loss[bad].isnan()) and bool(grads[0][bad].isnan().all())
+        Reference(x[on], w, b, reduction="none", **held).check(loss[on], [grads[0][on]], dtype)
