@@ -1,4 +1,4 @@
-"""ctypes binding of libjabas_sync.so (the C ABI declared in include/jabas_sync.h and include/jabas_loss.h).
+"""ctypes binding of libjabas_sync.so (the C ABI declared in include/jabas_sync.h, include/jabas_loss.h and include/jabas_muon.h).
 
 The structures below mirror the headers field for field. There is no fallback: when
 the shared library is missing, :func:`lib` raises, and every product path that reaches
@@ -28,6 +28,9 @@ STATS_NONE, STATS_FULL, STATS_SIMILARITY, STATS_GRAM = 0, 1, 2, 3
 
 LOSS_MAX_ENTRIES = 255
 LOSS_NONE, LOSS_MEAN, LOSS_SUM = 0, 1, 2
+
+MUON_MAX_STEPS = 32
+MUON_MAX_SIDE, MUON_MAX_LENGTH = 1 << 16, 1 << 22
 
 STAT_DOT_AB, STAT_NORM_A, STAT_NORM_B, STAT_NORM_AGG, STAT_NORM_VSW0 = 0, 1, 2, 3, 4
 
@@ -120,6 +123,58 @@ class JabasLoss(C.Structure):
     ]
 
 
+class JabasNewtonSchulz(C.Structure):
+    _fields_ = [
+        ("a", C.c_double),
+        ("b", C.c_double),
+        ("c", C.c_double),
+        ("eps", C.c_double),
+        ("steps", C.c_int32),
+        ("precision", C.c_int32),
+    ]
+
+
+class JabasOrthogonalize(C.Structure):
+    _fields_ = [
+        ("in", C.c_void_p),
+        ("out", C.c_void_p),
+        ("batch", C.c_int64),
+        ("rows", C.c_int64),
+        ("cols", C.c_int64),
+        ("in_batch_stride", C.c_int64),
+        ("in_row_stride", C.c_int64),
+        ("dtype", C.c_int32),
+        ("reserved", C.c_int32),
+        ("ns", JabasNewtonSchulz),
+    ]
+
+
+class JabasMatrix(C.Structure):
+    _fields_ = [
+        ("grad", C.c_void_p),
+        ("momentum", C.c_void_p),
+        ("param", C.c_void_p),
+        ("fanout", C.c_void_p * (MAX_K - 1)),
+        ("rows", C.c_int64),
+        ("cols", C.c_int64),
+        ("lr_factor", C.c_double),
+        ("group", C.c_uint32),
+        ("n_fanout", C.c_uint32),
+    ]
+
+
+class JabasMuonArgs(C.Structure):
+    _fields_ = [
+        ("ns", JabasNewtonSchulz),
+        ("momentum", C.c_double),
+        ("nesterov", C.c_int32),
+        ("n_groups", C.c_int32),
+        ("lr", C.c_double * MAX_GROUPS),
+        ("weight_decay", C.c_double * MAX_GROUPS),
+        ("grad_scale", C.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); one entry per symbol jabas_sync.h declares.
 SIGNATURES = {
     "jabas_sync_version": (C.c_char_p, []),
@@ -170,6 +225,16 @@ LOSS_SIGNATURES = {
                                       C.c_void_p, C.c_size_t, C.c_void_p]),
 }
 
+# jabas_muon.h
+MUON_SIGNATURES = {
+    "jabas_orthogonalize_workspace_bytes": (C.c_size_t, [C.POINTER(JabasOrthogonalize)]),
+    "jabas_orthogonalize": (C.c_int, [C.POINTER(JabasOrthogonalize), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "jabas_muon_plan_bytes": (C.c_size_t, [C.POINTER(JabasMatrix), C.c_uint32, C.c_int32]),
+    "jabas_muon_plan_encode": (C.c_int, [C.POINTER(JabasMatrix), C.c_uint32, C.c_int32, C.c_void_p, C.c_size_t]),
+    "jabas_muon_workspace_bytes": (C.c_size_t, [C.c_void_p]),
+    "jabas_muon_step": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(JabasMuonArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+}
+
 _lib = None
 
 
@@ -194,7 +259,7 @@ def lib():
                 f"{LIB_PATH} is not built; run `python -c 'import __graft_entry__ as g; g.build()'` "
                 "or `make -C jabas_amd/csrc` (needs hipcc). There is no CPU fallback.")
         handle = C.CDLL(LIB_PATH)
-        for name, (res, args) in (SIGNATURES | LOSS_SIGNATURES).items():
+        for name, (res, args) in (SIGNATURES | LOSS_SIGNATURES | MUON_SIGNATURES).items():
             try:
                 fn = getattr(handle, name)
             except AttributeError:

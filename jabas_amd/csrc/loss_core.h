@@ -1,4 +1,4 @@
-// The matrix product under the losses' kernels: a workgroup's tile of out[n][m] = sum_k a[m][k] b[n][k] in registers.
+// The matrix product under the kernels of the losses and of the orthogonalised update: a workgroup's tile of out[n][m] = sum_k a[m][k] b[n][k] in registers.
 #pragma once
 
 #include "loss_internal.h"
@@ -35,7 +35,8 @@ struct BF16 {
 //   contiguous inner axis, one plane: rows of 128 bytes, chunk c of row r at c ^ (r / 2 % 8); two planes, each by itself: rows of 64
 //     bytes, chunk c at c ^ (r / 4 % 4). A fragment is one 16-byte read of 32 rows, 16 of them at a time over 64 banks.
 //     Measured: 230 bytes per clock and CU, against 120 with r % 8;
-//   rows of k: chunk c of row k at c ^ 4 (k % 4): the transposing 8-byte reads take four rows and 32 bytes of each at a time.
+//   rows of k: chunk c of row k at c ^ 4 (k % 4): the transposing 8-byte reads take four rows and 32 bytes of each at a time
+//     (tiles of 64, whose rows are half as long as the banks: c ^ 4 (k / 2 % 2)).
 // The last fragments of a step are in registers before the barrier that gives its stage to the loads of the step after the
 // next, and are multiplied behind it, while the next step's first fragments are read: neither the barrier nor the first read
 // leaves the matrix cores waiting. Reads and loads go between the products one by one: in a row in front of them they fill the
@@ -63,6 +64,12 @@ struct Core {
     // element e of a block: m = block_m, n = 32 j + lane % 32; four consecutive e are four consecutive m
     static __device__ int block_m(int i, int e) { return i * 32 + 8 * (e >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (e & 3); }
 
+    // What the chunks of row k of a tile of rows of k are turned by.
+    template <int T>
+    static __device__ int turned(int k) {
+        static_assert(T >= 64, "eight chunks a row at least");
+        return T >= 128 ? (k & 3) << 2 : (k & 2) << 1;
+    }
     // An operand's tile on its way: a uniform base per plane, which moves from step to step, and offsets of the lane's chunks.
     template <int T, bool TR>
     struct Source {
@@ -81,7 +88,7 @@ struct Core {
             for (int i = 0; i < kEach; ++i) {
                 const int f = i * kThreads + t;                 // the chunk's place in the plane's tile
                 if (TR) {
-                    const int k = f / (T / 8), c = (f % (T / 8)) ^ ((k & 3) << 2);
+                    const int k = f / (T / 8), c = (f % (T / 8)) ^ turned<T>(k);
                     const int col = min(first + c * 8, o.rows - 8);        // past the end: read again, never written
                     offset[i] = 2 * (static_cast<uint32_t>(k) * static_cast<uint32_t>(o.stride) + col);
                 } else {
@@ -108,7 +115,7 @@ struct Core {
         if (TR) {
             const int k = (P == 2 ? plane * 32 : 0) + kk * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2);
             const int m = at + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-            const int c = (m >> 3) ^ ((k & 3) << 2);
+            const int c = (m >> 3) ^ turned<T>(k);
             const char* p = tile + k * (T * 2) + c * 16 + (m & 4) * 2;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * (T * 2)));

@@ -1,0 +1,515 @@
+// Entry points of the orthogonalised update: argument validation, plans, workspace layout, and the order of the launches.
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+#include <new>
+#include <numeric>
+#include <vector>
+
+#include "muon_internal.h"
+
+#define JABAS_API extern "C" __attribute__((visibility("default")))
+
+namespace jabas {
+namespace muon {
+namespace {
+
+inline int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+inline bool misaligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
+constexpr int64_t kMaxSlots = int64_t{1} << 23;     // a launch has less than 2^32 threads, up to 512 a workgroup
+
+// What the products' factors are multiplied by, powers of two: no entry of a matrix is larger than its largest singular value, and how far
+// the polynomial lets those grow is known. Entries then lie under 2^14, and steps of fp16's second plane are 2^-38 of the largest or finer.
+struct Scales {
+    double x[JABAS_MUON_MAX_STEPS + 1], a[JABAS_MUON_MAX_STEPS], b[JABAS_MUON_MAX_STEPS];
+};
+double scale_for(double most) {
+    if (!(most > 0.0)) return 16384.0;
+    return ldexp(1.0, std::min(40, 14 - static_cast<int>(ceil(log2(most)))));
+}
+int scales_of(const JabasNewtonSchulz& ns, Scales& s) {
+    if (ns.precision != JABAS_F32 && ns.precision != JABAS_BF16) return JABAS_ERR_DTYPE;
+    if (ns.steps < 1 || ns.steps > JABAS_MUON_MAX_STEPS || !isfinite(ns.a) || !isfinite(ns.b) || !isfinite(ns.c)) return JABAS_ERR_OPT;
+    if (!(ns.eps >= 1e-30) || !isfinite(ns.eps)) return JABAS_ERR_OPT;
+    double most = 1.0;          // the largest singular value is at most the length, one
+    for (int k = 0; k < ns.steps; ++k) {
+        const double end = most * most;
+        const auto second = [&](double t) { return fabs(ns.b * t + ns.c * t * t); };
+        const auto value = [&](double t) { return sqrt(t) * fabs(ns.a + ns.b * t + ns.c * t * t); };
+        double b = second(end), next = value(end);
+        if (ns.c != 0.0) {
+            const double t = -ns.b / (2.0 * ns.c), root = 9.0 * ns.b * ns.b - 20.0 * ns.a * ns.c;
+            if (t > 0.0 && t < end) b = std::max(b, second(t));
+            if (root >= 0.0)
+                for (double sign : {-1.0, 1.0}) {
+                    const double at = (-3.0 * ns.b + sign * sqrt(root)) / (10.0 * ns.c);
+                    if (at > 0.0 && at < end) next = std::max(next, value(at));
+                }
+        } else if (ns.b != 0.0) {
+            const double at = -ns.a / (3.0 * ns.b);
+            if (at > 0.0 && at < end) next = std::max(next, value(at));
+        }
+        if (!(next <= 256.0) || !(b <= 65536.0)) return JABAS_ERR_OPT;
+        s.x[k] = scale_for(most);
+        s.a[k] = scale_for(end);
+        s.b[k] = scale_for(b);
+        most = std::max(next, 1e-6);
+    }
+    s.x[ns.steps] = 1.0;
+    return JABAS_OK;
+}
+
+bool shape_fits(int64_t rows, int64_t cols) {
+    return std::min(rows, cols) <= JABAS_MUON_MAX_SIDE && std::max(rows, cols) <= JABAS_MUON_MAX_LENGTH;
+}
+
+// Sides, padding and partial sums; places come from whoever lays the workspace out.
+void describe(Matrix& x, int64_t rows, int64_t cols) {
+    x.rows = static_cast<int32_t>(rows);
+    x.cols = static_cast<int32_t>(cols);
+    x.tall = rows > cols;
+    x.m = x.tall ? x.cols : x.rows;
+    x.n = x.tall ? x.rows : x.cols;
+    x.pad_m = static_cast<int32_t>(round_up(x.m, kPad));
+    x.pad_n = static_cast<int32_t>(round_up(x.n, kPad));
+    x.x_plane = static_cast<int64_t>(x.pad_m) * x.pad_n;
+    x.a_plane = static_cast<int64_t>(x.pad_m) * x.pad_m;
+    const int64_t count = rows * cols, chunk = std::max<int64_t>(kMinChunk, round_up((count + kParts - 1) / kParts, 1024));
+    x.chunk = static_cast<int32_t>(chunk);
+    x.parts = static_cast<int32_t>((count + chunk - 1) / chunk);
+}
+// halves of the workspace: X twice in two planes, A and B in as many as the products take
+int64_t halves_of(const Matrix& x, int planes) { return 4 * x.x_plane + 2 * planes * x.a_plane; }
+int64_t lay_tiles(const Matrix& x) { return static_cast<int64_t>(x.pad_m / kLay) * (x.pad_n / kLay); }
+
+// Tile of the products of some matrices: the one that the model says ends first. A CU holds one workgroup of 256, two of 128, four of 64; `step` is a
+// round's time for 64 of the inner axis, kStart what a tile's start and results cost.
+struct Tile {
+    int size, slots;
+    double step;
+};
+constexpr Tile kTiles[] = {{256, 256, 1.0}, {128, 512, 0.6}, {64, 1024, 0.36}};
+constexpr double kStart = 4.0;
+struct Load {
+    double sum[3] = {0, 0, 0}, longest[3] = {0, 0, 0};
+    void add(int t, double tiles, double steps) {
+        sum[t] += tiles * (steps + kStart) * kTiles[t].step / kTiles[t].slots;
+        longest[t] = std::max(longest[t], (steps + kStart) * kTiles[t].step);
+    }
+    int best() const {
+        int at = 0;
+        double least = 0.0;
+        for (int t = 0; t < 3; ++t) {
+            const double time = std::max(sum[t], longest[t]);
+            if (t == 0 || time < least) {
+                least = time;
+                at = t;
+            }
+        }
+        return kTiles[at].size;
+    }
+};
+void add_symmetric(Load& l, const Matrix& x, double count) {
+    for (int t = 0; t < 3; ++t) l.add(t, count * symmetric_tiles(x.m, kTiles[t].size), (x.pad_n + x.pad_m) / 64.0);
+}
+void add_update(Load& l, const Matrix& x, double count) {
+    for (int t = 0; t < 3; ++t) l.add(t, count * update_tiles(x.m, x.n, kTiles[t].size), x.pad_m / 64.0);
+}
+
+enum { kMomentum, kLayOut, kSymmetric, kUpdate, kKinds };
+
+// The launches of some matrices that share a workspace.
+struct Run {
+    Work work[kKinds];
+    int tile_symmetric, tile_update;
+    int planes, dtype, nesterov;
+    float momentum, fresh;
+    const float* grad_scale;
+};
+int run(const Run& r, const JabasNewtonSchulz& ns, const Scales& s, UpdateArgs& last, hipStream_t stream) {
+    PassArgs pass{r.work[kMomentum], r.dtype, r.nesterov, r.momentum, r.fresh, r.grad_scale, ns.eps, static_cast<float>(s.x[0])};
+    int status = launch_momentum(pass, stream);
+    if (status != JABAS_OK) return status;
+    pass.w = r.work[kLayOut];
+    if ((status = launch_lay(pass, stream)) != JABAS_OK) return status;
+    for (int k = 0; k < ns.steps; ++k) {
+        SymmetricArgs first{r.work[kSymmetric], k & 1, 0.0f, static_cast<float>(s.a[k] / s.x[k] / s.x[k])};
+        if ((status = launch_symmetric(first, false, r.planes, r.tile_symmetric, stream)) != JABAS_OK) return status;
+        first.own = static_cast<float>(ns.b * s.b[k] / s.a[k]);
+        first.product = static_cast<float>(ns.c * s.b[k] / s.a[k] / s.a[k]);
+        if ((status = launch_symmetric(first, true, r.planes, r.tile_symmetric, stream)) != JABAS_OK) return status;
+        last.w = r.work[kUpdate];
+        last.from = k & 1;
+        last.last = k + 1 == ns.steps;
+        last.own = static_cast<float>(ns.a * s.x[k + 1] / s.x[k]);
+        last.product = static_cast<float>(s.x[k + 1] / s.b[k] / s.x[k]);
+        if ((status = launch_update(last, r.planes, r.tile_update, stream)) != JABAS_OK) return status;
+    }
+    return JABAS_OK;
+}
+
+// ---- a batch of one shape
+
+// Matrices that go through the workspace together: as many as 256 MiB hold, what the chip's last cache holds between the products. Together they
+// fill the chip long before: a matrix whose share is smaller than this / 8 is small.
+constexpr int64_t kTogether = int64_t{256} << 20;
+
+struct Batch {
+    Matrix x;
+    int planes;
+    int64_t at_once, sums_bytes, bytes;
+};
+int describe_batch(const JabasOrthogonalize* o, Batch& b, Scales& s) {
+    if (!o) return JABAS_ERR_NULL;
+    if (o->dtype != JABAS_F32 && o->dtype != JABAS_BF16) return JABAS_ERR_DTYPE;
+    const int status = scales_of(o->ns, s);
+    if (status != JABAS_OK) return status;
+    if (o->batch < 0 || o->rows < 0 || o->cols < 0 || !shape_fits(o->rows, o->cols) || o->batch > (int64_t{1} << 31)) return JABAS_ERR_SIZE;
+    b.planes = o->ns.precision == JABAS_F32 ? 2 : 1;
+    b.bytes = 256;
+    b.at_once = 0;
+    if (!o->batch || !o->rows || !o->cols) return JABAS_OK;
+    memset(&b.x, 0, sizeof b.x);
+    describe(b.x, o->rows, o->cols);
+    const int64_t size = o->dtype == JABAS_F32 ? 4 : 2;
+    if (!o->in || !o->out) return JABAS_ERR_NULL;
+    if (misaligned(o->in, size) || misaligned(o->out, size)) return JABAS_ERR_ALIGN;
+    constexpr int64_t kMaxStride = int64_t{1} << 40;
+    if (o->in_row_stride < o->cols || o->in_row_stride > kMaxStride || o->in_batch_stride < 0 || o->in_batch_stride > kMaxStride) return JABAS_ERR_SIZE;
+    const char *in = static_cast<const char*>(o->in), *out = static_cast<const char*>(o->out);
+    const int64_t in_bytes = size * ((o->batch - 1) * o->in_batch_stride + (o->rows - 1) * o->in_row_stride + o->cols), out_bytes = size * o->batch * o->rows * o->cols;
+    if (in < out + out_bytes && out < in + in_bytes) return JABAS_ERR_ALIAS;
+    b.x.src_stride = o->in_row_stride;
+    const size_t quad = 4 * size;
+    b.x.src_quads = !misaligned(o->in, quad) && o->in_row_stride % 4 == 0 && (o->batch == 1 || o->in_batch_stride % 4 == 0);
+    b.x.out_quads = !misaligned(o->out, quad) && o->cols % 4 == 0;
+    const int64_t each = halves_of(b.x, b.planes);
+    // launches count their workgroups in 32 bits
+    const int64_t most = kMaxSlots / std::max({lay_tiles(b.x), static_cast<int64_t>(b.x.parts), update_tiles(b.x.m, b.x.n, 64), symmetric_tiles(b.x.m, 64)});
+    if (most < 1) return JABAS_ERR_SIZE;
+    b.at_once = std::min({o->batch, std::max<int64_t>(1, kTogether / (2 * each)), most});
+    b.sums_bytes = round_up(8 * b.at_once * b.x.parts, 256);
+    b.bytes = b.sums_bytes + round_up(2 * b.at_once * each, 256);
+    return JABAS_OK;
+}
+
+// ---- lists
+
+constexpr uint32_t kMagic = 0x4d4e5331;
+struct Part {
+    uint64_t slots_at[kKinds];
+    uint32_t total[kKinds];
+    int32_t tile_symmetric, tile_update;
+};
+struct Header {
+    uint32_t magic, n, n_parts, n_groups;
+    int32_t precision, reserved;
+    uint64_t bytes, matrices_at, fanout_at, parts_at, sums_bytes, workspace;
+};
+
+struct Span {
+    const char* p;
+    int64_t bytes;
+    bool written;
+};
+
+int check_matrix(const JabasMatrix& j) {
+    if (!j.grad || !j.momentum || !j.param) return JABAS_ERR_NULL;
+    if (j.rows < 1 || j.cols < 1 || !shape_fits(j.rows, j.cols)) return JABAS_ERR_SIZE;
+    if (j.group >= JABAS_MAX_GROUPS) return JABAS_ERR_GROUP;
+    if (j.n_fanout > JABAS_MAX_K - 1) return JABAS_ERR_K;
+    if (!isfinite(j.lr_factor)) return JABAS_ERR_OPT;
+    Span all[JABAS_MAX_K + 2];
+    int n = 0;
+    const int64_t bytes = 4 * j.rows * j.cols;
+    all[n++] = {reinterpret_cast<const char*>(j.grad), bytes, false};
+    all[n++] = {reinterpret_cast<const char*>(j.momentum), bytes, true};
+    all[n++] = {reinterpret_cast<const char*>(j.param), bytes, true};
+    for (uint32_t f = 0; f < j.n_fanout; ++f) {
+        if (!j.fanout[f]) return JABAS_ERR_NULL;
+        all[n++] = {reinterpret_cast<const char*>(j.fanout[f]), bytes, true};
+    }
+    for (int a = 0; a < n; ++a) {
+        if (misaligned(all[a].p, 4)) return JABAS_ERR_ALIGN;
+        for (int b = 0; b < a; ++b)
+            if ((all[a].written || all[b].written) && all[a].p < all[b].p + bytes && all[b].p < all[a].p + bytes) return JABAS_ERR_ALIAS;
+    }
+    return JABAS_OK;
+}
+
+// Slots of one kind for matrices [first, last): each matrix's tiles are dealt out to the eight dies in runs, dies in turn where a matrix has fewer than
+// eight, and die d has slots d, d + 8, ... . The matrices come with the longest tiles first.
+void deal(std::vector<Slot>& out, const std::vector<int64_t>& tiles, uint32_t first) {
+    std::vector<Slot> die[8];
+    int turn = 0;
+    for (size_t i = 0; i < tiles.size(); ++i) {
+        const int64_t each = tiles[i] / 8, left = tiles[i] % 8;
+        uint32_t at = 0;
+        for (int d = 0; d < 8; ++d) {
+            const int64_t here = each + (d < left);
+            for (int64_t t = 0; t < here; ++t) die[(turn + d) & 7].push_back({first + static_cast<uint32_t>(i), at++});
+        }
+        turn = (turn + static_cast<int>(left)) & 7;
+    }
+    // `turn` keeps the dies within one slot of each other, those from 0 on the longer ones
+    const int64_t total = std::accumulate(tiles.begin(), tiles.end(), int64_t{0});
+    for (int64_t s = 0; s < total; ++s) out.push_back(die[s & 7][s >> 3]);
+}
+
+struct Built {
+    std::vector<Matrix> matrices;
+    std::vector<uint64_t> fanout;
+    std::vector<Part> parts;
+    std::vector<Slot> slots;        // a part's kinds one after another
+    Header head;
+};
+
+int build(const JabasMatrix* list, uint32_t n, int32_t precision, Built& b) {
+    if (!list) return JABAS_ERR_NULL;
+    if (n < 1 || n > (1u << 20)) return JABAS_ERR_SIZE;
+    if (precision != JABAS_F32 && precision != JABAS_BF16) return JABAS_ERR_DTYPE;
+    const int planes = precision == JABAS_F32 ? 2 : 1;
+    b.head = Header{};
+    std::vector<uint32_t> order(n);
+    std::iota(order.begin(), order.end(), 0u);
+    for (uint32_t i = 0; i < n; ++i) {
+        const int status = check_matrix(list[i]);
+        if (status != JABAS_OK) return status;
+        b.head.n_groups = std::max(b.head.n_groups, list[i].group + 1);
+    }
+    const auto sides = [&](uint32_t i) { return std::minmax(list[i].rows, list[i].cols); };
+    std::stable_sort(order.begin(), order.end(), [&](uint32_t i, uint32_t j) {
+        const auto x = sides(i), y = sides(j);
+        return x.first != y.first ? x.first > y.first : x.second > y.second;
+    });
+    for (uint32_t i : order) {
+        const JabasMatrix& j = list[i];
+        Matrix x{};
+        describe(x, j.rows, j.cols);
+        x.src = j.grad;
+        x.momentum = j.momentum;
+        x.out = j.param;
+        x.src_stride = j.cols;
+        x.src_quads = !misaligned(j.grad, 16) && !misaligned(j.momentum, 16) && j.cols % 4 == 0;
+        x.out_quads = !misaligned(j.param, 16) && j.cols % 4 == 0;
+        for (uint32_t f = 0; f < j.n_fanout; ++f) x.out_quads = x.out_quads && !misaligned(j.fanout[f], 16);
+        x.group = static_cast<int32_t>(j.group);
+        x.lr_factor = static_cast<float>(j.lr_factor);
+        x.n_fanout = j.n_fanout;
+        x.fanout_at = static_cast<uint32_t>(b.fanout.size());
+        for (uint32_t f = 0; f < j.n_fanout; ++f) b.fanout.push_back(reinterpret_cast<uint64_t>(j.fanout[f]));
+        b.matrices.push_back(x);
+    }
+    uint64_t halves_most = 0, sums_most = 0;
+    for (uint32_t first = 0; first < n;) {
+        int64_t halves = 0, sums = 0, slots[kKinds] = {0, 0, 0, 0};
+        uint32_t last = first;
+        while (last < n) {
+            Matrix& x = b.matrices[last];
+            const int64_t need = halves_of(x, planes);
+            const int64_t more[kKinds] = {x.parts, lay_tiles(x), symmetric_tiles(x.m, 64), update_tiles(x.m, x.n, 64)};
+            bool full = last > first && 2 * (halves + need) > kTogether;
+            for (int k = 0; k < kKinds; ++k) {
+                if (more[k] > kMaxSlots) return JABAS_ERR_SIZE;
+                full = full || slots[k] + more[k] > kMaxSlots;
+            }
+            if (full) break;
+            x.x_at = halves;
+            x.a_at = halves + 4 * x.x_plane;
+            x.part_at = sums;
+            halves += need;
+            sums += x.parts;
+            for (int k = 0; k < kKinds; ++k) slots[k] += more[k];
+            ++last;
+        }
+        halves_most = std::max<uint64_t>(halves_most, halves);
+        sums_most = std::max<uint64_t>(sums_most, sums);
+        Load symmetric, update;
+        for (uint32_t i = first; i < last; ++i) {
+            add_symmetric(symmetric, b.matrices[i], 1);
+            add_update(update, b.matrices[i], 1);
+        }
+        Part p{};
+        p.tile_symmetric = symmetric.best();
+        p.tile_update = update.best();
+        for (int k = 0; k < kKinds; ++k) {
+            std::vector<int64_t> tiles;
+            for (uint32_t i = first; i < last; ++i) {
+                const Matrix& x = b.matrices[i];
+                tiles.push_back(k == kMomentum ? x.parts : k == kLayOut ? lay_tiles(x) : k == kSymmetric ? symmetric_tiles(x.m, p.tile_symmetric) : update_tiles(x.m, x.n, p.tile_update));
+            }
+            p.slots_at[k] = b.slots.size();
+            deal(b.slots, tiles, first);
+            p.total[k] = static_cast<uint32_t>(b.slots.size() - p.slots_at[k]);
+        }
+        b.parts.push_back(p);
+        first = last;
+    }
+    Header& h = b.head;
+    h.magic = kMagic;
+    h.n = n;
+    h.n_parts = static_cast<uint32_t>(b.parts.size());
+    h.precision = precision;
+    h.matrices_at = round_up(sizeof(Header), 16);
+    h.fanout_at = h.matrices_at + round_up(sizeof(Matrix) * n, 16);
+    h.parts_at = h.fanout_at + round_up(8 * b.fanout.size(), 16);
+    const uint64_t slots_at = h.parts_at + round_up(sizeof(Part) * b.parts.size(), 16);
+    for (Part& p : b.parts)
+        for (uint64_t& at : p.slots_at) at = slots_at + at * sizeof(Slot);
+    h.bytes = round_up(slots_at + b.slots.size() * sizeof(Slot), 16);
+    h.sums_bytes = round_up(8 * sums_most, 256);
+    h.workspace = h.sums_bytes + round_up(2 * halves_most, 256);
+    return JABAS_OK;
+}
+
+// Nothing that C++ throws leaves the library; there is too little host memory where it does.
+template <class F>
+int guarded(const F& f) {
+    try {
+        return f();
+    } catch (...) {
+        return JABAS_ERR_SIZE;
+    }
+}
+
+const Header* header_of(const void* blob) {
+    const Header* h = static_cast<const Header*>(blob);
+    return h && !misaligned(blob, 8) && h->magic == kMagic && h->n_parts ? h : nullptr;
+}
+
+}  // namespace
+}  // namespace muon
+}  // namespace jabas
+
+using namespace jabas::muon;
+
+JABAS_API size_t jabas_orthogonalize_workspace_bytes(const JabasOrthogonalize* o) {
+    Batch b;
+    Scales s;
+    return describe_batch(o, b, s) == JABAS_OK ? static_cast<size_t>(b.bytes) : 0;
+}
+
+JABAS_API int jabas_orthogonalize(const JabasOrthogonalize* o, void* workspace, size_t workspace_bytes, jabas_stream_t stream) {
+    Batch b;
+    Scales s;
+    const int status = describe_batch(o, b, s);
+    if (status != JABAS_OK) return status;
+    if (!b.at_once) return JABAS_OK;
+    if (!workspace || misaligned(workspace, 256) || workspace_bytes < static_cast<size_t>(b.bytes)) return JABAS_ERR_WORKSPACE;
+    const Matrix& x = b.x;
+    const int64_t size = o->dtype == JABAS_F32 ? 4 : 2, each = halves_of(x, b.planes);
+    for (int64_t done = 0; done < o->batch; done += b.at_once) {
+        const int64_t here = std::min(b.at_once, o->batch - done);
+        Load symmetric, update;
+        add_symmetric(symmetric, x, static_cast<double>(here));
+        add_update(update, x, static_cast<double>(here));
+        Run r{};
+        r.tile_symmetric = symmetric.best();
+        r.tile_update = update.best();
+        r.planes = b.planes;
+        r.dtype = o->dtype;
+        Work w{};
+        w.one = x;
+        w.one.src = static_cast<const char*>(o->in) + size * done * o->in_batch_stride;
+        w.one.out = static_cast<char*>(o->out) + size * done * o->rows * o->cols;
+        w.one.a_at = here * 4 * x.x_plane;
+        w.src_step = size * o->in_batch_stride;
+        w.out_step = size * o->rows * o->cols;
+        w.x_step = 4 * x.x_plane;
+        w.a_step = each - w.x_step;
+        w.part_step = x.parts;
+        w.sums = static_cast<double*>(workspace);
+        w.halves = static_cast<char*>(workspace) + b.sums_bytes;
+        const int64_t per[kKinds] = {x.parts, lay_tiles(x), symmetric_tiles(x.m, r.tile_symmetric), update_tiles(x.m, x.n, r.tile_update)};
+        for (int k = 0; k < kKinds; ++k) {
+            r.work[k] = w;
+            r.work[k].per = static_cast<int32_t>(per[k]);
+            r.work[k].total = static_cast<uint32_t>(per[k] * here);
+        }
+        UpdateArgs last{};
+        last.out_dtype = o->dtype;
+        const int launched = run(r, o->ns, s, last, static_cast<hipStream_t>(stream));
+        if (launched != JABAS_OK) return launched;
+    }
+    return JABAS_OK;
+}
+
+JABAS_API size_t jabas_muon_plan_bytes(const JabasMatrix* matrices, uint32_t n, int32_t precision) {
+    size_t bytes = 0;
+    const int status = guarded([&] {
+        Built b;
+        const int built = build(matrices, n, precision, b);
+        if (built == JABAS_OK) bytes = b.head.bytes;
+        return built;
+    });
+    return status == JABAS_OK ? bytes : 0;
+}
+
+JABAS_API int jabas_muon_plan_encode(const JabasMatrix* matrices, uint32_t n, int32_t precision, void* host_blob, size_t blob_bytes) {
+    return guarded([&]() -> int {
+        Built b;
+        const int status = build(matrices, n, precision, b);
+        if (status != JABAS_OK) return status;
+        if (!host_blob) return JABAS_ERR_NULL;
+        if (misaligned(host_blob, 8) || blob_bytes < b.head.bytes) return JABAS_ERR_PLAN;
+        char* at = static_cast<char*>(host_blob);
+        memset(at, 0, b.head.bytes);
+        memcpy(at, &b.head, sizeof(Header));
+        memcpy(at + b.head.matrices_at, b.matrices.data(), sizeof(Matrix) * n);
+        if (!b.fanout.empty()) memcpy(at + b.head.fanout_at, b.fanout.data(), 8 * b.fanout.size());
+        memcpy(at + b.head.parts_at, b.parts.data(), sizeof(Part) * b.parts.size());
+        memcpy(at + b.parts[0].slots_at[0], b.slots.data(), sizeof(Slot) * b.slots.size());
+        return JABAS_OK;
+    });
+}
+
+JABAS_API size_t jabas_muon_workspace_bytes(const void* host_blob) {
+    const Header* h = header_of(host_blob);
+    return h ? h->workspace : 0;
+}
+
+JABAS_API int jabas_muon_step(const void* plan_host, const void* plan_dev, const JabasMuonArgs* args, void* workspace, size_t workspace_bytes,
+                              jabas_stream_t stream) {
+    if (!plan_host || !plan_dev || !args) return JABAS_ERR_NULL;
+    const Header* h = header_of(plan_host);
+    if (!h || misaligned(plan_dev, 16)) return JABAS_ERR_PLAN;
+    Scales s;
+    const int status = scales_of(args->ns, s);
+    if (status != JABAS_OK) return status;
+    if (args->ns.precision != h->precision) return JABAS_ERR_PLAN;
+    if (!(args->momentum >= 0.0 && args->momentum < 1.0)) return JABAS_ERR_OPT;
+    if (args->n_groups < static_cast<int32_t>(h->n_groups) || args->n_groups > JABAS_MAX_GROUPS) return JABAS_ERR_GROUP;
+    if (!workspace || misaligned(workspace, 256) || workspace_bytes < h->workspace) return JABAS_ERR_WORKSPACE;
+    const char *host = static_cast<const char*>(plan_host), *dev = static_cast<const char*>(plan_dev);
+    const Part* parts = reinterpret_cast<const Part*>(host + h->parts_at);
+    Work w{};
+    w.table = reinterpret_cast<const Matrix*>(dev + h->matrices_at);
+    w.fanout = reinterpret_cast<const uint64_t*>(dev + h->fanout_at);
+    w.sums = static_cast<double*>(workspace);
+    w.halves = static_cast<char*>(workspace) + h->sums_bytes;
+    UpdateArgs last{};
+    for (int g = 0; g < args->n_groups; ++g) {
+        last.lr[g] = static_cast<float>(args->lr[g]);
+        last.keep[g] = static_cast<float>(1.0 - args->lr[g] * args->weight_decay[g]);
+    }
+    for (uint32_t p = 0; p < h->n_parts; ++p) {
+        Run r{};
+        r.tile_symmetric = parts[p].tile_symmetric;
+        r.tile_update = parts[p].tile_update;
+        r.planes = h->precision == JABAS_F32 ? 2 : 1;
+        r.dtype = JABAS_F32;
+        r.nesterov = args->nesterov != 0;
+        r.momentum = static_cast<float>(args->momentum);
+        r.fresh = static_cast<float>(1.0 - args->momentum);
+        r.grad_scale = args->grad_scale;
+        for (int k = 0; k < kKinds; ++k) {
+            r.work[k] = w;
+            r.work[k].slots = reinterpret_cast<const Slot*>(dev + parts[p].slots_at[k]);
+            r.work[k].total = parts[p].total[k];
+        }
+        const int launched = run(r, args->ns, s, last, static_cast<hipStream_t>(stream));
+        if (launched != JABAS_OK) return launched;
+    }
+    return JABAS_OK;
+}

@@ -1,0 +1,88 @@
+// Shared by the sources of the orthogonalised update.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "jabas_muon.h"
+
+namespace jabas {
+namespace muon {
+
+constexpr int kPad = 64;            // sides of the copies that the products read are multiples of this
+constexpr int kParts = 256;         // partial sums of a matrix's length
+constexpr int kMinChunk = 4096;     // elements of one of them, at least
+constexpr int kLay = 64;            // tile of the pass that lays a matrix out
+
+// One matrix as the kernels see it. The products work on X, m x n with m <= n: the matrix, or (tall) its transpose.
+struct Matrix {
+    const void* src;                // the gradient
+    float* momentum;                // NULL: none, X is made of src
+    void* out;                      // the weights (with momentum), else where X goes
+    int64_t src_stride;             // of a row
+    int64_t x_at, a_at, part_at;    // places in the workspace: X (4 planes: two buffers of two) and A, B in halves, partial sums in doubles
+    int64_t x_plane, a_plane;       // halves apart
+    int32_t rows, cols;             // of src and out
+    int32_t m, n, pad_m, pad_n;
+    int32_t tall;
+    int32_t src_quads, out_quads;   // four elements at a time: all rows of src (and momentum), of out (and replicas) allow it
+    int32_t parts, chunk;           // partial sums, elements of each
+    int32_t group;
+    float lr_factor;
+    uint32_t n_fanout, fanout_at;   // replicas: pointers in the list's table
+};
+
+// Which workgroup does what. A list: `table` and a slot {matrix, tile} for every workgroup. A batch: matrix 0 and what lies between it and
+// the next one.
+struct Slot {
+    uint32_t matrix, tile;
+};
+struct Work {
+    const Matrix* table;
+    const Slot* slots;
+    const uint64_t* fanout;
+    Matrix one;
+    int64_t src_step, out_step;     // bytes
+    int64_t x_step, a_step, part_step;
+    int32_t per;                    // tiles of a matrix
+    uint32_t total;                 // workgroups that have something to do
+    void* halves;                   // workspace
+    double* sums;
+};
+
+// A pass over the gradients: momentum and partial sums (launch_momentum), or the copy (launch_lay).
+struct PassArgs {
+    Work w;
+    int32_t dtype;                  // of src
+    int32_t nesterov;
+    float momentum, fresh;          // momentum and 1 - momentum
+    const float* grad_scale;
+    double eps;
+    float scale;                    // of X's planes
+};
+int launch_momentum(const PassArgs& a, hipStream_t stream);
+int launch_lay(const PassArgs& a, hipStream_t stream);
+
+// X X^T (second: b A + c A A), written whole though half of it is computed; scales: powers of two.
+struct SymmetricArgs {
+    Work w;
+    int32_t from;                   // buffer of X
+    float own, product;             // result = own A + product acc
+};
+// X <- a X + B X
+struct UpdateArgs {
+    Work w;
+    int32_t from;
+    int32_t last;                   // goes to out, scaled by 1
+    int32_t out_dtype;              // without weights
+    float own, product;
+    float lr[JABAS_MAX_GROUPS], keep[JABAS_MAX_GROUPS];     // keep = 1 - lr weight_decay
+};
+int launch_symmetric(const SymmetricArgs& a, bool second, int planes, int tile, hipStream_t stream);
+int launch_update(const UpdateArgs& a, int planes, int tile, hipStream_t stream);
+
+inline int64_t symmetric_tiles(int64_t m, int tile) { const int64_t t = (m + tile - 1) / tile; return t * (t + 1) / 2; }
+inline int64_t update_tiles(int64_t m, int64_t n, int tile) { return (m + tile - 1) / tile * ((n + tile - 1) / tile); }
+
+}  // namespace muon
+}  // namespace jabas

@@ -18,8 +18,16 @@ from .sync import SpanSpec, SyncPlan, StepScalars, MomentArena, MOMENT_BLOCK_LOG
 class VSWFlatSync:
     def __init__(self, specs, batches, grad_dtype=torch.float32, opt=None, device="cuda", in_place=None,
                  n_fanout=0, per_tensor_spans=False, caps=None, keep_clipped_grads=True, write_aggregate=True,
-                 moment_block_log2=MOMENT_BLOCK_LOG2):
+                 moment_block_log2=MOMENT_BLOCK_LOG2, shapes=None):
+        """``opt`` of kind "muon" (``optim.ShardMuon``): dict(kind="muon", momentum=, nesterov=, groups=[dict(lr=, weight_decay=,
+        use_muon=True)], optionally adjust_lr_fn, ns_steps, ns_coefficients, ns_eps, ns_dtype, and betas and eps of the AdamW that
+        groups with use_muon=False follow); ``shapes``: the sizes of every parameter of ``specs``, in order. Its step aggregates first and
+        then updates from the aggregate, which therefore is always written. state1 holds the matrices' momentum and the others' exp_avg,
+        state2 the others' exp_avg_sq."""
         self.K = len(batches)
+        self._muon = opt is not None and opt["kind"] == "muon"
+        if self._muon:
+            write_aggregate, moment_block_log2 = True, 0
         # Adam's moments (exp_avg, exp_avg_sq, amsgrad's maximum) live in ONE arena that alternates blocks of
         # 2**moment_block_log2 elements of each (sync.MomentArena): the kernels stream that 2-6 % faster than
         # arenas of their own. ``state1`` / ``state2`` / ``state3`` then are flat COPIES made on access
@@ -52,7 +60,9 @@ class VSWFlatSync:
             self.agg = self.grads[0]
         else:                                    # an arena of its own, unless nothing will ever be written to it
             self.agg = torch.zeros(n, dtype=torch.float32, device=self.device) if self.write_aggregate else None
-        kind = opt_kind(opt)
+        kind = self._kind()
+        if self._muon:
+            self._matrices = self._check_muon(shapes)
         self.param = self._state = None
         self.moments = None
         self.fanout = []
@@ -126,8 +136,96 @@ class VSWFlatSync:
         names = ("state1", "state2", "state3")
         return {names[j]: st[j][off:off + numel] for j in range(len(st))}
 
+    def _kind(self):
+        """JABAS_OPT_* of the spans' launches."""
+        return L.OPT_ADAMW if self._muon else opt_kind(self.opt)
+
+    # ---- matrices whose update is orthogonalised -----------------------------------
+    def _check_muon(self, shapes):
+        """{parameter: (rows, cols)} of the groups with use_muon."""
+        groups = self.opt["groups"]
+        if not 1 <= len(groups) <= L.MAX_GROUPS:
+            raise ValueError(f"1..{L.MAX_GROUPS} parameter groups supported, got {len(groups)}")
+        if shapes is None or len(shapes) != len(self.layout.specs):
+            raise ValueError("kind 'muon' needs the shape of every parameter (shapes=)")
+        found = {}
+        for i, (spec, shape) in enumerate(zip(self.layout.specs, shapes)):
+            count = 1
+            for n in shape:
+                count *= int(n)
+            if count != spec.numel:
+                raise ValueError(f"{spec.name}: {spec.numel} elements cannot have shape {tuple(shape)}")
+            if spec.group < len(groups) and groups[spec.group].get("use_muon", True):
+                if len(shape) < 2 or not count:
+                    raise ValueError(f"{spec.name}: shape {tuple(shape)} is no matrix: give its group use_muon=False")
+                found[i] = (int(shape[0]), count // int(shape[0]))
+        return found
+
+    def _build_muon_plans(self):
+        from .optim.muon import MuonPlan, lr_factor
+        whole, rest = [], []
+        for (off, numel, _bounds, _bucket) in self.layout.spans:
+            sl = slice(off, off + numel)
+            whole.append(SpanSpec([g[sl] for g in self.grads], agg_out=self.agg[sl]))
+        for bucket in self.layout.buckets:          # stretches without a matrix
+            run = []
+            for i in [*bucket.param_ids, None]:
+                if i is not None and i not in self._matrices:
+                    if self.layout.specs[i].numel:
+                        run.append(i)
+                elif run:
+                    off = self.layout.param_offset[run[0]]
+                    sl = slice(off, self.layout.param_offset[run[-1]] + self.layout.specs[run[-1]].numel)
+                    bounds = []
+                    for j in run:
+                        group = self.layout.specs[j].group
+                        if not bounds or bounds[-1][1] != group:
+                            bounds.append((self.layout.param_offset[j] - off, group))
+                    rest.append(SpanSpec([self.agg[sl]], param=self.param[sl], fanout=[f[sl] for f in self.fanout], bounds=bounds,
+                                         **self.state_of_span(off, sl.stop - off)))
+                    run = []
+        self.plan = SyncPlan(whole, L.OPT_NONE)
+        self._plan_rest = SyncPlan(rest, L.OPT_ADAMW) if rest else None
+        items = [dict(grad=self.agg_view(i), momentum=self.state_view(0, i), param=self.param_view(i), rows=rows, cols=cols,
+                      group=self.layout.specs[i].group, lr_factor=lr_factor(self.opt.get("adjust_lr_fn"), rows, cols),
+                      fanout=[self._view(f, i) for f in self.fanout]) for i, (rows, cols) in self._matrices.items()]
+        self._plan_matrices = MuonPlan(items, self.opt.get("ns_dtype", torch.float32)) if items else None
+        self._plan_scale = None
+
+    def _queue_muon(self, stats, lr_scale, stream, clip_norm, accumulations):
+        from .optim.muon import COEFFICIENTS, make_muon_args
+        opt, clipped = self.opt, self._clipped(clip_norm)
+        level = stats if stats or not clipped else "similarity"
+        rows = self.plan.run(self.step_args(stats=level, with_opt=False, accumulations=accumulations), stream=stream)
+        coef = None
+        if clipped:
+            if self._coef is None:
+                self._coef = torch.ones(1, dtype=torch.float32, device=self.device)
+            coef = clip_coef(rows, clip_norm, out=self._coef, stream=stream)
+            if self.keep_clipped_grads:             # the aggregate itself becomes the clipped one
+                if self._plan_scale is None:
+                    self._plan_scale = SyncPlan([SpanSpec([self.agg[off:off + n]], agg_out=self.agg[off:off + n]) for off, n, _, _ in self.layout.spans])
+                self._plan_scale.run(make_step_args((1,), torch.float32, grad_scale=coef), stream=stream)
+                coef = None
+        if self._plan_rest is not None:
+            adam = dict(kind="adamw", betas=opt.get("betas", (0.9, 0.999)), eps=opt.get("eps", 1e-8), groups=opt["groups"])
+            self._plan_rest.run(make_step_args((1,), torch.float32, opt=adam, step=self.step_count + 1, lr_scale=lr_scale, grad_scale=coef),
+                                stream=stream)
+        if self._plan_matrices is not None:
+            self._plan_matrices.run(make_muon_args(
+                opt["groups"], momentum=opt.get("momentum", 0.95), nesterov=opt.get("nesterov", True), steps=opt.get("ns_steps", 5),
+                coefficients=opt.get("ns_coefficients", COEFFICIENTS), eps=opt.get("ns_eps", 1e-7), dtype=opt.get("ns_dtype", torch.float32),
+                lr_scale=lr_scale, grad_scale=coef), stream=stream)
+        return rows if stats else None
+
     def _build_plan(self):
-        kind = opt_kind(self.opt)
+        if self._muon:
+            self._build_muon_plans()
+            self.span_bucket = [s[3] for s in self.layout.spans]
+            self._plan_agg = self._plan_opt = self._coef = None
+            self._generation = getattr(self, "_generation", 0) + 1
+            return
+        kind = self._kind()
         spans = []
         for (off, numel, bounds, _bucket) in self.layout.spans:
             sl = slice(off, off + numel)
@@ -220,6 +318,8 @@ class VSWFlatSync:
                               first_step=self.step_count == 0, lr_scale=lr_scale, grad_scale=self._coef)
 
     def _queue(self, stats, lr_scale, stream, clip_norm, accumulations, scalars):
+        if self._muon:
+            return self._queue_muon(stats, lr_scale, stream, clip_norm, accumulations)
         if self._clipped(clip_norm) and self._plan_agg is None:
             self._build_clip_plans()
         args = self._update_args(stats, lr_scale, clip_norm, accumulations)
@@ -242,6 +342,8 @@ class VSWFlatSync:
         ``accumulations`` are fixed by the recording; ``reconfigure`` invalidates it."""
         if self.opt is None:
             raise ValueError("nothing moves between the steps of an engine without optimizer: record its launch directly")
+        if self._muon:
+            raise ValueError("orthogonalised updates take the step's scalars by value only: such a step cannot be replayed")
         if self.opt.get("amsgrad", False):
             raise ValueError("the amsgrad kernels take the step's scalars by value only: an amsgrad step cannot be replayed")
         return GraphedStep(self, stats, clip_norm, accumulations)

@@ -336,7 +336,10 @@ class LocalBucketSync:
             return self
         if self.optimizer is not None:
             raise RuntimeError("another optimizer is already bound")
-        self.opt = opt_from_torch_optimizer(optimizer)
+        opt = opt_from_torch_optimizer(optimizer)
+        if opt["kind"] == "muon":
+            raise TypeError("orthogonalised updates are no part of a bucket's launch: hand such an optimizer to VSWSyncTrainer, or call its step")
+        self.opt = opt
         self.optimizer = optimizer
         self._group_of = {id(p): gi for gi, g in enumerate(optimizer.param_groups) for p in g["params"]}
         self.grad_clip = float(getattr(optimizer, "grad_clip", float("inf")))

@@ -1,3 +1,4 @@
 from .shard import ShardSGD, ShardAdam, ShardAdamW, ShardGNMTAdam
+from .muon import ShardMuon, orthogonalize
 
-__all__ = ["ShardSGD", "ShardAdam", "ShardAdamW", "ShardGNMTAdam"]
+__all__ = ["ShardSGD", "ShardAdam", "ShardAdamW", "ShardGNMTAdam", "ShardMuon", "orthogonalize"]

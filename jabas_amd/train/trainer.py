@@ -117,15 +117,42 @@ def tag_parameter_indices(model):
     return model
 
 
+def _is_muon(optimizer):
+    from ..optim import ShardMuon
+    return isinstance(optimizer, (ShardMuon, getattr(torch.optim, "Muon", ShardMuon)))
+
+
+_MUON_KEYS = (("momentum", "momentum"), ("nesterov", "nesterov"), ("ns_coefficients", "ns_coefficients"), ("ns_steps", "ns_steps"), ("ns_eps", "eps"),
+              ("adjust_lr_fn", "adjust_lr_fn"), ("ns_dtype", "ns_dtype"))
+
+
+def _read_muon(opt, groups):
+    """What a launch takes once, of the groups it serves: the matrices' for the orthogonalised update, the others' for AdamW."""
+    for wanted, keys in ((True, _MUON_KEYS), (False, (("betas", "betas"), ("eps", "eps")))):
+        mine = [g for g in groups if bool(g.get("use_muon", True)) == wanted]
+        for name, key in keys:
+            values = [tuple(g[key]) if isinstance(g[key], (tuple, list)) else g[key] for g in mine if key in g]
+            if any(v != values[0] for v in values):
+                raise ValueError(f"parameter groups differ in {key!r}: one value per launch is supported")
+            if values:
+                opt[name] = values[0]
+
+
 def opt_from_torch_optimizer(optimizer):
     """Hyperparameter dictionary (the form ``sync.make_step_args`` takes) of a torch.optim.SGD / Adam /
     AdamW or a jabas_amd.optim.Shard* object. One momentum / betas / eps for all groups, as the
-    kernel takes them per launch; learning rate and weight decay per group."""
+    kernel takes them per launch; learning rate and weight decay per group. torch.optim.Muon and ShardMuon: the
+    dictionary that ``VSWFlatSync`` takes for them."""
     from ..optim import ShardSGD, ShardAdam, ShardAdamW
     groups = optimizer.param_groups
     if not groups:
         raise ValueError("optimizer has no parameter groups")
     g0 = groups[0]
+    if _is_muon(optimizer):
+        opt = dict(kind="muon", groups=[dict(lr=float(g["lr"]), weight_decay=float(g.get("weight_decay", 0.0)), use_muon=bool(g.get("use_muon", True)))
+                                        for g in groups])
+        _read_muon(opt, groups)
+        return opt
 
     def same(key):
         vals = [g[key] for g in groups]
@@ -146,7 +173,7 @@ def opt_from_torch_optimizer(optimizer):
         opt = dict(kind="adamw" if adamw else "adam", betas=(float(b1), float(b2)), eps=float(same("eps")),
                    amsgrad=bool(same("amsgrad")) if "amsgrad" in g0 else False)
     else:
-        raise TypeError(f"unsupported optimizer type {type(optimizer).__name__}: SGD, Adam, AdamW or their "
+        raise TypeError(f"unsupported optimizer type {type(optimizer).__name__}: SGD, Adam, AdamW, Muon or their "
                         "Shard counterparts")
     opt["groups"] = [dict(lr=float(g["lr"]), weight_decay=float(g.get("weight_decay", 0.0))) for g in groups]
     return opt
@@ -162,6 +189,14 @@ def refresh_opt_from_torch_optimizer(opt, optimizer):
     for mine, theirs in zip(opt["groups"], groups):
         mine["lr"] = float(theirs["lr"])
         mine["weight_decay"] = float(theirs.get("weight_decay", 0.0))
+    if opt["kind"] == "muon":
+        if [m["use_muon"] for m in opt["groups"]] != [bool(g.get("use_muon", True)) for g in groups]:
+            raise ValueError("a parameter group's use_muon changed after the state arenas were laid out")
+        fixed = opt.get("adjust_lr_fn"), opt.get("ns_dtype")
+        _read_muon(opt, groups)
+        if (opt.get("adjust_lr_fn"), opt.get("ns_dtype")) != fixed:
+            raise ValueError("adjust_lr_fn and ns_dtype are part of the launches' plan: they cannot change after it was made")
+        return
     g0 = groups[0]
     keys = ("momentum", "dampening", "nesterov") if opt["kind"] == "sgd" else ("betas", "eps")
     for key in keys:
@@ -249,7 +284,7 @@ class VSWSyncTrainer:
 
     def prepare_weight_sync_method(self, optimizer, scheduler=None, param_groups_func=None):
         """Counterpart of jabas/train/trainer.py:88-98: takes the optimizer the caller built over
-        ``main_model``'s parameters (torch.optim.SGD / Adam / AdamW or ShardSGD / ShardAdam / ShardAdamW,
+        ``main_model``'s parameters (torch.optim.SGD / Adam / AdamW / Muon or ShardSGD / ShardAdam / ShardAdamW / ShardMuon,
         examples/resnet50/main.py:351-363) and an optional LR scheduler that is stepped once per sync
         step. Parameter groups of the optimizer become the kernel's parameter groups."""
         if self.main_model is None:
@@ -291,7 +326,8 @@ class VSWSyncTrainer:
         self.engine = VSWFlatSync(specs, self.local_batch_sizes, grad_dtype=self.grad_dtype, opt=self.opt,
                                   device=self.gpu, n_fanout=0 if self.share_weights else max(1, self.num_models - 1),
                                   keep_clipped_grads=self.keep_grads, write_aggregate=self.keep_grads,
-                                  moment_block_log2=sync.MOMENT_BLOCK_LOG2 if self.interleave_moments else 0)
+                                  moment_block_log2=sync.MOMENT_BLOCK_LOG2 if self.interleave_moments else 0,
+                                  shapes=[tuple(p.shape) for p in params])
         if self.num_models == 1 and not self.share_weights:
             self.engine.reconfigure(self.local_batch_sizes)       # keeps the fan-out slot for later replicas
         self.local_models = [model] + [copy.deepcopy(model) for _ in range(self.num_models - 1)]
@@ -325,7 +361,9 @@ class VSWSyncTrainer:
         sgd = self.opt["kind"] == "sgd"
         for i, p in enumerate(self.main_model.parameters()):
             st = optimizer.state[p]
-            if sgd:
+            if self.opt["kind"] == "muon" and i in eng._matrices:
+                st["momentum_buffer"] = eng.state_view(0, i).view(p.shape)
+            elif sgd:
                 if eng.n_state:
                     st["momentum_buffer"] = eng.state_view(0, i).view(p.shape)
             else:
@@ -382,7 +420,8 @@ class VSWSyncTrainer:
         steps, has_momentum = set(), False
         for i, p in enumerate(self.main_model.parameters()):
             st = self.main_optimizer.state.get(p, {})
-            for key, j in keys:
+            matrix = self.opt["kind"] == "muon" and i in eng._matrices
+            for key, j in (("momentum_buffer", 0),) if matrix else keys:
                 if j >= eng.n_state:
                     continue
                 loaded = st.get(key)
@@ -397,8 +436,8 @@ class VSWSyncTrainer:
         if len(steps) > 1:
             raise ValueError(f"parameters at different step counts {sorted(steps)}: one fused launch cannot mirror that")
         eng.step_count = steps.pop() if steps else (1 if has_momentum else 0)
-        self.opt["groups"] = [dict(lr=float(g["lr"]), weight_decay=float(g.get("weight_decay", 0.0)))
-                              for g in self.main_optimizer.param_groups]
+        for mine, g in zip(self.opt["groups"], self.main_optimizer.param_groups):
+            mine["lr"], mine["weight_decay"] = float(g["lr"]), float(g.get("weight_decay", 0.0))
         self._step_tensor = torch.full((), float(eng.step_count), dtype=torch.float32)
         self._expose_state(self.main_optimizer, moments=eng.state_is_live)
         torch.cuda.synchronize(self.gpu)
