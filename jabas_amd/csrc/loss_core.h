@@ -45,15 +45,22 @@ struct BF16 {
 // 128 x 128, which read LDS a third less, came out even.
 // The loads are inline assembly because the compiler would wait for all of them before any later LDS read; they have no
 // register outputs, and the wait in front of the barrier covers them.
-template <class E, int P, int TM, int TN, int WM, int WN, bool TA, bool TB, bool RA, bool RB>
+//
+// S: stages of LDS. Two keep a CU's matrix cores busy where it has work for two workgroups or a large tile; where a CU has one small tile, what a step
+// takes is the way of its loads (0.5 to 0.9 us behind a kernel that wrote them on another die), so that more of them are sent ahead.
+//
+// L (two planes): they lie in one line, 32 elements of the first and the same 32 of the second by turns, so that a row of a step is a whole line of 128
+// bytes for either kind of operand. Loads of half lines reach 60 % of the rate (16 KB a workgroup and step from the caches: 0.24 us against 0.14).
+template <class E, int P, int TM, int TN, int WM, int WN, bool TA, bool TB, bool RA, bool RB, int S = 2, bool L = false>
 struct Core {
     static constexpr bool kTa = TA, kTb = TB;
     static constexpr int kM = TM, kN = TN, kThreads = 64 * WM * WN;
     static constexpr int kI = TM / WM / 32, kJ = TN / WN / 32;
-    static constexpr int kBytesA = TM * 128, kBytesB = TN * 128, kStage = kBytesA + kBytesB;
+    static constexpr int kBytesA = TM * 128, kBytesB = TN * 128, kStage = kBytesA + kBytesB, kStages = S;
     static constexpr int kLoadsA = TM * 8 / kThreads, kLoadsB = TN * 8 / kThreads;
     static constexpr int kStep = P == 2 ? 32 : 64;      // of the inner axis
     static constexpr int kParts = kStep / 16;
+    static_assert(P == 2 || !L, "one plane has its lines to itself");
     static_assert(kLoadsA % P == 0 && kLoadsB % P == 0, "a load takes one plane");
     using vec = typename E::vec;
 
@@ -73,8 +80,8 @@ struct Core {
     // An operand's tile on its way: a uniform base per plane, which moves from step to step, and offsets of the lane's chunks.
     template <int T, bool TR>
     struct Source {
-        static constexpr int kLoads = T * 8 / kThreads, kEach = kLoads / P;
-        uint64_t base[P];
+        static constexpr int kLoads = T * 8 / kThreads, kBases = L && !TR ? 1 : P, kEach = kLoads / kBases;
+        uint64_t base[kBases];
         int64_t step;
         uint32_t offset[kEach];
 
@@ -82,17 +89,18 @@ struct Core {
             const int t = threadIdx.x;
             const uint64_t p = reinterpret_cast<uint64_t>(o.p) + (TR ? 0 : 2 * static_cast<int64_t>(first) * o.stride);
 #pragma unroll
-            for (int q = 0; q < P; ++q) base[q] = p + 2 * q * o.plane;
-            step = 2 * (TR ? kStep * o.stride : kStep);
+            for (int q = 0; q < kBases; ++q) base[q] = p + 2 * q * o.plane;
+            step = 2 * (TR ? kStep * o.stride : L ? 2 * kStep : kStep);
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
                 const int f = i * kThreads + t;                 // the chunk's place in the plane's tile
                 if (TR) {
                     const int k = f / (T / 8), c = (f % (T / 8)) ^ turned<T>(k);
                     const int col = min(first + c * 8, o.rows - 8);        // past the end: read again, never written
-                    offset[i] = 2 * (static_cast<uint32_t>(k) * static_cast<uint32_t>(o.stride) + col);
+                    offset[i] = 2 * (static_cast<uint32_t>(k) * static_cast<uint32_t>(o.stride) + (L ? (col >> 5) * 64 + (col & 31) : col));
                 } else {
-                    const int r = P == 2 ? f >> 2 : f >> 3, c = P == 2 ? (f & 3) ^ ((r >> 2) & 3) : (f & 7) ^ ((r >> 1) & 7);
+                    constexpr bool kHalf = P == 2 && !L;
+                    const int r = kHalf ? f >> 2 : f >> 3, c = kHalf ? (f & 3) ^ ((r >> 2) & 3) : (f & 7) ^ ((r >> 1) & 7);
                     offset[i] = 2 * (static_cast<uint32_t>(min(first + r, o.rows - 1) - first) * static_cast<uint32_t>(o.stride) + c * 8);
                 }
             }
@@ -105,7 +113,7 @@ struct Core {
         }
         __device__ void advance() {
 #pragma unroll
-            for (int q = 0; q < P; ++q) base[q] += step;
+            for (int q = 0; q < kBases; ++q) base[q] += step;
         }
     };
 
@@ -121,8 +129,8 @@ struct Core {
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * (T * 2)));
             return __builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
-        const int r = at + (lane & 31), c = kk * 2 + (lane >> 5);
-        if (P == 2) return *reinterpret_cast<const vec*>(tile + plane * (T * 64) + r * 64 + ((c ^ ((r >> 2) & 3)) * 16));
+        const int r = at + (lane & 31), c = (L ? plane * 4 : 0) + kk * 2 + (lane >> 5);
+        if (P == 2 && !L) return *reinterpret_cast<const vec*>(tile + plane * (T * 64) + r * 64 + ((c ^ ((r >> 2) & 3)) * 16));
         return *reinterpret_cast<const vec*>(tile + r * 128 + ((c ^ ((r >> 1) & 7)) * 16));
     }
 
@@ -162,11 +170,15 @@ struct Core {
         }
     }
 
-    static __device__ void arrive() {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // `more`: the loads of the S - 2 steps behind the one that is waited for are all on their way.
+    static __device__ void arrive(bool more) {
+        constexpr int kBehind = (S - 2) * (kLoadsA + kLoadsB);
+        static_assert(kBehind < 64, "what the counter holds");
+        if (S > 2 && more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(kBehind) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
 
-    // smem: 2 kStage bytes of LDS. `depth`: a multiple of 64, zeros in the operands beyond what counts. `prepare()` runs while the first
+    // smem: S kStage bytes of LDS. `depth`: a multiple of 64, zeros in the operands beyond what counts. `prepare()` runs while the first
     // step's operands are on their way; the sums start from `start(i, e)`, asked behind a barrier that follows it. All waves are
     // past their reads of smem when this returns.
     template <class Prepare, class Start>
@@ -186,12 +198,15 @@ struct Core {
         const int steps = depth / kStep;        // at least one
         constexpr int kLoads = kLoadsA + kLoadsB;
 #pragma unroll
-        for (int l = 0; l < kLoads; ++l) load(0, l);
-        prepare();
-        arrive();
-        if (steps > 1)
+        for (int p = 0; p < S - 1; ++p)
+            if (p == 0 || p < steps)
 #pragma unroll
-            for (int l = 0; l < kLoads / 2; ++l) load(1, l);
+                for (int l = 0; l < kLoads; ++l) load(p, l);
+        prepare();
+        arrive(steps >= S - 1);
+        if (steps >= S)
+#pragma unroll
+            for (int l = 0; l < kLoads / 2; ++l) load(S - 1, l);
 #pragma unroll
         for (int i = 0; i < kI; ++i)
 #pragma unroll
@@ -203,38 +218,44 @@ struct Core {
         Fragments f[2];
 #pragma unroll
         for (int r = 0; r < kReads; ++r) read(f[0], smem, 0, r);
-        // One step. `next`: there is another, the second half of whose loads goes between the first products; `after`: there is one more, the
-        // first half of whose loads goes between the last products, behind the barrier that frees its stage.
-        const auto pass = [&](int s, auto next, auto after) {
-            const char* stage = smem + (s & 1) * kStage;
+        // One step, s, in stage `at`. `next`: there is a step s + S - 1, the second half of whose loads goes between the first products; `after`: there is
+        // one more, the first half of whose loads goes between the last products, behind the barrier that frees this stage.
+        int at = 0;
+        const auto pass = [&](auto next, auto after) {
+            const char* stage = smem + at * kStage;
+            const int following = at + 1 == S ? 0 : at + 1, before = at == 0 ? S - 1 : at - 1;
 #pragma unroll
             for (int kk = 0; kk < kParts; ++kk) {
                 const bool first = kk == 0, last = kk + 1 == kParts;
-                if (last) arrive();
+                if (last) arrive(next());
                 __builtin_amdgcn_sched_barrier(0);
                 multiply(f[kk & 1], [&](int t) {
                     const auto share = [&](int n, int at) { return min(n, at * n * 5 / (4 * kProducts)); };     // done at four fifths of the products
 #pragma unroll
                     for (int r = share(kReads, t); r < share(kReads, t + 1); ++r) {       // of the next part; behind the last step: read, not used
-                        if (last) read(f[0], smem + ((s + 1) & 1) * kStage, 0, r);
+                        if (last) read(f[0], smem + following * kStage, 0, r);
                         else read(f[(kk + 1) & 1], stage, kk + 1, r);
                     }
                     if (first && next())
 #pragma unroll
-                        for (int l = kLoads / 2 + t * (kLoads - kLoads / 2) / kProducts; l < kLoads / 2 + (t + 1) * (kLoads - kLoads / 2) / kProducts; ++l) load((s + 1) & 1, l);
+                        for (int l = kLoads / 2 + t * (kLoads - kLoads / 2) / kProducts; l < kLoads / 2 + (t + 1) * (kLoads - kLoads / 2) / kProducts; ++l) load(before, l);
                     if (last && after())
 #pragma unroll
-                        for (int l = t * (kLoads / 2) / kProducts; l < (t + 1) * (kLoads / 2) / kProducts; ++l) load(s & 1, l);
+                        for (int l = t * (kLoads / 2) / kProducts; l < (t + 1) * (kLoads / 2) / kProducts; ++l) load(at, l);
                     __builtin_amdgcn_sched_barrier(0);
                 });
             }
+            at = following;
         };
         const auto yes = [] { return true; };
         const auto no = [] { return false; };
         int s = 0;
-        for (; s + 2 < steps; ++s) pass(s, yes, yes);
-        if (s + 1 < steps) pass(s++, yes, no);
-        pass(s, no, no);
+        for (; s + S < steps; ++s) pass(yes, yes);
+        if (s + S == steps) {
+            pass(yes, no);
+            ++s;
+        }
+        for (; s < steps; ++s) pass(no, no);
     }
 };
 

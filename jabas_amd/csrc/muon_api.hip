@@ -83,38 +83,52 @@ void describe(Matrix& x, int64_t rows, int64_t cols) {
 int64_t halves_of(const Matrix& x, int planes) { return 4 * x.x_plane + 2 * planes * x.a_plane; }
 int64_t lay_tiles(const Matrix& x) { return static_cast<int64_t>(x.pad_m / kLay) * (x.pad_n / kLay); }
 
-// Tile of the products of some matrices: the one that the model says ends first. A CU holds one workgroup of 256, two of 128, four of 64; `step` is a
-// round's time for 64 of the inner axis, kStart what a tile's start and results cost.
-struct Tile {
-    int size, slots;
-    double step;
+// Which kernel the products of some matrices take: the one whose time, by what was measured, is least. `each` workgroups of a kernel share a CU; a round of
+// them takes `start` us and `step` us for 64 of the inner axis, `alone` where the launch leaves most CUs with one or none. Measured, us, X X^T and then
+// a X + B X, for kSmall, kSmallMany, kMiddle, kMiddleDeep, kLarge (fp32; bf16 next):
+//   12 x  768 x  768   31 32 32 25 54    53 53 44 44 61     18 18 20 18 29    32 28 25 30 31
+//    6 x 1024 x 4096  105 109 110 84 233  203 180 151 168 170   52 52 49 39 84   114 96 75 94 80
+//        1024 x 4096   32 58 92 60 217    37 36 35 30 71     18 33 43 29 79    23 20 20 18 32
+//    3 x 2048 x 2048  112 98 89 87 132   206 183 147 148 151   54 49 37 44 52    91 87 68 73 61
+//        4096 x 4096  329 298 246 240 250  508 471 360 365 327  163 133 108 109 93   249 222 145 159 127
+//   64 x  129 x  257    9 10 13 11 23     14 13 16 19 25      7 7 9 8 12      13 10 12 16 17
+//    4 x  384 x  384    8 10 14 13 31      8 9 15 13 32       6 7 11 11 19     7 7 11 10 19
+struct Cost {
+    int each;
+    double start, alone, step;
 };
-constexpr Tile kTiles[] = {{256, 256, 1.0}, {128, 512, 0.6}, {64, 1024, 0.36}};
-constexpr double kStart = 4.0;
+constexpr Cost kCosts[2][kKernels] = {{{2, 3.0, 0.20, 0.40}, {4, 3.5, 0.50, 0.75}, {2, 7.0, 0.62, 1.00}, {1, 6.0, 0.38, 0.53}, {1, 12.0, 1.25, 1.75}},
+                                      {{2, 3.0, 0.45, 0.82}, {4, 3.5, 0.90, 1.60}, {2, 8.0, 1.35, 2.65}, {1, 6.0, 0.95, 1.30}, {1, 12.0, 3.40, 4.80}}};
+constexpr double kMostCus = 160.0, kCus = 256.0;
 struct Load {
-    double sum[3] = {0, 0, 0}, longest[3] = {0, 0, 0};
-    void add(int t, double tiles, double steps) {
-        sum[t] += tiles * (steps + kStart) * kTiles[t].step / kTiles[t].slots;
-        longest[t] = std::max(longest[t], (steps + kStart) * kTiles[t].step);
+    int planes;
+    double tiles[kKernels] = {}, sum[kKernels] = {}, longest[kKernels] = {};
+    explicit Load(int planes) : planes(planes) {}
+    void add(int kind, double count, double steps, int products) {
+        const Cost& c = kCosts[planes - 1][kind];
+        tiles[kind] += count;
+        sum[kind] += count * (products * c.start + steps * c.step);
+        longest[kind] = std::max(longest[kind], products * c.start + steps * c.alone);
     }
-    int best() const {
+    Kind best() const {
         int at = 0;
         double least = 0.0;
-        for (int t = 0; t < 3; ++t) {
-            const double time = std::max(sum[t], longest[t]);
-            if (t == 0 || time < least) {
+        for (int k = 0; k < kKernels; ++k) {
+            const double here = kCus * kCosts[planes - 1][k].each;
+            const double time = tiles[k] <= kMostCus ? longest[k] : std::max(longest[k], ceil(tiles[k] / here) * sum[k] / tiles[k]);
+            if (k == 0 || time < least) {
                 least = time;
-                at = t;
+                at = k;
             }
         }
-        return kTiles[at].size;
+        return static_cast<Kind>(at);
     }
 };
 void add_symmetric(Load& l, const Matrix& x, double count) {
-    for (int t = 0; t < 3; ++t) l.add(t, count * symmetric_tiles(x.m, kTiles[t].size), (x.pad_n + x.pad_m) / 64.0);
+    for (int k = 0; k < kKernels; ++k) l.add(k, count * symmetric_tiles(x.m, kTile[k]), (x.pad_n + x.pad_m) / 64.0, 2);
 }
 void add_update(Load& l, const Matrix& x, double count) {
-    for (int t = 0; t < 3; ++t) l.add(t, count * update_tiles(x.m, x.n, kTiles[t].size), x.pad_m / 64.0);
+    for (int k = 0; k < kKernels; ++k) l.add(k, count * update_tiles(x.m, x.n, kTile[k]), x.pad_m / 64.0, 1);
 }
 
 enum { kMomentum, kLayOut, kSymmetric, kUpdate, kKinds };
@@ -122,37 +136,36 @@ enum { kMomentum, kLayOut, kSymmetric, kUpdate, kKinds };
 // The launches of some matrices that share a workspace.
 struct Run {
     Work work[kKinds];
-    int tile_symmetric, tile_update;
+    Kind symmetric, update;
     int planes, dtype, nesterov;
     float momentum, fresh;
     const float* grad_scale;
 };
 int run(const Run& r, const JabasNewtonSchulz& ns, const Scales& s, UpdateArgs& last, hipStream_t stream) {
-    PassArgs pass{r.work[kMomentum], r.dtype, r.nesterov, r.momentum, r.fresh, r.grad_scale, ns.eps, static_cast<float>(s.x[0])};
+    PassArgs pass{r.work[kMomentum], r.dtype, r.nesterov, r.momentum, r.fresh, r.grad_scale, ns.eps, static_cast<float>(s.x[0]), r.planes};
     int status = launch_momentum(pass, stream);
     if (status != JABAS_OK) return status;
     pass.w = r.work[kLayOut];
     if ((status = launch_lay(pass, stream)) != JABAS_OK) return status;
     for (int k = 0; k < ns.steps; ++k) {
         SymmetricArgs first{r.work[kSymmetric], k & 1, 0.0f, static_cast<float>(s.a[k] / s.x[k] / s.x[k])};
-        if ((status = launch_symmetric(first, false, r.planes, r.tile_symmetric, stream)) != JABAS_OK) return status;
+        if ((status = launch_symmetric(first, false, r.planes, r.symmetric, stream)) != JABAS_OK) return status;
         first.own = static_cast<float>(ns.b * s.b[k] / s.a[k]);
         first.product = static_cast<float>(ns.c * s.b[k] / s.a[k] / s.a[k]);
-        if ((status = launch_symmetric(first, true, r.planes, r.tile_symmetric, stream)) != JABAS_OK) return status;
+        if ((status = launch_symmetric(first, true, r.planes, r.symmetric, stream)) != JABAS_OK) return status;
         last.w = r.work[kUpdate];
         last.from = k & 1;
         last.last = k + 1 == ns.steps;
         last.own = static_cast<float>(ns.a * s.x[k + 1] / s.x[k]);
         last.product = static_cast<float>(s.x[k + 1] / s.b[k] / s.x[k]);
-        if ((status = launch_update(last, r.planes, r.tile_update, stream)) != JABAS_OK) return status;
+        if ((status = launch_update(last, r.planes, r.update, stream)) != JABAS_OK) return status;
     }
     return JABAS_OK;
 }
 
 // ---- a batch of one shape
 
-// Matrices that go through the workspace together: as many as 256 MiB hold, what the chip's last cache holds between the products. Together they
-// fill the chip long before: a matrix whose share is smaller than this / 8 is small.
+// Matrices that go through the workspace together: as many as 256 MiB hold, what the chip's last cache holds between the products.
 constexpr int64_t kTogether = int64_t{256} << 20;
 
 struct Batch {
@@ -191,6 +204,8 @@ int describe_batch(const JabasOrthogonalize* o, Batch& b, Scales& s) {
     b.at_once = std::min({o->batch, std::max<int64_t>(1, kTogether / (2 * each)), most});
     b.sums_bytes = round_up(8 * b.at_once * b.x.parts, 256);
     b.bytes = b.sums_bytes + round_up(2 * b.at_once * each, 256);
+    const int64_t turns = (o->batch + b.at_once - 1) / b.at_once;
+    b.at_once = (o->batch + turns - 1) / turns;         // turns of one size: a short last one would leave CUs idle
     return JABAS_OK;
 }
 
@@ -200,7 +215,7 @@ constexpr uint32_t kMagic = 0x4d4e5331;
 struct Part {
     uint64_t slots_at[kKinds];
     uint32_t total[kKinds];
-    int32_t tile_symmetric, tile_update;
+    int32_t symmetric, update;      // kernels of the products
 };
 struct Header {
     uint32_t magic, n, n_parts, n_groups;
@@ -302,17 +317,21 @@ int build(const JabasMatrix* list, uint32_t n, int32_t precision, Built& b) {
         b.matrices.push_back(x);
     }
     uint64_t halves_most = 0, sums_most = 0;
+    int64_t left = 0;
+    for (const Matrix& x : b.matrices) left += halves_of(x, planes);
     for (uint32_t first = 0; first < n;) {
+        // parts of about one size: a small last one would leave CUs idle
+        const int64_t share = left / ((2 * left + kTogether - 1) / kTogether);
         int64_t halves = 0, sums = 0, slots[kKinds] = {0, 0, 0, 0};
         uint32_t last = first;
         while (last < n) {
             Matrix& x = b.matrices[last];
             const int64_t need = halves_of(x, planes);
             const int64_t more[kKinds] = {x.parts, lay_tiles(x), symmetric_tiles(x.m, 64), update_tiles(x.m, x.n, 64)};
-            bool full = last > first && 2 * (halves + need) > kTogether;
+            bool full = last > first && (2 * (halves + need) > kTogether || halves + need / 2 > share);
             for (int k = 0; k < kKinds; ++k) {
                 if (more[k] > kMaxSlots) return JABAS_ERR_SIZE;
-                full = full || slots[k] + more[k] > kMaxSlots;
+                full = full || (last > first && slots[k] + more[k] > kMaxSlots);
             }
             if (full) break;
             x.x_at = halves;
@@ -323,21 +342,22 @@ int build(const JabasMatrix* list, uint32_t n, int32_t precision, Built& b) {
             for (int k = 0; k < kKinds; ++k) slots[k] += more[k];
             ++last;
         }
+        left -= halves;
         halves_most = std::max<uint64_t>(halves_most, halves);
         sums_most = std::max<uint64_t>(sums_most, sums);
-        Load symmetric, update;
+        Load symmetric(planes), update(planes);
         for (uint32_t i = first; i < last; ++i) {
             add_symmetric(symmetric, b.matrices[i], 1);
             add_update(update, b.matrices[i], 1);
         }
         Part p{};
-        p.tile_symmetric = symmetric.best();
-        p.tile_update = update.best();
+        p.symmetric = symmetric.best();
+        p.update = update.best();
         for (int k = 0; k < kKinds; ++k) {
             std::vector<int64_t> tiles;
             for (uint32_t i = first; i < last; ++i) {
                 const Matrix& x = b.matrices[i];
-                tiles.push_back(k == kMomentum ? x.parts : k == kLayOut ? lay_tiles(x) : k == kSymmetric ? symmetric_tiles(x.m, p.tile_symmetric) : update_tiles(x.m, x.n, p.tile_update));
+                tiles.push_back(k == kMomentum ? x.parts : k == kLayOut ? lay_tiles(x) : k == kSymmetric ? symmetric_tiles(x.m, kTile[p.symmetric]) : update_tiles(x.m, x.n, kTile[p.update]));
             }
             p.slots_at[k] = b.slots.size();
             deal(b.slots, tiles, first);
@@ -401,12 +421,12 @@ JABAS_API int jabas_orthogonalize(const JabasOrthogonalize* o, void* workspace, 
     const int64_t size = o->dtype == JABAS_F32 ? 4 : 2, each = halves_of(x, b.planes);
     for (int64_t done = 0; done < o->batch; done += b.at_once) {
         const int64_t here = std::min(b.at_once, o->batch - done);
-        Load symmetric, update;
+        Load symmetric(b.planes), update(b.planes);
         add_symmetric(symmetric, x, static_cast<double>(here));
         add_update(update, x, static_cast<double>(here));
         Run r{};
-        r.tile_symmetric = symmetric.best();
-        r.tile_update = update.best();
+        r.symmetric = symmetric.best();
+        r.update = update.best();
         r.planes = b.planes;
         r.dtype = o->dtype;
         Work w{};
@@ -421,7 +441,7 @@ JABAS_API int jabas_orthogonalize(const JabasOrthogonalize* o, void* workspace, 
         w.part_step = x.parts;
         w.sums = static_cast<double*>(workspace);
         w.halves = static_cast<char*>(workspace) + b.sums_bytes;
-        const int64_t per[kKinds] = {x.parts, lay_tiles(x), symmetric_tiles(x.m, r.tile_symmetric), update_tiles(x.m, x.n, r.tile_update)};
+        const int64_t per[kKinds] = {x.parts, lay_tiles(x), symmetric_tiles(x.m, kTile[r.symmetric]), update_tiles(x.m, x.n, kTile[r.update])};
         for (int k = 0; k < kKinds; ++k) {
             r.work[k] = w;
             r.work[k].per = static_cast<int32_t>(per[k]);
@@ -495,8 +515,8 @@ JABAS_API int jabas_muon_step(const void* plan_host, const void* plan_dev, const
     }
     for (uint32_t p = 0; p < h->n_parts; ++p) {
         Run r{};
-        r.tile_symmetric = parts[p].tile_symmetric;
-        r.tile_update = parts[p].tile_update;
+        r.symmetric = static_cast<Kind>(parts[p].symmetric);
+        r.update = static_cast<Kind>(parts[p].update);
         r.planes = h->precision == JABAS_F32 ? 2 : 1;
         r.dtype = JABAS_F32;
         r.nesterov = args->nesterov != 0;

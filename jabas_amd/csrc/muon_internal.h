@@ -10,7 +10,7 @@ namespace jabas {
 namespace muon {
 
 constexpr int kPad = 64;            // sides of the copies that the products read are multiples of this
-constexpr int kParts = 256;         // partial sums of a matrix's length
+constexpr int kParts = 1024;        // partial sums of a matrix's length, at most
 constexpr int kMinChunk = 4096;     // elements of one of them, at least
 constexpr int kLay = 64;            // tile of the pass that lays a matrix out
 
@@ -20,8 +20,8 @@ struct Matrix {
     float* momentum;                // NULL: none, X is made of src
     void* out;                      // the weights (with momentum), else where X goes
     int64_t src_stride;             // of a row
-    int64_t x_at, a_at, part_at;    // places in the workspace: X (4 planes: two buffers of two) and A, B in halves, partial sums in doubles
-    int64_t x_plane, a_plane;       // halves apart
+    int64_t x_at, a_at, part_at;    // places in the workspace: X (two buffers of two planes) and A, B in halves, partial sums in doubles
+    int64_t x_plane, a_plane;       // halves of a plane of X, of A
     int32_t rows, cols;             // of src and out
     int32_t m, n, pad_m, pad_n;
     int32_t tall;
@@ -31,6 +31,15 @@ struct Matrix {
     float lr_factor;
     uint32_t n_fanout, fanout_at;   // replicas: pointers in the list's table
 };
+
+// Where element (row, col) of a matrix with `pad` columns lies, in halves, and how far behind its first plane its second is. Products of two planes read them
+// from one line, 32 of either by turns; a product of one plane reads nothing of the second.
+template <int P>
+__host__ __device__ inline int64_t stride_of(int pad) { return P == 2 ? 2 * static_cast<int64_t>(pad) : pad; }
+template <int P>
+__host__ __device__ inline int64_t half_at(int row, int col, int pad) { return row * stride_of<P>(pad) + (P == 2 ? (col >> 5) * 64 + (col & 31) : col); }
+template <int P>
+__host__ __device__ inline int64_t second_of(int64_t plane) { return P == 2 ? 32 : plane; }
 
 // Which workgroup does what. A list: `table` and a slot {matrix, tile} for every workgroup. A batch: matrix 0 and what lies between it and
 // the next one.
@@ -59,6 +68,7 @@ struct PassArgs {
     const float* grad_scale;
     double eps;
     float scale;                    // of X's planes
+    int32_t planes;                 // of the products
 };
 int launch_momentum(const PassArgs& a, hipStream_t stream);
 int launch_lay(const PassArgs& a, hipStream_t stream);
@@ -78,8 +88,11 @@ struct UpdateArgs {
     float own, product;
     float lr[JABAS_MAX_GROUPS], keep[JABAS_MAX_GROUPS];     // keep = 1 - lr weight_decay
 };
-int launch_symmetric(const SymmetricArgs& a, bool second, int planes, int tile, hipStream_t stream);
-int launch_update(const UpdateArgs& a, int planes, int tile, hipStream_t stream);
+// The products' kernels: their tiles and what tells them apart.
+enum Kind { kSmall, kSmallMany, kMiddle, kMiddleDeep, kLarge, kKernels };     // 64, four stages or two; 128, two stages or four; 256
+constexpr int kTile[kKernels] = {64, 64, 128, 128, 256};
+int launch_symmetric(const SymmetricArgs& a, bool second, int planes, Kind kind, hipStream_t stream);
+int launch_update(const UpdateArgs& a, int planes, Kind kind, hipStream_t stream);
 
 inline int64_t symmetric_tiles(int64_t m, int tile) { const int64_t t = (m + tile - 1) / tile; return t * (t + 1) / 2; }
 inline int64_t update_tiles(int64_t m, int64_t n, int tile) { return (m + tile - 1) / tile * ((n + tile - 1) / tile); }

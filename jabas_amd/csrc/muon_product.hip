@@ -22,18 +22,16 @@ __device__ inline uint16_t to_bf16(float x) {
 }
 
 // Eight values and their planes.
+template <int P>
+struct Planes {
+    f16x8 v[P];
+};
 struct Eight {
     float v[8];
-    __device__ void add_planes(const _Float16* hi, const _Float16* lo, float factor) {
-        const f16x8 h = *reinterpret_cast<const f16x8*>(hi);
-        if (lo) {
-            const f16x8 l = *reinterpret_cast<const f16x8*>(lo);
+    template <int P>
+    __device__ void add(const Planes<P>& x, float factor) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = fmaf(static_cast<float>(h[e]) + static_cast<float>(l[e]), factor, v[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = fmaf(static_cast<float>(h[e]), factor, v[e]);
-        }
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(static_cast<float>(x.v[0][e]) + (P == 2 ? static_cast<float>(x.v[P - 1][e]) : 0.0f), factor, v[e]);
     }
     __device__ void put_planes(_Float16* hi, _Float16* lo) const {
         f16x8 h, l;
@@ -80,6 +78,21 @@ struct Staged {
         for (int h = 0; h < 2; ++h) *reinterpret_cast<f32x4*>(chunk(r, (col >> 2) + h)) = f32x4{x.v[h * 4], x.v[h * 4 + 1], x.v[h * 4 + 2], x.v[h * 4 + 3]};
     }
     __device__ float at(int r, int col) const { return chunk(r, col >> 2)[col & 3]; }
+    // Eights of a row are taken kGroup at a time, group g of block column j, and those of the matrix that is added to are read a group ahead.
+    static constexpr int kEach = C::kI * 2, kGroup = kEach < 4 ? kEach : 4, kGroups = kEach / kGroup;
+    static __device__ int row(int t) { return (t * 64 + static_cast<int>(threadIdx.x & 63)) / (C::kI * 4); }
+    static __device__ int col(int t) { return (t * 64 + static_cast<int>(threadIdx.x & 63)) % (C::kI * 4) * 8; }
+    // Q planes of a matrix laid out for products of P
+    template <int P, int Q>
+    static __device__ void fetch(Planes<Q> (&x)[kGroup], int g, const _Float16* from, int64_t plane, int row0, int rows, int col0, int cols) {
+#pragma unroll
+        for (int t = 0; t < kGroup; ++t) {
+            const int r = row0 + row(g * kGroup + t), c = col0 + col(g * kGroup + t);
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+                if (r < rows && c < cols) x[t].v[q] = *reinterpret_cast<const f16x8*>(from + half_at<P>(r, c, cols) + q * second_of<P>(plane));
+        }
+    }
 };
 
 // LDS written by a wave is read by other lanes of it behind this.
@@ -89,58 +102,237 @@ __device__ inline void wave_done() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// Tile `tile` of those on and under the diagonal, row by row.
+__device__ inline void triangle(uint32_t tile, int& tm, int& tn) {
+    int row = static_cast<int>((sqrtf(8.0f * tile + 1.0f) - 1.0f) * 0.5f);         // the last row that starts at or before `tile`
+    while (static_cast<uint32_t>(row) * (row + 1) / 2 > tile) --row;
+    while (static_cast<uint32_t>(row + 1) * (row + 2) / 2 <= tile) ++row;
+    tn = row;
+    tm = static_cast<int>(tile - static_cast<uint32_t>(row) * (row + 1) / 2);
+}
+
 // A = X X^T, or (SECOND) B = b A + c A A: tiles on and under the diagonal, written where they are and mirrored.
 template <int P, class C, bool SECOND>
 __global__ __launch_bounds__(C::kThreads) void symmetric_kernel(SymmetricArgs a) {
-    __shared__ __align__(16) char smem[2 * C::kStage];
+    __shared__ __align__(16) char smem[C::kStages * C::kStage];
     Place at;
     if (!place_of(a.w, at)) return;
     const Matrix& x = at.x;
-    int tn = static_cast<int>((sqrtf(8.0f * at.tile + 1.0f) - 1.0f) * 0.5f);        // the last row of tiles that starts at or before `tile`
-    while (static_cast<uint32_t>(tn * (tn + 1)) / 2 > at.tile) --tn;
-    while (static_cast<uint32_t>((tn + 1) * (tn + 2)) / 2 <= at.tile) ++tn;
-    const int tm = at.tile - tn * (tn + 1) / 2, m0 = tm * C::kM, n0 = tn * C::kN, lane = threadIdx.x & 63;
+    int tm, tn;
+    triangle(at.tile, tm, tn);
+    const int m0 = tm * C::kM, n0 = tn * C::kN, lane = threadIdx.x & 63;
     _Float16* base = static_cast<_Float16*>(a.w.halves);
     _Float16 *own = base + x.a_at, *to = own + (SECOND ? P * x.a_plane : 0);
-    const Operand o = SECOND ? Operand{own, x.pad_m, x.a_plane, x.m} : Operand{base + x.x_at + a.from * 2 * x.x_plane, x.pad_n, x.x_plane, x.m};
+    const Operand o = SECOND ? Operand{own, stride_of<P>(x.pad_m), second_of<P>(x.a_plane), x.m}
+                             : Operand{base + x.x_at + a.from * 2 * x.x_plane, stride_of<P>(x.pad_n), second_of<P>(x.x_plane), x.m};
     C c;
     c.run(o, o, m0, n0, SECOND ? x.pad_m : x.pad_n, smem, [] {}, [](int, int) { return 0.0f; });
     const Staged<C> staged(smem);
+    using S = Staged<C>;
     const int wm = m0 + C::wave_m(), wn = n0 + C::wave_n();
+    Planes<P> beside[2][S::kGroup];
+    if (SECOND) S::template fetch<P, P>(beside[0], 0, own, x.a_plane, wn, x.m, wm, x.pad_m);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < C::kJ; ++j) {
         wave_done();
         staged.put(c, j, a.product);
         wave_done();
-#pragma unroll 2
-        for (int t = 0; t < C::kI * 2; ++t) {
-            const int f = t * 64 + lane, r = f / (C::kI * 4), col = f % (C::kI * 4) * 8, row = wn + j * 32 + r, m = wm + col;
-            if (row >= x.m || m >= x.pad_m) continue;
-            Eight v;
-            staged.get(r, col, v);
-            const int64_t place = static_cast<int64_t>(row) * x.pad_m + m;
-            if (SECOND) {
-                v.add_planes(own + place, P == 2 ? own + x.a_plane + place : nullptr, a.own);
-                staged.set(r, col, v);
-            }
-            if (m + 8 > x.m)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v.v[e] = m + e < x.m ? v.v[e] : 0.0f;
-            v.put_planes(to + place, P == 2 ? to + x.a_plane + place : nullptr);
+        for (int g = 0; g < S::kGroups; ++g) {
+            const int now = j * S::kGroups + g, after = now + 1;
+            if (SECOND && after < C::kJ * S::kGroups)
+                S::template fetch<P, P>(beside[after & 1], after % S::kGroups, own, x.a_plane, wn + after / S::kGroups * 32, x.m, wm, x.pad_m);
+#pragma unroll
+            for (int t = 0; t < S::kGroup; ++t) {
+                const int r = S::row(g * S::kGroup + t), col = S::col(g * S::kGroup + t), row = wn + j * 32 + r, m = wm + col;
+                if (row >= x.m || m >= x.pad_m) continue;
+                Eight v;
+                staged.get(r, col, v);
+                const int64_t place = half_at<P>(row, m, x.pad_m);
+                if (SECOND) {
+                    v.add(beside[now & 1][t], a.own);
+                    staged.set(r, col, v);
+                }
+                if (m + 8 > x.m)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v.v[e] = m + e < x.m ? v.v[e] : 0.0f;
+                v.put_planes(to + place, P == 2 ? to + place + second_of<P>(x.a_plane) : nullptr);
+            }
         }
         if (tm == tn) continue;
         wave_done();
 #pragma unroll 2
         for (int t = 0; t < C::kI * 2; ++t) {       // column wm + col of the tile is row of the mirrored one
-            const int f = t * 64 + lane, col = f % (C::kI * 32), r = f / (C::kI * 32) * 8, row = wm + col, m = wn + j * 32 + r;
+            const int f = t * 64 + lane, col = f / 4, r = f % 4 * 8, row = wm + col, m = wn + j * 32 + r;
             if (row >= x.m || m >= x.pad_m) continue;
             Eight v;
 #pragma unroll
             for (int e = 0; e < 8; ++e) v.v[e] = m + e < x.m ? staged.at(r + e, col) : 0.0f;
-            const int64_t place = static_cast<int64_t>(row) * x.pad_m + m;
-            v.put_planes(to + place, P == 2 ? to + x.a_plane + place : nullptr);
+            const int64_t place = half_at<P>(row, m, x.pad_m);
+            v.put_planes(to + place, P == 2 ? to + place + second_of<P>(x.a_plane) : nullptr);
         }
+    }
+}
+
+// Tiles of 64 x 64, for launches that leave a CU one or a few of them: what a step takes then is the way of its loads (about half a microsecond
+// behind a kernel that wrote them on another die) and the chain of barrier, LDS read and product. So S stages of LDS are on their way at once, a wave
+// has all it multiplies in a step in registers a step ahead, and the four waves are two halves of the inner axis by two halves of n, which reads LDS less
+// than four quarters of the tile do. The halves' sums meet in LDS.
+template <int P, bool TA, int S>
+struct Deep {
+    using C = Core<F16, P, 64, 64, 2, 2, TA, false, false, false, 2, P == 2>;
+    static constexpr int kThreads = 256, kLoads = C::kLoadsA + C::kLoadsB, kHalf = C::kParts / 2, kRow = 68;    // kRow: floats of a row of sums
+    static constexpr int kBytes = S * C::kStage > 64 * kRow * 4 ? S * C::kStage : 64 * kRow * 4;
+    static_assert((S - 1) * kLoads < 64, "what the counter holds");
+
+    struct Fragments {
+        f16x8 a[kHalf][2][P], b[kHalf][P];
+    };
+    static __device__ int half() { return (threadIdx.x >> 6) & 1; }
+    static __device__ int column() { return (threadIdx.x >> 7) * 32; }
+
+    static __device__ void read(Fragments& f, const char* stage) {
+#pragma unroll
+        for (int k = 0; k < kHalf; ++k) {
+            const int kk = half() * kHalf + k;
+#pragma unroll
+            for (int q = 0; q < P; ++q) {
+                f.b[k][q] = C::template fragment<64, false>(stage + C::kBytesA, column(), kk, q);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) f.a[k][i][q] = C::template fragment<64, TA>(stage, i * 32, kk, q);
+            }
+        }
+    }
+    static __device__ void multiply(const Fragments& f, loss::f32x16 (&acc)[2]) {
+#pragma unroll
+        for (int k = 0; k < kHalf; ++k) {
+            if (P == 2) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) acc[i] = F16::mfma(f.a[k][i][P - 1], f.b[k][0], acc[i]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) acc[i] = F16::mfma(f.a[k][i][0], f.b[k][P - 1], acc[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) acc[i] = F16::mfma(f.a[k][i][0], f.b[k][0], acc[i]);
+        }
+    }
+    // Waits until at most `Behind` steps' loads are on their way, and for the other waves.
+    template <int Behind>
+    static __device__ void arrive() {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(Behind * kLoads) : "memory");
+    }
+
+    // The tile's sums times `factor`, row n of kRow floats, in smem. Everyone may read them when this returns.
+    static __device__ float* run(const Operand& a, const Operand& b, int m0, int n0, int depth, float factor, char* smem) {
+        typename C::template Source<64, TA> sa(a, m0);
+        typename C::template Source<64, false> sb(b, n0);
+        const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem));
+        const auto load = [&](int stage) {
+            const uint32_t to = lds + stage * C::kStage;
+#pragma unroll
+            for (int l = 0; l < C::kLoadsA; ++l) sa.issue(to, l);
+#pragma unroll
+            for (int l = 0; l < C::kLoadsB; ++l) sb.issue(to + C::kBytesA, l);
+            sa.advance();
+            sb.advance();
+        };
+        const int steps = depth / C::kStep;     // at least one
+        for (int s = 0; s < min(S, steps); ++s) load(s);
+        loss::f32x16 acc[2] = {};
+        if (steps >= S) arrive<S - 1>();
+        else arrive<0>();
+        Fragments f[2];
+        read(f[0], smem);
+        int at = 0;
+        // Step s, whose fragments are `now`.
+        const auto pass = [&](int s, const Fragments& now, Fragments& next) {
+            if (s + S <= steps) arrive<S - 2>();
+            else arrive<0>();
+            const int following = at + 1 == S ? 0 : at + 1;
+            if (s + S < steps) load(at);
+            read(next, smem + following * C::kStage);       // behind the last step: read, not used
+            multiply(now, acc);
+            at = following;
+        };
+        int s = 0;
+        for (; s + 2 <= steps; s += 2) {
+            pass(s, f[0], f[1]);
+            pass(s + 1, f[1], f[0]);
+        }
+        if (s < steps) pass(s, f[0], f[1]);
+        arrive<0>();
+        float* sums = reinterpret_cast<float*>(smem);
+        const int lane = threadIdx.x & 63;
+        const auto quad = [&](int i, int q) { return reinterpret_cast<f32x4*>(sums + (column() + (lane & 31)) * kRow + i * 32 + q * 8 + (lane >> 5) * 4); };
+        const auto value = [&](int i, int q) { return f32x4{acc[i][q * 4], acc[i][q * 4 + 1], acc[i][q * 4 + 2], acc[i][q * 4 + 3]}; };
+        if (half() == 0)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) *quad(i, q) = value(i, q);
+        __syncthreads();
+        if (half() == 1)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) *quad(i, q) = (*quad(i, q) + value(i, q)) * factor;
+        __syncthreads();
+        return sums;
+    }
+    // Eight `t` (of two) of a thread: its row and column in the tile.
+    static __device__ int row(int t) { return t * 32 + (threadIdx.x >> 3); }
+    static __device__ int col() { return (threadIdx.x & 7) * 8; }
+};
+
+template <int P, bool SECOND, int S>
+__global__ __launch_bounds__(256) void symmetric_deep_kernel(SymmetricArgs a) {
+    using D = Deep<P, false, S>;
+    __shared__ __align__(16) char smem[D::kBytes];
+    Place at;
+    if (!place_of(a.w, at)) return;
+    const Matrix& x = at.x;
+    int tm, tn;
+    triangle(at.tile, tm, tn);
+    const int m0 = tm * 64, n0 = tn * 64;
+    _Float16* base = static_cast<_Float16*>(a.w.halves);
+    _Float16 *own = base + x.a_at, *to = own + (SECOND ? P * x.a_plane : 0);
+    const Operand o = SECOND ? Operand{own, stride_of<P>(x.pad_m), second_of<P>(x.a_plane), x.m}
+                             : Operand{base + x.x_at + a.from * 2 * x.x_plane, stride_of<P>(x.pad_n), second_of<P>(x.x_plane), x.m};
+    float* sums = D::run(o, o, m0, n0, SECOND ? x.pad_m : x.pad_n, a.product, smem);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int r = D::row(t), row = n0 + r, m = m0 + D::col();
+        if (row >= x.m || m >= x.pad_m) continue;
+        const int64_t place = half_at<P>(row, m, x.pad_m);
+        Eight v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v.v[e] = sums[r * D::kRow + D::col() + e];
+        if (SECOND) {
+            Planes<P> p;
+#pragma unroll
+            for (int q = 0; q < P; ++q) p.v[q] = *reinterpret_cast<const f16x8*>(own + place + q * second_of<P>(x.a_plane));
+            v.add(p, a.own);
+            if (tm != tn)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sums[r * D::kRow + D::col() + e] = v.v[e];
+        }
+        if (m + 8 > x.m)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v.v[e] = m + e < x.m ? v.v[e] : 0.0f;
+        v.put_planes(to + place, P == 2 ? to + place + second_of<P>(x.a_plane) : nullptr);
+    }
+    if (tm == tn) return;
+    if (SECOND) __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {       // column m0 + col of the tile is a row of the mirrored one
+        const int col = D::row(t), r = D::col(), row = m0 + col, m = n0 + r;
+        if (row >= x.m || m >= x.pad_m) continue;
+        Eight v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v.v[e] = m + e < x.m ? sums[(r + e) * D::kRow + col] : 0.0f;
+        const int64_t place = half_at<P>(row, m, x.pad_m);
+        v.put_planes(to + place, P == 2 ? to + place + second_of<P>(x.a_plane) : nullptr);
     }
 }
 
@@ -196,61 +388,139 @@ __device__ inline void put_out(const UpdateArgs& a, const Matrix& x, int row, in
     }
 }
 
+// Tile `tile` of across x down, in bands of eight of m, so that tiles in flight together share their operands' rows.
+__device__ inline void band(uint32_t tile, int across, int down, int& tm, int& tn) {
+    const int which = static_cast<int>(tile / (8u * down)), first = which * 8, height = min(8, across - first), in = static_cast<int>(tile - which * 8u * down);
+    tm = first + in % height;
+    tn = in / height;
+}
+
 // X <- a X + B X, in planes, or at the last step to the weights. X lies with its rows of k: transposing reads take it as it is.
 template <int P, class C>
 __global__ __launch_bounds__(C::kThreads) void update_kernel(UpdateArgs a) {
-    __shared__ __align__(16) char smem[2 * C::kStage];
+    __shared__ __align__(16) char smem[C::kStages * C::kStage];
     Place at;
     if (!place_of(a.w, at)) return;
     const Matrix& x = at.x;
-    // bands of eight tiles of m, so that tiles in flight together share their operands' rows
-    const int across = (x.n + C::kM - 1) / C::kM, down = (x.m + C::kN - 1) / C::kN;
-    const int band = at.tile / (8 * down), first = band * 8, height = min(8, across - first), in = at.tile - band * 8 * down;
-    const int m0 = (first + in % height) * C::kM, n0 = in / height * C::kN, lane = threadIdx.x & 63;
+    int m0, n0;
+    band(at.tile, (x.n + C::kM - 1) / C::kM, (x.m + C::kN - 1) / C::kN, m0, n0);
+    m0 *= C::kM;
+    n0 *= C::kN;
+    const int lane = threadIdx.x & 63;
     _Float16* base = static_cast<_Float16*>(a.w.halves);
     const _Float16* from = base + x.x_at + a.from * 2 * x.x_plane;
     _Float16* to = base + x.x_at + (1 - a.from) * 2 * x.x_plane;
     C c;
-    c.run(Operand{from, x.pad_n, x.x_plane, x.pad_n}, Operand{base + x.a_at + P * x.a_plane, x.pad_m, x.a_plane, x.m}, m0, n0, x.pad_m, smem, [] {},
+    c.run(Operand{from, stride_of<P>(x.pad_n), second_of<P>(x.x_plane), x.pad_n},
+          Operand{base + x.a_at + P * x.a_plane, stride_of<P>(x.pad_m), second_of<P>(x.a_plane), x.m}, m0, n0, x.pad_m, smem, [] {},
           [](int, int) { return 0.0f; });
     const Staged<C> staged(smem);
+    using S = Staged<C>;
     const int wm = m0 + C::wave_m(), wn = n0 + C::wave_n();
+    Planes<2> beside[2][S::kGroup];
+    S::template fetch<P, 2>(beside[0], 0, from, x.x_plane, wn, x.m, wm, x.pad_n);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < C::kJ; ++j) {
         wave_done();
         staged.put(c, j, a.product);
         wave_done();
-#pragma unroll 2
-        for (int t = 0; t < C::kI * 2; ++t) {
-            const int f = t * 64 + lane, r = f / (C::kI * 4), col = f % (C::kI * 4) * 8, row = wn + j * 32 + r, m = wm + col;
-            if (row >= (a.last ? x.m : x.pad_m) || m >= x.pad_n) continue;
-            const int64_t place = static_cast<int64_t>(row) * x.pad_n + m;
-            Eight v;
-            staged.get(r, col, v);
-            v.add_planes(from + place, from + x.x_plane + place, a.own);
-            if (!a.last) {
-                if (row >= x.m)         // the next product takes these rows of k as well
+#pragma unroll
+        for (int g = 0; g < S::kGroups; ++g) {
+            const int now = j * S::kGroups + g, after = now + 1;
+            if (after < C::kJ * S::kGroups)
+                S::template fetch<P, 2>(beside[after & 1], after % S::kGroups, from, x.x_plane, wn + after / S::kGroups * 32, x.m, wm, x.pad_n);
+#pragma unroll
+            for (int t = 0; t < S::kGroup; ++t) {
+                const int r = S::row(g * S::kGroup + t), col = S::col(g * S::kGroup + t), row = wn + j * 32 + r, m = wm + col;
+                if (row >= (a.last ? x.m : x.pad_m) || m >= x.pad_n) continue;
+                const int64_t place = half_at<P>(row, m, x.pad_n);
+                Eight v;
+                if (row < x.m) {
+                    staged.get(r, col, v);
+                    v.add(beside[now & 1][t], a.own);
+                } else {            // the next product takes these rows of k as well
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v.v[e] = 0.0f;
-                v.put_planes(to + place, to + x.x_plane + place);
-            } else if (x.tall) {
-                staged.set(r, col, v);
-            } else if (m < x.n) {
+                }
+                if (a.last) staged.set(r, col, v);
+                else v.put_planes(to + place, to + place + second_of<P>(x.x_plane));
+            }
+        }
+        if (!a.last) continue;
+        wave_done();
+        if (x.tall) {
+#pragma unroll 1
+            for (int t = 0; t < C::kI * 4; ++t) {       // column wm + col of X is a row of the weights
+                const int f = t * 64 + lane, r = f % 8 * 4, col = f / 8, row = wm + col, m = wn + j * 32 + r;
+                if (row >= x.rows || m >= x.cols) continue;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = staged.at(r + e, col);
+                put_out<4>(a, x, row, m, v);
+            }
+        } else {
+#pragma unroll 1
+            for (int t = 0; t < S::kEach; ++t) {
+                const int r = S::row(t), col = S::col(t), row = wn + j * 32 + r, m = wm + col;
+                if (row >= x.rows || m >= x.cols) continue;
+                Eight v;
+                staged.get(r, col, v);
                 put_out<8>(a, x, row, m, v.v);
             }
         }
-        if (!a.last || !x.tall) continue;
-        wave_done();
-#pragma unroll 2
-        for (int t = 0; t < C::kI * 4; ++t) {       // column wm + col of X is a row of the weights
-            const int f = t * 64 + lane, r = f % 8 * 4, col = f / 8, row = wm + col, m = wn + j * 32 + r;
-            if (row >= x.rows || m >= x.cols) continue;
-            float v[4];
+    }
+}
+
+// The same with small tiles.
+template <int P, int S>
+__global__ __launch_bounds__(256) void update_deep_kernel(UpdateArgs a) {
+    using D = Deep<P, true, S>;
+    __shared__ __align__(16) char smem[D::kBytes];
+    Place at;
+    if (!place_of(a.w, at)) return;
+    const Matrix& x = at.x;
+    int m0, n0;
+    band(at.tile, (x.n + 63) / 64, (x.m + 63) / 64, m0, n0);
+    m0 *= 64;
+    n0 *= 64;
+    _Float16* base = static_cast<_Float16*>(a.w.halves);
+    const _Float16* from = base + x.x_at + a.from * 2 * x.x_plane;
+    _Float16* to = base + x.x_at + (1 - a.from) * 2 * x.x_plane;
+    float* sums = D::run(Operand{from, stride_of<P>(x.pad_n), second_of<P>(x.x_plane), x.pad_n},
+          Operand{base + x.a_at + P * x.a_plane, stride_of<P>(x.pad_m), second_of<P>(x.a_plane), x.m}, m0, n0, x.pad_m, a.product, smem);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = staged.at(r + e, col);
-            put_out<4>(a, x, row, m, v);
+    for (int t = 0; t < 2; ++t) {
+        const int r = D::row(t), row = n0 + r, m = m0 + D::col();       // whole rows of the padded copy, up to pad_m and pad_n
+        const int64_t place = half_at<P>(row, m, x.pad_n);
+        Eight v;
+        if (row < x.m) {
+            Planes<2> p;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) p.v[q] = *reinterpret_cast<const f16x8*>(from + place + q * second_of<P>(x.x_plane));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v.v[e] = sums[r * D::kRow + D::col() + e];
+            v.add(p, a.own);
+        } else {                    // the next product takes these rows of k as well
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v.v[e] = 0.0f;
         }
+        if (!a.last) v.put_planes(to + place, to + place + second_of<P>(x.x_plane));
+        else if (x.tall)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sums[r * D::kRow + D::col() + e] = v.v[e];
+        else if (row < x.m && m < x.n) put_out<8>(a, x, row, m, v.v);
+    }
+    if (!a.last || !x.tall) return;
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {       // column m0 + col of X is a row of the weights
+        const int col = D::row(t), r = D::col(), row = m0 + col, m = n0 + r;
+        if (row >= x.rows || m >= x.cols) continue;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = sums[(r + e) * D::kRow + col];
+        put_out<8>(a, x, row, m, v);
     }
 }
 
@@ -260,27 +530,50 @@ int launch(K kernel, int threads, const A& args, hipStream_t stream) {
     return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3(args.w.total), dim3(threads), params, 0, stream) == hipSuccess ? JABAS_OK : JABAS_ERR_LAUNCH;
 }
 
-template <int P, int T, int WM, int WN>
+template <int P, int T, int WM, int WN, int S = 2>
 int symmetric(const SymmetricArgs& a, bool second, hipStream_t stream) {
-    using C = Core<F16, P, T, T, WM, WN, false, false, false, false>;
+    using C = Core<F16, P, T, T, WM, WN, false, false, false, false, S, P == 2>;
     return second ? launch(symmetric_kernel<P, C, true>, C::kThreads, a, stream) : launch(symmetric_kernel<P, C, false>, C::kThreads, a, stream);
 }
-template <int P, int T, int WM, int WN>
+template <int P, int T, int WM, int WN, int S = 2>
 int update(const UpdateArgs& a, hipStream_t stream) {
-    using C = Core<F16, P, T, T, WM, WN, true, false, false, false>;
+    using C = Core<F16, P, T, T, WM, WN, true, false, false, false, S, P == 2>;
     return launch(update_kernel<P, C>, C::kThreads, a, stream);
+}
+
+template <int P, int S>
+int symmetric_deep(const SymmetricArgs& a, bool second, hipStream_t stream) {
+    return second ? launch(symmetric_deep_kernel<P, true, S>, 256, a, stream) : launch(symmetric_deep_kernel<P, false, S>, 256, a, stream);
+}
+
+template <int P>
+int symmetric(const SymmetricArgs& a, bool second, Kind kind, hipStream_t stream) {
+    switch (kind) {
+        case kSmall: return symmetric_deep<P, 4>(a, second, stream);
+        case kSmallMany: return symmetric_deep<P, 2>(a, second, stream);
+        case kMiddle: return symmetric<P, 128, 2, 2, 2>(a, second, stream);
+        case kMiddleDeep: return symmetric<P, 128, 2, 2, 4>(a, second, stream);
+        default: return symmetric<P, 256, 2, 4>(a, second, stream);
+    }
+}
+template <int P>
+int update(const UpdateArgs& a, Kind kind, hipStream_t stream) {
+    switch (kind) {
+        case kSmall: return launch(update_deep_kernel<P, 4>, 256, a, stream);
+        case kSmallMany: return launch(update_deep_kernel<P, 2>, 256, a, stream);
+        case kMiddle: return update<P, 128, 2, 2, 2>(a, stream);
+        case kMiddleDeep: return update<P, 128, 2, 2, 4>(a, stream);
+        default: return update<P, 256, 2, 4>(a, stream);
+    }
 }
 
 }  // namespace
 
-int launch_symmetric(const SymmetricArgs& a, bool second, int planes, int tile, hipStream_t stream) {
-    if (planes == 2) return tile == 256 ? symmetric<2, 256, 2, 4>(a, second, stream) : tile == 128 ? symmetric<2, 128, 2, 2>(a, second, stream) : symmetric<2, 64, 2, 2>(a, second, stream);
-    return tile == 256 ? symmetric<1, 256, 2, 4>(a, second, stream) : tile == 128 ? symmetric<1, 128, 2, 2>(a, second, stream) : symmetric<1, 64, 2, 2>(a, second, stream);
+int launch_symmetric(const SymmetricArgs& a, bool second, int planes, Kind kind, hipStream_t stream) {
+    return planes == 2 ? symmetric<2>(a, second, kind, stream) : symmetric<1>(a, second, kind, stream);
 }
-
-int launch_update(const UpdateArgs& a, int planes, int tile, hipStream_t stream) {
-    if (planes == 2) return tile == 256 ? update<2, 256, 2, 4>(a, stream) : tile == 128 ? update<2, 128, 2, 2>(a, stream) : update<2, 64, 2, 2>(a, stream);
-    return tile == 256 ? update<1, 256, 2, 4>(a, stream) : tile == 128 ? update<1, 128, 2, 2>(a, stream) : update<1, 64, 2, 2>(a, stream);
+int launch_update(const UpdateArgs& a, int planes, Kind kind, hipStream_t stream) {
+    return planes == 2 ? update<2>(a, kind, stream) : update<1>(a, kind, stream);
 }
 
 }  // namespace muon

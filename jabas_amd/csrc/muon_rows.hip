@@ -102,7 +102,7 @@ __global__ __launch_bounds__(256) void momentum_kernel(PassArgs a) {
 // X = u / max(|u|, eps) as two planes of fp16 (hi + lo), the shorter side first, zeros to multiples of 64; 64 x 64 of it a workgroup. The update is made
 // once more of gradient and momentum: as many bytes as writing and reading it would be.
 // Bound by memory: 8 bytes an element in, 4 out.
-template <class T>
+template <class T, int P>
 __global__ __launch_bounds__(256) void lay_kernel(PassArgs a) {
     Place at;
     if (!place_of(a.w, at)) return;
@@ -141,7 +141,9 @@ __global__ __launch_bounds__(256) void lay_kernel(PassArgs a) {
             for (int e = 0; e < 4; ++e) tile[r + p * 16][(threadIdx.x & 15) * 4 + e] = u[e];
         }
     }
-    double sum = sum_of_wave(static_cast<int>(threadIdx.x) < x.parts ? a.w.sums[x.part_at + threadIdx.x] : 0.0);
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < x.parts; i += 256) sum += a.w.sums[x.part_at + i];
+    sum = sum_of_wave(sum);
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
     __syncthreads();
     sum = (waves[0] + waves[1]) + (waves[2] + waves[3]);
@@ -159,9 +161,9 @@ __global__ __launch_bounds__(256) void lay_kernel(PassArgs a) {
             hi[e] = static_cast<_Float16>(v);
             lo[e] = static_cast<_Float16>(v - static_cast<float>(hi[e]));
         }
-        const int64_t place = static_cast<int64_t>(i0 + i) * x.pad_n + j0 + j;
+        const int64_t place = half_at<P>(i0 + i, j0 + j, x.pad_n);
         *reinterpret_cast<f16x8*>(to + place) = hi;
-        *reinterpret_cast<f16x8*>(to + x.x_plane + place) = lo;
+        *reinterpret_cast<f16x8*>(to + place + second_of<P>(x.x_plane)) = lo;
     }
 }
 
@@ -177,7 +179,8 @@ int launch_momentum(const PassArgs& a, hipStream_t stream) {
     return a.dtype == JABAS_F32 ? launch(momentum_kernel<float>, a, stream) : launch(momentum_kernel<uint16_t>, a, stream);
 }
 int launch_lay(const PassArgs& a, hipStream_t stream) {
-    return a.dtype == JABAS_F32 ? launch(lay_kernel<float>, a, stream) : launch(lay_kernel<uint16_t>, a, stream);
+    if (a.planes == 2) return a.dtype == JABAS_F32 ? launch(lay_kernel<float, 2>, a, stream) : launch(lay_kernel<uint16_t, 2>, a, stream);
+    return a.dtype == JABAS_F32 ? launch(lay_kernel<float, 1>, a, stream) : launch(lay_kernel<uint16_t, 1>, a, stream);
 }
 
 }  // namespace muon
