@@ -170,12 +170,8 @@ struct Core {
         }
     }
 
-    // `more`: the loads of the S - 2 steps behind the one that is waited for are all on their way.
-    static __device__ void arrive(bool more) {
-        constexpr int kBehind = (S - 2) * (kLoadsA + kLoadsB);
-        static_assert(kBehind < 64, "what the counter holds");
-        if (S > 2 && more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(kBehind) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    static __device__ void arrive() {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
 
     // smem: S kStage bytes of LDS. `depth`: a multiple of 64, zeros in the operands beyond what counts. `prepare()` runs while the first
@@ -183,6 +179,7 @@ struct Core {
     // past their reads of smem when this returns.
     template <class Prepare, class Start>
     __device__ void run(const Operand& a, const Operand& b, int m0, int n0, int depth, char* smem, const Prepare& prepare, const Start& start) {
+        if constexpr (S > 2) return run_ahead(a, b, m0, n0, depth, smem, prepare, start);
         Source<TM, TA> sa(a, m0);
         Source<TN, TB> sb(b, n0);
         const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem));
@@ -198,8 +195,85 @@ struct Core {
         const int steps = depth / kStep;        // at least one
         constexpr int kLoads = kLoadsA + kLoadsB;
 #pragma unroll
+        for (int l = 0; l < kLoads; ++l) load(0, l);
+        prepare();
+        arrive();
+        if (steps > 1)
+#pragma unroll
+            for (int l = 0; l < kLoads / 2; ++l) load(1, l);
+#pragma unroll
+        for (int i = 0; i < kI; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float x = start(i, e);
+#pragma unroll
+                for (int j = 0; j < kJ; ++j) acc[i][j][e] = x;
+            }
+        Fragments f[2];
+#pragma unroll
+        for (int r = 0; r < kReads; ++r) read(f[0], smem, 0, r);
+        // One step. `next`: there is another, the second half of whose loads goes between the first products; `after`: there is one more, the
+        // first half of whose loads goes between the last products, behind the barrier that frees its stage.
+        const auto pass = [&](int s, auto next, auto after) {
+            const char* stage = smem + (s & 1) * kStage;
+#pragma unroll
+            for (int kk = 0; kk < kParts; ++kk) {
+                const bool first = kk == 0, last = kk + 1 == kParts;
+                if (last) arrive();
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(f[kk & 1], [&](int t) {
+                    const auto share = [&](int n, int at) { return min(n, at * n * 5 / (4 * kProducts)); };     // done at four fifths of the products
+#pragma unroll
+                    for (int r = share(kReads, t); r < share(kReads, t + 1); ++r) {       // of the next part; behind the last step: read, not used
+                        if (last) read(f[0], smem + ((s + 1) & 1) * kStage, 0, r);
+                        else read(f[(kk + 1) & 1], stage, kk + 1, r);
+                    }
+                    if (first && next())
+#pragma unroll
+                        for (int l = kLoads / 2 + t * (kLoads - kLoads / 2) / kProducts; l < kLoads / 2 + (t + 1) * (kLoads - kLoads / 2) / kProducts; ++l) load((s + 1) & 1, l);
+                    if (last && after())
+#pragma unroll
+                        for (int l = t * (kLoads / 2) / kProducts; l < (t + 1) * (kLoads / 2) / kProducts; ++l) load(s & 1, l);
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+            }
+        };
+        const auto yes = [] { return true; };
+        const auto no = [] { return false; };
+        int s = 0;
+        for (; s + 2 < steps; ++s) pass(s, yes, yes);
+        if (s + 1 < steps) pass(s++, yes, no);
+        pass(s, no, no);
+    }
+
+private:
+    // The same with more than two stages: step s lies in stage s % S, and the loads of step s + S - 1 are the last on their way while it is multiplied.
+    template <class Prepare, class Start>
+    __device__ void run_ahead(const Operand& a, const Operand& b, int m0, int n0, int depth, char* smem, const Prepare& prepare, const Start& start) {
+        Source<TM, TA> sa(a, m0);
+        Source<TN, TB> sb(b, n0);
+        const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem));
+        constexpr int kLoads = kLoadsA + kLoadsB;
+        const auto load = [&](int stage, int l) {
+            const uint32_t to = lds + stage * kStage;
+            if (l < kLoadsA) sa.issue(to, l);
+            else sb.issue(to + kBytesA, l - kLoadsA);
+            if (l == kLoads - 1) {
+                sa.advance();
+                sb.advance();
+            }
+        };
+        // Waits for a step; `more`: the S - 2 steps behind it are all on their way.
+        const auto arrive = [](bool more) {
+            constexpr int kBehind = (S - 2) * kLoads;
+            static_assert(kBehind < 64, "what the counter holds");
+            if (more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(kBehind) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        };
+        const int steps = depth / kStep;        // at least one
+#pragma unroll
         for (int p = 0; p < S - 1; ++p)
-            if (p == 0 || p < steps)
+            if (p < steps)
 #pragma unroll
                 for (int l = 0; l < kLoads; ++l) load(p, l);
         prepare();
@@ -218,7 +292,7 @@ struct Core {
         Fragments f[2];
 #pragma unroll
         for (int r = 0; r < kReads; ++r) read(f[0], smem, 0, r);
-        // One step, s, in stage `at`. `next`: there is a step s + S - 1, the second half of whose loads goes between the first products; `after`: there is
+        // One step, in stage `at`. `next`: there is a step S - 1 further on, the second half of whose loads goes between the first products; `after`: there is
         // one more, the first half of whose loads goes between the last products, behind the barrier that frees this stage.
         int at = 0;
         const auto pass = [&](auto next, auto after) {
@@ -230,9 +304,9 @@ struct Core {
                 if (last) arrive(next());
                 __builtin_amdgcn_sched_barrier(0);
                 multiply(f[kk & 1], [&](int t) {
-                    const auto share = [&](int n, int at) { return min(n, at * n * 5 / (4 * kProducts)); };     // done at four fifths of the products
+                    const auto share = [&](int n, int at) { return min(n, at * n * 5 / (4 * kProducts)); };
 #pragma unroll
-                    for (int r = share(kReads, t); r < share(kReads, t + 1); ++r) {       // of the next part; behind the last step: read, not used
+                    for (int r = share(kReads, t); r < share(kReads, t + 1); ++r) {
                         if (last) read(f[0], smem + following * kStage, 0, r);
                         else read(f[(kk + 1) & 1], stage, kk + 1, r);
                     }
