@@ -137,27 +137,34 @@ enum { kMomentum, kLayOut, kSymmetric, kUpdate, kKinds };
 struct Run {
     Work work[kKinds];
     Kind symmetric, update;
+    int tiny;                       // blocks of tiny_fits, or 0
     int planes, dtype, nesterov;
     float momentum, fresh;
     const float* grad_scale;
 };
 int run(const Run& r, const JabasNewtonSchulz& ns, const Scales& s, UpdateArgs& last, hipStream_t stream) {
     PassArgs pass{r.work[kMomentum], r.dtype, r.nesterov, r.momentum, r.fresh, r.grad_scale, ns.eps, static_cast<float>(s.x[0]), r.planes};
+    TinyStep steps[JABAS_MUON_MAX_STEPS];
+    for (int k = 0; k < ns.steps; ++k)
+        steps[k] = {static_cast<float>(s.a[k] / s.x[k] / s.x[k]), static_cast<float>(ns.b * s.b[k] / s.a[k]), static_cast<float>(ns.c * s.b[k] / s.a[k] / s.a[k]),
+                    static_cast<float>(ns.a * s.x[k + 1] / s.x[k]), static_cast<float>(s.x[k + 1] / s.b[k] / s.x[k])};
+    if (r.tiny) {
+        TinyArgs all{pass, last.out, ns.steps, {}};
+        std::copy(steps, steps + ns.steps, all.step);
+        return launch_tiny(all, r.tiny, stream);
+    }
     int status = launch_momentum(pass, stream);
     if (status != JABAS_OK) return status;
     pass.w = r.work[kLayOut];
     if ((status = launch_lay(pass, stream)) != JABAS_OK) return status;
     for (int k = 0; k < ns.steps; ++k) {
-        SymmetricArgs first{r.work[kSymmetric], k & 1, 0.0f, static_cast<float>(s.a[k] / s.x[k] / s.x[k])};
-        if ((status = launch_symmetric(first, false, r.planes, r.symmetric, stream)) != JABAS_OK) return status;
-        first.own = static_cast<float>(ns.b * s.b[k] / s.a[k]);
-        first.product = static_cast<float>(ns.c * s.b[k] / s.a[k] / s.a[k]);
-        if ((status = launch_symmetric(first, true, r.planes, r.symmetric, stream)) != JABAS_OK) return status;
+        if ((status = launch_symmetric({r.work[kSymmetric], k & 1, 0.0f, steps[k].first}, false, r.planes, r.symmetric, stream)) != JABAS_OK) return status;
+        if ((status = launch_symmetric({r.work[kSymmetric], k & 1, steps[k].second_own, steps[k].second}, true, r.planes, r.symmetric, stream)) != JABAS_OK) return status;
         last.w = r.work[kUpdate];
         last.from = k & 1;
         last.last = k + 1 == ns.steps;
-        last.own = static_cast<float>(ns.a * s.x[k + 1] / s.x[k]);
-        last.product = static_cast<float>(s.x[k + 1] / s.b[k] / s.x[k]);
+        last.own = steps[k].update_own;
+        last.product = steps[k].update;
         if ((status = launch_update(last, r.planes, r.update, stream)) != JABAS_OK) return status;
     }
     return JABAS_OK;
@@ -168,9 +175,11 @@ int run(const Run& r, const JabasNewtonSchulz& ns, const Scales& s, UpdateArgs& 
 // Matrices that go through the workspace together: as many as 256 MiB hold, what the chip's last cache holds between the products.
 constexpr int64_t kTogether = int64_t{256} << 20;
 
+inline int blocks_of(const Matrix& x) { return (x.m + 31) / 32; }
+
 struct Batch {
     Matrix x;
-    int planes;
+    int planes, tiny;
     int64_t at_once, sums_bytes, bytes;
 };
 int describe_batch(const JabasOrthogonalize* o, Batch& b, Scales& s) {
@@ -197,6 +206,11 @@ int describe_batch(const JabasOrthogonalize* o, Batch& b, Scales& s) {
     const size_t quad = 4 * size;
     b.x.src_quads = !misaligned(o->in, quad) && o->in_row_stride % 4 == 0 && (o->batch == 1 || o->in_batch_stride % 4 == 0);
     b.x.out_quads = !misaligned(o->out, quad) && o->cols % 4 == 0;
+    b.tiny = tiny_fits(blocks_of(b.x), b.x.n) ? blocks_of(b.x) : 0;
+    if (b.tiny) {
+        b.at_once = std::min(o->batch, kMaxSlots / 2);
+        return JABAS_OK;
+    }
     const int64_t each = halves_of(b.x, b.planes);
     // launches count their workgroups in 32 bits
     const int64_t most = kMaxSlots / std::max({lay_tiles(b.x), static_cast<int64_t>(b.x.parts), update_tiles(b.x.m, b.x.n, 64), symmetric_tiles(b.x.m, 64)});
@@ -219,7 +233,7 @@ struct Part {
 };
 struct Header {
     uint32_t magic, n, n_parts, n_groups;
-    int32_t precision, reserved;
+    int32_t precision, tiny;
     uint64_t bytes, matrices_at, fanout_at, parts_at, sums_bytes, workspace;
 };
 
@@ -316,10 +330,22 @@ int build(const JabasMatrix* list, uint32_t n, int32_t precision, Built& b) {
         for (uint32_t f = 0; f < j.n_fanout; ++f) b.fanout.push_back(reinterpret_cast<uint64_t>(j.fanout[f]));
         b.matrices.push_back(x);
     }
+    // the matrices come with the longest shorter side first
+    const int blocks = blocks_of(b.matrices[0]);
+    bool tiny = n <= kMaxSlots / 2;
+    for (const Matrix& x : b.matrices) tiny = tiny && tiny_fits(blocks, x.n);
+    b.head.tiny = tiny ? blocks : 0;
     uint64_t halves_most = 0, sums_most = 0;
     int64_t left = 0;
     for (const Matrix& x : b.matrices) left += halves_of(x, planes);
     for (uint32_t first = 0; first < n;) {
+        if (tiny) {
+            Part p{};
+            deal(b.slots, std::vector<int64_t>(n, 1), 0);
+            p.total[kMomentum] = n;
+            b.parts.push_back(p);
+            break;
+        }
         // parts of about one size: a small last one would leave CUs idle
         const int64_t share = left / ((2 * left + kTogether - 1) / kTogether);
         int64_t halves = 0, sums = 0, slots[kKinds] = {0, 0, 0, 0};
@@ -379,7 +405,7 @@ int build(const JabasMatrix* list, uint32_t n, int32_t precision, Built& b) {
         for (uint64_t& at : p.slots_at) at = slots_at + at * sizeof(Slot);
     h.bytes = round_up(slots_at + b.slots.size() * sizeof(Slot), 16);
     h.sums_bytes = round_up(8 * sums_most, 256);
-    h.workspace = h.sums_bytes + round_up(2 * halves_most, 256);
+    h.workspace = std::max<uint64_t>(256, h.sums_bytes + round_up(2 * halves_most, 256));
     return JABAS_OK;
 }
 
@@ -429,6 +455,7 @@ JABAS_API int jabas_orthogonalize(const JabasOrthogonalize* o, void* workspace, 
         r.update = update.best();
         r.planes = b.planes;
         r.dtype = o->dtype;
+        r.tiny = b.tiny;
         Work w{};
         w.one = x;
         w.one.src = static_cast<const char*>(o->in) + size * done * o->in_batch_stride;
@@ -440,15 +467,15 @@ JABAS_API int jabas_orthogonalize(const JabasOrthogonalize* o, void* workspace, 
         w.a_step = each - w.x_step;
         w.part_step = x.parts;
         w.sums = static_cast<double*>(workspace);
-        w.halves = static_cast<char*>(workspace) + b.sums_bytes;
-        const int64_t per[kKinds] = {x.parts, lay_tiles(x), symmetric_tiles(x.m, kTile[r.symmetric]), update_tiles(x.m, x.n, kTile[r.update])};
+        w.halves = static_cast<char*>(workspace) + (b.tiny ? 0 : b.sums_bytes);
+        const int64_t per[kKinds] = {b.tiny ? 1 : x.parts, lay_tiles(x), symmetric_tiles(x.m, kTile[r.symmetric]), update_tiles(x.m, x.n, kTile[r.update])};
         for (int k = 0; k < kKinds; ++k) {
             r.work[k] = w;
             r.work[k].per = static_cast<int32_t>(per[k]);
             r.work[k].total = static_cast<uint32_t>(per[k] * here);
         }
         UpdateArgs last{};
-        last.out_dtype = o->dtype;
+        last.out.dtype = o->dtype;
         const int launched = run(r, o->ns, s, last, static_cast<hipStream_t>(stream));
         if (launched != JABAS_OK) return launched;
     }
@@ -510,13 +537,14 @@ JABAS_API int jabas_muon_step(const void* plan_host, const void* plan_dev, const
     w.halves = static_cast<char*>(workspace) + h->sums_bytes;
     UpdateArgs last{};
     for (int g = 0; g < args->n_groups; ++g) {
-        last.lr[g] = static_cast<float>(args->lr[g]);
-        last.keep[g] = static_cast<float>(1.0 - args->lr[g] * args->weight_decay[g]);
+        last.out.lr[g] = static_cast<float>(args->lr[g]);
+        last.out.keep[g] = static_cast<float>(1.0 - args->lr[g] * args->weight_decay[g]);
     }
     for (uint32_t p = 0; p < h->n_parts; ++p) {
         Run r{};
         r.symmetric = static_cast<Kind>(parts[p].symmetric);
         r.update = static_cast<Kind>(parts[p].update);
+        r.tiny = h->tiny;
         r.planes = h->precision == JABAS_F32 ? 2 : 1;
         r.dtype = JABAS_F32;
         r.nesterov = args->nesterov != 0;

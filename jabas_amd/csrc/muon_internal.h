@@ -79,20 +79,38 @@ struct SymmetricArgs {
     int32_t from;                   // buffer of X
     float own, product;             // result = own A + product acc
 };
+// The last step's result: into the weights (lr by group, keep = 1 - lr weight_decay), or as it is, of `dtype`.
+struct Out {
+    int32_t dtype;
+    float lr[JABAS_MAX_GROUPS], keep[JABAS_MAX_GROUPS];
+};
 // X <- a X + B X
 struct UpdateArgs {
     Work w;
     int32_t from;
     int32_t last;                   // goes to out, scaled by 1
-    int32_t out_dtype;              // without weights
     float own, product;
-    float lr[JABAS_MAX_GROUPS], keep[JABAS_MAX_GROUPS];     // keep = 1 - lr weight_decay
+    Out out;
 };
 // The products' kernels: their tiles and what tells them apart.
 enum Kind { kSmall, kSmallMany, kMiddle, kMiddleDeep, kLarge, kKernels };     // 64, four stages or two; 128, two stages or four; 256
 constexpr int kTile[kKernels] = {64, 64, 128, 128, 256};
 int launch_symmetric(const SymmetricArgs& a, bool second, int planes, Kind kind, hipStream_t stream);
 int launch_update(const UpdateArgs& a, int planes, Kind kind, hipStream_t stream);
+
+// Everything of small matrices in one launch, one workgroup each. `blocks` of 32 cover the shorter side of all of them.
+constexpr int kTinyBytes = 160 * 1024 - 256;        // of LDS
+struct TinyStep {
+    float first, second_own, second, update_own, update;
+};
+struct TinyArgs {
+    PassArgs pass;
+    Out out;
+    int32_t steps;
+    TinyStep step[JABAS_MUON_MAX_STEPS];
+};
+bool tiny_fits(int blocks, int64_t n);
+int launch_tiny(const TinyArgs& a, int blocks, hipStream_t stream);
 
 inline int64_t symmetric_tiles(int64_t m, int tile) { const int64_t t = (m + tile - 1) / tile; return t * (t + 1) / 2; }
 inline int64_t update_tiles(int64_t m, int64_t n, int tile) { return (m + tile - 1) / tile * ((n + tile - 1) / tile); }

@@ -3,6 +3,7 @@
 
 #include "loss_core.h"
 #include "muon_internal.h"
+#include "muon_put.h"
 #include "muon_work.h"
 
 namespace jabas {
@@ -14,12 +15,6 @@ using loss::F16;
 using loss::Operand;
 using loss::f16x8;
 using loss::f32x4;
-
-__device__ inline uint16_t to_bf16(float x) {
-    const uint32_t u = __float_as_uint(x);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return static_cast<uint16_t>((u >> 16) | 0x40);
-    return static_cast<uint16_t>((u + 0x7fffu + ((u >> 16) & 1)) >> 16);
-}
 
 // Eight values and their planes.
 template <int P>
@@ -336,58 +331,6 @@ __global__ __launch_bounds__(256) void symmetric_deep_kernel(SymmetricArgs a) {
     }
 }
 
-// Where a step's last product goes: `count` (up to V) results of consecutive columns of a row of the matrix as the caller has it.
-template <int V>
-__device__ inline void put_out(const UpdateArgs& a, const Matrix& x, int row, int col, const float* v) {
-    const int64_t place = static_cast<int64_t>(row) * x.cols + col;
-    const int count = min(V, x.cols - col);
-    if (!x.momentum) {
-        if (a.out_dtype == JABAS_F32) {
-            float* out = static_cast<float*>(x.out) + place;
-            if (x.out_quads)
-#pragma unroll
-                for (int e = 0; e < V; e += 4) { if (e < count) *reinterpret_cast<f32x4*>(out + e) = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]}; }
-            else
-#pragma unroll
-                for (int e = 0; e < V; ++e) { if (e < count) out[e] = v[e]; }
-        } else {
-            uint16_t* out = static_cast<uint16_t*>(x.out) + place;
-            if (x.out_quads)
-#pragma unroll
-                for (int e = 0; e < V; e += 4) {
-                    if (e < count)
-                        *reinterpret_cast<uint2*>(out + e) = make_uint2(to_bf16(v[e]) | static_cast<uint32_t>(to_bf16(v[e + 1])) << 16,
-                                                                        to_bf16(v[e + 2]) | static_cast<uint32_t>(to_bf16(v[e + 3])) << 16);
-                }
-            else
-#pragma unroll
-                for (int e = 0; e < V; ++e) { if (e < count) out[e] = to_bf16(v[e]); }
-        }
-        return;
-    }
-    const float lr = a.lr[x.group] * x.lr_factor, keep = a.keep[x.group];
-    float* w = static_cast<float*>(x.out) + place;
-    if (x.out_quads) {
-#pragma unroll
-        for (int e = 0; e < V; e += 4) {
-            if (e >= count) continue;
-            f32x4 now = *reinterpret_cast<const f32x4*>(w + e);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) now[i] = fmaf(-lr, v[e + i], now[i] * keep);
-            *reinterpret_cast<f32x4*>(w + e) = now;
-            for (uint32_t f = 0; f < x.n_fanout; ++f) *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(a.w.fanout[x.fanout_at + f]) + place + e) = now;
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            if (e >= count) continue;
-            const float now = fmaf(-lr, v[e], w[e] * keep);
-            w[e] = now;
-            for (uint32_t f = 0; f < x.n_fanout; ++f) reinterpret_cast<float*>(a.w.fanout[x.fanout_at + f])[place + e] = now;
-        }
-    }
-}
-
 // Tile `tile` of across x down, in bands of eight of m, so that tiles in flight together share their operands' rows.
 __device__ inline void band(uint32_t tile, int across, int down, int& tm, int& tn) {
     const int which = static_cast<int>(tile / (8u * down)), first = which * 8, height = min(8, across - first), in = static_cast<int>(tile - which * 8u * down);
@@ -457,7 +400,7 @@ __global__ __launch_bounds__(C::kThreads) void update_kernel(UpdateArgs a) {
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = staged.at(r + e, col);
-                put_out<4>(a, x, row, m, v);
+                put_out<4>(a.out, a.w.fanout, x, row, m, v);
             }
         } else {
 #pragma unroll 1
@@ -466,7 +409,7 @@ __global__ __launch_bounds__(C::kThreads) void update_kernel(UpdateArgs a) {
                 if (row >= x.rows || m >= x.cols) continue;
                 Eight v;
                 staged.get(r, col, v);
-                put_out<8>(a, x, row, m, v.v);
+                put_out<8>(a.out, a.w.fanout, x, row, m, v.v);
             }
         }
     }
@@ -509,7 +452,7 @@ __global__ __launch_bounds__(256) void update_deep_kernel(UpdateArgs a) {
         else if (x.tall)
 #pragma unroll
             for (int e = 0; e < 8; ++e) sums[r * D::kRow + D::col() + e] = v.v[e];
-        else if (row < x.m && m < x.n) put_out<8>(a, x, row, m, v.v);
+        else if (row < x.m && m < x.n) put_out<8>(a.out, a.w.fanout, x, row, m, v.v);
     }
     if (!a.last || !x.tall) return;
     __syncthreads();
@@ -520,7 +463,7 @@ __global__ __launch_bounds__(256) void update_deep_kernel(UpdateArgs a) {
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = sums[(r + e) * D::kRow + col];
-        put_out<8>(a, x, row, m, v);
+        put_out<8>(a.out, a.w.fanout, x, row, m, v);
     }
 }
 

@@ -10,36 +10,12 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 template <class T>
-__device__ inline float element(const T* p, int64_t i) {
-    if constexpr (sizeof(T) == 4) return p[i];
-    else return __uint_as_float(static_cast<uint32_t>(p[i]) << 16);
-}
-template <class T>
 __device__ inline f32x4 quad(const T* p, int64_t i) {
     if constexpr (sizeof(T) == 4) return *reinterpret_cast<const f32x4*>(p + i);
     else {
         const uint2 v = *reinterpret_cast<const uint2*>(p + i);
         return f32x4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u)};
     }
-}
-
-struct Mix {
-    float momentum, fresh, scale;
-    int nesterov;
-    __device__ explicit Mix(const PassArgs& a) : momentum(a.momentum), fresh(a.fresh), scale(1.0f), nesterov(a.nesterov) {
-        if (a.grad_scale) {
-            const float c = *a.grad_scale;
-            if (c < 1.0f) scale = c;        // a NaN is no bound
-        }
-    }
-    __device__ float buffer(float g, float buf) const { return fmaf(fresh, g - buf, buf); }
-    __device__ float update(float g, float buf) const { return nesterov ? fmaf(momentum, buf - g, g) : buf; }
-};
-
-__device__ inline double sum_of_wave(double x) {
-#pragma unroll
-    for (int i = 32; i; i >>= 1) x += __shfl_xor(x, i);
-    return x;
 }
 
 // buf' = buf + (1 - momentum) (g - buf), written, and the sum of squares of what is to be orthogonalised, in 64 bits: in 32 a matrix of 10^7

@@ -1,4 +1,4 @@
-// What a workgroup of the orthogonalised update works on.
+// What a workgroup of the orthogonalised update works on, and what it makes of a gradient.
 #pragma once
 
 #include "muon_internal.h"
@@ -32,6 +32,31 @@ __device__ inline bool place_of(const Work& w, Place& at) {
     at.x.a_at += i * w.a_step;
     at.x.part_at += i * w.part_step;
     return true;
+}
+
+template <class T>
+__device__ inline float element(const T* p, int64_t i) {
+    if constexpr (sizeof(T) == 4) return p[i];
+    else return __uint_as_float(static_cast<uint32_t>(p[i]) << 16);
+}
+// Momentum and update of an element.
+struct Mix {
+    float momentum, fresh, scale;
+    int nesterov;
+    __device__ explicit Mix(const PassArgs& a) : momentum(a.momentum), fresh(a.fresh), scale(1.0f), nesterov(a.nesterov) {
+        if (a.grad_scale) {
+            const float c = *a.grad_scale;
+            if (c < 1.0f) scale = c;        // a NaN is no bound
+        }
+    }
+    __device__ float buffer(float g, float buf) const { return fmaf(fresh, g - buf, buf); }
+    __device__ float update(float g, float buf) const { return nesterov ? fmaf(momentum, buf - g, g) : buf; }
+};
+
+__device__ inline double sum_of_wave(double x) {
+#pragma unroll
+    for (int i = 32; i; i >>= 1) x += __shfl_xor(x, i);
+    return x;
 }
 
 }  // namespace muon
