@@ -3,6 +3,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <map>
 #include <new>
 #include <numeric>
 #include <vector>
@@ -83,9 +84,9 @@ void describe(Matrix& x, int64_t rows, int64_t cols) {
 int64_t halves_of(const Matrix& x, int planes) { return 4 * x.x_plane + 2 * planes * x.a_plane; }
 int64_t lay_tiles(const Matrix& x) { return static_cast<int64_t>(x.pad_m / kLay) * (x.pad_n / kLay); }
 
-// Which kernel the products of some matrices take: the one whose time, by what was measured, is least. `each` workgroups of a kernel share a CU; a round of
-// them takes `start` us and `step` us for 64 of the inner axis, `alone` where the launch leaves most CUs with one or none. Measured, us, X X^T and then
-// a X + B X, for kSmall, kSmallMany, kMiddle, kMiddleDeep, kLarge (fp32; bf16 next):
+// Which kernel a product of some matrices takes: the one that ends first by what was measured. `each` workgroups of a kernel share a CU; a tile takes `start`
+// us and, for 64 of the inner axis, `first` us in X X^T and A A or `update` us in a X + B X with the chip full, `alone` with most CUs idle. Measured, us,
+// X X^T and then a X + B X, for kSmall, kSmallMany, kMiddle, kMiddleDeep, kLarge (fp32; bf16 next):
 //   12 x  768 x  768   31 32 32 25 54    53 53 44 44 61     18 18 20 18 29    32 28 25 30 31
 //    6 x 1024 x 4096  105 109 110 84 233  203 180 151 168 170   52 52 49 39 84   114 96 75 94 80
 //        1024 x 4096   32 58 92 60 217    37 36 35 30 71     18 33 43 29 79    23 20 20 18 32
@@ -95,48 +96,88 @@ int64_t lay_tiles(const Matrix& x) { return static_cast<int64_t>(x.pad_m / kLay)
 //    4 x  384 x  384    8 10 14 13 31      8 9 15 13 32       6 7 11 11 19     7 7 11 10 19
 struct Cost {
     int each;
-    double start, alone, step;
+    double start, alone, symmetric, update;
 };
-constexpr Cost kCosts[2][kKernels] = {{{2, 3.0, 0.20, 0.40}, {4, 3.5, 0.50, 0.75}, {2, 7.0, 0.62, 1.00}, {1, 6.0, 0.38, 0.53}, {1, 12.0, 1.25, 1.75}},
-                                      {{2, 3.0, 0.45, 0.82}, {4, 3.5, 0.90, 1.60}, {2, 8.0, 1.35, 2.65}, {1, 6.0, 0.95, 1.30}, {1, 12.0, 3.40, 4.80}}};
-constexpr double kMostCus = 160.0, kCus = 256.0;
-struct Load {
-    int planes;
-    double tiles[kKernels] = {}, sum[kKernels] = {}, longest[kKernels] = {};
-    explicit Load(int planes) : planes(planes) {}
-    void add(int kind, double count, double steps, int products) {
-        const Cost& c = kCosts[planes - 1][kind];
-        tiles[kind] += count;
-        sum[kind] += count * (products * c.start + steps * c.step);
-        longest[kind] = std::max(longest[kind], products * c.start + steps * c.alone);
-    }
-    Kind best() const {
-        int at = 0;
-        double least = 0.0;
-        for (int k = 0; k < kKernels; ++k) {
-            const double here = kCus * kCosts[planes - 1][k].each;
-            const double time = tiles[k] <= kMostCus ? longest[k] : std::max(longest[k], ceil(tiles[k] / here) * sum[k] / tiles[k]);
-            if (k == 0 || time < least) {
-                least = time;
-                at = k;
+constexpr Cost kCosts[2][kKernels] = {
+    {{2, 2.5, 0.20, 0.38, 0.46}, {4, 4.0, 0.50, 0.75, 0.75}, {2, 7.0, 0.62, 0.90, 1.00}, {1, 5.0, 0.38, 0.53, 0.60}, {1, 13.0, 1.25, 1.75, 1.75}},
+    {{2, 3.5, 0.45, 0.76, 0.95}, {4, 4.5, 0.90, 1.60, 1.60}, {2, 8.0, 1.35, 2.60, 2.65}, {1, 6.0, 0.95, 1.15, 1.35}, {1, 18.0, 3.40, 4.75, 4.75}}};
+constexpr int64_t kCus = 256, kFew = 160;
+constexpr double kLaunch = 4.0;                 // us of a launch, beside its tiles
+
+enum Product { kFirst, kSecond, kUpdate, kProducts };
+struct Shape {
+    int32_t m, n, pad_m, pad_n;
+    int64_t count;
+    Shape(const Matrix& x, int64_t count) : m(x.m), n(x.n), pad_m(x.pad_m), pad_n(x.pad_n), count(count) {}
+    int64_t tiles(Product p, Kind k) const { return p == kUpdate ? update_tiles(m, n, kTile[k]) : symmetric_tiles(m, kTile[k]); }
+    double steps(Product p) const { return (p == kFirst ? pad_n : pad_m) / 64.0; }
+};
+
+// When `slots` workgroups are done with tiles of given lengths, longest first, each taken by whoever is free first.
+struct Tiles {
+    double length;
+    int64_t count;
+};
+double makespan(std::vector<Tiles> work, int64_t slots) {
+    std::sort(work.begin(), work.end(), [](const Tiles& a, const Tiles& b) { return a.length > b.length; });
+    std::map<double, int64_t> free_at{{0.0, slots}};
+    double end = 0.0;
+    for (Tiles& w : work)
+        while (w.count > 0) {
+            const auto next = free_at.begin();
+            if (free_at.size() == 1 && w.count >= 4 * slots) {         // whole rounds
+                const int64_t rounds = w.count / slots - 1;
+                const double until = next->first + rounds * w.length;
+                w.count -= rounds * slots;
+                free_at = {{until, slots}};
+                end = std::max(end, until);
+                continue;
             }
+            const int64_t take = std::min(w.count, next->second);
+            const double until = next->first + w.length;
+            w.count -= take;
+            end = std::max(end, until);
+            if ((next->second -= take) == 0) free_at.erase(next);
+            free_at[until] += take;
         }
-        return static_cast<Kind>(at);
-    }
-};
-void add_symmetric(Load& l, const Matrix& x, double count) {
-    for (int k = 0; k < kKernels; ++k) l.add(k, count * symmetric_tiles(x.m, kTile[k]), (x.pad_n + x.pad_m) / 64.0, 2);
-}
-void add_update(Load& l, const Matrix& x, double count) {
-    for (int k = 0; k < kKernels; ++k) l.add(k, count * update_tiles(x.m, x.n, kTile[k]), x.pad_m / 64.0, 1);
+    return end;
 }
 
-enum { kMomentum, kLayOut, kSymmetric, kUpdate, kKinds };
+double time_of(const Shape* shapes, size_t n, Product p, Kind k, int planes) {
+    const Cost& c = kCosts[planes - 1][k];
+    int64_t total = 0;
+    for (size_t i = 0; i < n; ++i) total += shapes[i].count * shapes[i].tiles(p, k);
+    const double step = total <= kFew ? c.alone : p == kUpdate ? c.update : c.symmetric;
+    if (n == 1) return kLaunch + (total + kCus * c.each - 1) / (kCus * c.each) * (c.start + shapes[0].steps(p) * step);
+    std::vector<Tiles> work;
+    for (size_t i = 0; i < n; ++i) work.push_back({c.start + shapes[i].steps(p) * step, shapes[i].count * shapes[i].tiles(p, k)});
+    return kLaunch + makespan(work, kCus * c.each);
+}
+Kind kernel_of(const Shape* shapes, size_t n, Product p, int planes, double* time = nullptr) {
+    int at = 0;
+    double least = 0.0;
+    for (int k = 0; k < kKernels; ++k) {
+        const double here = time_of(shapes, n, p, static_cast<Kind>(k), planes);
+        if (k == 0 || here < least) {
+            least = here;
+            at = k;
+        }
+    }
+    if (time) *time += least;
+    return static_cast<Kind>(at);
+}
+double step_of(const Shape* shapes, size_t n, int planes) {
+    double time = 0.0;
+    for (int p = 0; p < kProducts; ++p) kernel_of(shapes, n, static_cast<Product>(p), planes, &time);
+    return time;
+}
+
+enum { kMomentum = kProducts, kLayOut, kKinds };        // launches of their own beside the products
 
 // The launches of some matrices that share a workspace.
 struct Run {
     Work work[kKinds];
-    Kind symmetric, update;
+    Kind kernel[kProducts];
     int tiny;                       // blocks of tiny_fits, or 0
     int planes, dtype, nesterov;
     float momentum, fresh;
@@ -158,22 +199,24 @@ int run(const Run& r, const JabasNewtonSchulz& ns, const Scales& s, UpdateArgs& 
     pass.w = r.work[kLayOut];
     if ((status = launch_lay(pass, stream)) != JABAS_OK) return status;
     for (int k = 0; k < ns.steps; ++k) {
-        if ((status = launch_symmetric({r.work[kSymmetric], k & 1, 0.0f, steps[k].first}, false, r.planes, r.symmetric, stream)) != JABAS_OK) return status;
-        if ((status = launch_symmetric({r.work[kSymmetric], k & 1, steps[k].second_own, steps[k].second}, true, r.planes, r.symmetric, stream)) != JABAS_OK) return status;
+        if ((status = launch_symmetric({r.work[kFirst], k & 1, 0.0f, steps[k].first}, false, r.planes, r.kernel[kFirst], stream)) != JABAS_OK) return status;
+        if ((status = launch_symmetric({r.work[kSecond], k & 1, steps[k].second_own, steps[k].second}, true, r.planes, r.kernel[kSecond], stream)) != JABAS_OK) return status;
         last.w = r.work[kUpdate];
         last.from = k & 1;
         last.last = k + 1 == ns.steps;
         last.own = steps[k].update_own;
         last.product = steps[k].update;
-        if ((status = launch_update(last, r.planes, r.update, stream)) != JABAS_OK) return status;
+        if ((status = launch_update(last, r.planes, r.kernel[kUpdate], stream)) != JABAS_OK) return status;
     }
     return JABAS_OK;
 }
 
 // ---- a batch of one shape
 
-// Matrices that go through the workspace together: as many as 256 MiB hold, what the chip's last cache holds between the products.
-constexpr int64_t kTogether = int64_t{256} << 20;
+// Matrices that go through the workspace together take at most this, or are one. How many do is what ends first by the costs above: the last tiles of a launch
+// leave CUs idle, and a launch has its own time.
+constexpr int64_t kTogether = int64_t{512} << 20;
+constexpr int64_t kTurns = 16;          // ways of cutting that are tried
 
 inline int blocks_of(const Matrix& x) { return (x.m + 31) / 32; }
 
@@ -218,8 +261,20 @@ int describe_batch(const JabasOrthogonalize* o, Batch& b, Scales& s) {
     b.at_once = std::min({o->batch, std::max<int64_t>(1, kTogether / (2 * each)), most});
     b.sums_bytes = round_up(8 * b.at_once * b.x.parts, 256);
     b.bytes = b.sums_bytes + round_up(2 * b.at_once * each, 256);
-    const int64_t turns = (o->batch + b.at_once - 1) / b.at_once;
-    b.at_once = (o->batch + turns - 1) / turns;         // turns of one size: a short last one would leave CUs idle
+    const int64_t least = (o->batch + b.at_once - 1) / b.at_once;
+    double best = 0.0;
+    for (int64_t turns = least; o->batch > 1 && turns < least + kTurns && turns <= o->batch; ++turns) {
+        const int64_t here = (o->batch + turns - 1) / turns;        // turns of one size: a short last one would leave CUs idle
+        const int64_t whole = o->batch / here, rest = o->batch - whole * here;
+        const Shape both[2] = {Shape(b.x, here), Shape(b.x, rest)};
+        double time = whole * step_of(both, 1, b.planes);
+        if (rest) time += step_of(both + 1, 1, b.planes);
+        if (turns == least || time < best) {
+            best = time;
+            b.at_once = here;
+        }
+        if (here == 1) break;
+    }
     return JABAS_OK;
 }
 
@@ -229,7 +284,8 @@ constexpr uint32_t kMagic = 0x4d4e5331;
 struct Part {
     uint64_t slots_at[kKinds];
     uint32_t total[kKinds];
-    int32_t symmetric, update;      // kernels of the products
+    int32_t kernel[kProducts];
+    int32_t reserved;
 };
 struct Header {
     uint32_t magic, n, n_parts, n_groups;
@@ -267,23 +323,79 @@ int check_matrix(const JabasMatrix& j) {
     return JABAS_OK;
 }
 
-// Slots of one kind for matrices [first, last): each matrix's tiles are dealt out to the eight dies in runs, dies in turn where a matrix has fewer than
-// eight, and die d has slots d, d + 8, ... . The matrices come with the longest tiles first.
-void deal(std::vector<Slot>& out, const std::vector<int64_t>& tiles, uint32_t first) {
+// Slots of one launch: every matrix's tiles are dealt out to the eight dies in runs, dies in turn where a matrix has fewer than eight, and die d has slots
+// d, d + 8, ... . `work`: matrices and their tiles, the longest first.
+struct Dealt {
+    uint32_t matrix;
+    int64_t tiles;
+};
+void deal(std::vector<Slot>& out, const std::vector<Dealt>& work) {
     std::vector<Slot> die[8];
     int turn = 0;
-    for (size_t i = 0; i < tiles.size(); ++i) {
-        const int64_t each = tiles[i] / 8, left = tiles[i] % 8;
+    int64_t total = 0;
+    for (const Dealt& w : work) {
+        const int64_t each = w.tiles / 8, left = w.tiles % 8;
         uint32_t at = 0;
         for (int d = 0; d < 8; ++d) {
             const int64_t here = each + (d < left);
-            for (int64_t t = 0; t < here; ++t) die[(turn + d) & 7].push_back({first + static_cast<uint32_t>(i), at++});
+            for (int64_t t = 0; t < here; ++t) die[(turn + d) & 7].push_back({w.matrix, at++});
         }
         turn = (turn + static_cast<int>(left)) & 7;
+        total += w.tiles;
     }
     // `turn` keeps the dies within one slot of each other, those from 0 on the longer ones
-    const int64_t total = std::accumulate(tiles.begin(), tiles.end(), int64_t{0});
     for (int64_t s = 0; s < total; ++s) out.push_back(die[s & 7][s >> 3]);
+}
+
+std::vector<Shape> shapes_of(const std::vector<Matrix>& all, uint32_t first, uint32_t last) {
+    std::vector<Shape> shapes;
+    for (uint32_t i = first; i < last; ++i) {
+        if (!shapes.empty() && shapes.back().m == all[i].m && shapes.back().n == all[i].n) ++shapes.back().count;
+        else shapes.emplace_back(all[i], 1);
+    }
+    return shapes;
+}
+
+// Ends of the parts of a list that go through the workspace one after another, of about one size.
+int cut(const std::vector<Matrix>& all, int planes, std::vector<uint32_t>& ends) {
+    const uint32_t n = static_cast<uint32_t>(all.size());
+    int64_t whole = 0;
+    for (const Matrix& x : all) whole += 2 * halves_of(x, planes);
+    double best = 0.0;
+    const int64_t least = (whole + kTogether - 1) / kTogether;
+    for (int64_t parts = least; parts < least + kTurns && parts <= n; ++parts) {
+        std::vector<uint32_t> here;
+        double time = 0.0;
+        int64_t left = whole;
+        for (uint32_t first = 0; first < n;) {
+            const int64_t share = left / std::max<int64_t>(1, parts - static_cast<int64_t>(here.size()));
+            int64_t bytes = 0, slots[kKinds] = {};
+            uint32_t last = first;
+            for (; last < n; ++last) {
+                const Matrix& x = all[last];
+                const int64_t need = 2 * halves_of(x, planes), tiles = update_tiles(x.m, x.n, 64);
+                const int64_t more[kKinds] = {symmetric_tiles(x.m, 64), symmetric_tiles(x.m, 64), tiles, x.parts, lay_tiles(x)};
+                bool full = last > first && (bytes + need > kTogether || bytes + need / 2 > share);
+                for (int k = 0; k < kKinds; ++k) {
+                    if (more[k] > kMaxSlots) return JABAS_ERR_SIZE;
+                    full = full || (last > first && slots[k] + more[k] > kMaxSlots);
+                }
+                if (full) break;
+                bytes += need;
+                for (int k = 0; k < kKinds; ++k) slots[k] += more[k];
+            }
+            const std::vector<Shape> shapes = shapes_of(all, first, last);
+            time += step_of(shapes.data(), shapes.size(), planes);
+            left -= bytes;
+            here.push_back(last);
+            first = last;
+        }
+        if (ends.empty() || time < best) {
+            best = time;
+            ends = here;
+        }
+    }
+    return JABAS_OK;
 }
 
 struct Built {
@@ -336,61 +448,48 @@ int build(const JabasMatrix* list, uint32_t n, int32_t precision, Built& b) {
     for (const Matrix& x : b.matrices) tiny = tiny && tiny_fits(blocks, x.n);
     b.head.tiny = tiny ? blocks : 0;
     uint64_t halves_most = 0, sums_most = 0;
-    int64_t left = 0;
-    for (const Matrix& x : b.matrices) left += halves_of(x, planes);
-    for (uint32_t first = 0; first < n;) {
-        if (tiny) {
-            Part p{};
-            deal(b.slots, std::vector<int64_t>(n, 1), 0);
-            p.total[kMomentum] = n;
-            b.parts.push_back(p);
-            break;
-        }
-        // parts of about one size: a small last one would leave CUs idle
-        const int64_t share = left / ((2 * left + kTogether - 1) / kTogether);
-        int64_t halves = 0, sums = 0, slots[kKinds] = {0, 0, 0, 0};
-        uint32_t last = first;
-        while (last < n) {
-            Matrix& x = b.matrices[last];
-            const int64_t need = halves_of(x, planes);
-            const int64_t more[kKinds] = {x.parts, lay_tiles(x), symmetric_tiles(x.m, 64), update_tiles(x.m, x.n, 64)};
-            bool full = last > first && (2 * (halves + need) > kTogether || halves + need / 2 > share);
-            for (int k = 0; k < kKinds; ++k) {
-                if (more[k] > kMaxSlots) return JABAS_ERR_SIZE;
-                full = full || (last > first && slots[k] + more[k] > kMaxSlots);
-            }
-            if (full) break;
-            x.x_at = halves;
-            x.a_at = halves + 4 * x.x_plane;
-            x.part_at = sums;
-            halves += need;
-            sums += x.parts;
-            for (int k = 0; k < kKinds; ++k) slots[k] += more[k];
-            ++last;
-        }
-        left -= halves;
-        halves_most = std::max<uint64_t>(halves_most, halves);
-        sums_most = std::max<uint64_t>(sums_most, sums);
-        Load symmetric(planes), update(planes);
-        for (uint32_t i = first; i < last; ++i) {
-            add_symmetric(symmetric, b.matrices[i], 1);
-            add_update(update, b.matrices[i], 1);
-        }
+    if (tiny) {
+        std::vector<Dealt> work;
+        for (uint32_t i = 0; i < n; ++i) work.push_back({i, 1});
         Part p{};
-        p.symmetric = symmetric.best();
-        p.update = update.best();
-        for (int k = 0; k < kKinds; ++k) {
-            std::vector<int64_t> tiles;
-            for (uint32_t i = first; i < last; ++i) {
-                const Matrix& x = b.matrices[i];
-                tiles.push_back(k == kMomentum ? x.parts : k == kLayOut ? lay_tiles(x) : k == kSymmetric ? symmetric_tiles(x.m, kTile[p.symmetric]) : update_tiles(x.m, x.n, kTile[p.update]));
-            }
-            p.slots_at[k] = b.slots.size();
-            deal(b.slots, tiles, first);
-            p.total[k] = static_cast<uint32_t>(b.slots.size() - p.slots_at[k]);
-        }
+        deal(b.slots, work);
+        p.total[kMomentum] = n;
         b.parts.push_back(p);
-        first = last;
+    } else {
+        std::vector<uint32_t> ends;
+        const int status = cut(b.matrices, planes, ends);
+        if (status != JABAS_OK) return status;
+        uint32_t first = 0;
+        for (uint32_t last : ends) {
+            int64_t halves = 0, sums = 0;
+            for (uint32_t i = first; i < last; ++i) {
+                Matrix& x = b.matrices[i];
+                x.x_at = halves;
+                x.a_at = halves + 4 * x.x_plane;
+                x.part_at = sums;
+                halves += halves_of(x, planes);
+                sums += x.parts;
+            }
+            halves_most = std::max<uint64_t>(halves_most, halves);
+            sums_most = std::max<uint64_t>(sums_most, sums);
+            const std::vector<Shape> shapes = shapes_of(b.matrices, first, last);
+            Part p{};
+            for (int k = 0; k < kProducts; ++k) p.kernel[k] = kernel_of(shapes.data(), shapes.size(), static_cast<Product>(k), planes);
+            for (int k = 0; k < kKinds; ++k) {
+                std::vector<Dealt> work;
+                for (uint32_t i = first; i < last; ++i) {
+                    const Matrix& x = b.matrices[i];
+                    work.push_back({i, k == kMomentum ? x.parts : k == kLayOut ? lay_tiles(x) : Shape(x, 1).tiles(static_cast<Product>(k), static_cast<Kind>(p.kernel[k]))});
+                }
+                if (k == kFirst)
+                    std::stable_sort(work.begin(), work.end(), [&](const Dealt& v, const Dealt& w) { return b.matrices[v.matrix].n > b.matrices[w.matrix].n; });
+                p.slots_at[k] = b.slots.size();
+                deal(b.slots, work);
+                p.total[k] = static_cast<uint32_t>(b.slots.size() - p.slots_at[k]);
+            }
+            b.parts.push_back(p);
+            first = last;
+        }
     }
     Header& h = b.head;
     h.magic = kMagic;
@@ -433,10 +532,10 @@ using namespace jabas::muon;
 JABAS_API size_t jabas_orthogonalize_workspace_bytes(const JabasOrthogonalize* o) {
     Batch b;
     Scales s;
-    return describe_batch(o, b, s) == JABAS_OK ? static_cast<size_t>(b.bytes) : 0;
+    return guarded([&] { return describe_batch(o, b, s); }) == JABAS_OK ? static_cast<size_t>(b.bytes) : 0;
 }
 
-JABAS_API int jabas_orthogonalize(const JabasOrthogonalize* o, void* workspace, size_t workspace_bytes, jabas_stream_t stream) {
+static int orthogonalize(const JabasOrthogonalize* o, void* workspace, size_t workspace_bytes, jabas_stream_t stream) {
     Batch b;
     Scales s;
     const int status = describe_batch(o, b, s);
@@ -447,12 +546,10 @@ JABAS_API int jabas_orthogonalize(const JabasOrthogonalize* o, void* workspace, 
     const int64_t size = o->dtype == JABAS_F32 ? 4 : 2, each = halves_of(x, b.planes);
     for (int64_t done = 0; done < o->batch; done += b.at_once) {
         const int64_t here = std::min(b.at_once, o->batch - done);
-        Load symmetric(b.planes), update(b.planes);
-        add_symmetric(symmetric, x, static_cast<double>(here));
-        add_update(update, x, static_cast<double>(here));
         Run r{};
-        r.symmetric = symmetric.best();
-        r.update = update.best();
+        const Shape shape(x, here);
+        if (!b.tiny)
+            for (int k = 0; k < kProducts; ++k) r.kernel[k] = kernel_of(&shape, 1, static_cast<Product>(k), b.planes);
         r.planes = b.planes;
         r.dtype = o->dtype;
         r.tiny = b.tiny;
@@ -468,7 +565,10 @@ JABAS_API int jabas_orthogonalize(const JabasOrthogonalize* o, void* workspace, 
         w.part_step = x.parts;
         w.sums = static_cast<double*>(workspace);
         w.halves = static_cast<char*>(workspace) + (b.tiny ? 0 : b.sums_bytes);
-        const int64_t per[kKinds] = {b.tiny ? 1 : x.parts, lay_tiles(x), symmetric_tiles(x.m, kTile[r.symmetric]), update_tiles(x.m, x.n, kTile[r.update])};
+        int64_t per[kKinds];
+        for (int k = 0; k < kProducts; ++k) per[k] = b.tiny ? 0 : shape.tiles(static_cast<Product>(k), r.kernel[k]);
+        per[kMomentum] = b.tiny ? 1 : x.parts;
+        per[kLayOut] = lay_tiles(x);
         for (int k = 0; k < kKinds; ++k) {
             r.work[k] = w;
             r.work[k].per = static_cast<int32_t>(per[k]);
@@ -480,6 +580,10 @@ JABAS_API int jabas_orthogonalize(const JabasOrthogonalize* o, void* workspace, 
         if (launched != JABAS_OK) return launched;
     }
     return JABAS_OK;
+}
+
+JABAS_API int jabas_orthogonalize(const JabasOrthogonalize* o, void* workspace, size_t workspace_bytes, jabas_stream_t stream) {
+    return guarded([&] { return orthogonalize(o, workspace, workspace_bytes, stream); });
 }
 
 JABAS_API size_t jabas_muon_plan_bytes(const JabasMatrix* matrices, uint32_t n, int32_t precision) {
@@ -542,8 +646,7 @@ JABAS_API int jabas_muon_step(const void* plan_host, const void* plan_dev, const
     }
     for (uint32_t p = 0; p < h->n_parts; ++p) {
         Run r{};
-        r.symmetric = static_cast<Kind>(parts[p].symmetric);
-        r.update = static_cast<Kind>(parts[p].update);
+        for (int k = 0; k < kProducts; ++k) r.kernel[k] = static_cast<Kind>(parts[p].kernel[k]);
         r.tiny = h->tiny;
         r.planes = h->precision == JABAS_F32 ? 2 : 1;
         r.dtype = JABAS_F32;

@@ -106,7 +106,7 @@ def test_nothing_to_do_launches_nothing(empty):
 def test_the_workspace_does_not_grow_with_the_batch():
     sizes = [L.lib().jabas_orthogonalize_workspace_bytes(C.byref(_batch(batch=n, rows=1024, cols=1024, in_row_stride=1024, in_batch_stride=1 << 20,
                                                                         out=1 << 45))) for n in (1, 4, 100, 1000)]
-    assert sizes[0] < sizes[1] < sizes[2] == sizes[3] < 260 << 20
+    assert sizes[0] < sizes[1] < sizes[2] == sizes[3] < 520 << 20
 
 
 @pytest.mark.parametrize("change,status", [
@@ -135,7 +135,7 @@ def test_plans_and_their_workspace():
     status, blob, size = _encode(*[_matrix(i, rows=1024, cols=4096) for i in range(40)], _matrix(40, rows=3, cols=5, group=2))
     assert status == L.OK
     ws = lib.jabas_muon_workspace_bytes(blob.data_ptr())
-    assert 0 < ws < 260 << 20 and ws % 256 == 0                # 40 matrices of 80 MB go through it some at a time
+    assert 0 < ws < 520 << 20 and ws % 256 == 0                # 40 matrices of 80 MB go through it some at a time
     again = _encode(*[_matrix(i, rows=1024, cols=4096) for i in range(40)], _matrix(40, rows=3, cols=5, group=2))[1]
     assert torch.equal(blob, again)
     table, n = _list(_matrix())
