@@ -329,7 +329,7 @@ struct Dealt {
     uint32_t matrix;
     int64_t tiles;
 };
-void deal(std::vector<Slot>& out, const std::vector<Dealt>& work) {
+void deal(std::vector<Slot>& out, const std::vector<Dealt>& work, const std::vector<Matrix>& all) {
     std::vector<Slot> die[8];
     int turn = 0;
     int64_t total = 0;
@@ -338,7 +338,7 @@ void deal(std::vector<Slot>& out, const std::vector<Dealt>& work) {
         uint32_t at = 0;
         for (int d = 0; d < 8; ++d) {
             const int64_t here = each + (d < left);
-            for (int64_t t = 0; t < here; ++t) die[(turn + d) & 7].push_back({w.matrix, at++});
+            for (int64_t t = 0; t < here; ++t) die[(turn + d) & 7].push_back({w.matrix, at++, all[w.matrix].m, all[w.matrix].n, all[w.matrix].x_at, all[w.matrix].a_at});
         }
         turn = (turn + static_cast<int>(left)) & 7;
         total += w.tiles;
@@ -452,7 +452,7 @@ int build(const JabasMatrix* list, uint32_t n, int32_t precision, Built& b) {
         std::vector<Dealt> work;
         for (uint32_t i = 0; i < n; ++i) work.push_back({i, 1});
         Part p{};
-        deal(b.slots, work);
+        deal(b.slots, work, b.matrices);
         p.total[kMomentum] = n;
         b.parts.push_back(p);
     } else {
@@ -484,7 +484,7 @@ int build(const JabasMatrix* list, uint32_t n, int32_t precision, Built& b) {
                 if (k == kFirst)
                     std::stable_sort(work.begin(), work.end(), [&](const Dealt& v, const Dealt& w) { return b.matrices[v.matrix].n > b.matrices[w.matrix].n; });
                 p.slots_at[k] = b.slots.size();
-                deal(b.slots, work);
+                deal(b.slots, work, b.matrices);
                 p.total[k] = static_cast<uint32_t>(b.slots.size() - p.slots_at[k]);
             }
             b.parts.push_back(p);

@@ -43,8 +43,10 @@ __host__ __device__ inline int64_t second_of(int64_t plane) { return P == 2 ? 32
 
 // Which workgroup does what. A list: `table` and a slot {matrix, tile} for every workgroup. A batch: matrix 0 and what lies between it and
 // the next one.
-struct Slot {
+struct Slot {                       // with what the products need of the matrix, so that they start one read of memory earlier
     uint32_t matrix, tile;
+    int32_t m, n;
+    int64_t x_at, a_at;
 };
 struct Work {
     const Matrix* table;

@@ -77,6 +77,7 @@ struct Staged {
     static constexpr int kEach = C::kI * 2, kGroup = kEach < 4 ? kEach : 4, kGroups = kEach / kGroup;
     static __device__ int row(int t) { return (t * 64 + static_cast<int>(threadIdx.x & 63)) / (C::kI * 4); }
     static __device__ int col(int t) { return (t * 64 + static_cast<int>(threadIdx.x & 63)) % (C::kI * 4) * 8; }
+    static constexpr bool kEarly = C::kM < 256;         // the first group is on its way while the products are made: large tiles have no registers for it
     // Q planes of a matrix laid out for products of P
     template <int P, int Q>
     static __device__ void fetch(Planes<Q> (&x)[kGroup], int g, const _Float16* from, int64_t plane, int row0, int rows, int col0, int cols) {
@@ -110,23 +111,23 @@ __device__ inline void triangle(uint32_t tile, int& tm, int& tn) {
 template <int P, class C, bool SECOND>
 __global__ __launch_bounds__(C::kThreads) void symmetric_kernel(SymmetricArgs a) {
     __shared__ __align__(16) char smem[C::kStages * C::kStage];
-    Place at;
-    if (!place_of(a.w, at)) return;
-    const Matrix& x = at.x;
+    Sides x;
+    if (!sides_of(a.w, x)) return;
     int tm, tn;
-    triangle(at.tile, tm, tn);
+    triangle(x.tile, tm, tn);
     const int m0 = tm * C::kM, n0 = tn * C::kN, lane = threadIdx.x & 63;
     _Float16* base = static_cast<_Float16*>(a.w.halves);
     _Float16 *own = base + x.a_at, *to = own + (SECOND ? P * x.a_plane : 0);
     const Operand o = SECOND ? Operand{own, stride_of<P>(x.pad_m), second_of<P>(x.a_plane), x.m}
                              : Operand{base + x.x_at + a.from * 2 * x.x_plane, stride_of<P>(x.pad_n), second_of<P>(x.x_plane), x.m};
-    C c;
-    c.run(o, o, m0, n0, SECOND ? x.pad_m : x.pad_n, smem, [] {}, [](int, int) { return 0.0f; });
-    const Staged<C> staged(smem);
     using S = Staged<C>;
     const int wm = m0 + C::wave_m(), wn = n0 + C::wave_n();
     Planes<P> beside[2][S::kGroup];
-    if (SECOND) S::template fetch<P, P>(beside[0], 0, own, x.a_plane, wn, x.m, wm, x.pad_m);
+    const auto fetch_first = [&] { S::template fetch<P, P>(beside[0], 0, own, x.a_plane, wn, x.m, wm, x.pad_m); };
+    C c;
+    c.run(o, o, m0, n0, SECOND ? x.pad_m : x.pad_n, smem, [&] { if (SECOND && S::kEarly) fetch_first(); }, [](int, int) { return 0.0f; });
+    const S staged(smem);
+    if (SECOND && !S::kEarly) fetch_first();
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < C::kJ; ++j) {
@@ -284,16 +285,22 @@ template <int P, bool SECOND, int S>
 __global__ __launch_bounds__(256) void symmetric_deep_kernel(SymmetricArgs a) {
     using D = Deep<P, false, S>;
     __shared__ __align__(16) char smem[D::kBytes];
-    Place at;
-    if (!place_of(a.w, at)) return;
-    const Matrix& x = at.x;
+    Sides x;
+    if (!sides_of(a.w, x)) return;
     int tm, tn;
-    triangle(at.tile, tm, tn);
+    triangle(x.tile, tm, tn);
     const int m0 = tm * 64, n0 = tn * 64;
     _Float16* base = static_cast<_Float16*>(a.w.halves);
     _Float16 *own = base + x.a_at, *to = own + (SECOND ? P * x.a_plane : 0);
     const Operand o = SECOND ? Operand{own, stride_of<P>(x.pad_m), second_of<P>(x.a_plane), x.m}
                              : Operand{base + x.x_at + a.from * 2 * x.x_plane, stride_of<P>(x.pad_n), second_of<P>(x.x_plane), x.m};
+    Planes<P> beside[2];            // on their way while the products are made
+    if (SECOND)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int q = 0; q < P; ++q)
+                beside[t].v[q] = *reinterpret_cast<const f16x8*>(own + half_at<P>(min(n0 + D::row(t), x.m - 1), min(m0 + D::col(), x.pad_m - 8), x.pad_m) + q * second_of<P>(x.a_plane));
     float* sums = D::run(o, o, m0, n0, SECOND ? x.pad_m : x.pad_n, a.product, smem);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -304,10 +311,7 @@ __global__ __launch_bounds__(256) void symmetric_deep_kernel(SymmetricArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v.v[e] = sums[r * D::kRow + D::col() + e];
         if (SECOND) {
-            Planes<P> p;
-#pragma unroll
-            for (int q = 0; q < P; ++q) p.v[q] = *reinterpret_cast<const f16x8*>(own + place + q * second_of<P>(x.a_plane));
-            v.add(p, a.own);
+            v.add(beside[t], a.own);
             if (tm != tn)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sums[r * D::kRow + D::col() + e] = v.v[e];
@@ -342,26 +346,26 @@ __device__ inline void band(uint32_t tile, int across, int down, int& tm, int& t
 template <int P, class C>
 __global__ __launch_bounds__(C::kThreads) void update_kernel(UpdateArgs a) {
     __shared__ __align__(16) char smem[C::kStages * C::kStage];
-    Place at;
-    if (!place_of(a.w, at)) return;
-    const Matrix& x = at.x;
+    Sides x;
+    if (!sides_of(a.w, x)) return;
     int m0, n0;
-    band(at.tile, (x.n + C::kM - 1) / C::kM, (x.m + C::kN - 1) / C::kN, m0, n0);
+    band(x.tile, (x.n + C::kM - 1) / C::kM, (x.m + C::kN - 1) / C::kN, m0, n0);
     m0 *= C::kM;
     n0 *= C::kN;
     const int lane = threadIdx.x & 63;
     _Float16* base = static_cast<_Float16*>(a.w.halves);
     const _Float16* from = base + x.x_at + a.from * 2 * x.x_plane;
     _Float16* to = base + x.x_at + (1 - a.from) * 2 * x.x_plane;
-    C c;
-    c.run(Operand{from, stride_of<P>(x.pad_n), second_of<P>(x.x_plane), x.pad_n},
-          Operand{base + x.a_at + P * x.a_plane, stride_of<P>(x.pad_m), second_of<P>(x.a_plane), x.m}, m0, n0, x.pad_m, smem, [] {},
-          [](int, int) { return 0.0f; });
-    const Staged<C> staged(smem);
     using S = Staged<C>;
     const int wm = m0 + C::wave_m(), wn = n0 + C::wave_n();
     Planes<2> beside[2][S::kGroup];
-    S::template fetch<P, 2>(beside[0], 0, from, x.x_plane, wn, x.m, wm, x.pad_n);
+    const auto fetch_first = [&] { S::template fetch<P, 2>(beside[0], 0, from, x.x_plane, wn, x.m, wm, x.pad_n); };
+    C c;
+    c.run(Operand{from, stride_of<P>(x.pad_n), second_of<P>(x.x_plane), x.pad_n},
+          Operand{base + x.a_at + P * x.a_plane, stride_of<P>(x.pad_m), second_of<P>(x.a_plane), x.m}, m0, n0, x.pad_m, smem,
+          [&] { if (S::kEarly) fetch_first(); }, [](int, int) { return 0.0f; });
+    const S staged(smem);
+    if (!S::kEarly) fetch_first();
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < C::kJ; ++j) {
@@ -392,24 +396,25 @@ __global__ __launch_bounds__(C::kThreads) void update_kernel(UpdateArgs a) {
         }
         if (!a.last) continue;
         wave_done();
-        if (x.tall) {
+        const Matrix out = matrix_of(a.w, x.matrix);
+        if (out.tall) {
 #pragma unroll 1
             for (int t = 0; t < C::kI * 4; ++t) {       // column wm + col of X is a row of the weights
                 const int f = t * 64 + lane, r = f % 8 * 4, col = f / 8, row = wm + col, m = wn + j * 32 + r;
-                if (row >= x.rows || m >= x.cols) continue;
+                if (row >= out.rows || m >= out.cols) continue;
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = staged.at(r + e, col);
-                put_out<4>(a.out, a.w.fanout, x, row, m, v);
+                put_out<4>(a.out, a.w.fanout, out, row, m, v);
             }
         } else {
 #pragma unroll 1
             for (int t = 0; t < S::kEach; ++t) {
                 const int r = S::row(t), col = S::col(t), row = wn + j * 32 + r, m = wm + col;
-                if (row >= x.rows || m >= x.cols) continue;
+                if (row >= out.rows || m >= out.cols) continue;
                 Eight v;
                 staged.get(r, col, v);
-                put_out<8>(a.out, a.w.fanout, x, row, m, v.v);
+                put_out<8>(a.out, a.w.fanout, out, row, m, v.v);
             }
         }
     }
@@ -420,50 +425,54 @@ template <int P, int S>
 __global__ __launch_bounds__(256) void update_deep_kernel(UpdateArgs a) {
     using D = Deep<P, true, S>;
     __shared__ __align__(16) char smem[D::kBytes];
-    Place at;
-    if (!place_of(a.w, at)) return;
-    const Matrix& x = at.x;
+    Sides x;
+    if (!sides_of(a.w, x)) return;
     int m0, n0;
-    band(at.tile, (x.n + 63) / 64, (x.m + 63) / 64, m0, n0);
+    band(x.tile, (x.n + 63) / 64, (x.m + 63) / 64, m0, n0);
     m0 *= 64;
     n0 *= 64;
     _Float16* base = static_cast<_Float16*>(a.w.halves);
     const _Float16* from = base + x.x_at + a.from * 2 * x.x_plane;
     _Float16* to = base + x.x_at + (1 - a.from) * 2 * x.x_plane;
+    Planes<2> beside[2];            // on their way while the products are made
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+            beside[t].v[q] = *reinterpret_cast<const f16x8*>(from + half_at<P>(n0 + D::row(t), m0 + D::col(), x.pad_n) + q * second_of<P>(x.x_plane));
     float* sums = D::run(Operand{from, stride_of<P>(x.pad_n), second_of<P>(x.x_plane), x.pad_n},
-          Operand{base + x.a_at + P * x.a_plane, stride_of<P>(x.pad_m), second_of<P>(x.a_plane), x.m}, m0, n0, x.pad_m, a.product, smem);
+                         Operand{base + x.a_at + P * x.a_plane, stride_of<P>(x.pad_m), second_of<P>(x.a_plane), x.m}, m0, n0, x.pad_m, a.product, smem);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const int r = D::row(t), row = n0 + r, m = m0 + D::col();       // whole rows of the padded copy, up to pad_m and pad_n
-        const int64_t place = half_at<P>(row, m, x.pad_n);
         Eight v;
         if (row < x.m) {
-            Planes<2> p;
-#pragma unroll
-            for (int q = 0; q < 2; ++q) p.v[q] = *reinterpret_cast<const f16x8*>(from + place + q * second_of<P>(x.x_plane));
 #pragma unroll
             for (int e = 0; e < 8; ++e) v.v[e] = sums[r * D::kRow + D::col() + e];
-            v.add(p, a.own);
+            v.add(beside[t], a.own);
         } else {                    // the next product takes these rows of k as well
 #pragma unroll
             for (int e = 0; e < 8; ++e) v.v[e] = 0.0f;
         }
-        if (!a.last) v.put_planes(to + place, to + place + second_of<P>(x.x_plane));
-        else if (x.tall)
+        if (a.last) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) sums[r * D::kRow + D::col() + e] = v.v[e];
-        else if (row < x.m && m < x.n) put_out<8>(a.out, a.w.fanout, x, row, m, v.v);
+        } else {
+            const int64_t place = half_at<P>(row, m, x.pad_n);
+            v.put_planes(to + place, to + place + second_of<P>(x.x_plane));
+        }
     }
-    if (!a.last || !x.tall) return;
+    if (!a.last) return;
     __syncthreads();
+    const Matrix out = matrix_of(a.w, x.matrix);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {       // column m0 + col of X is a row of the weights
-        const int col = D::row(t), r = D::col(), row = m0 + col, m = n0 + r;
-        if (row >= x.rows || m >= x.cols) continue;
+    for (int t = 0; t < 2; ++t) {       // where X is the transpose, column m0 + D::row(t) of it is a row of the weights
+        const int row = (out.tall ? m0 : n0) + D::row(t), col = (out.tall ? n0 : m0) + D::col();
+        if (row >= out.rows || col >= out.cols) continue;
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = sums[(r + e) * D::kRow + col];
-        put_out<8>(a.out, a.w.fanout, x, row, m, v);
+        for (int e = 0; e < 8; ++e) v[e] = out.tall ? sums[(D::col() + e) * D::kRow + D::row(t)] : sums[D::row(t) * D::kRow + D::col() + e];
+        put_out<8>(a.out, a.w.fanout, out, row, col, v);
     }
 }
 

@@ -23,9 +23,9 @@ __device__ inline f32x4 quad(const T* p, int64_t i) {
 // Bound by memory, 12 bytes an element (without momentum 2 or 4).
 template <class T>
 __global__ __launch_bounds__(256) void momentum_kernel(PassArgs a) {
-    Place at;
-    if (!place_of(a.w, at)) return;
-    const Matrix& x = at.x;
+    Sides at;
+    if (!sides_of(a.w, at)) return;
+    const Matrix x = matrix_of(a.w, at.matrix);
     const T* src = static_cast<const T*>(x.src);
     const Mix mix(a);
     const int64_t count = static_cast<int64_t>(x.rows) * x.cols, begin = static_cast<int64_t>(at.tile) * x.chunk;
@@ -80,9 +80,9 @@ __global__ __launch_bounds__(256) void momentum_kernel(PassArgs a) {
 // Bound by memory: 8 bytes an element in, 4 out.
 template <class T, int P>
 __global__ __launch_bounds__(256) void lay_kernel(PassArgs a) {
-    Place at;
-    if (!place_of(a.w, at)) return;
-    const Matrix& x = at.x;
+    Sides at;
+    if (!sides_of(a.w, at)) return;
+    const Matrix x = matrix_of(a.w, at.matrix);
     const T* src = static_cast<const T*>(x.src);
     const Mix mix(a);
     __shared__ double waves[4];

@@ -78,9 +78,9 @@ template <class T, int MB>
 __global__ __launch_bounds__(kThreads) void tiny_kernel(TinyArgs a) {
     __shared__ __align__(16) char smem[kTinyBytes];
     __shared__ double waves[kWaves];
-    Place at;
-    if (!place_of(a.pass.w, at)) return;
-    const Matrix& x = at.x;
+    Sides at;
+    if (!sides_of(a.pass.w, at)) return;
+    const Matrix x = matrix_of(a.pass.w, at.matrix);
     constexpr int kM = MB * 32;
     const int cols = (x.n + 31) & ~31, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const Held A{reinterpret_cast<_Float16*>(smem), tiny_row(kM), kM * tiny_row(kM)};
