@@ -74,8 +74,9 @@ typedef struct JabasMatrix {
 
 /* The launch-invariant description of a list of matrices, as jabas_plan_encode makes one of spans: validated and encoded
  * into host memory, copied to the device once by the caller (16-byte aligned), both passed to every step. Pure host code.
- * Matrices go through the workspace some at a time, in order of their work, so that it does not grow with the list. */
-size_t jabas_muon_plan_bytes(const JabasMatrix* matrices, uint32_t n, int32_t precision);       /* 0: refused by encode */
+ * Matrices go through the workspace some at a time, in order of their sides, so that it does not grow past 512 MiB with the
+ * list (one that needs more is alone in it). At most 2^20 matrices. */
+size_t jabas_muon_plan_bytes(const JabasMatrix* matrices, uint32_t n, int32_t precision);       /* what is enough; 0: refused by encode */
 int jabas_muon_plan_encode(const JabasMatrix* matrices, uint32_t n, int32_t precision, void* host_blob, size_t blob_bytes);
 size_t jabas_muon_workspace_bytes(const void* host_blob);       /* 0 on a malformed blob */
 
@@ -88,7 +89,7 @@ typedef struct JabasMuonArgs {
     const float* grad_scale;        /* device scalar c or NULL: gradients are multiplied by c when c < 1 (clipping) */
 } JabasMuonArgs;
 
-/* 3 launches and 3 for every Newton-Schulz step but the first's, per part of the list. */
+/* Two launches and three for every Newton-Schulz step, per part of the list; one in all where a workgroup's LDS holds any of the matrices. */
 int jabas_muon_step(const void* plan_host, const void* plan_dev, const JabasMuonArgs* args,
                     void* workspace, size_t workspace_bytes, jabas_stream_t stream);
 

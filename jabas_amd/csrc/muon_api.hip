@@ -251,7 +251,7 @@ int describe_batch(const JabasOrthogonalize* o, Batch& b, Scales& s) {
     b.x.out_quads = !misaligned(o->out, quad) && o->cols % 4 == 0;
     b.tiny = tiny_fits(blocks_of(b.x), b.x.n) ? blocks_of(b.x) : 0;
     if (b.tiny) {
-        b.at_once = std::min(o->batch, kMaxSlots / 2);
+        b.at_once = std::min(o->batch, kMaxSlots / 4);          // of 1024 threads
         return JABAS_OK;
     }
     const int64_t each = halves_of(b.x, b.planes);
@@ -280,7 +280,7 @@ int describe_batch(const JabasOrthogonalize* o, Batch& b, Scales& s) {
 
 // ---- lists
 
-constexpr uint32_t kMagic = 0x4d4e5331;
+constexpr uint32_t kMagic = 0x4d4e5331, kMaxMatrices = 1u << 20;
 struct Part {
     uint64_t slots_at[kKinds];
     uint32_t total[kKinds];
@@ -408,7 +408,7 @@ struct Built {
 
 int build(const JabasMatrix* list, uint32_t n, int32_t precision, Built& b) {
     if (!list) return JABAS_ERR_NULL;
-    if (n < 1 || n > (1u << 20)) return JABAS_ERR_SIZE;
+    if (n < 1 || n > kMaxMatrices) return JABAS_ERR_SIZE;
     if (precision != JABAS_F32 && precision != JABAS_BF16) return JABAS_ERR_DTYPE;
     const int planes = precision == JABAS_F32 ? 2 : 1;
     b.head = Header{};
@@ -444,7 +444,7 @@ int build(const JabasMatrix* list, uint32_t n, int32_t precision, Built& b) {
     }
     // the matrices come with the longest shorter side first
     const int blocks = blocks_of(b.matrices[0]);
-    bool tiny = n <= kMaxSlots / 2;
+    bool tiny = true;
     for (const Matrix& x : b.matrices) tiny = tiny && tiny_fits(blocks, x.n);
     b.head.tiny = tiny ? blocks : 0;
     uint64_t halves_most = 0, sums_most = 0;
@@ -587,14 +587,18 @@ JABAS_API int jabas_orthogonalize(const JabasOrthogonalize* o, void* workspace, 
 }
 
 JABAS_API size_t jabas_muon_plan_bytes(const JabasMatrix* matrices, uint32_t n, int32_t precision) {
-    size_t bytes = 0;
-    const int status = guarded([&] {
-        Built b;
-        const int built = build(matrices, n, precision, b);
-        if (built == JABAS_OK) bytes = b.head.bytes;
-        return built;
-    });
-    return status == JABAS_OK ? bytes : 0;
+    if (!matrices || n < 1 || n > kMaxMatrices || (precision != JABAS_F32 && precision != JABAS_BF16)) return 0;
+    // every launch with the smallest tiles, every matrix a part
+    uint64_t slots = 0, fanout = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+        if (check_matrix(matrices[i]) != JABAS_OK) return 0;
+        Matrix x{};
+        describe(x, matrices[i].rows, matrices[i].cols);
+        slots += x.parts + lay_tiles(x) + 2 * symmetric_tiles(x.m, 64) + update_tiles(x.m, x.n, 64);
+        fanout += matrices[i].n_fanout;
+    }
+    return static_cast<size_t>(round_up(sizeof(Header), 16) + round_up(sizeof(Matrix) * n, 16) + round_up(8 * fanout, 16) + round_up(sizeof(Part) * n, 16) +
+                               round_up(sizeof(Slot) * slots, 16));
 }
 
 JABAS_API int jabas_muon_plan_encode(const JabasMatrix* matrices, uint32_t n, int32_t precision, void* host_blob, size_t blob_bytes) {
