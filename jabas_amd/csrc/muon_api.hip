@@ -80,6 +80,9 @@ void describe(Matrix& x, int64_t rows, int64_t cols) {
     x.chunk = static_cast<int32_t>(chunk);
     x.parts = static_cast<int32_t>((count + chunk - 1) / chunk);
 }
+// Behind them, of any call: tiles' sums of launches that share tiles between workgroups, and the tiles' tickets.
+constexpr int64_t kSplitUnits = 256, kSplitTiles = 64;      // workgroups and tiles of a launch that shares tiles, at most
+constexpr int64_t kShareBytes = kSplitUnits * (4096 + 1) * 4;
 // halves of the workspace: X twice in two planes, A and B in as many as the products take
 int64_t halves_of(const Matrix& x, int planes) { return 4 * x.x_plane + 2 * planes * x.a_plane; }
 int64_t lay_tiles(const Matrix& x) { return static_cast<int64_t>(x.pad_m / kLay) * (x.pad_n / kLay); }
@@ -102,7 +105,7 @@ constexpr Cost kCosts[2][kKernels] = {
     {{2, 2.5, 0.20, 0.38, 0.46}, {4, 4.0, 0.50, 0.75, 0.75}, {2, 7.0, 0.62, 0.90, 1.00}, {1, 5.0, 0.38, 0.53, 0.60}, {1, 13.0, 1.25, 1.75, 1.75}},
     {{2, 3.5, 0.45, 0.76, 0.95}, {4, 4.5, 0.90, 1.60, 1.60}, {2, 8.0, 1.35, 2.60, 2.65}, {1, 6.0, 0.95, 1.15, 1.35}, {1, 18.0, 3.40, 4.75, 4.75}}};
 constexpr int64_t kCus = 256, kFew = 160;
-constexpr double kLaunch = 4.0;                 // us of a launch, beside its tiles
+constexpr double kLaunch = 4.0, kJoin = 4.0;    // us of a launch, beside its tiles, and of tiles' parts that meet
 
 enum Product { kFirst, kSecond, kUpdate, kProducts };
 struct Shape {
@@ -143,14 +146,29 @@ double makespan(std::vector<Tiles> work, int64_t slots) {
     return end;
 }
 
+// Workgroups that share a tile's inner axis, where a launch (of `total` tiles) leaves most CUs idle and the axis is long: the parts meet through memory, which
+// takes 4 us with few of them and 6 with many. Without and with it, us of a call: 256 x 4096 fp32 241 and 155, four of 64 x 4096 222 and 126, 21
+// convolutions' matrices (43 tiles) 159 and 153; but 1000 x 384 and four of 384 x 384 (two workgroups to each of 105 tiles) 166 and 202, 1000 x 2048 bf16 183 and 241.
+constexpr int64_t kMostSplits = 8;
+int splits_of(const Shape& s, Product p, Kind k, int64_t total, int planes) {
+    if (p != kFirst || k != kSmall || total > kSplitTiles) return 1;     // A A has no long axis where there are few tiles
+    const int64_t splits = std::min({kSplitUnits / std::max<int64_t>(total, 1), static_cast<int64_t>(s.steps(p)) / (planes == 2 ? 6 : 12), kMostSplits});
+    return splits >= 3 ? static_cast<int>(splits) : 1;
+}
+
 double time_of(const Shape* shapes, size_t n, Product p, Kind k, int planes) {
     const Cost& c = kCosts[planes - 1][k];
-    int64_t total = 0;
-    for (size_t i = 0; i < n; ++i) total += shapes[i].count * shapes[i].tiles(p, k);
-    const double step = total <= kFew ? c.alone : p == kUpdate ? c.update : c.symmetric;
-    if (n == 1) return kLaunch + (total + kCus * c.each - 1) / (kCus * c.each) * (c.start + shapes[0].steps(p) * step);
+    int64_t tiles = 0, units = 0;
+    for (size_t i = 0; i < n; ++i) tiles += shapes[i].count * shapes[i].tiles(p, k);
+    for (size_t i = 0; i < n; ++i) units += shapes[i].count * shapes[i].tiles(p, k) * splits_of(shapes[i], p, k, tiles, planes);
+    const double step = units <= kFew ? c.alone : p == kUpdate ? c.update : c.symmetric;
+    const auto work_of = [&](const Shape& s) {
+        const int splits = splits_of(s, p, k, tiles, planes);
+        return Tiles{c.start + s.steps(p) / splits * step + (splits > 1 ? kJoin : 0.0), s.count * s.tiles(p, k) * splits};
+    };
+    if (n == 1) return kLaunch + (units + kCus * c.each - 1) / (kCus * c.each) * work_of(shapes[0]).length;
     std::vector<Tiles> work;
-    for (size_t i = 0; i < n; ++i) work.push_back({c.start + shapes[i].steps(p) * step, shapes[i].count * shapes[i].tiles(p, k)});
+    for (size_t i = 0; i < n; ++i) work.push_back(work_of(shapes[i]));
     return kLaunch + makespan(work, kCus * c.each);
 }
 Kind kernel_of(const Shape* shapes, size_t n, Product p, int planes, double* time = nullptr) {
@@ -182,9 +200,11 @@ struct Run {
     int planes, dtype, nesterov;
     float momentum, fresh;
     const float* grad_scale;
+    float* shares;
 };
 int run(const Run& r, const JabasNewtonSchulz& ns, const Scales& s, UpdateArgs& last, hipStream_t stream) {
-    PassArgs pass{r.work[kMomentum], r.dtype, r.nesterov, r.momentum, r.fresh, r.grad_scale, ns.eps, static_cast<float>(s.x[0]), r.planes};
+    PassArgs pass{r.work[kMomentum], r.dtype, r.nesterov, r.momentum, r.fresh, r.grad_scale, ns.eps, static_cast<float>(s.x[0]), r.planes,
+                  r.shares ? reinterpret_cast<uint32_t*>(r.shares + kSplitUnits * 4096) : nullptr, r.shares ? static_cast<uint32_t>(kSplitUnits) : 0};
     TinyStep steps[JABAS_MUON_MAX_STEPS];
     for (int k = 0; k < ns.steps; ++k)
         steps[k] = {static_cast<float>(s.a[k] / s.x[k] / s.x[k]), static_cast<float>(ns.b * s.b[k] / s.a[k]), static_cast<float>(ns.c * s.b[k] / s.a[k] / s.a[k]),
@@ -199,8 +219,8 @@ int run(const Run& r, const JabasNewtonSchulz& ns, const Scales& s, UpdateArgs& 
     pass.w = r.work[kLayOut];
     if ((status = launch_lay(pass, stream)) != JABAS_OK) return status;
     for (int k = 0; k < ns.steps; ++k) {
-        if ((status = launch_symmetric({r.work[kFirst], k & 1, 0.0f, steps[k].first}, false, r.planes, r.kernel[kFirst], stream)) != JABAS_OK) return status;
-        if ((status = launch_symmetric({r.work[kSecond], k & 1, steps[k].second_own, steps[k].second}, true, r.planes, r.kernel[kSecond], stream)) != JABAS_OK) return status;
+        if ((status = launch_symmetric({r.work[kFirst], k & 1, 0.0f, steps[k].first, r.shares, pass.tickets}, false, r.planes, r.kernel[kFirst], stream)) != JABAS_OK) return status;
+        if ((status = launch_symmetric({r.work[kSecond], k & 1, steps[k].second_own, steps[k].second, nullptr, nullptr}, true, r.planes, r.kernel[kSecond], stream)) != JABAS_OK) return status;
         last.w = r.work[kUpdate];
         last.from = k & 1;
         last.last = k + 1 == ns.steps;
@@ -215,7 +235,7 @@ int run(const Run& r, const JabasNewtonSchulz& ns, const Scales& s, UpdateArgs& 
 
 // Matrices that go through the workspace together take at most this, or are one. How many do is what ends first by the costs above: the last tiles of a launch
 // leave CUs idle, and a launch has its own time.
-constexpr int64_t kTogether = int64_t{512} << 20;
+constexpr int64_t kTogether = int64_t{500} << 20;
 constexpr int64_t kTurns = 16;          // ways of cutting that are tried
 
 inline int blocks_of(const Matrix& x) { return (x.m + 31) / 32; }
@@ -260,7 +280,7 @@ int describe_batch(const JabasOrthogonalize* o, Batch& b, Scales& s) {
     if (most < 1) return JABAS_ERR_SIZE;
     b.at_once = std::min({o->batch, std::max<int64_t>(1, kTogether / (2 * each)), most});
     b.sums_bytes = round_up(8 * b.at_once * b.x.parts, 256);
-    b.bytes = b.sums_bytes + round_up(2 * b.at_once * each, 256);
+    b.bytes = b.sums_bytes + round_up(2 * b.at_once * each, 256) + kShareBytes;
     const int64_t least = (o->batch + b.at_once - 1) / b.at_once;
     double best = 0.0;
     for (int64_t turns = least; o->batch > 1 && turns < least + kTurns && turns <= o->batch; ++turns) {
@@ -327,7 +347,8 @@ int check_matrix(const JabasMatrix& j) {
 // d, d + 8, ... . `work`: matrices and their tiles, the longest first.
 struct Dealt {
     uint32_t matrix;
-    int64_t tiles;
+    int64_t tiles;                  // workgroups
+    int32_t splits;
 };
 void deal(std::vector<Slot>& out, const std::vector<Dealt>& work, const std::vector<Matrix>& all) {
     std::vector<Slot> die[8];
@@ -335,10 +356,10 @@ void deal(std::vector<Slot>& out, const std::vector<Dealt>& work, const std::vec
     int64_t total = 0;
     for (const Dealt& w : work) {
         const int64_t each = w.tiles / 8, left = w.tiles % 8;
-        uint32_t at = 0;
+        Slot s{w.matrix, 0, all[w.matrix].m, all[w.matrix].n, all[w.matrix].x_at, all[w.matrix].a_at, static_cast<uint32_t>(total), w.splits};
         for (int d = 0; d < 8; ++d) {
             const int64_t here = each + (d < left);
-            for (int64_t t = 0; t < here; ++t) die[(turn + d) & 7].push_back({w.matrix, at++, all[w.matrix].m, all[w.matrix].n, all[w.matrix].x_at, all[w.matrix].a_at});
+            for (int64_t t = 0; t < here; ++t, ++s.tile) die[(turn + d) & 7].push_back(s);
         }
         turn = (turn + static_cast<int>(left)) & 7;
         total += w.tiles;
@@ -450,7 +471,7 @@ int build(const JabasMatrix* list, uint32_t n, int32_t precision, Built& b) {
     uint64_t halves_most = 0, sums_most = 0;
     if (tiny) {
         std::vector<Dealt> work;
-        for (uint32_t i = 0; i < n; ++i) work.push_back({i, 1});
+        for (uint32_t i = 0; i < n; ++i) work.push_back({i, 1, 1});
         Part p{};
         deal(b.slots, work, b.matrices);
         p.total[kMomentum] = n;
@@ -477,9 +498,18 @@ int build(const JabasMatrix* list, uint32_t n, int32_t precision, Built& b) {
             for (int k = 0; k < kProducts; ++k) p.kernel[k] = kernel_of(shapes.data(), shapes.size(), static_cast<Product>(k), planes);
             for (int k = 0; k < kKinds; ++k) {
                 std::vector<Dealt> work;
+                int64_t total = 0;
+                for (const Shape& s : shapes) total += k < kProducts ? s.count * s.tiles(static_cast<Product>(k), static_cast<Kind>(p.kernel[k])) : 0;
                 for (uint32_t i = first; i < last; ++i) {
                     const Matrix& x = b.matrices[i];
-                    work.push_back({i, k == kMomentum ? x.parts : k == kLayOut ? lay_tiles(x) : Shape(x, 1).tiles(static_cast<Product>(k), static_cast<Kind>(p.kernel[k]))});
+                    if (k >= kProducts) {
+                        work.push_back({i, k == kMomentum ? x.parts : lay_tiles(x), 1});
+                        continue;
+                    }
+                    const Shape one(x, 1);
+                    const Product product = static_cast<Product>(k);
+                    const int splits = splits_of(one, product, static_cast<Kind>(p.kernel[k]), total, planes);
+                    work.push_back({i, one.tiles(product, static_cast<Kind>(p.kernel[k])) * splits, splits});
                 }
                 if (k == kFirst)
                     std::stable_sort(work.begin(), work.end(), [&](const Dealt& v, const Dealt& w) { return b.matrices[v.matrix].n > b.matrices[w.matrix].n; });
@@ -504,7 +534,7 @@ int build(const JabasMatrix* list, uint32_t n, int32_t precision, Built& b) {
         for (uint64_t& at : p.slots_at) at = slots_at + at * sizeof(Slot);
     h.bytes = round_up(slots_at + b.slots.size() * sizeof(Slot), 16);
     h.sums_bytes = round_up(8 * sums_most, 256);
-    h.workspace = std::max<uint64_t>(256, h.sums_bytes + round_up(2 * halves_most, 256));
+    h.workspace = tiny ? 256 : h.sums_bytes + round_up(2 * halves_most, 256) + kShareBytes;
     return JABAS_OK;
 }
 
@@ -569,8 +599,14 @@ static int orthogonalize(const JabasOrthogonalize* o, void* workspace, size_t wo
         for (int k = 0; k < kProducts; ++k) per[k] = b.tiny ? 0 : shape.tiles(static_cast<Product>(k), r.kernel[k]);
         per[kMomentum] = b.tiny ? 1 : x.parts;
         per[kLayOut] = lay_tiles(x);
+        if (!b.tiny) r.shares = reinterpret_cast<float*>(static_cast<char*>(workspace) + (b.bytes - kShareBytes));
         for (int k = 0; k < kKinds; ++k) {
             r.work[k] = w;
+            r.work[k].splits = 1;
+            if (k < kProducts && !b.tiny) {
+                r.work[k].splits = splits_of(shape, static_cast<Product>(k), r.kernel[k], per[k] * here, b.planes);
+                per[k] *= r.work[k].splits;
+            }
             r.work[k].per = static_cast<int32_t>(per[k]);
             r.work[k].total = static_cast<uint32_t>(per[k] * here);
         }
@@ -594,7 +630,8 @@ JABAS_API size_t jabas_muon_plan_bytes(const JabasMatrix* matrices, uint32_t n, 
         if (check_matrix(matrices[i]) != JABAS_OK) return 0;
         Matrix x{};
         describe(x, matrices[i].rows, matrices[i].cols);
-        slots += x.parts + lay_tiles(x) + 2 * symmetric_tiles(x.m, 64) + update_tiles(x.m, x.n, 64);
+        const int64_t symmetric = symmetric_tiles(x.m, 64);
+        slots += x.parts + lay_tiles(x) + symmetric + std::min(kMostSplits * symmetric, symmetric + kSplitUnits) + update_tiles(x.m, x.n, 64);
         fanout += matrices[i].n_fanout;
     }
     return static_cast<size_t>(round_up(sizeof(Header), 16) + round_up(sizeof(Matrix) * n, 16) + round_up(8 * fanout, 16) + round_up(sizeof(Part) * n, 16) +
@@ -652,6 +689,7 @@ JABAS_API int jabas_muon_step(const void* plan_host, const void* plan_dev, const
         Run r{};
         for (int k = 0; k < kProducts; ++k) r.kernel[k] = static_cast<Kind>(parts[p].kernel[k]);
         r.tiny = h->tiny;
+        if (!r.tiny) r.shares = reinterpret_cast<float*>(static_cast<char*>(workspace) + (h->workspace - kShareBytes));
         r.planes = h->precision == JABAS_F32 ? 2 : 1;
         r.dtype = JABAS_F32;
         r.nesterov = args->nesterov != 0;

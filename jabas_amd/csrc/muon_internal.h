@@ -47,6 +47,8 @@ struct Slot {                       // with what the products need of the matrix
     uint32_t matrix, tile;
     int32_t m, n;
     int64_t x_at, a_at;
+    uint32_t unit;                  // of the matrix's first workgroup in this launch
+    int32_t splits;                 // workgroups that share a tile's inner axis: workgroup s of a tile is `tile` = s tiles + tile
 };
 struct Work {
     const Matrix* table;
@@ -55,7 +57,7 @@ struct Work {
     Matrix one;
     int64_t src_step, out_step;     // bytes
     int64_t x_step, a_step, part_step;
-    int32_t per;                    // tiles of a matrix
+    int32_t per, splits;            // workgroups of a matrix, and of a tile
     uint32_t total;                 // workgroups that have something to do
     void* halves;                   // workspace
     double* sums;
@@ -71,6 +73,8 @@ struct PassArgs {
     double eps;
     float scale;                    // of X's planes
     int32_t planes;                 // of the products
+    uint32_t* tickets;              // launch_momentum: set to zero
+    uint32_t n_tickets;
 };
 int launch_momentum(const PassArgs& a, hipStream_t stream);
 int launch_lay(const PassArgs& a, hipStream_t stream);
@@ -80,6 +84,8 @@ struct SymmetricArgs {
     Work w;
     int32_t from;                   // buffer of X
     float own, product;             // result = own A + product acc
+    float* shares;                  // a tile's sums over a part of the inner axis, 4096 of every workgroup
+    uint32_t* tickets;              // how many of a tile's workgroups are done; zero before and after
 };
 // The last step's result: into the weights (lr by group, keep = 1 - lr weight_decay), or as it is, of `dtype`.
 struct Out {

@@ -281,14 +281,55 @@ struct Deep {
     static __device__ int col() { return (threadIdx.x & 7) * 8; }
 };
 
+// A tile's sums over the parts of the inner axis that its workgroups took, added up in their order by the one that is done last; false in the others.
+// The parts go past the dies' own caches, where every wave waits for its stores to arrive before the workgroup counts as done.
+template <class D>
+__device__ inline bool join(float* sums, float* shares, uint32_t* ticket, int splits, uint32_t split, int64_t apart) {
+    __shared__ uint32_t done;
+    uint64_t* mine = reinterpret_cast<uint64_t*>(shares + split * apart);
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+        const int f = t * 256 + threadIdx.x;
+        __hip_atomic_store(mine + f, *reinterpret_cast<const uint64_t*>(sums + (f >> 5) * D::kRow + (f & 31) * 2), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) done = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (done + 1 != static_cast<uint32_t>(splits)) return false;
+    float2 sum[8];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) sum[t] = make_float2(0.0f, 0.0f);
+    for (int s = 0; s < splits; ++s) {
+        const uint64_t* from = reinterpret_cast<const uint64_t*>(shares + s * apart);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            const uint64_t v = __hip_atomic_load(from + t * 256 + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            sum[t].x += __uint_as_float(static_cast<uint32_t>(v));
+            sum[t].y += __uint_as_float(static_cast<uint32_t>(v >> 32));
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+        const int f = t * 256 + threadIdx.x;
+        *reinterpret_cast<float2*>(sums + (f >> 5) * D::kRow + (f & 31) * 2) = sum[t];
+    }
+    if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);      // for the next launch
+    __syncthreads();
+    return true;
+}
+
 template <int P, bool SECOND, int S>
 __global__ __launch_bounds__(256) void symmetric_deep_kernel(SymmetricArgs a) {
     using D = Deep<P, false, S>;
     __shared__ __align__(16) char smem[D::kBytes];
     Sides x;
     if (!sides_of(a.w, x)) return;
+    const int side = (x.m + 63) / 64;
+    const uint32_t tiles = static_cast<uint32_t>(side) * (side + 1) / 2;
+    const uint32_t split = !SECOND && x.splits > 1 ? x.tile / tiles : 0, tile = x.tile - split * tiles;
     int tm, tn;
-    triangle(x.tile, tm, tn);
+    triangle(tile, tm, tn);
     const int m0 = tm * 64, n0 = tn * 64;
     _Float16* base = static_cast<_Float16*>(a.w.halves);
     _Float16 *own = base + x.a_at, *to = own + (SECOND ? P * x.a_plane : 0);
@@ -301,7 +342,20 @@ __global__ __launch_bounds__(256) void symmetric_deep_kernel(SymmetricArgs a) {
 #pragma unroll
             for (int q = 0; q < P; ++q)
                 beside[t].v[q] = *reinterpret_cast<const f16x8*>(own + half_at<P>(min(n0 + D::row(t), x.m - 1), min(m0 + D::col(), x.pad_m - 8), x.pad_m) + q * second_of<P>(x.a_plane));
-    float* sums = D::run(o, o, m0, n0, SECOND ? x.pad_m : x.pad_n, a.product, smem);
+    // this workgroup's part of the inner axis: steps of 64, of which the host gives every workgroup some
+    const int whole = SECOND ? x.pad_m : x.pad_n;
+    Operand part = o;
+    int depth = whole;
+    if (!SECOND && x.splits > 1) {
+        const int first = split * (whole / 64) / x.splits * 64, last = (split + 1) * (whole / 64) / x.splits * 64;
+        part.p = static_cast<const _Float16*>(o.p) + static_cast<int64_t>(first) * P;
+        depth = last - first;
+    }
+    float* sums = D::run(part, part, m0, n0, depth, a.product, smem);
+    if (!SECOND && x.splits > 1) {
+        const uint32_t at = x.unit + tile;
+        if (!join<D>(sums, a.shares + static_cast<int64_t>(at) * 4096, a.tickets + at, x.splits, split, static_cast<int64_t>(tiles) * 4096)) return;
+    }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const int r = D::row(t), row = n0 + r, m = m0 + D::col();

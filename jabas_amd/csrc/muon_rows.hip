@@ -23,6 +23,7 @@ __device__ inline f32x4 quad(const T* p, int64_t i) {
 // Bound by memory, 12 bytes an element (without momentum 2 or 4).
 template <class T>
 __global__ __launch_bounds__(256) void momentum_kernel(PassArgs a) {
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < a.n_tickets; i += gridDim.x * 256) a.tickets[i] = 0;
     Sides at;
     if (!sides_of(a.w, at)) return;
     const Matrix x = matrix_of(a.w, at.matrix);

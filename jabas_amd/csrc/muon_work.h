@@ -15,6 +15,8 @@ struct Sides {
     uint32_t matrix, tile;
     int32_t m, n, pad_m, pad_n;
     int64_t x_at, a_at, x_plane, a_plane;
+    uint32_t unit;
+    int32_t splits;
     __device__ void pad() {
         pad_m = (m + kPad - 1) / kPad * kPad;
         pad_n = (n + kPad - 1) / kPad * kPad;
@@ -36,6 +38,8 @@ __device__ inline bool sides_of(const Work& w, Sides& at) {
         at.n = s.n;
         at.x_at = s.x_at;
         at.a_at = s.a_at;
+        at.unit = s.unit;
+        at.splits = s.splits;
     } else {
         const uint32_t die = block & 7, each = w.total >> 3, left = w.total & 7;
         const uint32_t slot = die * each + min(die, left) + (block >> 3);
@@ -45,6 +49,8 @@ __device__ inline bool sides_of(const Work& w, Sides& at) {
         at.n = w.one.n;
         at.x_at = w.one.x_at + at.matrix * w.x_step;
         at.a_at = w.one.a_at + at.matrix * w.a_step;
+        at.unit = at.matrix * w.per;
+        at.splits = w.splits;
     }
     at.pad();
     return true;

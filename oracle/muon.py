@@ -1,4 +1,4 @@
-"""The orthogonalised update in 64 bits on the CPU, from its definition, and how far roundings of its factors carry."""
+"""The orthogonalised update in 64 bits (on the CPU, large ones elsewhere), from its definition, and how far roundings of its factors carry."""
 import math
 
 import torch
@@ -10,16 +10,16 @@ def _rounded(x, bits, gen):
     """x off by up to half a step of `bits` bits, evenly: what a factor of so many bits is."""
     if bits is None:
         return x
-    return x * (1.0 + (2.0 * torch.rand(x.shape, generator=gen, dtype=x.dtype) - 1.0) * 2.0 ** -bits)
+    return x * (1.0 + (2.0 * torch.rand(x.shape, generator=gen, dtype=x.dtype, device=x.device) - 1.0) * 2.0 ** -bits)
 
 
-def newton_schulz(g, steps=5, coefficients=COEFFICIENTS, eps=1e-7, factor_bits=None, own_bits=None, seed=0):
+def newton_schulz(g, steps=5, coefficients=COEFFICIENTS, eps=1e-7, factor_bits=None, own_bits=None, seed=0, device="cpu"):
     """g (..., rows, cols). ``factor_bits``: of the products' factors; ``own_bits``: of the running matrix itself."""
     if g.shape[-2] > g.shape[-1]:
-        return newton_schulz(g.transpose(-1, -2), steps, coefficients, eps, factor_bits, own_bits, seed).transpose(-1, -2)
-    gen = torch.Generator().manual_seed(seed)
+        return newton_schulz(g.transpose(-1, -2), steps, coefficients, eps, factor_bits, own_bits, seed, device).transpose(-1, -2)
+    gen = torch.Generator(device).manual_seed(seed)
     a, b, c = coefficients
-    x = g.detach().cpu().double()
+    x = g.detach().to(device).double()
     x = x / x.square().sum((-2, -1), keepdim=True).sqrt().clamp(min=eps)
     for _ in range(steps):
         x = _rounded(x, own_bits, gen)
@@ -32,7 +32,7 @@ def newton_schulz(g, steps=5, coefficients=COEFFICIENTS, eps=1e-7, factor_bits=N
 
 def off_by(x, y):
     """Length of the difference over the length of y."""
-    x, y = x.detach().cpu().double(), y.detach().cpu().double()
+    x, y = x.detach().to(y.device).double(), y.detach().double()
     length = float(y.norm())
     return float((x - y).norm()) / length if length else float((x - y).norm())
 

@@ -71,6 +71,60 @@ def test_tiles_of_every_size_that_end_inside(gpu, dtype, rows, cols):
         _close(o, x[0])
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(250, 4000), (3, 64, 9001), (2, 3001, 130), (448, 4100), (1, 20, 20000)])
+def test_long_matrices_whose_tiles_are_shared(gpu, dtype, shape):
+    """Few tiles over a long axis: workgroups share them. The last to finish adds up, in a fixed order, and the tickets are good for the next call."""
+    x = _matrices(*shape, kind="steep").to(TYPES[dtype])
+    held = x.to(gpu)
+    first = optim.orthogonalize(held)
+    for one, o in zip(x.view(-1, *shape[-2:]), first.view(-1, *shape[-2:])):
+        _close(o, one)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = []
+    for s in streams * 4:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append(optim.orthogonalize(held))
+    torch.cuda.synchronize()
+    assert all(torch.equal(first, o) for o in outs)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(4096, 4096), (2500, 5000), (6, 1030, 2050)])
+def test_large_matrices(gpu, dtype, shape):
+    x = _matrices(*shape, kind="steep").to(TYPES[dtype]).to(gpu)
+    got = optim.orthogonalize(x)
+    far, e = M.allowed(x, dtype == "bf16", device=gpu)
+    for o, y in zip(got.view(-1, *shape[-2:]), e.view(-1, *shape[-2:])):
+        assert M.off_by(o, y) <= far
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_very_many_small_matrices(gpu, dtype):
+    x = _matrices(70001, 5, 3).to(TYPES[dtype])
+    got = optim.orthogonalize(x.to(gpu))
+    _close(got, x)
+    for i in (0, 1, 65535, 65536, 70000):
+        _close(got[i], x[i])
+
+
+def test_calls_that_overlap(gpu):
+    """Two streams at once, other shapes and inputs on either."""
+    a, b = [_matrices(200, 300, seed=s).to(gpu) for s in range(6)], [_matrices(4, 64, 3000, seed=s).to(gpu) for s in range(6)]
+    alone = [optim.orthogonalize(x) for x in a], [optim.orthogonalize(x) for x in b]
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = [], []
+    for x, y in zip(a, b):
+        for z, s, out in zip((x, y), streams, outs):
+            with torch.cuda.stream(s):
+                out.append(optim.orthogonalize(z))
+    torch.cuda.synchronize()
+    for one, two in zip(alone, outs):
+        assert all(torch.equal(o, t) for o, t in zip(one, two))
+
+
 def test_a_batch_that_goes_through_the_workspace_some_at_a_time(gpu):
     x = torch.randn(40, 512, 1024, generator=torch.Generator(gpu).manual_seed(0), device=gpu)
     got = optim.orthogonalize(x)
@@ -385,6 +439,48 @@ def test_replicas_receive_the_weights(gpu):
                 assert torch.equal(p, q) and torch.equal(p, r)
             else:
                 assert torch.equal(q, old)
+
+
+@pytest.mark.parametrize("shapes", [[(16, 16), (64, 40), (33, 64), (1, 9), (50, 3)], [(128, 100), (97, 128), (20, 6, 3, 3)], [(30, 1000), (700, 17)], [(60, 500)], [(300, 90), (5, 5)]])
+def test_lists_of_small_matrices(gpu, shapes):
+    """What a workgroup's LDS holds is stepped in one launch: weights off the 16-byte lines, replicas, decay, state that is kept."""
+    gen = _gen(9)
+    params, twins, stores = [], [], []
+    for i, s in enumerate(shapes):
+        n = torch.Size(s).numel()
+        stores.append(torch.full((n + 8,), 5.0, device=gpu))
+        params.append(torch.nn.Parameter(stores[-1][i % 4 + 1:i % 4 + 1 + n].view(s)))
+        twins.append(torch.nn.Parameter(torch.zeros(s, device=gpu)))
+        with torch.no_grad():
+            params[-1].copy_(torch.randn(s, generator=gen) * 0.05)
+    opt = optim.ShardMuon(params, lr=0.02, weight_decay=0.2).attach_replicas(params, twins)
+    exp = Expected(opt)
+    for step in range(3):
+        grads = _gradients(shapes, seed=100 + step)
+        for p, g in zip(params, grads):
+            p.grad = g.to(gpu)
+        opt.param_groups[0]["nesterov"] = step != 1
+        exp.before()
+        opt.step()
+        for i, (p, g, q, st) in enumerate(zip(params, grads, twins, stores)):
+            exp.check(p, g)
+            assert torch.equal(p, q)
+            assert (st[:i % 4 + 1] == 5.0).all() and (st[i % 4 + 1 + p.numel():] == 5.0).all()
+
+
+def test_a_list_with_long_matrices(gpu):
+    shapes = [(64, 4000), (3000, 200), (40, 50), (130, 1500)]
+    params = _parameters(gpu, shapes)
+    opt = optim.ShardMuon(params, lr=0.02)
+    exp = Expected(opt)
+    for step in range(3):
+        grads = _gradients(shapes, seed=110 + step)
+        for p, g in zip(params, grads):
+            p.grad = g.to(gpu)
+        exp.before()
+        opt.step()
+        for p, g in zip(params, grads):
+            exp.check(p, g)
 
 
 def test_lists_that_go_through_the_workspace_some_at_a_time(gpu):
