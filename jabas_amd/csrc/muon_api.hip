@@ -105,6 +105,9 @@ constexpr Cost kCosts[2][kKernels] = {
     {{2, 2.5, 0.20, 0.38, 0.46}, {4, 4.0, 0.50, 0.75, 0.75}, {2, 7.0, 0.62, 0.90, 1.00}, {1, 5.0, 0.38, 0.53, 0.60}, {1, 13.0, 1.25, 1.75, 1.75}},
     {{2, 3.5, 0.45, 0.76, 0.95}, {4, 4.5, 0.90, 1.60, 1.60}, {2, 8.0, 1.35, 2.60, 2.65}, {1, 6.0, 0.95, 1.15, 1.35}, {1, 18.0, 3.40, 4.75, 4.75}}};
 constexpr int64_t kCus = 256, kFew = 160;
+// Tiles of 64 of a symmetric product, which read every row most often, wait for memory where a matrix has more than kNear bytes: 4096 x 4096 above takes 1.25
+// (fp32) and 1.18 times (bf16) what the steps of 6 of 1024 x 4096 make it, two of 2048 x 4096 with two of 1024 x 4096 200 us for 160.
+constexpr double kNear = 16 << 20, kFar = 1.25;
 constexpr double kLaunch = 4.0, kJoin = 4.0;    // us of a launch, beside its tiles, and of tiles' parts that meet
 
 enum Product { kFirst, kSecond, kUpdate, kProducts };
@@ -164,7 +167,8 @@ double time_of(const Shape* shapes, size_t n, Product p, Kind k, int planes) {
     const double step = units <= kFew ? c.alone : p == kUpdate ? c.update : c.symmetric;
     const auto work_of = [&](const Shape& s) {
         const int splits = splits_of(s, p, k, tiles, planes);
-        return Tiles{c.start + s.steps(p) / splits * step + (splits > 1 ? kJoin : 0.0), s.count * s.tiles(p, k) * splits};
+        const double far = k == kSmall && p != kUpdate && 2 * planes * 64 * s.steps(p) * s.pad_m > kNear ? kFar : 1.0;
+        return Tiles{c.start + s.steps(p) / splits * step * far + (splits > 1 ? kJoin : 0.0), s.count * s.tiles(p, k) * splits};
     };
     if (n == 1) return kLaunch + (units + kCus * c.each - 1) / (kCus * c.each) * work_of(shapes[0]).length;
     std::vector<Tiles> work;
