@@ -17,8 +17,8 @@
  * update that looks at a whole matrix.
  *
  * Precision. precision JABAS_F32: every factor of a product is two fp16 planes, a product three of theirs: 22 bits of X's
- * entries down to 2^-14 of its largest singular value, steps of 2^-36 below. JABAS_BF16: one plane and one product, 11 bits of each factor; X itself
- * keeps 22, so that directions that are weak in G do not lose theirs to the rounding of strong ones. Sums are fp32, |G|_F fp64.
+ * entries down to 2^-14 of the largest singular value that it can have (1 at first, then what the polynomial makes of that), steps of 2^-36
+ * of it below. JABAS_BF16: one plane and one product, 11 bits of each factor; X itself keeps 22, so that directions that are weak in G do not lose theirs to the rounding of strong ones. Sums are fp32, |G|_F fp64.
  * A matrix that holds an infinity or a NaN becomes NaN as a whole.
  *
  * Conventions are those of jabas_sync.h: caller-owned device memory, no allocation, no synchronisation, all work on the

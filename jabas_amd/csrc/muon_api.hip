@@ -21,7 +21,7 @@ inline bool misaligned(const void* p, size_t to) { return reinterpret_cast<uintp
 constexpr int64_t kMaxSlots = int64_t{1} << 23;     // a launch has less than 2^32 threads, up to 512 a workgroup
 
 // What the products' factors are multiplied by, powers of two: no entry of a matrix is larger than its largest singular value, and how far
-// the polynomial lets those grow is known. Entries then lie under 2^14, and steps of fp16's second plane are 2^-38 of the largest or finer.
+// the polynomial lets those grow is known. The bound goes to between 2^13 and 2^14, and fp16's finest step, 2^-24, is 2^-37 of it or finer.
 struct Scales {
     double x[JABAS_MUON_MAX_STEPS + 1], a[JABAS_MUON_MAX_STEPS], b[JABAS_MUON_MAX_STEPS];
 };

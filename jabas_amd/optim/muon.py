@@ -128,6 +128,11 @@ def orthogonalize(x, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
     return _launch(x, torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out, steps, coefficients, eps)
 
 
+def _recording(x):
+    """Whether launches on x's device are being recorded in a graph."""
+    return x.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 # ------------------------------------------------------------------------------------------------------------------- plans
 class MuonPlan:
     """A validated, device-resident list of matrices; ``run`` queues their step. ``items``: dicts of ``grad``, ``momentum``, ``param``
@@ -138,6 +143,8 @@ class MuonPlan:
     def __init__(self, items, dtype=torch.float32):
         if not items:
             raise ValueError("a plan needs at least one matrix")
+        if _recording(items[0]["grad"]):
+            raise RuntimeError("a list of matrices is prepared before its step is recorded")
         self.precision = _PRECISION[dtype]
         self.device = items[0]["grad"].device
         table = (L.JabasMatrix * len(items))()
@@ -224,7 +231,10 @@ class ShardMuon(_ShardOptimizer):
 
     ``ns_dtype``: torch.float32 (22 bits of every factor in the products) or torch.bfloat16 (11 bits and a third of the products:
     the update is off by about 2e-3 of its length). A parameter group with ``use_muon=False`` is updated by AdamW with the group's ``betas`` and
-    ``eps`` (``adam_eps`` unless the group names one): biases, norms, embeddings. ``step(gradients)``, ``attach_replicas``: as for the others."""
+    ``eps`` (``adam_eps`` unless the group names one): biases, norms, embeddings. ``step(gradients)``, ``attach_replicas``: as for the others.
+
+    Parameters and gradients are float32 on one GPU, parameters contiguous. A step can be recorded in a graph from the third on with the same
+    gradients' memory (the first makes the state, the second the list of matrices); learning rates and the like are then the recorded ones."""
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_coefficients=COEFFICIENTS, eps=1e-7, ns_steps=5,
                  adjust_lr_fn=None, ns_dtype=torch.float32, betas=(0.9, 0.999), adam_eps=1e-8):
@@ -234,6 +244,7 @@ class ShardMuon(_ShardOptimizer):
             raise ValueError("Invalid weight_decay value: {}".format(weight_decay))
         self._adam_eps = adam_eps
         self._adam = None
+        self._recorded = {}         # plans that a graph's launches read
         super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov, ns_coefficients=tuple(ns_coefficients),
                                       eps=eps, ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn, ns_dtype=ns_dtype, use_muon=True, betas=betas,
                                       amsgrad=False))
@@ -283,6 +294,9 @@ class ShardMuon(_ShardOptimizer):
     def _state_names(self):
         return ("momentum_buffer",)
 
+    def _signature(self, counts, params, grads, where, states):
+        return super()._signature(counts, params, grads, where, states) + tuple([p.shape for p in params])
+
     def _others(self):
         """The AdamW that updates the groups without orthogonalisation, on this optimizer's groups and state."""
         groups = [g for g in self.param_groups if not g["use_muon"]]
@@ -321,15 +335,15 @@ class ShardMuon(_ShardOptimizer):
                 loss = closure()
         if gradients is not None:
             gradients = list(gradients)
+        matched = self._matched(gradients)
+        states = list(map(self.state.get, matched[1]))
+        sig = self._signature(*matched, states)
+        if matched[1] and sig not in self._recipes and _recording(matched[1][0]):
+            raise RuntimeError("a step is prepared before it is recorded: take two with these gradients first")
         others = self._others()
         if others is not None:
             others.step(gradients)
-        matched = self._matched(gradients)
-        if not matched[1]:
-            return loss
-        states = list(map(self.state.get, matched[1]))
-        sig = self._signature(*matched, states)
-        if self._replay(self._recipes.get(sig)):
+        if not matched[1] or self._replay(self._recipes.get(sig)):
             return loss
         self._volatile, launches, self._late_copies = False, [], []
         batches = {}
@@ -361,6 +375,8 @@ class ShardMuon(_ShardOptimizer):
 
     def _queue(self, plan, key, places):
         momentum, nesterov, coefficients, eps, steps, dtype = key
+        if torch.cuda.is_current_stream_capturing():
+            self._recorded[id(plan)] = plan
         plan.run(make_muon_args([self.param_groups[gi] for gi in places], momentum=momentum, nesterov=nesterov, steps=steps,
                                 coefficients=coefficients, eps=eps, dtype=dtype))
 

@@ -582,6 +582,63 @@ def test_a_step_recorded_in_a_graph(gpu):
         optim.orthogonalize(params[0].detach())
 
 
+def test_a_recorded_step_outlives_the_optimizers_other_lists(gpu):
+    params = [torch.nn.Parameter(torch.randn(s, generator=torch.Generator(gpu).manual_seed(5), device=gpu)) for s in ((40, 200), (300, 70))]
+    opt = optim.ShardMuon(params, lr=0.02)
+    opt._max_cached_plans = 2
+    exp = Expected(opt)
+    mine = [torch.zeros_like(p) for p in params]
+
+    def steps(grads, n=1):
+        for p, g in zip(params, grads):
+            p.grad = g
+        for _ in range(n):
+            opt.step()
+
+    def some(seed):
+        return [torch.randn(p.shape, generator=torch.Generator(gpu).manual_seed(seed), device=gpu) for p in params]
+
+    first = some(0)
+    with pytest.raises(RuntimeError, match="recorded"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            steps(first)
+    assert not any(opt.state.values())          # memory of a graph that never ran is no state
+    steps(some(1), 2)
+    steps(mine, 2)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    others = [some(seed) for seed in range(2, 8)]
+    for seed in range(3):
+        for other in others:            # more lists than are kept
+            steps(other, 2)
+        grads = some(10 + seed)
+        for g, new in zip(mine, grads):
+            g.copy_(new)
+        exp.before()
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, g in zip(params, grads):
+            exp.check(p, g)
+
+
+def test_a_parameter_that_changes_its_shape_in_place(gpu):
+    p = torch.nn.Parameter(torch.randn(30, 80, device=gpu))
+    p.grad = torch.randn(30, 80, device=gpu)
+    opt = optim.ShardMuon([p], lr=0.02)
+    opt.step()
+    opt.step()
+    grad = p.grad
+    p.grad = None
+    p.data, p.grad = p.data.view(80, 30), None
+    p.grad = grad.view(80, 30)
+    opt.state[p]["momentum_buffer"] = opt.state[p]["momentum_buffer"].view(80, 30)
+    exp = Expected(opt)
+    exp.before()
+    opt.step()
+    exp.check(p, p.grad)
+
+
 # ------------------------------------------------------------------------------------------------ the engine's and the trainer's step
 def _engine(gpu, batches, dtype, shapes, n_fanout=0, caps=None, **kw):
     from jabas_amd.engine import VSWFlatSync
