@@ -107,7 +107,10 @@ __device__ inline void triangle(uint32_t tile, int& tm, int& tn) {
     tm = static_cast<int>(tile - static_cast<uint32_t>(row) * (row + 1) / 2);
 }
 
-// A = X X^T, or (SECOND) B = b A + c A A: tiles on and under the diagonal, written where they are and mirrored.
+// A = X X^T, or (SECOND) B = b A + c A A: tiles on and under the diagonal, written where they are and mirrored, because half the products are then enough.
+// Bound by the matrix cores where tiles fill the chip's rounds: of 4096 x 16384 (bf16, tiles of 256) X X^T takes 355 us, 774 TFLOP/s counted by half, but 136 tiles
+// for 256 CUs; four of 1024 x 4096 and four of 1024 x 1024 (fp32, tiles of 128) 94 us, 688 counted three times; twelve of 768 x 768 (252 tiles of 12 steps) 28 us, 592:
+// a tile's start and end are about 6 us whatever its length, a launch 4.
 template <int P, class C, bool SECOND>
 __global__ __launch_bounds__(C::kThreads) void symmetric_kernel(SymmetricArgs a) {
     __shared__ __align__(16) char smem[C::kStages * C::kStage];
@@ -175,6 +178,9 @@ __global__ __launch_bounds__(C::kThreads) void symmetric_kernel(SymmetricArgs a)
 // behind a kernel that wrote them on another die) and the chain of barrier, LDS read and product. So S stages of LDS are on their way at once, a wave
 // has all it multiplies in a step in registers a step ahead, and the four waves are two halves of the inner axis by two halves of n, which reads LDS less
 // than four quarters of the tile do. The halves' sums meet in LDS.
+// A step of 64 of two planes takes 0.45 us with one tile a CU. Two stages leave room for four tiles a CU: a X + B X of 6 of 1024 x 4096 takes 180 us
+// with them and 203 with four stages, of one of 1024 x 4096 36 and 37. 21 convolutions' matrices (43 tiles, up to 1152 long) take 12, 6 and 8.5 us for X X^T,
+// A A and a X + B X, of which the launch and the first loads are about 4 each.
 template <int P, bool TA, int S>
 struct Deep {
     using C = Core<F16, P, 64, 64, 2, 2, TA, false, false, false, 2, P == 2>;
@@ -282,7 +288,8 @@ struct Deep {
 };
 
 // A tile's sums over the parts of the inner axis that its workgroups took, added up in their order by the one that is done last; false in the others.
-// The parts go past the dies' own caches, where every wave waits for its stores to arrive before the workgroup counts as done.
+// The parts go past the dies' own caches, where every wave waits for its stores to arrive before the workgroup counts as done. 256 x 4096 in fp32 (10 tiles) takes
+// 155 us a call with 8 workgroups a tile and 241 with one.
 template <class D>
 __device__ inline bool join(float* sums, float* shares, uint32_t* ticket, int splits, uint32_t split, int64_t apart) {
     __shared__ uint32_t done;
@@ -397,6 +404,8 @@ __device__ inline void band(uint32_t tile, int across, int down, int& tm, int& t
 }
 
 // X <- a X + B X, in planes, or at the last step to the weights. X lies with its rows of k: transposing reads take it as it is.
+// Bound by the matrix cores, and in large ones by the power that they take: 4096 x 16384 bf16 507 us, 1084 TFLOP/s (the library's plain product of that shape 1243);
+// 8 of 4096 x 1024 and two of 4096 x 2048 fp32 996 counted three times (1204); one of 4096 x 1024, 256 tiles of 128, 32 us and 794.
 template <int P, class C>
 __global__ __launch_bounds__(C::kThreads) void update_kernel(UpdateArgs a) {
     __shared__ __align__(16) char smem[C::kStages * C::kStage];

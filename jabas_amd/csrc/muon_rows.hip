@@ -20,7 +20,8 @@ __device__ inline f32x4 quad(const T* p, int64_t i) {
 
 // buf' = buf + (1 - momentum) (g - buf), written, and the sum of squares of what is to be orthogonalised, in 64 bits: in 32 a matrix of 10^7
 // entries would be off by 1e-5, and entries under 1e-19 would not count.
-// Bound by memory, 12 bytes an element (without momentum 2 or 4).
+// Bound by memory, 12 bytes an element (without momentum 2 or 4). A matrix has at most 1024 chunks: whoever needs the length adds that many up. 4 of 1024 x 1024
+// and 4 of 1024 x 4096 (21 M elements) take 48 us, 5.2 TB/s; one of 4096 x 1024 10 us; twelve of 768 x 768 fp32 without momentum 7.4.
 template <class T>
 __global__ __launch_bounds__(256) void momentum_kernel(PassArgs a) {
     for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < a.n_tickets; i += gridDim.x * 256) a.tickets[i] = 0;
@@ -78,7 +79,8 @@ __global__ __launch_bounds__(256) void momentum_kernel(PassArgs a) {
 
 // X = u / max(|u|, eps) as two planes of fp16 (hi + lo), the shorter side first, zeros to multiples of 64; 64 x 64 of it a workgroup. The update is made
 // once more of gradient and momentum: as many bytes as writing and reading it would be.
-// Bound by memory: 8 bytes an element in, 4 out.
+// Bound by memory: 8 bytes an element in, 4 out; those matrices 51 us, 4.9 TB/s, one of 4096 x 1024 12 us. The tile goes through LDS whichever way it lies, so that
+// tall matrices' rows are read and X's rows are written in full lines.
 template <class T, int P>
 __global__ __launch_bounds__(256) void lay_kernel(PassArgs a) {
     Sides at;
