@@ -81,7 +81,7 @@ void describe(Matrix& x, int64_t rows, int64_t cols) {
     x.parts = static_cast<int32_t>((count + chunk - 1) / chunk);
 }
 // Behind them, of any call: tiles' sums of launches that share tiles between workgroups, and the tiles' tickets.
-constexpr int64_t kSplitUnits = 256, kSplitTiles = 64;      // workgroups and tiles of a launch that shares tiles, at most
+constexpr int64_t kSplitUnits = 512;        // workgroups of a launch that shares tiles, at most
 constexpr int64_t kShareBytes = kSplitUnits * (4096 + 1) * 4;
 // halves of the workspace: X twice in two planes, A and B in as many as the products take
 int64_t halves_of(const Matrix& x, int planes) { return 4 * x.x_plane + 2 * planes * x.a_plane; }
@@ -149,12 +149,13 @@ double makespan(std::vector<Tiles> work, int64_t slots) {
     return end;
 }
 
-// Workgroups that share a tile's inner axis, where a launch (of `total` tiles) leaves most CUs idle and the axis is long: the parts meet through memory, which
-// takes 4 us with few of them and 6 with many. Without and with it, us of a call: 256 x 4096 fp32 241 and 155, four of 64 x 4096 222 and 126, 21
-// convolutions' matrices (43 tiles) 159 and 153; but 1000 x 384 and four of 384 x 384 (two workgroups to each of 105 tiles) 166 and 202, 1000 x 2048 bf16 183 and 241.
+// Workgroups that share a tile's inner axis, where a launch (of `total` tiles) leaves CUs room for more and the axis is long: the parts meet through memory, which
+// takes 4 us with few of them and 6 with many. Without and with it, us of a call: 256 x 4096 fp32 241 and 149, four of 64 x 4096 222 and 121, a step of 21
+// convolutions' matrices (43 tiles) 159 and 148, of one of 4096 x 1024 (136 tiles, three workgroups each) 388 and 353, 1024 x 4096 bf16 230 and 222; but
+// with two workgroups a tile 768 x 768 fp32 168 and 175, 1000 x 2048 bf16 180 and 189.
 constexpr int64_t kMostSplits = 8;
 int splits_of(const Shape& s, Product p, Kind k, int64_t total, int planes) {
-    if (p != kFirst || k != kSmall || total > kSplitTiles) return 1;     // A A has no long axis where there are few tiles
+    if (p != kFirst || k != kSmall) return 1;       // A A has no long axis where there are few tiles
     const int64_t splits = std::min({kSplitUnits / std::max<int64_t>(total, 1), static_cast<int64_t>(s.steps(p)) / (planes == 2 ? 6 : 12), kMostSplits});
     return splits >= 3 ? static_cast<int>(splits) : 1;
 }

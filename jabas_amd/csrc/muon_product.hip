@@ -179,7 +179,7 @@ __global__ __launch_bounds__(C::kThreads) void symmetric_kernel(SymmetricArgs a)
 // has all it multiplies in a step in registers a step ahead, and the four waves are two halves of the inner axis by two halves of n, which reads LDS less
 // than four quarters of the tile do. The halves' sums meet in LDS.
 // A step of 64 of two planes takes 0.45 us with one tile a CU. Two stages leave room for four tiles a CU: a X + B X of 6 of 1024 x 4096 takes 180 us
-// with them and 203 with four stages, of one of 1024 x 4096 36 and 37. 21 convolutions' matrices (43 tiles, up to 1152 long) take 12, 6 and 8.5 us for X X^T,
+// with them and 203 with four stages, of one of 1024 x 4096 36 and 37. 21 convolutions' matrices (43 tiles, up to 1152 long) take 11, 6 and 8 us for X X^T,
 // A A and a X + B X, of which the launch and the first loads are about 4 each.
 template <int P, bool TA, int S>
 struct Deep {
@@ -288,8 +288,9 @@ struct Deep {
 };
 
 // A tile's sums over the parts of the inner axis that its workgroups took, added up in their order by the one that is done last; false in the others.
-// The parts go past the dies' own caches, where every wave waits for its stores to arrive before the workgroup counts as done. 256 x 4096 in fp32 (10 tiles) takes
-// 155 us a call with 8 workgroups a tile and 241 with one.
+// The parts are written and read past the dies' own caches, and every wave waits for its stores to arrive before the workgroup counts as done: that is all the
+// order there has to be, so the ticket is a relaxed one (an acquiring and releasing one has the die's L2 written back and emptied under its other workgroups:
+// 448 x 4096 fp32 206 us a call, with the relaxed one 197). 256 x 4096 (10 tiles) takes 149 us with 8 workgroups a tile and 241 with one.
 template <class D>
 __device__ inline bool join(float* sums, float* shares, uint32_t* ticket, int splits, uint32_t split, int64_t apart) {
     __shared__ uint32_t done;
@@ -301,7 +302,7 @@ __device__ inline bool join(float* sums, float* shares, uint32_t* ticket, int sp
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (threadIdx.x == 0) done = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    if (threadIdx.x == 0) done = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     if (done + 1 != static_cast<uint32_t>(splits)) return false;
     float2 sum[8];
@@ -405,7 +406,7 @@ __device__ inline void band(uint32_t tile, int across, int down, int& tm, int& t
 
 // X <- a X + B X, in planes, or at the last step to the weights. X lies with its rows of k: transposing reads take it as it is.
 // Bound by the matrix cores, and in large ones by the power that they take: 4096 x 16384 bf16 507 us, 1084 TFLOP/s (the library's plain product of that shape 1243);
-// 8 of 4096 x 1024 and two of 4096 x 2048 fp32 996 counted three times (1204); one of 4096 x 1024, 256 tiles of 128, 32 us and 794.
+// 8 of 4096 x 1024 and two of 4096 x 2048 fp32 996 counted three times (1204); one of 4096 x 1024, 256 tiles of 128, 32 us and 803.
 template <int P, class C>
 __global__ __launch_bounds__(C::kThreads) void update_kernel(UpdateArgs a) {
     __shared__ __align__(16) char smem[C::kStages * C::kStage];

@@ -72,7 +72,7 @@ def test_tiles_of_every_size_that_end_inside(gpu, dtype, rows, cols):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
-@pytest.mark.parametrize("shape", [(250, 4000), (3, 64, 9001), (2, 3001, 130), (448, 4100), (1, 20, 20000)])
+@pytest.mark.parametrize("shape", [(250, 4000), (3, 64, 9001), (2, 3001, 130), (448, 4100), (1, 20, 20000), (800, 2100), (2600, 1000)])
 def test_long_matrices_whose_tiles_are_shared(gpu, dtype, shape):
     """Few tiles over a long axis: workgroups share them. The last to finish adds up, in a fixed order, and the tickets are good for the next call."""
     x = _matrices(*shape, kind="steep").to(TYPES[dtype])
