@@ -388,7 +388,8 @@ int cut(const std::vector<Matrix>& all, int planes, std::vector<uint32_t>& ends)
     int64_t whole = 0;
     for (const Matrix& x : all) whole += 2 * halves_of(x, planes);
     double best = 0.0;
-    const int64_t least = (whole + kTogether - 1) / kTogether;
+    // matrices that need more than kTogether are alone in their parts: there are never more parts than matrices
+    const int64_t least = std::min<int64_t>((whole + kTogether - 1) / kTogether, n);
     for (int64_t parts = least; parts < least + kTurns && parts <= n; ++parts) {
         std::vector<uint32_t> here;
         double time = 0.0;
@@ -421,7 +422,7 @@ int cut(const std::vector<Matrix>& all, int planes, std::vector<uint32_t>& ends)
             ends = here;
         }
     }
-    return JABAS_OK;
+    return ends.empty() ? JABAS_ERR_SIZE : JABAS_OK;
 }
 
 struct Built {

@@ -502,6 +502,28 @@ def test_lists_that_go_through_the_workspace_some_at_a_time(gpu):
         exp.check(params[i], grads[i])
 
 
+@pytest.mark.parametrize("ns_dtype", [torch.float32, torch.bfloat16])
+def test_lists_with_matrices_too_large_to_share_the_workspace(gpu, ns_dtype):
+    """Feed-forward weights, each of which is alone in its part, among small ones; the second step, whose momentum is the first one's."""
+    shapes = [(300, 129), (4096, 16384), (64, 64), (14336, 4096)]
+    gen = torch.Generator(gpu).manual_seed(3)
+    params = [torch.nn.Parameter(torch.randn(*s, generator=gen, device=gpu) * 0.05) for s in shapes]
+    opt = optim.ShardMuon(params, lr=0.02, weight_decay=0.1, ns_dtype=ns_dtype)
+    for step in range(2):
+        for p in params:
+            p.grad = torch.randn(p.shape, generator=gen, device=gpu) * 1e-3
+        held = [(p.detach().double(), opt.state[p]["momentum_buffer"].double() if step else 0.0) for p in params]
+        opt.step()
+    for p, (old, buf) in zip(params, held):
+        g = p.grad.double()
+        buf = buf + (1.0 - 0.95) * (g - buf)
+        assert float((opt.state[p]["momentum_buffer"].double() - buf).norm()) <= 2.0 ** -22 * float(buf.norm() + g.norm())
+        far, o = M.allowed(g + 0.95 * (buf - g), ns_dtype is torch.bfloat16, device=gpu)
+        rate = 0.02 * M.lr_factor(None, *p.shape)
+        new = old * (1.0 - 0.02 * 0.1) - rate * o
+        assert float((p.detach().double() - new).norm()) <= rate * far * float(o.norm()) + 2.0 ** -22 * float(old.norm())
+
+
 def test_checkpoints_go_to_torch_and_back(gpu):
     shapes = [(40, 30), (30, 64)]
     params, theirs = _parameters(gpu, shapes), _parameters(gpu, shapes)

@@ -3,6 +3,7 @@ import ctypes as C
 import os
 import re
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -142,6 +143,29 @@ def test_plans_and_their_workspace():
     assert lib.jabas_muon_plan_encode(table, n, L.F32, blob.data_ptr(), 64) == L.ERR_PLAN
     assert lib.jabas_muon_plan_encode(table, n, L.F32, None, size) == L.ERR_NULL
     assert lib.jabas_muon_workspace_bytes(None) == 0 and lib.jabas_muon_workspace_bytes(torch.zeros(64, dtype=torch.int64).data_ptr()) == 0
+
+
+LARGE = {"feed_forward": [(4096, 16384)], "tall": [(14336, 4096)], "vocabulary": [(50257, 1600)], "three": [(32000, 4096)] * 3, "square": [(6144, 6144)] * 2,
+         "mixed": [(32000, 4096), (1024, 1024), (32000, 4096)], "among_small": [(64, 64), (4096, 16384), (100, 70), (1000, 2048)]}
+
+
+@pytest.mark.parametrize("precision", [L.F32, L.BF16])
+@pytest.mark.parametrize("shapes", LARGE.values(), ids=LARGE)
+def test_matrices_too_large_to_share_the_workspace(shapes, precision):
+    """One that needs more than the 500 MiB that several may share goes through alone. In a process of its own: a crash of the encoder is a failure here."""
+    code = ("import sys; sys.path.insert(0, 'tests'); import test_muon_cabi_host as t\n"
+            f"print(*t._workspaces({shapes!r}, {precision}))")
+    run = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, env={**os.environ, "PYTHONPATH": ROOT})
+    assert run.returncode == 0, (run.returncode, run.stderr)
+    status, whole, *alone = [int(x) for x in run.stdout.split()]
+    assert status == L.OK
+    assert max(max(alone), 400 << 20) <= whole <= max(max(alone), 520 << 20)
+
+
+def _workspaces(shapes, precision):
+    lib, table = L.lib(), [_matrix(i, rows=r, cols=c) for i, (r, c) in enumerate(shapes)]
+    status, blob, _ = _encode(*table, precision=precision)
+    return [status] + [lib.jabas_muon_workspace_bytes(b.data_ptr()) for b in (blob, *[_encode(m, precision=precision)[1] for m in table])]
 
 
 def test_steps_that_are_refused():
