@@ -13,6 +13,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib as L
 from ..loss import _direct
@@ -100,9 +101,11 @@ def orthogonalize(x, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
 
     ``coefficients`` (a, b, c) may not let singular values grow past 256. ``out``: contiguous, of x's shape and type, not overlapping it.
     Leading sizes are a batch; sides up to 65536 x 4194304. There is no derivative: an ``x`` that requires grad is refused while
-    gradients are recorded."""
+    gradients are recorded, and so is a tangent."""
     if not isinstance(x, torch.Tensor):
         raise TypeError("x: expected a tensor")
+    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in (x, out)):
+        raise RuntimeError("orthogonalize has no forward-mode derivative")
     if not x.is_cuda:
         raise ValueError(f"x: must live on the GPU, got {x.device}")
     if x.dtype not in _PRECISION:

@@ -272,6 +272,22 @@ def test_recorded_calls_answer_for_other_inputs(gpu, dtype):
     assert torch.equal(traced(y), expected * 2)
 
 
+def test_a_tangent_is_refused_and_not_lost(gpu):
+    import torch.autograd.forward_ad as fwd
+    x, out = torch.randn(30, 20, device=gpu), torch.empty(30, 20, device=gpu)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            optim.orthogonalize(dual)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            optim.orthogonalize(dual)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            optim.orthogonalize(x, out=fwd.make_dual(out, torch.ones_like(x)))
+        assert torch.equal(optim.orthogonalize(fwd.unpack_dual(dual).primal), optim.orthogonalize(x))
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(optim.orthogonalize, (x,), (torch.ones_like(x),))
+
+
 # ----------------------------------------------------------------------------------------------------------- ShardMuon
 SHAPES = [(64, 64), (33, 70), (100, 30), (20, 6, 3, 3), (1, 50), (300, 129), (7,), (129,)]
 

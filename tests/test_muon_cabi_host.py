@@ -194,6 +194,20 @@ def test_tensors_that_are_refused():
         optim.orthogonalize([[1.0]])
 
 
+def test_a_tangent_is_refused_and_not_lost():
+    import torch.autograd.forward_ad as fwd
+    x = torch.randn(3, 4)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones(3, 4))
+        for call in (lambda: optim.orthogonalize(dual), lambda: optim.orthogonalize(x, out=dual)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with pytest.raises(ValueError, match="GPU"):
+            optim.orthogonalize(x)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(optim.orthogonalize, (x,), (torch.ones(3, 4),))
+
+
 def test_optimizers_that_are_refused():
     p = lambda *s: torch.nn.Parameter(torch.zeros(*s))
     with pytest.raises(ValueError, match="no matrix"):
