@@ -128,7 +128,11 @@ def orthogonalize(x, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
     if not _direct(x, out):
         made = torch.ops.jabas.orthogonalize(x, int(steps), [float(c) for c in coefficients], float(eps))
         return made if out is None else out.copy_(made)
-    return _launch(x, torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out, steps, coefficients, eps)
+    if out is None:
+        return _launch(x, torch.empty(x.shape, dtype=x.dtype, device=x.device), steps, coefficients, eps)
+    _launch(x, out, steps, coefficients, eps)
+    torch.autograd.graph.increment_version(out)     # autograd does not see the launch: whoever saved out is told
+    return out
 
 
 def _recording(x):

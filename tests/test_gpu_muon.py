@@ -235,6 +235,17 @@ def test_out(gpu):
             optim.orthogonalize(x, out=bad)
 
 
+def test_what_was_saved_of_out_is_known_to_have_changed(gpu):
+    x, out = _matrices(30, 40).to(gpu), _matrices(30, 40, seed=1).to(gpu)
+    w = torch.ones(30, 40, device=gpu, requires_grad=True)
+    y = (w * out).sum()                                     # keeps out for its backward pass
+    before = out._version
+    optim.orthogonalize(x, out=out)
+    assert out._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
 def test_refusals(gpu):
     x = _matrices(30, 40).to(gpu)
     with pytest.raises(RuntimeError, match="no derivative"):
