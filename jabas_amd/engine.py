@@ -195,27 +195,30 @@ class VSWFlatSync:
     def _queue_muon(self, stats, lr_scale, stream, clip_norm, accumulations):
         from .optim.muon import COEFFICIENTS, make_muon_args
         opt, clipped = self.opt, self._clipped(clip_norm)
+        if clipped and self._coef is None:
+            self._coef = torch.ones(1, dtype=torch.float32, device=self.device)
+        # whatever is refused is refused before anything is launched
+        coef = self._coef if clipped and not self.keep_clipped_grads else None
+        if self._plan_rest is not None:
+            adam = dict(kind="adamw", betas=opt.get("betas", (0.9, 0.999)), eps=opt.get("eps", 1e-8), groups=opt["groups"])
+            rest = make_step_args((1,), torch.float32, opt=adam, step=self.step_count + 1, lr_scale=lr_scale, grad_scale=coef)
+        if self._plan_matrices is not None:
+            matrices = make_muon_args(
+                opt["groups"], momentum=opt.get("momentum", 0.95), nesterov=opt.get("nesterov", True), steps=opt.get("ns_steps", 5),
+                coefficients=opt.get("ns_coefficients", COEFFICIENTS), eps=opt.get("ns_eps", 1e-7), dtype=opt.get("ns_dtype", torch.float32),
+                lr_scale=lr_scale, grad_scale=coef)
         level = stats if stats or not clipped else "similarity"
         rows = self.plan.run(self.step_args(stats=level, with_opt=False, accumulations=accumulations), stream=stream)
-        coef = None
         if clipped:
-            if self._coef is None:
-                self._coef = torch.ones(1, dtype=torch.float32, device=self.device)
-            coef = clip_coef(rows, clip_norm, out=self._coef, stream=stream)
+            clip_coef(rows, clip_norm, out=self._coef, stream=stream)
             if self.keep_clipped_grads:             # the aggregate itself becomes the clipped one
                 if self._plan_scale is None:
                     self._plan_scale = SyncPlan([SpanSpec([self.agg[off:off + n]], agg_out=self.agg[off:off + n]) for off, n, _, _ in self.layout.spans])
-                self._plan_scale.run(make_step_args((1,), torch.float32, grad_scale=coef), stream=stream)
-                coef = None
+                self._plan_scale.run(make_step_args((1,), torch.float32, grad_scale=self._coef), stream=stream)
         if self._plan_rest is not None:
-            adam = dict(kind="adamw", betas=opt.get("betas", (0.9, 0.999)), eps=opt.get("eps", 1e-8), groups=opt["groups"])
-            self._plan_rest.run(make_step_args((1,), torch.float32, opt=adam, step=self.step_count + 1, lr_scale=lr_scale, grad_scale=coef),
-                                stream=stream)
+            self._plan_rest.run(rest, stream=stream)
         if self._plan_matrices is not None:
-            self._plan_matrices.run(make_muon_args(
-                opt["groups"], momentum=opt.get("momentum", 0.95), nesterov=opt.get("nesterov", True), steps=opt.get("ns_steps", 5),
-                coefficients=opt.get("ns_coefficients", COEFFICIENTS), eps=opt.get("ns_eps", 1e-7), dtype=opt.get("ns_dtype", torch.float32),
-                lr_scale=lr_scale, grad_scale=coef), stream=stream)
+            self._plan_matrices.run(matrices, stream=stream)
         return rows if stats else None
 
     def _build_plan(self):

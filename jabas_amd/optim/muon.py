@@ -49,6 +49,12 @@ def _grown(status, coefficients, where):
     L.check(status, where)
 
 
+def _check_growth(ns):
+    """Whether the library takes the polynomial, asked without a launch."""
+    if not L.lib().jabas_orthogonalize_workspace_bytes(C.byref(L.JabasOrthogonalize(dtype=L.F32, ns=ns))):
+        raise ValueError(_GROWN.format((ns.a, ns.b, ns.c)))
+
+
 # ---------------------------------------------------------------------------------------------------------- orthogonalize
 def _launch(x, out, steps, coefficients, eps):
     if x.device.index != torch._C._cuda_getDevice():
@@ -200,6 +206,7 @@ def make_muon_args(groups, *, momentum, nesterov, steps=5, coefficients=COEFFICI
         raise ValueError(f"momentum must be in [0, 1), got {momentum}")
     a = L.JabasMuonArgs()
     a.ns = _newton_schulz(steps, coefficients, eps, dtype)
+    _check_growth(a.ns)
     a.momentum, a.nesterov, a.n_groups = float(momentum), int(bool(nesterov)), len(groups)
     for i, g in enumerate(groups):
         a.lr[i], a.weight_decay[i] = float(g["lr"]) * float(lr_scale), float(g.get("weight_decay", 0.0))
@@ -277,9 +284,7 @@ class ShardMuon(_ShardOptimizer):
             return
         if not 0.0 <= group["momentum"] < 1.0:
             raise ValueError("Invalid momentum value: {}".format(group["momentum"]))
-        o = L.JabasOrthogonalize(dtype=L.F32, ns=_newton_schulz(group["ns_steps"], group["ns_coefficients"], group["eps"], group["ns_dtype"]))
-        if not L.lib().jabas_orthogonalize_workspace_bytes(C.byref(o)):
-            raise ValueError(_GROWN.format(tuple(group["ns_coefficients"])))
+        _check_growth(_newton_schulz(group["ns_steps"], group["ns_coefficients"], group["eps"], group["ns_dtype"]))
         for p in group["params"]:
             lr_factor(group["adjust_lr_fn"], *matrix_shape(p))
 
@@ -347,11 +352,24 @@ class ShardMuon(_ShardOptimizer):
         sig = self._signature(*matched, states)
         if matched[1] and sig not in self._recipes and _recording(matched[1][0]):
             raise RuntimeError("a step is prepared before it is recorded: take two with these gradients first")
+        launches, held = self._remembered(sig), None        # held: copies of gradients that the launches are to read
+        if matched[1] and launches is None:
+            launches, held = self._prepare_launches(matched)
+        # whatever is refused is refused here, before any weight moves
+        runs = [(plan, self._args(key, places)) for plan, key, places, _ in launches or ()]
         others = self._others()
         if others is not None:
             others.step(gradients)
-        if not matched[1] or self._replay(self._recipes.get(sig)):
-            return loss
+        for plan, args in runs:
+            if torch.cuda.is_current_stream_capturing():
+                self._recorded[id(plan)] = plan
+            plan.run(args)
+        if held is not None and not self._volatile:
+            self._remember(sig, launches)
+        return loss
+
+    def _prepare_launches(self, matched):
+        """[(plan, what its launch takes one value of, its groups, their adjust_lr_fn)] of a call, and what has to live until they are queued."""
         self._volatile, launches, self._late_copies = False, [], []
         batches = {}
         for gi, p, g in self._pairs(*matched):
@@ -375,17 +393,12 @@ class ShardMuon(_ShardOptimizer):
                     raise RuntimeError(f"more than {L.MAX_GROUPS} parameter groups in one launch")
             plan = self._plan([item for _, item in items], key[-1], keep=not self._volatile)
             launches.append((plan, key, list(slots), [self.param_groups[gi]["adjust_lr_fn"] for gi in slots]))
-            self._queue(plan, key, list(slots))
-        if not self._volatile:
-            self._remember(sig, launches)
-        return loss
+        return launches, batches
 
-    def _queue(self, plan, key, places):
+    def _args(self, key, places):
         momentum, nesterov, coefficients, eps, steps, dtype = key
-        if torch.cuda.is_current_stream_capturing():
-            self._recorded[id(plan)] = plan
-        plan.run(make_muon_args([self.param_groups[gi] for gi in places], momentum=momentum, nesterov=nesterov, steps=steps,
-                                coefficients=coefficients, eps=eps, dtype=dtype))
+        return make_muon_args([self.param_groups[gi] for gi in places], momentum=momentum, nesterov=nesterov, steps=steps,
+                              coefficients=coefficients, eps=eps, dtype=dtype)
 
     def _plan(self, items, dtype, keep):
         if not keep:                                  # names copies that are gone after this call
@@ -399,17 +412,12 @@ class ShardMuon(_ShardOptimizer):
             plan = self._plans[key] = MuonPlan(items, dtype)
         return plan
 
-    def _replay(self, recipe):
-        """Repeats a remembered call with the groups' values of now. False (and nothing done) when one changed that the launches were
-        split by or that their plans hold."""
-        if recipe is None:
-            return False
-        launches, _ = recipe
-        for _, key, places, adjust in launches:
+    def _remembered(self, sig):
+        """The launches of a remembered call, None when a value changed that they were split by or that their plans hold."""
+        launches, _ = self._recipes.get(sig, (None, None))
+        for _, key, places, adjust in launches or ():
             for gi, how in zip(places, adjust):
                 group = self.param_groups[gi]
                 if self._key(group) != key or group["adjust_lr_fn"] != how:
-                    return False
-        for plan, key, places, _ in launches:
-            self._queue(plan, key, places)
-        return True
+                    return None
+        return launches

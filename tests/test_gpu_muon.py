@@ -688,6 +688,63 @@ def test_a_parameter_that_changes_its_shape_in_place(gpu):
     exp.check(p, p.grad)
 
 
+def _held(opt, params):
+    return [p.detach().clone() for p in params] + [v.clone() for p in params for v in opt.state.get(p, {}).values() if torch.is_tensor(v)]
+
+
+def test_a_call_that_is_refused_moves_nothing(gpu):
+    """Matrices are looked over before AdamW updates the others: whoever mends the call and takes it again updates them once."""
+    params = _parameters(gpu)
+    opt = optim.ShardMuon(_split(params), lr=0.02)
+    grads = [g.to(gpu) for g in _gradients()]
+    for p, g in zip(params, grads):
+        p.grad = g
+    opt.step()
+    opt.step()
+    vector, matrix, group = params[-1], params[0], opt.param_groups[0]
+    good = dict(group)
+
+    def refused(error, gradients=None, **kw):
+        held, count = _held(opt, params), opt.state[vector]["step"]
+        group.update(kw)
+        with pytest.raises(error):
+            opt.step(gradients)
+        group.update(good)
+        assert opt.state[vector]["step"] == count
+        assert all(torch.equal(a, b) for a, b in zip(held, _held(opt, params)))
+
+    for kw in (dict(momentum=1.0), dict(ns_steps=0), dict(eps=0.0), dict(ns_coefficients=(30.0, 40.0, 5.0)), dict(adjust_lr_fn="none")):
+        refused(ValueError, **kw)
+    halves = [g.bfloat16() for g in grads]
+    for i, h in enumerate(halves):
+        h.index = i
+    refused(TypeError, gradients=halves)
+    held = matrix.data
+    matrix.data = held.t().contiguous().t()
+    refused(ValueError)
+    matrix.data = held
+    buf = opt.state[matrix]["momentum_buffer"]
+    opt.state[matrix]["momentum_buffer"] = buf.bfloat16()
+    refused(ValueError)
+    opt.state[matrix]["momentum_buffer"] = buf
+    exp = Expected(opt)
+    exp.before()
+    opt.step()
+    for p, g in zip(params, grads):
+        exp.check(p, g.cpu())
+
+
+def test_too_many_groups_move_nothing(gpu):
+    params = [torch.nn.Parameter(torch.randn(3, 4, device=gpu)) for _ in range(17)] + [torch.nn.Parameter(torch.randn(5, device=gpu))]
+    for p in params:
+        p.grad = torch.ones_like(p)
+    opt = optim.ShardMuon([dict(params=[p]) for p in params[:-1]] + [dict(params=params[-1:], use_muon=False)])
+    held = [p.detach().clone() for p in params]
+    with pytest.raises(RuntimeError, match="groups"):
+        opt.step()
+    assert all(torch.equal(p, h) for p, h in zip(params, held)) and not opt.state.get(params[-1])
+
+
 # ------------------------------------------------------------------------------------------------ the engine's and the trainer's step
 def _engine(gpu, batches, dtype, shapes, n_fanout=0, caps=None, **kw):
     from jabas_amd.engine import VSWFlatSync
@@ -854,3 +911,19 @@ def test_trainer_takes_torchs_own_and_follows_its_groups(gpu):
     t.compute(_data(gpu, (4, 4), 3))
     with pytest.raises(ValueError, match="part of the launches' plan"):
         t.step()
+
+
+@pytest.mark.parametrize("change,error", [(dict(momentum=1.0), ValueError), (dict(ns_steps=0), ValueError), (dict(ns_eps=0.0), ValueError),
+                                          (dict(ns_coefficients=(30.0, 40.0, 5.0)), ValueError)])
+def test_an_engines_step_that_is_refused_moves_nothing(gpu, change, error):
+    shapes = [(64, 64), (7,), (300, 129)]
+    eng = _engine(gpu, (4, 4), torch.float32, shapes, in_place=False)
+    for a in (eng.param, *eng.grads):
+        a.copy_(torch.randn(a.numel(), generator=_gen(8)) * 0.05)
+    eng.step()
+    held = [t.clone() for t in (eng.param, eng.state1, eng.state2)]
+    eng.opt.update(change)
+    for clip in (None, 0.1):
+        with pytest.raises(error):
+            eng.step(clip_norm=clip)
+    assert eng.step_count == 1 and all(torch.equal(a, b) for a, b in zip(held, (eng.param, eng.state1, eng.state2)))
