@@ -248,7 +248,8 @@ class ShardMuon(_ShardOptimizer):
     ``eps`` (``adam_eps`` unless the group names one): biases, norms, embeddings. ``step(gradients)``, ``attach_replicas``: as for the others.
 
     Parameters and gradients are float32 on one GPU, parameters contiguous. A step can be recorded in a graph from the third on with the same
-    gradients' memory (the first makes the state, the second the list of matrices); learning rates and the like are then the recorded ones."""
+    gradients' memory (the first makes the state, the second the list of matrices); learning rates and the like are then the recorded ones. One that
+    updates anything by AdamW is refused while recording: its step count could not rise."""
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_coefficients=COEFFICIENTS, eps=1e-7, ns_steps=5,
                  adjust_lr_fn=None, ns_dtype=torch.float32, betas=(0.9, 0.999), adam_eps=1e-8):
@@ -355,9 +356,11 @@ class ShardMuon(_ShardOptimizer):
         launches, held = self._remembered(sig), None        # held: copies of gradients that the launches are to read
         if matched[1] and launches is None:
             launches, held = self._prepare_launches(matched)
+        others = self._others()
+        if others is not None and torch.cuda.is_current_stream_capturing() and others._matched(gradients)[1]:
+            raise RuntimeError("AdamW's bias corrections are by value: a step that updates anything by it cannot be recorded")
         # whatever is refused is refused here, before any weight moves
         runs = [(plan, self._args(key, places)) for plan, key, places, _ in launches or ()]
-        others = self._others()
         if others is not None:
             others.step(gradients)
         for plan, args in runs:

@@ -745,6 +745,29 @@ def test_too_many_groups_move_nothing(gpu):
     assert all(torch.equal(p, h) for p, h in zip(params, held)) and not opt.state.get(params[-1])
 
 
+def test_a_step_that_updates_others_by_adamw_is_not_recorded(gpu):
+    """Its bias corrections are by value: a replay would repeat the recorded ones, and no count would rise."""
+    params = _parameters(gpu)
+    opt = optim.ShardMuon(_split(params), lr=0.02)
+    grads = _gradients()
+    for some in (params, params[-1:]):
+        for p, g in zip(params, grads):
+            p.grad = g.to(gpu) if any(q is p for q in some) else None
+        for _ in range(3):
+            opt.step()
+        torch.cuda.synchronize()
+        held, count = _held(opt, params), opt.state[params[-1]]["step"]
+        with pytest.raises(RuntimeError, match="recorded"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                opt.step()
+        torch.cuda.synchronize()
+        assert opt.state[params[-1]]["step"] == count and all(torch.equal(a, b) for a, b in zip(held, _held(opt, params)))
+    exp = Expected(opt)                     # and eager steps go on from there
+    exp.before()
+    opt.step()
+    exp.check(params[-1], grads[-1])
+
+
 # ------------------------------------------------------------------------------------------------ the engine's and the trainer's step
 def _engine(gpu, batches, dtype, shapes, n_fanout=0, caps=None, **kw):
     from jabas_amd.engine import VSWFlatSync
