@@ -308,7 +308,7 @@ class ShardMuon(_ShardOptimizer):
         return ("momentum_buffer",)
 
     def _signature(self, counts, params, grads, where, states):
-        return super()._signature(counts, params, grads, where, states) + tuple([p.shape for p in params])
+        return super()._signature(counts, params, grads, where, states) + tuple([p.shape for p in params]) + tuple([g.dtype for g in grads])
 
     def _others(self):
         """The AdamW that updates the groups without orthogonalisation, on this optimizer's groups and state."""

@@ -745,6 +745,21 @@ def test_too_many_groups_move_nothing(gpu):
     assert all(torch.equal(p, h) for p, h in zip(params, held)) and not opt.state.get(params[-1])
 
 
+def test_a_gradient_of_another_type_at_the_same_address(gpu):
+    p = torch.nn.Parameter(torch.randn(64, 64, device=gpu))
+    opt = optim.ShardMuon([p], lr=0.02)
+    p.index = 0
+    g = torch.randn(64, 64, device=gpu)
+    half = g.view(torch.bfloat16).view(-1)[:4096].view(64, 64)
+    g.index = half.index = 0
+    for _ in range(3):
+        opt.step([g])
+    held = p.detach().clone()
+    with pytest.raises(TypeError):
+        opt.step([half])
+    assert torch.equal(p, held)
+
+
 def test_a_step_that_updates_others_by_adamw_is_not_recorded(gpu):
     """Its bias corrections are by value: a replay would repeat the recorded ones, and no count would rise."""
     params = _parameters(gpu)
