@@ -146,6 +146,8 @@ class VSWFlatSync:
         groups = self.opt["groups"]
         if not 1 <= len(groups) <= L.MAX_GROUPS:
             raise ValueError(f"1..{L.MAX_GROUPS} parameter groups supported, got {len(groups)}")
+        if self.opt.get("amsgrad", False) or any(g.get("amsgrad", False) for g in groups if not g.get("use_muon", True)):
+            raise ValueError("the sync step has no amsgrad beside orthogonalised updates")
         if shapes is None or len(shapes) != len(self.layout.specs):
             raise ValueError("kind 'muon' needs the shape of every parameter (shapes=)")
         found = {}

@@ -136,6 +136,8 @@ def _read_muon(opt, groups):
                 raise ValueError(f"parameter groups differ in {key!r}: one value per launch is supported")
             if values:
                 opt[name] = values[0]
+    if any(g.get("amsgrad", False) for g in groups if not g.get("use_muon", True)):
+        raise ValueError("the sync step has no amsgrad beside orthogonalised updates")
 
 
 def opt_from_torch_optimizer(optimizer):

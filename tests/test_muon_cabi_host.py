@@ -245,3 +245,24 @@ def test_the_bucket_launches_refuse_it():
     with pytest.raises(TypeError, match="no part of a bucket's launch"):
         local.bind_optimizer(opt)
     assert local.optimizer is None
+
+
+def test_amsgrad_is_refused_where_the_sync_step_would_drop_it():
+    from jabas_amd.engine import VSWFlatSync
+    from jabas_amd.train.trainer import opt_from_torch_optimizer, refresh_opt_from_torch_optimizer
+    from jabas_amd.workloads import ParamSpec
+    groups = [dict(params=[torch.nn.Parameter(torch.zeros(3, 4))]), dict(params=[torch.nn.Parameter(torch.zeros(3))], use_muon=False, amsgrad=True)]
+    opt = optim.ShardMuon(groups)
+    with pytest.raises(ValueError, match="amsgrad"):
+        opt_from_torch_optimizer(opt)
+    opt.param_groups[1]["amsgrad"] = False
+    got = opt_from_torch_optimizer(opt)
+    opt.param_groups[1]["amsgrad"] = True
+    with pytest.raises(ValueError, match="amsgrad"):
+        refresh_opt_from_torch_optimizer(got, opt)
+    opt.param_groups[1]["amsgrad"], opt.param_groups[0]["amsgrad"] = False, True        # of the matrices: means nothing
+    opt_from_torch_optimizer(opt)
+    specs = [ParamSpec("a", 12, 0), ParamSpec("b", 3, 1)]
+    for where in (dict(amsgrad=True), dict(groups=[dict(lr=0.1), dict(lr=0.1, use_muon=False, amsgrad=True)])):
+        with pytest.raises(ValueError, match="amsgrad"):
+            VSWFlatSync(specs, (1,), opt={**dict(kind="muon", groups=[dict(lr=0.1), dict(lr=0.1, use_muon=False)]), **where}, device="cpu", shapes=[(3, 4), (3,)])
