@@ -194,10 +194,11 @@ def refresh_opt_from_torch_optimizer(opt, optimizer):
     if opt["kind"] == "muon":
         if [m["use_muon"] for m in opt["groups"]] != [bool(g.get("use_muon", True)) for g in groups]:
             raise ValueError("a parameter group's use_muon changed after the state arenas were laid out")
-        fixed = opt.get("adjust_lr_fn"), opt.get("ns_dtype")
-        _read_muon(opt, groups)
-        if (opt.get("adjust_lr_fn"), opt.get("ns_dtype")) != fixed:
+        now = dict(opt)
+        _read_muon(now, groups)
+        if any(now.get(name) != opt.get(name) for name in ("adjust_lr_fn", "ns_dtype")):
             raise ValueError("adjust_lr_fn and ns_dtype are part of the launches' plan: they cannot change after it was made")
+        opt.update(now)
         return
     g0 = groups[0]
     keys = ("momentum", "dampening", "nesterov") if opt["kind"] == "sgd" else ("betas", "eps")

@@ -965,3 +965,23 @@ def test_an_engines_step_that_is_refused_moves_nothing(gpu, change, error):
         with pytest.raises(error):
             eng.step(clip_norm=clip)
     assert eng.step_count == 1 and all(torch.equal(a, b) for a, b in zip(held, (eng.param, eng.state1, eng.state2)))
+
+
+def test_trainer_goes_on_refusing_what_its_plans_cannot_follow(gpu):
+    from jabas_amd.train import VSWSyncTrainer
+    t = VSWSyncTrainer(gpu, (4, 4))
+    t.prepare_stream_parallel(_Net(5, bias=False), torch.nn.MSELoss())
+    opt = optim.ShardMuon(t.main_model.parameters(), lr=0.02)
+    t.prepare_weight_sync_method(opt)
+    held = [p.detach().clone() for p in t.main_model.parameters()]
+    for key, value in (("adjust_lr_fn", "match_rms_adamw"), ("ns_dtype", torch.bfloat16)):
+        before = opt.param_groups[0][key]
+        opt.param_groups[0][key] = value
+        for seed in range(3):
+            t.compute(_data(gpu, (4, 4), seed))
+            with pytest.raises(ValueError, match="part of the launches' plan"):
+                t.step()
+        opt.param_groups[0][key] = before
+    assert all(torch.equal(p, old) for p, old in zip(t.main_model.parameters(), held))
+    t.step()
+    assert not any(torch.equal(p, old) for p, old in zip(t.main_model.parameters(), held))

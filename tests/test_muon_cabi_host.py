@@ -266,3 +266,19 @@ def test_amsgrad_is_refused_where_the_sync_step_would_drop_it():
     for where in (dict(amsgrad=True), dict(groups=[dict(lr=0.1), dict(lr=0.1, use_muon=False, amsgrad=True)])):
         with pytest.raises(ValueError, match="amsgrad"):
             VSWFlatSync(specs, (1,), opt={**dict(kind="muon", groups=[dict(lr=0.1), dict(lr=0.1, use_muon=False)]), **where}, device="cpu", shapes=[(3, 4), (3,)])
+
+
+def test_a_refused_change_of_the_groups_is_refused_again():
+    from jabas_amd.train.trainer import opt_from_torch_optimizer, refresh_opt_from_torch_optimizer
+    opt = optim.ShardMuon([torch.nn.Parameter(torch.zeros(3, 4))])
+    got = opt_from_torch_optimizer(opt)
+    for key, value in (("adjust_lr_fn", "match_rms_adamw"), ("ns_dtype", torch.bfloat16)):
+        before = opt.param_groups[0][key]
+        opt.param_groups[0][key] = value
+        for _ in range(2):
+            with pytest.raises(ValueError, match="part of the launches' plan"):
+                refresh_opt_from_torch_optimizer(got, opt)
+        opt.param_groups[0][key] = before
+    opt.param_groups[0]["momentum"] = 0.5
+    refresh_opt_from_torch_optimizer(got, opt)
+    assert got == opt_from_torch_optimizer(opt)
