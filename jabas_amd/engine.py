@@ -150,7 +150,7 @@ class VSWFlatSync:
             raise ValueError("the sync step has no amsgrad beside orthogonalised updates")
         if shapes is None or len(shapes) != len(self.layout.specs):
             raise ValueError("kind 'muon' needs the shape of every parameter (shapes=)")
-        found = {}
+        self._kinds, found = self._group_kinds(), {}
         for i, (spec, shape) in enumerate(zip(self.layout.specs, shapes)):
             count = 1
             for n in shape:
@@ -193,6 +193,14 @@ class VSWFlatSync:
                       fanout=[self._view(f, i) for f in self.fanout]) for i, (rows, cols) in self._matrices.items()]
         self._plan_matrices = MuonPlan(items, self.opt.get("ns_dtype", torch.float32)) if items else None
         self._plan_scale = None
+        self._planned = self._plan_holds()
+
+    def _plan_holds(self):
+        """What of ``opt`` the launches were made for."""
+        return self.opt.get("adjust_lr_fn"), self.opt.get("ns_dtype", torch.float32)
+
+    def _group_kinds(self):
+        return [bool(g.get("use_muon", True)) for g in self.opt["groups"]]
 
     def _queue_muon(self, stats, lr_scale, stream, clip_norm, accumulations):
         from .optim.muon import COEFFICIENTS, make_muon_args
@@ -200,6 +208,8 @@ class VSWFlatSync:
         if clipped and self._coef is None:
             self._coef = torch.ones(1, dtype=torch.float32, device=self.device)
         # whatever is refused is refused before anything is launched
+        if self._planned != self._plan_holds() or self._kinds != self._group_kinds():
+            raise ValueError("adjust_lr_fn, ns_dtype and use_muon are part of the launches' plan: they cannot change after it was made")
         coef = self._coef if clipped and not self.keep_clipped_grads else None
         if self._plan_rest is not None:
             adam = dict(kind="adamw", betas=opt.get("betas", (0.9, 0.999)), eps=opt.get("eps", 1e-8), groups=opt["groups"])

@@ -985,3 +985,20 @@ def test_trainer_goes_on_refusing_what_its_plans_cannot_follow(gpu):
     assert all(torch.equal(p, old) for p, old in zip(t.main_model.parameters(), held))
     t.step()
     assert not any(torch.equal(p, old) for p, old in zip(t.main_model.parameters(), held))
+
+
+@pytest.mark.parametrize("change", [dict(ns_dtype=torch.bfloat16), dict(adjust_lr_fn="match_rms_adamw"),
+                                    dict(groups=[dict(lr=0.02, use_muon=False), dict(lr=1e-3, use_muon=False)])])
+def test_an_engines_step_that_its_plans_cannot_follow_moves_nothing(gpu, change):
+    eng = _engine(gpu, (4, 4), torch.float32, [(64, 64), (7,), (300, 129)], in_place=False)
+    for a in (eng.param, *eng.grads):
+        a.copy_(torch.randn(a.numel(), generator=_gen(8)) * 0.05)
+    held, before = [t.clone() for t in (eng.param, eng.state1, eng.state2, eng.agg)], dict(eng.opt)
+    eng.opt.update(change)
+    with pytest.raises(ValueError, match="part of the launches' plan"):
+        eng.step()
+    assert eng.step_count == 0 and all(torch.equal(a, b) for a, b in zip(held, (eng.param, eng.state1, eng.state2, eng.agg)))
+    eng.opt.clear()
+    eng.opt.update(before)
+    eng.step()
+    assert not torch.equal(held[0], eng.param)
