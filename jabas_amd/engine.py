@@ -21,7 +21,8 @@ class VSWFlatSync:
                  moment_block_log2=MOMENT_BLOCK_LOG2, shapes=None):
         """``opt`` of kind "muon" (``optim.ShardMuon``): dict(kind="muon", momentum=, nesterov=, groups=[dict(lr=, weight_decay=,
         use_muon=True)], optionally adjust_lr_fn, ns_steps, ns_coefficients, ns_eps, ns_dtype, and betas and eps of the AdamW that
-        groups with use_muon=False follow); ``shapes``: the sizes of every parameter of ``specs``, in order. Its step aggregates first and
+        groups with use_muon=False follow); ``shapes``: the sizes of every parameter of ``specs``, in order, None in the
+        place of one that no group updates (its weights stay as they are). Its step aggregates first and
         then updates from the aggregate, which therefore is always written. state1 holds the matrices' momentum and the others' exp_avg,
         state2 the others' exp_avg_sq."""
         self.K = len(batches)
@@ -142,7 +143,7 @@ class VSWFlatSync:
 
     # ---- matrices whose update is orthogonalised -----------------------------------
     def _check_muon(self, shapes):
-        """{parameter: (rows, cols)} of the groups with use_muon."""
+        """{parameter: (rows, cols)} of the groups with use_muon; parameters that nothing updates go to ``_held``."""
         groups = self.opt["groups"]
         if not 1 <= len(groups) <= L.MAX_GROUPS:
             raise ValueError(f"1..{L.MAX_GROUPS} parameter groups supported, got {len(groups)}")
@@ -150,8 +151,11 @@ class VSWFlatSync:
             raise ValueError("the sync step has no amsgrad beside orthogonalised updates")
         if shapes is None or len(shapes) != len(self.layout.specs):
             raise ValueError("kind 'muon' needs the shape of every parameter (shapes=)")
-        self._kinds, found = self._group_kinds(), {}
+        self._kinds, self._held, found = self._group_kinds(), set(), {}
         for i, (spec, shape) in enumerate(zip(self.layout.specs, shapes)):
+            if shape is None:
+                self._held.add(i)
+                continue
             count = 1
             for n in shape:
                 count *= int(n)
@@ -169,10 +173,10 @@ class VSWFlatSync:
         for (off, numel, _bounds, _bucket) in self.layout.spans:
             sl = slice(off, off + numel)
             whole.append(SpanSpec([g[sl] for g in self.grads], agg_out=self.agg[sl]))
-        for bucket in self.layout.buckets:          # stretches without a matrix
+        for bucket in self.layout.buckets:          # stretches without a matrix, or a parameter that nothing updates
             run = []
             for i in [*bucket.param_ids, None]:
-                if i is not None and i not in self._matrices:
+                if i is not None and i not in self._matrices and i not in self._held:
                     if self.layout.specs[i].numel:
                         run.append(i)
                 elif run:

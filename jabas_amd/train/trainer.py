@@ -330,7 +330,7 @@ class VSWSyncTrainer:
                                   device=self.gpu, n_fanout=0 if self.share_weights else max(1, self.num_models - 1),
                                   keep_clipped_grads=self.keep_grads, write_aggregate=self.keep_grads,
                                   moment_block_log2=sync.MOMENT_BLOCK_LOG2 if self.interleave_moments else 0,
-                                  shapes=[tuple(p.shape) for p in params])
+                                  shapes=[tuple(p.shape) if not group_of or id(p) in group_of else None for p in params])
         if self.num_models == 1 and not self.share_weights:
             self.engine.reconfigure(self.local_batch_sizes)       # keeps the fan-out slot for later replicas
         self.local_models = [model] + [copy.deepcopy(model) for _ in range(self.num_models - 1)]
@@ -352,6 +352,10 @@ class VSWSyncTrainer:
                     optimizer.register_load_state_dict_post_hook(adopt)
         torch.cuda.synchronize(self.gpu)
 
+    def _left_alone(self):
+        """Parameters outside every group, which an optimizer of orthogonalised updates does not touch."""
+        return self.engine._held if self.opt["kind"] == "muon" else ()
+
     _MOMENT_KEYS = ("exp_avg", "exp_avg_sq", "max_exp_avg_sq")
 
     def _expose_state(self, optimizer, moments=True):
@@ -363,6 +367,8 @@ class VSWSyncTrainer:
         eng = self.engine
         sgd = self.opt["kind"] == "sgd"
         for i, p in enumerate(self.main_model.parameters()):
+            if i in self._left_alone():
+                continue
             st = optimizer.state[p]
             if self.opt["kind"] == "muon" and i in eng._matrices:
                 st["momentum_buffer"] = eng.state_view(0, i).view(p.shape)
@@ -422,6 +428,8 @@ class VSWSyncTrainer:
         keys = (("momentum_buffer", 0),) if sgd else tuple((k, j) for j, k in enumerate(self._MOMENT_KEYS))
         steps, has_momentum = set(), False
         for i, p in enumerate(self.main_model.parameters()):
+            if i in self._left_alone():
+                continue
             st = self.main_optimizer.state.get(p, {})
             matrix = self.opt["kind"] == "muon" and i in eng._matrices
             for key, j in (("momentum_buffer", 0),) if matrix else keys:

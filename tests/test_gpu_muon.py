@@ -951,6 +951,32 @@ def test_trainer_takes_torchs_own_and_follows_its_groups(gpu):
         t.step()
 
 
+def test_trainer_leaves_parameters_outside_the_groups_alone(gpu):
+    """A frozen bias needs no group, a frozen matrix is not decayed, and checkpoints hold neither."""
+    from jabas_amd.train import VSWSyncTrainer
+    for share in (True, False):
+        t = VSWSyncTrainer(gpu, (4, 4), interval=2, share_weights=share, clip_norm=0.05)
+        net = _Net(6)
+        for p in (net.a.weight, net.b.bias):
+            p.requires_grad_(False)
+        t.prepare_stream_parallel(net, torch.nn.MSELoss())
+        mine = t.main_model
+        t.prepare_weight_sync_method(optim.ShardMuon([dict(params=[mine.b.weight]), dict(params=[mine.a.bias], use_muon=False, lr=1e-2)], lr=0.02, weight_decay=0.3))
+        held = [p.detach().clone() for p in mine.parameters()]
+        for step in range(3):
+            t.compute(_data(gpu, (4, 4), 50 + step))
+            t.step()
+        for p, q, old in zip(mine.parameters(), t.local_models[1].parameters(), held):
+            assert torch.equal(p, q) and torch.equal(p, old) == (not p.requires_grad)
+        state = t.state_dict()
+        assert len(state["optimizer"]["state"]) == 2
+        t.load_state_dict(state)
+        t.compute(_data(gpu, (4, 4), 60))
+        t.step()
+        for p, old in zip(mine.parameters(), held):
+            assert torch.equal(p, old) == (not p.requires_grad)
+
+
 @pytest.mark.parametrize("change,error", [(dict(momentum=1.0), ValueError), (dict(ns_steps=0), ValueError), (dict(ns_eps=0.0), ValueError),
                                           (dict(ns_coefficients=(30.0, 40.0, 5.0)), ValueError)])
 def test_an_engines_step_that_is_refused_moves_nothing(gpu, change, error):
@@ -1002,3 +1028,26 @@ def test_an_engines_step_that_its_plans_cannot_follow_moves_nothing(gpu, change)
     eng.opt.update(before)
     eng.step()
     assert not torch.equal(held[0], eng.param)
+
+
+def test_engine_leaves_parameters_without_a_shape_alone(gpu):
+    """Between matrices and between vectors, in one bucket with them; they count for the aggregate and its norm."""
+    from jabas_amd.engine import VSWFlatSync
+    from jabas_amd.workloads import ParamSpec
+    shapes = [(7,), (64, 40), (9,), (11,), (33, 70), (5,), (3,)]
+    alone = {1, 3, 6}
+    specs = [ParamSpec(f"p{i}", torch.Size(s).numel(), 0 if len(s) > 1 else 1) for i, s in enumerate(shapes)]
+    opt = dict(kind="muon", groups=[dict(lr=0.02, weight_decay=0.5), dict(lr=1e-2, weight_decay=0.5, use_muon=False)])
+    eng = VSWFlatSync(specs, (4, 4), opt=opt, device=gpu, in_place=False, n_fanout=1, shapes=[None if i in alone else s for i, s in enumerate(shapes)])
+    for a in (eng.param, *eng.grads):
+        a.copy_(torch.randn(a.numel(), generator=_gen(8)))
+    eng.fanout[0].copy_(eng.param)
+    held = [eng.param_view(i).clone() for i in range(len(shapes))]
+    for _ in range(2):
+        eng.step(clip_norm=1e6)
+        eng.reconfigure((4, 4))
+    for i, old in enumerate(held):
+        assert torch.equal(eng.param_view(i), old) == (i in alone)
+        assert torch.equal(eng._view(eng.fanout[0], i), eng.param_view(i))
+        assert torch.allclose(eng.agg_view(i), eng.grad_view(0, i) / 2 + eng.grad_view(1, i) / 2)
+        assert bool(eng.state_view(0, i).any()) == (i not in alone)
