@@ -1051,3 +1051,37 @@ def test_engine_leaves_parameters_without_a_shape_alone(gpu):
         assert torch.equal(eng._view(eng.fanout[0], i), eng.param_view(i))
         assert torch.allclose(eng.agg_view(i), eng.grad_view(0, i) / 2 + eng.grad_view(1, i) / 2)
         assert bool(eng.state_view(0, i).any()) == (i not in alone)
+
+
+@pytest.mark.parametrize("dtype,clip,keep,ns_dtype", [("fp32", None, True, torch.float32), ("fp32", 0.02, False, torch.float32), ("bf16", 0.02, False, torch.bfloat16),
+                                                      ("bf16", 0.02, True, torch.float32)])
+def test_engine_steps_of_larger_matrices(gpu, dtype, clip, keep, ns_dtype):
+    """Matrices that no workgroup holds alone: the clipping coefficient is read by both passes over the aggregate, which have to agree on it."""
+    shapes, batches = [(300, 129), (129,), (200, 700), (5,), (64, 64)], (4, 2, 2)
+    eng = _engine(gpu, batches, TYPES[dtype], shapes, n_fanout=2, caps=(200000,), keep_clipped_grads=keep)
+    eng.opt["ns_dtype"] = ns_dtype
+    eng.reconfigure(batches)
+    gen, bf16 = _gen(17), ns_dtype is torch.bfloat16
+    for i in range(len(shapes)):
+        eng.param_view(i).copy_(torch.randn(eng.layout.specs[i].numel, generator=gen) * 0.05)
+    for step in range(1, 4):
+        grads = [[(torch.randn(s, generator=gen) * 1e-2).to(TYPES[dtype]) for s in shapes] for _ in batches]
+        for k, mine in enumerate(grads):
+            for i, g in enumerate(mine):
+                eng.grad_view(k, i).copy_(g.reshape(-1))
+        mean = [sum(mine[i].double() * (b / sum(batches)) for mine, b in zip(grads, batches)) for i in range(len(shapes))]
+        coef = min(1.0, clip / (float(torch.cat([g.reshape(-1) for g in mean]).norm()) + 1e-6)) if clip else 1.0
+        assert not clip or coef < 0.1
+        old = [(eng.param_view(i).cpu(), eng.state_view(0, i).cpu(), eng.state_view(1, i).cpu()) for i in range(len(shapes))]
+        eng.step(clip_norm=clip)
+        for i, s in enumerate(shapes):
+            g, (p, m, v), got = mean[i] * coef, old[i], eng.param_view(i).cpu().double()
+            if len(s) > 1:
+                new, buf, far = M.muon_step(p.view(s), g, m.view(s), 0.02, 0.1, 0.9, True, bf16=bf16)
+                assert float((got.view(s) - new).norm()) <= far
+                assert float((eng.state_view(0, i).cpu().double().view(s) - buf).norm()) <= 1e-6 * (float(buf.norm()) + float(g.norm()))
+            else:
+                new, _, _ = M.adamw_step(p, g, m, v, step, 1e-3, 0.0, (0.8, 0.95))
+                assert torch.allclose(got, new, rtol=1e-5, atol=1e-7)
+            for f in eng.fanout:
+                assert torch.equal(eng._view(f, i), eng.param_view(i))
