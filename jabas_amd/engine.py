@@ -199,6 +199,11 @@ class VSWFlatSync:
         self._plan_scale = None
         self._planned = self._plan_holds()
 
+    def _filled(self, stream):
+        """A step's own stream waits for what the step has just made, which the current one fills."""
+        if stream is not None:
+            stream.wait_stream(torch.cuda.current_stream(self.device))
+
     def _plan_holds(self):
         """What of ``opt`` the launches were made for."""
         return self.opt.get("adjust_lr_fn"), self.opt.get("ns_dtype", torch.float32)
@@ -211,6 +216,7 @@ class VSWFlatSync:
         opt, clipped = self.opt, self._clipped(clip_norm)
         if clipped and self._coef is None:
             self._coef = torch.ones(1, dtype=torch.float32, device=self.device)
+            self._filled(stream)
         # whatever is refused is refused before anything is launched
         if self._planned != self._plan_holds() or self._kinds != self._group_kinds():
             raise ValueError("adjust_lr_fn, ns_dtype and use_muon are part of the launches' plan: they cannot change after it was made")
@@ -230,6 +236,7 @@ class VSWFlatSync:
             if self.keep_clipped_grads:             # the aggregate itself becomes the clipped one
                 if self._plan_scale is None:
                     self._plan_scale = SyncPlan([SpanSpec([self.agg[off:off + n]], agg_out=self.agg[off:off + n]) for off, n, _, _ in self.layout.spans])
+                    self._filled(stream)
                 self._plan_scale.run(make_step_args((1,), torch.float32, grad_scale=self._coef), stream=stream)
         if self._plan_rest is not None:
             self._plan_rest.run(rest, stream=stream)
@@ -341,6 +348,7 @@ class VSWFlatSync:
             return self._queue_muon(stats, lr_scale, stream, clip_norm, accumulations)
         if self._clipped(clip_norm) and self._plan_agg is None:
             self._build_clip_plans()
+            self._filled(stream)
         args = self._update_args(stats, lr_scale, clip_norm, accumulations)
         if scalars is not None:
             scalars.attach(args)

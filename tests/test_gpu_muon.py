@@ -1085,3 +1085,33 @@ def test_engine_steps_of_larger_matrices(gpu, dtype, clip, keep, ns_dtype):
                 assert torch.allclose(got, new, rtol=1e-5, atol=1e-7)
             for f in eng.fanout:
                 assert torch.equal(eng._view(f, i), eng.param_view(i))
+
+
+@pytest.mark.parametrize("kind", ["muon", "adamw"])
+@pytest.mark.parametrize("keep", [True, False])
+def test_a_first_clipped_step_on_another_stream(gpu, kind, keep):
+    """What such a step makes for itself is filled on the current stream, which has work of its own to do first."""
+    from jabas_amd.engine import VSWFlatSync
+    from jabas_amd.workloads import ParamSpec
+    shapes = [(64, 64), (7,), (300, 129)]
+    specs = [ParamSpec(f"p{i}", torch.Size(s).numel(), 0 if len(s) > 1 else 1) for i, s in enumerate(shapes)]
+    opt = dict(kind=kind, momentum=0.9, nesterov=True, betas=(0.8, 0.95), eps=1e-8, groups=[dict(lr=0.02, weight_decay=0.1), dict(lr=1e-3, weight_decay=0.0, use_muon=False)])
+
+    def engine():
+        eng = VSWFlatSync(specs, (4, 4), opt=opt, device=gpu, in_place=False, shapes=shapes, keep_clipped_grads=keep, write_aggregate=False)
+        for a in (eng.param, *eng.grads):
+            a.copy_(torch.randn(a.numel(), generator=_gen(8)) * 0.05)
+        return eng
+
+    here, there, side = engine(), engine(), torch.cuda.Stream()
+    here.step(clip_norm=0.5)
+    busy = torch.randn(4096, 4096, device=gpu)
+    busy @ busy
+    torch.cuda.synchronize()
+    for _ in range(40):
+        busy = busy @ busy
+    there.step(clip_norm=0.5, stream=side)
+    torch.cuda.synchronize()
+    for a, b in ((here._coef, there._coef), (here.param, there.param), (here.agg, there.agg)):
+        assert torch.equal(a, b)
+    assert float(here._coef) < 0.2
