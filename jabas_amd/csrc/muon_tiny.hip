@@ -71,8 +71,9 @@ __device__ inline void wave_done() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// The shorter side takes MB blocks of 32. X and A (then B, in its place) lie in LDS in two planes whatever the type: the products are none of
-// the time. A block of A a wave; X is worked on in columns of 32, each by one wave that reads all of it before it writes, so X needs no second copy.
+// The shorter side takes MB blocks of 32. X and A (then B, in its place) lie in LDS in two planes of fp16 whatever the type (22 bits, as
+// the larger matrices' fp32 form; bf16's result is then off by its own rounding alone): the products are none of the time. A block of A a wave;
+// X is worked on in columns of 32, each by one wave that reads all of it before it writes, so X needs no second copy.
 // Bound by the way through LDS and the barriers, four a step: 64 x 64 takes 24 us, where the launches of the larger
 // matrices' kernels took 60. Three sums at once, blocks under the diagonal mirrored, the inner axis shared between waves were no faster.
 template <class T, int MB>

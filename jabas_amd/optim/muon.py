@@ -6,7 +6,10 @@ products: with X of the shorter side first, X = G / max(|G|, eps), then X <- a X
 reference has no such optimizer; the surface is that of ``torch.optim.Muon`` with the conventions of the other ``Shard``
 optimizers beside it (``step(gradients)``, replicas, state in the caller's hands).
 
-Everything runs on the current stream of the tensors' device, without synchronisation; there is no CPU path.
+Everything runs on the current stream of the tensors' device; there is no CPU path. Launches are queued without synchronisation. A list of
+matrices that a step has not seen (gradients in other memory make it another) is laid out on the host first and copied to the
+device, and the host waits for that copy: 96 matrices of 1024 x 1024 to 1024 x 4096 take 5 to 30 ms and 10 MB of tables. Gradients that keep their memory
+(``zero_grad(set_to_none=False)``, a bucket's views, the engine's arenas) are laid out once.
 """
 import ctypes as C
 import math
